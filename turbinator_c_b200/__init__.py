@@ -66,6 +66,23 @@ class LaunchOpts(_c.Structure):
     ]
 
 
+#: Argument types of the entry points of include/turbinator/training/cuda_learner.h
+#: (called through turbinator_c_b200/learner.py).
+_LEARNER_ARGUMENTS = {
+    "tb_cuda_group_norm_workspace": [_vp],
+    "tb_cuda_group_norm_device": [_vp] * 9,
+    "tb_cuda_group_norm_backward_device": [_vp] * 12,
+    "tb_cuda_gated_recurrence_workspace": [_vp],
+    "tb_cuda_gated_recurrence_device": [_vp] * 13,
+    "tb_cuda_gated_recurrence_backward_device": [_vp] * 17,
+    "tb_cuda_route_experts_workspace": [_vp],
+    "tb_cuda_route_experts_device": [_vp] * 10,
+    "tb_cuda_route_experts_backward_device": [_vp] * 6,
+    "tb_cuda_combine_experts_device": [_vp] * 6,
+    "tb_cuda_combine_experts_backward_device": [_vp] * 8,
+}
+
+
 def _bind(lib: ctypes.CDLL, name: str, restype, argtypes) -> None:
     fn = getattr(lib, name)
     fn.restype = restype
@@ -103,6 +120,8 @@ def load_library() -> ctypes.CDLL:
           [_vp, _vp, _vp, _vp, _sz, _vp, _c.POINTER(LaunchOpts)])
     _bind(lib, "tb_features_launch", _c.c_int,
           [_vp, _vp, _vp, _vp, _sz, _vp, _c.POINTER(LaunchOpts)])
+    for name, args in _LEARNER_ARGUMENTS.items():
+        _bind(lib, name, _sz if name.endswith("_workspace") else _c.c_int, args)
     _bind(lib, "tb_status_take", _c.c_int, [_vp, _c.POINTER(_c.c_uint)])
     _bind(lib, "tb_features_staged_config", _c.c_int,
           [_c.POINTER(_c.c_int)] * 5)
@@ -403,3 +422,14 @@ def generate(seed: int, first: int, count: int, *, total: Optional[int] = None,
                       None if camf is None else camf[s], threads)
         i = j
     return obs, mission, cams, camf
+
+
+# ---- learner layers (include/turbinator/training/cuda_learner.h) ----
+
+from .learner import (  # noqa: E402  (needs the helpers above)
+    ExpertCombineDesc, ExpertRouteDesc, GatedRecurrenceDesc, GroupNormDesc, RECURRENCE_CHECKPOINT, TB_ACT_GELU,
+    TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU, TB_SCORE_SIGMOID, TB_SCORE_SOFTMAX, TB_TYPE_BF16, TB_TYPE_F16, TB_TYPE_F32,
+    tb_cuda_combine_experts_backward_device, tb_cuda_combine_experts_device, tb_cuda_gated_recurrence_backward_device,
+    tb_cuda_gated_recurrence_device, tb_cuda_gated_recurrence_workspace, tb_cuda_group_norm_backward_device,
+    tb_cuda_group_norm_device, tb_cuda_group_norm_workspace, tb_cuda_route_experts_backward_device,
+    tb_cuda_route_experts_device, tb_cuda_route_experts_workspace)
