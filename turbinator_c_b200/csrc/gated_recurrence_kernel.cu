@@ -1,15 +1,40 @@
 /*
  * Gated linear recurrence with resets: forward and backward
  * (include/turbinator/training/cuda_learner.h).
+ *
+ * h_t = a_t h_(t-1) + b_t is a chain over t for each channel, but steps compose:
+ * a span of steps maps the state before it, h, to A h + H, so spans can be
+ * taken apart and joined.  A warp takes 16 steps of 32 or 64 channels, a CTA
+ * of four warps 64 steps; the spans of a sequence are joined across CTAs while
+ * they all run, so every input is read once whatever the split:
+ *
+ *   - Work items (span, sequence, channels) are handed out by a counter in the
+ *     order of the spans.  A CTA takes the next item only once it runs, and an
+ *     item waits only for earlier items, so the earliest unfinished one can
+ *     always go on.
+ *   - Each item publishes its (A, H), and then the state after it.  The state
+ *     before an item is the nearest published state folded forward through the
+ *     (A, H) of the spans between, one fma each: the same operations in the
+ *     same order from wherever the fold starts, so the bits do not depend on
+ *     timing.
+ *   - The wait for earlier spans is bounded by ~1 s of the GPU's clock, after
+ *     which the status word of the stream gets the timeout bit
+ *     (tb_cuda_synchronize reports it) and the kernel goes on to its end.
+ *
+ * The backward pass is the same scan in the other direction over
+ * c_t = a_t (dh_t + c_(t+1)), the gradient of the state before step t; the
+ * states that it needs are recomputed within 16 steps from the saved ones.
  */
+#include "tb_features_internal.h"
 #include "tb_learner.cuh"
 
 using namespace tb_learn;
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kCheckpoint = TB_RECURRENCE_CHECKPOINT;
+constexpr int kSteps = TB_RECURRENCE_CHECKPOINT; /* steps of a warp's span */
+constexpr int kWarps = 4;                        /* warps, and spans, of a CTA for sequences of more steps */
+constexpr unsigned long long kWaitNs = 1000000000ull;
 
 struct RecurrenceShape {
     size_t sequences, steps, channels;
@@ -17,124 +42,627 @@ struct RecurrenceShape {
     float scale;
 };
 
-__device__ __forceinline__ float softplus(float l) { return fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))); }
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
-
-__device__ __forceinline__ size_t live_steps(const RecurrenceShape &d, const int32_t *lengths, size_t b) {
-    if (!lengths) return d.steps;
-    const int32_t n = lengths[b];
-    return n < 0 ? 0 : static_cast<size_t>(n) < d.steps ? static_cast<size_t>(n) : d.steps;
-}
-
-struct Gates {
-    float log_a, a, beta, open, gate, x;
+struct ForwardArgs {
+    RecurrenceShape d;
+    const void *x, *rec, *inp;
+    const float *decay, *state_in;
+    const uint8_t *reset;
+    const int32_t *lengths;
+    void *h;
+    float *state_out, *checkpoints;
+    int in_piece, out_piece; /* bytes of a piece that rows move in */
 };
 
-template <class T>
-__device__ __forceinline__ Gates gates_of(const T *x, const T *rec, const T *inp, size_t at, float rate, bool reset) {
-    Gates g;
-    g.open = sigmoid(to_float(rec[at]));
-    g.gate = sigmoid(to_float(inp[at]));
-    g.x = to_float(x[at]);
-    g.log_a = rate * g.open;
-    g.a = reset ? 0.0f : expf(g.log_a);
-    g.beta = reset ? 1.0f : sqrtf(-expm1f(2.0f * g.log_a));
-    return g;
-}
+struct BackwardArgs {
+    RecurrenceShape d;
+    const void *x, *rec, *inp, *dh;
+    const float *decay, *checkpoints, *dstate_out;
+    const uint8_t *reset;
+    const int32_t *lengths;
+    void *dx, *drec, *dinp;
+    float *partial, *dstate_in; /* partial [spans, sequences, channels] */
+    int in_piece, dh_piece, out_piece;
+};
 
-/* One thread per (sequence, channel). */
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-recurrence_forward(RecurrenceShape d, const T *x, const T *rec, const T *inp, const float *decay,
-                   const uint8_t *reset, const int32_t *lengths, const float *state_in, T *h, float *state_out,
-                   float *checkpoints) {
-    const size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= d.sequences * d.channels) return;
-    const size_t b = i / d.channels, c = i % d.channels;
-    const size_t live = live_steps(d, lengths, b), saved = (d.steps + kCheckpoint - 1) / kCheckpoint;
-    const float rate = -d.scale * softplus(decay[c]);
-    float s = state_in ? state_in[i] : 0.0f;
-    for (size_t t = 0; t < d.steps; ++t) {
-        if (checkpoints && t % kCheckpoint == 0) checkpoints[(b * saved + t / kCheckpoint) * d.channels + c] = s;
-        float out = 0.0f;
-        if (t < live) {
-            const Gates g = gates_of(x, rec, inp, b * d.is + t * d.it + c, rate, reset && reset[b * d.steps + t]);
-            s = g.a * s + g.beta * g.gate * g.x;
-            out = s;
-        }
-        h[b * d.os + t * d.ot + c] = from_float<T>(out);
+/* The scan over spans: workspace and shape. */
+struct Spans {
+    unsigned *ticket, *flag; /* flag [spans, tiles]: 1 (A, H) there, 2 the state after it too */
+    float *map, *state;      /* [spans, tiles, 2, channels of a tile], [.., channels of a tile] */
+    unsigned spans, tiles, items, tiles_per_sequence;
+    unsigned *status;
+};
+
+__device__ __forceinline__ float softplus(float l) { return fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))); }
+
+/* Steps of a sequence that count, from step t0 on, at most kSteps. */
+__device__ __forceinline__ int live_steps(const RecurrenceShape &d, const int32_t *lengths, size_t b, size_t t0) {
+    size_t live = d.steps;
+    if (lengths) {
+        const int32_t n = lengths[b];
+        live = n < 0 ? 0 : static_cast<size_t>(n) < d.steps ? static_cast<size_t>(n) : d.steps;
     }
-    if (state_out) state_out[i] = s;
+    if (live <= t0) return 0;
+    return live - t0 < kSteps ? static_cast<int>(live - t0) : kSteps;
 }
 
-/* One thread per (sequence, channel); partial [sequences, channels]. */
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-recurrence_backward(RecurrenceShape d, const T *x, const T *rec, const T *inp, const float *decay,
-                    const uint8_t *reset, const int32_t *lengths, const float *checkpoints, const T *dh,
-                    const float *dstate_out, T *dx, T *drec, T *dinp, float *partial, float *dstate_in) {
-    const size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= d.sequences * d.channels) return;
-    const size_t b = i / d.channels, c = i % d.channels;
-    const size_t live = live_steps(d, lengths, b), saved = (d.steps + kCheckpoint - 1) / kCheckpoint;
-    const float rate = -d.scale * softplus(decay[c]);
-    float carry = dstate_out ? dstate_out[i] : 0.0f, sum = 0.0f;
-    for (size_t k = saved; k-- > 0;) {
-        float before[kCheckpoint];
-        float s = checkpoints[(b * saved + k) * d.channels + c];
+/* One step's decay.  p = e^(log a) - 1 keeps the digits of 1 - a^2 = -p (2 + p)
+ * where a is near 1: below 0.35 from its series (the next term is below 2e-8
+ * of p), past it from e^x. */
+struct Decay {
+    float log_a, a, beta;
+};
+__device__ __forceinline__ Decay decay_of(float rate, float open) {
+    Decay s;
+    s.log_a = rate * open;
+    const float l = s.log_a;
+    float q = fmaf(l, 1.0f / 5040.0f, 1.0f / 720.0f);
+    q = fmaf(q, l, 1.0f / 120.0f);
+    q = fmaf(q, l, 1.0f / 24.0f);
+    q = fmaf(q, l, 1.0f / 6.0f);
+    q = fmaf(q, l, 0.5f);
+    q = fmaf(q, l, 1.0f);
+    const float e = fast_exp2(kLog2e * l);
+    const bool near = l > -0.35f;
+    const float p = near ? l * q : e - 1.0f;
+    s.a = near ? 1.0f + p : e;
+    s.beta = fast_sqrt(-p * (2.0f + p));
+    return s;
+}
+
+/* ---- rows between global and the warp's shared memory ---- */
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void *from, int bytes) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+template <class T, int CT, int BYTES>
+__device__ __forceinline__ void load_pieces(T *to, const T *from, size_t stride, int rows, int columns, int lane) {
+    constexpr int kPer = CT * static_cast<int>(sizeof(T)) / BYTES; /* pieces of a row */
+    constexpr int kRows = 32 / kPer < 1 ? 1 : 32 / kPer;           /* rows at a time */
+    constexpr int kLanes = kPer < 32 ? kPer : 32;
+    const int row = lane / kLanes;
 #pragma unroll
-        for (int j = 0; j < kCheckpoint; ++j) {
-            const size_t t = k * kCheckpoint + j;
-            before[j] = s;
-            if (t < live) {
-                const Gates g = gates_of(x, rec, inp, b * d.is + t * d.it + c, rate, reset && reset[b * d.steps + t]);
-                s = g.a * s + g.beta * g.gate * g.x;
-            }
+    for (int i = 0; i < kPer / kLanes; ++i) {
+        const int piece = lane % kLanes + i * kLanes;
+        const int left = columns * static_cast<int>(sizeof(T)) - piece * BYTES;
+        if (left <= 0) continue;
+        const char *f = reinterpret_cast<const char *>(from + row * stride) + piece * BYTES;
+        const uint32_t t = shared_address(to + row * CT) + piece * BYTES;
+#pragma unroll
+        for (int r = 0; r < kSteps; r += kRows)
+            if (row + r < rows)
+                copy_async<BYTES>(t + r * CT * static_cast<int>(sizeof(T)), f + r * stride * sizeof(T),
+                                  left < BYTES ? left : BYTES);
+    }
+}
+
+/* Starts copying rows x columns elements into to [kSteps][CT]; `piece` bytes at a time (16, 4: asynchronous). */
+template <class T, int CT>
+__device__ __forceinline__ void load_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
+    if (piece == 16) {
+        load_pieces<T, CT, 16>(to, from, stride, rows, columns, lane);
+    } else if (piece == 4) {
+        load_pieces<T, CT, 4>(to, from, stride, rows, columns, lane);
+    } else {
+        for (int c = lane; c < columns; c += 32)
+#pragma unroll
+            for (int r = 0; r < kSteps; ++r)
+                if (r < rows) to[r * CT + c] = from[r * stride + c];
+    }
+}
+
+/* rows x columns elements of from [kSteps][CT] to global memory. */
+template <class T, int CT>
+__device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
+    if (piece == 16) {
+        constexpr int kPer = CT * static_cast<int>(sizeof(T)) / 16, kRows = 32 / kPer;
+        constexpr int kIn = 16 / static_cast<int>(sizeof(T));
+        const int row = lane / kPer, c = lane % kPer * kIn;
+        const T *f = from + row * CT + c;
+        T *t = to + row * stride + c;
+        if (c + kIn <= columns) {
+#pragma unroll
+            for (int r = 0; r < kSteps; r += kRows)
+                if (row + r < rows)
+                    *reinterpret_cast<Pack<T, kIn> *>(t + r * stride) =
+                        *reinterpret_cast<const Pack<T, kIn> *>(f + r * CT);
+        } else {
+            for (int r = 0; row + r < rows; r += kRows)
+                for (int i = 0; c + i < columns; ++i) t[r * stride + i] = f[r * CT + i];
         }
+    } else {
+        for (int c = lane; c < columns; c += 32)
 #pragma unroll
-        for (int j = kCheckpoint - 1; j >= 0; --j) {
-            const size_t t = k * kCheckpoint + j;
-            if (t >= d.steps) continue;
-            const size_t to = b * d.gs + t * d.gt + c;
-            float gx = 0.0f, gr = 0.0f, gi = 0.0f;
-            if (t < live) {
-                const bool anew = reset && reset[b * d.steps + t];
-                const Gates g = gates_of(x, rec, inp, b * d.is + t * d.it + c, rate, anew);
-                const float total = to_float(dh[b * d.os + t * d.ot + c]) + carry;
-                const float u = g.gate * g.x;
-                carry = g.a * total;
-                gx = total * g.beta * g.gate;
-                gi = gx * g.x * (1.0f - g.gate);
-                if (!anew && g.beta > 0.0f) {
-                    const float dlog = carry * (before[j] - g.a / g.beta * u);
-                    gr = dlog * g.log_a * (1.0f - g.open);
-                    sum += dlog * g.open;
+            for (int r = 0; r < kSteps; ++r)
+                if (r < rows) to[r * stride + c] = from[r * CT + c];
+    }
+}
+
+/* Bit j: step t0 + j starts anew. */
+__device__ __forceinline__ unsigned reset_bits(const uint8_t *reset, size_t at, int live, int lane) {
+    return reset ? __ballot_sync(0xffffffffu, lane < live && reset[at + lane]) : 0u;
+}
+
+/* ---- the scan over spans ---- */
+
+__device__ __forceinline__ unsigned load_acquire(const unsigned *p) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_release(unsigned *p, unsigned v) {
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ unsigned long long clock_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+template <int V> struct Lane {
+    float v[V];
+};
+
+template <int CT, int V>
+__device__ __forceinline__ void publish(const Spans &s, size_t item, unsigned what, const Lane<V> &a, const Lane<V> &b,
+                                        int lane) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (what == 2) {
+            __stcg(s.state + item * CT + lane * V + v, a.v[v]);
+        } else {
+            __stcg(s.map + item * 2 * CT + lane * V + v, a.v[v]);
+            __stcg(s.map + item * 2 * CT + CT + lane * V + v, b.v[v]);
+        }
+    }
+    __syncwarp();
+    if (lane == 0) {
+        __threadfence();
+        store_release(s.flag + item, what);
+    }
+}
+
+/* The state before span `span` > 0 of a tile; one warp. */
+template <int CT, int V>
+__device__ Lane<V> state_before(const Spans &s, unsigned span, unsigned tile, int lane) {
+    Lane<V> h;
+    int back = static_cast<int>(span) - 1; /* the last span of the window */
+    unsigned long long since = 0;
+    for (;;) { /* the nearest span whose state is there, every (A, H) from it on being there */
+        const int at = back - lane;
+        const unsigned f = at >= 0 ? load_acquire(s.flag + static_cast<size_t>(at) * s.tiles + tile) : 1u;
+        const unsigned ready = __ballot_sync(0xffffffffu, f == 2), missing = __ballot_sync(0xffffffffu, f == 0);
+        const unsigned before = ready ? (ready & (~ready + 1)) - 1 : 0xffffffffu;
+        if (!(missing & before)) {
+            if (ready) {
+                back -= __ffs(ready) - 1;
+                break;
+            }
+            back -= 32;
+            continue;
+        }
+        if (!since) since = clock_ns();
+        else if (clock_ns() - since > kWaitNs) {
+            if (lane == 0) atomicOr(s.status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
+#pragma unroll
+            for (int v = 0; v < V; ++v) h.v[v] = 0.0f;
+            return h;
+        }
+    }
+    __syncwarp();
+    const size_t first = static_cast<size_t>(back) * s.tiles + tile;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + first * CT + lane * V + v);
+#pragma unroll 4
+    for (unsigned j = back + 1; j < span; ++j) {
+        const float *m = s.map + (static_cast<size_t>(j) * s.tiles + tile) * 2 * CT + lane * V;
+#pragma unroll
+        for (int v = 0; v < V; ++v) h.v[v] = fmaf(__ldcg(m + v), h.v[v], __ldcg(m + CT + v));
+    }
+    return h;
+}
+
+/* Joins a CTA's spans.  Each warp brings its span's (A, H) of V channels a
+ * lane, in the order of the scan; returns the state before each warp's span.
+ * `after`: the state after the CTA's spans, of warp 0.  The barriers order
+ * *next (the CTA's next item) too. */
+template <int CT, int V, int WARPS>
+__device__ __forceinline__ Lane<V> join(const Spans &s, unsigned item, unsigned span, unsigned tile, const Lane<V> &map_a,
+                                        const Lane<V> &map_h, const Lane<V> &initial, float (*sa)[CT], float (*sh)[CT],
+                                        float *carry, int order, int warp, int lane, Lane<V> *after) {
+    if constexpr (WARPS == 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) after->v[v] = fmaf(map_a.v[v], initial.v[v], map_h.v[v]);
+        return initial;
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            sa[order][lane * V + v] = map_a.v[v];
+            sh[order][lane * V + v] = map_h.v[v];
+        }
+        Lane<V> h = initial; /* where the span before is done already, its state is read beside the inputs */
+        bool known = span == 0;
+        if (warp == 0 && span > 0) {
+            const size_t prev = static_cast<size_t>(span - 1) * s.tiles + tile;
+            if (load_acquire(s.flag + prev) == 2) {
+                known = true;
+#pragma unroll
+                for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + prev * CT + lane * V + v);
+            }
+            known = __all_sync(0xffffffffu, known);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            Lane<V> a, b;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                a.v[v] = 1.0f;
+                b.v[v] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float aw = sa[w][lane * V + v];
+                    b.v[v] = fmaf(aw, b.v[v], sh[w][lane * V + v]);
+                    a.v[v] *= aw;
                 }
             }
-            dx[to] = from_float<T>(gx);
-            drec[to] = from_float<T>(gr);
-            dinp[to] = from_float<T>(gi);
+            const bool last = span + 1 == s.spans;
+            if (!known) {
+                if (!last) publish<CT, V>(s, item, 1, a, b, lane);
+                h = state_before<CT, V>(s, span, tile, lane);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                carry[lane * V + v] = h.v[v];
+                after->v[v] = fmaf(a.v[v], h.v[v], b.v[v]);
+            }
+            if (!last) publish<CT, V>(s, item, 2, *after, b, lane);
         }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            h.v[v] = carry[lane * V + v];
+            for (int w = 0; w < order; ++w) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
+        }
+        return h;
     }
-    if (dstate_in) dstate_in[i] = carry;
-    partial[i] = sum;
 }
 
-__global__ void __launch_bounds__(kThreads)
-recurrence_decay(RecurrenceShape d, const float *decay, const float *partial, float *ddecay) {
-    const size_t c = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (c >= d.channels) return;
-    float s = 0.0f;
-    for (size_t b = 0; b < d.sequences; ++b) s += partial[b * d.channels + c];
-    ddecay[c] = -d.scale * sigmoid(decay[c]) * s;
+/* The items of a CTA: by the counter where spans wait for one another, else every gridDim.x-th. */
+struct Items {
+    bool counted;
+    unsigned now, next;
+};
+
+template <int WARPS> __device__ __forceinline__ Items first_items(const Spans &s, unsigned *mailbox) {
+    Items i;
+    i.counted = s.spans > 1;
+    if (!i.counted) {
+        i.now = blockIdx.x;
+        i.next = blockIdx.x + gridDim.x;
+    } else {
+        if (threadIdx.x == 0) {
+            mailbox[0] = atomicAdd(s.ticket, 1u);
+            mailbox[1] = atomicAdd(s.ticket, 1u);
+        }
+        __syncthreads();
+        i.now = mailbox[0];
+        i.next = mailbox[1];
+    }
+    return i;
 }
+
+/* ---- forward ---- */
+
+/* Lanes of V channels: 64 channels (128 bytes) a row for 16-bit types, 32 for f32. */
+template <class T> constexpr int kForwardV = sizeof(T) == 2 ? 2 : 1;
+
+template <class T, int V, bool SPECIAL>
+__device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *is, const float *rate, int live,
+                                             unsigned anew, float (&prod)[kSteps][V], float (&local)[kSteps][V], int lane) {
+    constexpr int CT = 32 * V;
+    float a_all[V], h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        a_all[v] = 1.0f;
+        h[v] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(xs + j * CT + lane * V);
+        const Pack<T, V> r = *reinterpret_cast<const Pack<T, V> *>(rs + j * CT + lane * V);
+        const Pack<T, V> i = *reinterpret_cast<const Pack<T, V> *>(is + j * CT + lane * V);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Decay s = decay_of(rate[v], fast_sigmoid(to_float(r.v[v])));
+            const float u = fast_sigmoid(to_float(i.v[v])) * to_float(x.v[v]);
+            float a = s.a, b = s.beta * u;
+            if (SPECIAL) {
+                if (anew >> j & 1) {
+                    a = 0.0f;
+                    b = u;
+                }
+                if (j >= live) {
+                    a = 1.0f;
+                    b = 0.0f;
+                }
+            }
+            a_all[v] *= a;
+            h[v] = fmaf(a, h[v], b);
+            prod[j][v] = a_all[v];
+            local[j][v] = h[v];
+        }
+    }
+}
+
+template <class T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(const ForwardArgs p, const Spans s) {
+    constexpr int V = kForwardV<T>, CT = 32 * V;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ float sa[WARPS][CT], sh[WARPS][CT], carry[CT];
+    __shared__ unsigned mailbox[2];
+    const RecurrenceShape &d = p.d;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 3 * kSteps * CT; /* two stages of x, rec, inp */
+    const size_t saved = (d.steps + kSteps - 1) / kSteps;
+
+    const auto start = [&](unsigned item, int stage) {
+        if (item < s.items) {
+            const unsigned span = item / s.tiles, tile = item % s.tiles;
+            const size_t b = tile / s.tiles_per_sequence, c = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
+            const size_t t = (static_cast<size_t>(span) * WARPS + warp) * kSteps;
+            const int live = live_steps(d, p.lengths, b, t);
+            const int columns = d.channels - c < CT ? static_cast<int>(d.channels - c) : CT;
+            const size_t at = b * d.is + t * d.it + c;
+            T *to = slots + stage * 3 * kSteps * CT;
+            load_rows<T, CT>(to, static_cast<const T *>(p.x) + at, d.it, live, columns, p.in_piece, lane);
+            load_rows<T, CT>(to + kSteps * CT, static_cast<const T *>(p.rec) + at, d.it, live, columns, p.in_piece, lane);
+            load_rows<T, CT>(to + 2 * kSteps * CT, static_cast<const T *>(p.inp) + at, d.it, live, columns, p.in_piece, lane);
+        }
+        copies_end();
+    };
+
+    Items items = first_items<WARPS>(s, mailbox);
+    int stage = 0;
+    start(items.now, stage);
+    while (items.now < s.items) {
+        const unsigned item = items.now, span = item / s.tiles, tile = item % s.tiles;
+        const size_t b = tile / s.tiles_per_sequence, c0 = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
+        const size_t t = (static_cast<size_t>(span) * WARPS + warp) * kSteps;
+        const int live = live_steps(d, p.lengths, b, t);
+        const int rows = t >= d.steps ? 0 : d.steps - t < kSteps ? static_cast<int>(d.steps - t) : kSteps;
+        const int columns = d.channels - c0 < CT ? static_cast<int>(d.channels - c0) : CT;
+        T *const xs = slots + stage * 3 * kSteps * CT;
+        start(items.next, stage ^ 1);
+        unsigned then = 0;
+        if (items.counted && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
+        const unsigned anew = reset_bits(p.reset, b * d.steps + t, live, lane);
+        float rate[V];
+        Lane<V> initial;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const size_t c = c0 + lane * V + v;
+            rate[v] = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
+            initial.v[v] = span == 0 && p.state_in && c < d.channels ? p.state_in[b * d.channels + c] : 0.0f;
+        }
+        copies_wait<1>();
+        __syncwarp();
+        float prod[kSteps][V], local[kSteps][V];
+        if (live == kSteps && !anew)
+            forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+        else
+            forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+        Lane<V> map_a, map_h, after;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            map_a.v[v] = prod[kSteps - 1][v];
+            map_h.v[v] = local[kSteps - 1][v];
+        }
+        const Lane<V> h0 = join<CT, V, WARPS>(s, item, span, tile, map_a, map_h, initial, sa, sh, carry, warp, warp, lane,
+                                              &after);
+        if (items.counted && threadIdx.x == 0) mailbox[0] = then;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const size_t c = c0 + lane * V + v;
+            if (c >= d.channels) continue;
+            if (p.checkpoints && rows > 0) p.checkpoints[(b * saved + t / kSteps) * d.channels + c] = h0.v[v];
+            if (p.state_out && warp == 0 && span + 1 == s.spans) p.state_out[b * d.channels + c] = after.v[v];
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                o.v[v] = from_float<T>(j < live ? fmaf(prod[j][v], h0.v[v], local[j][v]) : 0.0f);
+            *reinterpret_cast<Pack<T, V> *>(xs + j * CT + lane * V) = o;
+        }
+        __syncwarp();
+        store_rows<T, CT>(static_cast<T *>(p.h) + b * d.os + t * d.ot + c0, xs, d.ot, rows, columns, p.out_piece, lane);
+        if (WARPS > 1) __syncthreads(); /* mailbox, and sa, sh, carry are free again */
+        else __syncwarp();
+        items.now = items.next;
+        items.next = items.counted ? mailbox[0] : items.next + gridDim.x;
+        stage ^= 1;
+    }
+}
+
+/* ---- backward ---- */
+
+/* One channel a lane: the gates of 16 steps stay in registers. */
+template <class T, bool SPECIAL>
+__device__ __forceinline__ void backward_gates(const T *xs, const T *rs, const T *is, float rate, int live, unsigned anew,
+                                               float h, float (&open)[kSteps], float (&gate)[kSteps], float (&a)[kSteps],
+                                               float (&beta)[kSteps], float (&before)[kSteps], int lane) {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        open[j] = fast_sigmoid(to_float(rs[j * 32 + lane]));
+        gate[j] = fast_sigmoid(to_float(is[j * 32 + lane]));
+        const Decay s = decay_of(rate, open[j]);
+        a[j] = s.a;
+        beta[j] = s.beta;
+        if (SPECIAL) {
+            if (anew >> j & 1) {
+                a[j] = 0.0f;
+                beta[j] = 1.0f;
+            }
+            if (j >= live) { /* changes no state; its gradients are not taken */
+                a[j] = 1.0f;
+                beta[j] = 0.0f;
+            }
+        }
+        before[j] = h;
+        const float b = beta[j] * gate[j] * to_float(xs[j * 32 + lane]);
+        h = fmaf(a[j], h, SPECIAL && j >= live ? 0.0f : b);
+    }
+}
+
+template <class T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(const BackwardArgs p, const Spans s) {
+    constexpr int CT = 32;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ float sa[WARPS][CT], sh[WARPS][CT], carry[CT], sums[WARPS][CT];
+    __shared__ unsigned mailbox[2];
+    const RecurrenceShape &d = p.d;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    constexpr int kSlot = kSteps * CT;
+    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
+    const size_t saved = (d.steps + kSteps - 1) / kSteps;
+
+    /* spans in the order of the scan: the last steps first */
+    const auto step_of = [&](unsigned span) {
+        return (static_cast<size_t>(s.spans - 1 - span) * WARPS + warp) * kSteps;
+    };
+    const auto start = [&](unsigned item, int stage) {
+        if (item < s.items) {
+            const unsigned tile = item % s.tiles;
+            const size_t b = tile / s.tiles_per_sequence, c = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
+            const size_t t = step_of(item / s.tiles);
+            const int live = live_steps(d, p.lengths, b, t);
+            const int columns = d.channels - c < CT ? static_cast<int>(d.channels - c) : CT;
+            const size_t at = b * d.is + t * d.it + c;
+            T *to = slots + stage * 4 * kSlot;
+            load_rows<T, CT>(to, static_cast<const T *>(p.x) + at, d.it, live, columns, p.in_piece, lane);
+            load_rows<T, CT>(to + kSlot, static_cast<const T *>(p.rec) + at, d.it, live, columns, p.in_piece, lane);
+            load_rows<T, CT>(to + 2 * kSlot, static_cast<const T *>(p.inp) + at, d.it, live, columns, p.in_piece, lane);
+            load_rows<T, CT>(to + 3 * kSlot, static_cast<const T *>(p.dh) + b * d.os + t * d.ot + c, d.ot, live, columns,
+                             p.dh_piece, lane);
+        }
+        copies_end();
+    };
+
+    Items items = first_items<WARPS>(s, mailbox);
+    int stage = 0;
+    start(items.now, stage);
+    while (items.now < s.items) {
+        const unsigned item = items.now, span = item / s.tiles, tile = item % s.tiles;
+        const size_t b = tile / s.tiles_per_sequence, c0 = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
+        const size_t c = c0 + lane, t = step_of(span);
+        const int live = live_steps(d, p.lengths, b, t);
+        const int rows = t >= d.steps ? 0 : d.steps - t < kSteps ? static_cast<int>(d.steps - t) : kSteps;
+        const int columns = d.channels - c0 < CT ? static_cast<int>(d.channels - c0) : CT;
+        const bool in = c < d.channels;
+        T *const xs = slots + stage * 4 * kSlot;
+        start(items.next, stage ^ 1);
+        unsigned then = 0;
+        if (items.counted && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
+        const unsigned anew = reset_bits(p.reset, b * d.steps + t, live, lane);
+        const float rate = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
+        const float h = in && rows > 0 ? p.checkpoints[(b * saved + t / kSteps) * d.channels + c] : 0.0f;
+        Lane<1> initial, map_a, map_h, after;
+        initial.v[0] = span == 0 && p.dstate_out && in ? p.dstate_out[b * d.channels + c] : 0.0f;
+        copies_wait<1>();
+        __syncwarp();
+        float open[kSteps], gate[kSteps], a[kSteps], beta[kSteps], before[kSteps];
+        const bool plain = live == kSteps && !anew;
+        if (plain)
+            backward_gates<T, false>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, open, gate, a, beta, before, lane);
+        else
+            backward_gates<T, true>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, open, gate, a, beta, before, lane);
+        map_a.v[0] = 1.0f;
+        map_h.v[0] = 0.0f;
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const float g = j < live ? to_float(xs[3 * kSlot + j * CT + lane]) : 0.0f;
+            map_h.v[0] = a[j] * (g + map_h.v[0]);
+            map_a.v[0] *= a[j];
+        }
+        float grad = join<CT, 1, WARPS>(s, item, span, tile, map_a, map_h, initial, sa, sh, carry, WARPS - 1 - warp, warp,
+                                        lane, &after).v[0];
+        if (items.counted && threadIdx.x == 0) mailbox[0] = then;
+        if (p.dstate_in && in && warp == 0 && span + 1 == s.spans) p.dstate_in[b * d.channels + c] = after.v[0];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const int at = j * CT + lane;
+            float gx = 0.0f, gr = 0.0f, gi = 0.0f;
+            if (j < live) {
+                const float total = grad + to_float(xs[3 * kSlot + at]), x = to_float(xs[at]);
+                grad = a[j] * total;
+                gx = total * beta[j] * gate[j];
+                gi = gx * x * (1.0f - gate[j]);
+                if (!(anew >> j & 1) && beta[j] > 0.0f) {
+                    const float dlog = grad * (before[j] - a[j] * fast_rcp(beta[j]) * gate[j] * x) * open[j];
+                    gr = dlog * rate * (1.0f - open[j]);
+                    sum += dlog;
+                }
+            }
+            xs[at] = from_float<T>(gx);
+            xs[kSlot + at] = from_float<T>(gr);
+            xs[2 * kSlot + at] = from_float<T>(gi);
+        }
+        if (p.partial) {
+            if (WARPS > 1) {
+                sums[warp][lane] = sum;
+                __syncthreads();
+                if (warp == 0) {
+                    sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WARPS; ++w) sum += sums[w][lane];
+                }
+            }
+            if (warp == 0 && in) p.partial[(static_cast<size_t>(span) * d.sequences + b) * d.channels + c] = sum;
+        }
+        __syncwarp();
+        const size_t to = b * d.gs + t * d.gt + c0;
+        store_rows<T, CT>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
+        store_rows<T, CT>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
+        store_rows<T, CT>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
+        if (WARPS > 1) __syncthreads(); /* mailbox, and sa, sh, carry, sums are free again */
+        else __syncwarp();
+        items.now = items.next;
+        items.next = items.counted ? mailbox[0] : items.next + gridDim.x;
+        stage ^= 1;
+    }
+}
+
+/* ddecay from the sums of dlog a / rate over all steps: parts [parts, channels]. */
+__global__ void __launch_bounds__(256)
+recurrence_decay(const float *decay, const float *parts, size_t rows, size_t channels, float scale, float *ddecay) {
+    const size_t c = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= channels) return;
+    float s = 0.0f;
+    for (size_t r = 0; r < rows; ++r) s += parts[r * channels + c];
+    ddecay[c] = -scale / (1.0f + expf(-decay[c])) * s;
+}
+
+/* ---- host side ---- */
 
 bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     if (!d || !d->sequences || !d->steps || !d->channels || !type_known(d->type) || !(d->decay_scale >= 0.0f) ||
         d->steps > 0x7fffffffu)
         return false;
-    size_t rows, all;
-    if (!product(d->sequences, d->channels, 0x7fffffffu, &rows) || !product(rows, d->steps, SIZE_MAX / 64, &all))
+    size_t rows, all, items;
+    if (!product(d->sequences, d->channels, 0x7fffffffu, &rows) || !product(rows, d->steps, SIZE_MAX / 64, &all) ||
+        !product(d->sequences * ((d->channels + 31) / 32), (d->steps + kSteps - 1) / kSteps, 0x7fffffffu, &items))
         return false;
     s->sequences = d->sequences;
     s->steps = d->steps;
@@ -149,12 +677,76 @@ bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     return s->it >= d->channels && s->ot >= d->channels && s->gt >= d->channels;
 }
 
+struct Layout {
+    Spans spans;
+    size_t flags_bytes, bytes;
+};
+
+/* `warps` spans of 16 steps a CTA, `tile` channels. */
+Layout spans_of(const RecurrenceShape &d, int warps, int tile, void *workspace) {
+    Layout l{};
+    Spans &s = l.spans;
+    s.spans = static_cast<unsigned>((d.steps + warps * kSteps - 1) / (warps * kSteps));
+    s.tiles_per_sequence = static_cast<unsigned>((d.channels + tile - 1) / tile);
+    s.tiles = static_cast<unsigned>(d.sequences * s.tiles_per_sequence);
+    s.items = s.spans * s.tiles;
+    if (s.spans > 1) {
+        char *at = static_cast<char *>(workspace);
+        l.flags_bytes = align_up(16 + static_cast<size_t>(s.items) * 4, 16);
+        const size_t row = static_cast<size_t>(s.items) * tile * sizeof(float);
+        s.ticket = reinterpret_cast<unsigned *>(at);
+        s.flag = s.ticket + 4;
+        s.map = reinterpret_cast<float *>(at + l.flags_bytes);
+        s.state = reinterpret_cast<float *>(at + l.flags_bytes + 2 * row);
+        l.bytes = l.flags_bytes + 3 * row;
+    }
+    return l;
+}
+
+int warps_for(const RecurrenceShape &d) { return d.steps <= kSteps ? 1 : kWarps; }
+int forward_tile(int type) { return type == TB_TYPE_F32 ? 32 : 64; }
+
+/* Rows of partial sums for ddecay, and behind them the parts that they are first summed into. */
+size_t partial_rows(const RecurrenceShape &d, unsigned spans) { return d.sequences * spans; }
+size_t partial_bytes(const RecurrenceShape &d, unsigned spans) {
+    const size_t rows = partial_rows(d, spans);
+    return (rows + column_parts(rows)) * d.channels * sizeof(float);
+}
+
+/* Largest piece that every row of a tensor starts and goes on at. */
+int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t size, int least) {
+    const size_t all = reinterpret_cast<uintptr_t>(p) | sequence_stride * size | step_stride * size;
+    return all % 16 == 0 ? 16 : all % 4 == 0 && least == 4 ? 4 : 0;
+}
+
+/* Launches a kernel of persistent CTAs over l's items. */
+template <class Kernel, class Args>
+int launch_items(Kernel kernel, const Args &args, Layout &l, int warps, size_t shared, cudaStream_t st) {
+    int dev = 0, sms = 0, per_sm = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, shared) != cudaSuccess)
+        return 0;
+    if (l.spans.spans > 1) {
+        l.spans.status = tb_status_slot(st);
+        if (!l.spans.status || cudaMemsetAsync(l.spans.ticket, 0, l.flags_bytes, st) != cudaSuccess) return 0;
+    }
+    const unsigned most = static_cast<unsigned>(sms * per_sm);
+    kernel<<<l.spans.items < most ? l.spans.items : most, warps * 32, shared, st>>>(args, l.spans);
+    return launched();
+}
+
 } /* namespace */
 
 extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_desc *desc) {
     RecurrenceShape s;
     if (!recurrence_shape(desc, &s)) return 0;
-    return s.sequences * s.channels * sizeof(float);
+    const int warps = warps_for(s);
+    const Layout f = spans_of(s, warps, forward_tile(desc->type), nullptr), b = spans_of(s, warps, 32, nullptr);
+    const size_t back = align_up(b.bytes, 16) + partial_bytes(s, b.spans.spans);
+    return f.bytes > back ? f.bytes : back;
 }
 
 extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *desc, const void *x,
@@ -170,14 +762,19 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
         !aligned(checkpoints, 4) || !aligned(workspace, 16) || h == x || h == recurrence_gate || h == input_gate)
         return 0;
     cudaGetLastError(); /* report these launches only */
+    ForwardArgs p{s, x, recurrence_gate, input_gate, decay, state_in, reset, lengths, h, state_out, checkpoints, 0, 0};
+    const uintptr_t in = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(recurrence_gate) |
+                         reinterpret_cast<uintptr_t>(input_gate);
+    p.in_piece = piece_of(reinterpret_cast<const void *>(in), s.is, s.it, size, 4);
+    p.out_piece = piece_of(h, s.os, s.ot, size, 16);
+    const int warps = warps_for(s), tile = forward_tile(desc->type);
+    Layout l = spans_of(s, warps, tile, workspace);
+    const size_t shared = static_cast<size_t>(warps) * 2 * 3 * kSteps * tile * size;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        const unsigned grid = static_cast<unsigned>((s.sequences * s.channels + kThreads - 1) / kThreads);
-        recurrence_forward<T><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-            s, static_cast<const T *>(x), static_cast<const T *>(recurrence_gate),
-            static_cast<const T *>(input_gate), decay, reset, lengths, state_in, static_cast<T *>(h), state_out,
-            checkpoints);
-        return launched();
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        return warps == 1 ? launch_items(recurrence_forward<T, 1>, p, l, 1, shared, st)
+                          : launch_items(recurrence_forward<T, kWarps>, p, l, kWarps, shared, st);
     });
 }
 
@@ -197,26 +794,37 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
         !aligned(ddecay, 4) || !aligned(dstate_in, 4) || !aligned(workspace, 16))
         return 0;
     const void *in[] = {x, recurrence_gate, input_gate, dh}, *out[] = {dx, drecurrence_gate, dinput_gate};
+    uintptr_t ins = 0, outs = 0;
     for (int i = 0; i < 3; ++i) {
         for (const void *p : in)
             if (out[i] == p) return 0;
         if (out[i] == out[(i + 1) % 3]) return 0;
+        ins |= reinterpret_cast<uintptr_t>(in[i]);
+        outs |= reinterpret_cast<uintptr_t>(out[i]);
     }
     cudaGetLastError(); /* report these launches only */
-    return with_type(desc->type, [&](auto t) {
+    const int warps = warps_for(s);
+    Layout l = spans_of(s, warps, 32, workspace);
+    float *partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + align_up(l.bytes, 16));
+    BackwardArgs p{s, x, recurrence_gate, input_gate, dh, decay, checkpoints, dstate_out, reset, lengths, dx,
+                   drecurrence_gate, dinput_gate, ddecay ? partial : nullptr, dstate_in, 0, 0, 0};
+    p.in_piece = piece_of(reinterpret_cast<const void *>(ins), s.is, s.it, size, 4);
+    p.dh_piece = piece_of(dh, s.os, s.ot, size, 4);
+    p.out_piece = piece_of(reinterpret_cast<const void *>(outs), s.gs, s.gt, size, 16);
+    const size_t shared = static_cast<size_t>(warps) * 2 * 4 * kSteps * 32 * size;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        float *partial = static_cast<float *>(workspace);
-        const unsigned grid = static_cast<unsigned>((s.sequences * s.channels + kThreads - 1) / kThreads);
-        recurrence_backward<T><<<grid, kThreads, 0, st>>>(
-            s, static_cast<const T *>(x), static_cast<const T *>(recurrence_gate),
-            static_cast<const T *>(input_gate), decay, reset, lengths, checkpoints, static_cast<const T *>(dh),
-            dstate_out, static_cast<T *>(dx), static_cast<T *>(drecurrence_gate), static_cast<T *>(dinput_gate),
-            partial, dstate_in);
-        if (!launched()) return 0;
-        if (ddecay)
-            recurrence_decay<<<static_cast<unsigned>((s.channels + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-                s, decay, partial, ddecay);
-        return launched();
+        return warps == 1 ? launch_items(recurrence_backward<T, 1>, p, l, 1, shared, st)
+                          : launch_items(recurrence_backward<T, kWarps>, p, l, kWarps, shared, st);
     });
+    if (!ok || !ddecay) return ok;
+    const size_t rows = partial_rows(s, l.spans.spans), parts = column_parts(rows);
+    float *sums = partial + rows * s.channels;
+    column_sums<<<dim3(static_cast<unsigned>((s.channels + 31) / 32), static_cast<unsigned>(parts)), kColumnThreads, 0,
+                  st>>>(partial, rows, s.channels, sums);
+    if (!launched()) return 0;
+    recurrence_decay<<<static_cast<unsigned>((s.channels + 255) / 256), 256, 0, st>>>(decay, sums, parts, s.channels,
+                                                                                    s.scale, ddecay);
+    return launched();
 }

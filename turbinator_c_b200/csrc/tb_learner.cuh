@@ -45,6 +45,65 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+/* ---- functions of the special unit, subnormal results flushed ---- */
+
+__device__ __forceinline__ float fast_exp2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float fast_rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float fast_sqrt(float v) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float kLog2e = 1.44269504f;
+/* 1 / (1 + e^-v): a few units in the last place (2 from each function, one
+ * from the argument's product for |v| < 8, where it matters). */
+__device__ __forceinline__ float fast_sigmoid(float v) { return fast_rcp(1.0f + fast_exp2(-kLog2e * v)); }
+
+/* ---- sums over the rows of partial [rows, columns] in f32 ---- */
+
+constexpr int kColumnThreads = 512;       /* 32 columns x 16 rows at a time */
+constexpr size_t kColumnRows = 512;       /* rows that one CTA sums */
+constexpr size_t kColumnParts = 64;       /* parts of the rows at most */
+
+/* Part blockIdx.y of the rows of 32 columns; out [gridDim.y, columns]. */
+static __global__ void __launch_bounds__(kColumnThreads)
+column_sums(const float *partial, size_t rows, size_t columns, float *out) {
+    __shared__ float sums[16][33];
+    const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
+    const size_t c = static_cast<size_t>(blockIdx.x) * 32 + lane;
+    const size_t per = (rows + gridDim.y - 1) / gridDim.y, first = per * blockIdx.y;
+    const size_t last = first + per < rows ? first + per : rows;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < columns) {
+        size_t r = first + row;
+        for (; r + 48 < last; r += 64)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += partial[(r + 16 * i) * columns + c];
+        for (; r < last; r += 16) s[0] += partial[r * columns + c];
+    }
+    sums[row][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (row == 0 && c < columns) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += sums[i][lane];
+        out[blockIdx.y * columns + c] = t;
+    }
+}
+
+inline size_t column_parts(size_t rows) {
+    const size_t p = (rows + kColumnRows - 1) / kColumnRows;
+    return p < kColumnParts ? p : kColumnParts;
+}
+
 /* ---- host side ---- */
 
 inline size_t type_size(int type) { return type == TB_TYPE_F32 ? 4 : 2; }
