@@ -85,28 +85,48 @@ __device__ __forceinline__ int live_steps(const RecurrenceShape &d, const int32_
     return live - t0 < kSteps ? static_cast<int>(live - t0) : kSteps;
 }
 
-/* One step's decay.  p = e^(log a) - 1 keeps the digits of 1 - a^2 = -p (2 + p)
- * where a is near 1: below 0.35 from its series (the next term is below 2e-8
- * of p), past it from e^x. */
+/* e^l - 1 for -kNear <= l <= 0 from its series; the next term is below 2e-8
+ * of it. */
+constexpr float kNear = 0.35f;
+__device__ __forceinline__ F2 expm1_near(F2 l) {
+    F2 q = fma2(l, both(1.0f / 5040.0f), both(1.0f / 720.0f));
+    q = fma2(q, l, both(1.0f / 120.0f));
+    q = fma2(q, l, both(1.0f / 24.0f));
+    q = fma2(q, l, both(1.0f / 6.0f));
+    q = fma2(q, l, both(0.5f));
+    q = fma2(q, l, both(1.0f));
+    return mul2(l, q);
+}
+
+/* Decays of two steps or channels.  p = e^(log a) - 1 keeps the digits of
+ * 1 - a^2 = -p (2 + p) where a is near 1.  NEAR: no log a of the warp can be
+ * below -kNear (sigmoid <= 1, so the rates decide), which saves the
+ * exponential and the choice: 19 of the 50 instructions of a pair's step. */
 struct Decay {
-    float log_a, a, beta;
+    F2 a, beta;
 };
-__device__ __forceinline__ Decay decay_of(float rate, float open) {
-    Decay s;
-    s.log_a = rate * open;
-    const float l = s.log_a;
-    float q = fmaf(l, 1.0f / 5040.0f, 1.0f / 720.0f);
-    q = fmaf(q, l, 1.0f / 120.0f);
-    q = fmaf(q, l, 1.0f / 24.0f);
-    q = fmaf(q, l, 1.0f / 6.0f);
-    q = fmaf(q, l, 0.5f);
-    q = fmaf(q, l, 1.0f);
-    const float e = fast_exp2(kLog2e * l);
-    const bool near = l > -0.35f;
-    const float p = near ? l * q : e - 1.0f;
-    s.a = near ? 1.0f + p : e;
-    s.beta = fast_sqrt(-p * (2.0f + p));
-    return s;
+template <bool NEAR> __device__ __forceinline__ Decay decay_of(F2 rate, F2 open) {
+    const F2 l = mul2(rate, open);
+    F2 p = expm1_near(l), a = add2(p, both(1.0f));
+    if (!NEAR) {
+        float l0, l1, p0, p1, a0, a1;
+        split(l, l0, l1);
+        split(p, p0, p1);
+        split(a, a0, a1);
+        if (!(l0 >= -kNear)) {
+            a0 = fast_exp2(kLog2e * l0);
+            p0 = a0 - 1.0f;
+        }
+        if (!(l1 >= -kNear)) {
+            a1 = fast_exp2(kLog2e * l1);
+            p1 = a1 - 1.0f;
+        }
+        a = pair(a0, a1);
+        p = pair(p0, p1);
+    }
+    float s0, s1;
+    split(mul2(p, fma2(p, both(-1.0f), both(-2.0f))), s0, s1);
+    return {a, pair(fast_sqrt(s0), fast_sqrt(s1))};
 }
 
 /* ---- rows between global and the warp's shared memory ---- */
@@ -226,10 +246,7 @@ __device__ __forceinline__ void publish(const Spans &s, size_t item, unsigned wh
         }
     }
     __syncwarp();
-    if (lane == 0) {
-        __threadfence();
-        store_release(s.flag + item, what);
-    }
+    if (lane == 0) store_release(s.flag + item, what); /* after the warp's stores */
 }
 
 /* The state before span `span` > 0 of a tile; one warp. */
@@ -315,9 +332,8 @@ __device__ __forceinline__ Lane<V> join(const Spans &s, unsigned item, unsigned 
                     a.v[v] *= aw;
                 }
             }
-            const bool last = span + 1 == s.spans;
             if (!known) {
-                if (!last) publish<CT, V>(s, item, 1, a, b, lane);
+                if (span + 1 != s.spans) publish<CT, V>(s, item, 1, a, b, lane);
                 h = state_before<CT, V>(s, span, tile, lane);
             }
 #pragma unroll
@@ -325,9 +341,9 @@ __device__ __forceinline__ Lane<V> join(const Spans &s, unsigned item, unsigned 
                 carry[lane * V + v] = h.v[v];
                 after->v[v] = fmaf(a.v[v], h.v[v], b.v[v]);
             }
-            if (!last) publish<CT, V>(s, item, 2, *after, b, lane);
         }
         __syncthreads();
+        if (warp == 0 && span + 1 != s.spans) publish<CT, V>(s, item, 2, *after, *after, lane);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             h.v[v] = carry[lane * V + v];
@@ -366,40 +382,56 @@ template <int WARPS> __device__ __forceinline__ Items first_items(const Spans &s
 /* Lanes of V channels: 64 channels (128 bytes) a row for 16-bit types, 32 for f32. */
 template <class T> constexpr int kForwardV = sizeof(T) == 2 ? 2 : 1;
 
-template <class T, int V, bool SPECIAL>
+/* Pairs: two channels of a lane (V = 2), or two steps of its channel.  FAST:
+ * the rates are NEAR, every step is live and none starts anew. */
+template <class T, int V, bool FAST>
 __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *is, const float *rate, int live,
                                              unsigned anew, float (&prod)[kSteps][V], float (&local)[kSteps][V], int lane) {
     constexpr int CT = 32 * V;
-    float a_all[V], h[V];
+    constexpr int second = V == 2 ? 1 : CT; /* from a pair's first element to its second */
+    float a_one = 1.0f, h_one = 0.0f;
+    F2 a_all = both(1.0f), h = both(0.0f);
+    const F2 rates = pair(rate[0], rate[V - 1]);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        a_all[v] = 1.0f;
-        h[v] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(xs + j * CT + lane * V);
-        const Pack<T, V> r = *reinterpret_cast<const Pack<T, V> *>(rs + j * CT + lane * V);
-        const Pack<T, V> i = *reinterpret_cast<const Pack<T, V> *>(is + j * CT + lane * V);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const Decay s = decay_of(rate[v], fast_sigmoid(to_float(r.v[v])));
-            const float u = fast_sigmoid(to_float(i.v[v])) * to_float(x.v[v]);
-            float a = s.a, b = s.beta * u;
-            if (SPECIAL) {
-                if (anew >> j & 1) {
-                    a = 0.0f;
-                    b = u;
-                }
-                if (j >= live) {
-                    a = 1.0f;
-                    b = 0.0f;
-                }
+    for (int j = 0; j < kSteps; j += 3 - V) {
+        const int at = j * CT + lane * V;
+        const auto two = [&](const T *p) {
+            if constexpr (V == 2) {
+                const Pack<T, 2> v = *reinterpret_cast<const Pack<T, 2> *>(p + at);
+                return pair(to_float(v.v[0]), to_float(v.v[1]));
+            } else {
+                return pair(to_float(p[at]), to_float(p[at + second]));
             }
-            a_all[v] *= a;
-            h[v] = fmaf(a, h[v], b);
-            prod[j][v] = a_all[v];
-            local[j][v] = h[v];
+        };
+        const Decay s = decay_of<FAST>(rates, sigmoid2(two(rs)));
+        const F2 u = mul2(sigmoid2(two(is)), two(xs));
+        F2 a = s.a, b = mul2(s.beta, u);
+        if (!FAST) {
+            float a0, a1, b0, b1, u0, u1;
+            split(a, a0, a1);
+            split(b, b0, b1);
+            split(u, u0, u1);
+            const int j1 = V == 2 ? j : j + 1;
+            if (anew >> j & 1) a0 = 0.0f, b0 = u0;
+            if (anew >> j1 & 1) a1 = 0.0f, b1 = u1;
+            if (j >= live) a0 = 1.0f, b0 = 0.0f;
+            if (j1 >= live) a1 = 1.0f, b1 = 0.0f;
+            a = pair(a0, a1);
+            b = pair(b0, b1);
+        }
+        if constexpr (V == 2) {
+            a_all = mul2(a_all, a);
+            h = fma2(a, h, b);
+            split(a_all, prod[j][0], prod[j][1]);
+            split(h, local[j][0], local[j][1]);
+        } else {
+            float a0, a1, b0, b1;
+            split(a, a0, a1);
+            split(b, b0, b1);
+            prod[j][0] = a_one *= a0;
+            local[j][0] = h_one = fmaf(a0, h_one, b0);
+            prod[j + 1][0] = a_one *= a1;
+            local[j + 1][0] = h_one = fmaf(a1, h_one, b1);
         }
     }
 }
@@ -457,10 +489,10 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
         copies_wait<1>();
         __syncwarp();
         float prod[kSteps][V], local[kSteps][V];
-        if (live == kSteps && !anew)
-            forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
-        else
+        if (live == kSteps && !anew && __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear))
             forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+        else
+            forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
         Lane<V> map_a, map_h, after;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -478,12 +510,18 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
             if (p.state_out && warp == 0 && span + 1 == s.spans) p.state_out[b * d.channels + c] = after.v[v];
         }
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                o.v[v] = from_float<T>(j < live ? fmaf(prod[j][v], h0.v[v], local[j][v]) : 0.0f);
-            *reinterpret_cast<Pack<T, V> *>(xs + j * CT + lane * V) = o;
+        for (int j = 0; j < kSteps; j += 3 - V) {
+            float o0, o1;
+            split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(h0.v[0], h0.v[V - 1]),
+                       pair(local[j][0], local[j + 2 - V][V - 1])), o0, o1);
+            if constexpr (V == 2) {
+                Pack<T, 2> o = {{from_float<T>(o0), from_float<T>(o1)}};
+                if (j >= live) o = {{from_float<T>(0.0f), from_float<T>(0.0f)}};
+                *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = o;
+            } else {
+                xs[j * CT + lane] = from_float<T>(j < live ? o0 : 0.0f);
+                xs[(j + 1) * CT + lane] = from_float<T>(j + 1 < live ? o1 : 0.0f);
+            }
         }
         __syncwarp();
         store_rows<T, CT>(static_cast<T *>(p.h) + b * d.os + t * d.ot + c0, xs, d.ot, rows, columns, p.out_piece, lane);
@@ -497,31 +535,46 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
 
 /* ---- backward ---- */
 
-/* One channel a lane: the gates of 16 steps stay in registers. */
-template <class T, bool SPECIAL>
+/* One channel a lane, pairs of steps.  For each step what the gradients need
+ * of it: a; w = beta gate, so that dx = total w; z = x (1 - gate), so that
+ * dinp = dx z; q = open (h_(t-1) - a/beta gate x), so that a total q is
+ * dlog a times open; m = 1 - open. */
+template <class T, bool FAST>
 __device__ __forceinline__ void backward_gates(const T *xs, const T *rs, const T *is, float rate, int live, unsigned anew,
-                                               float h, float (&open)[kSteps], float (&gate)[kSteps], float (&a)[kSteps],
-                                               float (&beta)[kSteps], float (&before)[kSteps], int lane) {
+                                               float h, float (&a)[kSteps], float (&w)[kSteps], float (&z)[kSteps],
+                                               float (&q)[kSteps], float (&m)[kSteps], int lane) {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        open[j] = fast_sigmoid(to_float(rs[j * 32 + lane]));
-        gate[j] = fast_sigmoid(to_float(is[j * 32 + lane]));
-        const Decay s = decay_of(rate, open[j]);
-        a[j] = s.a;
-        beta[j] = s.beta;
-        if (SPECIAL) {
-            if (anew >> j & 1) {
-                a[j] = 0.0f;
-                beta[j] = 1.0f;
-            }
-            if (j >= live) { /* changes no state; its gradients are not taken */
-                a[j] = 1.0f;
-                beta[j] = 0.0f;
-            }
+    for (int j = 0; j < kSteps; j += 2) {
+        const int at = j * 32 + lane;
+        const auto two = [&](const T *p) { return pair(to_float(p[at]), to_float(p[at + 32])); };
+        const F2 open = sigmoid2(two(rs)), gate = sigmoid2(two(is)), x = two(xs);
+        const Decay s = decay_of<FAST>(both(rate), open);
+        const F2 u = mul2(gate, x);
+        float b0, b1, beta0, beta1, a0, a1, u0, u1;
+        split(s.a, a0, a1);
+        split(s.beta, beta0, beta1);
+        split(mul2(s.beta, u), b0, b1);
+        split(u, u0, u1);
+        /* where beta is 0 nothing decays: no gradient of log a */
+        float r0 = beta0 > 0.0f ? fast_rcp(beta0) : 0.0f, r1 = beta1 > 0.0f ? fast_rcp(beta1) : 0.0f;
+        bool g0 = beta0 > 0.0f, g1 = beta1 > 0.0f;
+        if (!FAST) {
+            if (anew >> j & 1) a0 = 0.0f, beta0 = 1.0f, b0 = u0, g0 = false;
+            if (anew >> (j + 1) & 1) a1 = 0.0f, beta1 = 1.0f, b1 = u1, g1 = false;
+            if (j >= live) a0 = 1.0f, b0 = 0.0f; /* changes no state; its gradients are not taken */
+            if (j + 1 >= live) a1 = 1.0f, b1 = 0.0f;
         }
-        before[j] = h;
-        const float b = beta[j] * gate[j] * to_float(xs[j * 32 + lane]);
-        h = fmaf(a[j], h, SPECIAL && j >= live ? 0.0f : b);
+        const float h1 = fmaf(a0, h, b0);
+        float q0, q1;
+        split(mul2(open, fma2(mul2(pair(a0, a1), pair(r0, r1)), mul2(u, both(-1.0f)), pair(h, h1))), q0, q1);
+        h = fmaf(a1, h1, b1);
+        a[j] = a0;
+        a[j + 1] = a1;
+        q[j] = g0 ? q0 : 0.0f;
+        q[j + 1] = g1 ? q1 : 0.0f;
+        split(mul2(pair(beta0, beta1), gate), w[j], w[j + 1]);
+        split(fma2(u, both(-1.0f), x), z[j], z[j + 1]);
+        split(fma2(open, both(-1.0f), both(1.0f)), m[j], m[j + 1]);
     }
 }
 
@@ -581,12 +634,11 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
         initial.v[0] = span == 0 && p.dstate_out && in ? p.dstate_out[b * d.channels + c] : 0.0f;
         copies_wait<1>();
         __syncwarp();
-        float open[kSteps], gate[kSteps], a[kSteps], beta[kSteps], before[kSteps];
-        const bool plain = live == kSteps && !anew;
-        if (plain)
-            backward_gates<T, false>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, open, gate, a, beta, before, lane);
+        float a[kSteps], w[kSteps], z[kSteps], q[kSteps], m[kSteps];
+        if (live == kSteps && !anew && __all_sync(0xffffffffu, rate >= -kNear))
+            backward_gates<T, true>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
         else
-            backward_gates<T, true>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, open, gate, a, beta, before, lane);
+            backward_gates<T, false>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
         map_a.v[0] = 1.0f;
         map_h.v[0] = 0.0f;
 #pragma unroll
@@ -599,26 +651,34 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
                                         lane, &after).v[0];
         if (items.counted && threadIdx.x == 0) mailbox[0] = then;
         if (p.dstate_in && in && warp == 0 && span + 1 == s.spans) p.dstate_in[b * d.channels + c] = after.v[0];
-        float sum = 0.0f;
+        F2 sums2 = both(0.0f);
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
+        for (int j = kSteps - 2; j >= 0; j -= 2) {
             const int at = j * CT + lane;
-            float gx = 0.0f, gr = 0.0f, gi = 0.0f;
-            if (j < live) {
-                const float total = grad + to_float(xs[3 * kSlot + at]), x = to_float(xs[at]);
-                grad = a[j] * total;
-                gx = total * beta[j] * gate[j];
-                gi = gx * x * (1.0f - gate[j]);
-                if (!(anew >> j & 1) && beta[j] > 0.0f) {
-                    const float dlog = grad * (before[j] - a[j] * fast_rcp(beta[j]) * gate[j] * x) * open[j];
-                    gr = dlog * rate * (1.0f - open[j]);
-                    sum += dlog;
-                }
-            }
-            xs[at] = from_float<T>(gx);
-            xs[kSlot + at] = from_float<T>(gr);
-            xs[2 * kSlot + at] = from_float<T>(gi);
+            const bool on0 = j < live, on1 = j + 1 < live;
+            const float total1 = grad + (on1 ? to_float(xs[3 * kSlot + at + CT]) : 0.0f), grad1 = a[j + 1] * total1;
+            const float total0 = grad1 + (on0 ? to_float(xs[3 * kSlot + at]) : 0.0f);
+            grad = a[j] * total0;
+            const F2 gx = mul2(pair(total0, total1), pair(w[j], w[j + 1]));
+            const F2 dlog = mul2(pair(grad, grad1), pair(q[j], q[j + 1]));
+            float x0, x1, r0, r1, i0, i1, d0, d1;
+            split(gx, x0, x1);
+            split(mul2(gx, pair(z[j], z[j + 1])), i0, i1);
+            split(dlog, d0, d1);
+            split(mul2(mul2(dlog, both(rate)), pair(m[j], m[j + 1])), r0, r1);
+            if (!on0) x0 = i0 = r0 = d0 = 0.0f;
+            if (!on1) x1 = i1 = r1 = d1 = 0.0f;
+            sums2 = add2(sums2, pair(d0, d1));
+            xs[at] = from_float<T>(x0);
+            xs[at + CT] = from_float<T>(x1);
+            xs[kSlot + at] = from_float<T>(r0);
+            xs[kSlot + at + CT] = from_float<T>(r1);
+            xs[2 * kSlot + at] = from_float<T>(i0);
+            xs[2 * kSlot + at + CT] = from_float<T>(i1);
         }
+        float sum, sum_odd;
+        split(sums2, sum, sum_odd);
+        sum += sum_odd;
         if (p.partial) {
             if (WARPS > 1) {
                 sums[warp][lane] = sum;

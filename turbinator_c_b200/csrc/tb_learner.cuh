@@ -67,6 +67,41 @@ constexpr float kLog2e = 1.44269504f;
  * from the argument's product for |v| < 8, where it matters). */
 __device__ __forceinline__ float fast_sigmoid(float v) { return fast_rcp(1.0f + fast_exp2(-kLog2e * v)); }
 
+/* ---- two f32 values in one register pair, each operation on both ---- */
+
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(F2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 both(float v) { return pair(v, v); }
+/* fast_sigmoid of both. */
+__device__ __forceinline__ F2 sigmoid2(F2 v) {
+    float a, b;
+    split(mul2(v, both(-kLog2e)), a, b);
+    split(add2(pair(fast_exp2(a), fast_exp2(b)), both(1.0f)), a, b);
+    return pair(fast_rcp(a), fast_rcp(b));
+}
+
 /* ---- sums over the rows of partial [rows, columns] in f32 ---- */
 
 constexpr int kColumnThreads = 512;       /* 32 columns x 16 rows at a time */
