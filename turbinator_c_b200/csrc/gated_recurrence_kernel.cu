@@ -69,20 +69,39 @@ struct Spans {
     unsigned *ticket, *flag; /* flag [spans, tiles]: 1 (A, H) there, 2 the state after it too */
     float *map, *state;      /* [spans, tiles, 2, channels of a tile], [.., channels of a tile] */
     unsigned spans, tiles, items, tiles_per_sequence;
+    unsigned magic_tiles, magic_sequence; /* floor(2^32 / tiles), floor(2^32 / tiles_per_sequence) */
     unsigned *status;
 };
 
-__device__ __forceinline__ float softplus(float l) { return fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))); }
+/* log(1 + e^l) = max(l, 0) + log(1 + e) with e = e^-|l|, log(1 + e) =
+ * 2 artanh(e / (2 + e)), whose argument is at most 1/3: the series' next term
+ * is below 2e-8 of it.  The exponent keeps the part that its product rounds
+ * off, so that a far negative l has all its digits. */
+__device__ __forceinline__ float softplus(float l) {
+    const float n = -fabsf(l), t = n * kLog2e;
+    float e = fast_exp2(t);
+    e = fmaf(e, fmaf(n, kLog2e, -t) * 0.69314718f, e);
+    const float r = e * fast_rcp(2.0f + e), q = r * r;
+    float f = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+    f = fmaf(f, q, 1.0f / 9.0f);
+    f = fmaf(f, q, 1.0f / 7.0f);
+    f = fmaf(f, q, 1.0f / 5.0f);
+    f = fmaf(f, q, 1.0f / 3.0f);
+    f = fmaf(f, q, 1.0f);
+    return fmaxf(l, 0.0f) + 2.0f * r * f;
+}
 
-/* Steps of a sequence that count, from step t0 on, at most kSteps. */
-__device__ __forceinline__ int live_steps(const RecurrenceShape &d, const int32_t *lengths, size_t b, size_t t0) {
-    size_t live = d.steps;
-    if (lengths) {
-        const int32_t n = lengths[b];
-        live = n < 0 ? 0 : static_cast<size_t>(n) < d.steps ? static_cast<size_t>(n) : d.steps;
-    }
-    if (live <= t0) return 0;
-    return live - t0 < kSteps ? static_cast<int>(live - t0) : kSteps;
+/* Steps of sequence b that count. */
+__device__ __forceinline__ int live_of(const RecurrenceShape &d, const int32_t *lengths, size_t b) {
+    const int steps = static_cast<int>(d.steps);
+    if (!lengths) return steps;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n < steps ? n : steps;
+}
+/* Of `live` steps those of the span from step t on. */
+__device__ __forceinline__ int of_span(int live, int t) {
+    const int n = live - t;
+    return n < 0 ? 0 : n < kSteps ? n : kSteps;
 }
 
 /* e^l - 1 for -kNear <= l <= 0 from its series; the next term is below 2e-8
@@ -145,39 +164,47 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
-template <class T, int CT, int BYTES>
-__device__ __forceinline__ void load_pieces(T *to, const T *from, size_t stride, int rows, int columns, int lane) {
-    constexpr int kPer = CT * static_cast<int>(sizeof(T)) / BYTES; /* pieces of a row */
-    constexpr int kRows = 32 / kPer < 1 ? 1 : 32 / kPer;           /* rows at a time */
-    constexpr int kLanes = kPer < 32 ? kPer : 32;
-    const int row = lane / kLanes;
+/* N tensors of the same strides, at the same place: from[n] to
+ * to + n * kSteps * CT, BYTES at a time. */
+template <class T, int CT, int BYTES, int N, bool FULL>
+__device__ __forceinline__ void load_pieces(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows,
+                                            int columns, int lane) {
+    constexpr int kSize = static_cast<int>(sizeof(T));
+    constexpr int kPer = CT * kSize / BYTES; /* pieces of a row, at most 32 */
+    constexpr int kRows = 32 / kPer;         /* rows at a time */
+    const int row = lane / kPer, piece = lane % kPer;
+    const int left = columns * kSize - piece * BYTES;
+    if (!FULL && left <= 0) return;
+    const int bytes = FULL || left > BYTES ? BYTES : left;
+    const size_t first = (at + row * stride) * kSize + piece * BYTES, step = stride * kSize * kRows;
+    const uint32_t t = shared_address(to + row * CT) + piece * BYTES;
 #pragma unroll
-    for (int i = 0; i < kPer / kLanes; ++i) {
-        const int piece = lane % kLanes + i * kLanes;
-        const int left = columns * static_cast<int>(sizeof(T)) - piece * BYTES;
-        if (left <= 0) continue;
-        const char *f = reinterpret_cast<const char *>(from + row * stride) + piece * BYTES;
-        const uint32_t t = shared_address(to + row * CT) + piece * BYTES;
+    for (int n = 0; n < N; ++n) {
+        const char *f = reinterpret_cast<const char *>(from[n]) + first;
 #pragma unroll
-        for (int r = 0; r < kSteps; r += kRows)
-            if (row + r < rows)
-                copy_async<BYTES>(t + r * CT * static_cast<int>(sizeof(T)), f + r * stride * sizeof(T),
-                                  left < BYTES ? left : BYTES);
+        for (int r = 0; r < kSteps; r += kRows) {
+            if (FULL || row + r < rows) copy_async<BYTES>(t + (n * kSteps + r) * CT * kSize, f, bytes);
+            f += step;
+        }
     }
 }
 
-/* Starts copying rows x columns elements into to [kSteps][CT]; `piece` bytes at a time (16, 4: asynchronous). */
-template <class T, int CT>
-__device__ __forceinline__ void load_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
+/* Starts copying rows x columns elements of N tensors into [N][kSteps][CT];
+ * `piece` bytes at a time (16, 4: asynchronous). */
+template <class T, int CT, int N>
+__device__ __forceinline__ void load_rows(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows, int columns,
+                                          int piece, int lane) {
     if (piece == 16) {
-        load_pieces<T, CT, 16>(to, from, stride, rows, columns, lane);
+        if (rows == kSteps && columns == CT) load_pieces<T, CT, 16, N, true>(to, from, at, stride, rows, columns, lane);
+        else load_pieces<T, CT, 16, N, false>(to, from, at, stride, rows, columns, lane);
     } else if (piece == 4) {
-        load_pieces<T, CT, 4>(to, from, stride, rows, columns, lane);
+        load_pieces<T, CT, 4, N, false>(to, from, at, stride, rows, columns, lane);
     } else {
-        for (int c = lane; c < columns; c += 32)
+        for (int n = 0; n < N; ++n)
+            for (int c = lane; c < columns; c += 32)
 #pragma unroll
-            for (int r = 0; r < kSteps; ++r)
-                if (r < rows) to[r * CT + c] = from[r * stride + c];
+                for (int r = 0; r < kSteps; ++r)
+                    if (r < rows) to[(n * kSteps + r) * CT + c] = from[n][at + r * stride + c];
     }
 }
 
@@ -297,84 +324,108 @@ template <int CT, int V, int WARPS>
 __device__ __forceinline__ Lane<V> join(const Spans &s, unsigned item, unsigned span, unsigned tile, const Lane<V> &map_a,
                                         const Lane<V> &map_h, const Lane<V> &initial, float (*sa)[CT], float (*sh)[CT],
                                         float *carry, int order, int warp, int lane, Lane<V> *after) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        sa[order][lane * V + v] = map_a.v[v];
+        sh[order][lane * V + v] = map_h.v[v];
+    }
+    Lane<V> h = initial; /* where the span before is done already, its state is read beside the inputs */
+    bool known = span == 0;
+    if (warp == 0 && span > 0) {
+        const size_t prev = static_cast<size_t>(span - 1) * s.tiles + tile;
+        if (load_acquire(s.flag + prev) == 2) {
+            known = true;
+#pragma unroll
+            for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + prev * CT + lane * V + v);
+        }
+        known = __all_sync(0xffffffffu, known);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        Lane<V> a, b;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            a.v[v] = 1.0f;
+            b.v[v] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float aw = sa[w][lane * V + v];
+                b.v[v] = fmaf(aw, b.v[v], sh[w][lane * V + v]);
+                a.v[v] *= aw;
+            }
+        }
+        if (!known) {
+            if (span + 1 != s.spans) publish<CT, V>(s, item, 1, a, b, lane);
+            h = state_before<CT, V>(s, span, tile, lane);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            carry[lane * V + v] = h.v[v];
+            after->v[v] = fmaf(a.v[v], h.v[v], b.v[v]);
+        }
+    }
+    __syncthreads();
+    if (warp == 0 && span + 1 != s.spans) publish<CT, V>(s, item, 2, *after, *after, lane);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        h.v[v] = carry[lane * V + v];
+        for (int w = 0; w < order; ++w) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
+    }
+    return h;
+}
+
+/* The same where one CTA takes a tile's spans in turn (STRIP): every warp folds
+ * all four spans, which leaves the state after them with each.  buffer: of two,
+ * in turn, so that one barrier does. */
+template <int CT, int V, int WARPS>
+__device__ __forceinline__ Lane<V> join_strip(const Lane<V> &map_a, const Lane<V> &map_h, Lane<V> *state, float (*sa)[CT],
+                                              float (*sh)[CT], int order, int lane) {
+    Lane<V> h = *state;
     if constexpr (WARPS == 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) after->v[v] = fmaf(map_a.v[v], initial.v[v], map_h.v[v]);
-        return initial;
+        for (int v = 0; v < V; ++v) state->v[v] = fmaf(map_a.v[v], h.v[v], map_h.v[v]);
+        return h;
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             sa[order][lane * V + v] = map_a.v[v];
             sh[order][lane * V + v] = map_h.v[v];
         }
-        Lane<V> h = initial; /* where the span before is done already, its state is read beside the inputs */
-        bool known = span == 0;
-        if (warp == 0 && span > 0) {
-            const size_t prev = static_cast<size_t>(span - 1) * s.tiles + tile;
-            if (load_acquire(s.flag + prev) == 2) {
-                known = true;
-#pragma unroll
-                for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + prev * CT + lane * V + v);
-            }
-            known = __all_sync(0xffffffffu, known);
-        }
         __syncthreads();
-        if (warp == 0) {
-            Lane<V> a, b;
+        Lane<V> mine = h;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                a.v[v] = 1.0f;
-                b.v[v] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float aw = sa[w][lane * V + v];
-                    b.v[v] = fmaf(aw, b.v[v], sh[w][lane * V + v]);
-                    a.v[v] *= aw;
-                }
+                if (w == order) mine.v[v] = h.v[v];
+                h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
             }
-            if (!known) {
-                if (span + 1 != s.spans) publish<CT, V>(s, item, 1, a, b, lane);
-                h = state_before<CT, V>(s, span, tile, lane);
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                carry[lane * V + v] = h.v[v];
-                after->v[v] = fmaf(a.v[v], h.v[v], b.v[v]);
-            }
-        }
-        __syncthreads();
-        if (warp == 0 && span + 1 != s.spans) publish<CT, V>(s, item, 2, *after, *after, lane);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h.v[v] = carry[lane * V + v];
-            for (int w = 0; w < order; ++w) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
-        }
-        return h;
+        *state = h;
+        return mine;
     }
 }
 
-/* The items of a CTA: by the counter where spans wait for one another, else every gridDim.x-th. */
-struct Items {
-    bool counted;
-    unsigned now, next;
+/* Where a CTA works: spans of a tile.  STRIP: all spans of every gridDim.x-th
+ * tile, in turn.  Else single items, by the counter. */
+struct Place {
+    unsigned span, tile;
+    unsigned b;
+    int c0, live; /* first channel, steps of the sequence that count */
 };
 
-template <int WARPS> __device__ __forceinline__ Items first_items(const Spans &s, unsigned *mailbox) {
-    Items i;
-    i.counted = s.spans > 1;
-    if (!i.counted) {
-        i.now = blockIdx.x;
-        i.next = blockIdx.x + gridDim.x;
-    } else {
-        if (threadIdx.x == 0) {
-            mailbox[0] = atomicAdd(s.ticket, 1u);
-            mailbox[1] = atomicAdd(s.ticket, 1u);
-        }
-        __syncthreads();
-        i.now = mailbox[0];
-        i.next = mailbox[1];
-    }
-    return i;
+__device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
+    unsigned q = __umulhi(v, magic); /* floor(2^32 / by): at most 2 below */
+    unsigned r = v - q * by;
+    if (r >= by) ++q, r -= by;
+    if (r >= by) ++q;
+    return q;
+}
+
+template <int CT>
+__device__ __forceinline__ void settle(Place &at, const RecurrenceShape &d, const int32_t *lengths, const Spans &s) {
+    at.b = divided(at.tile, s.tiles_per_sequence, s.magic_sequence);
+    at.c0 = static_cast<int>(at.tile - at.b * s.tiles_per_sequence) * CT;
+    at.live = live_of(d, lengths, at.b);
 }
 
 /* ---- forward ---- */
@@ -436,78 +487,113 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
     }
 }
 
-template <class T, int WARPS>
+/* The next place of the CTA (STRIP). */
+template <int CT>
+__device__ __forceinline__ Place strip_next(const Place &at, const RecurrenceShape &d, const int32_t *lengths, const Spans &s) {
+    Place next = at;
+    if (++next.span == s.spans) {
+        next.span = 0;
+        next.tile += gridDim.x;
+        if (next.tile < s.tiles) settle<CT>(next, d, lengths, s);
+    }
+    return next;
+}
+
+template <class T, int WARPS, bool STRIP>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(const ForwardArgs p, const Spans s) {
     constexpr int V = kForwardV<T>, CT = 32 * V;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float sa[WARPS][CT], sh[WARPS][CT], carry[CT];
+    __shared__ float sa[STRIP ? 2 : 1][WARPS][CT], sh[STRIP ? 2 : 1][WARPS][CT], carry[CT];
     __shared__ unsigned mailbox[2];
     const RecurrenceShape &d = p.d;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, steps = static_cast<int>(d.steps);
     T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 3 * kSteps * CT; /* two stages of x, rec, inp */
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
 
-    const auto start = [&](unsigned item, int stage) {
-        if (item < s.items) {
-            const unsigned span = item / s.tiles, tile = item % s.tiles;
-            const size_t b = tile / s.tiles_per_sequence, c = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
-            const size_t t = (static_cast<size_t>(span) * WARPS + warp) * kSteps;
-            const int live = live_steps(d, p.lengths, b, t);
-            const int columns = d.channels - c < CT ? static_cast<int>(d.channels - c) : CT;
-            const size_t at = b * d.is + t * d.it + c;
-            T *to = slots + stage * 3 * kSteps * CT;
-            load_rows<T, CT>(to, static_cast<const T *>(p.x) + at, d.it, live, columns, p.in_piece, lane);
-            load_rows<T, CT>(to + kSteps * CT, static_cast<const T *>(p.rec) + at, d.it, live, columns, p.in_piece, lane);
-            load_rows<T, CT>(to + 2 * kSteps * CT, static_cast<const T *>(p.inp) + at, d.it, live, columns, p.in_piece, lane);
-        }
-        copies_end();
+    const auto start = [&](const Place &to, int stage) {
+        const int t = static_cast<int>(to.span * WARPS + warp) * kSteps, left = static_cast<int>(d.channels) - to.c0;
+        const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
+        load_rows<T, CT, 3>(slots + stage * 3 * kSteps * CT, from, to.b * d.is + t * d.it + to.c0, d.it,
+                            of_span(to.live, t), left < CT ? left : CT, p.in_piece, lane);
     };
 
-    Items items = first_items<WARPS>(s, mailbox);
+    Place at{}, next{};
+    unsigned item = 0, next_item = 0; /* !STRIP */
+    const auto place = [&](Place &to, unsigned i) {
+        to.span = divided(i, s.tiles, s.magic_tiles);
+        to.tile = i - to.span * s.tiles;
+        settle<CT>(to, d, p.lengths, s);
+    };
+    const auto in_range = [&](const Place &to, unsigned i) { return STRIP ? to.tile < s.tiles : i < s.items; };
+    if (STRIP) {
+        at.tile = blockIdx.x;
+        if (at.tile < s.tiles) settle<CT>(at, d, p.lengths, s);
+    } else {
+        if (threadIdx.x == 0) {
+            mailbox[0] = atomicAdd(s.ticket, 1u);
+            mailbox[1] = atomicAdd(s.ticket, 1u);
+        }
+        __syncthreads();
+        item = mailbox[0];
+        next_item = mailbox[1];
+        if (item < s.items) place(at, item);
+    }
     int stage = 0;
-    start(items.now, stage);
-    while (items.now < s.items) {
-        const unsigned item = items.now, span = item / s.tiles, tile = item % s.tiles;
-        const size_t b = tile / s.tiles_per_sequence, c0 = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
-        const size_t t = (static_cast<size_t>(span) * WARPS + warp) * kSteps;
-        const int live = live_steps(d, p.lengths, b, t);
-        const int rows = t >= d.steps ? 0 : d.steps - t < kSteps ? static_cast<int>(d.steps - t) : kSteps;
-        const int columns = d.channels - c0 < CT ? static_cast<int>(d.channels - c0) : CT;
+    if (in_range(at, item)) start(at, 0);
+    copies_end();
+    float rate[V];
+    Lane<V> state;
+    bool near = false, fresh = true;
+    while (in_range(at, item)) {
+        const int t = static_cast<int>(at.span * WARPS + warp) * kSteps;
+        const int live = of_span(at.live, t), rows = of_span(steps, t);
+        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
         T *const xs = slots + stage * 3 * kSteps * CT;
-        start(items.next, stage ^ 1);
+        if (STRIP) next = strip_next<CT>(at, d, p.lengths, s);
+        else if (next_item < s.items) place(next, next_item);
+        if (in_range(next, next_item)) start(next, stage ^ 1);
+        copies_end();
         unsigned then = 0;
-        if (items.counted && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
-        const unsigned anew = reset_bits(p.reset, b * d.steps + t, live, lane);
-        float rate[V];
-        Lane<V> initial;
+        if (!STRIP && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
+        const unsigned anew = reset_bits(p.reset, at.b * d.steps + t, live, lane);
+        if (!STRIP || fresh) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const size_t c = c0 + lane * V + v;
-            rate[v] = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
-            initial.v[v] = span == 0 && p.state_in && c < d.channels ? p.state_in[b * d.channels + c] : 0.0f;
+            for (int v = 0; v < V; ++v) {
+                const size_t c = at.c0 + lane * V + v;
+                const bool in = c < d.channels;
+                rate[v] = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
+                state.v[v] = at.span == 0 && p.state_in && in ? p.state_in[at.b * d.channels + c] : 0.0f;
+            }
+            near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
         }
         copies_wait<1>();
         __syncwarp();
         float prod[kSteps][V], local[kSteps][V];
-        if (live == kSteps && !anew && __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear))
+        if (live == kSteps && !anew && near)
             forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
         else
             forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
-        Lane<V> map_a, map_h, after;
+        Lane<V> map_a, map_h, h0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             map_a.v[v] = prod[kSteps - 1][v];
             map_h.v[v] = local[kSteps - 1][v];
         }
-        const Lane<V> h0 = join<CT, V, WARPS>(s, item, span, tile, map_a, map_h, initial, sa, sh, carry, warp, warp, lane,
-                                              &after);
-        if (items.counted && threadIdx.x == 0) mailbox[0] = then;
+        if constexpr (STRIP) {
+            h0 = join_strip<CT, V, WARPS>(map_a, map_h, &state, sa[stage], sh[stage], warp, lane);
+        } else {
+            const Lane<V> initial = state;
+            h0 = join<CT, V, WARPS>(s, item, at.span, at.tile, map_a, map_h, initial, sa[0], sh[0], carry, warp, warp, lane,
+                                    &state);
+            if (threadIdx.x == 0) mailbox[0] = then;
+        }
+        const bool last = at.span + 1 == s.spans;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const size_t c = c0 + lane * V + v;
+            const size_t c = at.c0 + lane * V + v;
             if (c >= d.channels) continue;
-            if (p.checkpoints && rows > 0) p.checkpoints[(b * saved + t / kSteps) * d.channels + c] = h0.v[v];
-            if (p.state_out && warp == 0 && span + 1 == s.spans) p.state_out[b * d.channels + c] = after.v[v];
+            if (p.checkpoints && rows > 0) p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] = h0.v[v];
+            if (last && p.state_out && warp == 0) p.state_out[at.b * d.channels + c] = state.v[v];
         }
 #pragma unroll
         for (int j = 0; j < kSteps; j += 3 - V) {
@@ -515,20 +601,27 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
             split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(h0.v[0], h0.v[V - 1]),
                        pair(local[j][0], local[j + 2 - V][V - 1])), o0, o1);
             if constexpr (V == 2) {
-                Pack<T, 2> o = {{from_float<T>(o0), from_float<T>(o1)}};
-                if (j >= live) o = {{from_float<T>(0.0f), from_float<T>(0.0f)}};
-                *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = o;
+                *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = {{from_float<T>(o0), from_float<T>(o1)}};
             } else {
-                xs[j * CT + lane] = from_float<T>(j < live ? o0 : 0.0f);
-                xs[(j + 1) * CT + lane] = from_float<T>(j + 1 < live ? o1 : 0.0f);
+                xs[j * CT + lane] = from_float<T>(o0);
+                xs[(j + 1) * CT + lane] = from_float<T>(o1);
             }
         }
+        if (live < kSteps) { /* steps past the sequence's length */
+            for (int j = live; j < kSteps; ++j)
+                for (int v = 0; v < V; ++v) xs[j * CT + lane * V + v] = from_float<T>(0.0f);
+        }
         __syncwarp();
-        store_rows<T, CT>(static_cast<T *>(p.h) + b * d.os + t * d.ot + c0, xs, d.ot, rows, columns, p.out_piece, lane);
-        if (WARPS > 1) __syncthreads(); /* mailbox, and sa, sh, carry are free again */
-        else __syncwarp();
-        items.now = items.next;
-        items.next = items.counted ? mailbox[0] : items.next + gridDim.x;
+        store_rows<T, CT>(static_cast<T *>(p.h) + at.b * d.os + t * d.ot + at.c0, xs, d.ot, rows, columns, p.out_piece, lane);
+        if (STRIP) {
+            __syncwarp();
+            fresh = last;
+        } else {
+            __syncthreads(); /* mailbox, and sa, sh, carry are free again */
+            item = next_item;
+            next_item = mailbox[0];
+        }
+        at = next;
         stage ^= 1;
     }
 }
@@ -578,64 +671,84 @@ __device__ __forceinline__ void backward_gates(const T *xs, const T *rs, const T
     }
 }
 
-template <class T, int WARPS>
+template <class T, int WARPS, bool STRIP>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(const BackwardArgs p, const Spans s) {
     constexpr int CT = 32;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float sa[WARPS][CT], sh[WARPS][CT], carry[CT], sums[WARPS][CT];
+    __shared__ float sa[STRIP ? 2 : 1][WARPS][CT], sh[STRIP ? 2 : 1][WARPS][CT], carry[CT], sums[WARPS][CT];
     __shared__ unsigned mailbox[2];
     const RecurrenceShape &d = p.d;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, steps = static_cast<int>(d.steps);
     constexpr int kSlot = kSteps * CT;
     T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
 
     /* spans in the order of the scan: the last steps first */
-    const auto step_of = [&](unsigned span) {
-        return (static_cast<size_t>(s.spans - 1 - span) * WARPS + warp) * kSteps;
-    };
-    const auto start = [&](unsigned item, int stage) {
-        if (item < s.items) {
-            const unsigned tile = item % s.tiles;
-            const size_t b = tile / s.tiles_per_sequence, c = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
-            const size_t t = step_of(item / s.tiles);
-            const int live = live_steps(d, p.lengths, b, t);
-            const int columns = d.channels - c < CT ? static_cast<int>(d.channels - c) : CT;
-            const size_t at = b * d.is + t * d.it + c;
-            T *to = slots + stage * 4 * kSlot;
-            load_rows<T, CT>(to, static_cast<const T *>(p.x) + at, d.it, live, columns, p.in_piece, lane);
-            load_rows<T, CT>(to + kSlot, static_cast<const T *>(p.rec) + at, d.it, live, columns, p.in_piece, lane);
-            load_rows<T, CT>(to + 2 * kSlot, static_cast<const T *>(p.inp) + at, d.it, live, columns, p.in_piece, lane);
-            load_rows<T, CT>(to + 3 * kSlot, static_cast<const T *>(p.dh) + b * d.os + t * d.ot + c, d.ot, live, columns,
-                             p.dh_piece, lane);
-        }
-        copies_end();
+    const auto step_of = [&](unsigned span) { return static_cast<int>((s.spans - 1 - span) * WARPS + warp) * kSteps; };
+    const auto start = [&](const Place &to, int stage) {
+        const int t = step_of(to.span), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
+        const int live = of_span(to.live, t);
+        const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
+        const T *const dh[1] = {static_cast<const T *>(p.dh)};
+        load_rows<T, CT, 3>(slots + stage * 4 * kSlot, from, to.b * d.is + t * d.it + to.c0, d.it, live, columns,
+                            p.in_piece, lane);
+        load_rows<T, CT, 1>(slots + stage * 4 * kSlot + 3 * kSlot, dh, to.b * d.os + t * d.ot + to.c0, d.ot, live, columns,
+                            p.dh_piece, lane);
     };
 
-    Items items = first_items<WARPS>(s, mailbox);
+    Place at{}, next{};
+    unsigned item = 0, next_item = 0; /* !STRIP */
+    const auto place = [&](Place &to, unsigned i) {
+        to.span = divided(i, s.tiles, s.magic_tiles);
+        to.tile = i - to.span * s.tiles;
+        settle<CT>(to, d, p.lengths, s);
+    };
+    const auto in_range = [&](const Place &to, unsigned i) { return STRIP ? to.tile < s.tiles : i < s.items; };
+    if (STRIP) {
+        at.tile = blockIdx.x;
+        if (at.tile < s.tiles) settle<CT>(at, d, p.lengths, s);
+    } else {
+        if (threadIdx.x == 0) {
+            mailbox[0] = atomicAdd(s.ticket, 1u);
+            mailbox[1] = atomicAdd(s.ticket, 1u);
+        }
+        __syncthreads();
+        item = mailbox[0];
+        next_item = mailbox[1];
+        if (item < s.items) place(at, item);
+    }
     int stage = 0;
-    start(items.now, stage);
-    while (items.now < s.items) {
-        const unsigned item = items.now, span = item / s.tiles, tile = item % s.tiles;
-        const size_t b = tile / s.tiles_per_sequence, c0 = static_cast<size_t>(tile % s.tiles_per_sequence) * CT;
-        const size_t c = c0 + lane, t = step_of(span);
-        const int live = live_steps(d, p.lengths, b, t);
-        const int rows = t >= d.steps ? 0 : d.steps - t < kSteps ? static_cast<int>(d.steps - t) : kSteps;
-        const int columns = d.channels - c0 < CT ? static_cast<int>(d.channels - c0) : CT;
+    if (in_range(at, item)) start(at, 0);
+    copies_end();
+    float rate = 0.0f, sum_all = 0.0f;
+    Lane<1> state;
+    bool near = false, fresh = true;
+    while (in_range(at, item)) {
+        const int t = step_of(at.span);
+        const int live = of_span(at.live, t), rows = of_span(steps, t);
+        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+        const size_t c = at.c0 + lane;
         const bool in = c < d.channels;
         T *const xs = slots + stage * 4 * kSlot;
-        start(items.next, stage ^ 1);
+        if (STRIP) next = strip_next<CT>(at, d, p.lengths, s);
+        else if (next_item < s.items) place(next, next_item);
+        if (in_range(next, next_item)) start(next, stage ^ 1);
+        copies_end();
         unsigned then = 0;
-        if (items.counted && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
-        const unsigned anew = reset_bits(p.reset, b * d.steps + t, live, lane);
-        const float rate = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
-        const float h = in && rows > 0 ? p.checkpoints[(b * saved + t / kSteps) * d.channels + c] : 0.0f;
-        Lane<1> initial, map_a, map_h, after;
-        initial.v[0] = span == 0 && p.dstate_out && in ? p.dstate_out[b * d.channels + c] : 0.0f;
+        if (!STRIP && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
+        const unsigned anew = reset_bits(p.reset, at.b * d.steps + t, live, lane);
+        if (!STRIP || fresh) {
+            rate = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
+            state.v[0] = at.span == 0 && p.dstate_out && in ? p.dstate_out[at.b * d.channels + c] : 0.0f;
+            near = __all_sync(0xffffffffu, rate >= -kNear);
+            sum_all = 0.0f;
+        }
+        const float h = in && rows > 0 ? p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] : 0.0f;
+        Lane<1> map_a, map_h;
         copies_wait<1>();
         __syncwarp();
         float a[kSteps], w[kSteps], z[kSteps], q[kSteps], m[kSteps];
-        if (live == kSteps && !anew && __all_sync(0xffffffffu, rate >= -kNear))
+        if (live == kSteps && !anew && near)
             backward_gates<T, true>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
         else
             backward_gates<T, false>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
@@ -647,10 +760,17 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
             map_h.v[0] = a[j] * (g + map_h.v[0]);
             map_a.v[0] *= a[j];
         }
-        float grad = join<CT, 1, WARPS>(s, item, span, tile, map_a, map_h, initial, sa, sh, carry, WARPS - 1 - warp, warp,
-                                        lane, &after).v[0];
-        if (items.counted && threadIdx.x == 0) mailbox[0] = then;
-        if (p.dstate_in && in && warp == 0 && span + 1 == s.spans) p.dstate_in[b * d.channels + c] = after.v[0];
+        float grad;
+        const bool last = at.span + 1 == s.spans;
+        if constexpr (STRIP) {
+            grad = join_strip<CT, 1, WARPS>(map_a, map_h, &state, sa[stage], sh[stage], WARPS - 1 - warp, lane).v[0];
+        } else {
+            const Lane<1> initial = state;
+            grad = join<CT, 1, WARPS>(s, item, at.span, at.tile, map_a, map_h, initial, sa[0], sh[0], carry,
+                                      WARPS - 1 - warp, warp, lane, &state).v[0];
+            if (threadIdx.x == 0) mailbox[0] = then;
+        }
+        if (last && p.dstate_in && in && warp == 0) p.dstate_in[at.b * d.channels + c] = state.v[0];
         F2 sums2 = both(0.0f);
 #pragma unroll
         for (int j = kSteps - 2; j >= 0; j -= 2) {
@@ -679,27 +799,34 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
         float sum, sum_odd;
         split(sums2, sum, sum_odd);
         sum += sum_odd;
-        if (p.partial) {
-            if (WARPS > 1) {
-                sums[warp][lane] = sum;
-                __syncthreads();
-                if (warp == 0) {
-                    sum = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < WARPS; ++w) sum += sums[w][lane];
-                }
-            }
-            if (warp == 0 && in) p.partial[(static_cast<size_t>(span) * d.sequences + b) * d.channels + c] = sum;
-        }
         __syncwarp();
-        const size_t to = b * d.gs + t * d.gt + c0;
+        const size_t to = at.b * d.gs + t * d.gt + at.c0;
         store_rows<T, CT>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
         store_rows<T, CT>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
         store_rows<T, CT>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
-        if (WARPS > 1) __syncthreads(); /* mailbox, and sa, sh, carry, sums are free again */
-        else __syncwarp();
-        items.now = items.next;
-        items.next = items.counted ? mailbox[0] : items.next + gridDim.x;
+        sum_all = STRIP ? sum_all + sum : sum;
+        if (p.partial && (!STRIP || last)) {
+            if (WARPS > 1) {
+                sums[warp][lane] = sum_all;
+                __syncthreads();
+                if (warp == 0) {
+                    sum_all = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < WARPS; ++i) sum_all += sums[i][lane];
+                }
+            }
+            const size_t row = STRIP ? at.b : static_cast<size_t>(at.span) * d.sequences + at.b;
+            if (warp == 0 && in) p.partial[row * d.channels + c] = sum_all;
+        }
+        if (STRIP) {
+            __syncwarp();
+            fresh = last;
+        } else {
+            __syncthreads(); /* mailbox, and sa, sh, carry, sums are free again */
+            item = next_item;
+            next_item = mailbox[0];
+        }
+        at = next;
         stage ^= 1;
     }
 }
@@ -737,6 +864,11 @@ bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     return s->it >= d->channels && s->ot >= d->channels && s->gt >= d->channels;
 }
 
+/* A tile's spans are taken in turn by one CTA where there are at least kStrip
+ * tiles, else by different CTAs. */
+constexpr unsigned kStrip = 296;
+bool strips(const Spans &s) { return s.spans == 1 || s.tiles >= kStrip; }
+
 struct Layout {
     Spans spans;
     size_t flags_bytes, bytes;
@@ -750,7 +882,9 @@ Layout spans_of(const RecurrenceShape &d, int warps, int tile, void *workspace) 
     s.tiles_per_sequence = static_cast<unsigned>((d.channels + tile - 1) / tile);
     s.tiles = static_cast<unsigned>(d.sequences * s.tiles_per_sequence);
     s.items = s.spans * s.tiles;
-    if (s.spans > 1) {
+    s.magic_tiles = static_cast<unsigned>(0xffffffffull / s.tiles);
+    s.magic_sequence = static_cast<unsigned>(0xffffffffull / s.tiles_per_sequence);
+    if (!strips(s)) {
         char *at = static_cast<char *>(workspace);
         l.flags_bytes = align_up(16 + static_cast<size_t>(s.items) * 4, 16);
         const size_t row = static_cast<size_t>(s.items) * tile * sizeof(float);
@@ -767,9 +901,9 @@ int warps_for(const RecurrenceShape &d) { return d.steps <= kSteps ? 1 : kWarps;
 int forward_tile(int type) { return type == TB_TYPE_F32 ? 32 : 64; }
 
 /* Rows of partial sums for ddecay, and behind them the parts that they are first summed into. */
-size_t partial_rows(const RecurrenceShape &d, unsigned spans) { return d.sequences * spans; }
-size_t partial_bytes(const RecurrenceShape &d, unsigned spans) {
-    const size_t rows = partial_rows(d, spans);
+size_t partial_rows(const RecurrenceShape &d, const Spans &s) { return strips(s) ? d.sequences : d.sequences * s.spans; }
+size_t partial_bytes(const RecurrenceShape &d, const Spans &s) {
+    const size_t rows = partial_rows(d, s);
     return (rows + column_parts(rows)) * d.channels * sizeof(float);
 }
 
@@ -781,7 +915,9 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
 
 /* Launches a kernel of persistent CTAs over l's items. */
 template <class Kernel, class Args>
-int launch_items(Kernel kernel, const Args &args, Layout &l, int warps, size_t shared, cudaStream_t st) {
+int launch_items(Kernel strip, Kernel single, const Args &args, Layout &l, int warps, size_t shared, cudaStream_t st) {
+    const bool in_turn = strips(l.spans);
+    const Kernel kernel = in_turn ? strip : single;
     int dev = 0, sms = 0, per_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
@@ -789,12 +925,12 @@ int launch_items(Kernel kernel, const Args &args, Layout &l, int warps, size_t s
             cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, shared) != cudaSuccess)
         return 0;
-    if (l.spans.spans > 1) {
+    if (!in_turn) {
         l.spans.status = tb_status_slot(st);
         if (!l.spans.status || cudaMemsetAsync(l.spans.ticket, 0, l.flags_bytes, st) != cudaSuccess) return 0;
     }
-    const unsigned most = static_cast<unsigned>(sms * per_sm);
-    kernel<<<l.spans.items < most ? l.spans.items : most, warps * 32, shared, st>>>(args, l.spans);
+    const unsigned most = static_cast<unsigned>(sms * per_sm), work = in_turn ? l.spans.tiles : l.spans.items;
+    kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args, l.spans);
     return launched();
 }
 
@@ -805,7 +941,7 @@ extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_d
     if (!recurrence_shape(desc, &s)) return 0;
     const int warps = warps_for(s);
     const Layout f = spans_of(s, warps, forward_tile(desc->type), nullptr), b = spans_of(s, warps, 32, nullptr);
-    const size_t back = align_up(b.bytes, 16) + partial_bytes(s, b.spans.spans);
+    const size_t back = align_up(b.bytes, 16) + partial_bytes(s, b.spans);
     return f.bytes > back ? f.bytes : back;
 }
 
@@ -833,8 +969,9 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return warps == 1 ? launch_items(recurrence_forward<T, 1>, p, l, 1, shared, st)
-                          : launch_items(recurrence_forward<T, kWarps>, p, l, kWarps, shared, st);
+        return warps == 1 ? launch_items(recurrence_forward<T, 1, true>, recurrence_forward<T, 1, true>, p, l, 1, shared, st)
+                          : launch_items(recurrence_forward<T, kWarps, true>, recurrence_forward<T, kWarps, false>, p, l,
+                                         kWarps, shared, st);
     });
 }
 
@@ -875,11 +1012,12 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return warps == 1 ? launch_items(recurrence_backward<T, 1>, p, l, 1, shared, st)
-                          : launch_items(recurrence_backward<T, kWarps>, p, l, kWarps, shared, st);
+        return warps == 1 ? launch_items(recurrence_backward<T, 1, true>, recurrence_backward<T, 1, true>, p, l, 1, shared, st)
+                          : launch_items(recurrence_backward<T, kWarps, true>, recurrence_backward<T, kWarps, false>, p, l,
+                                         kWarps, shared, st);
     });
     if (!ok || !ddecay) return ok;
-    const size_t rows = partial_rows(s, l.spans.spans), parts = column_parts(rows);
+    const size_t rows = partial_rows(s, l.spans), parts = column_parts(rows);
     float *sums = partial + rows * s.channels;
     column_sums<<<dim3(static_cast<unsigned>((s.channels + 31) / 32), static_cast<unsigned>(parts)), kColumnThreads, 0,
                   st>>>(partial, rows, s.channels, sums);
