@@ -4,28 +4,23 @@
  *
  * h_t = a_t h_(t-1) + b_t is a chain over t for each channel, but steps compose:
  * a span of steps maps the state before it, h, to A h + H, so spans can be
- * taken apart and joined.  A warp takes 16 steps of 32 or 64 channels, a CTA
- * of four warps 64 steps; the spans of a sequence are joined across CTAs while
- * they all run, so every input is read once whatever the split:
+ * taken apart and joined.  A warp takes spans of 16 steps of 32 or 64 channels
+ * (a tile); the warps of a CTA take consecutive spans of one tile, join them in
+ * shared memory and go on together, the state in registers.  Inputs are staged
+ * by asynchronous copies one round ahead; outputs leave through the same slots.
  *
- *   - Work items (span, sequence, channels) are handed out by a counter in the
- *     order of the spans.  A CTA takes the next item only once it runs, and an
- *     item waits only for earlier items, so the earliest unfinished one can
- *     always go on.
- *   - Each item publishes its (A, H), and then the state after it.  The state
- *     before an item is the nearest published state folded forward through the
- *     (A, H) of the spans between, one fma each: the same operations in the
- *     same order from wherever the fold starts, so the bits do not depend on
- *     timing.
- *   - The wait for earlier spans is bounded by ~1 s of the GPU's clock, after
- *     which the status word of the stream gets the timeout bit
- *     (tb_cuda_synchronize reports it) and the kernel goes on to its end.
+ * Where tiles alone cannot fill the GPU, the steps are cut into strips and a
+ * first kernel finds each strip's map, from which every strip's first state
+ * follows: the inputs of the maps are read twice (three of the forward pass's
+ * four tensors, two of the backward pass's seven), but nothing waits.  (The
+ * strips joined in one kernel through published maps, each waiting for those
+ * before it, was measured at 372 to 685 us on three logs of 30,011 steps: a
+ * CTA that waits publishes its next map late, and so all wait.)
  *
  * The backward pass is the same scan in the other direction over
  * c_t = a_t (dh_t + c_(t+1)), the gradient of the state before step t; the
  * states that it needs are recomputed within 16 steps from the saved ones.
  */
-#include "tb_features_internal.h"
 #include "tb_learner.cuh"
 
 using namespace tb_learn;
@@ -33,8 +28,7 @@ using namespace tb_learn;
 namespace {
 
 constexpr int kSteps = TB_RECURRENCE_CHECKPOINT; /* steps of a warp's span */
-constexpr int kWarps = 4;                        /* warps, and spans, of a CTA for sequences of more steps */
-constexpr unsigned long long kWaitNs = 1000000000ull;
+constexpr int kWarps = 4;                        /* warps of a CTA at most */
 
 struct RecurrenceShape {
     size_t sequences, steps, channels;
@@ -64,13 +58,12 @@ struct BackwardArgs {
     int in_piece, dh_piece, out_piece;
 };
 
-/* The scan over spans: workspace and shape. */
-struct Spans {
-    unsigned *ticket, *flag; /* flag [spans, tiles]: 1 (A, H) there, 2 the state after it too */
-    float *map, *state;      /* [spans, tiles, 2, channels of a tile], [.., channels of a tile] */
-    unsigned spans, tiles, items, tiles_per_sequence;
-    unsigned magic_tiles, magic_sequence; /* floor(2^32 / tiles), floor(2^32 / tiles_per_sequence) */
-    unsigned *status;
+/* Who takes what: tiles of channels times strips of rounds (a span for each
+ * of the CTA's warps), one unit of work each; unit = strip * tiles + tile. */
+struct Split {
+    unsigned tiles, tiles_per_sequence, rounds, strips, strip_rounds;
+    unsigned magic_tiles, magic_sequence; /* floor((2^32 - 1) / tiles), .. / tiles_per_sequence) */
+    float *maps;                          /* [tiles, strips, 2, channels of a tile] where strips > 1 */
 };
 
 /* log(1 + e^l) = max(l, 0) + log(1 + e) with e = e^-|l|, log(1 + e) =
@@ -235,197 +228,148 @@ __device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, 
     }
 }
 
-/* Bit j: step t0 + j starts anew. */
-__device__ __forceinline__ unsigned reset_bits(const uint8_t *reset, size_t at, int live, int lane) {
-    return reset ? __ballot_sync(0xffffffffu, lane < live && reset[at + lane]) : 0u;
+/* Whether step t0 + lane starts anew. */
+__device__ __forceinline__ unsigned reset_byte(const uint8_t *reset, size_t at, int live, int lane) {
+    return reset && lane < live ? reset[at + lane] : 0u;
 }
 
 /* ---- the scan over spans ---- */
-
-__device__ __forceinline__ unsigned load_acquire(const unsigned *p) {
-    unsigned v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void store_release(unsigned *p, unsigned v) {
-    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-__device__ __forceinline__ unsigned long long clock_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 
 template <int V> struct Lane {
     float v[V];
 };
 
+/* Joins the spans of a CTA's round: each warp brings its span's map of V
+ * channels a lane (`order`: its place in the scan) and the state before the
+ * round; it leaves with the state before its own span, *state with that after
+ * the round.  Every warp folds all spans, so one barrier a round does, given
+ * buffers sa, sh that alternate. */
 template <int CT, int V>
-__device__ __forceinline__ void publish(const Spans &s, size_t item, unsigned what, const Lane<V> &a, const Lane<V> &b,
-                                        int lane) {
+__device__ __forceinline__ Lane<V> join(const Lane<V> &map_a, const Lane<V> &map_h, Lane<V> *state, float (*sa)[CT],
+                                        float (*sh)[CT], int order, int warps, int lane) {
+    Lane<V> h = *state, mine = h;
+    if (warps == 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (what == 2) {
-            __stcg(s.state + item * CT + lane * V + v, a.v[v]);
-        } else {
-            __stcg(s.map + item * 2 * CT + lane * V + v, a.v[v]);
-            __stcg(s.map + item * 2 * CT + CT + lane * V + v, b.v[v]);
-        }
+        for (int v = 0; v < V; ++v) state->v[v] = fmaf(map_a.v[v], h.v[v], map_h.v[v]);
+        return mine;
     }
-    __syncwarp();
-    if (lane == 0) store_release(s.flag + item, what); /* after the warp's stores */
-}
-
-/* The state before span `span` > 0 of a tile; one warp. */
-template <int CT, int V>
-__device__ Lane<V> state_before(const Spans &s, unsigned span, unsigned tile, int lane) {
-    Lane<V> h;
-    int back = static_cast<int>(span) - 1; /* the last span of the window */
-    unsigned long long since = 0;
-    for (;;) { /* the nearest span whose state is there, every (A, H) from it on being there */
-        const int at = back - lane;
-        const unsigned f = at >= 0 ? load_acquire(s.flag + static_cast<size_t>(at) * s.tiles + tile) : 1u;
-        const unsigned ready = __ballot_sync(0xffffffffu, f == 2), missing = __ballot_sync(0xffffffffu, f == 0);
-        const unsigned before = ready ? (ready & (~ready + 1)) - 1 : 0xffffffffu;
-        if (!(missing & before)) {
-            if (ready) {
-                back -= __ffs(ready) - 1;
-                break;
-            }
-            back -= 32;
-            continue;
-        }
-        if (!since) since = clock_ns();
-        else if (clock_ns() - since > kWaitNs) {
-            if (lane == 0) atomicOr(s.status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
-#pragma unroll
-            for (int v = 0; v < V; ++v) h.v[v] = 0.0f;
-            return h;
-        }
-    }
-    __syncwarp();
-    const size_t first = static_cast<size_t>(back) * s.tiles + tile;
-#pragma unroll
-    for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + first * CT + lane * V + v);
-#pragma unroll 4
-    for (unsigned j = back + 1; j < span; ++j) {
-        const float *m = s.map + (static_cast<size_t>(j) * s.tiles + tile) * 2 * CT + lane * V;
-#pragma unroll
-        for (int v = 0; v < V; ++v) h.v[v] = fmaf(__ldcg(m + v), h.v[v], __ldcg(m + CT + v));
-    }
-    return h;
-}
-
-/* Joins a CTA's spans.  Each warp brings its span's (A, H) of V channels a
- * lane, in the order of the scan; returns the state before each warp's span.
- * `after`: the state after the CTA's spans, of warp 0.  The barriers order
- * *next (the CTA's next item) too. */
-template <int CT, int V, int WARPS>
-__device__ __forceinline__ Lane<V> join(const Spans &s, unsigned item, unsigned span, unsigned tile, const Lane<V> &map_a,
-                                        const Lane<V> &map_h, const Lane<V> &initial, float (*sa)[CT], float (*sh)[CT],
-                                        float *carry, int order, int warp, int lane, Lane<V> *after) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         sa[order][lane * V + v] = map_a.v[v];
         sh[order][lane * V + v] = map_h.v[v];
     }
-    Lane<V> h = initial; /* where the span before is done already, its state is read beside the inputs */
-    bool known = span == 0;
-    if (warp == 0 && span > 0) {
-        const size_t prev = static_cast<size_t>(span - 1) * s.tiles + tile;
-        if (load_acquire(s.flag + prev) == 2) {
-            known = true;
-#pragma unroll
-            for (int v = 0; v < V; ++v) h.v[v] = __ldcg(s.state + prev * CT + lane * V + v);
-        }
-        known = __all_sync(0xffffffffu, known);
-    }
     __syncthreads();
-    if (warp == 0) {
-        Lane<V> a, b;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w >= warps) break;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            a.v[v] = 1.0f;
-            b.v[v] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float aw = sa[w][lane * V + v];
-                b.v[v] = fmaf(aw, b.v[v], sh[w][lane * V + v]);
-                a.v[v] *= aw;
-            }
-        }
-        if (!known) {
-            if (span + 1 != s.spans) publish<CT, V>(s, item, 1, a, b, lane);
-            h = state_before<CT, V>(s, span, tile, lane);
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            carry[lane * V + v] = h.v[v];
-            after->v[v] = fmaf(a.v[v], h.v[v], b.v[v]);
+            if (w == order) mine.v[v] = h.v[v];
+            h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
         }
     }
-    __syncthreads();
-    if (warp == 0 && span + 1 != s.spans) publish<CT, V>(s, item, 2, *after, *after, lane);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        h.v[v] = carry[lane * V + v];
-        for (int w = 0; w < order; ++w) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
-    }
-    return h;
+    *state = h;
+    return mine;
 }
 
-/* The same where one CTA takes a tile's spans in turn (STRIP): every warp folds
- * all four spans, which leaves the state after them with each.  buffer: of two,
- * in turn, so that one barrier does. */
-template <int CT, int V, int WARPS>
-__device__ __forceinline__ Lane<V> join_strip(const Lane<V> &map_a, const Lane<V> &map_h, Lane<V> *state, float (*sa)[CT],
-                                              float (*sh)[CT], int order, int lane) {
-    Lane<V> h = *state;
-    if constexpr (WARPS == 1) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) state->v[v] = fmaf(map_a.v[v], h.v[v], map_h.v[v]);
-        return h;
-    } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            sa[order][lane * V + v] = map_a.v[v];
-            sh[order][lane * V + v] = map_h.v[v];
-        }
-        __syncthreads();
-        Lane<V> mine = h;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (w == order) mine.v[v] = h.v[v];
-                h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
-            }
-        *state = h;
-        return mine;
-    }
-}
-
-/* Where a CTA works: spans of a tile.  STRIP: all spans of every gridDim.x-th
- * tile, in turn.  Else single items, by the counter. */
+/* Where a CTA works: a round of a strip of a tile. */
 struct Place {
-    unsigned span, tile;
-    unsigned b;
+    unsigned round, last; /* rounds of the scan's order: this one, the strip's last */
+    unsigned unit, b;
     int c0, live; /* first channel, steps of the sequence that count */
 };
 
 __device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
-    unsigned q = __umulhi(v, magic); /* floor(2^32 / by): at most 2 below */
+    unsigned q = __umulhi(v, magic); /* at most 2 below */
     unsigned r = v - q * by;
     if (r >= by) ++q, r -= by;
     if (r >= by) ++q;
     return q;
 }
 
+/* The first round of a unit. */
 template <int CT>
-__device__ __forceinline__ void settle(Place &at, const RecurrenceShape &d, const int32_t *lengths, const Spans &s) {
-    at.b = divided(at.tile, s.tiles_per_sequence, s.magic_sequence);
-    at.c0 = static_cast<int>(at.tile - at.b * s.tiles_per_sequence) * CT;
+__device__ __forceinline__ Place place_of(unsigned unit, const RecurrenceShape &d, const int32_t *lengths, const Split &s) {
+    Place at;
+    at.unit = unit;
+    const unsigned strip = divided(unit, s.tiles, s.magic_tiles), tile = unit - strip * s.tiles;
+    at.round = strip * s.strip_rounds;
+    at.last = at.round + s.strip_rounds < s.rounds ? at.round + s.strip_rounds - 1 : s.rounds - 1;
+    at.b = divided(tile, s.tiles_per_sequence, s.magic_sequence);
+    at.c0 = static_cast<int>(tile - at.b * s.tiles_per_sequence) * CT;
     at.live = live_of(d, lengths, at.b);
+    return at;
+}
+
+/* The round after it, of the next unit of the CTA at the strip's end. */
+template <int CT>
+__device__ __forceinline__ Place place_after(const Place &at, const RecurrenceShape &d, const int32_t *lengths, const Split &s) {
+    Place next = at;
+    if (++next.round <= at.last) return next;
+    next.unit = at.unit + gridDim.x;
+    if (next.unit < s.tiles * s.strips) next = place_of<CT>(next.unit, d, lengths, s);
+    return next;
+}
+
+/* The state before a strip from `initial`, that before the first one: through
+ * the maps of the strips before it, four parts of them at a time, one for each
+ * of the warps that there are. */
+template <int CT, int V>
+__device__ Lane<V> before_strip(const Split &s, unsigned unit, const Lane<V> &initial, float (*sa)[CT], float (*sh)[CT],
+                                int warp, int warps, int lane) {
+    Lane<V> h = initial;
+    const unsigned strip = divided(unit, s.tiles, s.magic_tiles), tile = unit - strip * s.tiles;
+    const unsigned each = (strip + warps - 1) / warps, first = warp * each;
+    const unsigned last = first + each < strip ? first + each : strip;
+    float a[V], b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+    const float *m = s.maps + (static_cast<size_t>(tile) * s.strips + first) * 2 * CT + lane * V;
+#pragma unroll 8
+    for (unsigned i = first; i < last; ++i, m += 2 * CT)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            b[v] = fmaf(m[v], b[v], m[CT + v]);
+            a[v] *= m[v];
+        }
+    __syncthreads(); /* the round before has read sa, sh */
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        sa[warp][lane * V + v] = a[v];
+        sh[warp][lane * V + v] = b[v];
+    }
+    __syncthreads();
+    for (int w = 0; w < warps; ++w)
+#pragma unroll
+        for (int v = 0; v < V; ++v) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
+    __syncthreads(); /* sa, sh are free again */
+    return h;
+}
+
+/* A strip's map from those of its warps' parts, in the order of the scan. */
+template <int CT, int V>
+__device__ __forceinline__ void leave_map(const Split &s, unsigned unit, const Lane<V> &a, const Lane<V> &b, float (*sa)[CT],
+                                          float (*sh)[CT], int order, int warps, int lane) {
+    __syncthreads(); /* the unit before has read sa, sh */
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        sa[order][lane * V + v] = a.v[v];
+        sh[order][lane * V + v] = b.v[v];
+    }
+    __syncthreads();
+    if (order != 0) return;
+    const unsigned strip = divided(unit, s.tiles, s.magic_tiles), tile = unit - strip * s.tiles;
+    float *m = s.maps + (static_cast<size_t>(tile) * s.strips + strip) * 2 * CT + lane * V;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float all = 1.0f, h = 0.0f;
+        for (int w = 0; w < warps; ++w) {
+            all *= sa[w][lane * V + v];
+            h = fmaf(sa[w][lane * V + v], h, sh[w][lane * V + v]);
+        }
+        m[v] = all;
+        m[CT + v] = h;
+    }
 }
 
 /* ---- forward ---- */
@@ -487,84 +431,50 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
     }
 }
 
-/* The next place of the CTA (STRIP). */
-template <int CT>
-__device__ __forceinline__ Place strip_next(const Place &at, const RecurrenceShape &d, const int32_t *lengths, const Spans &s) {
-    Place next = at;
-    if (++next.span == s.spans) {
-        next.span = 0;
-        next.tile += gridDim.x;
-        if (next.tile < s.tiles) settle<CT>(next, d, lengths, s);
-    }
-    return next;
-}
-
-template <class T, int WARPS, bool STRIP>
-__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(const ForwardArgs p, const Spans s) {
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(const ForwardArgs p, const Split s) {
     constexpr int V = kForwardV<T>, CT = 32 * V;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float sa[STRIP ? 2 : 1][WARPS][CT], sh[STRIP ? 2 : 1][WARPS][CT], carry[CT];
-    __shared__ unsigned mailbox[2];
+    __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT];
     const RecurrenceShape &d = p.d;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, steps = static_cast<int>(d.steps);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, steps = static_cast<int>(d.steps);
     T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 3 * kSteps * CT; /* two stages of x, rec, inp */
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
+    const unsigned units = s.tiles * s.strips;
 
+    const auto step_of = [&](const Place &to) { return static_cast<int>(to.round * warps + warp) * kSteps; };
     const auto start = [&](const Place &to, int stage) {
-        const int t = static_cast<int>(to.span * WARPS + warp) * kSteps, left = static_cast<int>(d.channels) - to.c0;
+        const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0;
         const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
         load_rows<T, CT, 3>(slots + stage * 3 * kSteps * CT, from, to.b * d.is + t * d.it + to.c0, d.it,
                             of_span(to.live, t), left < CT ? left : CT, p.in_piece, lane);
+        return reset_byte(p.reset, to.b * d.steps + t, of_span(to.live, t), lane);
     };
 
-    Place at{}, next{};
-    unsigned item = 0, next_item = 0; /* !STRIP */
-    const auto place = [&](Place &to, unsigned i) {
-        to.span = divided(i, s.tiles, s.magic_tiles);
-        to.tile = i - to.span * s.tiles;
-        settle<CT>(to, d, p.lengths, s);
-    };
-    const auto in_range = [&](const Place &to, unsigned i) { return STRIP ? to.tile < s.tiles : i < s.items; };
-    if (STRIP) {
-        at.tile = blockIdx.x;
-        if (at.tile < s.tiles) settle<CT>(at, d, p.lengths, s);
-    } else {
-        if (threadIdx.x == 0) {
-            mailbox[0] = atomicAdd(s.ticket, 1u);
-            mailbox[1] = atomicAdd(s.ticket, 1u);
-        }
-        __syncthreads();
-        item = mailbox[0];
-        next_item = mailbox[1];
-        if (item < s.items) place(at, item);
-    }
+    Place at = place_of<CT>(blockIdx.x, d, p.lengths, s);
     int stage = 0;
-    if (in_range(at, item)) start(at, 0);
+    unsigned flag = start(at, 0); /* of the step that is the lane's number */
     copies_end();
     float rate[V];
     Lane<V> state;
     bool near = false, fresh = true;
-    while (in_range(at, item)) {
-        const int t = static_cast<int>(at.span * WARPS + warp) * kSteps;
-        const int live = of_span(at.live, t), rows = of_span(steps, t);
-        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+    while (at.unit < units) {
+        const int t = step_of(at), live = of_span(at.live, t), rows = of_span(steps, t);
         T *const xs = slots + stage * 3 * kSteps * CT;
-        if (STRIP) next = strip_next<CT>(at, d, p.lengths, s);
-        else if (next_item < s.items) place(next, next_item);
-        if (in_range(next, next_item)) start(next, stage ^ 1);
+        const unsigned anew = __ballot_sync(0xffffffffu, flag);
+        const Place next = place_after<CT>(at, d, p.lengths, s);
+        if (next.unit < units) flag = start(next, stage ^ 1);
         copies_end();
-        unsigned then = 0;
-        if (!STRIP && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
-        const unsigned anew = reset_bits(p.reset, at.b * d.steps + t, live, lane);
-        if (!STRIP || fresh) {
+        if (fresh) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const size_t c = at.c0 + lane * V + v;
                 const bool in = c < d.channels;
                 rate[v] = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
-                state.v[v] = at.span == 0 && p.state_in && in ? p.state_in[at.b * d.channels + c] : 0.0f;
+                state.v[v] = p.state_in && in ? p.state_in[at.b * d.channels + c] : 0.0f;
             }
             near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
+            if (at.round > 0) state = before_strip<CT, V>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
         copies_wait<1>();
         __syncwarp();
@@ -573,27 +483,21 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
             forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
         else
             forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
-        Lane<V> map_a, map_h, h0;
+        Lane<V> map_a, map_h;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             map_a.v[v] = prod[kSteps - 1][v];
             map_h.v[v] = local[kSteps - 1][v];
         }
-        if constexpr (STRIP) {
-            h0 = join_strip<CT, V, WARPS>(map_a, map_h, &state, sa[stage], sh[stage], warp, lane);
-        } else {
-            const Lane<V> initial = state;
-            h0 = join<CT, V, WARPS>(s, item, at.span, at.tile, map_a, map_h, initial, sa[0], sh[0], carry, warp, warp, lane,
-                                    &state);
-            if (threadIdx.x == 0) mailbox[0] = then;
-        }
-        const bool last = at.span + 1 == s.spans;
+        const Lane<V> h0 = join<CT, V>(map_a, map_h, &state, sa[stage], sh[stage], warp, warps, lane);
+        fresh = at.round == at.last;
+        const bool ends = at.round + 1 == s.rounds && p.state_out && warp == 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const size_t c = at.c0 + lane * V + v;
             if (c >= d.channels) continue;
             if (p.checkpoints && rows > 0) p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] = h0.v[v];
-            if (last && p.state_out && warp == 0) p.state_out[at.b * d.channels + c] = state.v[v];
+            if (ends) p.state_out[at.b * d.channels + c] = state.v[v];
         }
 #pragma unroll
         for (int j = 0; j < kSteps; j += 3 - V) {
@@ -612,17 +516,69 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_forward(con
                 for (int v = 0; v < V; ++v) xs[j * CT + lane * V + v] = from_float<T>(0.0f);
         }
         __syncwarp();
-        store_rows<T, CT>(static_cast<T *>(p.h) + at.b * d.os + t * d.ot + at.c0, xs, d.ot, rows, columns, p.out_piece, lane);
-        if (STRIP) {
-            __syncwarp();
-            fresh = last;
-        } else {
-            __syncthreads(); /* mailbox, and sa, sh, carry are free again */
-            item = next_item;
-            next_item = mailbox[0];
-        }
+        const int left = static_cast<int>(d.channels) - at.c0;
+        store_rows<T, CT>(static_cast<T *>(p.h) + at.b * d.os + t * d.ot + at.c0, xs, d.ot, rows, left < CT ? left : CT,
+                          p.out_piece, lane);
+        __syncwarp();
         at = next;
         stage ^= 1;
+    }
+}
+
+/* The maps of the strips, all but the last: each warp takes consecutive spans. */
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_maps(const ForwardArgs p, const Split s) {
+    constexpr int V = kForwardV<T>, CT = 32 * V;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ float sa[kWarps][CT], sh[kWarps][CT];
+    const RecurrenceShape &d = p.d;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 3 * kSteps * CT;
+    const unsigned units = s.tiles * (s.strips - 1);
+    for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const Place at = place_of<CT>(unit, d, p.lengths, s);
+        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+        const int first = static_cast<int>(at.round * warps + warp * s.strip_rounds), spans = static_cast<int>(s.strip_rounds);
+        const auto start = [&](int span, int stage) {
+            const int t = (first + span) * kSteps, live = of_span(at.live, t);
+            const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
+            load_rows<T, CT, 3>(slots + stage * 3 * kSteps * CT, from, at.b * d.is + t * d.it + at.c0, d.it, live, columns,
+                                p.in_piece, lane);
+            return reset_byte(p.reset, at.b * d.steps + t, live, lane);
+        };
+        unsigned flag = start(0, 0);
+        copies_end();
+        float rate[V];
+        Lane<V> a, b;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const size_t c = at.c0 + lane * V + v;
+            rate[v] = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
+            a.v[v] = 1.0f;
+            b.v[v] = 0.0f;
+        }
+        const bool near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
+        for (int i = 0; i < spans; ++i) {
+            const int live = of_span(at.live, (first + i) * kSteps);
+            const unsigned anew = __ballot_sync(0xffffffffu, flag);
+            const T *xs = slots + (i & 1) * 3 * kSteps * CT;
+            if (i + 1 < spans) flag = start(i + 1, (i + 1) & 1);
+            copies_end();
+            copies_wait<1>();
+            __syncwarp();
+            float prod[kSteps][V], local[kSteps][V];
+            if (live == kSteps && !anew && near)
+                forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+            else
+                forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                b.v[v] = fmaf(prod[kSteps - 1][v], b.v[v], local[kSteps - 1][v]);
+                a.v[v] *= prod[kSteps - 1][v];
+            }
+            __syncwarp();
+        }
+        leave_map<CT, V>(s, unit, a, b, sa, sh, warp, warps, lane);
     }
 }
 
@@ -671,22 +627,24 @@ __device__ __forceinline__ void backward_gates(const T *xs, const T *rs, const T
     }
 }
 
-template <class T, int WARPS, bool STRIP>
-__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(const BackwardArgs p, const Spans s) {
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(const BackwardArgs p, const Split s) {
     constexpr int CT = 32;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float sa[STRIP ? 2 : 1][WARPS][CT], sh[STRIP ? 2 : 1][WARPS][CT], carry[CT], sums[WARPS][CT];
-    __shared__ unsigned mailbox[2];
+    __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT], sums[kWarps][CT];
     const RecurrenceShape &d = p.d;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, steps = static_cast<int>(d.steps);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, steps = static_cast<int>(d.steps);
     constexpr int kSlot = kSteps * CT;
     T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
+    const unsigned units = s.tiles * s.strips;
 
-    /* spans in the order of the scan: the last steps first */
-    const auto step_of = [&](unsigned span) { return static_cast<int>((s.spans - 1 - span) * WARPS + warp) * kSteps; };
+    /* rounds in the order of the scan: the last steps first */
+    const auto step_of = [&](const Place &to) {
+        return static_cast<int>((s.rounds - 1 - to.round) * warps + warp) * kSteps;
+    };
     const auto start = [&](const Place &to, int stage) {
-        const int t = step_of(to.span), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
+        const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
         const int live = of_span(to.live, t);
         const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
         const T *const dh[1] = {static_cast<const T *>(p.dh)};
@@ -694,56 +652,42 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
                             p.in_piece, lane);
         load_rows<T, CT, 1>(slots + stage * 4 * kSlot + 3 * kSlot, dh, to.b * d.os + t * d.ot + to.c0, d.ot, live, columns,
                             p.dh_piece, lane);
+        return reset_byte(p.reset, to.b * d.steps + t, live, lane);
+    };
+    const auto saved_state = [&](const Place &to) {
+        const int t = step_of(to), c = to.c0 + lane;
+        return c < static_cast<int>(d.channels) && t < steps
+                   ? p.checkpoints[(to.b * saved + t / kSteps) * d.channels + c] : 0.0f;
     };
 
-    Place at{}, next{};
-    unsigned item = 0, next_item = 0; /* !STRIP */
-    const auto place = [&](Place &to, unsigned i) {
-        to.span = divided(i, s.tiles, s.magic_tiles);
-        to.tile = i - to.span * s.tiles;
-        settle<CT>(to, d, p.lengths, s);
-    };
-    const auto in_range = [&](const Place &to, unsigned i) { return STRIP ? to.tile < s.tiles : i < s.items; };
-    if (STRIP) {
-        at.tile = blockIdx.x;
-        if (at.tile < s.tiles) settle<CT>(at, d, p.lengths, s);
-    } else {
-        if (threadIdx.x == 0) {
-            mailbox[0] = atomicAdd(s.ticket, 1u);
-            mailbox[1] = atomicAdd(s.ticket, 1u);
-        }
-        __syncthreads();
-        item = mailbox[0];
-        next_item = mailbox[1];
-        if (item < s.items) place(at, item);
-    }
+    Place at = place_of<CT>(blockIdx.x, d, p.lengths, s);
     int stage = 0;
-    if (in_range(at, item)) start(at, 0);
+    unsigned flag = start(at, 0); /* of the step that is the lane's number */
+    float h_next = saved_state(at);
     copies_end();
     float rate = 0.0f, sum_all = 0.0f;
     Lane<1> state;
     bool near = false, fresh = true;
-    while (in_range(at, item)) {
-        const int t = step_of(at.span);
-        const int live = of_span(at.live, t), rows = of_span(steps, t);
-        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+    while (at.unit < units) {
+        const int t = step_of(at), live = of_span(at.live, t), rows = of_span(steps, t);
         const size_t c = at.c0 + lane;
         const bool in = c < d.channels;
         T *const xs = slots + stage * 4 * kSlot;
-        if (STRIP) next = strip_next<CT>(at, d, p.lengths, s);
-        else if (next_item < s.items) place(next, next_item);
-        if (in_range(next, next_item)) start(next, stage ^ 1);
+        const unsigned anew = __ballot_sync(0xffffffffu, flag);
+        const float h = h_next;
+        const Place next = place_after<CT>(at, d, p.lengths, s);
+        if (next.unit < units) {
+            flag = start(next, stage ^ 1);
+            h_next = saved_state(next);
+        }
         copies_end();
-        unsigned then = 0;
-        if (!STRIP && threadIdx.x == 0) then = atomicAdd(s.ticket, 1u);
-        const unsigned anew = reset_bits(p.reset, at.b * d.steps + t, live, lane);
-        if (!STRIP || fresh) {
+        if (fresh) {
             rate = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
-            state.v[0] = at.span == 0 && p.dstate_out && in ? p.dstate_out[at.b * d.channels + c] : 0.0f;
+            state.v[0] = p.dstate_out && in ? p.dstate_out[at.b * d.channels + c] : 0.0f;
             near = __all_sync(0xffffffffu, rate >= -kNear);
             sum_all = 0.0f;
+            if (at.round > 0) state = before_strip<CT, 1>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        const float h = in && rows > 0 ? p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] : 0.0f;
         Lane<1> map_a, map_h;
         copies_wait<1>();
         __syncwarp();
@@ -760,17 +704,9 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
             map_h.v[0] = a[j] * (g + map_h.v[0]);
             map_a.v[0] *= a[j];
         }
-        float grad;
-        const bool last = at.span + 1 == s.spans;
-        if constexpr (STRIP) {
-            grad = join_strip<CT, 1, WARPS>(map_a, map_h, &state, sa[stage], sh[stage], WARPS - 1 - warp, lane).v[0];
-        } else {
-            const Lane<1> initial = state;
-            grad = join<CT, 1, WARPS>(s, item, at.span, at.tile, map_a, map_h, initial, sa[0], sh[0], carry,
-                                      WARPS - 1 - warp, warp, lane, &state).v[0];
-            if (threadIdx.x == 0) mailbox[0] = then;
-        }
-        if (last && p.dstate_in && in && warp == 0) p.dstate_in[at.b * d.channels + c] = state.v[0];
+        float grad = join<CT, 1>(map_a, map_h, &state, sa[stage], sh[stage], warps - 1 - warp, warps, lane).v[0];
+        fresh = at.round == at.last;
+        if (at.round + 1 == s.rounds && p.dstate_in && in && warp == 0) p.dstate_in[at.b * d.channels + c] = state.v[0];
         F2 sums2 = both(0.0f);
 #pragma unroll
         for (int j = kSteps - 2; j >= 0; j -= 2) {
@@ -801,33 +737,88 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_backward(co
         sum += sum_odd;
         __syncwarp();
         const size_t to = at.b * d.gs + t * d.gt + at.c0;
+        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
         store_rows<T, CT>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
         store_rows<T, CT>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
         store_rows<T, CT>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
-        sum_all = STRIP ? sum_all + sum : sum;
-        if (p.partial && (!STRIP || last)) {
-            if (WARPS > 1) {
-                sums[warp][lane] = sum_all;
-                __syncthreads();
-                if (warp == 0) {
-                    sum_all = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < WARPS; ++i) sum_all += sums[i][lane];
-                }
+        sum_all += sum;
+        if (fresh && p.partial) {
+            sums[warp][lane] = sum_all;
+            __syncthreads();
+            if (warp == 0 && in) {
+                sum_all = 0.0f;
+                for (int i = 0; i < warps; ++i) sum_all += sums[i][lane];
+                const size_t strip = divided(at.unit, s.tiles, s.magic_tiles);
+                p.partial[(strip * d.sequences + at.b) * d.channels + c] = sum_all;
             }
-            const size_t row = STRIP ? at.b : static_cast<size_t>(at.span) * d.sequences + at.b;
-            if (warp == 0 && in) p.partial[row * d.channels + c] = sum_all;
+            __syncthreads(); /* sums is free again */
         }
-        if (STRIP) {
-            __syncwarp();
-            fresh = last;
-        } else {
-            __syncthreads(); /* mailbox, and sa, sh, carry, sums are free again */
-            item = next_item;
-            next_item = mailbox[0];
-        }
+        __syncwarp();
         at = next;
         stage ^= 1;
+    }
+}
+
+/* The maps of the strips, all but the last of the scan: of rec and dh alone. */
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_maps(const BackwardArgs p, const Split s) {
+    constexpr int CT = 32, kSlot = kSteps * CT;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ float sa[kWarps][CT], sh[kWarps][CT];
+    const RecurrenceShape &d = p.d;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot;
+    const unsigned units = s.tiles * (s.strips - 1);
+    for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const Place at = place_of<CT>(unit, d, p.lengths, s);
+        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+        /* the strip's spans from its last steps on; warp 0 takes the first ones of the scan */
+        const int spans = static_cast<int>(s.strip_rounds);
+        const int top = static_cast<int>((s.rounds - at.round) * warps) - 1 - warp * spans;
+        const auto start = [&](int span, int stage) {
+            const int t = (top - span) * kSteps, live = of_span(at.live, t);
+            const T *const rec[1] = {static_cast<const T *>(p.rec)}, *const dh[1] = {static_cast<const T *>(p.dh)};
+            load_rows<T, CT, 1>(slots + stage * 2 * kSlot, rec, at.b * d.is + t * d.it + at.c0, d.it, live, columns,
+                                p.in_piece, lane);
+            load_rows<T, CT, 1>(slots + stage * 2 * kSlot + kSlot, dh, at.b * d.os + t * d.ot + at.c0, d.ot, live, columns,
+                                p.dh_piece, lane);
+            return reset_byte(p.reset, at.b * d.steps + t, live, lane);
+        };
+        unsigned flag = start(0, 0);
+        copies_end();
+        const size_t c = at.c0 + lane;
+        const float rate = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
+        Lane<1> all, grad;
+        all.v[0] = 1.0f;
+        grad.v[0] = 0.0f;
+        for (int i = 0; i < spans; ++i) {
+            const int live = of_span(at.live, (top - i) * kSteps);
+            const unsigned anew = __ballot_sync(0xffffffffu, flag);
+            const T *rs = slots + (i & 1) * 2 * kSlot;
+            if (i + 1 < spans) flag = start(i + 1, (i + 1) & 1);
+            copies_end();
+            copies_wait<1>();
+            __syncwarp();
+#pragma unroll
+            for (int j = kSteps - 2; j >= 0; j -= 2) {
+                const int to = j * CT + lane;
+                const Decay k = decay_of<false>(both(rate), sigmoid2(pair(to_float(rs[to]), to_float(rs[to + CT]))));
+                float a0, a1;
+                split(k.a, a0, a1);
+                if (anew >> j & 1) a0 = 0.0f;
+                if (anew >> (j + 1) & 1) a1 = 0.0f;
+                if (j + 1 < live) {
+                    grad.v[0] = a1 * (to_float(rs[kSlot + to + CT]) + grad.v[0]);
+                    all.v[0] *= a1;
+                }
+                if (j < live) {
+                    grad.v[0] = a0 * (to_float(rs[kSlot + to]) + grad.v[0]);
+                    all.v[0] *= a0;
+                }
+            }
+            __syncwarp();
+        }
+        leave_map<CT, 1>(s, unit, all, grad, sa, sh, warp, warps, lane);
     }
 }
 
@@ -864,45 +855,40 @@ bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     return s->it >= d->channels && s->ot >= d->channels && s->gt >= d->channels;
 }
 
-/* A tile's spans are taken in turn by one CTA where there are at least kStrip
- * tiles, else by different CTAs. */
-constexpr unsigned kStrip = 296;
-bool strips(const Spans &s) { return s.spans == 1 || s.tiles >= kStrip; }
+constexpr unsigned kFill = 16 * 148;   /* warps that the kernels' registers leave room for on the GPU */
+constexpr unsigned kLeastRounds = 2;   /* of a strip */
 
-struct Layout {
-    Spans spans;
-    size_t flags_bytes, bytes;
-};
-
-/* `warps` spans of 16 steps a CTA, `tile` channels. */
-Layout spans_of(const RecurrenceShape &d, int warps, int tile, void *workspace) {
-    Layout l{};
-    Spans &s = l.spans;
-    s.spans = static_cast<unsigned>((d.steps + warps * kSteps - 1) / (warps * kSteps));
+/* Warps: as many as leave every tile room on the GPU at once.  Strips: where
+ * tiles of four warps take less than a third of the room. */
+Split split_of(const RecurrenceShape &d, int tile, int *warps) {
+    Split s{};
     s.tiles_per_sequence = static_cast<unsigned>((d.channels + tile - 1) / tile);
     s.tiles = static_cast<unsigned>(d.sequences * s.tiles_per_sequence);
-    s.items = s.spans * s.tiles;
+    const unsigned spans = static_cast<unsigned>((d.steps + kSteps - 1) / kSteps);
+    unsigned w = kFill / s.tiles;
+    w = w < 1 ? 1 : w > kWarps ? kWarps : w;
+    w = w > spans ? spans : w;
+    s.rounds = (spans + w - 1) / w;
+    unsigned strips = kFill / (s.tiles * w);
+    if (strips < 3) strips = 1;
+    const unsigned most = s.rounds / kLeastRounds;
+    if (strips > most) strips = most < 2 ? 1 : most;
+    s.strip_rounds = (s.rounds + strips - 1) / strips;
+    s.strips = (s.rounds + s.strip_rounds - 1) / s.strip_rounds;
     s.magic_tiles = static_cast<unsigned>(0xffffffffull / s.tiles);
     s.magic_sequence = static_cast<unsigned>(0xffffffffull / s.tiles_per_sequence);
-    if (!strips(s)) {
-        char *at = static_cast<char *>(workspace);
-        l.flags_bytes = align_up(16 + static_cast<size_t>(s.items) * 4, 16);
-        const size_t row = static_cast<size_t>(s.items) * tile * sizeof(float);
-        s.ticket = reinterpret_cast<unsigned *>(at);
-        s.flag = s.ticket + 4;
-        s.map = reinterpret_cast<float *>(at + l.flags_bytes);
-        s.state = reinterpret_cast<float *>(at + l.flags_bytes + 2 * row);
-        l.bytes = l.flags_bytes + 3 * row;
-    }
-    return l;
+    *warps = static_cast<int>(w);
+    return s;
+}
+size_t map_bytes(const Split &s, int tile) {
+    return s.strips > 1 ? static_cast<size_t>(s.tiles) * s.strips * 2 * tile * sizeof(float) : 0;
 }
 
-int warps_for(const RecurrenceShape &d) { return d.steps <= kSteps ? 1 : kWarps; }
 int forward_tile(int type) { return type == TB_TYPE_F32 ? 32 : 64; }
 
 /* Rows of partial sums for ddecay, and behind them the parts that they are first summed into. */
-size_t partial_rows(const RecurrenceShape &d, const Spans &s) { return strips(s) ? d.sequences : d.sequences * s.spans; }
-size_t partial_bytes(const RecurrenceShape &d, const Spans &s) {
+size_t partial_rows(const RecurrenceShape &d, const Split &s) { return d.sequences * s.strips; }
+size_t partial_bytes(const RecurrenceShape &d, const Split &s) {
     const size_t rows = partial_rows(d, s);
     return (rows + column_parts(rows)) * d.channels * sizeof(float);
 }
@@ -913,25 +899,26 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
     return all % 16 == 0 ? 16 : all % 4 == 0 && least == 4 ? 4 : 0;
 }
 
-/* Launches a kernel of persistent CTAs over l's items. */
+/* Launches the strips' maps, where there are strips, and the scan. */
 template <class Kernel, class Args>
-int launch_items(Kernel strip, Kernel single, const Args &args, Layout &l, int warps, size_t shared, cudaStream_t st) {
-    const bool in_turn = strips(l.spans);
-    const Kernel kernel = in_turn ? strip : single;
+int launch_scan(Kernel maps, Kernel scan, const Args &args, const Split &s, int warps, size_t shared, cudaStream_t st) {
     int dev = 0, sms = 0, per_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) !=
-            cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, warps * 32, shared) != cudaSuccess)
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return 0;
-    if (!in_turn) {
-        l.spans.status = tb_status_slot(st);
-        if (!l.spans.status || cudaMemsetAsync(l.spans.ticket, 0, l.flags_bytes, st) != cudaSuccess) return 0;
+    const Kernel kernels[2] = {maps, scan};
+    const unsigned work[2] = {s.tiles * (s.strips - 1), s.tiles * s.strips};
+    for (int i = 0; i < 2; ++i) {
+        if (work[i] == 0) continue;
+        if (cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) !=
+                cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernels[i], warps * 32, shared) != cudaSuccess)
+            return 0;
+        const unsigned most = static_cast<unsigned>(sms * per_sm);
+        kernels[i]<<<work[i] < most ? work[i] : most, warps * 32, shared, st>>>(args, s);
+        if (!launched()) return 0;
     }
-    const unsigned most = static_cast<unsigned>(sms * per_sm), work = in_turn ? l.spans.tiles : l.spans.items;
-    kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args, l.spans);
-    return launched();
+    return 1;
 }
 
 } /* namespace */
@@ -939,10 +926,12 @@ int launch_items(Kernel strip, Kernel single, const Args &args, Layout &l, int w
 extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_desc *desc) {
     RecurrenceShape s;
     if (!recurrence_shape(desc, &s)) return 0;
-    const int warps = warps_for(s);
-    const Layout f = spans_of(s, warps, forward_tile(desc->type), nullptr), b = spans_of(s, warps, 32, nullptr);
-    const size_t back = align_up(b.bytes, 16) + partial_bytes(s, b.spans);
-    return f.bytes > back ? f.bytes : back;
+    int warps;
+    const int tile = forward_tile(desc->type);
+    const size_t f = map_bytes(split_of(s, tile, &warps), tile);
+    const Split b = split_of(s, 32, &warps);
+    const size_t back = map_bytes(b, 32) + partial_bytes(s, b);
+    return f > back ? f : back;
 }
 
 extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *desc, const void *x,
@@ -963,15 +952,15 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
                          reinterpret_cast<uintptr_t>(input_gate);
     p.in_piece = piece_of(reinterpret_cast<const void *>(in), s.is, s.it, size, 4);
     p.out_piece = piece_of(h, s.os, s.ot, size, 16);
-    const int warps = warps_for(s), tile = forward_tile(desc->type);
-    Layout l = spans_of(s, warps, tile, workspace);
+    int warps;
+    const int tile = forward_tile(desc->type);
+    Split split = split_of(s, tile, &warps);
+    split.maps = static_cast<float *>(workspace);
     const size_t shared = static_cast<size_t>(warps) * 2 * 3 * kSteps * tile * size;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return warps == 1 ? launch_items(recurrence_forward<T, 1, true>, recurrence_forward<T, 1, true>, p, l, 1, shared, st)
-                          : launch_items(recurrence_forward<T, kWarps, true>, recurrence_forward<T, kWarps, false>, p, l,
-                                         kWarps, shared, st);
+        return launch_scan(recurrence_forward_maps<T>, recurrence_forward<T>, p, split, warps, shared,
+                           static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -1000,9 +989,10 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
         outs |= reinterpret_cast<uintptr_t>(out[i]);
     }
     cudaGetLastError(); /* report these launches only */
-    const int warps = warps_for(s);
-    Layout l = spans_of(s, warps, 32, workspace);
-    float *partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + align_up(l.bytes, 16));
+    int warps;
+    Split split = split_of(s, 32, &warps);
+    split.maps = static_cast<float *>(workspace);
+    float *partial = split.maps + map_bytes(split, 32) / sizeof(float);
     BackwardArgs p{s, x, recurrence_gate, input_gate, dh, decay, checkpoints, dstate_out, reset, lengths, dx,
                    drecurrence_gate, dinput_gate, ddecay ? partial : nullptr, dstate_in, 0, 0, 0};
     p.in_piece = piece_of(reinterpret_cast<const void *>(ins), s.is, s.it, size, 4);
@@ -1012,12 +1002,10 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return warps == 1 ? launch_items(recurrence_backward<T, 1, true>, recurrence_backward<T, 1, true>, p, l, 1, shared, st)
-                          : launch_items(recurrence_backward<T, kWarps, true>, recurrence_backward<T, kWarps, false>, p, l,
-                                         kWarps, shared, st);
+        return launch_scan(recurrence_backward_maps<T>, recurrence_backward<T>, p, split, warps, shared, st);
     });
     if (!ok || !ddecay) return ok;
-    const size_t rows = partial_rows(s, l.spans), parts = column_parts(rows);
+    const size_t rows = partial_rows(s, split), parts = column_parts(rows);
     float *sums = partial + rows * s.channels;
     column_sums<<<dim3(static_cast<unsigned>((s.channels + 31) / 32), static_cast<unsigned>(parts)), kColumnThreads, 0,
                   st>>>(partial, rows, s.channels, sums);
