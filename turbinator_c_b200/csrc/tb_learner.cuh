@@ -10,6 +10,9 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "turbinator/training/cuda_learner.h"
 
@@ -30,6 +33,61 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <class T, int N> struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
+
+/* A pack as the words it came in, taken apart where it is used. */
+template <class T, int N> struct alignas(sizeof(T) * N) Held {
+    uint32_t w[N * sizeof(T) / 4];
+};
+template <> struct Held<__nv_bfloat16, 1> {
+    uint16_t w[1];
+};
+template <> struct Held<__half, 1> {
+    uint16_t w[1];
+};
+template <class T, int N> __device__ __forceinline__ void unpack(const Held<T, N> &h, float (&f)[N]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __uint_as_float(h.w[i]);
+    } else if constexpr (N == 1) {
+        T v;
+        memcpy(&v, h.w, 2);
+        f[0] = to_float(v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&h.w[i]));
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            } else {
+                f[2 * i] = __uint_as_float(h.w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(h.w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+template <class T, int N> __device__ __forceinline__ Held<T, N> packed(const float (&f)[N]) {
+    Held<T, N> h;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) h.w[i] = __float_as_uint(f[i]);
+    } else if constexpr (N == 1) {
+        const T v = from_float<T>(f[0]);
+        memcpy(h.w, &v, 2);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                memcpy(&h.w[i], &t, 4);
+            } else {
+                const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                memcpy(&h.w[i], &t, 4);
+            }
+        }
+    }
+    return h;
+}
 
 /* ---- warp reductions (every lane receives the result) ---- */
 
