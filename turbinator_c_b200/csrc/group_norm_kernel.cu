@@ -3,9 +3,10 @@
  * (include/turbinator/training/cuda_learner.h).
  *
  * Bound: HBM, given that x (and dy) are read once.  A tile is some positions of
- * some whole groups of one sample; a CTA holds a tile in registers, so that mean,
- * variance about that mean, and result come from one read.  Threads form rows
- * of `lanes` packs, each thread keeping its channels over all its positions.
+ * some whole groups of one sample; a CTA keeps a tile in shared memory, filled
+ * by asynchronous copies, so that mean, variance about that mean, and result
+ * come from one read.  Threads form rows of `lanes` packs, each thread keeping
+ * its channels over all its positions.
  *
  *   - A sample's groups that fit one tile, or the tiles of one cluster (8 CTAs),
  *     take one kernel: the tiles' statistics meet in distributed shared memory.
@@ -43,97 +44,181 @@ struct Tiling {
     int pack;                /* elements of a load */
     int block_groups, lanes; /* groups and packs of a tile's row */
     int blocks, threads, rows_at_once;
-    size_t rows;             /* positions of a part */
-    size_t parts;
+    int rows, parts;         /* positions of a part */
+    int rows_held;           /* positions that the tile has room for */
+    unsigned magic_parts, magic_blocks, magic_lanes, magic_rows, magic_group; /* floor((2^32 - 1) / ..), rows: rows_at_once */
     bool fits;               /* the parts fit one cluster */
+    size_t tiles;            /* of all samples */
 };
 
-__device__ __forceinline__ float activate(float u, int act) {
-    if (act == TB_ACT_SILU) return u * fast_sigmoid(u);
-    if (act == TB_ACT_RELU) return u > 0.0f || u != u ? u : 0.0f;
-    if (act == TB_ACT_GELU) return 0.5f * u * (1.0f + erff(u * 0.70710678f));
-    return u;
+/* v / by for v < 2^31, from floor((2^32 - 1) / by). */
+__device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
+    unsigned q = __umulhi(v, magic); /* at most 2 below */
+    unsigned r = v - q * by;
+    if (r >= by) ++q, r -= by;
+    if (r >= by) ++q;
+    return q;
 }
 
-__device__ __forceinline__ float slope(float u, int act) {
+template <class V, int N> __device__ __forceinline__ void activate(V (&u)[N], int act) {
     if (act == TB_ACT_SILU) {
-        const float s = fast_sigmoid(u);
-        return s * (1.0f + u * (1.0f - s));
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = vmul(u[i], vsigmoid(u[i]));
+    } else if (act == TB_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = veach(u[i], [](float v) { return v > 0.0f || v != v ? v : 0.0f; });
+    } else if (act == TB_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = veach(u[i], [](float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678f)); });
     }
-    if (act == TB_ACT_RELU) return u > 0.0f ? 1.0f : 0.0f;
-    if (act == TB_ACT_GELU) return 0.5f * (1.0f + erff(u * 0.70710678f)) + u * expf(-0.5f * u * u) * 0.39894228f;
-    return 1.0f;
+}
+
+/* u becomes the activation's slope there. */
+template <class V, int N> __device__ __forceinline__ void slopes(V (&u)[N], int act) {
+    if (act == TB_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { /* s (1 + u (1 - s)) */
+            const V s = vsigmoid(u[i]);
+            const V t = vfma(s, vall<V>(-1.0f), vall<V>(1.0f));
+            u[i] = vmul(s, vfma(u[i], t, vall<V>(1.0f)));
+        }
+    } else if (act == TB_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = veach(u[i], [](float v) { return v > 0.0f ? 1.0f : 0.0f; });
+    } else if (act == TB_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            u[i] = veach(u[i], [](float v) {
+                return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * expf(-0.5f * v * v) * 0.39894228f;
+            });
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = vall<V>(1.0f);
+    }
 }
 
 /* ---- a tile ---- */
 
-/* Packs that a thread holds: 32 registers' worth. */
-template <class T, int PACK> constexpr int kHeld = PACK * sizeof(T) == 16 ? 8 : 32;
-
 /* Where a CTA and its thread are. */
 struct Seat {
-    size_t n, part;
-    int block, lane, row, c0; /* c0: the tile's first channel */
-    size_t first;             /* the tile's first position */
-    int rows;                 /* its positions */
-    bool in;                  /* the thread has a place in the rows */
-    int mine;                 /* positions of the thread */
+    unsigned n;
+    int part, block, lane, row, c0; /* c0: the tile's first channel */
+    int first, rows;                /* the tile's first position, its positions */
+    int mine;                       /* positions of the thread */
+    int groups, channels;           /* of the tile: fewer in a sample's last block */
+    bool in;                        /* the thread has a place in the rows */
 };
 
-__device__ __forceinline__ Seat seat_of(const NormShape &d, const Tiling &g, size_t tile) {
+__device__ __forceinline__ Seat seat_of(const NormShape &d, const Tiling &g, unsigned tile) {
     Seat s;
-    s.part = tile % g.parts; /* the parts of a cluster are neighbours */
-    s.block = static_cast<int>(tile / g.parts % g.blocks);
-    s.n = tile / g.parts / g.blocks;
+    const unsigned whole = divided(tile, g.parts, g.magic_parts);
+    s.part = static_cast<int>(tile - whole * g.parts); /* the parts of a cluster are neighbours */
+    s.n = divided(whole, g.blocks, g.magic_blocks);
+    s.block = static_cast<int>(whole - s.n * g.blocks);
     s.c0 = s.block * g.block_groups * d.per_group;
-    s.lane = threadIdx.x % g.lanes;
-    s.row = threadIdx.x / g.lanes;
+    s.row = static_cast<int>(divided(threadIdx.x, g.lanes, g.magic_lanes));
+    s.lane = static_cast<int>(threadIdx.x) - s.row * g.lanes;
     s.first = s.part * g.rows;
-    const size_t left = d.positions - s.first;
-    s.rows = static_cast<int>(left < g.rows ? left : g.rows);
-    s.in = s.row < g.rows_at_once;
-    s.mine = s.in && s.row < s.rows ? (s.rows - s.row + g.rows_at_once - 1) / g.rows_at_once : 0;
+    s.rows = min(static_cast<int>(d.positions) - s.first, g.rows);
+    s.groups = min(g.block_groups, d.groups - s.block * g.block_groups);
+    s.channels = s.groups * d.per_group;
+    s.in = s.row < g.rows_at_once && s.lane * g.pack < s.channels;
+    s.mine = s.in && s.row < s.rows
+                 ? static_cast<int>(divided(s.rows - s.row + g.rows_at_once - 1, g.rows_at_once, g.magic_rows)) : 0;
     return s;
 }
 
-template <class T, int PACK, int HELD>
-__device__ __forceinline__ void load_tile(Held<T, PACK> (&v)[HELD], const T *p, size_t stride, const Seat &s, const Tiling &g) {
+template <class T, int PACK> __device__ __forceinline__ void copy_pack(Held<T, PACK> *to, const T *from) {
+    const uint32_t t = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    if constexpr (PACK * sizeof(T) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(t), "l"(from) : "memory");
+    else if constexpr (PACK * sizeof(T) == 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(t), "l"(from) : "memory");
+    else
+        *to = *reinterpret_cast<const Held<T, PACK> *>(from);
+}
+
+/* Starts copying the thread's packs into its places of the tile (to[i * step]
+ * is its i-th); it reads no others, so that its own wait will do. */
+template <class T, int PACK>
+__device__ __forceinline__ void load_tile(Held<T, PACK> *to, int step, const T *p, size_t stride, const Seat &s, const Tiling &g) {
     p += (s.first + s.row) * stride + s.c0 + s.lane * PACK;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i < s.mine) v[i] = *reinterpret_cast<const Held<T, PACK> *>(p);
-        p += g.rows_at_once * stride;
+    const size_t jump = g.rows_at_once * stride;
+#pragma unroll 4
+    for (int i = 0; i < s.mine; ++i) {
+        copy_pack<T, PACK>(to, p);
+        to += step;
+        p += jump;
     }
+}
+__device__ __forceinline__ void tile_loaded() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+/* Per-channel values of a thread. */
+template <int PACK> struct Channels {
+    Array<PACK> v;
+};
+/* f(channel of the tile) for each of the thread's; of its first where it has none. */
+template <int PACK, class F> __device__ __forceinline__ Channels<PACK> channels_of(const Seat &s, F &&f) {
+    float t[PACK];
+#pragma unroll
+    for (int k = 0; k < PACK; ++k) t[k] = f(s.in ? s.lane * PACK + k : 0);
+    Channels<PACK> r;
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) r.v[k] = vload<typename Values<PACK>::V>(t + 2 * k);
+    return r;
+}
+__device__ __forceinline__ int group_of(int channel, const NormShape &d, const Tiling &g) {
+    return static_cast<int>(divided(channel, d.per_group, g.magic_group));
+}
+
+template <class T, int PACK>
+__device__ __forceinline__ void taken(const Held<T, PACK> &h, Array<PACK> &v) {
+    float e[PACK];
+    unpack(h, e);
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) v[k] = vload<typename Values<PACK>::V>(e + 2 * k);
+}
+template <class T, int PACK> __device__ __forceinline__ void put(T *to, const Array<PACK> &v) {
+    float e[PACK];
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(e + 2 * k, v[k]);
+    *reinterpret_cast<Held<T, PACK> *>(to) = packed<T, PACK>(e);
 }
 
 /* ---- sums over a tile ---- */
 
-/* Shared memory of a tile: rows of per-channel partial sums (pitch channels +
- * 4), channel totals, and per group four values. */
+/* Shared memory of a tile: the tile (x, then dy), rows of per-channel partial
+ * sums (pitch channels + 4), channel totals, and per group four values. */
 struct Sums {
     float *rows, *channel, *group;
+    unsigned char *tile;
     int pitch;
 };
 __device__ __forceinline__ Sums sums_of(float *shared, const NormShape &d, const Tiling &g) {
     Sums s;
     const int channels = g.lanes * g.pack;
-    s.pitch = channels + 4;
+    s.pitch = ((channels + 3) & ~3) + 4;
     s.rows = shared;
     s.channel = shared + g.rows_at_once * s.pitch;
     s.group = s.channel + 2 * ((channels + 3) & ~3);
+    s.tile = reinterpret_cast<unsigned char *>(s.group + 4 * g.block_groups);
     return s;
 }
-size_t sums_bytes(const Tiling &g) {
-    const size_t channels = static_cast<size_t>(g.lanes) * g.pack;
-    return (g.rows_at_once * (channels + 4) + 2 * ((channels + 3) & ~size_t(3)) + 4 * g.block_groups) * sizeof(float);
+size_t shared_bytes(const Tiling &g, size_t size, int tensors) {
+    const size_t channels = (static_cast<size_t>(g.lanes) * g.pack + 3) & ~size_t(3);
+    return (g.rows_at_once * (channels + 4) + 2 * channels + 4 * g.block_groups) * sizeof(float) +
+           static_cast<size_t>(tensors) * g.rows_held * g.lanes * g.pack * size;
 }
 
-/* channel[c] = the sum over the CTA's rows of each thread's own[PACK]; ends
+/* channel[c] = the sum over the CTA's rows of each thread's own values; ends
  * with the totals visible to all. */
 template <int PACK>
-__device__ __forceinline__ void channel_totals(const float (&own)[PACK], float *channel, const Sums &s, const Seat &at,
+__device__ __forceinline__ void channel_totals(const Array<PACK> &sums, float *channel, const Sums &s, const Seat &at,
                                                const Tiling &g) {
     if (at.in) {
+        float own[PACK];
+#pragma unroll
+        for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(own + 2 * k, sums[k]);
         float *to = s.rows + at.row * s.pitch + at.lane * PACK;
         if constexpr (PACK % 4 == 0) {
 #pragma unroll
@@ -146,7 +231,7 @@ __device__ __forceinline__ void channel_totals(const float (&own)[PACK], float *
     }
     __syncthreads();
     /* `share` neighbouring threads for each channel */
-    const int channels = g.lanes * PACK;
+    const int channels = at.channels;
     int share = 1;
     while (share < 32 && share * 2 * channels <= static_cast<int>(blockDim.x)) share *= 2;
     const int mine = threadIdx.x % share;
@@ -163,15 +248,15 @@ __device__ __forceinline__ void channel_totals(const float (&own)[PACK], float *
 
 /* f(group, sum over its channels of value(channel)) for each of the tile's groups, by one thread each. */
 template <class Value, class F>
-__device__ __forceinline__ void group_totals(const NormShape &d, const Tiling &g, Value &&value, F &&f) {
+__device__ __forceinline__ void group_totals(const NormShape &d, const Seat &at, Value &&value, F &&f) {
     if (d.per_group <= 32) {
-        for (int i = threadIdx.x; i < g.block_groups; i += blockDim.x) {
+        for (int i = threadIdx.x; i < at.groups; i += blockDim.x) {
             float t = 0.0f;
             for (int c = i * d.per_group; c < (i + 1) * d.per_group; ++c) t += value(c);
             f(i, t);
         }
     } else {
-        for (int i = threadIdx.x / 32; i < g.block_groups; i += blockDim.x / 32) {
+        for (int i = threadIdx.x / 32; i < at.groups; i += blockDim.x / 32) {
             float t = 0.0f;
             for (int c = threadIdx.x % 32; c < d.per_group; c += 32) t += value(i * d.per_group + c);
             t = warp_sum(t);
@@ -184,82 +269,67 @@ __device__ __forceinline__ void group_totals(const NormShape &d, const Tiling &g
 
 /* Leaves the tile's own mean and squares about it of each group in
  * s.group[2 * group], [2 * group + 1]; visible to all. */
-template <class T, int PACK, int HELD>
-__device__ __forceinline__ void tile_statistics(const Held<T, PACK> (&v)[HELD], const Sums &s, const Seat &at, const NormShape &d,
-                                                const Tiling &g) {
-    float own[PACK];
+template <class T, int PACK>
+__device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int step, const Sums &s, const Seat &at,
+                                                const NormShape &d, const Tiling &g) {
+    using V = typename Values<PACK>::V;
+    constexpr int N = Values<PACK>::kCount;
+    Array<PACK> own, e;
 #pragma unroll
-    for (int k = 0; k < PACK; ++k) own[k] = 0.0f;
+    for (int k = 0; k < N; ++k) own[k] = vall<V>(0.0f);
+#pragma unroll 4
+    for (int i = 0; i < at.mine; ++i) {
+        taken<T, PACK>(tile[i * step], e);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        if (i < at.mine) {
-            float e[PACK];
-            unpack(v[i], e);
-#pragma unroll
-            for (int k = 0; k < PACK; ++k) own[k] += e[k];
-        }
+        for (int k = 0; k < N; ++k) own[k] = vadd(own[k], e[k]);
+    }
     channel_totals<PACK>(own, s.channel, s, at, g);
     const float count = static_cast<float>(at.rows) * static_cast<float>(d.per_group);
-    group_totals(d, g, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i] = t / count; });
+    group_totals(d, at, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i] = t / count; });
     __syncthreads();
-    float mean[PACK];
+    const Channels<PACK> less = channels_of<PACK>(at, [&](int c) { return -s.group[2 * group_of(c, d, g)]; });
 #pragma unroll
-    for (int k = 0; k < PACK; ++k) {
-        mean[k] = at.in ? s.group[2 * ((at.lane * PACK + k) / d.per_group)] : 0.0f;
-        own[k] = 0.0f;
-    }
+    for (int k = 0; k < N; ++k) own[k] = vall<V>(0.0f);
+#pragma unroll 4
+    for (int i = 0; i < at.mine; ++i) {
+        taken<T, PACK>(tile[i * step], e);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        if (i < at.mine) {
-            float e[PACK];
-            unpack(v[i], e);
-#pragma unroll
-            for (int k = 0; k < PACK; ++k) {
-                const float off = e[k] - mean[k];
-                own[k] = fmaf(off, off, own[k]);
-            }
+        for (int k = 0; k < N; ++k) {
+            const V off = vadd(e[k], less.v[k]);
+            own[k] = vfma(off, off, own[k]);
         }
+    }
     channel_totals<PACK>(own, s.channel, s, at, g);
-    group_totals(d, g, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i + 1] = t; });
+    group_totals(d, at, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i + 1] = t; });
     __syncthreads();
 }
 
 /* A thread's channels: u = (x - mean) scale + shift. */
 template <int PACK> struct Affine {
-    float mean[PACK], scale[PACK], shift[PACK];
+    Channels<PACK> less, scale, shift; /* less = -mean */
 };
-
-template <class T, int PACK, int HELD>
-__device__ __forceinline__ void write_tile(const Held<T, PACK> (&v)[HELD], const Affine<PACK> &f, T *p, size_t stride, int act,
-                                           const Seat &s, const Tiling &g) {
-    p += (s.first + s.row) * stride + s.c0 + s.lane * PACK;
+template <int PACK>
+__device__ __forceinline__ void result(Array<PACK> &e, const Affine<PACK> &f, int act) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i < s.mine) {
-            float e[PACK];
-            unpack(v[i], e);
-#pragma unroll
-            for (int k = 0; k < PACK; ++k) e[k] = activate(fmaf(e[k] - f.mean[k], f.scale[k], f.shift[k]), act);
-            *reinterpret_cast<Held<T, PACK> *>(p) = packed<T, PACK>(e);
-        }
-        p += g.rows_at_once * stride;
-    }
+    for (int k = 0; k < Values<PACK>::kCount; ++k) e[k] = vfma(vadd(e[k], f.less.v[k]), f.scale.v[k], f.shift.v[k]);
+    activate(e, act);
 }
 
 /* The tile's statistics and, where the whole sample's groups are in the
  * cluster, its result; else the statistics go to partial [samples, blocks,
  * parts, 2 block_groups]. */
 template <class T, int PACK, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, T *y, float *mean_out,
                    float *rstd_out, float *partial) {
     extern __shared__ __align__(16) float shared[];
-    constexpr int HELD = kHeld<T, PACK>;
     const Seat at = seat_of(d, g, blockIdx.x);
     const Sums s = sums_of(shared, d, g);
-    Held<T, PACK> v[HELD];
-    load_tile(v, x + at.n * d.xs, d.xp, at, g);
-    tile_statistics(v, s, at, d, g);
+    Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
+    const int step = g.rows_at_once * g.lanes;
+    load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
+    tile_loaded();
+    tile_statistics<T, PACK>(tile, step, s, at, d, g);
     if constexpr (!WHOLE) {
         for (int i = threadIdx.x; i < 2 * g.block_groups; i += blockDim.x)
             partial[static_cast<size_t>(blockIdx.x) * 2 * g.block_groups + i] = s.group[i];
@@ -267,29 +337,28 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
         float *merged = s.group + 2 * g.block_groups;
         cg::cluster_group cluster = cg::this_cluster();
         if (g.parts > 1) cluster.sync();
-        for (int i = threadIdx.x; i < g.block_groups; i += blockDim.x) {
+        for (int i = threadIdx.x; i < at.groups; i += blockDim.x) {
             float mean = s.group[2 * i], squares = s.group[2 * i + 1];
             const float total = static_cast<float>(d.positions) * static_cast<float>(d.per_group);
             if (g.parts > 1) { /* in the parts' order */
+                const auto rows = [&](int r) {
+                    return static_cast<float>(r + 1 < g.parts ? g.rows : static_cast<int>(d.positions) - r * g.rows);
+                };
                 float sum = 0.0f;
-                for (unsigned r = 0; r < g.parts; ++r) {
-                    const float rows = static_cast<float>(r + 1 < g.parts ? g.rows : d.positions - r * g.rows);
-                    sum += rows * cluster.map_shared_rank(s.group, r)[2 * i];
-                }
+                for (int r = 0; r < g.parts; ++r) sum += rows(r) * cluster.map_shared_rank(s.group, r)[2 * i];
                 mean = sum / static_cast<float>(d.positions);
                 squares = 0.0f;
-                for (unsigned r = 0; r < g.parts; ++r) {
-                    const float rows = static_cast<float>(r + 1 < g.parts ? g.rows : d.positions - r * g.rows);
+                for (int r = 0; r < g.parts; ++r) {
                     const float *other = cluster.map_shared_rank(s.group, r) + 2 * i;
                     const float off = other[0] - mean;
-                    squares += fmaf(rows * static_cast<float>(d.per_group) * off, off, other[1]);
+                    squares += fmaf(rows(r) * static_cast<float>(d.per_group) * off, off, other[1]);
                 }
             }
             const float rstd = 1.0f / sqrtf(squares / total + d.epsilon);
             merged[2 * i] = mean;
             merged[2 * i + 1] = rstd;
             if (mean_out && at.part == 0) {
-                const size_t to = at.n * d.groups + at.block * g.block_groups + i;
+                const size_t to = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups + i;
                 mean_out[to] = mean;
                 rstd_out[to] = rstd;
             }
@@ -297,14 +366,21 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
         if (g.parts > 1) cluster.barrier_arrive(); /* no CTA leaves before the others have read */
         __syncthreads();
         Affine<PACK> f;
-#pragma unroll
-        for (int k = 0; k < PACK; ++k) {
-            const int c = at.lane * PACK + k, i = at.in ? c / d.per_group : 0;
-            f.mean[k] = merged[2 * i];
-            f.scale[k] = merged[2 * i + 1] * (gamma && at.in ? gamma[at.c0 + c] : 1.0f);
-            f.shift[k] = beta && at.in ? beta[at.c0 + c] : 0.0f;
+        f.less = channels_of<PACK>(at, [&](int c) { return -merged[2 * group_of(c, d, g)]; });
+        f.scale = channels_of<PACK>(at, [&](int c) {
+            return merged[2 * group_of(c, d, g) + 1] * (gamma ? gamma[at.c0 + c] : 1.0f);
+        });
+        f.shift = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
+        T *p = y + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
+        const size_t jump = g.rows_at_once * d.yp;
+#pragma unroll 2
+        for (int i = 0; i < at.mine; ++i) {
+            Array<PACK> e;
+            taken<T, PACK>(tile[i * step], e);
+            result<PACK>(e, f, d.act);
+            put<T, PACK>(p, e);
+            p += jump;
         }
-        write_tile(v, f, y + at.n * d.ys, d.yp, d.act, at, g);
         if (g.parts > 1) cluster.barrier_wait();
     }
 }
@@ -318,12 +394,14 @@ norm_merge(NormShape d, Tiling g, const float *partial, float *mean_out, float *
     const size_t n = at / d.groups, block = group / g.block_groups;
     const float *p = partial + (n * g.blocks + block) * g.parts * 2 * g.block_groups + 2 * (group % g.block_groups);
     const size_t pitch = 2 * g.block_groups;
-    const auto rows = [&](size_t r) { return static_cast<float>(r + 1 < g.parts ? g.rows : d.positions - r * g.rows); };
+    const auto rows = [&](int r) {
+        return static_cast<float>(r + 1 < g.parts ? g.rows : static_cast<int>(d.positions) - r * g.rows);
+    };
     float sum = 0.0f;
-    for (size_t r = lane; r < g.parts; r += 32) sum += rows(r) * p[r * pitch];
+    for (int r = lane; r < g.parts; r += 32) sum += rows(r) * p[r * pitch];
     const float mean = warp_sum(sum) / static_cast<float>(d.positions);
     float squares = 0.0f;
-    for (size_t r = lane; r < g.parts; r += 32) {
+    for (int r = lane; r < g.parts; r += 32) {
         const float off = p[r * pitch] - mean;
         squares += fmaf(rows(r) * static_cast<float>(d.per_group) * off, off, p[r * pitch + 1]);
     }
@@ -334,132 +412,160 @@ norm_merge(NormShape d, Tiling g, const float *partial, float *mean_out, float *
     }
 }
 
+/* Packs that a thread of the second read has under way. */
+constexpr int kAhead = 4;
+
 /* The result from given statistics. */
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                    const float *rstd, T *y) {
-    constexpr int HELD = kHeld<T, PACK>;
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
-    Held<T, PACK> v[HELD];
-    load_tile(v, x + at.n * d.xs, d.xp, at, g);
+    const T *from = x + at.n * d.xs + (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
+    T *to = y + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
+    const size_t from_jump = g.rows_at_once * d.xp, to_jump = g.rows_at_once * d.yp;
+    const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Affine<PACK> f;
+    f.less = channels_of<PACK>(at, [&](int c) { return -mean[first + group_of(c, d, g)]; });
+    f.scale = channels_of<PACK>(at, [&](int c) {
+        return rstd[first + group_of(c, d, g)] * (gamma ? gamma[at.c0 + c] : 1.0f);
+    });
+    f.shift = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
+    for (int i = 0; i < at.mine; i += kAhead) {
+        Held<T, PACK> v[kAhead];
 #pragma unroll
-    for (int k = 0; k < PACK; ++k) {
-        const int c = at.c0 + (at.in ? at.lane * PACK + k : 0);
-        const size_t i = at.n * d.groups + c / d.per_group;
-        f.mean[k] = mean[i];
-        f.scale[k] = rstd[i] * (gamma ? gamma[c] : 1.0f);
-        f.shift[k] = beta ? beta[c] : 0.0f;
+        for (int j = 0; j < kAhead; ++j)
+            if (i + j < at.mine) v[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * from_jump);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (i + j < at.mine) {
+                Array<PACK> e;
+                taken<T, PACK>(v[j], e);
+                result<PACK>(e, f, d.act);
+                put<T, PACK>(to + j * to_jump, e);
+            }
+        from += kAhead * from_jump;
+        to += kAhead * to_jump;
     }
-    write_tile(v, f, y + at.n * d.ys, d.yp, d.act, at, g);
 }
 
 /* ---- backward ---- */
 
-/* hat = (x - mean) rstd, u = hat gamma + beta. */
+/* z = x - mean, u = z scale + beta with scale = rstd gamma. */
 template <int PACK> struct Given {
-    float mean[PACK], rstd[PACK], gamma[PACK], beta[PACK];
+    Channels<PACK> less, scale, beta; /* less = -mean */
 };
 template <int PACK>
-__device__ __forceinline__ Given<PACK> given_of(const NormShape &d, const Seat &at, const float *gamma, const float *beta,
-                                                const float *mean, const float *rstd) {
+__device__ __forceinline__ Given<PACK> given_of(const NormShape &d, const Tiling &g, const Seat &at, const float *gamma,
+                                                const float *beta, const float *mean, const float *rstd) {
+    const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Given<PACK> f;
-#pragma unroll
-    for (int k = 0; k < PACK; ++k) {
-        const int c = at.c0 + (at.in ? at.lane * PACK + k : 0);
-        const size_t i = at.n * d.groups + c / d.per_group;
-        f.mean[k] = mean[i];
-        f.rstd[k] = rstd[i];
-        f.gamma[k] = gamma ? gamma[c] : 1.0f;
-        f.beta[k] = beta ? beta[c] : 0.0f;
-    }
+    f.less = channels_of<PACK>(at, [&](int c) { return -mean[first + group_of(c, d, g)]; });
+    f.scale = channels_of<PACK>(at, [&](int c) {
+        return rstd[first + group_of(c, d, g)] * (gamma ? gamma[at.c0 + c] : 1.0f);
+    });
+    f.beta = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
     return f;
 }
-
-/* Leaves per channel the sums of du in s.channel, of du hat behind them, and per
- * group those of du gamma and du gamma hat in s.group; visible to all. */
-template <class T, int PACK, int HELD>
-__device__ __forceinline__ void tile_gradients(const Held<T, PACK> (&v)[HELD], const Held<T, PACK> (&w)[HELD],
-                                               const Given<PACK> &f, const float *gamma, const Sums &s, const Seat &at,
-                                               const NormShape &d, const Tiling &g) {
-    float a[PACK], b[PACK];
+/* x becomes z, dy becomes du = dy act'(u). */
+template <int PACK>
+__device__ __forceinline__ void gradients(Array<PACK> &x, Array<PACK> &dy, const Given<PACK> &f, int act) {
+    Array<PACK> u;
 #pragma unroll
-    for (int k = 0; k < PACK; ++k) a[k] = b[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i)
-        if (i < at.mine) {
-            float e[PACK], dy[PACK];
-            unpack(v[i], e);
-            unpack(w[i], dy);
-#pragma unroll
-            for (int k = 0; k < PACK; ++k) {
-                const float hat = (e[k] - f.mean[k]) * f.rstd[k];
-                const float du = dy[k] * slope(fmaf(hat, f.gamma[k], f.beta[k]), d.act);
-                a[k] += du;
-                b[k] = fmaf(du, hat, b[k]);
-            }
-        }
-    float *const second = s.channel + ((g.lanes * PACK + 3) & ~3);
-    channel_totals<PACK>(a, s.channel, s, at, g);
-    channel_totals<PACK>(b, second, s, at, g);
-    const auto weighted = [&](const float *t) { return [=](int c) { return t[c] * (gamma ? gamma[at.c0 + c] : 1.0f); }; };
-    group_totals(d, g, weighted(s.channel), [&](int i, float t) { s.group[2 * i] = t; });
-    group_totals(d, g, weighted(second), [&](int i, float t) { s.group[2 * i + 1] = t; });
-    __syncthreads();
-}
-
-/* dx = rstd (du gamma - m1 - hat m2); m1, m2: the group's means of du gamma, du gamma hat. */
-template <class T, int PACK, int HELD>
-__device__ __forceinline__ void write_gradients(const Held<T, PACK> (&v)[HELD], const Held<T, PACK> (&w)[HELD],
-                                                const Given<PACK> &f, const float (&m1)[PACK], const float (&m2)[PACK], T *p,
-                                                const NormShape &d, const Seat &s, const Tiling &g) {
-    p += (s.first + s.row) * d.xp + s.c0 + s.lane * PACK;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i < s.mine) {
-            float e[PACK], dy[PACK];
-            unpack(v[i], e);
-            unpack(w[i], dy);
-#pragma unroll
-            for (int k = 0; k < PACK; ++k) {
-                const float hat = (e[k] - f.mean[k]) * f.rstd[k];
-                const float du = dy[k] * slope(fmaf(hat, f.gamma[k], f.beta[k]), d.act);
-                e[k] = f.rstd[k] * (fmaf(du, f.gamma[k], -m1[k]) - hat * m2[k]);
-            }
-            *reinterpret_cast<Held<T, PACK> *>(p) = packed<T, PACK>(e);
-        }
-        p += g.rows_at_once * d.xp;
+    for (int k = 0; k < Values<PACK>::kCount; ++k) {
+        x[k] = vadd(x[k], f.less.v[k]);
+        u[k] = vfma(x[k], f.scale.v[k], f.beta.v[k]);
     }
+    slopes(u, act);
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) dy[k] = vmul(dy[k], u[k]);
+}
+/* With hat = z rstd and m1, m2 the group's means of du gamma and du gamma hat:
+ * dx = rstd (du gamma - m1 - hat m2) = du scale + n1 + z n2. */
+template <int PACK> struct Less {
+    Channels<PACK> n1, n2; /* -rstd m1, -rstd^2 m2 */
+};
+template <int PACK>
+__device__ __forceinline__ Less<PACK> less_of(const NormShape &d, const Tiling &g, const Seat &at, const float *rstd,
+                                              const float *means) {
+    const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
+    Less<PACK> f;
+    f.n1 = channels_of<PACK>(at, [&](int c) {
+        const int i = group_of(c, d, g);
+        return -rstd[first + i] * means[2 * i];
+    });
+    f.n2 = channels_of<PACK>(at, [&](int c) {
+        const int i = group_of(c, d, g);
+        return -rstd[first + i] * rstd[first + i] * means[2 * i + 1];
+    });
+    return f;
+}
+template <int PACK>
+__device__ __forceinline__ void input_gradient(Array<PACK> &z, const Array<PACK> &du, const Given<PACK> &f,
+                                               const Less<PACK> &l) {
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k)
+        z[k] = vfma(du[k], f.scale.v[k], vfma(z[k], l.n2.v[k], l.n1.v[k]));
 }
 
 /* The tile's sums and, where the whole sample's groups are in the cluster, dx.
  * Per-channel sums go to partial [samples, parts, 2, channels], and where the
  * sample is larger the groups' to sums [samples, parts, 2, groups]. */
 template <class T, int PACK, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
 norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const T *dy, T *dx, float *partial, float *sums) {
+    using V = typename Values<PACK>::V;
+    constexpr int N = Values<PACK>::kCount;
     extern __shared__ __align__(16) float shared[];
-    constexpr int HELD = kHeld<T, PACK>;
     const Seat at = seat_of(d, g, blockIdx.x);
     const Sums s = sums_of(shared, d, g);
-    Held<T, PACK> v[HELD], w[HELD];
-    load_tile(v, x + at.n * d.xs, d.xp, at, g);
-    load_tile(w, dy + at.n * d.ys, d.yp, at, g);
-    const Given<PACK> f = given_of<PACK>(d, at, gamma, beta, mean, rstd);
-    tile_gradients(v, w, f, gamma, s, at, d, g);
-    const int channels = g.lanes * PACK, second = (channels + 3) & ~3;
+    const int step = g.rows_at_once * g.lanes;
+    Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
+    Held<T, PACK> *const tile_dy = tile + g.rows_held * g.lanes;
+    load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
+    load_tile<T, PACK>(tile_dy, step, dy + at.n * d.ys, d.yp, at, g);
+    const Given<PACK> f = given_of<PACK>(d, g, at, gamma, beta, mean, rstd);
+    tile_loaded();
+    {
+        Array<PACK> a, b;
+#pragma unroll
+        for (int k = 0; k < N; ++k) a[k] = b[k] = vall<V>(0.0f);
+#pragma unroll 2
+        for (int i = 0; i < at.mine; ++i) {
+            Array<PACK> z, du;
+            taken<T, PACK>(tile[i * step], z);
+            taken<T, PACK>(tile_dy[i * step], du);
+            gradients<PACK>(z, du, f, d.act);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                a[k] = vadd(a[k], du[k]);
+                b[k] = vfma(du[k], z[k], b[k]);
+            }
+        }
+        float *const second = s.channel + ((g.lanes * PACK + 3) & ~3);
+        const float *r = rstd + static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
+        const Channels<PACK> scale = channels_of<PACK>(at, [&](int c) { return r[group_of(c, d, g)]; });
+#pragma unroll
+        for (int k = 0; k < N; ++k) b[k] = vmul(b[k], scale.v[k]); /* of du z: of du hat */
+        channel_totals<PACK>(a, s.channel, s, at, g);
+        channel_totals<PACK>(b, second, s, at, g);
+        const auto weighted = [&](const float *t) { return [=](int c) { return t[c] * (gamma ? gamma[at.c0 + c] : 1.0f); }; };
+        group_totals(d, at, weighted(s.channel), [&](int i, float t) { s.group[2 * i] = t; });
+        group_totals(d, at, weighted(second), [&](int i, float t) { s.group[2 * i + 1] = t; });
+        __syncthreads();
+    }
+    const int second = (g.lanes * PACK + 3) & ~3;
     if (partial) {
-        float *to = partial + (at.n * g.parts + at.part) * 2 * d.channels + at.c0;
-        for (int c = threadIdx.x; c < channels; c += blockDim.x) {
+        float *to = partial + (static_cast<size_t>(at.n) * g.parts + at.part) * 2 * d.channels + at.c0;
+        for (int c = threadIdx.x; c < at.channels; c += blockDim.x) {
             to[c] = s.channel[c];
             to[d.channels + c] = s.channel[second + c];
         }
     }
     if constexpr (!WHOLE) {
-        float *to = sums + (at.n * g.parts + at.part) * 2 * d.groups + at.block * g.block_groups;
-        for (int i = threadIdx.x; i < g.block_groups; i += blockDim.x) {
+        float *to = sums + (static_cast<size_t>(at.n) * g.parts + at.part) * 2 * d.groups + at.block * g.block_groups;
+        for (int i = threadIdx.x; i < at.groups; i += blockDim.x) {
             to[i] = s.group[2 * i];
             to[d.groups + i] = s.group[2 * i + 1];
         }
@@ -468,22 +574,26 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
         cg::cluster_group cluster = cg::this_cluster();
         if (g.parts > 1) cluster.sync();
         const float count = static_cast<float>(d.positions) * static_cast<float>(d.per_group);
-        for (int i = threadIdx.x; i < 2 * g.block_groups; i += blockDim.x) {
+        for (int i = threadIdx.x; i < 2 * at.groups; i += blockDim.x) {
             float t = 0.0f;
-            for (unsigned r = 0; r < g.parts; ++r)
-                t += g.parts > 1 ? cluster.map_shared_rank(s.group, r)[i] : s.group[i];
+            for (int r = 0; r < g.parts; ++r) t += g.parts > 1 ? cluster.map_shared_rank(s.group, r)[i] : s.group[i];
             merged[i] = t / count;
         }
         if (g.parts > 1) cluster.barrier_arrive(); /* no CTA leaves before the others have read */
         __syncthreads();
-        float m1[PACK], m2[PACK];
-#pragma unroll
-        for (int k = 0; k < PACK; ++k) {
-            const int i = at.in ? (at.lane * PACK + k) / d.per_group : 0;
-            m1[k] = merged[2 * i];
-            m2[k] = merged[2 * i + 1];
+        const Less<PACK> l = less_of<PACK>(d, g, at, rstd, merged);
+        T *p = dx + at.n * d.xs + (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
+        const size_t jump = g.rows_at_once * d.xp;
+#pragma unroll 2
+        for (int i = 0; i < at.mine; ++i) {
+            Array<PACK> z, du;
+            taken<T, PACK>(tile[i * step], z);
+            taken<T, PACK>(tile_dy[i * step], du);
+            gradients<PACK>(z, du, f, d.act);
+            input_gradient<PACK>(z, du, f, l);
+            put<T, PACK>(p, z);
+            p += jump;
         }
-        write_gradients(v, w, f, m1, m2, dx + at.n * d.xs, d, at, g);
         if (g.parts > 1) cluster.barrier_wait();
     }
 }
@@ -511,23 +621,41 @@ norm_merge_sums(NormShape d, size_t parts, const float *sums, float *means) {
 }
 
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
 norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const float *means, const T *dy, T *dx) {
-    constexpr int HELD = kHeld<T, PACK>;
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
-    Held<T, PACK> v[HELD], w[HELD];
-    load_tile(v, x + at.n * d.xs, d.xp, at, g);
-    load_tile(w, dy + at.n * d.ys, d.yp, at, g);
-    const Given<PACK> f = given_of<PACK>(d, at, gamma, beta, mean, rstd);
-    float m1[PACK], m2[PACK];
+    const size_t corner = (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
+    const T *from = x + at.n * d.xs + corner;
+    const T *from_dy = dy + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
+    T *to = dx + at.n * d.xs + corner;
+    const size_t jump = g.rows_at_once * d.xp, dy_jump = g.rows_at_once * d.yp;
+    const Given<PACK> f = given_of<PACK>(d, g, at, gamma, beta, mean, rstd);
+    const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
+    const Less<PACK> l = less_of<PACK>(d, g, at, rstd, means + 2 * first);
+    constexpr int kPairs = kAhead / 2;
+    for (int i = 0; i < at.mine; i += kPairs) {
+        Held<T, PACK> v[kPairs], w[kPairs];
 #pragma unroll
-    for (int k = 0; k < PACK; ++k) {
-        const size_t i = at.n * d.groups + (at.c0 + (at.in ? at.lane * PACK + k : 0)) / d.per_group;
-        m1[k] = means[2 * i];
-        m2[k] = means[2 * i + 1];
+        for (int j = 0; j < kPairs; ++j)
+            if (i + j < at.mine) {
+                v[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * jump);
+                w[j] = *reinterpret_cast<const Held<T, PACK> *>(from_dy + j * dy_jump);
+            }
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j)
+            if (i + j < at.mine) {
+                Array<PACK> z, du;
+                taken<T, PACK>(v[j], z);
+                taken<T, PACK>(w[j], du);
+                gradients<PACK>(z, du, f, d.act);
+                input_gradient<PACK>(z, du, f, l);
+                put<T, PACK>(to + j * jump, z);
+            }
+        from += kPairs * jump;
+        from_dy += kPairs * dy_jump;
+        to += kPairs * jump;
     }
-    write_gradients(v, w, f, m1, m2, dx + at.n * d.xs, d, at, g);
 }
 
 /* dbeta and dgamma from parts [rows, 2, channels]. */
@@ -585,7 +713,9 @@ norm_forward_wide(NormShape d, const T *x, const float *gamma, const float *beta
         for (int c = threadIdx.x; c < d.per_group; c += kThreads) {
             const float scale = rstd * (gamma ? gamma[c0 + c] : 1.0f);
             const float u = fmaf(to_float(xs[p * d.xp + c]) - mean, scale, beta ? beta[c0 + c] : 0.0f);
-            y[n * d.ys + p * d.yp + c0 + c] = from_float<T>(activate(u, d.act));
+            float v[1] = {u};
+            activate(v, d.act);
+            y[n * d.ys + p * d.yp + c0 + c] = from_float<T>(v[0]);
         }
 }
 
@@ -602,7 +732,9 @@ norm_backward_wide(NormShape d, const T *x, const float *gamma, const float *bet
     float s1 = 0.0f, s2 = 0.0f;
     const auto gradient = [&](size_t p, int c, float ga, float be, float *hat) {
         *hat = (to_float(x[n * d.xs + p * d.xp + c]) - mean) * rstd;
-        return to_float(dy[n * d.ys + p * d.yp + c]) * slope(fmaf(*hat, ga, be), d.act);
+        float v[1] = {fmaf(*hat, ga, be)};
+        slopes(v, d.act);
+        return to_float(dy[n * d.ys + p * d.yp + c]) * v[0];
     };
     for (int c = c0 + threadIdx.x; c < c0 + d.per_group; c += kThreads) {
         const float ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f;
@@ -656,37 +788,51 @@ bool norm_shape(const tb_group_norm_desc *d, NormShape *s) {
     return true;
 }
 
+/* Bytes of a tile of one tensor: six such CTAs (backward: three) share an SM;
+ * the large size is for maps that fit a cluster by it. */
+constexpr size_t kTile = 32768, kLargeTile = 92160;
+
 /* Tiles for packs of `pack` elements; false where a group is wider than a
  * CTA's rows (or the tiles are too many to count). */
 bool tiling_of(const NormShape &d, int pack, size_t size, Tiling *g) {
-    const int held = pack * size == 16 ? 8 : 32;
     /* whole groups, whole packs, 128 bytes a row if there are: narrower rows
      * waste sectors, wider ones leave fewer and longer tiles */
-    int best = 0;
-    for (int i = 1; i <= d.groups && !best; ++i) {
-        if (d.groups % i || static_cast<size_t>(i) * d.per_group % pack) continue;
+    bool found = false;
+    for (int i = 1; i <= d.groups && !found; ++i) {
+        if (static_cast<size_t>(i) * d.per_group % pack) continue;
         const size_t lanes = static_cast<size_t>(i) * d.per_group / pack;
         if (lanes > kThreads) break;
         g->block_groups = i;
         g->lanes = static_cast<int>(lanes);
-        if (lanes * pack * size >= 128) best = i;
-        else if (i == d.groups) best = i;
-        else continue;
+        found = lanes * pack * size >= 128 || i == d.groups;
     }
-    if (!best) return false;
+    if (!found || d.positions > 0x3fffffffu) return false;
     g->pack = pack;
-    g->blocks = d.groups / g->block_groups;
+    g->blocks = (d.groups + g->block_groups - 1) / g->block_groups;
     const size_t packs = d.positions * g->lanes;
     const size_t threads = packs < kThreads ? align_up(packs, 32) : kThreads;
-    g->threads = static_cast<int>(threads < static_cast<size_t>(g->lanes) ? align_up(g->lanes, 32) : threads);
+    g->threads = static_cast<int>(threads);
     g->rows_at_once = g->threads / g->lanes;
-    const size_t most = static_cast<size_t>(g->rows_at_once) * held;
-    g->parts = (d.positions + most - 1) / most;
-    g->rows = (d.positions + g->parts - 1) / g->parts;
-    g->parts = (d.positions + g->rows - 1) / g->rows;
-    g->fits = g->parts <= kCluster;
-    size_t tiles;
-    return product(d.samples * g->blocks, g->parts, 0x7fffffffu, &tiles);
+    for (const size_t bytes : {kTile, kLargeTile, kTile}) {
+        const size_t turns = bytes / (static_cast<size_t>(g->rows_at_once) * g->lanes * pack * size);
+        const size_t most = static_cast<size_t>(g->rows_at_once) * (turns ? turns : 1);
+        const size_t parts = (d.positions + most - 1) / most;
+        const size_t rows = align_up((d.positions + parts - 1) / parts, g->rows_at_once);
+        if (product(d.samples * g->blocks, parts, 0x7fffffffu, &g->tiles) == false) return false;
+        g->rows = static_cast<int>(rows);
+        g->rows_held = static_cast<int>(rows);
+        g->parts = static_cast<int>((d.positions + rows - 1) / rows);
+        g->fits = g->parts <= kCluster;
+        if (g->fits) break;
+    }
+    g->tiles = d.samples * g->blocks * g->parts;
+    const auto magic = [](unsigned by) { return static_cast<unsigned>(0xffffffffull / by); };
+    g->magic_parts = magic(g->parts);
+    g->magic_blocks = magic(g->blocks);
+    g->magic_lanes = magic(g->lanes);
+    g->magic_rows = magic(g->rows_at_once);
+    g->magic_group = magic(d.per_group);
+    return true;
 }
 
 /* The widest pack that every row allows: 16 bytes, 4 bytes, an element. */
@@ -707,8 +853,11 @@ template <class T, class F> int with_pack(int pack, F &&f) {
 
 template <class Kernel, class... Args>
 int launch_tiles(Kernel kernel, const NormShape &d, const Tiling &g, bool clusters, size_t shared, cudaStream_t st, Args... args) {
+    if (shared > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
+        return 0;
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3(static_cast<unsigned>(d.samples * g.blocks * g.parts));
+    c.gridDim = dim3(static_cast<unsigned>(g.tiles));
     c.blockDim = dim3(static_cast<unsigned>(g.threads));
     c.dynamicSmemBytes = shared;
     c.stream = st;
@@ -725,7 +874,7 @@ int launch_tiles(Kernel kernel, const NormShape &d, const Tiling &g, bool cluste
 /* Workspace: the forward pass's partial statistics, or the backward pass's
  * per-channel rows with their column sums, group sums and means. */
 size_t forward_bytes(const NormShape &d, const Tiling &g) {
-    return (2 * d.samples * d.groups + d.samples * g.parts * 2 * d.groups) * sizeof(float);
+    return (2 * d.samples * d.groups + g.tiles * 2 * g.block_groups) * sizeof(float);
 }
 size_t backward_bytes(const NormShape &d, size_t parts) {
     const size_t rows = d.samples * parts;
@@ -779,11 +928,11 @@ extern "C" int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const v
         return with_pack<T>(pack, [&](auto p) {
             constexpr int P = decltype(p)::value;
             if (g.fits)
-                return launch_tiles(norm_forward_tiles<T, P, true>, s, g, true, sums_bytes(g), st, in, gamma, beta, out, mean,
+                return launch_tiles(norm_forward_tiles<T, P, true>, s, g, true, shared_bytes(g, size, 1), st, in, gamma, beta, out, mean,
                                     rstd, static_cast<float *>(nullptr));
             float *means = static_cast<float *>(workspace), *partial = means + 2 * s.samples * s.groups;
             float *m = mean ? mean : means, *r = rstd ? rstd : means + s.samples * s.groups;
-            if (!launch_tiles(norm_forward_tiles<T, P, false>, s, g, false, sums_bytes(g), st, in, gamma, beta, out, m, r, partial))
+            if (!launch_tiles(norm_forward_tiles<T, P, false>, s, g, false, shared_bytes(g, size, 1), st, in, gamma, beta, out, m, r, partial))
                 return 0;
             norm_merge<<<merge_grid(s), kThreads, 0, st>>>(s, g, partial, m, r);
             if (!launched()) return 0;
@@ -825,10 +974,10 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
             const int ok = with_pack<T>(pack, [&](auto p) {
                 constexpr int P = decltype(p)::value;
                 if (g.fits)
-                    return launch_tiles(norm_backward_tiles<T, P, true>, s, g, true, sums_bytes(g), st, in, gamma, beta, mean,
+                    return launch_tiles(norm_backward_tiles<T, P, true>, s, g, true, shared_bytes(g, size, 2), st, in, gamma, beta, mean,
                                         rstd, grad, out, rows_to, sums);
                 float *means = sums + rows * 2 * s.groups;
-                if (!launch_tiles(norm_backward_tiles<T, P, false>, s, g, false, sums_bytes(g), st, in, gamma, beta, mean, rstd,
+                if (!launch_tiles(norm_backward_tiles<T, P, false>, s, g, false, shared_bytes(g, size, 2), st, in, gamma, beta, mean, rstd,
                                   grad, out, rows_to, sums))
                     return 0;
                 norm_merge_sums<<<merge_grid(s), kThreads, 0, st>>>(s, g.parts, sums, means);

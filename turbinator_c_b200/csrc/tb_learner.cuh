@@ -160,6 +160,38 @@ __device__ __forceinline__ F2 sigmoid2(F2 v) {
     return pair(fast_rcp(a), fast_rcp(b));
 }
 
+/* The same operations on one value and on a pair, for code that takes either. */
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ F2 vadd(F2 a, F2 b) { return add2(a, b); }
+__device__ __forceinline__ F2 vmul(F2 a, F2 b) { return mul2(a, b); }
+__device__ __forceinline__ F2 vfma(F2 a, F2 b, F2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float vsigmoid(float v) { return fast_sigmoid(v); }
+__device__ __forceinline__ F2 vsigmoid(F2 v) { return sigmoid2(v); }
+template <class V> __device__ __forceinline__ V vall(float v);
+template <> __device__ __forceinline__ float vall<float>(float v) { return v; }
+template <> __device__ __forceinline__ F2 vall<F2>(float v) { return both(v); }
+/* f of each value. */
+template <class F> __device__ __forceinline__ float veach(float v, F &&f) { return f(v); }
+template <class F> __device__ __forceinline__ F2 veach(F2 v, F &&f) {
+    float a, b;
+    split(v, a, b);
+    return pair(f(a), f(b));
+}
+/* N values as pairs, or the one value. */
+template <int N> struct Values {
+    using V = std::conditional_t<N == 1, float, F2>;
+    static constexpr int kCount = N == 1 ? 1 : N / 2;
+};
+template <int N> using Array = typename Values<N>::V[Values<N>::kCount];
+template <class V> __device__ __forceinline__ V vload(const float *f) {
+    if constexpr (std::is_same<V, F2>::value) return pair(f[0], f[1]);
+    else return f[0];
+}
+__device__ __forceinline__ void vstore(float *f, float v) { f[0] = v; }
+__device__ __forceinline__ void vstore(float *f, F2 v) { split(v, f[0], f[1]); }
+
 /* ---- sums over the rows of partial [rows, columns] in f32 ---- */
 
 constexpr int kColumnThreads = 512;       /* 32 columns x 16 rows at a time */
