@@ -899,26 +899,16 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
     return all % 16 == 0 ? 16 : all % 4 == 0 && least == 4 ? 4 : 0;
 }
 
-/* Launches the strips' maps, where there are strips, and the scan. */
-template <class Kernel, class Args>
-int launch_scan(Kernel maps, Kernel scan, const Args &args, const Split &s, int warps, size_t shared, cudaStream_t st) {
-    int dev = 0, sms = 0, per_sm = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
-    const Kernel kernels[2] = {maps, scan};
-    const unsigned work[2] = {s.tiles * (s.strips - 1), s.tiles * s.strips};
-    for (int i = 0; i < 2; ++i) {
-        if (work[i] == 0) continue;
-        if (cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) !=
-                cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernels[i], warps * 32, shared) != cudaSuccess)
-            return 0;
-        const unsigned most = static_cast<unsigned>(sms * per_sm);
-        kernels[i]<<<work[i] < most ? work[i] : most, warps * 32, shared, st>>>(args, s);
-        if (!launched()) return 0;
-    }
-    return 1;
+/* Launches a kernel over `work` units: at most as many CTAs as its registers
+ * (16 warps an SM) leave room for, each taking every grid-th unit. */
+template <auto Kernel, class Args>
+int launch_units(unsigned work, const Args &args, const Split &s, int warps, size_t shared, cudaStream_t st) {
+    int dev = 0;
+    const int sms = multiprocessors(&dev);
+    if (!sms || !allow_shared<Kernel>(shared)) return 0;
+    const unsigned most = static_cast<unsigned>(sms) * (16 / warps);
+    Kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args, s);
+    return launched();
 }
 
 } /* namespace */
@@ -959,8 +949,11 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     const size_t shared = static_cast<size_t>(warps) * 2 * 3 * kSteps * tile * size;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return launch_scan(recurrence_forward_maps<T>, recurrence_forward<T>, p, split, warps, shared,
-                           static_cast<cudaStream_t>(stream));
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (split.strips > 1 &&
+            !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), p, split, warps, shared, st))
+            return 0;
+        return launch_units<recurrence_forward<T>>(split.tiles * split.strips, p, split, warps, shared, st);
     });
 }
 
@@ -1002,7 +995,10 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return launch_scan(recurrence_backward_maps<T>, recurrence_backward<T>, p, split, warps, shared, st);
+        if (split.strips > 1 &&
+            !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), p, split, warps, shared, st))
+            return 0;
+        return launch_units<recurrence_backward<T>>(split.tiles * split.strips, p, split, warps, shared, st);
     });
     if (!ok || !ddecay) return ok;
     const size_t rows = partial_rows(s, split), parts = column_parts(rows);

@@ -28,7 +28,7 @@ using namespace tb_learn;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kCluster = 8; /* CTAs of a cluster at most */
 
 struct NormShape {
@@ -171,6 +171,28 @@ __device__ __forceinline__ int group_of(int channel, const NormShape &d, const T
     return static_cast<int>(divided(channel, d.per_group, g.magic_group));
 }
 
+/* The same for f(group of the tile): once where packs do not cross groups. */
+template <int PACK, class F>
+__device__ __forceinline__ Channels<PACK> by_group(const Seat &s, const NormShape &d, const Tiling &g, F &&f) {
+    using V = typename Values<PACK>::V;
+    if (d.per_group % PACK) return channels_of<PACK>(s, [&](int c) { return f(group_of(c, d, g)); });
+    const V v = vall<V>(f(s.in ? group_of(s.lane * PACK, d, g) : 0));
+    Channels<PACK> r;
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) r.v[k] = v;
+    return r;
+}
+template <int PACK> __device__ __forceinline__ Channels<PACK> times(const Channels<PACK> &a, const Channels<PACK> &b) {
+    Channels<PACK> r;
+#pragma unroll
+    for (int k = 0; k < Values<PACK>::kCount; ++k) r.v[k] = vmul(a.v[k], b.v[k]);
+    return r;
+}
+/* Parameters of the thread's channels, or `other` where there are none. */
+template <int PACK> __device__ __forceinline__ Channels<PACK> parameters_of(const Seat &s, const float *p, float other) {
+    return channels_of<PACK>(s, [&](int c) { return p ? p[s.c0 + c] : other; });
+}
+
 template <class T, int PACK>
 __device__ __forceinline__ void taken(const Held<T, PACK> &h, Array<PACK> &v) {
     float e[PACK];
@@ -287,7 +309,7 @@ __device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int s
     const float count = static_cast<float>(at.rows) * static_cast<float>(d.per_group);
     group_totals(d, at, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i] = t / count; });
     __syncthreads();
-    const Channels<PACK> less = channels_of<PACK>(at, [&](int c) { return -s.group[2 * group_of(c, d, g)]; });
+    const Channels<PACK> less = by_group<PACK>(at, d, g, [&](int i) { return -s.group[2 * i]; });
 #pragma unroll
     for (int k = 0; k < N; ++k) own[k] = vall<V>(0.0f);
 #pragma unroll 4
@@ -319,7 +341,7 @@ __device__ __forceinline__ void result(Array<PACK> &e, const Affine<PACK> &f, in
  * cluster, its result; else the statistics go to partial [samples, blocks,
  * parts, 2 block_groups]. */
 template <class T, int PACK, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, 6)
 norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, T *y, float *mean_out,
                    float *rstd_out, float *partial) {
     extern __shared__ __align__(16) float shared[];
@@ -366,11 +388,10 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
         if (g.parts > 1) cluster.barrier_arrive(); /* no CTA leaves before the others have read */
         __syncthreads();
         Affine<PACK> f;
-        f.less = channels_of<PACK>(at, [&](int c) { return -merged[2 * group_of(c, d, g)]; });
-        f.scale = channels_of<PACK>(at, [&](int c) {
-            return merged[2 * group_of(c, d, g) + 1] * (gamma ? gamma[at.c0 + c] : 1.0f);
-        });
-        f.shift = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
+        f.less = by_group<PACK>(at, d, g, [&](int i) { return -merged[2 * i]; });
+        f.scale = times<PACK>(by_group<PACK>(at, d, g, [&](int i) { return merged[2 * i + 1]; }),
+                              parameters_of<PACK>(at, gamma, 1.0f));
+        f.shift = parameters_of<PACK>(at, beta, 0.0f);
         T *p = y + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
         const size_t jump = g.rows_at_once * d.yp;
 #pragma unroll 2
@@ -417,7 +438,7 @@ constexpr int kAhead = 4;
 
 /* The result from given statistics. */
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, 8)
 norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                    const float *rstd, T *y) {
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
@@ -426,11 +447,10 @@ norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const 
     const size_t from_jump = g.rows_at_once * d.xp, to_jump = g.rows_at_once * d.yp;
     const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Affine<PACK> f;
-    f.less = channels_of<PACK>(at, [&](int c) { return -mean[first + group_of(c, d, g)]; });
-    f.scale = channels_of<PACK>(at, [&](int c) {
-        return rstd[first + group_of(c, d, g)] * (gamma ? gamma[at.c0 + c] : 1.0f);
-    });
-    f.shift = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
+    f.less = by_group<PACK>(at, d, g, [&](int i) { return -mean[first + i]; });
+    f.scale = times<PACK>(by_group<PACK>(at, d, g, [&](int i) { return rstd[first + i]; }),
+                          parameters_of<PACK>(at, gamma, 1.0f));
+    f.shift = parameters_of<PACK>(at, beta, 0.0f);
     for (int i = 0; i < at.mine; i += kAhead) {
         Held<T, PACK> v[kAhead];
 #pragma unroll
@@ -460,11 +480,10 @@ __device__ __forceinline__ Given<PACK> given_of(const NormShape &d, const Tiling
                                                 const float *beta, const float *mean, const float *rstd) {
     const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Given<PACK> f;
-    f.less = channels_of<PACK>(at, [&](int c) { return -mean[first + group_of(c, d, g)]; });
-    f.scale = channels_of<PACK>(at, [&](int c) {
-        return rstd[first + group_of(c, d, g)] * (gamma ? gamma[at.c0 + c] : 1.0f);
-    });
-    f.beta = channels_of<PACK>(at, [&](int c) { return beta ? beta[at.c0 + c] : 0.0f; });
+    f.less = by_group<PACK>(at, d, g, [&](int i) { return -mean[first + i]; });
+    f.scale = times<PACK>(by_group<PACK>(at, d, g, [&](int i) { return rstd[first + i]; }),
+                          parameters_of<PACK>(at, gamma, 1.0f));
+    f.beta = parameters_of<PACK>(at, beta, 0.0f);
     return f;
 }
 /* x becomes z, dy becomes du = dy act'(u). */
@@ -490,14 +509,8 @@ __device__ __forceinline__ Less<PACK> less_of(const NormShape &d, const Tiling &
                                               const float *means) {
     const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Less<PACK> f;
-    f.n1 = channels_of<PACK>(at, [&](int c) {
-        const int i = group_of(c, d, g);
-        return -rstd[first + i] * means[2 * i];
-    });
-    f.n2 = channels_of<PACK>(at, [&](int c) {
-        const int i = group_of(c, d, g);
-        return -rstd[first + i] * rstd[first + i] * means[2 * i + 1];
-    });
+    f.n1 = by_group<PACK>(at, d, g, [&](int i) { return -rstd[first + i] * means[2 * i]; });
+    f.n2 = by_group<PACK>(at, d, g, [&](int i) { return -rstd[first + i] * rstd[first + i] * means[2 * i + 1]; });
     return f;
 }
 template <int PACK>
@@ -545,7 +558,7 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
         }
         float *const second = s.channel + ((g.lanes * PACK + 3) & ~3);
         const float *r = rstd + static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
-        const Channels<PACK> scale = channels_of<PACK>(at, [&](int c) { return r[group_of(c, d, g)]; });
+        const Channels<PACK> scale = by_group<PACK>(at, d, g, [&](int i) { return r[i]; });
 #pragma unroll
         for (int k = 0; k < N; ++k) b[k] = vmul(b[k], scale.v[k]); /* of du z: of du hat */
         channel_totals<PACK>(a, s.channel, s, at, g);
@@ -621,7 +634,7 @@ norm_merge_sums(NormShape d, size_t parts, const float *sums, float *means) {
 }
 
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const float *means, const T *dy, T *dx) {
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
@@ -851,11 +864,9 @@ template <class T, class F> int with_pack(int pack, F &&f) {
     return f(std::integral_constant<int, 1>{});
 }
 
-template <class Kernel, class... Args>
-int launch_tiles(Kernel kernel, const NormShape &d, const Tiling &g, bool clusters, size_t shared, cudaStream_t st, Args... args) {
-    if (shared > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
-        return 0;
+template <auto Kernel, class... Args>
+int launch_tiles(const NormShape &d, const Tiling &g, bool clusters, size_t shared, cudaStream_t st, Args... args) {
+    if (!allow_shared<Kernel>(shared)) return 0;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(static_cast<unsigned>(g.tiles));
     c.blockDim = dim3(static_cast<unsigned>(g.threads));
@@ -868,7 +879,7 @@ int launch_tiles(Kernel kernel, const NormShape &d, const Tiling &g, bool cluste
         c.attrs = &a;
         c.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&c, kernel, d, g, args...) == cudaSuccess;
+    return cudaLaunchKernelEx(&c, Kernel, d, g, args...) == cudaSuccess;
 }
 
 /* Workspace: the forward pass's partial statistics, or the backward pass's
@@ -928,15 +939,15 @@ extern "C" int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const v
         return with_pack<T>(pack, [&](auto p) {
             constexpr int P = decltype(p)::value;
             if (g.fits)
-                return launch_tiles(norm_forward_tiles<T, P, true>, s, g, true, shared_bytes(g, size, 1), st, in, gamma, beta, out, mean,
+                return launch_tiles<norm_forward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 1), st, in, gamma, beta, out, mean,
                                     rstd, static_cast<float *>(nullptr));
             float *means = static_cast<float *>(workspace), *partial = means + 2 * s.samples * s.groups;
             float *m = mean ? mean : means, *r = rstd ? rstd : means + s.samples * s.groups;
-            if (!launch_tiles(norm_forward_tiles<T, P, false>, s, g, false, shared_bytes(g, size, 1), st, in, gamma, beta, out, m, r, partial))
+            if (!launch_tiles<norm_forward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 1), st, in, gamma, beta, out, m, r, partial))
                 return 0;
             norm_merge<<<merge_grid(s), kThreads, 0, st>>>(s, g, partial, m, r);
             if (!launched()) return 0;
-            return launch_tiles(norm_forward_apply<T, P>, s, g, false, 0, st, in, gamma, beta, m, r, out);
+            return launch_tiles<norm_forward_apply<T, P>>(s, g, false, 0, st, in, gamma, beta, m, r, out);
         });
     });
 }
@@ -974,15 +985,15 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
             const int ok = with_pack<T>(pack, [&](auto p) {
                 constexpr int P = decltype(p)::value;
                 if (g.fits)
-                    return launch_tiles(norm_backward_tiles<T, P, true>, s, g, true, shared_bytes(g, size, 2), st, in, gamma, beta, mean,
+                    return launch_tiles<norm_backward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 2), st, in, gamma, beta, mean,
                                         rstd, grad, out, rows_to, sums);
                 float *means = sums + rows * 2 * s.groups;
-                if (!launch_tiles(norm_backward_tiles<T, P, false>, s, g, false, shared_bytes(g, size, 2), st, in, gamma, beta, mean, rstd,
+                if (!launch_tiles<norm_backward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 2), st, in, gamma, beta, mean, rstd,
                                   grad, out, rows_to, sums))
                     return 0;
                 norm_merge_sums<<<merge_grid(s), kThreads, 0, st>>>(s, g.parts, sums, means);
                 if (!launched()) return 0;
-                return launch_tiles(norm_backward_apply<T, P>, s, g, false, 0, st, in, gamma, beta, mean, rstd, means, grad,
+                return launch_tiles<norm_backward_apply<T, P>>(s, g, false, 0, st, in, gamma, beta, mean, rstd, means, grad,
                                     out);
             });
             if (!ok) return 0;

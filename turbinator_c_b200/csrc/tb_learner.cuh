@@ -12,6 +12,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "turbinator/training/cuda_learner.h"
@@ -248,6 +249,33 @@ template <class F> inline int with_type(int type, F &&f) {
     if (type == TB_TYPE_F32) return f(float{});
     if (type == TB_TYPE_BF16) return f(__nv_bfloat16{});
     return f(__half{});
+}
+
+/* Multiprocessors of the current device, 0 if there is none; asked once per device. */
+constexpr int kMaxDevices = 64;
+inline int multiprocessors(int *device) {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+    *device = dev;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+        known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+/* Lets a kernel have `shared` bytes of dynamic shared memory; set once per
+ * kernel and device, and again only where more is asked for. */
+template <auto Kernel> bool allow_shared(size_t shared) {
+    static std::atomic<size_t> allowed[kMaxDevices];
+    if (shared <= 48 * 1024) return true;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    if (shared <= allowed[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
+        return false;
+    allowed[dev].store(shared, std::memory_order_relaxed);
+    return true;
 }
 
 inline int launched() { return cudaGetLastError() == cudaSuccess; }
