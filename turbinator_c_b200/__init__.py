@@ -133,10 +133,12 @@ def _ptr(x) -> Optional[int]:
     """Address of a torch tensor, numpy array, raw int or None."""
     if x is None:
         return None
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)!r}")

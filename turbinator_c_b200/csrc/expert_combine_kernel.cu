@@ -1,6 +1,13 @@
 /*
  * The experts' rows back to their tokens: weighted sum and its gradient
  * (include/turbinator/training/cuda_learner.h).
+ *
+ * Bound: HBM; every named row is read once and every token's row read or
+ * written once.  Rows move in packs of 16 bytes; the slots of a token are few
+ * and known from one load, so the loads of all its rows are under way together.
+ * The forward pass gives a team of up to 32 lanes a token and 32 packs of its
+ * width; the backward pass gives a token one to eight warps, whose parts of
+ * <dout, row> meet in shared memory, in order.
  */
 #include "tb_learner.cuh"
 
@@ -10,49 +17,136 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 4; /* rows of a token under way at once */
 
 struct CombineShape {
     size_t tokens, rows, width, rows_stride, out_stride;
     int top_k;
 };
 
-/* One warp per token. */
-template <class T>
+/* lanes: of a team, a power of two; chunks: of lanes packs each, of a row. */
+template <class T, int PACK>
 __global__ void __launch_bounds__(kThreads)
-combine_forward(CombineShape d, const T *rows, const int32_t *position, const float *weights, T *out) {
-    const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-    if (t >= d.tokens) return;
-    for (size_t c = threadIdx.x % 32; c < d.width; c += 32) {
-        float s = 0.0f;
-        for (int j = 0; j < d.top_k; ++j) {
-            const int32_t p = position[t * d.top_k + j];
-            if (p < 0 || static_cast<size_t>(p) >= d.rows) continue;
-            s += (weights ? weights[t * d.top_k + j] : 1.0f) * to_float(rows[p * d.rows_stride + c]);
+combine_forward(CombineShape d, int lanes, int chunks, const T *rows, const int32_t *position, const float *weights, T *out) {
+    using V = typename Values<PACK>::V;
+    constexpr int N = Values<PACK>::kCount;
+    const size_t team = (static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x) / lanes;
+    const int lane = threadIdx.x % lanes;
+    const size_t t = team / chunks, c = ((team - t * chunks) * lanes + lane) * PACK;
+    const bool there = t < d.tokens;
+    Array<PACK> sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = vall<V>(0.0f);
+    for (int first = 0; first < d.top_k; first += lanes) { /* a slot for each lane */
+        int32_t p = -1;
+        float w = 1.0f;
+        if (there && first + lane < d.top_k) {
+            p = position[t * d.top_k + first + lane];
+            if (p >= 0 && static_cast<size_t>(p) >= d.rows) p = -1;
+            if (weights) w = weights[t * d.top_k + first + lane];
         }
-        out[t * d.out_stride + c] = from_float<T>(s);
-    }
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-combine_backward(CombineShape d, const T *rows, const int32_t *position, const float *weights, const T *dout,
-                 T *drows, float *dweights) {
-    const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-    if (t >= d.tokens) return;
-    for (int j = 0; j < d.top_k; ++j) {
-        const int32_t p = position[t * d.top_k + j];
-        const bool there = p >= 0 && static_cast<size_t>(p) < d.rows;
-        float dot = 0.0f;
-        if (there) {
-            const float w = weights ? weights[t * d.top_k + j] : 1.0f;
-            for (size_t c = threadIdx.x % 32; c < d.width; c += 32) {
-                const float g = to_float(dout[t * d.out_stride + c]);
-                if (dweights) dot += g * to_float(rows[p * d.rows_stride + c]);
-                drows[p * d.rows_stride + c] = from_float<T>(w * g);
+        const int slots = min(d.top_k - first, lanes);
+        for (int j = 0; j < slots; j += kAhead) {
+            Held<T, PACK> v[kAhead];
+            int32_t row[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                row[k] = __shfl_sync(0xffffffffu, p, min(j + k, slots - 1), lanes);
+                if (j + k >= slots || c >= d.width) row[k] = -1;
+                if (row[k] >= 0) v[k] = *reinterpret_cast<const Held<T, PACK> *>(rows + row[k] * d.rows_stride + c);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const V s = vall<V>(__shfl_sync(0xffffffffu, w, min(j + k, slots - 1), lanes));
+                if (row[k] < 0) continue;
+                float e[PACK];
+                unpack(v[k], e);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] = vfma(s, vload<V>(e + 2 * i), sum[i]);
             }
         }
-        dot = warp_sum(dot);
-        if (dweights && threadIdx.x % 32 == 0) dweights[t * d.top_k + j] = dot;
+    }
+    if (!there || c >= d.width) return;
+    float e[PACK];
+#pragma unroll
+    for (int i = 0; i < N; ++i) vstore(e + 2 * i, sum[i]);
+    *reinterpret_cast<Held<T, PACK> *>(out + t * d.out_stride + c) = packed<T, PACK>(e);
+}
+
+/* `warps` (1, 2, 4 or 8) take a token, every warps-th chunk of 32 packs each. */
+template <class T, int PACK>
+__global__ void __launch_bounds__(kThreads)
+combine_backward(CombineShape d, int warps, const T *rows, const int32_t *position, const float *weights, const T *dout,
+                 T *drows, float *dweights) {
+    using V = typename Values<PACK>::V;
+    constexpr int N = Values<PACK>::kCount;
+    __shared__ float dots[kWarps][TB_ROUTE_MAX_TOP_K];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % warps;
+    const size_t t = static_cast<size_t>(blockIdx.x) * (kWarps / warps) + warp / warps;
+    int32_t p = -1;
+    float w = 1.0f;
+    if (t < d.tokens && lane < d.top_k) {
+        p = position[t * d.top_k + lane];
+        if (p >= 0 && static_cast<size_t>(p) >= d.rows) p = -1;
+        if (weights) w = weights[t * d.top_k + lane];
+    }
+    float total = 0.0f; /* of slot `lane` */
+    if (t < d.tokens)
+        for (size_t base = static_cast<size_t>(part) * 32 * PACK; base < d.width; base += static_cast<size_t>(warps) * 32 * PACK) {
+            const size_t c = base + lane * PACK;
+            const bool in = c < d.width;
+            Array<PACK> g;
+            {
+                float e[PACK];
+                Held<T, PACK> v{};
+                if (in) v = *reinterpret_cast<const Held<T, PACK> *>(dout + t * d.out_stride + c);
+                unpack(v, e);
+#pragma unroll
+                for (int i = 0; i < N; ++i) g[i] = vload<V>(e + 2 * i);
+            }
+            for (int j = 0; j < d.top_k; j += kAhead) {
+                Held<T, PACK> v[kAhead];
+                int32_t row[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    row[k] = __shfl_sync(0xffffffffu, p, min(j + k, d.top_k - 1));
+                    if (j + k >= d.top_k || !in) row[k] = -1;
+                    if (row[k] >= 0 && dweights)
+                        v[k] = *reinterpret_cast<const Held<T, PACK> *>(rows + row[k] * d.rows_stride + c);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const V s = vall<V>(__shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1)));
+                    float dot = 0.0f;
+                    if (row[k] >= 0) {
+                        float e[PACK];
+#pragma unroll
+                        for (int i = 0; i < N; ++i) vstore(e + 2 * i, vmul(s, g[i]));
+                        *reinterpret_cast<Held<T, PACK> *>(drows + row[k] * d.rows_stride + c) = packed<T, PACK>(e);
+                        if (dweights) {
+                            unpack(v[k], e);
+                            V sum = vall<V>(0.0f);
+#pragma unroll
+                            for (int i = 0; i < N; ++i) sum = vfma(g[i], vload<V>(e + 2 * i), sum);
+                            float both[2] = {0.0f, 0.0f};
+                            vstore(both, sum);
+                            dot = both[0] + both[1];
+                        }
+                    }
+                    if (dweights) {
+                        dot = warp_sum(dot);
+                        if (lane == j + k) total += dot;
+                    }
+                }
+            }
+        }
+    if (!dweights) return;
+    dots[warp][lane] = total;
+    __syncthreads();
+    if (t < d.tokens && part == 0 && lane < d.top_k) {
+        float sum = 0.0f;
+        for (int i = 0; i < warps; ++i) sum += dots[warp + i][lane];
+        dweights[t * d.top_k + lane] = sum;
     }
 }
 
@@ -72,7 +166,11 @@ bool combine_shape(const tb_expert_combine_desc *d, CombineShape *s) {
            product(d->rows, s->rows_stride, SIZE_MAX / 64, &all) && product(d->tokens, s->out_stride, SIZE_MAX / 64, &all);
 }
 
-unsigned combine_grid(const CombineShape &s) { return static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps); }
+/* The packs that every row of both tensors allows. */
+int combine_pack(const CombineShape &s, size_t size, const void *a, const void *b, const void *c) {
+    return pack_of(reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
+                       (s.rows_stride | s.out_stride | s.width) * size, size);
+}
 
 } /* namespace */
 
@@ -86,9 +184,19 @@ extern "C" int tb_cuda_combine_experts_device(const tb_expert_combine_desc *desc
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        combine_forward<T><<<combine_grid(s), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-            s, static_cast<const T *>(rows), position, weights, static_cast<T *>(out));
-        return launched();
+        return with_pack<T>(combine_pack(s, size, rows, out, nullptr), [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            const size_t packs = (s.width + P - 1) / P;
+            int lanes = 1;
+            while (lanes < 32 && static_cast<size_t>(lanes) < packs) lanes *= 2;
+            const size_t chunks = (packs + lanes - 1) / lanes;
+            size_t teams;
+            if (!product(s.tokens, chunks, 0x7fffffffull * (kThreads / lanes) , &teams) || chunks > 0x7fffffffu) return 0;
+            combine_forward<T, P><<<static_cast<unsigned>((teams * lanes + kThreads - 1) / kThreads), kThreads, 0,
+                                    static_cast<cudaStream_t>(stream)>>>(
+                s, lanes, static_cast<int>(chunks), static_cast<const T *>(rows), position, weights, static_cast<T *>(out));
+            return launched();
+        });
     });
 }
 
@@ -107,9 +215,16 @@ extern "C" int tb_cuda_combine_experts_backward_device(const tb_expert_combine_d
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        combine_backward<T><<<combine_grid(s), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-            s, static_cast<const T *>(rows), position, weights, static_cast<const T *>(dout),
-            static_cast<T *>(drows), dweights);
-        return launched();
+        return with_pack<T>(combine_pack(s, size, rows, dout, drows), [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            int warps = 1;
+            while (warps < kWarps && static_cast<size_t>(warps) * 32 * P < s.width) warps *= 2;
+            const size_t per = kWarps / warps;
+            combine_backward<T, P><<<static_cast<unsigned>((s.tokens + per - 1) / per), kThreads, 0,
+                                     static_cast<cudaStream_t>(stream)>>>(
+                s, warps, static_cast<const T *>(rows), position, weights, static_cast<const T *>(dout),
+                static_cast<T *>(drows), dweights);
+            return launched();
+        });
     });
 }

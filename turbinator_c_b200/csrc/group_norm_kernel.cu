@@ -848,20 +848,10 @@ bool tiling_of(const NormShape &d, int pack, size_t size, Tiling *g) {
     return true;
 }
 
-/* The widest pack that every row allows: 16 bytes, 4 bytes, an element. */
+/* The widest pack that every row allows. */
 int pack_of(const NormShape &d, size_t size, const void *a, size_t as, size_t ap, const void *b, size_t bs, size_t bp) {
-    const size_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (as | ap | bs | bp) * size |
-                       static_cast<size_t>(d.channels) * size;
-    if (all % 16 == 0) return static_cast<int>(16 / size);
-    return all % 4 == 0 ? static_cast<int>(4 / size) : 1;
-}
-
-/* Calls f with the pack as a constant. */
-template <class T, class F> int with_pack(int pack, F &&f) {
-    if (pack == 16 / static_cast<int>(sizeof(T))) return f(std::integral_constant<int, 16 / static_cast<int>(sizeof(T))>{});
-    if constexpr (sizeof(T) == 2)
-        if (pack == 2) return f(std::integral_constant<int, 2>{});
-    return f(std::integral_constant<int, 1>{});
+    return tb_learn::pack_of(reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (as | ap | bs | bp) * size |
+                                 static_cast<size_t>(d.channels) * size, size);
 }
 
 template <auto Kernel, class... Args>

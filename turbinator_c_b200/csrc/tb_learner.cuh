@@ -278,6 +278,21 @@ template <auto Kernel> bool allow_shared(size_t shared) {
     return true;
 }
 
+/* A pack is 16 bytes, 4 bytes or an element: the widest one that divides all of
+ * `bits` (addresses, strides and widths in bytes, or-ed). */
+inline int pack_of(size_t bits, size_t size) {
+    if (bits % 16 == 0) return static_cast<int>(16 / size);
+    return bits % 4 == 0 ? static_cast<int>(4 / size) : 1;
+}
+
+/* Calls f with the pack as a constant. */
+template <class T, class F> inline int with_pack(int pack, F &&f) {
+    if (pack == 16 / static_cast<int>(sizeof(T))) return f(std::integral_constant<int, 16 / static_cast<int>(sizeof(T))>{});
+    if constexpr (sizeof(T) == 2)
+        if (pack == 2) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 1>{});
+}
+
 inline int launched() { return cudaGetLastError() == cudaSuccess; }
 
 } /* namespace tb_learn */
