@@ -1,6 +1,21 @@
 /*
  * Routing to experts: selection, weights, slot lists and the gradient of the
  * weights (include/turbinator/training/cuda_learner.h).
+ *
+ * Bound: the selection by issue (a few hundred instructions a token), the rest
+ * by latency: the logits are read once, the outputs written once.
+ *
+ * Selection, one warp a token, its experts in registers (NV consecutive ones a
+ * lane): the top_k-th largest of the lanes' maxima is a threshold that top_k
+ * values reach and every selected value reaches too, so that only the few
+ * values that reach it are gathered, one a lane, and each lane counts how many
+ * of them come before its own: that count is the slot.  Where more than 32
+ * reach it (ties), the best is taken top_k times instead.
+ *
+ * Slot lists: counts per tile of tokens, their prefix sums per expert, then
+ * each slot's place from a rank within its warp (match), within its tile and
+ * the prefix: no atomics decide an order.  A call of few slots does it all in
+ * one CTA.
  */
 #include "tb_learner.cuh"
 
@@ -8,9 +23,10 @@ using namespace tb_learn;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTileTokens = 128; /* tokens whose slots one CTA places */
+constexpr int kTileTokens = 64;  /* tokens whose slots one CTA selects and places */
+constexpr int kAloneSlots = 4096; /* slots that one CTA lists alone */
 constexpr float kNone = -INFINITY;
 
 struct RouteShape {
@@ -22,235 +38,414 @@ struct RouteShape {
 
 __device__ __forceinline__ float available(float logit) { return logit == logit ? logit : kNone; }
 
-/* The score's expression is the one whose bits the ranking is stated in:
- * expf, one addition, one division. */
+/* The sigmoid whose bits the ranking is stated in: expf, one addition, one division. */
 __device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
-
-/* Highest value of the warp's experts and the lowest index that has it;
- * index -1 where every value is -inf. */
-__device__ __forceinline__ int warp_best(const float *value, int count, int lane, float *best) {
-    float v = kNone;
-    int at = -1;
-    for (int e = lane; e < count; e += 32)
-        if (value[e] > v) {
-            v = value[e];
-            at = e;
-        }
-    const float top = warp_max(v);
-    int first = v == top && at >= 0 ? at : 0x7fffffff;
-    first = __reduce_min_sync(0xffffffffu, first);
-    *best = top;
-    return first == 0x7fffffff ? -1 : first;
+/* e^(l - most) for l <= most; the highest logits share where they are infinite. */
+__device__ __forceinline__ float softened(float l, float most) {
+    return l == most ? 1.0f : fast_exp2(kLog2e * (l - most));
 }
 
-/* One warp per token. */
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-route_select(RouteShape d, const T *logits, const float *bias, int32_t *ids, float *weights) {
-    extern __shared__ float shared[];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + warp;
-    float *logit = shared + warp * (2 * d.experts + d.groups), *value = logit + d.experts, *strength = value + d.experts;
-    if (t >= d.tokens) return;
-    float most = kNone;
-    for (int e = lane; e < d.experts; e += 32) {
-        logit[e] = available(to_float(logits[t * d.stride + e]));
-        most = fmaxf(most, logit[e]);
+/* Unsigned keys in the values' order; 0 for what cannot be taken. */
+__device__ __forceinline__ unsigned key_of(float v) {
+    const unsigned b = __float_as_uint(v + 0.0f); /* -0 ranks with 0 */
+    return v == kNone ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+/* NV logits from expert `first` on, -inf where there is none. */
+template <class T, int NV>
+__device__ __forceinline__ void load_logits(const T *row, int first, int experts, bool packs, float (&l)[NV]) {
+    constexpr int P = NV * sizeof(T) < 16 ? NV : 16 / sizeof(T);
+    if (packs && first + NV <= experts) {
+#pragma unroll
+        for (int i = 0; i < NV; i += P) {
+            const Pack<T, P> v = *reinterpret_cast<const Pack<T, P> *>(row + first + i);
+#pragma unroll
+            for (int j = 0; j < P; ++j) l[i + j] = available(to_float(v.v[j]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) l[i] = first + i < experts ? available(to_float(row[first + i])) : kNone;
     }
-    most = warp_max(most);
-    const bool soft = d.score == TB_SCORE_SOFTMAX;
-    float sum = 0.0f;
-    for (int e = lane; e < d.experts; e += 32) {
-        const float l = logit[e];
-        sum += l == kNone ? 0.0f : l == most ? 1.0f : expf(l - most);
+}
+
+/* Candidates of a warp, and room for a row of values where groups do not fall on lanes. */
+struct Gathered {
+    unsigned key[32];
+    int expert[32];
+    float logit[32];
+};
+
+/* Leaves in value[] what the token's chosen groups hold, kNone elsewhere.  A
+ * group is a run of lanes, or else read back from `row`. */
+template <int NV>
+__device__ __forceinline__ void keep_groups(const RouteShape &d, float (&value)[NV], float *row, int lane) {
+    const int per = d.experts / d.groups, first = lane * NV;
+    const int run = per / NV; /* lanes of a group */
+    if (per % NV == 0 && (run & (run - 1)) == 0) {
+        float a = kNone, b = kNone; /* the two best */
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            b = fmaxf(b, fminf(a, value[i]));
+            a = fmaxf(a, value[i]);
+        }
+        for (int o = 1; o < run; o *= 2) {
+            const float c = __shfl_xor_sync(0xffffffffu, a, o), e = __shfl_xor_sync(0xffffffffu, b, o);
+            b = fmaxf(fminf(a, c), fmaxf(b, e));
+            a = fmaxf(a, c);
+        }
+        const float strength = d.group_best == 2 && b > kNone ? a + b : a;
+        const int mine = lane / run;
+        int before = 0;
+        for (int g = 0; g < d.groups; ++g) {
+            const float other = __shfl_sync(0xffffffffu, strength, g * run);
+            before += other > strength || (other == strength && g < mine);
+        }
+        if (before >= d.top_groups || strength == kNone)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) value[i] = kNone;
+        return;
     }
-    sum = warp_sum(sum);
-    const auto score_of = [&](float l) {
-        if (l == kNone) return 0.0f;
-        return soft ? (l == most ? 1.0f : expf(l - most)) / sum : sigmoid(l);
-    };
-    const bool by_logit = !bias && (d.groups == 1 || d.group_best == 1);
-    for (int e = lane; e < d.experts; e += 32) {
-        const float l = logit[e];
-        value[e] = l == kNone || by_logit ? l : score_of(l) + (bias ? bias[e] : 0.0f);
+    float *const strength = row + d.experts;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (first + i < d.experts) row[first + i] = value[i];
+    __syncwarp();
+    for (int g = lane; g < d.groups; g += 32) {
+        float a = kNone, b = kNone;
+        for (int e = g * per; e < (g + 1) * per; ++e) {
+            b = fmaxf(b, fminf(a, row[e]));
+            a = fmaxf(a, row[e]);
+        }
+        strength[g] = d.group_best == 2 && b > kNone ? a + b : a;
     }
     __syncwarp();
-    if (d.groups > 1) {
-        const int per = d.experts / d.groups;
-        for (int g = lane; g < d.groups; g += 32) {
-            float a = kNone, b = kNone;
-            for (int e = g * per; e < (g + 1) * per; ++e) {
-                const float v = value[e];
-                if (v > a) {
-                    b = a;
-                    a = v;
-                } else if (v > b) {
-                    b = v;
+    int last = -1;
+    bool keep = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int g = (first + i) / per;
+        if (first + i < d.experts && g != last) {
+            last = g;
+            const float s = strength[g];
+            int before = 0;
+            for (int h = 0; h < d.groups; ++h) before += strength[h] > s || (strength[h] == s && h < g);
+            keep = before < d.top_groups && s > kNone;
+        }
+        if (!keep) value[i] = kNone;
+    }
+}
+
+/* One warp per token.  count: [tiles, experts] where the slots are listed by
+ * tiles, or NULL. */
+template <class T, int NV>
+__global__ void __launch_bounds__(kThreads)
+route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float *bias, int32_t *ids, float *weights,
+             int32_t *count) {
+    extern __shared__ float rows[]; /* of experts + groups a warp, where they are needed */
+    __shared__ Gathered gathered[kWarps];
+    __shared__ int hist[TB_ROUTE_MAX_EXPERTS];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, first = lane * NV;
+    Gathered &g = gathered[warp];
+    if (count) {
+        for (int e = threadIdx.x; e < d.experts; e += kThreads) hist[e] = 0;
+        __syncthreads();
+    }
+    const bool soft = d.score == TB_SCORE_SOFTMAX;
+    const bool scored = bias || (d.groups > 1 && d.group_best == 2); /* ranked, or grouped, by scores */
+    float b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) b[i] = bias && first + i < d.experts ? bias[first + i] : 0.0f;
+    const size_t begin = static_cast<size_t>(blockIdx.x) * per_cta;
+    const size_t end = begin + per_cta < d.tokens ? begin + per_cta : d.tokens;
+    for (size_t t = begin + warp; t < end; t += kWarps) {
+        float l[NV], value[NV];
+        load_logits<T, NV>(logits + t * d.stride, first, d.experts, packs, l);
+        float most = 0.0f, sum = 0.0f;
+        if (soft) {
+            most = kNone;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) most = fmaxf(most, l[i]);
+            most = warp_max(most);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) sum += l[i] == kNone ? 0.0f : softened(l[i], most);
+            sum = warp_sum(sum);
+        }
+        const auto score_of = [&](float v) { return v == kNone ? 0.0f : soft ? softened(v, most) / sum : sigmoid(v); };
+#pragma unroll
+        for (int i = 0; i < NV; ++i) value[i] = !scored || l[i] == kNone ? l[i] : score_of(l[i]) + b[i];
+        if (d.groups > 1) {
+            keep_groups<NV>(d, value, rows + warp * (d.experts + d.groups), lane);
+            if (scored && !bias)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) value[i] = value[i] == kNone ? kNone : l[i];
+        }
+        unsigned key[NV], top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            key[i] = key_of(value[i]);
+            top = max(top, key[i]);
+        }
+        /* the top_k-th largest of the lanes' maxima */
+        for (int j = 1; j < d.top_k; ++j) {
+            const unsigned best = __reduce_max_sync(0xffffffffu, top);
+            const unsigned have = __ballot_sync(0xffffffffu, top == best);
+            if (lane == __ffs(have) - 1) top = 0;
+        }
+        const unsigned least = max(__reduce_max_sync(0xffffffffu, top), 1u);
+        int found = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const unsigned have = __ballot_sync(0xffffffffu, key[i] >= least);
+            if (!have) continue;
+            const int to = found + __popc(have & ((1u << lane) - 1));
+            if (key[i] >= least && to < 32) {
+                g.key[to] = key[i];
+                g.expert[to] = first + i;
+                g.logit[to] = l[i];
+            }
+            found += __popc(have);
+        }
+        __syncwarp();
+        int slot = 32, expert = -1; /* of this lane's candidate */
+        float score = 0.0f;
+        if (found <= 32) {
+            const unsigned mine = lane < found ? g.key[lane] : 0u;
+            expert = lane < found ? g.expert[lane] : -1;
+            slot = 0;
+            for (int c = 0; c < found; ++c) {
+                const unsigned other = g.key[c];
+                slot += other > mine || (other == mine && g.expert[c] < expert);
+            }
+            if (lane < found && slot < d.top_k) score = score_of(g.logit[lane]);
+            if (lane >= found) slot = lane; /* an empty slot, if it is one */
+        } else {
+            for (int j = 0; j < d.top_k; ++j) { /* lane j takes the j-th best */
+                unsigned best = 0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) best = max(best, key[i]);
+                const unsigned all = __reduce_max_sync(0xffffffffu, best);
+                const int from = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
+                int at = 0;
+                float logit = 0.0f;
+#pragma unroll
+                for (int i = NV - 1; i >= 0; --i)
+                    if (key[i] == all) {
+                        at = first + i;
+                        logit = l[i];
+                    }
+                at = __shfl_sync(0xffffffffu, at, from);
+                logit = __shfl_sync(0xffffffffu, logit, from);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (first + i == at) key[i] = 0;
+                if (lane == j) {
+                    expert = at;
+                    score = score_of(logit);
                 }
             }
-            strength[g] = d.group_best == 2 && b > kNone ? a + b : a;
+            slot = lane;
         }
-        __syncwarp();
-        for (int r = 0; r < d.top_groups; ++r) {
-            float best;
-            const int g = warp_best(strength, d.groups, lane, &best);
-            if (g < 0) break;
-            __syncwarp();
-            if (lane == 0) strength[g] = NAN; /* chosen */
-            __syncwarp();
+        const bool takes = expert >= 0 && slot < d.top_k;
+        const float total = warp_sum(takes ? score : 0.0f);
+        if (slot < d.top_k) {
+            const float w = !d.renormalise ? score : total > 0.0f ? score / total : 0.0f;
+            ids[t * d.top_k + slot] = takes ? expert : -1;
+            weights[t * d.top_k + slot] = takes ? w * d.scale : 0.0f;
         }
-        for (int e = lane; e < d.experts; e += 32) {
-            const float s = strength[e / per];
-            if (s == s) value[e] = kNone;
-            else if (!bias && value[e] != kNone) value[e] = logit[e];
-        }
+        if (count && takes) atomicAdd(&hist[expert], 1);
         __syncwarp();
     }
-    float total = 0.0f, mine = 0.0f; /* lane j keeps slot j */
-    int id = -1;
-    for (int j = 0; j < d.top_k; ++j) {
-        float best;
-        const int e = warp_best(value, d.experts, lane, &best);
-        if (e < 0) break;
-        const float s = score_of(logit[e]);
-        total += s;
-        if (lane == j) {
-            id = e;
-            mine = s;
-        }
-        __syncwarp();
-        if (lane == 0) value[e] = kNone;
-        __syncwarp();
-    }
-    if (lane < d.top_k) {
-        ids[t * d.top_k + lane] = id;
-        const float w = !d.renormalise ? mine : total > 0.0f ? mine / total : 0.0f;
-        weights[t * d.top_k + lane] = w * d.scale;
+    if (count) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < d.experts; e += kThreads) count[static_cast<size_t>(blockIdx.x) * d.experts + e] = hist[e];
     }
 }
 
-/* How many slots of each tile go to each expert: count [tiles, experts]. */
+/* 32 experts a CTA: turns each tile's counts into those of the tiles before it; total [experts]. */
+__global__ void __launch_bounds__(1024) route_prefix(int tiles, int experts, int32_t *count, int32_t *total) {
+    __shared__ int sums[32][33];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
+    const int each = (tiles + 31) / 32, first = warp * each, last = min(first + each, tiles);
+    int s = 0;
+    if (e < experts)
+#pragma unroll 8
+        for (int b = first; b < last; ++b) s += count[static_cast<size_t>(b) * experts + e];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0) {
+        int before = 0;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) {
+            const int c = sums[w][lane];
+            sums[w][lane] = before;
+            before += c;
+        }
+        if (e < experts) total[e] = before;
+    }
+    __syncthreads();
+    s = sums[warp][lane];
+    if (e < experts)
+#pragma unroll 8
+        for (int b = first; b < last; ++b) {
+            const int c = count[static_cast<size_t>(b) * experts + e];
+            count[static_cast<size_t>(b) * experts + e] = s;
+            s += c;
+        }
+}
+
+/* Places the slots of a tile of tokens (ALONE: of all tokens).  Each warp takes
+ * consecutive slots; next[warp][expert] is where its next slot of the expert
+ * goes. */
+template <bool ALONE>
 __global__ void __launch_bounds__(kThreads)
-route_count(RouteShape d, const int32_t *ids, int32_t *count) {
-    __shared__ int hist[TB_ROUTE_MAX_EXPERTS];
-    for (int e = threadIdx.x; e < d.experts; e += kThreads) hist[e] = 0;
-    __syncthreads();
-    const size_t first = static_cast<size_t>(blockIdx.x) * kTileTokens;
-    const size_t last = first + kTileTokens < d.tokens ? first + kTileTokens : d.tokens;
-    for (size_t i = first * d.top_k + threadIdx.x; i < last * d.top_k; i += kThreads) {
-        const int32_t e = ids[i];
-        if (e >= 0) atomicAdd(&hist[e], 1);
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < d.experts; e += kThreads)
-        count[static_cast<size_t>(blockIdx.x) * d.experts + e] = hist[e];
-}
-
-/* Turns the counts into each tile's first place per expert, and writes the offsets. */
-__global__ void __launch_bounds__(1024)
-route_offsets(RouteShape d, int tiles, int32_t *count, int32_t *offsets) {
-    __shared__ int total[TB_ROUTE_MAX_EXPERTS + 1];
-    const int e = threadIdx.x;
-    if (e < d.experts) {
-        int s = 0;
-        for (int b = 0; b < tiles; ++b) s += count[static_cast<size_t>(b) * d.experts + e];
-        total[e] = s;
-    }
-    __syncthreads();
-    if (e == 0) {
-        int s = 0;
-        for (int i = 0; i < d.experts; ++i) {
-            const int c = total[i];
-            total[i] = s;
-            s += c;
-        }
-        total[d.experts] = s;
-    }
-    __syncthreads();
-    if (e < d.experts) {
-        int s = total[e];
-        for (int b = 0; b < tiles; ++b) {
-            const int c = count[static_cast<size_t>(b) * d.experts + e];
-            count[static_cast<size_t>(b) * d.experts + e] = s;
-            s += c;
-        }
-    }
-    for (int i = e; i <= d.experts; i += 1024) offsets[i] = total[i];
-}
-
-/* One warp per tile, its slots in order. */
-__global__ void __launch_bounds__(32)
-route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_t *offsets, int32_t *order,
+route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_t *total, int32_t *offsets, int32_t *order,
             int32_t *position) {
-    __shared__ int next[TB_ROUTE_MAX_EXPERTS];
-    const int lane = threadIdx.x;
-    for (int e = lane; e < d.experts; e += 32) next[e] = count[static_cast<size_t>(blockIdx.x) * d.experts + e];
-    __syncwarp();
-    const size_t first = static_cast<size_t>(blockIdx.x) * kTileTokens;
-    const size_t last = first + kTileTokens < d.tokens ? first + kTileTokens : d.tokens;
+    extern __shared__ int next[]; /* [kWarps][experts], then first[experts] */
+    __shared__ int part[kWarps];
+    int *const first = next + kWarps * d.experts;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const size_t slots = d.tokens * d.top_k;
-    for (size_t base = first * d.top_k; base < last * d.top_k; base += 32) {
+    const size_t begin = ALONE ? 0 : static_cast<size_t>(blockIdx.x) * kTileTokens * d.top_k;
+    const size_t end = ALONE || begin + static_cast<size_t>(kTileTokens) * d.top_k > slots
+                           ? slots : begin + static_cast<size_t>(kTileTokens) * d.top_k;
+    const size_t each = (end - begin + kThreads - 1) / kThreads * 32; /* of a warp, whole rows of lanes */
+    const size_t from = begin + warp * each, to = from + each < end ? from + each : end;
+    int *const own = next + warp * d.experts;
+    for (int i = threadIdx.x; i < kWarps * d.experts; i += kThreads) next[i] = 0;
+    __syncthreads();
+    for (size_t base = from; base < to; base += 32) {
+        const int e = base + lane < to ? ids[base + lane] : -1;
+        const unsigned peers = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && lane == __ffs(peers) - 1) own[e] += __popc(peers);
+        __syncwarp();
+    }
+    __syncthreads();
+    /* totals of the experts, then the experts before each: runs of experts a thread */
+    const int run = (d.experts + kThreads - 1) / kThreads, mine = threadIdx.x * run;
+    int sum = 0;
+    for (int i = 0; i < run; ++i) {
+        const int e = mine + i;
+        if (e >= d.experts) break;
+        int c = 0;
+        if (ALONE) {
+            for (int w = 0; w < kWarps; ++w) c += next[w * d.experts + e];
+        } else {
+            c = total[e];
+        }
+        first[e] = sum;
+        sum += c;
+    }
+    int before = sum; /* inclusive over the threads, then exclusive */
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    if (lane == 31) part[warp] = before;
+    __syncthreads();
+    before -= sum;
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before += all;
+        all += part[w];
+    }
+    for (int i = 0; i < run; ++i) {
+        const int e = mine + i;
+        if (e >= d.experts) break;
+        int at = first[e] + before;
+        if (blockIdx.x == 0) offsets[e] = at;
+        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * d.experts + e];
+        for (int w = 0; w < kWarps; ++w) {
+            const int c = next[w * d.experts + e];
+            next[w * d.experts + e] = at;
+            at += c;
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[d.experts] = all;
+    __syncthreads();
+    for (size_t base = from; base < to; base += 32) {
         const size_t i = base + lane;
-        const int e = i < last * d.top_k ? ids[i] : -1;
+        const int e = i < to ? ids[i] : -1;
         const unsigned peers = __match_any_sync(0xffffffffu, e);
         const int rank = __popc(peers & ((1u << lane) - 1));
-        int place = -1;
-        if (e >= 0) place = next[e] + rank;
+        const int place = e >= 0 ? own[e] + rank : -1;
         __syncwarp();
-        if (e >= 0 && rank == 0) next[e] += __popc(peers);
+        if (e >= 0 && rank == 0) own[e] += __popc(peers);
         __syncwarp();
         if (e >= 0) order[place] = static_cast<int32_t>(i);
-        if (i < last * d.top_k) position[i] = place;
+        if (i < to) position[i] = place;
     }
-    for (size_t i = offsets[d.experts] + static_cast<size_t>(blockIdx.x) * 32 + lane; i < slots;
-         i += static_cast<size_t>(gridDim.x) * 32)
+    for (size_t i = all + static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; i < slots;
+         i += static_cast<size_t>(gridDim.x) * kThreads)
         order[i] = -1;
 }
 
-/* One warp per token. */
+/* One warp per token.  Only the token's selected experts have a gradient of
+ * their score; through the softmax it reaches the others too, unless the
+ * weights are renormalised, when the row's sum cancels: dlogit_j = w_j (dw_j -
+ * sum dw w) of the selected alone, and no other logit is read. */
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-route_backward(RouteShape d, const T *logits, const int32_t *ids, const float *dweights, T *dlogits) {
-    extern __shared__ float shared[];
+route_backward(RouteShape d, bool packs, const T *logits, const int32_t *ids, const float *dweights, T *dlogits) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    constexpr int P = 16 / sizeof(T);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int pitch = (d.experts + P - 1) / P * P;
+    T *const row = reinterpret_cast<T *>(dynamic) + warp * pitch; /* the token's gradients */
     const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + warp;
-    float *logit = shared + warp * 2 * d.experts, *dscore = logit + d.experts;
     if (t >= d.tokens) return;
-    float most = kNone;
-    for (int e = lane; e < d.experts; e += 32) {
-        logit[e] = available(to_float(logits[t * d.stride + e]));
-        most = fmaxf(most, logit[e]);
-        dscore[e] = 0.0f;
-    }
-    most = warp_max(most);
-    const bool soft = d.score == TB_SCORE_SOFTMAX;
-    float sum = 0.0f;
-    for (int e = lane; e < d.experts; e += 32) {
-        const float l = logit[e];
-        sum += l == kNone ? 0.0f : l == most ? 1.0f : expf(l - most);
-    }
-    sum = warp_sum(sum);
-    const auto score_of = [&](float l) {
-        if (l == kNone) return 0.0f;
-        return soft ? (l == most ? 1.0f : expf(l - most)) / sum : sigmoid(l);
-    };
-    __syncwarp();
+    const T *const in = logits + t * d.stride;
+    T *const out = dlogits + t * d.stride;
+    const bool soft = d.score == TB_SCORE_SOFTMAX, dense = soft && !d.renormalise;
     const int id = lane < d.top_k ? ids[t * d.top_k + lane] : -1;
-    const bool there = id >= 0 && id < d.experts;
-    const float s = there ? score_of(logit[id]) : 0.0f;
-    float ds = there ? dweights[t * d.top_k + lane] * d.scale : 0.0f;
-    if (d.renormalise) {
-        const float total = warp_sum(s);
-        const float inner = warp_sum(ds * s);
-        ds = there && total > 0.0f ? (ds - inner / total) / total : 0.0f;
+    const float l = id >= 0 && id < d.experts ? available(to_float(in[id])) : kNone;
+    const bool there = l > kNone;
+    const float dw = there ? dweights[t * d.top_k + lane] * d.scale : 0.0f;
+    float gradient; /* of logit `id` */
+    float most = kNone, dot = 0.0f, sum = 1.0f;
+    if (soft) {
+        if (dense)
+            for (int e = lane; e < d.experts; e += 32) most = fmaxf(most, available(to_float(in[e])));
+        most = warp_max(fmaxf(most, l));
+        float s = there ? softened(l, most) : 0.0f;
+        if (dense) {
+            sum = 0.0f;
+            for (int e = lane; e < d.experts; e += 32) {
+                const float v = available(to_float(in[e]));
+                sum += v == kNone ? 0.0f : softened(v, most);
+            }
+        }
+        sum = warp_sum(dense ? sum : s);
+        s = sum > 0.0f ? s / sum : 0.0f;
+        dot = warp_sum(dw * s);
+        gradient = s * (dw - dot);
+    } else {
+        const float s = there ? sigmoid(l) : 0.0f;
+        float ds = dw;
+        if (d.renormalise) {
+            const float total = warp_sum(s), inner = warp_sum(dw * s);
+            ds = total > 0.0f ? (dw - inner / total) / total : 0.0f;
+        }
+        gradient = ds * s * (1.0f - s);
     }
-    if (there) dscore[id] = ds;
-    const float dot = warp_sum(ds * s);
+    for (int e = lane; e < pitch; e += 32) {
+        float v = 0.0f;
+        if (dense && e < d.experts) {
+            const float x = available(to_float(in[e]));
+            v = x == kNone ? 0.0f : -dot * (softened(x, most) / sum);
+        }
+        row[e] = from_float<T>(v);
+    }
     __syncwarp();
-    for (int e = lane; e < d.experts; e += 32) {
-        const float p = score_of(logit[e]);
-        const float g = soft ? p * (dscore[e] - dot) : dscore[e] * p * (1.0f - p);
-        dlogits[t * d.stride + e] = from_float<T>(g);
+    if (there) row[id] = from_float<T>(gradient);
+    __syncwarp();
+    if (packs) {
+        for (int e = lane * P; e < d.experts; e += 32 * P)
+            *reinterpret_cast<Pack<T, P> *>(out + e) = *reinterpret_cast<const Pack<T, P> *>(row + e);
+    } else {
+        for (int e = lane; e < d.experts; e += 32) out[e] = row[e];
     }
 }
 
@@ -279,13 +474,31 @@ bool route_shape(const tb_expert_route_desc *d, RouteShape *s) {
 }
 
 int route_tiles(const RouteShape &s) { return static_cast<int>((s.tokens + kTileTokens - 1) / kTileTokens); }
+bool route_alone(const RouteShape &s) { return s.tokens * s.top_k <= kAloneSlots; }
+
+/* Whether rows start on 16 bytes and hold whole packs of them. */
+template <class T> bool route_packs(const RouteShape &s, const void *a, const void *b) {
+    const size_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | s.stride * sizeof(T);
+    return (bits | s.experts * sizeof(T)) % 16 == 0;
+}
+
+template <class T, int NV>
+int launch_select(const RouteShape &s, const T *logits, const float *bias, int32_t *ids, float *weights, int32_t *count,
+                  cudaStream_t st) {
+    const int per_cta = count ? kTileTokens : kWarps;
+    const size_t shared = s.groups > 1 ? kWarps * (s.experts + s.groups) * sizeof(float) : 0;
+    if (!allow_shared<route_select<T, NV>>(shared)) return 0;
+    route_select<T, NV><<<static_cast<unsigned>((s.tokens + per_cta - 1) / per_cta), kThreads, shared, st>>>(
+        s, per_cta, route_packs<T>(s, logits, nullptr), logits, bias, ids, weights, count);
+    return launched();
+}
 
 } /* namespace */
 
 extern "C" size_t tb_cuda_route_experts_workspace(const tb_expert_route_desc *desc) {
     RouteShape s;
     if (!route_shape(desc, &s)) return 0;
-    return static_cast<size_t>(route_tiles(s)) * s.experts * sizeof(int32_t);
+    return (static_cast<size_t>(route_tiles(s)) + 1) * s.experts * sizeof(int32_t);
 }
 
 extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, const void *logits, const float *bias,
@@ -300,21 +513,30 @@ extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, co
         return 0;
     cudaGetLastError(); /* report these launches only */
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool alone = route_alone(s);
+    int32_t *count = static_cast<int32_t *>(workspace);
+    int32_t *const to = offsets && !alone ? count : nullptr;
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        route_select<T><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads,
-                          kWarps * (2 * s.experts + s.groups) * sizeof(float), st>>>(
-            s, static_cast<const T *>(logits), bias, ids, weights);
-        return launched();
+        const T *in = static_cast<const T *>(logits);
+        if (s.experts <= 32) return launch_select<T, 1>(s, in, bias, ids, weights, to, st);
+        if (s.experts <= 64) return launch_select<T, 2>(s, in, bias, ids, weights, to, st);
+        if (s.experts <= 128) return launch_select<T, 4>(s, in, bias, ids, weights, to, st);
+        if (s.experts <= 256) return launch_select<T, 8>(s, in, bias, ids, weights, to, st);
+        if (s.experts <= 512) return launch_select<T, 16>(s, in, bias, ids, weights, to, st);
+        return launch_select<T, 32>(s, in, bias, ids, weights, to, st);
     });
     if (!ok || !offsets) return ok;
-    int32_t *count = static_cast<int32_t *>(workspace);
+    const size_t shared = (kWarps + 1) * s.experts * sizeof(int);
+    if (alone) {
+        route_place<true><<<1, kThreads, shared, st>>>(s, ids, nullptr, nullptr, offsets, order, position);
+        return launched();
+    }
     const int tiles = route_tiles(s);
-    route_count<<<tiles, kThreads, 0, st>>>(s, ids, count);
+    int32_t *total = count + static_cast<size_t>(tiles) * s.experts;
+    route_prefix<<<(s.experts + 31) / 32, 1024, 0, st>>>(tiles, s.experts, count, total);
     if (!launched()) return 0;
-    route_offsets<<<1, 1024, 0, st>>>(s, tiles, count, offsets);
-    if (!launched()) return 0;
-    route_place<<<tiles, 32, 0, st>>>(s, ids, count, offsets, order, position);
+    route_place<false><<<tiles, kThreads, shared, st>>>(s, ids, count, total, offsets, order, position);
     return launched();
 }
 
@@ -328,9 +550,11 @@ extern "C" int tb_cuda_route_experts_backward_device(const tb_expert_route_desc 
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        route_backward<T><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads,
-                            kWarps * 2 * s.experts * sizeof(float), static_cast<cudaStream_t>(stream)>>>(
-            s, static_cast<const T *>(logits), ids, dweights, static_cast<T *>(dlogits));
+        const size_t shared = kWarps * align_up(s.experts * sizeof(T), 16);
+        route_backward<T><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads, shared,
+                            static_cast<cudaStream_t>(stream)>>>(
+            s, route_packs<T>(s, dlogits, nullptr), static_cast<const T *>(logits), ids, dweights,
+            static_cast<T *>(dlogits));
         return launched();
     });
 }

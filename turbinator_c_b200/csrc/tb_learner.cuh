@@ -268,7 +268,7 @@ inline int multiprocessors(int *device) {
  * kernel and device, and again only where more is asked for. */
 template <auto Kernel> bool allow_shared(size_t shared) {
     static std::atomic<size_t> allowed[kMaxDevices];
-    if (shared <= 48 * 1024) return true;
+    if (shared <= 32 * 1024) return true; /* 48 KB are allowed anyway, static shared memory included */
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
     if (shared <= allowed[dev].load(std::memory_order_relaxed)) return true;
