@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTileTokens = 64;  /* tokens whose slots one CTA selects and places */
+constexpr int kTileTokens = 32;   /* tokens that one CTA selects for and counts: four a warp */
+constexpr int kPlaceTiles = 4;    /* tiles whose slots one CTA places */
 constexpr int kAloneSlots = 4096; /* slots that one CTA lists alone */
 constexpr float kNone = -INFINITY;
 
@@ -45,35 +46,37 @@ __device__ __forceinline__ float softened(float l, float most) {
     return l == most ? 1.0f : fast_exp2(kLog2e * (l - most));
 }
 
-/* Unsigned keys in the values' order; 0 for what cannot be taken. */
+/* Unsigned keys in the values' order; 0 for what cannot be taken (-inf, NaN). */
 __device__ __forceinline__ unsigned key_of(float v) {
-    const unsigned b = __float_as_uint(v + 0.0f); /* -0 ranks with 0 */
-    return v == kNone ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+    const int b = __float_as_int(v + 0.0f); /* -0 ranks with 0 */
+    const unsigned k = static_cast<unsigned>(b ^ (b >> 31 | static_cast<int>(0x80000000u)));
+    return k - 0x00800000u <= 0xff800000u - 0x00800000u ? k : 0u; /* from the lowest finite value to +inf */
 }
 
-/* NV logits from expert `first` on, -inf where there is none. */
-template <class T, int NV>
-__device__ __forceinline__ void load_logits(const T *row, int first, int experts, bool packs, float (&l)[NV]) {
-    constexpr int P = NV * sizeof(T) < 16 ? NV : 16 / sizeof(T);
-    if (packs && first + NV <= experts) {
+/* NV logits of a token from expert `first` on, as they came: -inf where there is none. */
+template <class T, int NV> struct Logits {
+    static constexpr int P = NV * sizeof(T) < 16 ? NV : 16 / sizeof(T);
+    Pack<T, P> v[NV / P];
+
+    __device__ __forceinline__ void load(const T *row, int first, int experts, bool packs) {
+        if (packs && first + NV <= experts) {
 #pragma unroll
-        for (int i = 0; i < NV; i += P) {
-            const Pack<T, P> v = *reinterpret_cast<const Pack<T, P> *>(row + first + i);
+            for (int i = 0; i < NV / P; ++i) v[i] = *reinterpret_cast<const Pack<T, P> *>(row + first + i * P);
+        } else {
 #pragma unroll
-            for (int j = 0; j < P; ++j) l[i + j] = available(to_float(v.v[j]));
+            for (int i = 0; i < NV; ++i) v[i / P].v[i % P] = first + i < experts ? row[first + i] : from_float<T>(kNone);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) l[i] = first + i < experts ? available(to_float(row[first + i])) : kNone;
     }
-}
-
-/* Candidates of a warp, and room for a row of values where groups do not fall on lanes. */
-struct Gathered {
-    unsigned key[32];
-    int expert[32];
-    float logit[32];
+    __device__ __forceinline__ float operator[](int i) const { return to_float(v[i / P].v[i % P]); }
 };
+
+/* A warp's candidates: key, then the higher the lower the expert. */
+__device__ __forceinline__ unsigned long long candidate(unsigned key, int expert) {
+    return static_cast<unsigned long long>(key) << 32 | (0xffffffffu - static_cast<unsigned>(expert));
+}
+__device__ __forceinline__ int expert_of(unsigned long long c) {
+    return static_cast<int>(0xffffffffu - static_cast<unsigned>(c));
+}
 
 /* Leaves in value[] what the token's chosen groups hold, kNone elsewhere.  A
  * group is a run of lanes, or else read back from `row`. */
@@ -139,14 +142,14 @@ __device__ __forceinline__ void keep_groups(const RouteShape &d, float (&value)[
 /* One warp per token.  count: [tiles, experts] where the slots are listed by
  * tiles, or NULL. */
 template <class T, int NV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NV <= 8 ? 4 : 1)
 route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float *bias, int32_t *ids, float *weights,
              int32_t *count) {
     extern __shared__ float rows[]; /* of experts + groups a warp, where they are needed */
-    __shared__ Gathered gathered[kWarps];
+    __shared__ unsigned long long gathered[kWarps][32];
+    __shared__ unsigned keys[kWarps][NV][32];
     __shared__ int hist[TB_ROUTE_MAX_EXPERTS];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, first = lane * NV;
-    Gathered &g = gathered[warp];
     if (count) {
         for (int e = threadIdx.x; e < d.experts; e += kThreads) hist[e] = 0;
         __syncthreads();
@@ -158,66 +161,75 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
     for (int i = 0; i < NV; ++i) b[i] = bias && first + i < d.experts ? bias[first + i] : 0.0f;
     const size_t begin = static_cast<size_t>(blockIdx.x) * per_cta;
     const size_t end = begin + per_cta < d.tokens ? begin + per_cta : d.tokens;
+    Logits<T, NV> next;
+    if (begin + warp < end) next.load(logits + (begin + warp) * d.stride, first, d.experts, packs);
     for (size_t t = begin + warp; t < end; t += kWarps) {
-        float l[NV], value[NV];
-        load_logits<T, NV>(logits + t * d.stride, first, d.experts, packs, l);
-        float most = 0.0f, sum = 0.0f;
-        if (soft) {
+        const T *const in = logits + t * d.stride;
+        float value[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) value[i] = next[i];
+        if (t + kWarps < end) next.load(in + kWarps * d.stride, first, d.experts, packs);
+        if (scored || soft) /* elsewhere the keys see to it */
+#pragma unroll
+            for (int i = 0; i < NV; ++i) value[i] = available(value[i]);
+        float most = 0.0f, sum = 1.0f;
+        if (soft && (scored || !d.renormalise)) { /* else only the selected logits matter */
             most = kNone;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) most = fmaxf(most, l[i]);
+            for (int i = 0; i < NV; ++i) most = fmaxf(most, value[i]);
             most = warp_max(most);
+            sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) sum += l[i] == kNone ? 0.0f : softened(l[i], most);
+            for (int i = 0; i < NV; ++i) sum += value[i] == kNone ? 0.0f : softened(value[i], most);
             sum = warp_sum(sum);
         }
-        const auto score_of = [&](float v) { return v == kNone ? 0.0f : soft ? softened(v, most) / sum : sigmoid(v); };
+        if (scored || d.groups > 1) {
+            float l[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) value[i] = !scored || l[i] == kNone ? l[i] : score_of(l[i]) + b[i];
-        if (d.groups > 1) {
-            keep_groups<NV>(d, value, rows + warp * (d.experts + d.groups), lane);
-            if (scored && !bias)
+            for (int i = 0; i < NV; ++i) {
+                l[i] = value[i];
+                if (scored && l[i] != kNone)
+                    value[i] = (soft ? softened(l[i], most) / sum : sigmoid(l[i])) + b[i];
+            }
+            if (d.groups > 1) {
+                keep_groups<NV>(d, value, rows + warp * (d.experts + d.groups), lane);
+                if (scored && !bias)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) value[i] = value[i] == kNone ? kNone : l[i];
+                    for (int i = 0; i < NV; ++i) value[i] = value[i] == kNone ? kNone : l[i];
+            }
         }
         unsigned key[NV], top = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             key[i] = key_of(value[i]);
             top = max(top, key[i]);
+            keys[warp][i][lane] = key[i];
         }
-        /* the top_k-th largest of the lanes' maxima */
-        for (int j = 1; j < d.top_k; ++j) {
-            const unsigned best = __reduce_max_sync(0xffffffffu, top);
-            const unsigned have = __ballot_sync(0xffffffffu, top == best);
-            if (lane == __ffs(have) - 1) top = 0;
-        }
+        /* at most the top_k-th largest of the lanes' maxima: equal ones go together */
+        for (int j = 1; j < d.top_k; ++j)
+            if (top == __reduce_max_sync(0xffffffffu, top)) top = 0;
         const unsigned least = max(__reduce_max_sync(0xffffffffu, top), 1u);
-        int found = 0;
+        unsigned over = 0; /* the lane's that reach it */
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const unsigned have = __ballot_sync(0xffffffffu, key[i] >= least);
-            if (!have) continue;
+        for (int i = 0; i < NV; ++i) over |= static_cast<unsigned>(key[i] >= least) << i;
+        __syncwarp();
+        int found = 0;
+        for (unsigned have; (have = __ballot_sync(0xffffffffu, over)) != 0; over &= over - 1) {
             const int to = found + __popc(have & ((1u << lane) - 1));
-            if (key[i] >= least && to < 32) {
-                g.key[to] = key[i];
-                g.expert[to] = first + i;
-                g.logit[to] = l[i];
+            if (over && to < 32) {
+                const int i = __ffs(over) - 1;
+                gathered[warp][to] = candidate(keys[warp][i][lane], first + i);
             }
             found += __popc(have);
         }
         __syncwarp();
-        int slot = 32, expert = -1; /* of this lane's candidate */
-        float score = 0.0f;
+        int slot, expert = -1; /* of this lane's candidate */
         if (found <= 32) {
-            const unsigned mine = lane < found ? g.key[lane] : 0u;
-            expert = lane < found ? g.expert[lane] : -1;
+            const unsigned long long mine = lane < found ? gathered[warp][lane] : 0ull;
+            if (lane < found) expert = expert_of(mine);
             slot = 0;
-            for (int c = 0; c < found; ++c) {
-                const unsigned other = g.key[c];
-                slot += other > mine || (other == mine && g.expert[c] < expert);
-            }
-            if (lane < found && slot < d.top_k) score = score_of(g.logit[lane]);
+#pragma unroll 4
+            for (int c = 0; c < found; ++c) slot += gathered[warp][c] > mine;
             if (lane >= found) slot = lane; /* an empty slot, if it is one */
         } else {
             for (int j = 0; j < d.top_k; ++j) { /* lane j takes the j-th best */
@@ -227,31 +239,33 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
                 const unsigned all = __reduce_max_sync(0xffffffffu, best);
                 const int from = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
                 int at = 0;
-                float logit = 0.0f;
 #pragma unroll
                 for (int i = NV - 1; i >= 0; --i)
-                    if (key[i] == all) {
-                        at = first + i;
-                        logit = l[i];
-                    }
+                    if (key[i] == all) at = first + i;
                 at = __shfl_sync(0xffffffffu, at, from);
-                logit = __shfl_sync(0xffffffffu, logit, from);
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
                     if (first + i == at) key[i] = 0;
-                if (lane == j) {
-                    expert = at;
-                    score = score_of(logit);
-                }
+                if (lane == j) expert = at;
             }
             slot = lane;
         }
         const bool takes = expert >= 0 && slot < d.top_k;
-        const float total = warp_sum(takes ? score : 0.0f);
+        const float l = takes ? to_float(in[expert]) : kNone;
+        float score;
+        if (soft) {
+            if (!scored && d.renormalise) most = warp_max(l);
+            score = takes ? softened(l, most) / sum : 0.0f;
+        } else {
+            score = takes ? sigmoid(l) : 0.0f;
+        }
+        if (d.renormalise) {
+            const float total = warp_sum(score);
+            score = total > 0.0f ? score / total : 0.0f;
+        }
         if (slot < d.top_k) {
-            const float w = !d.renormalise ? score : total > 0.0f ? score / total : 0.0f;
-            ids[t * d.top_k + slot] = takes ? expert : -1;
-            weights[t * d.top_k + slot] = takes ? w * d.scale : 0.0f;
+            ids[t * d.top_k + slot] = expert;
+            weights[t * d.top_k + slot] = score * d.scale;
         }
         if (count && takes) atomicAdd(&hist[expert], 1);
         __syncwarp();
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(1024) route_prefix(int tiles, int experts, int
     const int each = (tiles + 31) / 32, first = warp * each, last = min(first + each, tiles);
     int s = 0;
     if (e < experts)
-#pragma unroll 8
+#pragma unroll 16
         for (int b = first; b < last; ++b) s += count[static_cast<size_t>(b) * experts + e];
     sums[warp][lane] = s;
     __syncthreads();
@@ -294,7 +308,7 @@ __global__ void __launch_bounds__(1024) route_prefix(int tiles, int experts, int
         }
 }
 
-/* Places the slots of a tile of tokens (ALONE: of all tokens).  Each warp takes
+/* Places the slots of kPlaceTiles tiles of tokens (ALONE: of all tokens).  Each warp takes
  * consecutive slots; next[warp][expert] is where its next slot of the expert
  * goes. */
 template <bool ALONE>
@@ -306,9 +320,9 @@ route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_
     int *const first = next + kWarps * d.experts;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const size_t slots = d.tokens * d.top_k;
-    const size_t begin = ALONE ? 0 : static_cast<size_t>(blockIdx.x) * kTileTokens * d.top_k;
-    const size_t end = ALONE || begin + static_cast<size_t>(kTileTokens) * d.top_k > slots
-                           ? slots : begin + static_cast<size_t>(kTileTokens) * d.top_k;
+    const size_t own_slots = static_cast<size_t>(kPlaceTiles * kTileTokens) * d.top_k;
+    const size_t begin = ALONE ? 0 : blockIdx.x * own_slots;
+    const size_t end = ALONE || begin + own_slots > slots ? slots : begin + own_slots;
     const size_t each = (end - begin + kThreads - 1) / kThreads * 32; /* of a warp, whole rows of lanes */
     const size_t from = begin + warp * each, to = from + each < end ? from + each : end;
     int *const own = next + warp * d.experts;
@@ -356,7 +370,7 @@ route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_
         if (e >= d.experts) break;
         int at = first[e] + before;
         if (blockIdx.x == 0) offsets[e] = at;
-        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * d.experts + e];
+        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * kPlaceTiles * d.experts + e];
         for (int w = 0; w < kWarps; ++w) {
             const int c = next[w * d.experts + e];
             next[w * d.experts + e] = at;
@@ -382,71 +396,112 @@ route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_
         order[i] = -1;
 }
 
-/* One warp per token.  Only the token's selected experts have a gradient of
- * their score; through the softmax it reaches the others too, unless the
- * weights are renormalised, when the row's sum cancels: dlogit_j = w_j (dw_j -
- * sum dw w) of the selected alone, and no other logit is read. */
+/* A row of gradients, from the warp's shared memory. */
+template <class T>
+__device__ __forceinline__ void store_row(T *out, const T *row, int experts, bool packs, int lane) {
+    constexpr int P = 16 / sizeof(T);
+    if (packs) {
+        for (int e = lane * P; e < experts; e += 32 * P)
+            *reinterpret_cast<Pack<T, P> *>(out + e) = *reinterpret_cast<const Pack<T, P> *>(row + e);
+    } else {
+        for (int e = lane; e < experts; e += 32) out[e] = row[e];
+    }
+}
+
+/* Sigmoid scores, and renormalised softmax scores, where the whole row's sum
+ * cancels: dlogit_j = w_j (dw_j - sum dw w).  Only the selected logits have a
+ * gradient, and no other is read.  A warp takes 32 / lanes tokens together, a
+ * lane a slot, then their rows one after the other. */
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-route_backward(RouteShape d, bool packs, const T *logits, const int32_t *ids, const float *dweights, T *dlogits) {
+route_backward_selected(RouteShape d, int lanes, bool packs, const T *logits, const int32_t *ids, const float *dweights,
+                        T *dlogits) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    constexpr int P = 16 / sizeof(T);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int pitch = (d.experts + P - 1) / P * P, tokens = 32 / lanes;
+    T *const row = reinterpret_cast<T *>(dynamic) + warp * pitch;
+    const size_t base = (static_cast<size_t>(blockIdx.x) * kWarps + warp) * tokens;
+    if (base >= d.tokens) return;
+    const size_t t = base + lane / lanes;
+    const int j = lane % lanes;
+    int id = -1;
+    float l = kNone, dw = 0.0f;
+    if (t < d.tokens && j < d.top_k) {
+        id = ids[t * d.top_k + j];
+        dw = dweights[t * d.top_k + j] * d.scale;
+        if (id >= 0 && id < d.experts) l = available(to_float(logits[t * d.stride + id]));
+    }
+    for (int e = lane * P; e < pitch; e += 32 * P) *reinterpret_cast<uint4 *>(row + e) = make_uint4(0u, 0u, 0u, 0u);
+    const bool there = l > kNone;
+    if (!there) dw = 0.0f;
+    const auto sum_of = [&](float v) {
+        for (int o = lanes / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    float gradient; /* of logit `id` */
+    if (d.score == TB_SCORE_SOFTMAX) {
+        float most = l;
+        for (int o = lanes / 2; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float s = there ? softened(l, most) : 0.0f;
+        const float total = sum_of(s);
+        s = there ? s / total : 0.0f;
+        gradient = s * (dw - sum_of(dw * s));
+    } else {
+        const float s = there ? fast_sigmoid(l) : 0.0f, rest = there ? fast_sigmoid(-l) : 0.0f;
+        float ds = dw;
+        if (d.renormalise) {
+            const float total = sum_of(s), inner = sum_of(dw * s);
+            ds = there && total > 0.0f ? (dw - inner / total) / total : 0.0f;
+        }
+        gradient = ds * s * rest;
+    }
+    for (int i = 0; i < tokens && base + i < d.tokens; ++i) {
+        const bool mine = there && lane / lanes == i;
+        __syncwarp();
+        if (mine) row[id] = from_float<T>(gradient);
+        __syncwarp();
+        store_row(dlogits + (base + i) * d.stride, row, d.experts, packs, lane);
+        __syncwarp();
+        if (mine) row[id] = from_float<T>(0.0f);
+    }
+}
+
+/* Softmax scores as they are: every logit of the row has a gradient, p_e (ds_e -
+ * sum ds p).  One warp per token. */
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+route_backward_dense(RouteShape d, bool packs, const T *logits, const int32_t *ids, const float *dweights, T *dlogits) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     constexpr int P = 16 / sizeof(T);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int pitch = (d.experts + P - 1) / P * P;
-    T *const row = reinterpret_cast<T *>(dynamic) + warp * pitch; /* the token's gradients */
+    T *const row = reinterpret_cast<T *>(dynamic) + warp * pitch;
     const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + warp;
     if (t >= d.tokens) return;
     const T *const in = logits + t * d.stride;
-    T *const out = dlogits + t * d.stride;
-    const bool soft = d.score == TB_SCORE_SOFTMAX, dense = soft && !d.renormalise;
     const int id = lane < d.top_k ? ids[t * d.top_k + lane] : -1;
     const float l = id >= 0 && id < d.experts ? available(to_float(in[id])) : kNone;
     const bool there = l > kNone;
     const float dw = there ? dweights[t * d.top_k + lane] * d.scale : 0.0f;
-    float gradient; /* of logit `id` */
-    float most = kNone, dot = 0.0f, sum = 1.0f;
-    if (soft) {
-        if (dense)
-            for (int e = lane; e < d.experts; e += 32) most = fmaxf(most, available(to_float(in[e])));
-        most = warp_max(fmaxf(most, l));
-        float s = there ? softened(l, most) : 0.0f;
-        if (dense) {
-            sum = 0.0f;
-            for (int e = lane; e < d.experts; e += 32) {
-                const float v = available(to_float(in[e]));
-                sum += v == kNone ? 0.0f : softened(v, most);
-            }
-        }
-        sum = warp_sum(dense ? sum : s);
-        s = sum > 0.0f ? s / sum : 0.0f;
-        dot = warp_sum(dw * s);
-        gradient = s * (dw - dot);
-    } else {
-        const float s = there ? sigmoid(l) : 0.0f;
-        float ds = dw;
-        if (d.renormalise) {
-            const float total = warp_sum(s), inner = warp_sum(dw * s);
-            ds = total > 0.0f ? (dw - inner / total) / total : 0.0f;
-        }
-        gradient = ds * s * (1.0f - s);
+    float most = kNone, sum = 0.0f;
+    for (int e = lane; e < d.experts; e += 32) most = fmaxf(most, available(to_float(in[e])));
+    most = warp_max(most);
+    for (int e = lane; e < d.experts; e += 32) {
+        const float v = available(to_float(in[e]));
+        sum += v == kNone ? 0.0f : softened(v, most);
     }
-    for (int e = lane; e < pitch; e += 32) {
-        float v = 0.0f;
-        if (dense && e < d.experts) {
-            const float x = available(to_float(in[e]));
-            v = x == kNone ? 0.0f : -dot * (softened(x, most) / sum);
-        }
-        row[e] = from_float<T>(v);
+    sum = warp_sum(sum);
+    const float over = sum > 0.0f ? 1.0f / sum : 0.0f, s = there ? softened(l, most) * over : 0.0f;
+    const float dot = warp_sum(dw * s);
+    for (int e = lane; e < d.experts; e += 32) {
+        const float v = available(to_float(in[e]));
+        row[e] = from_float<T>(v == kNone ? 0.0f : -dot * (softened(v, most) * over));
     }
     __syncwarp();
-    if (there) row[id] = from_float<T>(gradient);
+    if (there) row[id] = from_float<T>(s * (dw - dot));
     __syncwarp();
-    if (packs) {
-        for (int e = lane * P; e < d.experts; e += 32 * P)
-            *reinterpret_cast<Pack<T, P> *>(out + e) = *reinterpret_cast<const Pack<T, P> *>(row + e);
-    } else {
-        for (int e = lane; e < d.experts; e += 32) out[e] = row[e];
-    }
+    store_row(dlogits + t * d.stride, row, d.experts, packs, lane);
 }
 
 bool route_shape(const tb_expert_route_desc *d, RouteShape *s) {
@@ -536,7 +591,7 @@ extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, co
     int32_t *total = count + static_cast<size_t>(tiles) * s.experts;
     route_prefix<<<(s.experts + 31) / 32, 1024, 0, st>>>(tiles, s.experts, count, total);
     if (!launched()) return 0;
-    route_place<false><<<tiles, kThreads, shared, st>>>(s, ids, count, total, offsets, order, position);
+    route_place<false><<<(tiles + kPlaceTiles - 1) / kPlaceTiles, kThreads, shared, st>>>(s, ids, count, total, offsets, order, position);
     return launched();
 }
 
@@ -551,10 +606,22 @@ extern "C" int tb_cuda_route_experts_backward_device(const tb_expert_route_desc 
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         const size_t shared = kWarps * align_up(s.experts * sizeof(T), 16);
-        route_backward<T><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads, shared,
-                            static_cast<cudaStream_t>(stream)>>>(
-            s, route_packs<T>(s, dlogits, nullptr), static_cast<const T *>(logits), ids, dweights,
-            static_cast<T *>(dlogits));
+        const T *in = static_cast<const T *>(logits);
+        T *out = static_cast<T *>(dlogits);
+        const bool packs = route_packs<T>(s, dlogits, nullptr);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (s.score == TB_SCORE_SOFTMAX && !s.renormalise) {
+            if (!allow_shared<route_backward_dense<T>>(shared)) return 0;
+            route_backward_dense<T><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads, shared, st>>>(
+                s, packs, in, ids, dweights, out);
+            return launched();
+        }
+        int lanes = 1;
+        while (lanes < s.top_k) lanes *= 2;
+        const size_t per_cta = static_cast<size_t>(kWarps) * (32 / lanes);
+        if (!allow_shared<route_backward_selected<T>>(shared)) return 0;
+        route_backward_selected<T><<<static_cast<unsigned>((s.tokens + per_cta - 1) / per_cta), kThreads, shared, st>>>(
+            s, lanes, packs, in, ids, dweights, out);
         return launched();
     });
 }
