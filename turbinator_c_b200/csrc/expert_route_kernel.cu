@@ -25,8 +25,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTileTokens = 32;   /* tokens that one CTA selects for and counts: four a warp */
-constexpr int kPlaceTiles = 4;    /* tiles whose slots one CTA places */
+/* Tiles of tokens that one CTA each selects for, counts and places: as many as
+ * four CTAs on each of 148 SMs, so that all run at once and alike. */
+constexpr int kMostTiles = 4 * 148;
 constexpr int kAloneSlots = 4096; /* slots that one CTA lists alone */
 constexpr float kNone = -INFINITY;
 
@@ -308,21 +309,20 @@ __global__ void __launch_bounds__(1024) route_prefix(int tiles, int experts, int
         }
 }
 
-/* Places the slots of kPlaceTiles tiles of tokens (ALONE: of all tokens).  Each warp takes
+/* Places the slots of a tile of tokens (ALONE: of all tokens).  Each warp takes
  * consecutive slots; next[warp][expert] is where its next slot of the expert
  * goes. */
 template <bool ALONE>
 __global__ void __launch_bounds__(kThreads)
-route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_t *total, int32_t *offsets, int32_t *order,
+route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *count, const int32_t *total, int32_t *offsets, int32_t *order,
             int32_t *position) {
     extern __shared__ int next[]; /* [kWarps][experts], then first[experts] */
     __shared__ int part[kWarps];
     int *const first = next + kWarps * d.experts;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const size_t slots = d.tokens * d.top_k;
-    const size_t own_slots = static_cast<size_t>(kPlaceTiles * kTileTokens) * d.top_k;
-    const size_t begin = ALONE ? 0 : blockIdx.x * own_slots;
-    const size_t end = ALONE || begin + own_slots > slots ? slots : begin + own_slots;
+    const size_t own_slots = ALONE ? slots : static_cast<size_t>(tile_tokens) * d.top_k;
+    const size_t begin = blockIdx.x * own_slots, end = begin + own_slots < slots ? begin + own_slots : slots;
     const size_t each = (end - begin + kThreads - 1) / kThreads * 32; /* of a warp, whole rows of lanes */
     const size_t from = begin + warp * each, to = from + each < end ? from + each : end;
     int *const own = next + warp * d.experts;
@@ -370,7 +370,7 @@ route_place(RouteShape d, const int32_t *ids, const int32_t *count, const int32_
         if (e >= d.experts) break;
         int at = first[e] + before;
         if (blockIdx.x == 0) offsets[e] = at;
-        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * kPlaceTiles * d.experts + e];
+        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * d.experts + e];
         for (int w = 0; w < kWarps; ++w) {
             const int c = next[w * d.experts + e];
             next[w * d.experts + e] = at;
@@ -528,7 +528,14 @@ bool route_shape(const tb_expert_route_desc *d, RouteShape *s) {
     return true;
 }
 
-int route_tiles(const RouteShape &s) { return static_cast<int>((s.tokens + kTileTokens - 1) / kTileTokens); }
+/* Tokens of a tile: whole rounds of a CTA's warps. */
+int tile_tokens(const RouteShape &s) {
+    return static_cast<int>(align_up((s.tokens + kMostTiles - 1) / kMostTiles, kWarps));
+}
+int route_tiles(const RouteShape &s) {
+    const int each = tile_tokens(s);
+    return static_cast<int>((s.tokens + each - 1) / each);
+}
 bool route_alone(const RouteShape &s) { return s.tokens * s.top_k <= kAloneSlots; }
 
 /* Whether rows start on 16 bytes and hold whole packs of them. */
@@ -540,7 +547,7 @@ template <class T> bool route_packs(const RouteShape &s, const void *a, const vo
 template <class T, int NV>
 int launch_select(const RouteShape &s, const T *logits, const float *bias, int32_t *ids, float *weights, int32_t *count,
                   cudaStream_t st) {
-    const int per_cta = count ? kTileTokens : kWarps;
+    const int per_cta = count ? tile_tokens(s) : kWarps;
     const size_t shared = s.groups > 1 ? kWarps * (s.experts + s.groups) * sizeof(float) : 0;
     if (!allow_shared<route_select<T, NV>>(shared)) return 0;
     route_select<T, NV><<<static_cast<unsigned>((s.tokens + per_cta - 1) / per_cta), kThreads, shared, st>>>(
@@ -584,14 +591,14 @@ extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, co
     if (!ok || !offsets) return ok;
     const size_t shared = (kWarps + 1) * s.experts * sizeof(int);
     if (alone) {
-        route_place<true><<<1, kThreads, shared, st>>>(s, ids, nullptr, nullptr, offsets, order, position);
+        route_place<true><<<1, kThreads, shared, st>>>(s, 0, ids, nullptr, nullptr, offsets, order, position);
         return launched();
     }
     const int tiles = route_tiles(s);
     int32_t *total = count + static_cast<size_t>(tiles) * s.experts;
     route_prefix<<<(s.experts + 31) / 32, 1024, 0, st>>>(tiles, s.experts, count, total);
     if (!launched()) return 0;
-    route_place<false><<<(tiles + kPlaceTiles - 1) / kPlaceTiles, kThreads, shared, st>>>(s, ids, count, total, offsets, order, position);
+    route_place<false><<<tiles, kThreads, shared, st>>>(s, tile_tokens(s), ids, count, total, offsets, order, position);
     return launched();
 }
 
