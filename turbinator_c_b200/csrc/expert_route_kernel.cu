@@ -6,15 +6,16 @@
  * by latency: the logits are read once, the outputs written once.
  *
  * Selection, one warp a token, its experts in registers (NV consecutive ones a
- * lane): the top_k-th largest of the lanes' maxima is a threshold that top_k
- * values reach and every selected value reaches too, so that only the few
- * values that reach it are gathered, one a lane, and each lane counts how many
- * of them come before its own: that count is the slot.  Where more than 32
- * reach it (ties), the best is taken top_k times instead.
+ * lane): each lane sorts out its four best keys, then top_k times the best of
+ * the lanes' heads is taken and its lane moves on, three instructions of which
+ * look at all lanes.  Which of the lane's experts a key belongs to is looked up
+ * once at the end.  A lane that gives more than four (a few rows in 100,000 of
+ * random logits with top_k 8 of 256) sends the warp to a search of all keys.
  *
- * Slot lists: counts per tile of tokens, their prefix sums per expert, then
- * each slot's place from a rank within its warp (match), within its tile and
- * the prefix: no atomics decide an order.  A call of few slots does it all in
+ * Slot lists: a CTA on each SM selects for a tile of tokens and counts its
+ * slots per expert; a second kernel places each tile's slots behind those of
+ * the tiles before it: a rank within the warp (match), the warps before, the
+ * tiles before.  No atomics decide an order.  A call of few slots is listed by
  * one CTA.
  */
 #include "tb_learner.cuh"
@@ -25,10 +26,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-/* Tiles of tokens that one CTA each selects for, counts and places: as many as
- * four CTAs on each of 148 SMs, so that all run at once and alike. */
-constexpr int kMostTiles = 4 * 148;
+constexpr int kMostTiles = 148;   /* tiles of tokens: one on each SM */
+constexpr int kLeastTile = 8;     /* tokens */
+constexpr int kPlaceThreads = 512;
+constexpr int kPlaceWarps = kPlaceThreads / 32;
+constexpr int kHeld = 8;          /* rows of 32 slots that a placing warp keeps in registers */
 constexpr int kAloneSlots = 4096; /* slots that one CTA lists alone */
+constexpr int kHeads = 4;         /* best keys that a lane keeps sorted */
+
+/* Threads of a selecting CTA: what an SM has registers for. */
+constexpr int select_threads(int nv) { return nv <= 8 ? 1024 : nv <= 16 ? 512 : 256; }
 constexpr float kNone = -INFINITY;
 
 struct RouteShape {
@@ -54,6 +61,32 @@ __device__ __forceinline__ unsigned key_of(float v) {
     return k - 0x00800000u <= 0xff800000u - 0x00800000u ? k : 0u; /* from the lowest finite value to +inf */
 }
 
+/* The value of a key. */
+__device__ __forceinline__ float value_of(unsigned key) {
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+/* Keys of 16-bit logits that rank by themselves: 16 bits in the logits' order,
+ * then 65,535 less the expert, so that no two are equal and ties go to the
+ * lower expert. */
+template <class T> __device__ __forceinline__ unsigned tagged_key(T v, int expert) {
+    constexpr unsigned inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    constexpr unsigned low = (0xffffu - (0x8000u | inf) + 1) << 16, high = (inf | 0x8000u) << 16 | 0xffffu;
+    unsigned short h;
+    memcpy(&h, &v, 2);
+    int b = static_cast<int>(static_cast<unsigned>(h) << 16);
+    if (static_cast<unsigned>(b) == 0x80000000u) b = 0; /* -0 ranks with 0 */
+    unsigned k = static_cast<unsigned>(b ^ (b >> 31 | static_cast<int>(0x80000000u)));
+    k = (k & 0xffff0000u) + (0xffffu - static_cast<unsigned>(expert));
+    return k - low <= high - low ? k : 0u; /* from the lowest finite value to +inf */
+}
+template <class T> __device__ __forceinline__ float tagged_value(unsigned key) {
+    const unsigned short h = static_cast<unsigned short>(key & 0x80000000u ? key >> 16 ^ 0x8000u : ~key >> 16);
+    T v;
+    memcpy(&v, &h, 2);
+    return to_float(v);
+}
+
 /* NV logits of a token from expert `first` on, as they came: -inf where there is none. */
 template <class T, int NV> struct Logits {
     static constexpr int P = NV * sizeof(T) < 16 ? NV : 16 / sizeof(T);
@@ -68,15 +101,38 @@ template <class T, int NV> struct Logits {
             for (int i = 0; i < NV; ++i) v[i / P].v[i % P] = first + i < experts ? row[first + i] : from_float<T>(kNone);
         }
     }
-    __device__ __forceinline__ float operator[](int i) const { return to_float(v[i / P].v[i % P]); }
+    __device__ __forceinline__ T operator[](int i) const { return v[i / P].v[i % P]; }
 };
 
-/* A warp's candidates: key, then the higher the lower the expert. */
-__device__ __forceinline__ unsigned long long candidate(unsigned key, int expert) {
-    return static_cast<unsigned long long>(key) << 32 | (0xffffffffu - static_cast<unsigned>(expert));
-}
-__device__ __forceinline__ int expert_of(unsigned long long c) {
-    return static_cast<int>(0xffffffffu - static_cast<unsigned>(c));
+/* The kHeads largest of NV keys, descending (0 where there are fewer). */
+template <int NV> __device__ __forceinline__ void best_keys(const unsigned *key, unsigned (&head)[kHeads]) {
+    if constexpr (NV > 4) {
+        unsigned other[kHeads];
+        best_keys<NV / 2>(key, head);
+        best_keys<NV / 2>(key + NV / 2, other);
+        /* the larger of each pair of a descending and an ascending run is bitonic */
+#pragma unroll
+        for (int i = 0; i < 4; ++i) head[i] = max(head[i], other[3 - i]);
+#pragma unroll
+        for (int o = 2; o > 0; o /= 2)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!(i & o)) {
+                    const unsigned high = max(head[i], head[i + o]);
+                    head[i + o] = min(head[i], head[i + o]);
+                    head[i] = high;
+                }
+    } else {
+        constexpr int from[5] = {0, 2, 0, 1, 1}, to[5] = {1, 3, 2, 3, 2};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) head[i] = i < NV ? key[i] : 0u;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const unsigned high = max(head[from[i]], head[to[i]]);
+            head[to[i]] = min(head[from[i]], head[to[i]]);
+            head[from[i]] = high;
+        }
+    }
 }
 
 /* Leaves in value[] what the token's chosen groups hold, kNone elsewhere.  A
@@ -141,18 +197,19 @@ __device__ __forceinline__ void keep_groups(const RouteShape &d, float (&value)[
 }
 
 /* One warp per token.  count: [tiles, experts] where the slots are listed by
- * tiles, or NULL. */
-template <class T, int NV>
-__global__ void __launch_bounds__(kThreads, NV <= 8 ? 4 : 1)
+ * tiles, or NULL.  TAGGED: 16-bit logits rank by themselves, without groups. */
+template <class T, int NV, bool TAGGED>
+__global__ void __launch_bounds__(select_threads(NV), 1)
 route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float *bias, int32_t *ids, float *weights,
              int32_t *count) {
-    extern __shared__ float rows[]; /* of experts + groups a warp, where they are needed */
-    __shared__ unsigned long long gathered[kWarps][32];
-    __shared__ unsigned keys[kWarps][NV][32];
+    /* a warp's keys [NV][32]; then, where they are needed, rows of experts + groups a warp */
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ int hist[TB_ROUTE_MAX_EXPERTS];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, first = lane * NV;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, first = lane * NV, warps = blockDim.x / 32;
+    unsigned *const keys = reinterpret_cast<unsigned *>(dynamic) + warp * NV * 32;
+    float *const rows = reinterpret_cast<float *>(dynamic) + warps * NV * 32 + warp * (d.experts + d.groups);
     if (count) {
-        for (int e = threadIdx.x; e < d.experts; e += kThreads) hist[e] = 0;
+        for (int e = threadIdx.x; e < d.experts; e += blockDim.x) hist[e] = 0;
         __syncthreads();
     }
     const bool soft = d.score == TB_SCORE_SOFTMAX;
@@ -162,111 +219,143 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
     for (int i = 0; i < NV; ++i) b[i] = bias && first + i < d.experts ? bias[first + i] : 0.0f;
     const size_t begin = static_cast<size_t>(blockIdx.x) * per_cta;
     const size_t end = begin + per_cta < d.tokens ? begin + per_cta : d.tokens;
+    int lanes = 1; /* that slots take */
+    while (lanes < d.top_k) lanes *= 2;
     Logits<T, NV> next;
     if (begin + warp < end) next.load(logits + (begin + warp) * d.stride, first, d.experts, packs);
-    for (size_t t = begin + warp; t < end; t += kWarps) {
+    for (size_t t = begin + warp; t < end; t += warps) {
         const T *const in = logits + t * d.stride;
-        float value[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) value[i] = next[i];
-        if (t + kWarps < end) next.load(in + kWarps * d.stride, first, d.experts, packs);
-        if (scored || soft) /* elsewhere the keys see to it */
-#pragma unroll
-            for (int i = 0; i < NV; ++i) value[i] = available(value[i]);
         float most = 0.0f, sum = 1.0f;
-        if (soft && (scored || !d.renormalise)) { /* else only the selected logits matter */
-            most = kNone;
+        unsigned key[NV], head[kHeads];
+        const Logits<T, NV> now = next;
+        if (t + warps < end) next.load(in + warps * d.stride, first, d.experts, packs);
+        if constexpr (TAGGED) {
+            if (soft && !d.renormalise) {
+                most = kNone;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) most = fmaxf(most, value[i]);
-            most = warp_max(most);
-            sum = 0.0f;
+                for (int i = 0; i < NV; ++i) most = fmaxf(most, available(to_float(now[i])));
+                most = warp_max(most);
+                sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) sum += value[i] == kNone ? 0.0f : softened(value[i], most);
-            sum = warp_sum(sum);
-        }
-        if (scored || d.groups > 1) {
-            float l[NV];
+                for (int i = 0; i < NV; ++i) {
+                    const float v = available(to_float(now[i]));
+                    sum += v == kNone ? 0.0f : softened(v, most);
+                }
+                sum = warp_sum(sum);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) key[i] = tagged_key(now[i], first + i);
+        } else {
+            float value[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) value[i] = available(to_float(now[i]));
+            if (soft && (scored || !d.renormalise)) { /* else only the selected logits matter */
+                most = kNone;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) most = fmaxf(most, value[i]);
+                most = warp_max(most);
+                sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) sum += value[i] == kNone ? 0.0f : softened(value[i], most);
+                sum = warp_sum(sum);
+            }
+            if (scored || d.groups > 1) {
+                float l[NV];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    l[i] = value[i];
+                    if (scored && l[i] != kNone)
+                        value[i] = (soft ? softened(l[i], most) / sum : sigmoid(l[i])) + b[i];
+                }
+                if (d.groups > 1) {
+                    keep_groups<NV>(d, value, rows, lane);
+                    if (scored && !bias)
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) value[i] = value[i] == kNone ? kNone : l[i];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                l[i] = value[i];
-                if (scored && l[i] != kNone)
-                    value[i] = (soft ? softened(l[i], most) / sum : sigmoid(l[i])) + b[i];
-            }
-            if (d.groups > 1) {
-                keep_groups<NV>(d, value, rows + warp * (d.experts + d.groups), lane);
-                if (scored && !bias)
-#pragma unroll
-                    for (int i = 0; i < NV; ++i) value[i] = value[i] == kNone ? kNone : l[i];
+                key[i] = key_of(value[i]);
+                keys[i * 32 + lane] = key[i];
             }
         }
-        unsigned key[NV], top = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            key[i] = key_of(value[i]);
-            top = max(top, key[i]);
-            keys[warp][i][lane] = key[i];
-        }
-        /* at most the top_k-th largest of the lanes' maxima: equal ones go together */
-        for (int j = 1; j < d.top_k; ++j)
-            if (top == __reduce_max_sync(0xffffffffu, top)) top = 0;
-        const unsigned least = max(__reduce_max_sync(0xffffffffu, top), 1u);
-        unsigned over = 0; /* the lane's that reach it */
-#pragma unroll
-        for (int i = 0; i < NV; ++i) over |= static_cast<unsigned>(key[i] >= least) << i;
-        __syncwarp();
-        int found = 0;
-        for (unsigned have; (have = __ballot_sync(0xffffffffu, over)) != 0; over &= over - 1) {
-            const int to = found + __popc(have & ((1u << lane) - 1));
-            if (over && to < 32) {
-                const int i = __ffs(over) - 1;
-                gathered[warp][to] = candidate(keys[warp][i][lane], first + i);
+        best_keys<NV>(key, head);
+        unsigned mine = 0; /* lane j's: the j-th best key, and its lane */
+        int from = 0, given = 0, expert = -1;
+        for (int j = 0; j < d.top_k; ++j) {
+            const unsigned best = __reduce_max_sync(0xffffffffu, head[0]);
+            bool wins = head[0] == best;
+            if constexpr (!TAGGED) { /* of equal ones the first lane */
+                const int winner = __ffs(__ballot_sync(0xffffffffu, wins)) - 1;
+                if (lane == j) from = winner;
+                wins = lane == winner;
             }
-            found += __popc(have);
+            if (lane == j) mine = best;
+            if (wins) {
+                head[0] = head[1];
+                head[1] = head[2];
+                head[2] = head[3];
+                head[3] = 0;
+                ++given;
+            }
         }
-        __syncwarp();
-        int slot, expert = -1; /* of this lane's candidate */
-        if (found <= 32) {
-            const unsigned long long mine = lane < found ? gathered[warp][lane] : 0ull;
-            if (lane < found) expert = expert_of(mine);
-            slot = 0;
-#pragma unroll 4
-            for (int c = 0; c < found; ++c) slot += gathered[warp][c] > mine;
-            if (lane >= found) slot = lane; /* an empty slot, if it is one */
-        } else {
-            for (int j = 0; j < d.top_k; ++j) { /* lane j takes the j-th best */
+        /* a lane that gave all its heads: its fifth may belong */
+        if (NV > kHeads && __any_sync(0xffffffffu, given == kHeads)) {
+            mine = 0;
+            for (int j = 0; j < d.top_k; ++j) {
                 unsigned best = 0;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) best = max(best, key[i]);
                 const unsigned all = __reduce_max_sync(0xffffffffu, best);
-                const int from = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
-                int at = 0;
+                if (all == 0) break;
+                const int winner = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
+                int at = NV;
 #pragma unroll
                 for (int i = NV - 1; i >= 0; --i)
-                    if (key[i] == all) at = first + i;
-                at = __shfl_sync(0xffffffffu, at, from);
+                    if (key[i] == all) at = i;
+                at = __shfl_sync(0xffffffffu, at, winner);
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (first + i == at) key[i] = 0;
-                if (lane == j) expert = at;
+                    if (i == at && lane == winner) key[i] = 0;
+                if (lane == j) mine = all, expert = winner * NV + at;
             }
-            slot = lane;
+        } else if constexpr (TAGGED) {
+            if (mine != 0) expert = static_cast<int>(0xffffu - (mine & 0xffffu));
+        } else {
+            /* equal keys of one lane go to its experts in order */
+            __syncwarp();
+            const unsigned equal = __match_any_sync(0xffffffffu, mine) & ((1u << lane) - 1);
+            int skip = 0;
+            if (__any_sync(0xffffffffu, mine != 0 && equal != 0))
+                for (int j = 0; j < d.top_k; ++j) {
+                    const int other = __shfl_sync(0xffffffffu, from, j);
+                    skip += (equal >> j & 1) && other == from;
+                }
+            if (mine != 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (keys[i * 32 + from] == mine && skip-- == 0) expert = from * NV + i;
+            }
         }
-        const bool takes = expert >= 0 && slot < d.top_k;
-        const float l = takes ? to_float(in[expert]) : kNone;
+        const bool takes = expert >= 0;
+        float l = kNone;
+        if (takes) l = TAGGED ? tagged_value<T>(mine) : scored ? to_float(in[expert]) : value_of(mine);
         float score;
         if (soft) {
-            if (!scored && d.renormalise) most = warp_max(l);
-            score = takes ? softened(l, most) / sum : 0.0f;
+            if (!scored && d.renormalise) most = __shfl_sync(0xffffffffu, l, 0); /* the best comes first */
+            score = takes ? __fdividef(softened(l, most), sum) : 0.0f;
         } else {
             score = takes ? sigmoid(l) : 0.0f;
         }
         if (d.renormalise) {
-            const float total = warp_sum(score);
-            score = total > 0.0f ? score / total : 0.0f;
+            float total = score;
+            for (int o = lanes / 2; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+            score = total > 0.0f ? __fdividef(score, total) : 0.0f;
         }
-        if (slot < d.top_k) {
-            ids[t * d.top_k + slot] = expert;
-            weights[t * d.top_k + slot] = score * d.scale;
+        if (lane < d.top_k) {
+            ids[t * d.top_k + lane] = expert;
+            weights[t * d.top_k + lane] = score * d.scale;
         }
         if (count && takes) atomicAdd(&hist[expert], 1);
         __syncwarp();
@@ -277,76 +366,65 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
     }
 }
 
-/* 32 experts a CTA: turns each tile's counts into those of the tiles before it; total [experts]. */
-__global__ void __launch_bounds__(1024) route_prefix(int tiles, int experts, int32_t *count, int32_t *total) {
-    __shared__ int sums[32][33];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
-    const int each = (tiles + 31) / 32, first = warp * each, last = min(first + each, tiles);
-    int s = 0;
-    if (e < experts)
-#pragma unroll 16
-        for (int b = first; b < last; ++b) s += count[static_cast<size_t>(b) * experts + e];
-    sums[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0) {
-        int before = 0;
-#pragma unroll
-        for (int w = 0; w < 32; ++w) {
-            const int c = sums[w][lane];
-            sums[w][lane] = before;
-            before += c;
-        }
-        if (e < experts) total[e] = before;
-    }
-    __syncthreads();
-    s = sums[warp][lane];
-    if (e < experts)
-#pragma unroll 8
-        for (int b = first; b < last; ++b) {
-            const int c = count[static_cast<size_t>(b) * experts + e];
-            count[static_cast<size_t>(b) * experts + e] = s;
-            s += c;
-        }
-}
-
 /* Places the slots of a tile of tokens (ALONE: of all tokens).  Each warp takes
  * consecutive slots; next[warp][expert] is where its next slot of the expert
  * goes. */
 template <bool ALONE>
-__global__ void __launch_bounds__(kThreads)
-route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *count, const int32_t *total, int32_t *offsets, int32_t *order,
+__global__ void __launch_bounds__(kPlaceThreads)
+route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *count, int32_t *offsets, int32_t *order,
             int32_t *position) {
-    extern __shared__ int next[]; /* [kWarps][experts], then first[experts] */
-    __shared__ int part[kWarps];
-    int *const first = next + kWarps * d.experts;
+    /* next [kPlaceWarps][experts]; of all tiles and of those before [kPlaceWarps][experts] each; first [experts] */
+    extern __shared__ int next[];
+    __shared__ int part[kPlaceWarps];
+    int *const all_of = next + kPlaceWarps * d.experts, *const before_of = all_of + (ALONE ? 0 : kPlaceWarps * d.experts);
+    int *const first = before_of + (ALONE ? 0 : kPlaceWarps * d.experts);
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const size_t slots = d.tokens * d.top_k;
     const size_t own_slots = ALONE ? slots : static_cast<size_t>(tile_tokens) * d.top_k;
     const size_t begin = blockIdx.x * own_slots, end = begin + own_slots < slots ? begin + own_slots : slots;
-    const size_t each = (end - begin + kThreads - 1) / kThreads * 32; /* of a warp, whole rows of lanes */
+    const size_t each = (end - begin + kPlaceThreads - 1) / kPlaceThreads * 32; /* of a warp, whole rows of lanes */
     const size_t from = begin + warp * each, to = from + each < end ? from + each : end;
     int *const own = next + warp * d.experts;
-    for (int i = threadIdx.x; i < kWarps * d.experts; i += kThreads) next[i] = 0;
-    __syncthreads();
-    for (size_t base = from; base < to; base += 32) {
-        const int e = base + lane < to ? ids[base + lane] : -1;
+    for (int e = lane; e < d.experts; e += 32) own[e] = 0;
+    if (!ALONE) { /* every kPlaceWarps-th tile a warp */
+        const int tile = static_cast<int>(blockIdx.x), tiles = static_cast<int>(gridDim.x);
+        for (int e = lane; e < d.experts; e += 32) {
+            int all = 0, before = 0;
+#pragma unroll
+            for (int i = 0; i < (kMostTiles + kPlaceWarps - 1) / kPlaceWarps; ++i) { /* all under way at once */
+                const int b = warp + i * kPlaceWarps;
+                const int c = b < tiles ? count[static_cast<size_t>(b) * d.experts + e] : 0;
+                all += c;
+                before += b < tile ? c : 0;
+            }
+            all_of[warp * d.experts + e] = all;
+            before_of[warp * d.experts + e] = before;
+        }
+    }
+    __syncwarp();
+    int held[kHeld]; /* the warp's first rows of slots: most often all */
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) held[r] = from + r * 32 + lane < to ? ids[from + r * 32 + lane] : -1;
+    const auto expert_at = [&](size_t base) { return base + lane < to ? ids[base + lane] : -1; };
+    const auto count_row = [&](int e) {
         const unsigned peers = __match_any_sync(0xffffffffu, e);
         if (e >= 0 && lane == __ffs(peers) - 1) own[e] += __popc(peers);
         __syncwarp();
-    }
+    };
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+        if (from + r * 32 < to) count_row(held[r]);
+    for (size_t base = from + kHeld * 32; base < to; base += 32) count_row(expert_at(base));
     __syncthreads();
     /* totals of the experts, then the experts before each: runs of experts a thread */
-    const int run = (d.experts + kThreads - 1) / kThreads, mine = threadIdx.x * run;
+    const int run = (d.experts + kPlaceThreads - 1) / kPlaceThreads, mine = threadIdx.x * run;
     int sum = 0;
     for (int i = 0; i < run; ++i) {
         const int e = mine + i;
         if (e >= d.experts) break;
         int c = 0;
-        if (ALONE) {
-            for (int w = 0; w < kWarps; ++w) c += next[w * d.experts + e];
-        } else {
-            c = total[e];
-        }
+#pragma unroll
+        for (int w = 0; w < kPlaceWarps; ++w) c += (ALONE ? next : all_of)[w * d.experts + e];
         first[e] = sum;
         sum += c;
     }
@@ -361,7 +439,7 @@ route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *co
     before -= sum;
     int all = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kPlaceWarps; ++w) {
         if (w == warp) before += all;
         all += part[w];
     }
@@ -370,8 +448,11 @@ route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *co
         if (e >= d.experts) break;
         int at = first[e] + before;
         if (blockIdx.x == 0) offsets[e] = at;
-        if (!ALONE) at += count[static_cast<size_t>(blockIdx.x) * d.experts + e];
-        for (int w = 0; w < kWarps; ++w) {
+        if (!ALONE)
+#pragma unroll
+            for (int w = 0; w < kPlaceWarps; ++w) at += before_of[w * d.experts + e];
+#pragma unroll
+        for (int w = 0; w < kPlaceWarps; ++w) {
             const int c = next[w * d.experts + e];
             next[w * d.experts + e] = at;
             at += c;
@@ -379,9 +460,8 @@ route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *co
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[d.experts] = all;
     __syncthreads();
-    for (size_t base = from; base < to; base += 32) {
+    const auto place_row = [&](size_t base, int e) {
         const size_t i = base + lane;
-        const int e = i < to ? ids[i] : -1;
         const unsigned peers = __match_any_sync(0xffffffffu, e);
         const int rank = __popc(peers & ((1u << lane) - 1));
         const int place = e >= 0 ? own[e] + rank : -1;
@@ -390,9 +470,13 @@ route_place(RouteShape d, int tile_tokens, const int32_t *ids, const int32_t *co
         __syncwarp();
         if (e >= 0) order[place] = static_cast<int32_t>(i);
         if (i < to) position[i] = place;
-    }
-    for (size_t i = all + static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; i < slots;
-         i += static_cast<size_t>(gridDim.x) * kThreads)
+    };
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+        if (from + r * 32 < to) place_row(from + r * 32, held[r]);
+    for (size_t base = from + kHeld * 32; base < to; base += 32) place_row(base, expert_at(base));
+    for (size_t i = all + static_cast<size_t>(blockIdx.x) * kPlaceThreads + threadIdx.x; i < slots;
+         i += static_cast<size_t>(gridDim.x) * kPlaceThreads)
         order[i] = -1;
 }
 
@@ -528,9 +612,9 @@ bool route_shape(const tb_expert_route_desc *d, RouteShape *s) {
     return true;
 }
 
-/* Tokens of a tile: whole rounds of a CTA's warps. */
 int tile_tokens(const RouteShape &s) {
-    return static_cast<int>(align_up((s.tokens + kMostTiles - 1) / kMostTiles, kWarps));
+    const size_t each = (s.tokens + kMostTiles - 1) / kMostTiles;
+    return static_cast<int>(each < kLeastTile ? kLeastTile : each);
 }
 int route_tiles(const RouteShape &s) {
     const int each = tile_tokens(s);
@@ -547,11 +631,21 @@ template <class T> bool route_packs(const RouteShape &s, const void *a, const vo
 template <class T, int NV>
 int launch_select(const RouteShape &s, const T *logits, const float *bias, int32_t *ids, float *weights, int32_t *count,
                   cudaStream_t st) {
+    /* tiles: as wide as an SM takes; else one token a warp, on many SMs */
     const int per_cta = count ? tile_tokens(s) : kWarps;
-    const size_t shared = s.groups > 1 ? kWarps * (s.experts + s.groups) * sizeof(float) : 0;
-    if (!allow_shared<route_select<T, NV>>(shared)) return 0;
-    route_select<T, NV><<<static_cast<unsigned>((s.tokens + per_cta - 1) / per_cta), kThreads, shared, st>>>(
-        s, per_cta, route_packs<T>(s, logits, nullptr), logits, bias, ids, weights, count);
+    int threads = count ? select_threads(NV) : kThreads;
+    while (threads > kThreads && threads / 32 >= 2 * per_cta) threads /= 2;
+    const int warps = threads / 32;
+    const size_t shared = (static_cast<size_t>(warps) * NV * 32 + (s.groups > 1 ? warps * (s.experts + s.groups) : 0)) * 4;
+    const unsigned grid = static_cast<unsigned>((s.tokens + per_cta - 1) / per_cta);
+    const bool packs = route_packs<T>(s, logits, nullptr);
+    if constexpr (sizeof(T) == 2)
+        if (!bias && s.groups == 1) {
+            route_select<T, NV, true><<<grid, threads, 0, st>>>(s, per_cta, packs, logits, bias, ids, weights, count);
+            return launched();
+        }
+    if (!allow_shared<route_select<T, NV, false>>(shared)) return 0;
+    route_select<T, NV, false><<<grid, threads, shared, st>>>(s, per_cta, packs, logits, bias, ids, weights, count);
     return launched();
 }
 
@@ -560,7 +654,7 @@ int launch_select(const RouteShape &s, const T *logits, const float *bias, int32
 extern "C" size_t tb_cuda_route_experts_workspace(const tb_expert_route_desc *desc) {
     RouteShape s;
     if (!route_shape(desc, &s)) return 0;
-    return (static_cast<size_t>(route_tiles(s)) + 1) * s.experts * sizeof(int32_t);
+    return static_cast<size_t>(route_tiles(s)) * s.experts * sizeof(int32_t);
 }
 
 extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, const void *logits, const float *bias,
@@ -589,16 +683,15 @@ extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, co
         return launch_select<T, 32>(s, in, bias, ids, weights, to, st);
     });
     if (!ok || !offsets) return ok;
-    const size_t shared = (kWarps + 1) * s.experts * sizeof(int);
+    const size_t shared = ((alone ? 1 : 3) * kPlaceWarps + 1) * s.experts * sizeof(int);
     if (alone) {
-        route_place<true><<<1, kThreads, shared, st>>>(s, 0, ids, nullptr, nullptr, offsets, order, position);
-        return launched();
+        if (!allow_shared<route_place<true>>(shared)) return 0;
+        route_place<true><<<1, kPlaceThreads, shared, st>>>(s, 0, ids, nullptr, offsets, order, position);
+    } else {
+        if (!allow_shared<route_place<false>>(shared)) return 0;
+        route_place<false><<<route_tiles(s), kPlaceThreads, shared, st>>>(s, tile_tokens(s), ids, count, offsets, order,
+                                                                         position);
     }
-    const int tiles = route_tiles(s);
-    int32_t *total = count + static_cast<size_t>(tiles) * s.experts;
-    route_prefix<<<(s.experts + 31) / 32, 1024, 0, st>>>(tiles, s.experts, count, total);
-    if (!launched()) return 0;
-    route_place<false><<<tiles, kThreads, shared, st>>>(s, tile_tokens(s), ids, count, total, offsets, order, position);
     return launched();
 }
 
