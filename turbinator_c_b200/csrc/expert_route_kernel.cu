@@ -288,17 +288,14 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
             bool wins = head[0] == best;
             if constexpr (!TAGGED) { /* of equal ones the first lane */
                 const int winner = __ffs(__ballot_sync(0xffffffffu, wins)) - 1;
-                if (lane == j) from = winner;
+                from = lane == j ? winner : from;
                 wins = lane == winner;
             }
-            if (lane == j) mine = best;
-            if (wins) {
-                head[0] = head[1];
-                head[1] = head[2];
-                head[2] = head[3];
-                head[3] = 0;
-                ++given;
-            }
+            mine = lane == j ? best : mine;
+#pragma unroll
+            for (int i = 0; i + 1 < kHeads; ++i) head[i] = wins ? head[i + 1] : head[i];
+            head[kHeads - 1] = wins ? 0u : head[kHeads - 1];
+            given += wins;
         }
         /* a lane that gave all its heads: its fifth may belong */
         if (NV > kHeads && __any_sync(0xffffffffu, given == kHeads)) {
