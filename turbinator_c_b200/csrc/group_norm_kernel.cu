@@ -46,6 +46,7 @@ struct Tiling {
     int blocks, threads, rows_at_once;
     int rows, parts;         /* positions of a part */
     int rows_held;           /* positions that the tile has room for */
+    int share;               /* threads that add up a channel's total: a power of two */
     unsigned magic_parts, magic_blocks, magic_lanes, magic_rows, magic_group; /* floor((2^32 - 1) / ..), rows: rows_at_once */
     bool fits;               /* the parts fit one cluster */
     size_t tiles;            /* of all samples */
@@ -209,61 +210,63 @@ template <class T, int PACK> __device__ __forceinline__ void put(T *to, const Ar
 
 /* ---- sums over a tile ---- */
 
-/* Shared memory of a tile: the tile (x, then dy), rows of per-channel partial
- * sums (pitch channels + 4), channel totals, and per group four values. */
+/* Shared memory of a tile: rows of per-channel partial sums, of N values a
+ * channel, their totals, backward the channels' scale, per group four values,
+ * and the tile (x, then dy). */
 struct Sums {
-    float *rows, *channel, *group;
+    float *rows, *channel, *scale, *group;
     unsigned char *tile;
-    int pitch;
+    int channels, pitch; /* channels of a row, to whole 16 bytes; of N rows of them and a shift of banks */
 };
-__device__ __forceinline__ Sums sums_of(float *shared, const NormShape &d, const Tiling &g) {
+template <int N> __device__ __forceinline__ Sums sums_of(float *shared, const Tiling &g) {
     Sums s;
-    const int channels = g.lanes * g.pack;
-    s.pitch = ((channels + 3) & ~3) + 4;
+    s.channels = (g.lanes * g.pack + 3) & ~3;
+    s.pitch = N * s.channels + 4;
     s.rows = shared;
     s.channel = shared + g.rows_at_once * s.pitch;
-    s.group = s.channel + 2 * ((channels + 3) & ~3);
+    s.scale = s.channel + N * s.channels;
+    s.group = s.scale + (N > 1 ? s.channels : 0);
     s.tile = reinterpret_cast<unsigned char *>(s.group + 4 * g.block_groups);
     return s;
 }
-size_t shared_bytes(const Tiling &g, size_t size, int tensors) {
+/* n: 1 forward, 2 backward, of tensors as of values. */
+size_t shared_bytes(const Tiling &g, size_t size, int n) {
     const size_t channels = (static_cast<size_t>(g.lanes) * g.pack + 3) & ~size_t(3);
-    return (g.rows_at_once * (channels + 4) + 2 * channels + 4 * g.block_groups) * sizeof(float) +
-           static_cast<size_t>(tensors) * g.rows_held * g.lanes * g.pack * size;
+    return (g.rows_at_once * (n * channels + 4) + (n > 1 ? n + 1 : n) * channels + 4 * g.block_groups) * sizeof(float) +
+           static_cast<size_t>(n) * g.rows_held * g.lanes * g.pack * size;
 }
 
-/* channel[c] = the sum over the CTA's rows of each thread's own values; ends
- * with the totals visible to all. */
-template <int PACK>
-__device__ __forceinline__ void channel_totals(const Array<PACK> &sums, float *channel, const Sums &s, const Seat &at,
-                                               const Tiling &g) {
+/* channel[i * s.channels + c] = the sum over the CTA's rows of each thread's
+ * own[i]; ends with the totals visible to all. */
+template <int PACK, int N>
+__device__ __forceinline__ void channel_totals(const Array<PACK> (&own)[N], const Sums &s, const Seat &at, const Tiling &g) {
     if (at.in) {
-        float own[PACK];
 #pragma unroll
-        for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(own + 2 * k, sums[k]);
-        float *to = s.rows + at.row * s.pitch + at.lane * PACK;
-        if constexpr (PACK % 4 == 0) {
+        for (int i = 0; i < N; ++i) {
+            float e[PACK];
 #pragma unroll
-            for (int v = 0; v < PACK; v += 4)
-                *reinterpret_cast<float4 *>(to + v) = make_float4(own[v], own[v + 1], own[v + 2], own[v + 3]);
-        } else {
+            for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(e + 2 * k, own[i][k]);
+            float *to = s.rows + at.row * s.pitch + i * s.channels + at.lane * PACK;
+            if constexpr (PACK % 4 == 0) {
 #pragma unroll
-            for (int v = 0; v < PACK; ++v) to[v] = own[v];
+                for (int v = 0; v < PACK; v += 4)
+                    *reinterpret_cast<float4 *>(to + v) = make_float4(e[v], e[v + 1], e[v + 2], e[v + 3]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < PACK; ++v) to[v] = e[v];
+            }
         }
     }
     __syncthreads();
-    /* `share` neighbouring threads for each channel */
-    const int channels = at.channels;
-    int share = 1;
-    while (share < 32 && share * 2 * channels <= static_cast<int>(blockDim.x)) share *= 2;
-    const int mine = threadIdx.x % share;
-    for (int base = 0; base < channels; base += blockDim.x / share) {
-        const int c = base + threadIdx.x / share;
+    /* g.share neighbouring threads for each total */
+    const int mine = threadIdx.x & (g.share - 1);
+    for (int c = threadIdx.x / g.share; c < N * s.channels; c += blockDim.x / g.share) {
         float t = 0.0f;
-        if (c < channels)
-            for (int r = mine; r < g.rows_at_once; r += share) t += s.rows[r * s.pitch + c];
-        for (int o = 1; o < share; o *= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (c < channels && mine == 0) channel[c] = t;
+#pragma unroll 4
+        for (int r = mine; r < g.rows_at_once; r += g.share) t += s.rows[r * s.pitch + c];
+        /* whole warps are here: blockDim.x / share divides by 32 / share, and channels by 4 */
+        for (int o = 1; o < g.share; o *= 2) t += __shfl_xor_sync(__activemask(), t, o);
+        if (mine == 0) s.channel[c] = t;
     }
     __syncthreads();
 }
@@ -296,32 +299,32 @@ __device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int s
                                                 const NormShape &d, const Tiling &g) {
     using V = typename Values<PACK>::V;
     constexpr int N = Values<PACK>::kCount;
-    Array<PACK> own, e;
+    Array<PACK> own[1], e;
 #pragma unroll
-    for (int k = 0; k < N; ++k) own[k] = vall<V>(0.0f);
+    for (int k = 0; k < N; ++k) own[0][k] = vall<V>(0.0f);
 #pragma unroll 4
     for (int i = 0; i < at.mine; ++i) {
         taken<T, PACK>(tile[i * step], e);
 #pragma unroll
-        for (int k = 0; k < N; ++k) own[k] = vadd(own[k], e[k]);
+        for (int k = 0; k < N; ++k) own[0][k] = vadd(own[0][k], e[k]);
     }
-    channel_totals<PACK>(own, s.channel, s, at, g);
+    channel_totals<PACK, 1>(own, s, at, g);
     const float count = static_cast<float>(at.rows) * static_cast<float>(d.per_group);
     group_totals(d, at, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i] = t / count; });
     __syncthreads();
     const Channels<PACK> less = by_group<PACK>(at, d, g, [&](int i) { return -s.group[2 * i]; });
 #pragma unroll
-    for (int k = 0; k < N; ++k) own[k] = vall<V>(0.0f);
+    for (int k = 0; k < N; ++k) own[0][k] = vall<V>(0.0f);
 #pragma unroll 4
     for (int i = 0; i < at.mine; ++i) {
         taken<T, PACK>(tile[i * step], e);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const V off = vadd(e[k], less.v[k]);
-            own[k] = vfma(off, off, own[k]);
+            own[0][k] = vfma(off, off, own[0][k]);
         }
     }
-    channel_totals<PACK>(own, s.channel, s, at, g);
+    channel_totals<PACK, 1>(own, s, at, g);
     group_totals(d, at, [&](int c) { return s.channel[c]; }, [&](int i, float t) { s.group[2 * i + 1] = t; });
     __syncthreads();
 }
@@ -346,7 +349,7 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
                    float *rstd_out, float *partial) {
     extern __shared__ __align__(16) float shared[];
     const Seat at = seat_of(d, g, blockIdx.x);
-    const Sums s = sums_of(shared, d, g);
+    const Sums s = sums_of<1>(shared, g);
     Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
     const int step = g.rows_at_once * g.lanes;
     load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
@@ -500,16 +503,17 @@ __device__ __forceinline__ void gradients(Array<PACK> &x, Array<PACK> &dy, const
     for (int k = 0; k < Values<PACK>::kCount; ++k) dy[k] = vmul(dy[k], u[k]);
 }
 /* With hat = z rstd and m1, m2 the group's means of du gamma and du gamma hat:
- * dx = rstd (du gamma - m1 - hat m2) = du scale + n1 + z n2. */
+ * dx = rstd (du gamma - m1 - hat m2) = du scale + n1 + z n2.  The tiles sum du
+ * scale and du scale z, so with their means M1 = rstd m1 and M2 = m2. */
 template <int PACK> struct Less {
-    Channels<PACK> n1, n2; /* -rstd m1, -rstd^2 m2 */
+    Channels<PACK> n1, n2; /* -M1, -rstd^2 M2 */
 };
 template <int PACK>
 __device__ __forceinline__ Less<PACK> less_of(const NormShape &d, const Tiling &g, const Seat &at, const float *rstd,
                                               const float *means) {
     const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     Less<PACK> f;
-    f.n1 = by_group<PACK>(at, d, g, [&](int i) { return -rstd[first + i] * means[2 * i]; });
+    f.n1 = by_group<PACK>(at, d, g, [&](int i) { return -means[2 * i]; });
     f.n2 = by_group<PACK>(at, d, g, [&](int i) { return -rstd[first + i] * rstd[first + i] * means[2 * i + 1]; });
     return f;
 }
@@ -532,18 +536,21 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
     constexpr int N = Values<PACK>::kCount;
     extern __shared__ __align__(16) float shared[];
     const Seat at = seat_of(d, g, blockIdx.x);
-    const Sums s = sums_of(shared, d, g);
+    const Sums s = sums_of<2>(shared, g);
     const int step = g.rows_at_once * g.lanes;
     Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
     Held<T, PACK> *const tile_dy = tile + g.rows_held * g.lanes;
     load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
     load_tile<T, PACK>(tile_dy, step, dy + at.n * d.ys, d.yp, at, g);
     const Given<PACK> f = given_of<PACK>(d, g, at, gamma, beta, mean, rstd);
+    if (at.in && at.row == 0) /* for the groups' sums */
+#pragma unroll
+        for (int k = 0; k < N; ++k) vstore(s.scale + at.lane * PACK + 2 * k, f.scale.v[k]);
     tile_loaded();
     {
-        Array<PACK> a, b;
+        Array<PACK> own[2]; /* sums of du and of du z */
 #pragma unroll
-        for (int k = 0; k < N; ++k) a[k] = b[k] = vall<V>(0.0f);
+        for (int k = 0; k < N; ++k) own[0][k] = own[1][k] = vall<V>(0.0f);
 #pragma unroll 2
         for (int i = 0; i < at.mine; ++i) {
             Array<PACK> z, du;
@@ -552,28 +559,23 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
             gradients<PACK>(z, du, f, d.act);
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                a[k] = vadd(a[k], du[k]);
-                b[k] = vfma(du[k], z[k], b[k]);
+                own[0][k] = vadd(own[0][k], du[k]);
+                own[1][k] = vfma(du[k], z[k], own[1][k]);
             }
         }
-        float *const second = s.channel + ((g.lanes * PACK + 3) & ~3);
-        const float *r = rstd + static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
-        const Channels<PACK> scale = by_group<PACK>(at, d, g, [&](int i) { return r[i]; });
-#pragma unroll
-        for (int k = 0; k < N; ++k) b[k] = vmul(b[k], scale.v[k]); /* of du z: of du hat */
-        channel_totals<PACK>(a, s.channel, s, at, g);
-        channel_totals<PACK>(b, second, s, at, g);
-        const auto weighted = [&](const float *t) { return [=](int c) { return t[c] * (gamma ? gamma[at.c0 + c] : 1.0f); }; };
-        group_totals(d, at, weighted(s.channel), [&](int i, float t) { s.group[2 * i] = t; });
-        group_totals(d, at, weighted(second), [&](int i, float t) { s.group[2 * i + 1] = t; });
+        channel_totals<PACK, 2>(own, s, at, g);
+        /* scale = rstd gamma: these are rstd times the sums of du gamma and du gamma z */
+        const float *second = s.channel + s.channels;
+        group_totals(d, at, [&](int c) { return s.channel[c] * s.scale[c]; }, [&](int i, float t) { s.group[2 * i] = t; });
+        group_totals(d, at, [&](int c) { return second[c] * s.scale[c]; }, [&](int i, float t) { s.group[2 * i + 1] = t; });
         __syncthreads();
     }
-    const int second = (g.lanes * PACK + 3) & ~3;
+    const float *const rstd_of = rstd + static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     if (partial) {
         float *to = partial + (static_cast<size_t>(at.n) * g.parts + at.part) * 2 * d.channels + at.c0;
         for (int c = threadIdx.x; c < at.channels; c += blockDim.x) {
             to[c] = s.channel[c];
-            to[d.channels + c] = s.channel[second + c];
+            to[d.channels + c] = s.channel[s.channels + c] * rstd_of[group_of(c, d, g)]; /* of du hat */
         }
     }
     if constexpr (!WHOLE) {
@@ -839,6 +841,8 @@ bool tiling_of(const NormShape &d, int pack, size_t size, Tiling *g) {
         if (g->fits) break;
     }
     g->tiles = d.samples * g->blocks * g->parts;
+    g->share = 1;
+    while (g->share < 32 && g->share * 2 * g->lanes * pack <= g->threads) g->share *= 2;
     const auto magic = [](unsigned by) { return static_cast<unsigned>(0xffffffffull / by); };
     g->magic_parts = magic(g->parts);
     g->magic_blocks = magic(g->blocks);
