@@ -422,9 +422,11 @@ norm_merge(NormShape d, Tiling g, const float *partial, float *mean_out, float *
         return static_cast<float>(r + 1 < g.parts ? g.rows : static_cast<int>(d.positions) - r * g.rows);
     };
     float sum = 0.0f;
+#pragma unroll 8
     for (int r = lane; r < g.parts; r += 32) sum += rows(r) * p[r * pitch];
     const float mean = warp_sum(sum) / static_cast<float>(d.positions);
     float squares = 0.0f;
+#pragma unroll 8
     for (int r = lane; r < g.parts; r += 32) {
         const float off = p[r * pitch] - mean;
         squares += fmaf(rows(r) * static_cast<float>(d.per_group) * off, off, p[r * pitch + 1]);
@@ -441,7 +443,7 @@ constexpr int kAhead = 4;
 
 /* The result from given statistics. */
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 8)
+__global__ void __launch_bounds__(kThreads, 6)
 norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                    const float *rstd, T *y) {
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
@@ -454,11 +456,19 @@ norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const 
     f.scale = times<PACK>(by_group<PACK>(at, d, g, [&](int i) { return rstd[first + i]; }),
                           parameters_of<PACK>(at, gamma, 1.0f));
     f.shift = parameters_of<PACK>(at, beta, 0.0f);
+    Held<T, PACK> next[kAhead];
+    const auto load = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (i + j < at.mine) next[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * from_jump);
+        from += kAhead * from_jump;
+    };
+    load(0);
     for (int i = 0; i < at.mine; i += kAhead) {
         Held<T, PACK> v[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-            if (i + j < at.mine) v[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * from_jump);
+        for (int j = 0; j < kAhead; ++j) v[j] = next[j];
+        load(i + kAhead);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (i + j < at.mine) {
@@ -467,7 +477,6 @@ norm_forward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const 
                 result<PACK>(e, f, d.act);
                 put<T, PACK>(to + j * to_jump, e);
             }
-        from += kAhead * from_jump;
         to += kAhead * to_jump;
     }
 }
@@ -621,6 +630,7 @@ norm_merge_sums(NormShape d, size_t parts, const float *sums, float *means) {
     const int lane = threadIdx.x % 32;
     const size_t n = at / d.groups, i = at % d.groups;
     float a = 0.0f, b = 0.0f;
+#pragma unroll 8
     for (size_t r = lane; r < parts; r += 32) {
         const float *p = sums + (n * parts + r) * 2 * d.groups + i;
         a += p[0];
