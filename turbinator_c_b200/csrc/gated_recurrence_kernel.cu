@@ -27,7 +27,8 @@ using namespace tb_learn;
 
 namespace {
 
-constexpr int kSteps = TB_RECURRENCE_CHECKPOINT; /* steps of a warp's span */
+constexpr int kSteps = TB_RECURRENCE_CHECKPOINT; /* steps of a warp's span, forward */
+constexpr int kHalf = kSteps / 2;                /* and backward */
 constexpr int kWarps = 4;                        /* warps of a CTA at most */
 
 struct RecurrenceShape {
@@ -92,10 +93,7 @@ __device__ __forceinline__ int live_of(const RecurrenceShape &d, const int32_t *
     return n < 0 ? 0 : n < steps ? n : steps;
 }
 /* Of `live` steps those of the span from step t on. */
-__device__ __forceinline__ int of_span(int live, int t) {
-    const int n = live - t;
-    return n < 0 ? 0 : n < kSteps ? n : kSteps;
-}
+template <int STEPS = kSteps> __device__ __forceinline__ int of_span(int live, int t) { return min(max(live - t, 0), STEPS); }
 
 /* e^l - 1 for -kNear <= l <= 0 from its series; the next term is below 2e-8
  * of it. */
@@ -158,75 +156,81 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() {
 }
 
 /* N tensors of the same strides, at the same place: from[n] to
- * to + n * kSteps * CT, BYTES at a time. */
-template <class T, int CT, int BYTES, int N, bool FULL>
+ * to + n * STEPS * CT, BYTES at a time. */
+template <class T, int CT, int BYTES, int N, bool FULL, int STEPS>
 __device__ __forceinline__ void load_pieces(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows,
                                             int columns, int lane) {
     constexpr int kSize = static_cast<int>(sizeof(T));
-    constexpr int kPer = CT * kSize / BYTES; /* pieces of a row, at most 32 */
-    constexpr int kRows = 32 / kPer;         /* rows at a time */
-    const int row = lane / kPer, piece = lane % kPer;
-    const int left = columns * kSize - piece * BYTES;
-    if (!FULL && left <= 0) return;
-    const int bytes = FULL || left > BYTES ? BYTES : left;
-    const size_t first = (at + row * stride) * kSize + piece * BYTES, step = stride * kSize * kRows;
-    const uint32_t t = shared_address(to + row * CT) + piece * BYTES;
+    constexpr int kPer = CT * kSize / BYTES;          /* pieces of a row */
+    constexpr int kRows = kPer < 32 ? 32 / kPer : 1;  /* rows at a time */
+    constexpr int kTurns = kPer < 32 ? 1 : kPer / 32; /* pieces of a row a lane */
+    const int row = kPer < 32 ? lane / kPer : 0;
+    const size_t step = stride * kSize * kRows;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const char *f = reinterpret_cast<const char *>(from[n]) + first;
+    for (int u = 0; u < kTurns; ++u) {
+        const int piece = lane % (kPer < 32 ? kPer : 32) + 32 * u;
+        const int left = columns * kSize - piece * BYTES;
+        if (!FULL && left <= 0) return;
+        const int bytes = FULL || left > BYTES ? BYTES : left;
+        const size_t first = (at + row * stride) * kSize + piece * BYTES;
+        const uint32_t t = shared_address(to + row * CT) + piece * BYTES;
 #pragma unroll
-        for (int r = 0; r < kSteps; r += kRows) {
-            if (FULL || row + r < rows) copy_async<BYTES>(t + (n * kSteps + r) * CT * kSize, f, bytes);
-            f += step;
+        for (int n = 0; n < N; ++n) {
+            const char *f = reinterpret_cast<const char *>(from[n]) + first;
+#pragma unroll
+            for (int r = 0; r < STEPS; r += kRows) {
+                if (FULL || row + r < rows) copy_async<BYTES>(t + (n * STEPS + r) * CT * kSize, f, bytes);
+                f += step;
+            }
+        }
         }
     }
-}
 
-/* Starts copying rows x columns elements of N tensors into [N][kSteps][CT];
- * `piece` bytes at a time (16, 4: asynchronous). */
-template <class T, int CT, int N>
-__device__ __forceinline__ void load_rows(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows, int columns,
-                                          int piece, int lane) {
-    if (piece == 16) {
-        if (rows == kSteps && columns == CT) load_pieces<T, CT, 16, N, true>(to, from, at, stride, rows, columns, lane);
-        else load_pieces<T, CT, 16, N, false>(to, from, at, stride, rows, columns, lane);
-    } else if (piece == 4) {
-        load_pieces<T, CT, 4, N, false>(to, from, at, stride, rows, columns, lane);
-    } else {
-        for (int n = 0; n < N; ++n)
+    /* Starts copying rows x columns elements of N tensors into [N][STEPS][CT];
+     * `piece` bytes at a time (16, 4: asynchronous). */
+    template <class T, int CT, int N, int STEPS = kSteps>
+    __device__ __forceinline__ void load_rows(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows, int columns,
+                                              int piece, int lane) {
+        if (piece == 16) {
+            if (rows == STEPS && columns == CT) load_pieces<T, CT, 16, N, true, STEPS>(to, from, at, stride, rows, columns, lane);
+            else load_pieces<T, CT, 16, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
+        } else if (piece == 4) {
+            load_pieces<T, CT, 4, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
+        } else {
+            for (int n = 0; n < N; ++n)
+                for (int c = lane; c < columns; c += 32)
+#pragma unroll
+                    for (int r = 0; r < STEPS; ++r)
+                        if (r < rows) to[(n * STEPS + r) * CT + c] = from[n][at + r * stride + c];
+        }
+    }
+
+    /* rows x columns elements of from [STEPS][CT] to global memory. */
+    template <class T, int CT, int STEPS = kSteps>
+    __device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
+        if (piece == 16) {
+            constexpr int kPer = CT * static_cast<int>(sizeof(T)) / 16, kRows = 32 / kPer;
+            constexpr int kIn = 16 / static_cast<int>(sizeof(T));
+            const int row = lane / kPer, c = lane % kPer * kIn;
+            const T *f = from + row * CT + c;
+            T *t = to + row * stride + c;
+            if (c + kIn <= columns) {
+#pragma unroll
+                for (int r = 0; r < STEPS; r += kRows)
+                    if (row + r < rows)
+                        *reinterpret_cast<Pack<T, kIn> *>(t + r * stride) =
+                            *reinterpret_cast<const Pack<T, kIn> *>(f + r * CT);
+            } else {
+                for (int r = 0; row + r < rows; r += kRows)
+                    for (int i = 0; c + i < columns; ++i) t[r * stride + i] = f[r * CT + i];
+            }
+        } else {
             for (int c = lane; c < columns; c += 32)
 #pragma unroll
-                for (int r = 0; r < kSteps; ++r)
-                    if (r < rows) to[(n * kSteps + r) * CT + c] = from[n][at + r * stride + c];
-    }
-}
-
-/* rows x columns elements of from [kSteps][CT] to global memory. */
-template <class T, int CT>
-__device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
-    if (piece == 16) {
-        constexpr int kPer = CT * static_cast<int>(sizeof(T)) / 16, kRows = 32 / kPer;
-        constexpr int kIn = 16 / static_cast<int>(sizeof(T));
-        const int row = lane / kPer, c = lane % kPer * kIn;
-        const T *f = from + row * CT + c;
-        T *t = to + row * stride + c;
-        if (c + kIn <= columns) {
-#pragma unroll
-            for (int r = 0; r < kSteps; r += kRows)
-                if (row + r < rows)
-                    *reinterpret_cast<Pack<T, kIn> *>(t + r * stride) =
-                        *reinterpret_cast<const Pack<T, kIn> *>(f + r * CT);
-        } else {
-            for (int r = 0; row + r < rows; r += kRows)
-                for (int i = 0; c + i < columns; ++i) t[r * stride + i] = f[r * CT + i];
+                for (int r = 0; r < STEPS; ++r)
+                    if (r < rows) to[r * stride + c] = from[r * CT + c];
         }
-    } else {
-        for (int c = lane; c < columns; c += 32)
-#pragma unroll
-            for (int r = 0; r < kSteps; ++r)
-                if (r < rows) to[r * stride + c] = from[r * CT + c];
     }
-}
 
 /* Whether step t0 + lane starts anew. */
 __device__ __forceinline__ unsigned reset_byte(const uint8_t *reset, size_t at, int live, int lane) {
@@ -584,97 +588,140 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
 
 /* ---- backward ---- */
 
-/* One channel a lane, pairs of steps.  For each step what the gradients need
- * of it: a; w = beta gate, so that dx = total w; z = x (1 - gate), so that
- * dinp = dx z; q = open (h_(t-1) - a/beta gate x), so that a total q is
- * dlog a times open; m = 1 - open. */
-template <class T, bool FAST>
-__device__ __forceinline__ void backward_gates(const T *xs, const T *rs, const T *is, float rate, int live, unsigned anew,
-                                               float h, float (&a)[kSteps], float (&w)[kSteps], float (&z)[kSteps],
-                                               float (&q)[kSteps], float (&m)[kSteps], int lane) {
-#pragma unroll
-    for (int j = 0; j < kSteps; j += 2) {
-        const int at = j * 32 + lane;
-        const auto two = [&](const T *p) { return pair(to_float(p[at]), to_float(p[at + 32])); };
-        const F2 open = sigmoid2(two(rs)), gate = sigmoid2(two(is)), x = two(xs);
-        const Decay s = decay_of<FAST>(both(rate), open);
-        const F2 u = mul2(gate, x);
-        float b0, b1, beta0, beta1, a0, a1, u0, u1;
-        split(s.a, a0, a1);
-        split(s.beta, beta0, beta1);
-        split(mul2(s.beta, u), b0, b1);
-        split(u, u0, u1);
-        /* where beta is 0 nothing decays: no gradient of log a */
-        float r0 = beta0 > 0.0f ? fast_rcp(beta0) : 0.0f, r1 = beta1 > 0.0f ? fast_rcp(beta1) : 0.0f;
-        bool g0 = beta0 > 0.0f, g1 = beta1 > 0.0f;
-        if (!FAST) {
-            if (anew >> j & 1) a0 = 0.0f, beta0 = 1.0f, b0 = u0, g0 = false;
-            if (anew >> (j + 1) & 1) a1 = 0.0f, beta1 = 1.0f, b1 = u1, g1 = false;
-            if (j >= live) a0 = 1.0f, b0 = 0.0f; /* changes no state; its gradients are not taken */
-            if (j + 1 >= live) a1 = 1.0f, b1 = 0.0f;
-        }
-        const float h1 = fmaf(a0, h, b0);
-        float q0, q1;
-        split(mul2(open, fma2(mul2(pair(a0, a1), pair(r0, r1)), mul2(u, both(-1.0f)), pair(h, h1))), q0, q1);
-        h = fmaf(a1, h1, b1);
-        a[j] = a0;
-        a[j + 1] = a1;
-        q[j] = g0 ? q0 : 0.0f;
-        q[j + 1] = g1 ? q1 : 0.0f;
-        split(mul2(pair(beta0, beta1), gate), w[j], w[j + 1]);
-        split(fma2(u, both(-1.0f), x), z[j], z[j + 1]);
-        split(fma2(open, both(-1.0f), both(1.0f)), m[j], m[j + 1]);
-    }
+/* A span of kHalf steps of two channels a lane.  What the gradients need of a
+ * step: a; w = beta gate, so that dx = total w; z = x (1 - gate), so that dinp =
+ * dx z; m = 1 - open; and q = open (h_(t-1) - a / beta gate x), so that a total
+ * q is dlog a times open.  The span's first state h0 may not be known yet: q =
+ * near_q + far_q h0. */
+struct BackwardSpan {
+    F2 a[kHalf], w[kHalf], z[kHalf], m[kHalf], near_q[kHalf], far_q[kHalf];
+};
+
+template <class T, int CT> __device__ __forceinline__ F2 two_of(const T *row, int lane) {
+    const Pack<T, 2> v = *reinterpret_cast<const Pack<T, 2> *>(row + lane * 2);
+    return pair(to_float(v.v[0]), to_float(v.v[1]));
 }
 
+/* map_a, map_h: the span's map of the state. */
+template <class T, int CT>
+__device__ __forceinline__ void backward_span(const T *xs, const T *rs, const T *is, F2 rate, bool near, int live,
+                                              unsigned anew, BackwardSpan &g, F2 *map_a, F2 *map_h, int lane) {
+    F2 beta[kHalf], open[kHalf], u[kHalf]; /* u = gate x */
+#pragma unroll
+    for (int j = 0; j < kHalf; ++j) {
+        open[j] = sigmoid2(two_of<T, CT>(rs + j * CT, lane));
+        const F2 gate = sigmoid2(two_of<T, CT>(is + j * CT, lane)), x = two_of<T, CT>(xs + j * CT, lane);
+        const Decay s = decay_of<true>(rate, open[j]);
+        g.a[j] = s.a;
+        beta[j] = s.beta;
+        u[j] = mul2(gate, x);
+        g.z[j] = fma2(u[j], both(-1.0f), x);
+        g.w[j] = gate; /* times beta, below */
+    }
+    if (!near) {
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) {
+            const Decay s = decay_of<false>(rate, open[j]);
+            g.a[j] = s.a;
+            beta[j] = s.beta;
+        }
+    }
+    unsigned still = 0; /* steps whose log a has no gradient */
+    if (anew | (live < kHalf)) {
+        still = anew | ~((1u << live) - 1);
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) {
+            if (anew >> j & 1) g.a[j] = both(0.0f), beta[j] = both(1.0f);
+            if (j >= live) { /* changes no state, and its gradients are zero */
+                g.a[j] = both(1.0f);
+                beta[j] = u[j] = g.z[j] = g.w[j] = open[j] = both(0.0f);
+            }
+        }
+    }
+    F2 prod = both(1.0f), h = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < kHalf; ++j) {
+        float b0, b1;
+        split(beta[j], b0, b1);
+        g.w[j] = mul2(beta[j], g.w[j]);
+        g.m[j] = fma2(open[j], both(-1.0f), both(1.0f));
+        /* where beta is 0 nothing decays: log a has no gradient */
+        const F2 over = pair(b0 > 0.0f ? fast_rcp(b0) : 0.0f, b1 > 0.0f ? fast_rcp(b1) : 0.0f);
+        const F2 on = pair(b0 > 0.0f ? 1.0f : 0.0f, b1 > 0.0f ? 1.0f : 0.0f);
+        const F2 slope = mul2(open[j], on);
+        g.near_q[j] = mul2(slope, fma2(mul2(g.a[j], over), mul2(u[j], both(-1.0f)), h));
+        g.far_q[j] = mul2(slope, prod);
+        h = fma2(g.a[j], h, mul2(beta[j], u[j]));
+        prod = mul2(prod, g.a[j]);
+    }
+    if (still) {
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+            if (still >> j & 1) g.near_q[j] = g.far_q[j] = both(0.0f);
+    }
+    *map_a = prod;
+    *map_h = h;
+}
+
+/* Pairs of warps share 16 steps, so that the second's first state follows from
+ * the saved one through the first's map. */
 template <class T>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(const BackwardArgs p, const Split s) {
-    constexpr int CT = 32;
+    constexpr int CT = 64, kSlot = kHalf * CT;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT], sums[kWarps][CT];
+    __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT], forward_h[2][kWarps][CT], sums[kWarps][CT];
     const RecurrenceShape &d = p.d;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, steps = static_cast<int>(d.steps);
-    constexpr int kSlot = kSteps * CT;
     T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
     const unsigned units = s.tiles * s.strips;
 
     /* rounds in the order of the scan: the last steps first */
     const auto step_of = [&](const Place &to) {
-        return static_cast<int>((s.rounds - 1 - to.round) * warps + warp) * kSteps;
+        return static_cast<int>((s.rounds - 1 - to.round) * warps + warp) * kHalf;
     };
     const auto start = [&](const Place &to, int stage) {
         const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
-        const int live = of_span(to.live, t);
+        const int live = of_span<kHalf>(to.live, t);
         const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
         const T *const dh[1] = {static_cast<const T *>(p.dh)};
-        load_rows<T, CT, 3>(slots + stage * 4 * kSlot, from, to.b * d.is + t * d.it + to.c0, d.it, live, columns,
-                            p.in_piece, lane);
-        load_rows<T, CT, 1>(slots + stage * 4 * kSlot + 3 * kSlot, dh, to.b * d.os + t * d.ot + to.c0, d.ot, live, columns,
-                            p.dh_piece, lane);
+        load_rows<T, CT, 3, kHalf>(slots + stage * 4 * kSlot, from, to.b * d.is + t * d.it + to.c0, d.it, live, columns,
+                                   p.in_piece, lane);
+        load_rows<T, CT, 1, kHalf>(slots + stage * 4 * kSlot + 3 * kSlot, dh, to.b * d.os + t * d.ot + to.c0, d.ot, live,
+                                   columns, p.dh_piece, lane);
         return reset_byte(p.reset, to.b * d.steps + t, live, lane);
     };
+    /* two floats of the lane's channels, or zero */
+    const auto two_floats = [&](const float *row, int c) {
+        const int left = static_cast<int>(d.channels) - c;
+        return pair(left > 0 ? row[c] : 0.0f, left > 1 ? row[c + 1] : 0.0f);
+    };
     const auto saved_state = [&](const Place &to) {
-        const int t = step_of(to), c = to.c0 + lane;
-        return c < static_cast<int>(d.channels) && t < steps
-                   ? p.checkpoints[(to.b * saved + t / kSteps) * d.channels + c] : 0.0f;
+        const int t = step_of(to);
+        return t < steps ? two_floats(p.checkpoints + (to.b * saved + t / kSteps) * d.channels, to.c0 + lane * 2) : both(0.0f);
+    };
+    const auto put_floats = [&](float *row, int c, F2 v) {
+        float a, b;
+        split(v, a, b);
+        const int left = static_cast<int>(d.channels) - c;
+        if (left > 0) row[c] = a;
+        if (left > 1) row[c + 1] = b;
     };
 
     Place at = place_of<CT>(blockIdx.x, d, p.lengths, s);
     int stage = 0;
     unsigned flag = start(at, 0); /* of the step that is the lane's number */
-    float h_next = saved_state(at);
+    F2 h_next = saved_state(at);
     copies_end();
-    float rate = 0.0f, sum_all = 0.0f;
-    Lane<1> state;
+    F2 rate = both(0.0f), sum_all = both(0.0f);
+    Lane<2> state;
     bool near = false, fresh = true;
     while (at.unit < units) {
-        const int t = step_of(at), live = of_span(at.live, t), rows = of_span(steps, t);
-        const size_t c = at.c0 + lane;
-        const bool in = c < d.channels;
+        const int t = step_of(at), live = of_span<kHalf>(at.live, t), rows = of_span<kHalf>(steps, t);
+        const int c = at.c0 + lane * 2;
         T *const xs = slots + stage * 4 * kSlot;
         const unsigned anew = __ballot_sync(0xffffffffu, flag);
-        const float h = h_next;
+        F2 h0 = h_next;
         const Place next = place_after<CT>(at, d, p.lengths, s);
         if (next.unit < units) {
             flag = start(next, stage ^ 1);
@@ -682,74 +729,69 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
         }
         copies_end();
         if (fresh) {
-            rate = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
-            state.v[0] = p.dstate_out && in ? p.dstate_out[at.b * d.channels + c] : 0.0f;
-            near = __all_sync(0xffffffffu, rate >= -kNear);
-            sum_all = 0.0f;
-            if (at.round > 0) state = before_strip<CT, 1>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
+            float l0, l1;
+            split(two_floats(p.decay, c), l0, l1);
+            l0 = c < static_cast<int>(d.channels) ? -d.scale * softplus(l0) : 0.0f;
+            l1 = c + 1 < static_cast<int>(d.channels) ? -d.scale * softplus(l1) : 0.0f;
+            rate = pair(l0, l1);
+            near = __all_sync(0xffffffffu, fminf(l0, l1) >= -kNear);
+            const F2 last = p.dstate_out ? two_floats(p.dstate_out + at.b * d.channels, c) : both(0.0f);
+            split(last, state.v[0], state.v[1]);
+            sum_all = both(0.0f);
+            if (at.round > 0) state = before_strip<CT, 2>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        Lane<1> map_a, map_h;
         copies_wait<1>();
         __syncwarp();
-        float a[kSteps], w[kSteps], z[kSteps], q[kSteps], m[kSteps];
-        if (live == kSteps && !anew && near)
-            backward_gates<T, true>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
-        else
-            backward_gates<T, false>(xs, xs + kSlot, xs + 2 * kSlot, rate, live, anew, h, a, w, z, q, m, lane);
-        map_a.v[0] = 1.0f;
-        map_h.v[0] = 0.0f;
+        BackwardSpan g;
+        F2 map_a, map_h;
+        backward_span<T, CT>(xs, xs + kSlot, xs + 2 * kSlot, rate, near, live, anew, g, &map_a, &map_h, lane);
+        F2 grad = both(0.0f); /* the span's map of the gradient, from zero after it */
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
-            const float g = j < live ? to_float(xs[3 * kSlot + j * CT + lane]) : 0.0f;
-            map_h.v[0] = a[j] * (g + map_h.v[0]);
-            map_a.v[0] *= a[j];
-        }
-        float grad = join<CT, 1>(map_a, map_h, &state, sa[stage], sh[stage], warps - 1 - warp, warps, lane).v[0];
+        for (int j = kHalf - 1; j >= 0; --j)
+            grad = mul2(g.a[j], add2(j < live ? two_of<T, CT>(xs + 3 * kSlot + j * CT, lane) : both(0.0f), grad));
+        Lane<2> all, from_zero;
+        split(map_a, all.v[0], all.v[1]);
+        split(grad, from_zero.v[0], from_zero.v[1]);
+        if (warps > 1) split(map_h, forward_h[stage][warp][lane * 2], forward_h[stage][warp][lane * 2 + 1]);
+        const int order = warps - 1 - warp;
+        const Lane<2> after = join<CT, 2>(all, from_zero, &state, sa[stage], sh[stage], order, warps, lane);
+        grad = pair(after.v[0], after.v[1]);
+        if (warp & 1)
+            h0 = fma2(pair(sa[stage][order + 1][lane * 2], sa[stage][order + 1][lane * 2 + 1]), h0,
+                      pair(forward_h[stage][warp - 1][lane * 2], forward_h[stage][warp - 1][lane * 2 + 1]));
         fresh = at.round == at.last;
-        if (at.round + 1 == s.rounds && p.dstate_in && in && warp == 0) p.dstate_in[at.b * d.channels + c] = state.v[0];
-        F2 sums2 = both(0.0f);
+        if (at.round + 1 == s.rounds && p.dstate_in && warp == 0)
+            put_floats(p.dstate_in + at.b * d.channels, c, pair(state.v[0], state.v[1]));
 #pragma unroll
-        for (int j = kSteps - 2; j >= 0; j -= 2) {
-            const int at = j * CT + lane;
-            const bool on0 = j < live, on1 = j + 1 < live;
-            const float total1 = grad + (on1 ? to_float(xs[3 * kSlot + at + CT]) : 0.0f), grad1 = a[j + 1] * total1;
-            const float total0 = grad1 + (on0 ? to_float(xs[3 * kSlot + at]) : 0.0f);
-            grad = a[j] * total0;
-            const F2 gx = mul2(pair(total0, total1), pair(w[j], w[j + 1]));
-            const F2 dlog = mul2(pair(grad, grad1), pair(q[j], q[j + 1]));
-            float x0, x1, r0, r1, i0, i1, d0, d1;
-            split(gx, x0, x1);
-            split(mul2(gx, pair(z[j], z[j + 1])), i0, i1);
-            split(dlog, d0, d1);
-            split(mul2(mul2(dlog, both(rate)), pair(m[j], m[j + 1])), r0, r1);
-            if (!on0) x0 = i0 = r0 = d0 = 0.0f;
-            if (!on1) x1 = i1 = r1 = d1 = 0.0f;
-            sums2 = add2(sums2, pair(d0, d1));
-            xs[at] = from_float<T>(x0);
-            xs[at + CT] = from_float<T>(x1);
-            xs[kSlot + at] = from_float<T>(r0);
-            xs[kSlot + at + CT] = from_float<T>(r1);
-            xs[2 * kSlot + at] = from_float<T>(i0);
-            xs[2 * kSlot + at + CT] = from_float<T>(i1);
+        for (int j = kHalf - 1; j >= 0; --j) {
+            T *const to = xs + j * CT;
+            const F2 total = add2(grad, j < live ? two_of<T, CT>(to + 3 * kSlot, lane) : both(0.0f));
+            grad = mul2(g.a[j], total);
+            const F2 gx = mul2(total, g.w[j]), dlog = mul2(grad, fma2(g.far_q[j], h0, g.near_q[j]));
+            const auto leave = [&](T *row, F2 v) {
+                float v0, v1;
+                split(v, v0, v1);
+                *reinterpret_cast<Pack<T, 2> *>(row + lane * 2) = {{from_float<T>(v0), from_float<T>(v1)}};
+            };
+            leave(to, gx);
+            leave(to + kSlot, mul2(mul2(dlog, rate), g.m[j]));
+            leave(to + 2 * kSlot, mul2(gx, g.z[j]));
+            sum_all = add2(sum_all, dlog);
         }
-        float sum, sum_odd;
-        split(sums2, sum, sum_odd);
-        sum += sum_odd;
         __syncwarp();
         const size_t to = at.b * d.gs + t * d.gt + at.c0;
         const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
-        store_rows<T, CT>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
-        store_rows<T, CT>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
-        store_rows<T, CT>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
-        sum_all += sum;
+        store_rows<T, CT, kHalf>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
+        store_rows<T, CT, kHalf>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
+        store_rows<T, CT, kHalf>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
         if (fresh && p.partial) {
-            sums[warp][lane] = sum_all;
+            split(sum_all, sums[warp][lane * 2], sums[warp][lane * 2 + 1]);
             __syncthreads();
-            if (warp == 0 && in) {
-                sum_all = 0.0f;
-                for (int i = 0; i < warps; ++i) sum_all += sums[i][lane];
+            if (warp == 0) {
+                F2 sum = both(0.0f);
+                for (int i = 0; i < warps; ++i) sum = add2(sum, pair(sums[i][lane * 2], sums[i][lane * 2 + 1]));
                 const size_t strip = divided(at.unit, s.tiles, s.magic_tiles);
-                p.partial[(strip * d.sequences + at.b) * d.channels + c] = sum_all;
+                put_floats(p.partial + (strip * d.sequences + at.b) * d.channels, c, sum);
             }
             __syncthreads(); /* sums is free again */
         }
@@ -762,7 +804,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
 /* The maps of the strips, all but the last of the scan: of rec and dh alone. */
 template <class T>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_maps(const BackwardArgs p, const Split s) {
-    constexpr int CT = 32, kSlot = kSteps * CT;
+    constexpr int CT = 64, kSlot = kHalf * CT;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float sa[kWarps][CT], sh[kWarps][CT];
     const RecurrenceShape &d = p.d;
@@ -776,23 +818,22 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
         const int spans = static_cast<int>(s.strip_rounds);
         const int top = static_cast<int>((s.rounds - at.round) * warps) - 1 - warp * spans;
         const auto start = [&](int span, int stage) {
-            const int t = (top - span) * kSteps, live = of_span(at.live, t);
+            const int t = (top - span) * kHalf, live = of_span<kHalf>(at.live, t);
             const T *const rec[1] = {static_cast<const T *>(p.rec)}, *const dh[1] = {static_cast<const T *>(p.dh)};
-            load_rows<T, CT, 1>(slots + stage * 2 * kSlot, rec, at.b * d.is + t * d.it + at.c0, d.it, live, columns,
-                                p.in_piece, lane);
-            load_rows<T, CT, 1>(slots + stage * 2 * kSlot + kSlot, dh, at.b * d.os + t * d.ot + at.c0, d.ot, live, columns,
-                                p.dh_piece, lane);
+            load_rows<T, CT, 1, kHalf>(slots + stage * 2 * kSlot, rec, at.b * d.is + t * d.it + at.c0, d.it, live, columns,
+                                       p.in_piece, lane);
+            load_rows<T, CT, 1, kHalf>(slots + stage * 2 * kSlot + kSlot, dh, at.b * d.os + t * d.ot + at.c0, d.ot, live,
+                                       columns, p.dh_piece, lane);
             return reset_byte(p.reset, at.b * d.steps + t, live, lane);
         };
         unsigned flag = start(0, 0);
         copies_end();
-        const size_t c = at.c0 + lane;
-        const float rate = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
-        Lane<1> all, grad;
-        all.v[0] = 1.0f;
-        grad.v[0] = 0.0f;
+        const int c = at.c0 + lane * 2;
+        const float l0 = left > lane * 2 ? -d.scale * softplus(p.decay[c]) : 0.0f;
+        const float l1 = left > lane * 2 + 1 ? -d.scale * softplus(p.decay[c + 1]) : 0.0f;
+        F2 all = both(1.0f), grad = both(0.0f);
         for (int i = 0; i < spans; ++i) {
-            const int live = of_span(at.live, (top - i) * kSteps);
+            const int live = of_span<kHalf>(at.live, (top - i) * kHalf);
             const unsigned anew = __ballot_sync(0xffffffffu, flag);
             const T *rs = slots + (i & 1) * 2 * kSlot;
             if (i + 1 < spans) flag = start(i + 1, (i + 1) & 1);
@@ -800,25 +841,20 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
             copies_wait<1>();
             __syncwarp();
 #pragma unroll
-            for (int j = kSteps - 2; j >= 0; j -= 2) {
-                const int to = j * CT + lane;
-                const Decay k = decay_of<false>(both(rate), sigmoid2(pair(to_float(rs[to]), to_float(rs[to + CT]))));
-                float a0, a1;
-                split(k.a, a0, a1);
-                if (anew >> j & 1) a0 = 0.0f;
-                if (anew >> (j + 1) & 1) a1 = 0.0f;
-                if (j + 1 < live) {
-                    grad.v[0] = a1 * (to_float(rs[kSlot + to + CT]) + grad.v[0]);
-                    all.v[0] *= a1;
-                }
+            for (int j = kHalf - 1; j >= 0; --j) {
+                F2 a = decay_of<false>(pair(l0, l1), sigmoid2(two_of<T, CT>(rs + j * CT, lane))).a;
+                if (anew >> j & 1) a = both(0.0f);
                 if (j < live) {
-                    grad.v[0] = a0 * (to_float(rs[kSlot + to]) + grad.v[0]);
-                    all.v[0] *= a0;
+                    grad = mul2(a, add2(two_of<T, CT>(rs + kSlot + j * CT, lane), grad));
+                    all = mul2(all, a);
                 }
             }
             __syncwarp();
         }
-        leave_map<CT, 1>(s, unit, all, grad, sa, sh, warp, warps, lane);
+        Lane<2> map_a, map_h;
+        split(all, map_a.v[0], map_a.v[1]);
+        split(grad, map_h.v[0], map_h.v[1]);
+        leave_map<CT, 2>(s, unit, map_a, map_h, sa, sh, warp, warps, lane);
     }
 }
 
@@ -840,7 +876,7 @@ bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
         return false;
     size_t rows, all, items;
     if (!product(d->sequences, d->channels, 0x7fffffffu, &rows) || !product(rows, d->steps, SIZE_MAX / 64, &all) ||
-        !product(d->sequences * ((d->channels + 31) / 32), (d->steps + kSteps - 1) / kSteps, 0x7fffffffu, &items))
+        !product(d->sequences * ((d->channels + 31) / 32), (d->steps + kHalf - 1) / kHalf, 0x7fffffffu, &items))
         return false;
     s->sequences = d->sequences;
     s->steps = d->steps;
@@ -855,21 +891,32 @@ bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     return s->it >= d->channels && s->ot >= d->channels && s->gt >= d->channels;
 }
 
-constexpr unsigned kFill = 16 * 148;   /* warps that the kernels' registers leave room for on the GPU */
-constexpr unsigned kLeastRounds = 2;   /* of a strip */
+constexpr unsigned kSms = 148;
+constexpr unsigned kLeastRounds = 2; /* of a strip */
 
-/* Warps: as many as leave every tile room on the GPU at once.  Strips: where
- * tiles of four warps take less than a third of the room. */
-Split split_of(const RecurrenceShape &d, int tile, int *warps) {
+/* How a pass is laid out: steps of a span, channels of a tile, warps that an SM
+ * has registers and shared memory for. */
+struct Pass {
+    int span, tile;
+    unsigned room;
+};
+Pass forward_pass(int type) { return {kSteps, type == TB_TYPE_F32 ? 32 : 64, 16}; }
+Pass backward_pass(int type) { return {kHalf, 64, type == TB_TYPE_F32 ? 12u : 16u}; }
+
+/* Warps: as many as leave every tile room on the GPU at once (backward in
+ * pairs).  Strips: where tiles of four warps take less than a third of the
+ * room. */
+Split split_of(const RecurrenceShape &d, const Pass &p, int *warps) {
     Split s{};
-    s.tiles_per_sequence = static_cast<unsigned>((d.channels + tile - 1) / tile);
+    s.tiles_per_sequence = static_cast<unsigned>((d.channels + p.tile - 1) / p.tile);
     s.tiles = static_cast<unsigned>(d.sequences * s.tiles_per_sequence);
-    const unsigned spans = static_cast<unsigned>((d.steps + kSteps - 1) / kSteps);
-    unsigned w = kFill / s.tiles;
+    const unsigned spans = static_cast<unsigned>((d.steps + p.span - 1) / p.span), fill = p.room * kSms;
+    unsigned w = fill / s.tiles;
     w = w < 1 ? 1 : w > kWarps ? kWarps : w;
     w = w > spans ? spans : w;
+    if (p.span < kSteps && spans > 1) w = w < 4 ? 2 : 4;
     s.rounds = (spans + w - 1) / w;
-    unsigned strips = kFill / (s.tiles * w);
+    unsigned strips = fill / (s.tiles * w);
     if (strips < 3) strips = 1;
     const unsigned most = s.rounds / kLeastRounds;
     if (strips > most) strips = most < 2 ? 1 : most;
@@ -884,8 +931,6 @@ size_t map_bytes(const Split &s, int tile) {
     return s.strips > 1 ? static_cast<size_t>(s.tiles) * s.strips * 2 * tile * sizeof(float) : 0;
 }
 
-int forward_tile(int type) { return type == TB_TYPE_F32 ? 32 : 64; }
-
 /* Rows of partial sums for ddecay, and behind them the parts that they are first summed into. */
 size_t partial_rows(const RecurrenceShape &d, const Split &s) { return d.sequences * s.strips; }
 size_t partial_bytes(const RecurrenceShape &d, const Split &s) {
@@ -899,14 +944,15 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
     return all % 16 == 0 ? 16 : all % 4 == 0 && least == 4 ? 4 : 0;
 }
 
-/* Launches a kernel over `work` units: at most as many CTAs as its registers
- * (16 warps an SM) leave room for, each taking every grid-th unit. */
+/* Launches a kernel over `work` units: at most as many CTAs as there is room
+ * for, each taking every grid-th unit. */
 template <auto Kernel, class Args>
-int launch_units(unsigned work, const Args &args, const Split &s, int warps, size_t shared, cudaStream_t st) {
+int launch_units(unsigned work, const Args &args, const Split &s, const Pass &pass, int warps, size_t shared,
+                 cudaStream_t st) {
     int dev = 0;
     const int sms = multiprocessors(&dev);
     if (!sms || !allow_shared<Kernel>(shared)) return 0;
-    const unsigned most = static_cast<unsigned>(sms) * (16 / warps);
+    const unsigned most = static_cast<unsigned>(sms) * (pass.room / warps);
     Kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args, s);
     return launched();
 }
@@ -917,10 +963,10 @@ extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_d
     RecurrenceShape s;
     if (!recurrence_shape(desc, &s)) return 0;
     int warps;
-    const int tile = forward_tile(desc->type);
-    const size_t f = map_bytes(split_of(s, tile, &warps), tile);
-    const Split b = split_of(s, 32, &warps);
-    const size_t back = map_bytes(b, 32) + partial_bytes(s, b);
+    const Pass forward = forward_pass(desc->type), backward = backward_pass(desc->type);
+    const size_t f = map_bytes(split_of(s, forward, &warps), forward.tile);
+    const Split b = split_of(s, backward, &warps);
+    const size_t back = map_bytes(b, backward.tile) + partial_bytes(s, b);
     return f > back ? f : back;
 }
 
@@ -943,17 +989,17 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     p.in_piece = piece_of(reinterpret_cast<const void *>(in), s.is, s.it, size, 4);
     p.out_piece = piece_of(h, s.os, s.ot, size, 16);
     int warps;
-    const int tile = forward_tile(desc->type);
-    Split split = split_of(s, tile, &warps);
+    const Pass pass = forward_pass(desc->type);
+    Split split = split_of(s, pass, &warps);
     split.maps = static_cast<float *>(workspace);
-    const size_t shared = static_cast<size_t>(warps) * 2 * 3 * kSteps * tile * size;
+    const size_t shared = static_cast<size_t>(warps) * 2 * 3 * pass.span * pass.tile * size;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (split.strips > 1 &&
-            !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), p, split, warps, shared, st))
+            !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), p, split, pass, warps, shared, st))
             return 0;
-        return launch_units<recurrence_forward<T>>(split.tiles * split.strips, p, split, warps, shared, st);
+        return launch_units<recurrence_forward<T>>(split.tiles * split.strips, p, split, pass, warps, shared, st);
     });
 }
 
@@ -983,22 +1029,23 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     }
     cudaGetLastError(); /* report these launches only */
     int warps;
-    Split split = split_of(s, 32, &warps);
+    const Pass pass = backward_pass(desc->type);
+    Split split = split_of(s, pass, &warps);
     split.maps = static_cast<float *>(workspace);
-    float *partial = split.maps + map_bytes(split, 32) / sizeof(float);
+    float *partial = split.maps + map_bytes(split, pass.tile) / sizeof(float);
     BackwardArgs p{s, x, recurrence_gate, input_gate, dh, decay, checkpoints, dstate_out, reset, lengths, dx,
                    drecurrence_gate, dinput_gate, ddecay ? partial : nullptr, dstate_in, 0, 0, 0};
     p.in_piece = piece_of(reinterpret_cast<const void *>(ins), s.is, s.it, size, 4);
     p.dh_piece = piece_of(dh, s.os, s.ot, size, 4);
     p.out_piece = piece_of(reinterpret_cast<const void *>(outs), s.gs, s.gt, size, 16);
-    const size_t shared = static_cast<size_t>(warps) * 2 * 4 * kSteps * 32 * size;
+    const size_t shared = static_cast<size_t>(warps) * 2 * 4 * pass.span * pass.tile * size;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         if (split.strips > 1 &&
-            !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), p, split, warps, shared, st))
+            !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), p, split, pass, warps, shared, st))
             return 0;
-        return launch_units<recurrence_backward<T>>(split.tiles * split.strips, p, split, warps, shared, st);
+        return launch_units<recurrence_backward<T>>(split.tiles * split.strips, p, split, pass, warps, shared, st);
     });
     if (!ok || !ddecay) return ok;
     const size_t rows = partial_rows(s, split), parts = column_parts(rows);
