@@ -199,6 +199,8 @@ RECURRENCE_SHAPES = [
     (1, 1, 1, 0, 0), (3, 1, 64, 0, 0), (2, 2, 5, 0, 0), (2, 15, 33, 3, 1), (2, 16, 64, 0, 0), (1, 17, 130, 0, 0),
     (3, 100, 48, 16, 0), (2, 257, 64, 0, 0), (1, 1000, 96, 0, 0), (5, 129, 321, 0, 0), (1, 4099, 8, 0, 0),
     (40, 40, 256, 0, 0), (2, 333, 200, 8, 4),
+    # tiles enough that one CTA takes many rounds: bulk copies
+    (150, 260, 136, 0, 0), (600, 100, 72, 8, 0), (310, 300, 40, 8, 0),
 ]
 
 

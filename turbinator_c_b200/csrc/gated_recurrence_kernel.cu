@@ -7,7 +7,11 @@
  * taken apart and joined.  A warp takes spans of 16 steps of 32 or 64 channels
  * (a tile); the warps of a CTA take consecutive spans of one tile, join them in
  * shared memory and go on together, the state in registers.  Inputs are staged
- * by asynchronous copies one round ahead; outputs leave through the same slots.
+ * in shared memory one round ahead, outputs leave through the same slots: by
+ * bulk tensor copies that one lane starts (every row on 16 bytes; the lanes'
+ * own copies took 54 us of loads and 50 us of stores of a 285 us backward pass
+ * of 64 x 1,024 x 1,024 bf16, nearly all of it their instructions), else by
+ * asynchronous copies of 16 or 4 bytes, else element by element.
  *
  * Where tiles alone cannot fill the GPU, the steps are cut into strips and a
  * first kernel finds each strip's map, from which every strip's first state
@@ -21,7 +25,11 @@
  * c_t = a_t (dh_t + c_(t+1)), the gradient of the state before step t; the
  * states that it needs are recomputed within 16 steps from the saved ones.
  */
+#include <cuda.h> /* tensor maps */
+
+#include "tb_features_internal.h"
 #include "tb_learner.cuh"
+#include "tb_pipeline.cuh"
 
 using namespace tb_learn;
 
@@ -232,6 +240,57 @@ __device__ __forceinline__ void load_pieces(T *to, const T *const (&from)[N], si
         }
     }
 
+/* The same by bulk tensor copies: a box of steps x CT channels from one tensor.
+ * A box lies on 128 bytes of shared memory.  Where the dynamic part starts
+ * depends on the static part before it, so the first slot is moved up to the
+ * next such place; calls ask for as much more. */
+constexpr int kBoxAlign = 128;
+template <class T> __device__ __forceinline__ T *slots_of(unsigned char *dynamic) {
+    return reinterpret_cast<T *>(dynamic + (-shared_address(dynamic) & (kBoxAlign - 1)));
+}
+struct alignas(64) Maps {
+    CUtensorMap in[4], out[3]; /* x, rec, inp, dh; h or dx, drec, dinp */
+    unsigned *status;
+};
+constexpr unsigned long long kWaitNs = 1000000000ull;
+
+__device__ __forceinline__ void load_box(void *to, const CUtensorMap *map, int c, int t, int b, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(shared_address(to)), "l"(map), "r"(c), "r"(t), "r"(b), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap *map, const void *from, int c, int t, int b) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                 "r"(shared_address(from)), "r"(c), "r"(t), "r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ void boxes_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+/* The lane's stores have read their slots; or are done. */
+__device__ __forceinline__ void boxes_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void boxes_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+/* A warp's wait for its boxes, bounded: after a first timeout the stream's
+ * status word says so and the kernel goes to its end without waiting again. */
+struct BoxWait {
+    unsigned long long limit = kWaitNs;
+    __device__ __forceinline__ void operator()(uint32_t bar, unsigned parity, unsigned *status, int lane) {
+        if (tb_pipe::mbar_wait(bar, parity, limit)) return;
+        if (lane == 0) atomicOr(status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
+        limit = 0;
+    }
+    /* At the end: the lane's stores are done, and after a timeout boxes that are
+     * still under way get another moment before their slots go. */
+    __device__ __forceinline__ void finish(uint64_t (&bars)[2], int lane) {
+        if (lane != 0) return;
+        boxes_done();
+        if (limit != 0) return;
+        for (int n = 0; n < 2; ++n)
+            for (unsigned parity = 0; parity < 2; ++parity)
+                tb_pipe::mbar_wait(shared_address(&bars[n]), parity, kWaitNs / 8);
+    }
+};
+
 /* Whether step t0 + lane starts anew. */
 __device__ __forceinline__ unsigned reset_byte(const uint8_t *reset, size_t at, int live, int lane) {
     return reset && lane < live ? reset[at + lane] : 0u;
@@ -435,30 +494,56 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(const ForwardArgs p, const Split s) {
+/* BULK: by bulk tensor copies. */
+template <class T, bool BULK>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
+recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ Maps maps) {
     constexpr int V = kForwardV<T>, CT = 32 * V;
     extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ uint64_t bars[kWarps][2]; /* of a stage's boxes */
     __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT];
     const RecurrenceShape &d = p.d;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, steps = static_cast<int>(d.steps);
-    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 3 * kSteps * CT; /* two stages of x, rec, inp */
+    T *const slots = slots_of<T>(dynamic) + warp * 2 * 3 * kSteps * CT; /* two stages of x, rec, inp */
+    static_assert(kSteps * CT * sizeof(T) % kBoxAlign == 0, "a box's place");
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
     const unsigned units = s.tiles * s.strips;
 
     const auto step_of = [&](const Place &to) { return static_cast<int>(to.round * warps + warp) * kSteps; };
     const auto start = [&](const Place &to, int stage) {
         const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0;
+        if constexpr (BULK) {
+            if (lane == 0) {
+                boxes_read(); /* the slot's outputs of two rounds ago have left */
+                const uint32_t bar = shared_address(&bars[warp][stage]);
+                tb_pipe::mbar_arrive_expect_tx(bar, 3 * kSteps * CT * sizeof(T));
+                for (int n = 0; n < 3; ++n)
+                    load_box(slots + (stage * 3 + n) * kSteps * CT, &maps.in[n], to.c0, t, static_cast<int>(to.b), bar);
+            }
+            return;
+        }
         const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
         load_rows<T, CT, 3>(slots + stage * 3 * kSteps * CT, from, to.b * d.is + t * d.it + to.c0, d.it,
                             of_span(to.live, t), left < CT ? left : CT, p.in_piece, lane);
+        copies_end();
+    };
+    /* of the step that is the lane's number */
+    const auto reset_at = [&](const Place &to) {
+        const int t = step_of(to);
         return reset_byte(p.reset, to.b * d.steps + t, of_span(to.live, t), lane);
     };
+    BoxWait wait;
+    if (BULK && lane == 0) {
+        for (int n = 0; n < 2; ++n) tb_pipe::mbar_init(shared_address(&bars[warp][n]), 1);
+        tb_pipe::fence_mbar_init();
+    }
+    __syncwarp();
 
     Place at = place_of<CT>(blockIdx.x, d, p.lengths, s);
     int stage = 0;
-    unsigned flag = start(at, 0); /* of the step that is the lane's number */
-    copies_end();
+    unsigned parity = 0; /* of both stages' barriers */
+    start(at, 0);
+    unsigned flag = reset_at(at);
     float rate[V];
     Lane<V> state;
     bool near = false, fresh = true;
@@ -467,8 +552,12 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(c
         T *const xs = slots + stage * 3 * kSteps * CT;
         const unsigned anew = __ballot_sync(0xffffffffu, flag);
         const Place next = place_after<CT>(at, d, p.lengths, s);
-        if (next.unit < units) flag = start(next, stage ^ 1);
-        copies_end();
+        if (next.unit < units) {
+            flag = reset_at(next);
+            if (!BULK) start(next, stage ^ 1);
+        } else if (!BULK) {
+            copies_end();
+        }
         if (fresh) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -480,7 +569,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(c
             near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
             if (at.round > 0) state = before_strip<CT, V>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        copies_wait<1>();
+        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
+        else copies_wait<1>();
         __syncwarp();
         float prod[kSteps][V], local[kSteps][V];
         if (live == kSteps && !anew && near)
@@ -494,6 +584,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(c
             map_h.v[v] = local[kSteps - 1][v];
         }
         const Lane<V> h0 = join<CT, V>(map_a, map_h, &state, sa[stage], sh[stage], warp, warps, lane);
+        if (BULK && next.unit < units) start(next, stage ^ 1); /* half a round ahead: the other slot has been read */
         fresh = at.round == at.last;
         const bool ends = at.round + 1 == s.rounds && p.state_out && warp == 0;
 #pragma unroll
@@ -519,14 +610,25 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward(c
             for (int j = live; j < kSteps; ++j)
                 for (int v = 0; v < V; ++v) xs[j * CT + lane * V + v] = from_float<T>(0.0f);
         }
-        __syncwarp();
-        const int left = static_cast<int>(d.channels) - at.c0;
-        store_rows<T, CT>(static_cast<T *>(p.h) + at.b * d.os + t * d.ot + at.c0, xs, d.ot, rows, left < CT ? left : CT,
-                          p.out_piece, lane);
-        __syncwarp();
+        if constexpr (BULK) {
+            tb_pipe::fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0 && rows > 0) {
+                store_box(&maps.out[0], xs, at.c0, t, static_cast<int>(at.b));
+                boxes_end();
+            }
+        } else {
+            __syncwarp();
+            const int left = static_cast<int>(d.channels) - at.c0;
+            store_rows<T, CT>(static_cast<T *>(p.h) + at.b * d.os + t * d.ot + at.c0, xs, d.ot, rows, left < CT ? left : CT,
+                              p.out_piece, lane);
+            __syncwarp();
+        }
         at = next;
+        parity ^= stage; /* each stage's barrier turns once in two rounds */
         stage ^= 1;
     }
+    if constexpr (BULK) wait.finish(bars[warp], lane);
 }
 
 /* The maps of the strips, all but the last: each warp takes consecutive spans. */
@@ -645,12 +747,11 @@ __device__ __forceinline__ void backward_span(const T *xs, const T *rs, const T 
         split(beta[j], b0, b1);
         g.w[j] = mul2(beta[j], g.w[j]);
         g.m[j] = fma2(open[j], both(-1.0f), both(1.0f));
-        /* where beta is 0 nothing decays: log a has no gradient */
-        const F2 over = pair(b0 > 0.0f ? fast_rcp(b0) : 0.0f, b1 > 0.0f ? fast_rcp(b1) : 0.0f);
-        const F2 on = pair(b0 > 0.0f ? 1.0f : 0.0f, b1 > 0.0f ? 1.0f : 0.0f);
-        const F2 slope = mul2(open[j], on);
-        g.near_q[j] = mul2(slope, fma2(mul2(g.a[j], over), mul2(u[j], both(-1.0f)), h));
-        g.far_q[j] = mul2(slope, prod);
+        /* where beta is 0, open or the rate is, which are factors of both
+         * gradients: what stands for 1 / beta there only has to be finite */
+        const F2 over = pair(fast_rcp(fmaxf(b0, 1e-18f)), fast_rcp(fmaxf(b1, 1e-18f)));
+        g.near_q[j] = mul2(open[j], fma2(mul2(g.a[j], over), mul2(u[j], both(-1.0f)), h));
+        g.far_q[j] = mul2(open[j], prod);
         h = fma2(g.a[j], h, mul2(beta[j], u[j]));
         prod = mul2(prod, g.a[j]);
     }
@@ -665,14 +766,17 @@ __device__ __forceinline__ void backward_span(const T *xs, const T *rs, const T 
 
 /* Pairs of warps share 16 steps, so that the second's first state follows from
  * the saved one through the first's map. */
-template <class T>
-__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(const BackwardArgs p, const Split s) {
+template <class T, bool BULK>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
+recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__ Maps maps) {
     constexpr int CT = 64, kSlot = kHalf * CT;
     extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ uint64_t bars[kWarps][2]; /* of a stage's boxes */
     __shared__ float sa[2][kWarps][CT], sh[2][kWarps][CT], forward_h[2][kWarps][CT], sums[kWarps][CT];
     const RecurrenceShape &d = p.d;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, steps = static_cast<int>(d.steps);
-    T *const slots = reinterpret_cast<T *>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
+    T *const slots = slots_of<T>(dynamic) + warp * 2 * 4 * kSlot; /* two stages of x, rec, inp, dh */
+    static_assert(kSlot * sizeof(T) % kBoxAlign == 0, "a box's place");
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
     const unsigned units = s.tiles * s.strips;
 
@@ -683,22 +787,48 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
     const auto start = [&](const Place &to, int stage) {
         const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
         const int live = of_span<kHalf>(to.live, t);
+        if constexpr (BULK) {
+            if (lane == 0) {
+                boxes_read(); /* the slot's outputs of two rounds ago have left */
+                const uint32_t bar = shared_address(&bars[warp][stage]);
+                tb_pipe::mbar_arrive_expect_tx(bar, 4 * kSlot * sizeof(T));
+                for (int n = 0; n < 4; ++n)
+                    load_box(slots + (stage * 4 + n) * kSlot, &maps.in[n], to.c0, t, static_cast<int>(to.b), bar);
+            }
+            return;
+        }
         const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
         const T *const dh[1] = {static_cast<const T *>(p.dh)};
         load_rows<T, CT, 3, kHalf>(slots + stage * 4 * kSlot, from, to.b * d.is + t * d.it + to.c0, d.it, live, columns,
                                    p.in_piece, lane);
         load_rows<T, CT, 1, kHalf>(slots + stage * 4 * kSlot + 3 * kSlot, dh, to.b * d.os + t * d.ot + to.c0, d.ot, live,
                                    columns, p.dh_piece, lane);
-        return reset_byte(p.reset, to.b * d.steps + t, live, lane);
+        copies_end();
     };
+    /* of the step that is the lane's number */
+    const auto reset_at = [&](const Place &to) {
+        const int t = step_of(to);
+        return reset_byte(p.reset, to.b * d.steps + t, of_span<kHalf>(to.live, t), lane);
+    };
+    BoxWait wait;
+    if (BULK && lane == 0) {
+        for (int n = 0; n < 2; ++n) tb_pipe::mbar_init(shared_address(&bars[warp][n]), 1);
+        tb_pipe::fence_mbar_init();
+    }
+    __syncwarp();
     /* two floats of the lane's channels, or zero */
     const auto two_floats = [&](const float *row, int c) {
         const int left = static_cast<int>(d.channels) - c;
         return pair(left > 0 ? row[c] : 0.0f, left > 1 ? row[c + 1] : 0.0f);
     };
-    const auto saved_state = [&](const Place &to) {
+    /* the saved state of the place's 16 steps: a row that moves with the rounds of a unit */
+    const float *row = nullptr;
+    const size_t row_step = static_cast<size_t>(warps * kHalf / kSteps) * d.channels;
+    const auto saved_state = [&](const Place &to, bool anew) {
         const int t = step_of(to);
-        return t < steps ? two_floats(p.checkpoints + (to.b * saved + t / kSteps) * d.channels, to.c0 + lane * 2) : both(0.0f);
+        if (anew) row = p.checkpoints + (to.b * saved + t / kSteps) * d.channels;
+        else row -= row_step;
+        return t < steps ? two_floats(row, to.c0 + lane * 2) : both(0.0f);
     };
     const auto put_floats = [&](float *row, int c, F2 v) {
         float a, b;
@@ -710,9 +840,10 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
 
     Place at = place_of<CT>(blockIdx.x, d, p.lengths, s);
     int stage = 0;
-    unsigned flag = start(at, 0); /* of the step that is the lane's number */
-    F2 h_next = saved_state(at);
-    copies_end();
+    unsigned parity = 0; /* of both stages' barriers */
+    start(at, 0);
+    unsigned flag = reset_at(at);
+    F2 h_next = saved_state(at, true);
     F2 rate = both(0.0f), sum_all = both(0.0f);
     Lane<2> state;
     bool near = false, fresh = true;
@@ -724,10 +855,12 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
         F2 h0 = h_next;
         const Place next = place_after<CT>(at, d, p.lengths, s);
         if (next.unit < units) {
-            flag = start(next, stage ^ 1);
-            h_next = saved_state(next);
+            flag = reset_at(next);
+            h_next = saved_state(next, next.unit != at.unit);
+            if (!BULK) start(next, stage ^ 1);
+        } else if (!BULK) {
+            copies_end();
         }
-        copies_end();
         if (fresh) {
             float l0, l1;
             split(two_floats(p.decay, c), l0, l1);
@@ -740,7 +873,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
             sum_all = both(0.0f);
             if (at.round > 0) state = before_strip<CT, 2>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        copies_wait<1>();
+        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
+        else copies_wait<1>();
         __syncwarp();
         BackwardSpan g;
         F2 map_a, map_h;
@@ -759,6 +893,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
         if (warp & 1)
             h0 = fma2(pair(sa[stage][order + 1][lane * 2], sa[stage][order + 1][lane * 2 + 1]), h0,
                       pair(forward_h[stage][warp - 1][lane * 2], forward_h[stage][warp - 1][lane * 2 + 1]));
+        if (BULK && next.unit < units) start(next, stage ^ 1); /* half a round ahead: the other slot has been read */
         fresh = at.round == at.last;
         if (at.round + 1 == s.rounds && p.dstate_in && warp == 0)
             put_floats(p.dstate_in + at.b * d.channels, c, pair(state.v[0], state.v[1]));
@@ -778,12 +913,22 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
             leave(to + 2 * kSlot, mul2(gx, g.z[j]));
             sum_all = add2(sum_all, dlog);
         }
-        __syncwarp();
-        const size_t to = at.b * d.gs + t * d.gt + at.c0;
-        const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
-        store_rows<T, CT, kHalf>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
-        store_rows<T, CT, kHalf>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
-        store_rows<T, CT, kHalf>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
+        if constexpr (BULK) {
+            tb_pipe::fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0 && rows > 0) {
+                for (int n = 0; n < 3; ++n) store_box(&maps.out[n], xs + n * kSlot, at.c0, t, static_cast<int>(at.b));
+                boxes_end();
+            }
+        } else {
+            __syncwarp();
+            const size_t to = at.b * d.gs + t * d.gt + at.c0;
+            const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
+            store_rows<T, CT, kHalf>(static_cast<T *>(p.dx) + to, xs, d.gt, rows, columns, p.out_piece, lane);
+            store_rows<T, CT, kHalf>(static_cast<T *>(p.drec) + to, xs + kSlot, d.gt, rows, columns, p.out_piece, lane);
+            store_rows<T, CT, kHalf>(static_cast<T *>(p.dinp) + to, xs + 2 * kSlot, d.gt, rows, columns, p.out_piece, lane);
+            __syncwarp();
+        }
         if (fresh && p.partial) {
             split(sum_all, sums[warp][lane * 2], sums[warp][lane * 2 + 1]);
             __syncthreads();
@@ -795,10 +940,11 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward(
             }
             __syncthreads(); /* sums is free again */
         }
-        __syncwarp();
         at = next;
+        parity ^= stage; /* each stage's barrier turns once in two rounds */
         stage ^= 1;
     }
+    if constexpr (BULK) wait.finish(bars[warp], lane);
 }
 
 /* The maps of the strips, all but the last of the scan: of rec and dh alone. */
@@ -944,16 +1090,53 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
     return all % 16 == 0 ? 16 : all % 4 == 0 && least == 4 ? 4 : 0;
 }
 
+/* Tensor maps of [sequences, steps, channels] tensors in boxes of one warp's
+ * span and tile.  False where the driver has no such copies or refuses them. */
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+    static std::atomic<EncodeTiled> known{nullptr};
+    EncodeTiled f = known.load(std::memory_order_relaxed);
+    if (!f) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess)
+            return nullptr;
+        f = reinterpret_cast<EncodeTiled>(p);
+        known.store(f, std::memory_order_relaxed);
+    }
+    return f;
+}
+bool encode(CUtensorMap *map, int type, const void *tensor, const RecurrenceShape &d, size_t sequence_stride,
+            size_t step_stride, const Pass &pass) {
+    const EncodeTiled f = encoder();
+    const size_t size = type_size(type);
+    const cuuint64_t extent[3] = {d.channels, d.steps, d.sequences};
+    const cuuint64_t stride[2] = {step_stride * size, sequence_stride * size};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(pass.tile), static_cast<cuuint32_t>(pass.span), 1}, one[3] = {1, 1, 1};
+    const CUtensorMapDataType kind = type == TB_TYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : type == TB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return f && stride[0] < 1ull << 40 && stride[1] < 1ull << 40 &&
+           f(map, kind, 3, const_cast<void *>(tensor), extent, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+               CUDA_SUCCESS;
+}
+/* Bulk copies pay from this many rounds of a unit on: seven maps take the host
+ * a few microseconds, which short calls would wait for. */
+constexpr unsigned kBulkRounds = 4;
+
 /* Launches a kernel over `work` units: at most as many CTAs as there is room
  * for, each taking every grid-th unit. */
-template <auto Kernel, class Args>
-int launch_units(unsigned work, const Args &args, const Split &s, const Pass &pass, int warps, size_t shared,
-                 cudaStream_t st) {
+template <auto Kernel, class... Args>
+int launch_units(unsigned work, const Pass &pass, int warps, size_t shared, cudaStream_t st, const Args &...args) {
     int dev = 0;
     const int sms = multiprocessors(&dev);
     if (!sms || !allow_shared<Kernel>(shared)) return 0;
     const unsigned most = static_cast<unsigned>(sms) * (pass.room / warps);
-    Kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args, s);
+    Kernel<<<work < most ? work : most, warps * 32, shared, st>>>(args...);
     return launched();
 }
 
@@ -992,14 +1175,22 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     const Pass pass = forward_pass(desc->type);
     Split split = split_of(s, pass, &warps);
     split.maps = static_cast<float *>(workspace);
-    const size_t shared = static_cast<size_t>(warps) * 2 * 3 * pass.span * pass.tile * size;
+    const size_t shared = static_cast<size_t>(warps) * 2 * 3 * pass.span * pass.tile * size + kBoxAlign;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        if (split.strips > 1 &&
-            !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), p, split, pass, warps, shared, st))
+        if (split.strips > 1 && !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), pass, warps,
+                                                                          shared, st, p, split))
             return 0;
-        return launch_units<recurrence_forward<T>>(split.tiles * split.strips, p, split, pass, warps, shared, st);
+        const unsigned units = split.tiles * split.strips;
+        Maps maps{};
+        if (split.strip_rounds >= kBulkRounds && p.in_piece == 16 && p.out_piece == 16 &&
+            (maps.status = tb_status_slot(stream)) && encode(&maps.in[0], desc->type, x, s, s.is, s.it, pass) &&
+            encode(&maps.in[1], desc->type, recurrence_gate, s, s.is, s.it, pass) &&
+            encode(&maps.in[2], desc->type, input_gate, s, s.is, s.it, pass) &&
+            encode(&maps.out[0], desc->type, h, s, s.os, s.ot, pass))
+            return launch_units<recurrence_forward<T, true>>(units, pass, warps, shared, st, p, split, maps);
+        return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, maps);
     });
 }
 
@@ -1038,14 +1229,22 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     p.in_piece = piece_of(reinterpret_cast<const void *>(ins), s.is, s.it, size, 4);
     p.dh_piece = piece_of(dh, s.os, s.ot, size, 4);
     p.out_piece = piece_of(reinterpret_cast<const void *>(outs), s.gs, s.gt, size, 16);
-    const size_t shared = static_cast<size_t>(warps) * 2 * 4 * pass.span * pass.tile * size;
+    const size_t shared = static_cast<size_t>(warps) * 2 * 4 * pass.span * pass.tile * size + kBoxAlign;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ok = with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        if (split.strips > 1 &&
-            !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), p, split, pass, warps, shared, st))
+        if (split.strips > 1 && !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), pass, warps,
+                                                                           shared, st, p, split))
             return 0;
-        return launch_units<recurrence_backward<T>>(split.tiles * split.strips, p, split, pass, warps, shared, st);
+        const unsigned units = split.tiles * split.strips;
+        Maps maps{};
+        bool bulk = split.strip_rounds >= kBulkRounds && p.in_piece == 16 && p.dh_piece == 16 && p.out_piece == 16 &&
+                    (maps.status = tb_status_slot(stream));
+        for (int i = 0; i < 4 && bulk; ++i)
+            bulk = encode(&maps.in[i], desc->type, in[i], s, i < 3 ? s.is : s.os, i < 3 ? s.it : s.ot, pass);
+        for (int i = 0; i < 3 && bulk; ++i) bulk = encode(&maps.out[i], desc->type, out[i], s, s.gs, s.gt, pass);
+        return bulk ? launch_units<recurrence_backward<T, true>>(units, pass, warps, shared, st, p, split, maps)
+                    : launch_units<recurrence_backward<T, false>>(units, pass, warps, shared, st, p, split, maps);
     });
     if (!ok || !ddecay) return ok;
     const size_t rows = partial_rows(s, split), parts = column_parts(rows);
