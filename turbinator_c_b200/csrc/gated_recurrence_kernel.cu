@@ -103,12 +103,12 @@ __device__ __forceinline__ int live_of(const RecurrenceShape &d, const int32_t *
 /* Of `live` steps those of the span from step t on. */
 template <int STEPS = kSteps> __device__ __forceinline__ int of_span(int live, int t) { return min(max(live - t, 0), STEPS); }
 
-/* e^l - 1 for -kNear <= l <= 0 from its series; the next term is below 2e-8
- * of it. */
-constexpr float kNear = 0.35f;
-__device__ __forceinline__ F2 expm1_near(F2 l) {
-    F2 q = fma2(l, both(1.0f / 5040.0f), both(1.0f / 720.0f));
-    q = fma2(q, l, both(1.0f / 120.0f));
+/* e^l - 1 from its series, the next term below 5e-8 of it: for -kNear <= l <= 0
+ * with five terms, for -kSeries <= l with seven. */
+constexpr float kNear = 0.125f, kSeries = 0.35f;
+template <bool NEAR> __device__ __forceinline__ F2 expm1_series(F2 l) {
+    F2 q = both(1.0f / 120.0f);
+    if (!NEAR) q = fma2(fma2(l, both(1.0f / 5040.0f), both(1.0f / 720.0f)), l, q);
     q = fma2(q, l, both(1.0f / 24.0f));
     q = fma2(q, l, both(1.0f / 6.0f));
     q = fma2(q, l, both(0.5f));
@@ -119,23 +119,23 @@ __device__ __forceinline__ F2 expm1_near(F2 l) {
 /* Decays of two steps or channels.  p = e^(log a) - 1 keeps the digits of
  * 1 - a^2 = -p (2 + p) where a is near 1.  NEAR: no log a of the warp can be
  * below -kNear (sigmoid <= 1, so the rates decide), which saves the
- * exponential and the choice: 19 of the 50 instructions of a pair's step. */
+ * exponential, the choice and two terms. */
 struct Decay {
     F2 a, beta;
 };
 template <bool NEAR> __device__ __forceinline__ Decay decay_of(F2 rate, F2 open) {
     const F2 l = mul2(rate, open);
-    F2 p = expm1_near(l), a = add2(p, both(1.0f));
+    F2 p = expm1_series<NEAR>(l), a = add2(p, both(1.0f));
     if (!NEAR) {
         float l0, l1, p0, p1, a0, a1;
         split(l, l0, l1);
         split(p, p0, p1);
         split(a, a0, a1);
-        if (!(l0 >= -kNear)) {
+        if (!(l0 >= -kSeries)) {
             a0 = fast_exp2(kLog2e * l0);
             p0 = a0 - 1.0f;
         }
-        if (!(l1 >= -kNear)) {
+        if (!(l1 >= -kSeries)) {
             a1 = fast_exp2(kLog2e * l1);
             p1 = a1 - 1.0f;
         }
