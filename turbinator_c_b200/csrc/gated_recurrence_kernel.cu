@@ -252,6 +252,11 @@ struct alignas(64) Maps {
     CUtensorMap in[4], out[3]; /* x, rec, inp, dh; h or dx, drec, dinp */
     unsigned *status;
 };
+/* What a kernel without them takes in their place. */
+struct NoMaps {
+    unsigned *status;
+};
+template <bool BULK> using MapsOf = std::conditional_t<BULK, Maps, NoMaps>;
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
 __device__ __forceinline__ void load_box(void *to, const CUtensorMap *map, int c, int t, int b, uint32_t bar) {
@@ -497,7 +502,7 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
 /* BULK: by bulk tensor copies. */
 template <class T, bool BULK>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
-recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ Maps maps) {
+recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ MapsOf<BULK> maps) {
     constexpr int V = kForwardV<T>, CT = 32 * V;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ uint64_t bars[kWarps][2]; /* of a stage's boxes */
@@ -768,7 +773,7 @@ __device__ __forceinline__ void backward_span(const T *xs, const T *rs, const T 
  * the saved one through the first's map. */
 template <class T, bool BULK>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
-recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__ Maps maps) {
+recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__ MapsOf<BULK> maps) {
     constexpr int CT = 64, kSlot = kHalf * CT;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ uint64_t bars[kWarps][2]; /* of a stage's boxes */
@@ -1183,14 +1188,16 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
                                                                           shared, st, p, split))
             return 0;
         const unsigned units = split.tiles * split.strips;
+        if (split.strip_rounds < kBulkRounds)
+            return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
         Maps maps{};
-        if (split.strip_rounds >= kBulkRounds && p.in_piece == 16 && p.out_piece == 16 &&
+        if (p.in_piece == 16 && p.out_piece == 16 &&
             (maps.status = tb_status_slot(stream)) && encode(&maps.in[0], desc->type, x, s, s.is, s.it, pass) &&
             encode(&maps.in[1], desc->type, recurrence_gate, s, s.is, s.it, pass) &&
             encode(&maps.in[2], desc->type, input_gate, s, s.is, s.it, pass) &&
             encode(&maps.out[0], desc->type, h, s, s.os, s.ot, pass))
             return launch_units<recurrence_forward<T, true>>(units, pass, warps, shared, st, p, split, maps);
-        return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, maps);
+        return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
     });
 }
 
@@ -1244,7 +1251,7 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
             bulk = encode(&maps.in[i], desc->type, in[i], s, i < 3 ? s.is : s.os, i < 3 ? s.it : s.ot, pass);
         for (int i = 0; i < 3 && bulk; ++i) bulk = encode(&maps.out[i], desc->type, out[i], s, s.gs, s.gt, pass);
         return bulk ? launch_units<recurrence_backward<T, true>>(units, pass, warps, shared, st, p, split, maps)
-                    : launch_units<recurrence_backward<T, false>>(units, pass, warps, shared, st, p, split, maps);
+                    : launch_units<recurrence_backward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
     });
     if (!ok || !ddecay) return ok;
     const size_t rows = partial_rows(s, split), parts = column_parts(rows);

@@ -871,18 +871,20 @@ int pack_of(const NormShape &d, size_t size, const void *a, size_t as, size_t ap
 template <auto Kernel, class... Args>
 int launch_tiles(const NormShape &d, const Tiling &g, bool clusters, size_t shared, cudaStream_t st, Args... args) {
     if (!allow_shared<Kernel>(shared)) return 0;
+    if (!clusters || g.parts == 1) {
+        Kernel<<<static_cast<unsigned>(g.tiles), g.threads, shared, st>>>(d, g, args...);
+        return launched();
+    }
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(static_cast<unsigned>(g.tiles));
     c.blockDim = dim3(static_cast<unsigned>(g.threads));
     c.dynamicSmemBytes = shared;
     c.stream = st;
     cudaLaunchAttribute a{};
-    if (clusters && g.parts > 1) {
-        a.id = cudaLaunchAttributeClusterDimension;
-        a.val.clusterDim = {static_cast<unsigned>(g.parts), 1, 1};
-        c.attrs = &a;
-        c.numAttrs = 1;
-    }
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim = {static_cast<unsigned>(g.parts), 1, 1};
+    c.attrs = &a;
+    c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, Kernel, d, g, args...) == cudaSuccess;
 }
 
