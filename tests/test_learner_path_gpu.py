@@ -1,0 +1,160 @@
+"""The learner layers together: the example's training and acting, capture into a CUDA graph, and corners of the
+selection that random logits seldom reach."""
+from __future__ import annotations
+
+import importlib.util
+import os
+
+import pytest
+
+import turbinator_c_b200 as tb
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def example():
+    spec = importlib.util.spec_from_file_location("learner_step", os.path.join(ROOT, "examples", "learner_step.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_example_learns_and_acts_as_it_was_trained(example):
+    actor = example.Actor(dtype=torch.float32)
+    losses = example.train(actor, aircraft=8, steps=20, updates=30)
+    assert losses[-1] < 0.5 * losses[0], losses
+    proprio, luma, reset = example.trajectories(3, 18, seed=1)
+    with torch.no_grad():
+        whole = actor(proprio, luma, torch.zeros((3, actor.width), device="cuda"), reset)[0]
+    # two orders of the same sums in f32, through layers of a few hundred terms
+    assert torch.allclose(example.act(actor, proprio, luma, reset), whole, rtol=1e-3, atol=1e-3)
+
+
+def test_example_gradient_is_the_difference(example):
+    """The loss's change along a random direction of all parameters, by the layers' gradients and by differences."""
+    actor = example.Actor(width=32, experts=4, stem=16, dtype=torch.float32, seed=3)
+    proprio, luma, reset = example.trajectories(4, 17, seed=2)
+    first = torch.zeros((4, actor.width), device="cuda")
+
+    def loss():
+        guess, _, _ = actor(proprio[:, :-1], luma[:, :-1], first, reset[:, :-1].contiguous())
+        return (guess - proprio[:, 1:]).double().square().mean()
+
+    loss().backward()
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(0)
+    ways = [torch.randn(p.shape, generator=gen, device="cuda") * p.detach().abs().mean() for p in actor.parameters()]
+    # a few tokens may change experts along the way: the router keeps its logits
+    ways = [torch.zeros_like(w) if p is actor.router else w for p, w in zip(actor.parameters(), ways)]
+    slope = sum(float((p.grad.double() * w.double()).sum()) for p, w in zip(actor.parameters(), ways))
+
+    def at(step):
+        with torch.no_grad():
+            for p, w in zip(actor.parameters(), ways):
+                p.add_(w, alpha=step)
+            value = float(loss())
+            for p, w in zip(actor.parameters(), ways):
+                p.sub_(w, alpha=step)
+        return value
+
+    # the difference's own error: curvature (step^2) and f32 rounding of the loss (about 1e-6 / step)
+    step = 2e-3
+    assert abs((at(step) - at(-step)) / (2 * step) - slope) < 0.03 * abs(slope) + 2e-3
+
+
+def test_layers_captured_in_a_cuda_graph():
+    """A step of every layer, forward and backward, replays with the bits of the direct calls."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(4)
+    new = lambda *s, kind=torch.float32: torch.randn(s, generator=gen, device="cuda").to(kind)  # noqa: E731
+    bf = torch.bfloat16
+    n, p, c, g = 12, 300, 64, 8
+    norm = tb.GroupNormDesc(samples=n, positions=p, channels=c, groups=g, type=1, activation=2, epsilon=1e-5)
+    x, dy, gamma, beta = new(n, p, c, kind=bf), new(n, p, c, kind=bf), new(c), new(c)
+    y, dx, mean, rstd = torch.empty_like(x), torch.empty_like(x), new(n, g), new(n, g)
+    dgamma, dbeta = new(c), new(c)
+    b, t, d = 400, 300, 64  # many rounds: bulk copies; and strips, with three sequences
+    long = tb.GatedRecurrenceDesc(sequences=b, steps=t, channels=d, type=1, decay_scale=8.0)
+    few = tb.GatedRecurrenceDesc(sequences=3, steps=b * t // 3, channels=d, type=1, decay_scale=8.0)
+    seq = [new(b, t, d, kind=bf) for _ in range(4)]
+    decay, h = new(d) - 3, new(b, t, d, kind=bf)
+    saved = [new(b, -(-t // 16), d), new(3, -(-(b * t // 3) // 16), d)]
+    grads = [[torch.empty_like(h) for _ in range(3)] + [new(d)] for _ in range(2)]
+    tok, e, k = 3000, 96, 4
+    route = tb.ExpertRouteDesc(tokens=tok, experts=e, top_k=k, groups=1, top_groups=1, group_best=1, type=0, score=1,
+                               renormalise=1, weight_scale=1.0)
+    logits, bias, dw, dlogits = new(tok, e), new(e) * 0.01, new(tok, k), new(tok, e)
+    whole = lambda *s: torch.empty(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    ids, offsets, order, position, weights = whole(tok, k), whole(e + 1), whole(tok * k), whole(tok, k), new(tok, k)
+    comb = tb.ExpertCombineDesc(tokens=tok, rows=tok * k, width=72, top_k=k, type=1)
+    rows, out, dout = new(tok * k, 72, kind=bf), new(tok, 72, kind=bf), new(tok, 72, kind=bf)
+    drows, dweights = torch.empty_like(rows), new(tok, k)
+    need = max(tb.tb_cuda_group_norm_workspace(norm), tb.tb_cuda_gated_recurrence_workspace(long),
+               tb.tb_cuda_gated_recurrence_workspace(few), tb.tb_cuda_route_experts_workspace(route))
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+
+    def step():
+        assert tb.tb_cuda_group_norm_device(norm, x, gamma, beta, y, mean, rstd, work, s) == 1
+        assert tb.tb_cuda_group_norm_backward_device(norm, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta, work, s) == 1
+        for desc, keep, grad in zip((long, few), saved, grads):
+            assert tb.tb_cuda_gated_recurrence_device(desc, *seq[:3], decay, None, None, None, h, None, keep, work, s) == 1
+            assert tb.tb_cuda_gated_recurrence_backward_device(desc, *seq[:3], decay, None, None, keep, seq[3], None,
+                                                               *grad, None, work, s) == 1
+        assert tb.tb_cuda_route_experts_device(route, logits, bias, ids, weights, offsets, order, position, work, s) == 1
+        assert tb.tb_cuda_route_experts_backward_device(route, logits, ids, dw, dlogits, s) == 1
+        assert tb.tb_cuda_combine_experts_device(comb, rows, position, weights, out, s) == 1
+        assert tb.tb_cuda_combine_experts_backward_device(comb, rows, position, weights, dout, drows, dweights, s) == 1
+
+    outputs = [y, dx, mean, rstd, dgamma, dbeta, h, *saved, *grads[0], *grads[1], ids, weights, offsets, order, position,
+               dlogits, out, drows, dweights]
+    torch.cuda.synchronize()
+    step()
+    s.synchronize()
+    direct = [v.clone() for v in outputs]
+    for v in outputs:
+        v.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(direct, outputs))
+    assert tb.tb_cuda_synchronize(s) == 1
+
+
+@pytest.mark.parametrize("kind", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("experts", (64, 256, 512, 1000))
+def test_route_best_experts_next_to_each_other(kind, experts):
+    """All of a token's best experts in one run, wherever it starts, in any order of their logits, and with ties."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(7)
+    t, k = 200, 12
+    logits = torch.randn((t, experts), generator=gen, device="cuda").clamp(-3, 3)
+    for i in range(t):
+        first = (i * 7) % (experts - k - 4)
+        run = torch.randperm(k + 4, generator=gen, device="cuda").float() * 0.25 + 5.0
+        logits[i, first:first + k + 4] = 5.0 if i % 5 == 0 else run
+    logits = logits.to(kind)
+    desc = tb.ExpertRouteDesc(tokens=t, experts=experts, top_k=k, groups=1, top_groups=1, group_best=1,
+                              type={torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[kind], score=0, renormalise=1,
+                              weight_scale=1.0)
+    ids, weights = torch.empty((t, k), dtype=torch.int32, device="cuda"), torch.empty((t, k), device="cuda")
+    work = torch.empty(tb.tb_cuda_route_experts_workspace(desc), dtype=torch.uint8, device="cuda")
+    assert tb.tb_cuda_route_experts_device(desc, logits, None, ids, weights, None, None, None, work) == 1
+    torch.cuda.synchronize()
+    want = logits.float().sort(dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(ids.long(), want)
+    # with a bias (ranked by scores): the same experts where the bias is nothing and no two scores are alike
+    zero = torch.zeros(experts, device="cuda")
+    assert tb.tb_cuda_route_experts_device(desc, logits, zero, ids, weights, None, None, None, work) == 1
+    torch.cuda.synchronize()
+    distinct = torch.arange(t, device="cuda") % 5 != 0
+    assert torch.equal(ids.long()[distinct], want[distinct])
