@@ -28,7 +28,8 @@ using namespace tb_learn;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128;         /* of a CTA */
+constexpr int kBackwardThreads = 256;
 constexpr int kCluster = 8; /* CTAs of a cluster at most */
 
 struct NormShape {
@@ -45,8 +46,10 @@ struct Tiling {
     int block_groups, lanes; /* groups and packs of a tile's row */
     int blocks, threads, rows_at_once;
     int rows, parts;         /* positions of a part */
-    int rows_held;           /* positions that the tile has room for */
+    int turns;               /* packs of a thread that the tile has room for */
     int share;               /* threads that add up a channel's total: a power of two */
+    bool folds;              /* rows of a warp fold by shuffles: lanes divides 32 */
+    int sum_rows;            /* rows of partial sums that meet in shared memory */
     unsigned magic_parts, magic_blocks, magic_lanes, magic_rows, magic_group; /* floor((2^32 - 1) / ..), rows: rows_at_once */
     bool fits;               /* the parts fit one cluster */
     size_t tiles;            /* of all samples */
@@ -139,16 +142,17 @@ template <class T, int PACK> __device__ __forceinline__ void copy_pack(Held<T, P
         *to = *reinterpret_cast<const Held<T, PACK> *>(from);
 }
 
-/* Starts copying the thread's packs into its places of the tile (to[i * step]
- * is its i-th); it reads no others, so that its own wait will do. */
-template <class T, int PACK>
-__device__ __forceinline__ void load_tile(Held<T, PACK> *to, int step, const T *p, size_t stride, const Seat &s, const Tiling &g) {
+/* Starts copying the thread's packs into its places of the tile (to[i * STEP]
+ * is its i-th; STEP: of the widest CTA, so that places are known offsets); it
+ * reads no others, so that its own wait will do. */
+template <int STEP, class T, int PACK>
+__device__ __forceinline__ void load_tile(Held<T, PACK> *to, const T *p, size_t stride, const Seat &s, const Tiling &g) {
     p += (s.first + s.row) * stride + s.c0 + s.lane * PACK;
     const size_t jump = g.rows_at_once * stride;
 #pragma unroll 4
     for (int i = 0; i < s.mine; ++i) {
         copy_pack<T, PACK>(to, p);
-        to += step;
+        to += STEP;
         p += jump;
     }
 }
@@ -212,7 +216,7 @@ template <class T, int PACK> __device__ __forceinline__ void put(T *to, const Ar
 
 /* Shared memory of a tile: rows of per-channel partial sums, of N values a
  * channel, their totals, backward the channels' scale, per group four values,
- * and the tile (x, then dy). */
+ * and the tile (x, then du). */
 struct Sums {
     float *rows, *channel, *scale, *group;
     unsigned char *tile;
@@ -223,50 +227,65 @@ template <int N> __device__ __forceinline__ Sums sums_of(float *shared, const Ti
     s.channels = (g.lanes * g.pack + 3) & ~3;
     s.pitch = N * s.channels + 4;
     s.rows = shared;
-    s.channel = shared + g.rows_at_once * s.pitch;
+    s.channel = shared + g.sum_rows * s.pitch;
     s.scale = s.channel + N * s.channels;
     s.group = s.scale + (N > 1 ? s.channels : 0);
     s.tile = reinterpret_cast<unsigned char *>(s.group + 4 * g.block_groups);
     return s;
 }
-/* n: 1 forward, 2 backward, of tensors as of values. */
-size_t shared_bytes(const Tiling &g, size_t size, int n) {
+/* n: values a channel, 1 forward and 2 backward, where du is kept too, in f32. */
+size_t shared_bytes(const Tiling &g, size_t size, int n, bool du) {
     const size_t channels = (static_cast<size_t>(g.lanes) * g.pack + 3) & ~size_t(3);
-    return (g.rows_at_once * (n * channels + 4) + (n > 1 ? n + 1 : n) * channels + 4 * g.block_groups) * sizeof(float) +
-           static_cast<size_t>(n) * g.rows_held * g.lanes * g.pack * size;
+    const size_t places = static_cast<size_t>(g.turns) * (n > 1 ? kBackwardThreads : kThreads) * g.pack;
+    return (g.sum_rows * (n * channels + 4) + (n > 1 ? n + 1 : n) * channels + 4 * g.block_groups) * sizeof(float) +
+           places * (size + (du ? sizeof(float) : 0));
 }
 
 /* channel[i * s.channels + c] = the sum over the CTA's rows of each thread's
  * own[i]; ends with the totals visible to all. */
 template <int PACK, int N>
 __device__ __forceinline__ void channel_totals(const Array<PACK> (&own)[N], const Sums &s, const Seat &at, const Tiling &g) {
-    if (at.in) {
+    float e[N][PACK];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(e[i] + 2 * k, own[i][k]);
+    bool leaves = at.in;
+    int row = at.row;
+    if (g.folds) {
+        for (int o = g.lanes; o < 32; o *= 2)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int v = 0; v < PACK; ++v) e[i][v] += __shfl_xor_sync(0xffffffffu, e[i][v], o);
+        leaves = at.in && threadIdx.x % 32 < g.lanes;
+        row = threadIdx.x / 32;
+    }
+    if (leaves) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float e[PACK];
-#pragma unroll
-            for (int k = 0; k < Values<PACK>::kCount; ++k) vstore(e + 2 * k, own[i][k]);
-            float *to = s.rows + at.row * s.pitch + i * s.channels + at.lane * PACK;
+            float *to = s.rows + row * s.pitch + i * s.channels + at.lane * PACK;
             if constexpr (PACK % 4 == 0) {
 #pragma unroll
                 for (int v = 0; v < PACK; v += 4)
-                    *reinterpret_cast<float4 *>(to + v) = make_float4(e[v], e[v + 1], e[v + 2], e[v + 3]);
+                    *reinterpret_cast<float4 *>(to + v) = make_float4(e[i][v], e[i][v + 1], e[i][v + 2], e[i][v + 3]);
             } else {
 #pragma unroll
-                for (int v = 0; v < PACK; ++v) to[v] = e[v];
+                for (int v = 0; v < PACK; ++v) to[v] = e[i][v];
             }
         }
     }
     __syncthreads();
     /* g.share neighbouring threads for each total */
-    const int mine = threadIdx.x & (g.share - 1);
-    for (int c = threadIdx.x / g.share; c < N * s.channels; c += blockDim.x / g.share) {
+    const int mine = threadIdx.x & (g.share - 1), each = blockDim.x / g.share;
+    for (int base = 0; base < N * s.channels; base += each) {
+        const int c = base + threadIdx.x / g.share;
         float t = 0.0f;
+        if (c < N * s.channels)
 #pragma unroll 4
-        for (int r = mine; r < g.rows_at_once; r += g.share) t += s.rows[r * s.pitch + c];
-        /* whole warps are here: blockDim.x / share divides by 32 / share, and channels by 4 */
-        for (int o = 1; o < g.share; o *= 2) t += __shfl_xor_sync(__activemask(), t, o);
-        if (mine == 0) s.channel[c] = t;
+            for (int r = mine; r < g.sum_rows; r += g.share) t += s.rows[r * s.pitch + c];
+        for (int o = 1; o < g.share; o *= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (mine == 0 && c < N * s.channels) s.channel[c] = t;
     }
     __syncthreads();
 }
@@ -295,7 +314,7 @@ __device__ __forceinline__ void group_totals(const NormShape &d, const Seat &at,
 /* Leaves the tile's own mean and squares about it of each group in
  * s.group[2 * group], [2 * group + 1]; visible to all. */
 template <class T, int PACK>
-__device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int step, const Sums &s, const Seat &at,
+__device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, const Sums &s, const Seat &at,
                                                 const NormShape &d, const Tiling &g) {
     using V = typename Values<PACK>::V;
     constexpr int N = Values<PACK>::kCount;
@@ -304,7 +323,7 @@ __device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int s
     for (int k = 0; k < N; ++k) own[0][k] = vall<V>(0.0f);
 #pragma unroll 4
     for (int i = 0; i < at.mine; ++i) {
-        taken<T, PACK>(tile[i * step], e);
+        taken<T, PACK>(tile[i * kThreads], e);
 #pragma unroll
         for (int k = 0; k < N; ++k) own[0][k] = vadd(own[0][k], e[k]);
     }
@@ -317,7 +336,7 @@ __device__ __forceinline__ void tile_statistics(const Held<T, PACK> *tile, int s
     for (int k = 0; k < N; ++k) own[0][k] = vall<V>(0.0f);
 #pragma unroll 4
     for (int i = 0; i < at.mine; ++i) {
-        taken<T, PACK>(tile[i * step], e);
+        taken<T, PACK>(tile[i * kThreads], e);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const V off = vadd(e[k], less.v[k]);
@@ -351,10 +370,9 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
     const Seat at = seat_of(d, g, blockIdx.x);
     const Sums s = sums_of<1>(shared, g);
     Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
-    const int step = g.rows_at_once * g.lanes;
-    load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
+    load_tile<kThreads, T, PACK>(tile, x + at.n * d.xs, d.xp, at, g);
     tile_loaded();
-    tile_statistics<T, PACK>(tile, step, s, at, d, g);
+    tile_statistics<T, PACK>(tile, s, at, d, g);
     if constexpr (!WHOLE) {
         for (int i = threadIdx.x; i < 2 * g.block_groups; i += blockDim.x)
             partial[static_cast<size_t>(blockIdx.x) * 2 * g.block_groups + i] = s.group[i];
@@ -397,10 +415,10 @@ norm_forward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const 
         f.shift = parameters_of<PACK>(at, beta, 0.0f);
         T *p = y + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
         const size_t jump = g.rows_at_once * d.yp;
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < at.mine; ++i) {
             Array<PACK> e;
-            taken<T, PACK>(tile[i * step], e);
+            taken<T, PACK>(tile[i * kThreads], e);
             result<PACK>(e, f, d.act);
             put<T, PACK>(p, e);
             p += jump;
@@ -534,11 +552,13 @@ __device__ __forceinline__ void input_gradient(Array<PACK> &z, const Array<PACK>
         z[k] = vfma(du[k], f.scale.v[k], vfma(z[k], l.n2.v[k], l.n1.v[k]));
 }
 
-/* The tile's sums and, where the whole sample's groups are in the cluster, dx.
+/* The tile's sums and, where the whole sample's groups are in the cluster, dx:
+ * du, found once, waits for the sums in shared memory in f32 (twice the bytes
+ * of a 16-bit dy, but the activation's slope costs more than that again).
  * Per-channel sums go to partial [samples, parts, 2, channels], and where the
  * sample is larger the groups' to sums [samples, parts, 2, groups]. */
 template <class T, int PACK, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kBackwardThreads, 2)
 norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const T *dy, T *dx, float *partial, float *sums) {
     using V = typename Values<PACK>::V;
@@ -546,11 +566,26 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
     extern __shared__ __align__(16) float shared[];
     const Seat at = seat_of(d, g, blockIdx.x);
     const Sums s = sums_of<2>(shared, g);
-    const int step = g.rows_at_once * g.lanes;
+    constexpr int STEP = kBackwardThreads;
     Held<T, PACK> *const tile = reinterpret_cast<Held<T, PACK> *>(s.tile) + threadIdx.x;
-    Held<T, PACK> *const tile_dy = tile + g.rows_held * g.lanes;
-    load_tile<T, PACK>(tile, step, x + at.n * d.xs, d.xp, at, g);
-    load_tile<T, PACK>(tile_dy, step, dy + at.n * d.ys, d.yp, at, g);
+    V *const kept = reinterpret_cast<V *>(s.tile + static_cast<size_t>(g.turns) * STEP * sizeof(Held<T, PACK>)) +
+                    threadIdx.x; /* [turns][N][STEP] */
+    load_tile<STEP, T, PACK>(tile, x + at.n * d.xs, d.xp, at, g);
+    const T *from = dy + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
+    const size_t from_jump = g.rows_at_once * d.yp;
+    Held<T, PACK> next[kAhead];
+    const auto load = [&](int i) {
+        if (i + kAhead <= at.mine) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) next[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * from_jump);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (i + j < at.mine) next[j] = *reinterpret_cast<const Held<T, PACK> *>(from + j * from_jump);
+        }
+        from += kAhead * from_jump;
+    };
+    load(0);
     const Given<PACK> f = given_of<PACK>(d, g, at, gamma, beta, mean, rstd);
     if (at.in && at.row == 0) /* for the groups' sums */
 #pragma unroll
@@ -560,16 +595,30 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
         Array<PACK> own[2]; /* sums of du and of du z */
 #pragma unroll
         for (int k = 0; k < N; ++k) own[0][k] = own[1][k] = vall<V>(0.0f);
-#pragma unroll 2
-        for (int i = 0; i < at.mine; ++i) {
+        const auto take = [&](const Held<T, PACK> &w, int i) {
             Array<PACK> z, du;
-            taken<T, PACK>(tile[i * step], z);
-            taken<T, PACK>(tile_dy[i * step], du);
+            taken<T, PACK>(tile[i * STEP], z);
+            taken<T, PACK>(w, du);
             gradients<PACK>(z, du, f, d.act);
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 own[0][k] = vadd(own[0][k], du[k]);
                 own[1][k] = vfma(du[k], z[k], own[1][k]);
+                if (WHOLE) kept[(i * N + k) * STEP] = du[k];
+            }
+        };
+        for (int i = 0; i < at.mine; i += kAhead) {
+            Held<T, PACK> w[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) w[j] = next[j];
+            load(i + kAhead);
+            if (i + kAhead <= at.mine) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) take(w[j], i + j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kAhead - 1; ++j)
+                    if (i + j < at.mine) take(w[j], i + j);
             }
         }
         channel_totals<PACK, 2>(own, s, at, g);
@@ -608,12 +657,15 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
         const Less<PACK> l = less_of<PACK>(d, g, at, rstd, merged);
         T *p = dx + at.n * d.xs + (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
         const size_t jump = g.rows_at_once * d.xp;
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < at.mine; ++i) {
             Array<PACK> z, du;
-            taken<T, PACK>(tile[i * step], z);
-            taken<T, PACK>(tile_dy[i * step], du);
-            gradients<PACK>(z, du, f, d.act);
+            taken<T, PACK>(tile[i * STEP], z);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                z[k] = vadd(z[k], f.less.v[k]);
+                du[k] = kept[(i * N + k) * STEP];
+            }
             input_gradient<PACK>(z, du, f, l);
             put<T, PACK>(p, z);
             p += jump;
@@ -646,7 +698,7 @@ norm_merge_sums(NormShape d, size_t parts, const float *sums, float *means) {
 }
 
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kBackwardThreads, 2)
 norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const float *means, const T *dy, T *dx) {
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
@@ -813,20 +865,22 @@ bool norm_shape(const tb_group_norm_desc *d, NormShape *s) {
     return true;
 }
 
-/* Bytes of a tile of one tensor: six such CTAs (backward: three) share an SM;
- * the large size is for maps that fit a cluster by it. */
-constexpr size_t kTile = 32768, kLargeTile = 92160;
+/* Bytes of a tile of x: six such CTAs (backward, with du: two of 16-bit types,
+ * three of f32) share an SM; the large sizes are for maps that fit a cluster by
+ * them. */
+constexpr size_t kTile = 32768, kLargeTile = 92160, kLargeBackwardTile = 57344;
 
 /* Tiles for packs of `pack` elements; false where a group is wider than a
  * CTA's rows (or the tiles are too many to count). */
-bool tiling_of(const NormShape &d, int pack, size_t size, Tiling *g) {
+bool tiling_of(const NormShape &d, int pack, size_t size, bool backward, Tiling *g) {
+    const int most_threads = backward ? kBackwardThreads : kThreads;
     /* whole groups, whole packs, 128 bytes a row if there are: narrower rows
      * waste sectors, wider ones leave fewer and longer tiles */
     bool found = false;
     for (int i = 1; i <= d.groups && !found; ++i) {
         if (static_cast<size_t>(i) * d.per_group % pack) continue;
         const size_t lanes = static_cast<size_t>(i) * d.per_group / pack;
-        if (lanes > kThreads) break;
+        if (lanes > static_cast<size_t>(most_threads)) break;
         g->block_groups = i;
         g->lanes = static_cast<int>(lanes);
         found = lanes * pack * size >= 128 || i == d.groups;
@@ -835,22 +889,24 @@ bool tiling_of(const NormShape &d, int pack, size_t size, Tiling *g) {
     g->pack = pack;
     g->blocks = (d.groups + g->block_groups - 1) / g->block_groups;
     const size_t packs = d.positions * g->lanes;
-    const size_t threads = packs < kThreads ? align_up(packs, 32) : kThreads;
+    const size_t threads = packs < static_cast<size_t>(most_threads) ? align_up(packs, 32) : most_threads;
     g->threads = static_cast<int>(threads);
     g->rows_at_once = g->threads / g->lanes;
-    for (const size_t bytes : {kTile, kLargeTile, kTile}) {
-        const size_t turns = bytes / (static_cast<size_t>(g->rows_at_once) * g->lanes * pack * size);
+    for (const size_t bytes : {kTile, backward ? kLargeBackwardTile : kLargeTile, kTile}) {
+        const size_t turns = bytes / (static_cast<size_t>(most_threads) * pack * size);
         const size_t most = static_cast<size_t>(g->rows_at_once) * (turns ? turns : 1);
         const size_t parts = (d.positions + most - 1) / most;
         const size_t rows = align_up((d.positions + parts - 1) / parts, g->rows_at_once);
         if (product(d.samples * g->blocks, parts, 0x7fffffffu, &g->tiles) == false) return false;
         g->rows = static_cast<int>(rows);
-        g->rows_held = static_cast<int>(rows);
+        g->turns = static_cast<int>(rows / g->rows_at_once);
         g->parts = static_cast<int>((d.positions + rows - 1) / rows);
         g->fits = g->parts <= kCluster;
         if (g->fits) break;
     }
     g->tiles = d.samples * g->blocks * g->parts;
+    g->folds = 32 % g->lanes == 0;
+    g->sum_rows = g->folds ? g->threads / 32 : g->rows_at_once;
     g->share = 1;
     while (g->share < 32 && g->share * 2 * g->lanes * pack <= g->threads) g->share *= 2;
     const auto magic = [](unsigned by) { return static_cast<unsigned>(0xffffffffull / by); };
@@ -912,10 +968,9 @@ extern "C" size_t tb_cuda_group_norm_workspace(const tb_group_norm_desc *desc) {
     /* for whichever pack the pointers turn out to allow */
     for (int pack : {static_cast<int>(16 / size), static_cast<int>(4 / size), 1}) {
         Tiling g;
-        if (s.channels % pack || !tiling_of(s, pack, size, &g)) continue;
-        const size_t f = g.fits ? 0 : forward_bytes(s, g), b = backward_bytes(s, g.parts);
-        need = f > need ? f : need;
-        need = b > need ? b : need;
+        if (s.channels % pack) continue;
+        if (tiling_of(s, pack, size, false, &g) && !g.fits && forward_bytes(s, g) > need) need = forward_bytes(s, g);
+        if (tiling_of(s, pack, size, true, &g) && backward_bytes(s, g.parts) > need) need = backward_bytes(s, g.parts);
     }
     return need;
 }
@@ -937,7 +992,7 @@ extern "C" int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const v
         T *out = static_cast<T *>(y);
         Tiling g;
         const int pack = pack_of(s, size, x, s.xs, s.xp, y, s.ys, s.yp);
-        if (!tiling_of(s, pack, size, &g)) {
+        if (!tiling_of(s, pack, size, false, &g)) {
             norm_forward_wide<T><<<static_cast<unsigned>(s.samples * s.groups), kThreads, 0, st>>>(s, in, gamma, beta, out,
                                                                                              mean, rstd);
             return launched();
@@ -945,11 +1000,11 @@ extern "C" int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const v
         return with_pack<T>(pack, [&](auto p) {
             constexpr int P = decltype(p)::value;
             if (g.fits)
-                return launch_tiles<norm_forward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 1), st, in, gamma, beta, out, mean,
+                return launch_tiles<norm_forward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 1, false), st, in, gamma, beta, out, mean,
                                     rstd, static_cast<float *>(nullptr));
             float *means = static_cast<float *>(workspace), *partial = means + 2 * s.samples * s.groups;
             float *m = mean ? mean : means, *r = rstd ? rstd : means + s.samples * s.groups;
-            if (!launch_tiles<norm_forward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 1), st, in, gamma, beta, out, m, r, partial))
+            if (!launch_tiles<norm_forward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 1, false), st, in, gamma, beta, out, m, r, partial))
                 return 0;
             norm_merge<<<merge_grid(s), kThreads, 0, st>>>(s, g, partial, m, r);
             if (!launched()) return 0;
@@ -979,7 +1034,7 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
         float *partial = static_cast<float *>(workspace);
         const uintptr_t both = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dx);
         const int pack = pack_of(s, size, reinterpret_cast<const void *>(both), s.xs, s.xp, dy, s.ys, s.yp);
-        const bool wide = !tiling_of(s, pack, size, &g);
+        const bool wide = !tiling_of(s, pack, size, true, &g);
         const size_t rows = s.samples * (wide ? 1 : g.parts), parts = column_parts(rows);
         float *columns = partial + rows * 2 * s.channels, *sums = columns + parts * 2 * s.channels;
         float *rows_to = wide || dgamma || dbeta ? partial : nullptr;
@@ -991,10 +1046,10 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
             const int ok = with_pack<T>(pack, [&](auto p) {
                 constexpr int P = decltype(p)::value;
                 if (g.fits)
-                    return launch_tiles<norm_backward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 2), st, in, gamma, beta, mean,
+                    return launch_tiles<norm_backward_tiles<T, P, true>>(s, g, true, shared_bytes(g, size, 2, true), st, in, gamma, beta, mean,
                                         rstd, grad, out, rows_to, sums);
                 float *means = sums + rows * 2 * s.groups;
-                if (!launch_tiles<norm_backward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 2), st, in, gamma, beta, mean, rstd,
+                if (!launch_tiles<norm_backward_tiles<T, P, false>>(s, g, false, shared_bytes(g, size, 2, false), st, in, gamma, beta, mean, rstd,
                                   grad, out, rows_to, sums))
                     return 0;
                 norm_merge_sums<<<merge_grid(s), kThreads, 0, st>>>(s, g.parts, sums, means);
