@@ -53,7 +53,7 @@ combine_forward(CombineShape d, int lanes, int chunks, const T *rows, const int3
             for (int k = 0; k < kAhead; ++k) {
                 row[k] = __shfl_sync(0xffffffffu, p, min(j + k, slots - 1), lanes);
                 if (j + k >= slots || c >= d.width) row[k] = -1;
-                if (row[k] >= 0) v[k] = *reinterpret_cast<const Held<T, PACK> *>(rows + row[k] * d.rows_stride + c);
+                if (row[k] >= 0) v[k] = load_once<T, PACK>(rows + row[k] * d.rows_stride + c);
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
@@ -112,7 +112,7 @@ combine_backward(CombineShape d, int warps, const T *rows, const int32_t *positi
                     row[k] = __shfl_sync(0xffffffffu, p, min(j + k, d.top_k - 1));
                     if (j + k >= d.top_k || !in) row[k] = -1;
                     if (row[k] >= 0 && dweights)
-                        v[k] = *reinterpret_cast<const Held<T, PACK> *>(rows + row[k] * d.rows_stride + c);
+                        v[k] = load_once<T, PACK>(rows + row[k] * d.rows_stride + c);
                 }
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
@@ -122,7 +122,7 @@ combine_backward(CombineShape d, int warps, const T *rows, const int32_t *positi
                         float e[PACK];
 #pragma unroll
                         for (int i = 0; i < N; ++i) vstore(e + 2 * i, vmul(s, g[i]));
-                        *reinterpret_cast<Held<T, PACK> *>(drows + row[k] * d.rows_stride + c) = packed<T, PACK>(e);
+                        store_once<T, PACK>(drows + row[k] * d.rows_stride + c, packed<T, PACK>(e));
                         if (dweights) {
                             unpack(v[k], e);
                             V sum = vall<V>(0.0f);

@@ -90,6 +90,27 @@ template <class T, int N> __device__ __forceinline__ Held<T, N> packed(const flo
     return h;
 }
 
+/* The same to and from global memory for what is used once: first to leave L2. */
+template <class T, int N> __device__ __forceinline__ Held<T, N> load_once(const T *p) {
+    Held<T, N> h;
+    if constexpr (sizeof(h) == 16) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(p));
+        memcpy(&h, &v, 16);
+    } else {
+        h = *reinterpret_cast<const Held<T, N> *>(p);
+    }
+    return h;
+}
+template <class T, int N> __device__ __forceinline__ void store_once(T *p, const Held<T, N> &h) {
+    if constexpr (sizeof(h) == 16) {
+        uint4 v;
+        memcpy(&v, &h, 16);
+        __stcs(reinterpret_cast<uint4 *>(p), v);
+    } else {
+        *reinterpret_cast<Held<T, N> *>(p) = h;
+    }
+}
+
 /* ---- warp reductions (every lane receives the result) ---- */
 
 __device__ __forceinline__ float warp_sum(float v) {
