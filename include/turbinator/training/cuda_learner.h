@@ -53,8 +53,9 @@ extern "C" {
  *   u = gamma_c (x-mean) rstd + beta_c,  y = act(u) */
 typedef struct tb_group_norm_desc {
     size_t samples, positions, channels, groups; /* groups divides channels */
-    size_t x_sample_stride, x_position_stride;   /* of x and dx */
+    size_t x_sample_stride, x_position_stride;   /* of x */
     size_t y_sample_stride, y_position_stride;   /* of y and dy */
+    size_t dx_sample_stride, dx_position_stride; /* of dx */
     int type, activation;
     float epsilon;
 } tb_group_norm_desc;
@@ -69,7 +70,7 @@ int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const void *x, con
                               const float *beta, void *y, float *mean, float *rstd, void *workspace,
                               void *stream);
 
-/* dx as x, dgamma and dbeta [channels] f32 (each NULL: not written), from the
+/* dx [samples, positions, channels], dgamma and dbeta [channels] f32 (each NULL: not written), from the
  * forward pass's x, mean, rstd and dy.  dx may be dy or x (same strides). */
 int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc, const void *x, const float *gamma,
                                        const float *beta, const float *mean, const float *rstd,

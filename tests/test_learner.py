@@ -80,7 +80,7 @@ def _norm(**change):
 @pytest.mark.parametrize("change", [
     dict(samples=0), dict(positions=0), dict(channels=0), dict(groups=0), dict(groups=3), dict(type=3),
     dict(activation=4), dict(activation=-1), dict(epsilon=-1.0), dict(epsilon=float("nan")),
-    dict(x_position_stride=7), dict(y_position_stride=7), dict(samples=2 ** 40), dict(positions=2 ** 62),
+    dict(x_position_stride=7), dict(y_position_stride=7), dict(dx_position_stride=7), dict(samples=2 ** 40), dict(positions=2 ** 62),
     dict(channels=2 ** 33, groups=1)])
 def test_group_norm_refuses_descriptors(change):
     d = _norm(**change)
@@ -103,6 +103,8 @@ def test_group_norm_refuses_pointers():
         args = list(good)
         args[i] = bad
         assert tb.tb_cuda_group_norm_backward_device(_norm(), *args) == 0, (i, bad)
+    assert tb.tb_cuda_group_norm_backward_device(_norm(dx_position_stride=16), FAKE, None, None, FAKE, FAKE, 2 * FAKE,
+                                                 FAKE, None, None, FAKE) == 0
     assert tb.load_library().tb_cuda_group_norm_device(None, *good[:7], None) == 0
 
 

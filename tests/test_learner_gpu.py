@@ -59,7 +59,7 @@ NORM_SHAPES = [
     (1, 1, 4, 1, 0, 0), (2, 1, 64, 2, 0, 0), (3, 7, 24, 8, 0, 0), (2, 256, 32, 8, 0, 0), (5, 100, 64, 64, 0, 0),
     (2, 33, 15, 5, 0, 0), (2, 33, 21, 3, 1, 1), (1, 9, 7, 1, 0, 0), (3, 50, 96, 12, 32, 0), (2, 40, 48, 4, 8, 3),
     (1, 1024, 64, 8, 0, 0), (2, 5000, 16, 4, 0, 0), (1, 65536, 8, 2, 0, 0), (1, 300, 1000, 10, 0, 0),
-    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0),
+    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (2, 23296, 8, 2, 3, 0), (18, 900, 32, 4, 3, 1), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0),
 ]
 
 
@@ -72,7 +72,8 @@ def _norm_case(shape, kind, act, seed, params=True):
     beta = _normal(gen, c, scale=0.3) if params else None
     desc = tb.GroupNormDesc(samples=n, positions=p, channels=c, groups=g, type=code, activation=ACTS[act],
                             epsilon=1e-5, x_sample_stride=p * (c + pad), x_position_stride=c + pad,
-                            y_sample_stride=p * (c + pad), y_position_stride=c + pad)
+                            y_sample_stride=p * (c + pad), y_position_stride=c + pad,
+                            dx_sample_stride=p * (c + pad), dx_position_stride=c + pad)
     return gen, dtype, x, gamma, beta, desc
 
 
@@ -138,6 +139,13 @@ def test_group_norm_backward(shape, kind):
                                                      work) == 1
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(first, (dx, dgamma, dbeta)))
+        # a dense dx from strided x and dy, and nothing written past it
+        desc.dx_sample_stride = desc.dx_position_stride = 0
+        dense, whole = _lay(torch.full((n, p, c), NAN, device="cuda"), dtype)
+        assert tb.tb_cuda_group_norm_backward_device(desc, x, gamma, beta, mean, rstd, dy, dense, None, None, work) == 1
+        torch.cuda.synchronize()
+        ref.check(f"dense dx {act}", dense, want[0], errs[0])
+        assert _untouched(dense, whole, 0)
 
 
 def test_group_norm_in_place_and_partial_outputs():

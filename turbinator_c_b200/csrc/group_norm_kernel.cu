@@ -35,7 +35,7 @@ constexpr int kCluster = 8; /* CTAs of a cluster at most */
 struct NormShape {
     size_t samples, positions;
     int channels, groups, per_group;
-    size_t xs, xp, ys, yp; /* strides of samples and positions */
+    size_t xs, xp, ys, yp, gs, gp; /* strides of samples and positions: x; y and dy; dx */
     int act;
     float epsilon;
 };
@@ -655,8 +655,8 @@ norm_backward_tiles(NormShape d, Tiling g, const T *x, const float *gamma, const
         if (g.parts > 1) cluster.barrier_arrive(); /* no CTA leaves before the others have read */
         __syncthreads();
         const Less<PACK> l = less_of<PACK>(d, g, at, rstd, merged);
-        T *p = dx + at.n * d.xs + (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
-        const size_t jump = g.rows_at_once * d.xp;
+        T *p = dx + at.n * d.gs + (at.first + at.row) * d.gp + at.c0 + at.lane * PACK;
+        const size_t jump = g.rows_at_once * d.gp;
 #pragma unroll 4
         for (int i = 0; i < at.mine; ++i) {
             Array<PACK> z, du;
@@ -702,11 +702,10 @@ __global__ void __launch_bounds__(kBackwardThreads, 2)
 norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const float *beta, const float *mean,
                     const float *rstd, const float *means, const T *dy, T *dx) {
     const Seat at = seat_of(d, g, gridDim.x - 1 - blockIdx.x);
-    const size_t corner = (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
-    const T *from = x + at.n * d.xs + corner;
+    const T *from = x + at.n * d.xs + (at.first + at.row) * d.xp + at.c0 + at.lane * PACK;
     const T *from_dy = dy + at.n * d.ys + (at.first + at.row) * d.yp + at.c0 + at.lane * PACK;
-    T *to = dx + at.n * d.xs + corner;
-    const size_t jump = g.rows_at_once * d.xp, dy_jump = g.rows_at_once * d.yp;
+    T *to = dx + at.n * d.gs + (at.first + at.row) * d.gp + at.c0 + at.lane * PACK;
+    const size_t jump = g.rows_at_once * d.xp, dy_jump = g.rows_at_once * d.yp, to_jump = g.rows_at_once * d.gp;
     const Given<PACK> f = given_of<PACK>(d, g, at, gamma, beta, mean, rstd);
     const size_t first = static_cast<size_t>(at.n) * d.groups + at.block * g.block_groups;
     const Less<PACK> l = less_of<PACK>(d, g, at, rstd, means + 2 * first);
@@ -727,11 +726,11 @@ norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const
                 taken<T, PACK>(w[j], du);
                 gradients<PACK>(z, du, f, d.act);
                 input_gradient<PACK>(z, du, f, l);
-                put<T, PACK>(to + j * jump, z);
+                put<T, PACK>(to + j * to_jump, z);
             }
         from += kPairs * jump;
         from_dy += kPairs * dy_jump;
-        to += kPairs * jump;
+        to += kPairs * to_jump;
     }
 }
 
@@ -834,7 +833,7 @@ norm_backward_wide(NormShape d, const T *x, const float *gamma, const float *bet
         float hat;
         for (size_t p = 0; p < d.positions; ++p) {
             const float du = gradient(p, c, ga, be, &hat);
-            dx[n * d.xs + p * d.xp + c] = from_float<T>(rstd * (fmaf(du, ga, -s1) - hat * s2));
+            dx[n * d.gs + p * d.gp + c] = from_float<T>(rstd * (fmaf(du, ga, -s1) - hat * s2));
         }
     }
 }
@@ -859,7 +858,9 @@ bool norm_shape(const tb_group_norm_desc *d, NormShape *s) {
     s->yp = d->y_position_stride ? d->y_position_stride : d->channels;
     s->xs = d->x_sample_stride ? d->x_sample_stride : d->positions * s->xp;
     s->ys = d->y_sample_stride ? d->y_sample_stride : d->positions * s->yp;
-    if (s->xp < d->channels || s->yp < d->channels) return false;
+    s->gp = d->dx_position_stride ? d->dx_position_stride : d->channels;
+    s->gs = d->dx_sample_stride ? d->dx_sample_stride : d->positions * s->gp;
+    if (s->xp < d->channels || s->yp < d->channels || s->gp < d->channels) return false;
     s->act = d->activation;
     s->epsilon = d->epsilon;
     return true;
@@ -1022,7 +1023,8 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
     const size_t size = type_size(desc->type);
     if (!aligned(x, size) || !aligned(dy, size) || !aligned(dx, size) || !aligned(gamma, 4) || !aligned(beta, 4) ||
         !aligned(mean, 4) || !aligned(rstd, 4) || !aligned(dgamma, 4) || !aligned(dbeta, 4) ||
-        !aligned(workspace, 16) || (dx == dy && (s.xs != s.ys || s.xp != s.yp)))
+        !aligned(workspace, 16) || (dx == dy && (s.gs != s.ys || s.gp != s.yp)) ||
+        (dx == x && (s.gs != s.xs || s.gp != s.xp)))
         return 0;
     cudaGetLastError(); /* report these launches only */
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1032,8 +1034,8 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
         T *out = static_cast<T *>(dx);
         Tiling g;
         float *partial = static_cast<float *>(workspace);
-        const uintptr_t both = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dx);
-        const int pack = pack_of(s, size, reinterpret_cast<const void *>(both), s.xs, s.xp, dy, s.ys, s.yp);
+        const int both = pack_of(s, size, x, s.xs, s.xp, dy, s.ys, s.yp), own = pack_of(s, size, dx, s.gs, s.gp, dx, s.gs, s.gp);
+        const int pack = both < own ? both : own;
         const bool wide = !tiling_of(s, pack, size, true, &g);
         const size_t rows = s.samples * (wide ? 1 : g.parts), parts = column_parts(rows);
         float *columns = partial + rows * 2 * s.channels, *sums = columns + parts * 2 * s.channels;

@@ -37,7 +37,7 @@ class GroupNormDesc(_Desc):
 
     _fields_ = [(n, _c.c_size_t) for n in
                 ("samples", "positions", "channels", "groups", "x_sample_stride", "x_position_stride",
-                 "y_sample_stride", "y_position_stride")] + [
+                 "y_sample_stride", "y_position_stride", "dx_sample_stride", "dx_position_stride")] + [
         ("type", _c.c_int), ("activation", _c.c_int), ("epsilon", _c.c_float)]
 
 
