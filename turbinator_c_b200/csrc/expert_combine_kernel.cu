@@ -90,7 +90,8 @@ combine_backward(CombineShape d, int warps, const T *rows, const int32_t *positi
         if (p >= 0 && static_cast<size_t>(p) >= d.rows) p = -1;
         if (weights) w = weights[t * d.top_k + lane];
     }
-    float total = 0.0f; /* of slot `lane` */
+    dots[warp][lane] = 0.0f;
+    __syncwarp();
     if (t < d.tokens)
         for (size_t base = static_cast<size_t>(part) * 32 * PACK; base < d.width; base += static_cast<size_t>(warps) * 32 * PACK) {
             const size_t c = base + lane * PACK;
@@ -114,10 +115,11 @@ combine_backward(CombineShape d, int warps, const T *rows, const int32_t *positi
                     if (row[k] >= 0 && dweights)
                         v[k] = load_once<T, PACK>(rows + row[k] * d.rows_stride + c);
                 }
+                float dot[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     const V s = vall<V>(__shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1)));
-                    float dot = 0.0f;
+                    dot[k] = 0.0f;
                     if (row[k] >= 0) {
                         float e[PACK];
 #pragma unroll
@@ -130,18 +132,28 @@ combine_backward(CombineShape d, int warps, const T *rows, const int32_t *positi
                             for (int i = 0; i < N; ++i) sum = vfma(g[i], vload<V>(e + 2 * i), sum);
                             float both[2] = {0.0f, 0.0f};
                             vstore(both, sum);
-                            dot = both[0] + both[1];
+                            dot[k] = both[0] + both[1];
                         }
                     }
-                    if (dweights) {
-                        dot = warp_sum(dot);
-                        if (lane == j + k) total += dot;
+                }
+                if (dweights) { /* each half of the warp sums half of the slots, and so on, down to eight lanes a slot */
+                    int spread = 16;
+#pragma unroll
+                    for (int n = kAhead / 2; n; n /= 2, spread /= 2) {
+                        const bool high = lane & spread;
+#pragma unroll
+                        for (int k = 0; k < n; ++k) {
+                            const float mine = high ? dot[k + n] : dot[k];
+                            dot[k] = mine + __shfl_xor_sync(0xffffffffu, high ? dot[k] : dot[k + n], spread);
+                        }
                     }
+                    for (; spread; spread /= 2) dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], spread);
+                    const int slot = j + lane / (32 / kAhead);
+                    if (lane % (32 / kAhead) == 0 && slot < d.top_k) dots[warp][slot] += dot[0];
                 }
             }
         }
     if (!dweights) return;
-    dots[warp][lane] = total;
     __syncthreads();
     if (t < d.tokens && part == 0 && lane < d.top_k) {
         float sum = 0.0f;
