@@ -59,7 +59,7 @@ NORM_SHAPES = [
     (1, 1, 4, 1, 0, 0), (2, 1, 64, 2, 0, 0), (3, 7, 24, 8, 0, 0), (2, 256, 32, 8, 0, 0), (5, 100, 64, 64, 0, 0),
     (2, 33, 15, 5, 0, 0), (2, 33, 21, 3, 1, 1), (1, 9, 7, 1, 0, 0), (3, 50, 96, 12, 32, 0), (2, 40, 48, 4, 8, 3),
     (1, 1024, 64, 8, 0, 0), (2, 5000, 16, 4, 0, 0), (1, 65536, 8, 2, 0, 0), (1, 300, 1000, 10, 0, 0),
-    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (2, 23296, 8, 2, 3, 0), (18, 900, 32, 4, 3, 1), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0),
+    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (2, 23296, 8, 2, 3, 0), (18, 900, 32, 4, 3, 1), (700, 5, 12, 3, 0, 0), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0),
 ]
 
 
@@ -485,7 +485,8 @@ def test_route_backward(case, kind):
 # ---- combine ----
 
 COMBINE_SHAPES = [(1, 1, 1, 0, 0), (7, 2, 33, 0, 0), (61, 6, 520, 0, 0), (40, 8, 128, 8, 0), (30, 3, 264, 8, 4),
-                  (5, 32, 1000, 0, 0), (300, 4, 72, 3, 1), (20, 1, 4096, 0, 0), (10, 12, 2049, 0, 0)]
+                  (5, 32, 1000, 0, 0), (300, 4, 72, 3, 1), (20, 1, 4096, 0, 0), (10, 12, 2049, 0, 0),
+                  (50, 3, 36, 0, 0), (50, 5, 66, 8, 2)]
 
 
 @pytest.mark.parametrize("shape", COMBINE_SHAPES, ids=str)

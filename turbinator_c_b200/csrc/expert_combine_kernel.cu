@@ -178,10 +178,14 @@ bool combine_shape(const tb_expert_combine_desc *d, CombineShape *s) {
            product(d->rows, s->rows_stride, SIZE_MAX / 64, &all) && product(d->tokens, s->out_stride, SIZE_MAX / 64, &all);
 }
 
-/* The packs that every row of both tensors allows. */
-int combine_pack(const CombineShape &s, size_t size, const void *a, const void *b, const void *c) {
-    return pack_of(reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
-                       (s.rows_stride | s.out_stride | s.width) * size, size);
+/* Calls f with the widest pack that every row of the tensors allows, as a
+ * constant; 8 bytes too, for the widths that are no multiple of 16. */
+template <class T, class F>
+int with_row_pack(const CombineShape &s, const void *a, const void *b, const void *c, F &&f) {
+    const size_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
+                        (s.rows_stride | s.out_stride | s.width) * sizeof(T);
+    if (bits % 16 == 8) return f(std::integral_constant<int, 8 / static_cast<int>(sizeof(T))>{});
+    return with_pack<T>(pack_of(bits, sizeof(T)), f);
 }
 
 } /* namespace */
@@ -196,7 +200,7 @@ extern "C" int tb_cuda_combine_experts_device(const tb_expert_combine_desc *desc
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return with_pack<T>(combine_pack(s, size, rows, out, nullptr), [&](auto p) {
+        return with_row_pack<T>(s, rows, out, nullptr, [&](auto p) {
             constexpr int P = decltype(p)::value;
             const size_t packs = (s.width + P - 1) / P;
             int lanes = 1;
@@ -227,7 +231,7 @@ extern "C" int tb_cuda_combine_experts_backward_device(const tb_expert_combine_d
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return with_pack<T>(combine_pack(s, size, rows, dout, drows), [&](auto p) {
+        return with_row_pack<T>(s, rows, dout, drows, [&](auto p) {
             constexpr int P = decltype(p)::value;
             int warps = 1;
             while (warps < kWarps && static_cast<size_t>(warps) * 32 * P < s.width) warps *= 2;

@@ -1009,15 +1009,12 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
     }
 }
 
-/* ddecay from the sums of dlog a / rate over all steps: parts [parts, channels]. */
-__global__ void __launch_bounds__(256)
-recurrence_decay(const float *decay, const float *parts, size_t rows, size_t channels, float scale, float *ddecay) {
-    const size_t c = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= channels) return;
-    float s = 0.0f;
-    for (size_t r = 0; r < rows; ++r) s += parts[r * channels + c];
-    ddecay[c] = -scale / (1.0f + expf(-decay[c])) * s;
-}
+/* ddecay from the sums of dlog a / rate over all steps. */
+struct DecayGradient {
+    const float *decay;
+    float scale, *ddecay;
+    __device__ void operator()(size_t c, float sum) const { ddecay[c] = -scale / (1.0f + expf(-decay[c])) * sum; }
+};
 
 /* ---- host side ---- */
 
@@ -1254,12 +1251,5 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
                     : launch_units<recurrence_backward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
     });
     if (!ok || !ddecay) return ok;
-    const size_t rows = partial_rows(s, split), parts = column_parts(rows);
-    float *sums = partial + rows * s.channels;
-    column_sums<<<dim3(static_cast<unsigned>((s.channels + 31) / 32), static_cast<unsigned>(parts)), kColumnThreads, 0,
-                  st>>>(partial, rows, s.channels, sums);
-    if (!launched()) return 0;
-    recurrence_decay<<<static_cast<unsigned>((s.channels + 255) / 256), 256, 0, st>>>(decay, sums, parts, s.channels,
-                                                                                    s.scale, ddecay);
-    return launched();
+    return sum_columns(partial, partial_rows(s, split), s.channels, DecayGradient{decay, s.scale, ddecay}, st);
 }

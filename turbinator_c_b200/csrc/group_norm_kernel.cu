@@ -734,19 +734,18 @@ norm_backward_apply(NormShape d, Tiling g, const T *x, const float *gamma, const
     }
 }
 
-/* dbeta and dgamma from parts [rows, 2, channels]. */
-__global__ void __launch_bounds__(kThreads)
-norm_parameters(const float *parts, size_t rows, int channels, float *dgamma, float *dbeta) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= 2 * channels) return;
-    float s = 0.0f;
-    for (size_t r = 0; r < rows; ++r) s += parts[r * 2 * channels + c];
-    if (c < channels) {
-        if (dbeta) dbeta[c] = s;
-    } else if (dgamma) {
-        dgamma[c - channels] = s;
+/* dbeta and dgamma from the sums of rows [2, channels]. */
+struct Parameters {
+    int channels;
+    float *dgamma, *dbeta;
+    __device__ void operator()(size_t c, float sum) const {
+        if (c < static_cast<size_t>(channels)) {
+            if (dbeta) dbeta[c] = sum;
+        } else if (dgamma) {
+            dgamma[c - channels] = sum;
+        }
     }
-}
+};
 
 /* ---- groups wider than a CTA's rows: one CTA per (sample, group) ---- */
 
@@ -1062,12 +1061,7 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
             if (!ok) return 0;
         }
         if (!dgamma && !dbeta) return 1;
-        column_sums<<<dim3(static_cast<unsigned>((2 * s.channels + 31) / 32), static_cast<unsigned>(parts)), kColumnThreads,
-                      0, st>>>(partial, rows, 2 * static_cast<size_t>(s.channels), columns);
-        if (!launched()) return 0;
-        norm_parameters<<<(2 * s.channels + kThreads - 1) / kThreads, kThreads, 0, st>>>(columns, parts, s.channels, dgamma,
-                                                                                        dbeta);
-        return launched();
+        return sum_columns(partial, rows, 2 * static_cast<size_t>(s.channels), Parameters{s.channels, dgamma, dbeta}, st);
     });
     return ok_rows;
 }

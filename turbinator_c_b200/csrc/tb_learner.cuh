@@ -216,39 +216,63 @@ __device__ __forceinline__ void vstore(float *f, F2 v) { split(v, f[0], f[1]); }
 
 /* ---- sums over the rows of partial [rows, columns] in f32 ---- */
 
-constexpr int kColumnThreads = 512;       /* 32 columns x 16 rows at a time */
-constexpr size_t kColumnRows = 512;       /* rows that one CTA sums */
-constexpr size_t kColumnParts = 64;       /* parts of the rows at most */
+constexpr int kColumnThreads = 512;      /* 32 columns x 16 rows at a time */
+constexpr size_t kColumnRows = 256;      /* rows that one launch of one CTA a strip of columns sums */
+constexpr size_t kColumnPartRows = 128;  /* rows of a part where there are more */
+constexpr size_t kColumnParts = 128;     /* parts of the rows at most */
 
-/* Part blockIdx.y of the rows of 32 columns; out [gridDim.y, columns]. */
-static __global__ void __launch_bounds__(kColumnThreads)
-column_sums(const float *partial, size_t rows, size_t columns, float *out) {
+/* Part blockIdx.y of the rows of 32 columns; out [gridDim.y, columns], or
+ * last(column, sum) where the rows are one part. */
+template <class Last>
+__global__ void __launch_bounds__(kColumnThreads)
+column_sums(const float *partial, size_t rows, size_t columns, float *out, Last last) {
     __shared__ float sums[16][33];
     const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
     const size_t c = static_cast<size_t>(blockIdx.x) * 32 + lane;
     const size_t per = (rows + gridDim.y - 1) / gridDim.y, first = per * blockIdx.y;
-    const size_t last = first + per < rows ? first + per : rows;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const size_t end = first + per < rows ? first + per : rows;
+    float s[8] = {};
     if (c < columns) {
-        size_t r = first + row;
-        for (; r + 48 < last; r += 64)
+        for (size_t r = first + row; r < end; r += 128)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] += partial[(r + 16 * i) * columns + c];
-        for (; r < last; r += 16) s[0] += partial[r * columns + c];
+            for (int i = 0; i < 8; ++i)
+                if (r + 16 * i < end) s[i] += partial[(r + 16 * i) * columns + c];
     }
-    sums[row][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    sums[row][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (row == 0 && c < columns) {
         float t = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) t += sums[i][lane];
-        out[blockIdx.y * columns + c] = t;
+        if (gridDim.y == 1) last(c, t);
+        else out[blockIdx.y * columns + c] = t;
     }
 }
 
+/* Room behind the partial sums, in rows. */
 inline size_t column_parts(size_t rows) {
-    const size_t p = (rows + kColumnRows - 1) / kColumnRows;
+    if (rows <= kColumnRows) return 1;
+    const size_t p = (rows + kColumnPartRows - 1) / kColumnPartRows;
     return p < kColumnParts ? p : kColumnParts;
+}
+
+inline int launched() { return cudaGetLastError() == cudaSuccess; }
+
+/* Sums the columns of partial [rows, columns], last(column, sum) for each; the
+ * parts' sums go behind it. */
+template <class Last>
+int sum_columns(float *partial, size_t rows, size_t columns, Last last, cudaStream_t st) {
+    const unsigned wide = static_cast<unsigned>((columns + 31) / 32);
+    const size_t parts = column_parts(rows);
+    if (parts > 1) {
+        float *sums = partial + rows * columns;
+        column_sums<<<dim3(wide, static_cast<unsigned>(parts)), kColumnThreads, 0, st>>>(partial, rows, columns, sums, last);
+        if (!launched()) return 0;
+        partial = sums;
+        rows = parts;
+    }
+    column_sums<<<dim3(wide, 1), kColumnThreads, 0, st>>>(partial, rows, columns, static_cast<float *>(nullptr), last);
+    return launched();
 }
 
 /* ---- host side ---- */
@@ -313,8 +337,6 @@ template <class T, class F> inline int with_pack(int pack, F &&f) {
         if (pack == 2) return f(std::integral_constant<int, 2>{});
     return f(std::integral_constant<int, 1>{});
 }
-
-inline int launched() { return cudaGetLastError() == cudaSuccess; }
 
 } /* namespace tb_learn */
 
