@@ -59,7 +59,8 @@ NORM_SHAPES = [
     (1, 1, 4, 1, 0, 0), (2, 1, 64, 2, 0, 0), (3, 7, 24, 8, 0, 0), (2, 256, 32, 8, 0, 0), (5, 100, 64, 64, 0, 0),
     (2, 33, 15, 5, 0, 0), (2, 33, 21, 3, 1, 1), (1, 9, 7, 1, 0, 0), (3, 50, 96, 12, 32, 0), (2, 40, 48, 4, 8, 3),
     (1, 1024, 64, 8, 0, 0), (2, 5000, 16, 4, 0, 0), (1, 65536, 8, 2, 0, 0), (1, 300, 1000, 10, 0, 0),
-    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (2, 23296, 8, 2, 3, 0), (18, 900, 32, 4, 3, 1), (700, 5, 12, 3, 0, 0), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0),
+    (2, 20, 2304, 1, 0, 0), (300, 16, 128, 16, 0, 0), (2, 23296, 8, 2, 3, 0), (18, 900, 32, 4, 3, 1),
+    (700, 5, 12, 3, 0, 0), (1, 30000, 136, 17, 0, 0), (2, 700, 272, 2, 0, 0), (3, 3500, 64, 8, 0, 0),
 ]
 
 

@@ -865,10 +865,14 @@ bool norm_shape(const tb_group_norm_desc *d, NormShape *s) {
     return true;
 }
 
-/* Bytes of a tile of x: six such CTAs (backward, with du: two of 16-bit types,
- * three of f32) share an SM; the large sizes are for maps that fit a cluster by
- * them. */
-constexpr size_t kTile = 32768, kLargeTile = 92160, kLargeBackwardTile = 57344;
+/* Bytes of a tile of x at most: six such CTAs (backward, with du: two of 16-bit
+ * types, three of f32) share an SM.  64 channels of bf16, of 4,096 maps of 256
+ * positions: 61 us forward, 138 backward; tiles of 16 KB 88 and 232.  1,024 maps
+ * of 1,024 positions: 70 and 161 us; tiles of 56 KB 79 and 241; three kernels in
+ * the place of clusters 82 and 208.  Where eight such tiles do not hold a map,
+ * larger ones in a cluster lose against a second read of x: 512 maps of 4,096
+ * positions forward 199 us against 146, of 3,000 backward 392 against 289. */
+constexpr size_t kTile = 32768;
 
 /* Tiles for packs of `pack` elements; false where a group is wider than a
  * CTA's rows (or the tiles are too many to count). */
@@ -892,18 +896,15 @@ bool tiling_of(const NormShape &d, int pack, size_t size, bool backward, Tiling 
     const size_t threads = packs < static_cast<size_t>(most_threads) ? align_up(packs, 32) : most_threads;
     g->threads = static_cast<int>(threads);
     g->rows_at_once = g->threads / g->lanes;
-    for (const size_t bytes : {kTile, backward ? kLargeBackwardTile : kLargeTile, kTile}) {
-        const size_t turns = bytes / (static_cast<size_t>(most_threads) * pack * size);
-        const size_t most = static_cast<size_t>(g->rows_at_once) * (turns ? turns : 1);
-        const size_t parts = (d.positions + most - 1) / most;
-        const size_t rows = align_up((d.positions + parts - 1) / parts, g->rows_at_once);
-        if (product(d.samples * g->blocks, parts, 0x7fffffffu, &g->tiles) == false) return false;
-        g->rows = static_cast<int>(rows);
-        g->turns = static_cast<int>(rows / g->rows_at_once);
-        g->parts = static_cast<int>((d.positions + rows - 1) / rows);
-        g->fits = g->parts <= kCluster;
-        if (g->fits) break;
-    }
+    const size_t turns = kTile / (static_cast<size_t>(most_threads) * pack * size);
+    const size_t most = static_cast<size_t>(g->rows_at_once) * (turns ? turns : 1);
+    const size_t parts = (d.positions + most - 1) / most;
+    const size_t rows = align_up((d.positions + parts - 1) / parts, g->rows_at_once);
+    if (product(d.samples * g->blocks, parts, 0x7fffffffu, &g->tiles) == false) return false;
+    g->rows = static_cast<int>(rows);
+    g->turns = static_cast<int>(rows / g->rows_at_once);
+    g->parts = static_cast<int>((d.positions + rows - 1) / rows);
+    g->fits = g->parts <= kCluster;
     g->tiles = d.samples * g->blocks * g->parts;
     g->folds = 32 % g->lanes == 0;
     g->sum_rows = g->folds ? g->threads / 32 : g->rows_at_once;
