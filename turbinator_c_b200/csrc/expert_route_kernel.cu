@@ -3,7 +3,9 @@
  * weights (include/turbinator/training/cuda_learner.h).
  *
  * Bound: the selection by issue (a few hundred instructions a token), the rest
- * by latency: the logits are read once, the outputs written once.
+ * by latency: the logits are read once, the outputs written once.  65,536
+ * tokens, the best 8 of 256 experts, bf16: 51 us (selection 33, slot lists 13);
+ * the gradient of their weights 16 us, 4.35 TB/s, most of it dlogits' zeros.
  *
  * Selection, one warp a token, its experts in registers (NV consecutive ones a
  * lane): each lane sorts out its four best keys, then top_k times the best of
@@ -31,7 +33,7 @@ constexpr int kLeastTile = 8;     /* tokens */
 constexpr int kPlaceThreads = 512;
 constexpr int kPlaceWarps = kPlaceThreads / 32;
 constexpr int kHeld = 8;          /* rows of 32 slots that a placing warp keeps in registers */
-constexpr int kHeads = 4;         /* best keys that a lane keeps sorted */
+constexpr int kHeads = 4;         /* best keys that a lane keeps sorted; two: 72 us for 49 */
 
 /* Threads of a selecting CTA: what an SM has registers for. */
 constexpr int select_threads(int nv) { return nv <= 8 ? 1024 : nv <= 16 ? 512 : 256; }
@@ -196,7 +198,8 @@ __device__ __forceinline__ void keep_groups(const RouteShape &d, float (&value)[
 }
 
 /* One warp per token.  count: [tiles, experts] where the slots are listed by
- * tiles, or NULL.  TAGGED: 16-bit logits rank by themselves, without groups. */
+ * tiles, or NULL.  TAGGED: 16-bit logits rank by themselves, without groups,
+ * and share a key's word with their expert: 48 us for 58. */
 template <class T, int NV, bool TAGGED>
 __global__ void __launch_bounds__(select_threads(NV), 1)
 route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float *bias, int32_t *ids, float *weights,

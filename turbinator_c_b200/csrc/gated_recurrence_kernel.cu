@@ -8,15 +8,22 @@
  * (a tile); the warps of a CTA take consecutive spans of one tile, join them in
  * shared memory and go on together, the state in registers.  Inputs are staged
  * in shared memory one round ahead, outputs leave through the same slots: by
- * bulk tensor copies that one lane starts (every row on 16 bytes; the lanes'
- * own copies took 54 us of loads and 50 us of stores of a 285 us backward pass
- * of 64 x 1,024 x 1,024 bf16, nearly all of it their instructions), else by
+ * bulk tensor copies that one lane starts (every row on 16 bytes), else by
  * asynchronous copies of 16 or 4 bytes, else element by element.
+ *
+ * Bound: HBM with the gates' arithmetic close behind it (two sigmoids, a
+ * softplus' share, an exponential and a square root a step and channel, on
+ * packed pairs).  64 x 1,024 x 1,024 bf16, resets, states saved: forward 126 us
+ * (4.4 TB/s), backward 256 us (3.7 TB/s).  Without bulk copies 135 and 277 us
+ * (no resets: 120 and 243 with them); without the short series of decays that
+ * stay near 1, 147 and 274 us.
  *
  * Where tiles alone cannot fill the GPU, the steps are cut into strips and a
  * first kernel finds each strip's map, from which every strip's first state
  * follows: the inputs of the maps are read twice (three of the forward pass's
- * four tensors, two of the backward pass's seven), but nothing waits.  (The
+ * four tensors, two of the backward pass's seven), but nothing waits: three
+ * logs of 30,011 x 321 f32 take 280 us, without strips 1,135; 64 x 1,024 x 128
+ * bf16 backward 52 us and 81.  (The
  * strips joined in one kernel through published maps, each waiting for those
  * before it, was measured at 372 to 685 us on three logs of 30,011 steps: a
  * CTA that waits publishes its next map late, and so all wait.)
@@ -191,54 +198,54 @@ __device__ __forceinline__ void load_pieces(T *to, const T *const (&from)[N], si
                 f += step;
             }
         }
-        }
     }
+}
 
-    /* Starts copying rows x columns elements of N tensors into [N][STEPS][CT];
-     * `piece` bytes at a time (16, 4: asynchronous). */
-    template <class T, int CT, int N, int STEPS = kSteps>
-    __device__ __forceinline__ void load_rows(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows, int columns,
-                                              int piece, int lane) {
-        if (piece == 16) {
-            if (rows == STEPS && columns == CT) load_pieces<T, CT, 16, N, true, STEPS>(to, from, at, stride, rows, columns, lane);
-            else load_pieces<T, CT, 16, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
-        } else if (piece == 4) {
-            load_pieces<T, CT, 4, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
-        } else {
-            for (int n = 0; n < N; ++n)
-                for (int c = lane; c < columns; c += 32)
-#pragma unroll
-                    for (int r = 0; r < STEPS; ++r)
-                        if (r < rows) to[(n * STEPS + r) * CT + c] = from[n][at + r * stride + c];
-        }
-    }
-
-    /* rows x columns elements of from [STEPS][CT] to global memory. */
-    template <class T, int CT, int STEPS = kSteps>
-    __device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
-        if (piece == 16) {
-            constexpr int kPer = CT * static_cast<int>(sizeof(T)) / 16, kRows = 32 / kPer;
-            constexpr int kIn = 16 / static_cast<int>(sizeof(T));
-            const int row = lane / kPer, c = lane % kPer * kIn;
-            const T *f = from + row * CT + c;
-            T *t = to + row * stride + c;
-            if (c + kIn <= columns) {
-#pragma unroll
-                for (int r = 0; r < STEPS; r += kRows)
-                    if (row + r < rows)
-                        *reinterpret_cast<Pack<T, kIn> *>(t + r * stride) =
-                            *reinterpret_cast<const Pack<T, kIn> *>(f + r * CT);
-            } else {
-                for (int r = 0; row + r < rows; r += kRows)
-                    for (int i = 0; c + i < columns; ++i) t[r * stride + i] = f[r * CT + i];
-            }
-        } else {
+/* Starts copying rows x columns elements of N tensors into [N][STEPS][CT];
+ * `piece` bytes at a time (16, 4: asynchronous). */
+template <class T, int CT, int N, int STEPS = kSteps>
+__device__ __forceinline__ void load_rows(T *to, const T *const (&from)[N], size_t at, size_t stride, int rows, int columns,
+                                          int piece, int lane) {
+    if (piece == 16) {
+        if (rows == STEPS && columns == CT) load_pieces<T, CT, 16, N, true, STEPS>(to, from, at, stride, rows, columns, lane);
+        else load_pieces<T, CT, 16, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
+    } else if (piece == 4) {
+        load_pieces<T, CT, 4, N, false, STEPS>(to, from, at, stride, rows, columns, lane);
+    } else {
+        for (int n = 0; n < N; ++n)
             for (int c = lane; c < columns; c += 32)
 #pragma unroll
                 for (int r = 0; r < STEPS; ++r)
-                    if (r < rows) to[r * stride + c] = from[r * CT + c];
-        }
+                    if (r < rows) to[(n * STEPS + r) * CT + c] = from[n][at + r * stride + c];
     }
+}
+
+/* rows x columns elements of from [STEPS][CT] to global memory. */
+template <class T, int CT, int STEPS = kSteps>
+__device__ __forceinline__ void store_rows(T *to, const T *from, size_t stride, int rows, int columns, int piece, int lane) {
+    if (piece == 16) {
+        constexpr int kPer = CT * static_cast<int>(sizeof(T)) / 16, kRows = 32 / kPer;
+        constexpr int kIn = 16 / static_cast<int>(sizeof(T));
+        const int row = lane / kPer, c = lane % kPer * kIn;
+        const T *f = from + row * CT + c;
+        T *t = to + row * stride + c;
+        if (c + kIn <= columns) {
+#pragma unroll
+            for (int r = 0; r < STEPS; r += kRows)
+                if (row + r < rows)
+                    *reinterpret_cast<Pack<T, kIn> *>(t + r * stride) =
+                        *reinterpret_cast<const Pack<T, kIn> *>(f + r * CT);
+        } else {
+            for (int r = 0; row + r < rows; r += kRows)
+                for (int i = 0; c + i < columns; ++i) t[r * stride + i] = f[r * CT + i];
+        }
+    } else {
+        for (int c = lane; c < columns; c += 32)
+#pragma unroll
+            for (int r = 0; r < STEPS; ++r)
+                if (r < rows) to[r * stride + c] = from[r * CT + c];
+    }
+}
 
 /* The same by bulk tensor copies: a box of steps x CT channels from one tensor.
  * A box lies on 128 bytes of shared memory.  Where the dynamic part starts
@@ -1126,8 +1133,10 @@ bool encode(CUtensorMap *map, int type, const void *tensor, const RecurrenceShap
              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
                CUDA_SUCCESS;
 }
-/* Bulk copies pay from this many rounds of a unit on: seven maps take the host
- * a few microseconds, which short calls would wait for. */
+/* Bulk copies from this many rounds of a unit on: encoding the maps takes the
+ * host 1 to 2 us, which a call of one step of 64 x 512 channels (12 us of host
+ * work) waits for; on the GPU short units gain nothing (256 x 64 x 1,024 bf16:
+ * 34 us with them and without, of few rounds). */
 constexpr unsigned kBulkRounds = 4;
 
 /* Launches a kernel over `work` units: at most as many CTAs as there is room

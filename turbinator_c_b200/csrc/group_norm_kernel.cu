@@ -15,6 +15,10 @@
  *   - A group of more channels than a CTA has threads times its pack takes a
  *     CTA of its own and reads three times.
  *
+ * 4,096 maps of 256 x 64 bf16, silu: forward 61 us (4.4 TB/s), backward 143 us
+ * (2.8 TB/s: the activation's gradient, two sums a channel and du kept in f32 lie
+ * between the reads and the writes); 8 maps of 65,536 x 128: 87 us.
+ *
  * Statistics of tiles merge by counts, means and squares about the own mean, so
  * that a mean far from zero costs no digits.  Per-channel sums are the common
  * step of both directions: a pack may cross groups.
