@@ -22,7 +22,7 @@
  * first kernel finds each strip's map, from which every strip's first state
  * follows: the inputs of the maps are read twice (three of the forward pass's
  * four tensors, two of the backward pass's seven), but nothing waits: three
- * logs of 30,011 x 321 f32 take 280 us, without strips 1,135; 64 x 1,024 x 128
+ * logs of 15,005 to 30,011 x 321 f32 take 270 us, without strips 1,135; 64 x 1,024 x 128
  * bf16 backward 52 us and 81.  (The
  * strips joined in one kernel through published maps, each waiting for those
  * before it, was measured at 372 to 685 us on three logs of 30,011 steps: a
@@ -108,7 +108,8 @@ __device__ __forceinline__ int live_of(const RecurrenceShape &d, const int32_t *
     return n < 0 ? 0 : n < steps ? n : steps;
 }
 /* Of `live` steps those of the span from step t on. */
-template <int STEPS = kSteps> __device__ __forceinline__ int of_span(int live, int t) { return min(max(live - t, 0), STEPS); }
+__device__ __forceinline__ int of_span(int live, int t, int steps) { return min(max(live - t, 0), steps); }
+template <int STEPS = kSteps> __device__ __forceinline__ int of_span(int live, int t) { return of_span(live, t, STEPS); }
 
 /* e^l - 1 from its series, the next term below 5e-8 of it: for -kNear <= l <= 0
  * with five terms, for -kSeries <= l with seven. */
@@ -528,8 +529,9 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             if (lane == 0) {
                 boxes_read(); /* the slot's outputs of two rounds ago have left */
                 const uint32_t bar = shared_address(&bars[warp][stage]);
-                tb_pipe::mbar_arrive_expect_tx(bar, 3 * kSteps * CT * sizeof(T));
-                for (int n = 0; n < 3; ++n)
+                const bool any = t < to.live;
+                tb_pipe::mbar_arrive_expect_tx(bar, any ? 3 * kSteps * CT * sizeof(T) : 0);
+                for (int n = 0; n < 3 && any; ++n)
                     load_box(slots + (stage * 3 + n) * kSteps * CT, &maps.in[n], to.c0, t, static_cast<int>(to.b), bar);
             }
             return;
@@ -585,15 +587,22 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
         else copies_wait<1>();
         __syncwarp();
         float prod[kSteps][V], local[kSteps][V];
-        if (live == kSteps && !anew && near)
-            forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
-        else
-            forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
         Lane<V> map_a, map_h;
+        /* past the sequence's length nothing changes the state (three logs of up
+         * to 10,000 x 320 bf16: 38 us, with all spans computed 46) */
+        if (live == 0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            map_a.v[v] = prod[kSteps - 1][v];
-            map_h.v[v] = local[kSteps - 1][v];
+            for (int v = 0; v < V; ++v) map_a.v[v] = 1.0f, map_h.v[v] = 0.0f;
+        } else {
+            if (live == kSteps && !anew && near)
+                forward_span<T, V, true>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+            else
+                forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                map_a.v[v] = prod[kSteps - 1][v];
+                map_h.v[v] = local[kSteps - 1][v];
+            }
         }
         const Lane<V> h0 = join<CT, V>(map_a, map_h, &state, sa[stage], sh[stage], warp, warps, lane);
         if (BULK && next.unit < units) start(next, stage ^ 1); /* half a round ahead: the other slot has been read */
@@ -606,21 +615,25 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             if (p.checkpoints && rows > 0) p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] = h0.v[v];
             if (ends) p.state_out[at.b * d.channels + c] = state.v[v];
         }
+        if (live > 0) {
 #pragma unroll
-        for (int j = 0; j < kSteps; j += 3 - V) {
-            float o0, o1;
-            split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(h0.v[0], h0.v[V - 1]),
-                       pair(local[j][0], local[j + 2 - V][V - 1])), o0, o1);
-            if constexpr (V == 2) {
-                *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = {{from_float<T>(o0), from_float<T>(o1)}};
-            } else {
-                xs[j * CT + lane] = from_float<T>(o0);
-                xs[(j + 1) * CT + lane] = from_float<T>(o1);
+            for (int j = 0; j < kSteps; j += 3 - V) {
+                float o0, o1;
+                split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(h0.v[0], h0.v[V - 1]),
+                           pair(local[j][0], local[j + 2 - V][V - 1])), o0, o1);
+                if constexpr (V == 2) {
+                    *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = {{from_float<T>(o0), from_float<T>(o1)}};
+                } else {
+                    xs[j * CT + lane] = from_float<T>(o0);
+                    xs[(j + 1) * CT + lane] = from_float<T>(o1);
+                }
             }
         }
         if (live < kSteps) { /* steps past the sequence's length */
-            for (int j = live; j < kSteps; ++j)
-                for (int v = 0; v < V; ++v) xs[j * CT + lane * V + v] = from_float<T>(0.0f);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+                if (j >= live)
+                    for (int v = 0; v < V; ++v) xs[j * CT + lane * V + v] = from_float<T>(0.0f);
         }
         if constexpr (BULK) {
             tb_pipe::fence_proxy_async_shared();
@@ -656,7 +669,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
     for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const Place at = place_of<CT>(unit, d, p.lengths, s);
         const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
-        const int first = static_cast<int>(at.round * warps + warp * s.strip_rounds), spans = static_cast<int>(s.strip_rounds);
+        const int first = static_cast<int>(at.round * warps + warp * s.strip_rounds);
+        const int spans = of_span((at.live + kSteps - 1) / kSteps, first, static_cast<int>(s.strip_rounds)); /* that live */
         const auto start = [&](int span, int stage) {
             const int t = (first + span) * kSteps, live = of_span(at.live, t);
             const T *const from[3] = {static_cast<const T *>(p.x), static_cast<const T *>(p.rec), static_cast<const T *>(p.inp)};
@@ -984,13 +998,15 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
                                        columns, p.dh_piece, lane);
             return reset_byte(p.reset, at.b * d.steps + t, live, lane);
         };
-        unsigned flag = start(0, 0);
+        /* those past the sequence's length change nothing */
+        const int past = of_span(top + 1, (at.live + kHalf - 1) / kHalf, spans);
+        unsigned flag = past < spans ? start(past, past & 1) : 0;
         copies_end();
         const int c = at.c0 + lane * 2;
         const float l0 = left > lane * 2 ? -d.scale * softplus(p.decay[c]) : 0.0f;
         const float l1 = left > lane * 2 + 1 ? -d.scale * softplus(p.decay[c + 1]) : 0.0f;
         F2 all = both(1.0f), grad = both(0.0f);
-        for (int i = 0; i < spans; ++i) {
+        for (int i = past; i < spans; ++i) {
             const int live = of_span<kHalf>(at.live, (top - i) * kHalf);
             const unsigned anew = __ballot_sync(0xffffffffu, flag);
             const T *rs = slots + (i & 1) * 2 * kSlot;
