@@ -210,6 +210,10 @@ RECURRENCE_SHAPES = [
     (40, 40, 256, 0, 0), (2, 333, 200, 8, 4),
     # tiles enough that one CTA takes many rounds: bulk copies
     (150, 260, 136, 0, 0), (600, 100, 72, 8, 0), (310, 300, 40, 8, 0),
+    # few steps of many sequences
+    (700, 1, 190, 0, 0), (64, 1, 512, 0, 0), (3000, 3, 128, 8, 0), (90, 8, 37, 2, 1),
+    (5000, 2, 144, 0, 0), (40, 9, 64, 0, 0),
+    (1300, 16, 128, 0, 0), (1200, 17, 32, 0, 0),
 ]
 
 

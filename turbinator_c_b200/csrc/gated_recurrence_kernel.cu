@@ -714,6 +714,105 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
     }
 }
 
+/* ---- a few steps ---- */
+
+/* Floats of the thread's pack of channels; QUADS: rows of them on 16 bytes. */
+template <int PACK, bool QUADS> __device__ __forceinline__ void load_floats(const float *from, float (&to)[PACK]) {
+#pragma unroll
+    for (int i = 0; i < PACK; i += QUADS ? 4 : 1) {
+        if constexpr (QUADS) {
+            const float4 v = *reinterpret_cast<const float4 *>(from + i);
+            to[i] = v.x, to[i + 1] = v.y, to[i + 2] = v.z, to[i + 3] = v.w;
+        } else {
+            to[i] = from[i];
+        }
+    }
+}
+template <int PACK, bool QUADS> __device__ __forceinline__ void store_floats(float *to, const float (&from)[PACK]) {
+#pragma unroll
+    for (int i = 0; i < PACK; i += QUADS ? 4 : 1) {
+        if constexpr (QUADS)
+            *reinterpret_cast<float4 *>(to + i) = make_float4(from[i], from[i + 1], from[i + 2], from[i + 3]);
+        else
+            to[i] = from[i];
+    }
+}
+
+/* A few steps, as programs that act take them: a thread takes a pack of
+ * channels of every rows-th sequence through all steps, its rates found once.
+ * No step is computed that is not asked for: one step of 4,096 x 512 bf16 takes
+ * 9.3 us (2.3 TB/s), by spans of 16 steps 101; of 64 x 512 2.2 and 4.5 us. */
+constexpr int kFewSteps = 8, kMostSteps = kSteps, kFewThreads = 128;
+template <class T, int PACK, bool QUADS>
+__global__ void __launch_bounds__(kFewThreads)
+recurrence_few_steps(const ForwardArgs p, unsigned packs, unsigned rows) {
+    constexpr int N = (PACK + 1) / 2, kTogether = 2;
+    const RecurrenceShape &d = p.d;
+    const unsigned thread = blockIdx.x * kFewThreads + threadIdx.x;
+    if (thread >= packs * rows) return;
+    const size_t c = static_cast<size_t>(thread % packs) * PACK;
+    const int steps = static_cast<int>(d.steps);
+    /* one channel: a pair of which the second is idle */
+    const auto pairs = [](const float (&f)[PACK], int k) { return pair(f[2 * k], PACK > 1 ? f[PACK > 1 ? 2 * k + 1 : 0] : 0.0f); };
+    F2 rate[N];
+    {
+        float l[PACK];
+        load_floats<PACK, QUADS>(p.decay + c, l);
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) l[i] = -d.scale * softplus(l[i]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) rate[k] = pairs(l, k);
+    }
+    for (size_t b = thread / packs; b < d.sequences; b += rows) {
+        const int live = live_of(d, p.lengths, b);
+        float h[PACK];
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) h[i] = 0.0f;
+        if (p.state_in) load_floats<PACK, QUADS>(p.state_in + b * d.channels + c, h);
+        if (p.checkpoints) store_floats<PACK, QUADS>(p.checkpoints + b * d.channels + c, h); /* the only one */
+        const size_t in = b * d.is + c;
+        T *to = static_cast<T *>(p.h) + b * d.os + c;
+        for (int t = 0; t < steps; t += kTogether) {
+            Held<T, PACK> x[kTogether], rec[kTogether], inp[kTogether];
+            bool anew[kTogether];
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) {
+                if (t + j >= live) continue;
+                const size_t at = in + (t + j) * d.it;
+                x[j] = *reinterpret_cast<const Held<T, PACK> *>(static_cast<const T *>(p.x) + at);
+                rec[j] = *reinterpret_cast<const Held<T, PACK> *>(static_cast<const T *>(p.rec) + at);
+                inp[j] = *reinterpret_cast<const Held<T, PACK> *>(static_cast<const T *>(p.inp) + at);
+                anew[j] = p.reset && p.reset[b * d.steps + t + j];
+            }
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) {
+                if (t + j >= steps) break;
+                float out[PACK];
+#pragma unroll
+                for (int i = 0; i < PACK; ++i) out[i] = 0.0f;
+                if (t + j < live) {
+                    float xs[PACK], rs[PACK], is[PACK];
+                    unpack(x[j], xs);
+                    unpack(rec[j], rs);
+                    unpack(inp[j], is);
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const Decay s = decay_of<false>(rate[k], sigmoid2(pairs(rs, k)));
+                        const F2 u = mul2(sigmoid2(pairs(is, k)), pairs(xs, k));
+                        const F2 next = anew[j] ? u : fma2(s.a, pairs(h, k), mul2(s.beta, u));
+                        float h0, h1;
+                        split(next, h0, h1);
+                        h[2 * k] = out[2 * k] = h0;
+                        if (PACK > 1) h[2 * k + 1] = out[2 * k + 1] = h1;
+                    }
+                }
+                *reinterpret_cast<Held<T, PACK> *>(to + (t + j) * d.ot) = packed<T, PACK>(out);
+            }
+        }
+        if (p.state_out) store_floats<PACK, QUADS>(p.state_out + b * d.channels + c, h);
+    }
+}
+
 /* ---- backward ---- */
 
 /* A span of kHalf steps of two channels a lane.  What the gradients need of a
@@ -1167,6 +1266,39 @@ int launch_units(unsigned work, const Pass &pass, int warps, size_t shared, cuda
     return launched();
 }
 
+/* The few steps' pack: 16 bytes where these fill the GPU (500 x 1,024 f32, one
+ * step: 3.6 us, in packs of 4 bytes 5.7), else 4 bytes (64 x 512 bf16: 2.2 us,
+ * in packs of 16 bytes 2.6; 8 steps 4.1 and 6.3). */
+int few_steps_pack(const ForwardArgs &p, size_t size, bool *full) {
+    const RecurrenceShape &d = p.d;
+    const size_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.rec) |
+                       reinterpret_cast<uintptr_t>(p.inp) | reinterpret_cast<uintptr_t>(p.h) |
+                       (d.is | d.it | d.os | d.ot | d.channels) * size;
+    const int pack = pack_of(all, size);
+    *full = d.sequences * d.channels / pack >= kSms * 128;
+    return pack * size == 16 && !*full ? 4 / static_cast<int>(size) : pack;
+}
+template <class T> int launch_few_steps(const ForwardArgs &p, int pack, cudaStream_t st) {
+    const RecurrenceShape &d = p.d;
+    const auto bits = [](const void *a) { return reinterpret_cast<uintptr_t>(a); };
+    const bool quads = (bits(p.decay) | bits(p.state_in) | bits(p.state_out) | bits(p.checkpoints) | d.channels * 4) % 16 == 0;
+    return with_pack<T>(pack, [&](auto n) {
+        constexpr int PACK = decltype(n)::value;
+        const size_t packs = d.channels / PACK;
+        const size_t fill = (kSms * 2048 + packs - 1) / packs, rows = d.sequences < fill ? d.sequences : fill;
+        const unsigned grid = static_cast<unsigned>((packs * rows + kFewThreads - 1) / kFewThreads);
+        const unsigned a = static_cast<unsigned>(packs), b = static_cast<unsigned>(rows);
+        if constexpr (PACK % 4 == 0) {
+            if (quads) {
+                recurrence_few_steps<T, PACK, true><<<grid, kFewThreads, 0, st>>>(p, a, b);
+                return launched();
+            }
+        }
+        recurrence_few_steps<T, PACK, false><<<grid, kFewThreads, 0, st>>>(p, a, b);
+        return launched();
+    });
+}
+
 } /* namespace */
 
 extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_desc *desc) {
@@ -1194,6 +1326,13 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
         return 0;
     cudaGetLastError(); /* report these launches only */
     ForwardArgs p{s, x, recurrence_gate, input_gate, decay, state_in, reset, lengths, h, state_out, checkpoints, 0, 0};
+    /* 16 steps of 4,096 x 512 bf16: 62 us, by spans 100; of 64 x 512 5.9 and 4.0 */
+    bool full;
+    const int few = few_steps_pack(p, size, &full);
+    if (s.steps <= (full ? kMostSteps : kFewSteps))
+        return with_type(desc->type, [&](auto t) {
+            return launch_few_steps<decltype(t)>(p, few, static_cast<cudaStream_t>(stream));
+        });
     const uintptr_t in = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(recurrence_gate) |
                          reinterpret_cast<uintptr_t>(input_gate);
     p.in_piece = piece_of(reinterpret_cast<const void *>(in), s.is, s.it, size, 4);
