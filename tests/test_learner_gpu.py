@@ -214,6 +214,8 @@ RECURRENCE_SHAPES = [
     (700, 1, 190, 0, 0), (64, 1, 512, 0, 0), (3000, 3, 128, 8, 0), (90, 8, 37, 2, 1),
     (5000, 2, 144, 0, 0), (40, 9, 64, 0, 0),
     (1300, 16, 128, 0, 0), (1200, 17, 32, 0, 0),
+    # many rows, step by step
+    (600, 50, 136, 0, 0), (300, 37, 131, 0, 0), (1700, 20, 512, 0, 0), (2400, 21, 33, 0, 0),
 ]
 
 

@@ -207,6 +207,10 @@ extern "C" int tb_cuda_combine_experts_device(const tb_expert_combine_desc *desc
             const size_t packs = (s.width + P - 1) / P;
             int lanes = 1;
             while (lanes < 32 && static_cast<size_t>(lanes) < packs) lanes *= 2;
+            /* narrower teams where they idle less: 30,000 tokens x 4 x 320 bf16
+             * 23 us for 29, 29,875 x 3 x 35 f32 13.7 for 17.3 */
+            const auto places = [&](size_t n) { return (packs + n - 1) / n * n; };
+            while (lanes > 8 && places(lanes / 2) * 5 <= places(lanes) * 4) lanes /= 2;
             const size_t chunks = (packs + lanes - 1) / lanes;
             size_t teams;
             if (!product(s.tokens, chunks, 0x7fffffffull * (kThreads / lanes) , &teams) || chunks > 0x7fffffffu) return 0;

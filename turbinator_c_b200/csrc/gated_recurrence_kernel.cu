@@ -18,6 +18,9 @@
  * (no resets: 120 and 243 with them); without the short series of decays that
  * stay near 1, 147 and 274 us.
  *
+ * Calls of few steps or of very many rows go step by step, a thread a pack of
+ * channels (forward).
+ *
  * Where tiles alone cannot fill the GPU, the steps are cut into strips and a
  * first kernel finds each strip's map, from which every strip's first state
  * follows: the inputs of the maps are read twice (three of the forward pass's
@@ -714,7 +717,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
     }
 }
 
-/* ---- a few steps ---- */
+/* ---- step by step ---- */
 
 /* Floats of the thread's pack of channels; QUADS: rows of them on 16 bytes. */
 template <int PACK, bool QUADS> __device__ __forceinline__ void load_floats(const float *from, float (&to)[PACK]) {
@@ -738,17 +741,18 @@ template <int PACK, bool QUADS> __device__ __forceinline__ void store_floats(flo
     }
 }
 
-/* A few steps, as programs that act take them: a thread takes a pack of
- * channels of every rows-th sequence through all steps, its rates found once.
- * No step is computed that is not asked for: one step of 4,096 x 512 bf16 takes
- * 9.3 us (2.3 TB/s), by spans of 16 steps 101; of 64 x 512 2.2 and 4.5 us. */
-constexpr int kFewSteps = 8, kMostSteps = kSteps, kFewThreads = 128;
-template <class T, int PACK, bool QUADS>
-__global__ void __launch_bounds__(kFewThreads)
-recurrence_few_steps(const ForwardArgs p, unsigned packs, unsigned rows) {
-    constexpr int N = (PACK + 1) / 2, kTogether = 2;
+/* For few steps, as programs that act take them, and for many rows: a thread
+ * takes a pack of channels of every rows-th sequence through its steps, the
+ * loads of TOGETHER steps at once, its rates found once.  No step is computed
+ * that is not asked for, and no span is joined: one step of 4,096 x 512 bf16
+ * takes 9.3 us (2.3 TB/s), by spans 101; of 64 x 512 2.2 and 4.5 us. */
+constexpr int kFewSteps = 8, kSerialThreads = 128;
+template <class T, int PACK, bool QUADS, int TOGETHER>
+__global__ void __launch_bounds__(kSerialThreads)
+recurrence_serial(const ForwardArgs p, unsigned packs, unsigned rows) {
+    constexpr int N = (PACK + 1) / 2;
     const RecurrenceShape &d = p.d;
-    const unsigned thread = blockIdx.x * kFewThreads + threadIdx.x;
+    const unsigned thread = blockIdx.x * kSerialThreads + threadIdx.x;
     if (thread >= packs * rows) return;
     const size_t c = static_cast<size_t>(thread % packs) * PACK;
     const int steps = static_cast<int>(d.steps);
@@ -769,14 +773,18 @@ recurrence_few_steps(const ForwardArgs p, unsigned packs, unsigned rows) {
 #pragma unroll
         for (int i = 0; i < PACK; ++i) h[i] = 0.0f;
         if (p.state_in) load_floats<PACK, QUADS>(p.state_in + b * d.channels + c, h);
-        if (p.checkpoints) store_floats<PACK, QUADS>(p.checkpoints + b * d.channels + c, h); /* the only one */
+        float *saved = p.checkpoints ? p.checkpoints + b * ((d.steps + kSteps - 1) / kSteps) * d.channels + c : nullptr;
         const size_t in = b * d.is + c;
         T *to = static_cast<T *>(p.h) + b * d.os + c;
-        for (int t = 0; t < steps; t += kTogether) {
-            Held<T, PACK> x[kTogether], rec[kTogether], inp[kTogether];
-            bool anew[kTogether];
+        for (int t = 0; t < steps; t += TOGETHER) {
+            Held<T, PACK> x[TOGETHER], rec[TOGETHER], inp[TOGETHER];
+            bool anew[TOGETHER];
+            if (saved && t % kSteps == 0) {
+                store_floats<PACK, QUADS>(saved, h);
+                saved += d.channels;
+            }
 #pragma unroll
-            for (int j = 0; j < kTogether; ++j) {
+            for (int j = 0; j < TOGETHER; ++j) {
                 if (t + j >= live) continue;
                 const size_t at = in + (t + j) * d.it;
                 x[j] = *reinterpret_cast<const Held<T, PACK> *>(static_cast<const T *>(p.x) + at);
@@ -785,7 +793,7 @@ recurrence_few_steps(const ForwardArgs p, unsigned packs, unsigned rows) {
                 anew[j] = p.reset && p.reset[b * d.steps + t + j];
             }
 #pragma unroll
-            for (int j = 0; j < kTogether; ++j) {
+            for (int j = 0; j < TOGETHER; ++j) {
                 if (t + j >= steps) break;
                 float out[PACK];
 #pragma unroll
@@ -1266,19 +1274,26 @@ int launch_units(unsigned work, const Pass &pass, int warps, size_t shared, cuda
     return launched();
 }
 
-/* The few steps' pack: 16 bytes where these fill the GPU (500 x 1,024 f32, one
+/* The serial kernel's pack: 16 bytes where these fill the GPU (500 x 1,024 f32, one
  * step: 3.6 us, in packs of 4 bytes 5.7), else 4 bytes (64 x 512 bf16: 2.2 us,
  * in packs of 16 bytes 2.6; 8 steps 4.1 and 6.3). */
-int few_steps_pack(const ForwardArgs &p, size_t size, bool *full) {
+int serial_pack(const ForwardArgs &p, size_t size) {
     const RecurrenceShape &d = p.d;
     const size_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.rec) |
                        reinterpret_cast<uintptr_t>(p.inp) | reinterpret_cast<uintptr_t>(p.h) |
                        (d.is | d.it | d.os | d.ot | d.channels) * size;
     const int pack = pack_of(all, size);
-    *full = d.sequences * d.channels / pack >= kSms * 128;
-    return pack * size == 16 && !*full ? 4 / static_cast<int>(size) : pack;
+    const bool full = d.sequences * d.channels / pack >= kSms * 128;
+    return pack * size == 16 && !full ? 4 / static_cast<int>(size) : pack;
 }
-template <class T> int launch_few_steps(const ForwardArgs &p, int pack, cudaStream_t st) {
+/* Few steps, or threads that are enough: 1,000 x 100 x 321 f32 140 us, by spans
+ * 204, 4,096 x 64 x 512 bf16 230 and 264, 600 x 100 x 320 (24,000 threads) 46
+ * both; fewer where spans load element by element: 64 x 1,024 x 1,023 bf16 396
+ * and 551, 20 x 300 x 1,023 98 and 76. */
+bool goes_serial(const RecurrenceShape &d, size_t bytes, size_t threads) {
+    return d.steps <= kFewSteps || threads >= kSms * (bytes == 2 ? 256 : 512);
+}
+template <class T> int launch_serial(const ForwardArgs &p, int pack, cudaStream_t st) {
     const RecurrenceShape &d = p.d;
     const auto bits = [](const void *a) { return reinterpret_cast<uintptr_t>(a); };
     const bool quads = (bits(p.decay) | bits(p.state_in) | bits(p.state_out) | bits(p.checkpoints) | d.channels * 4) % 16 == 0;
@@ -1286,16 +1301,25 @@ template <class T> int launch_few_steps(const ForwardArgs &p, int pack, cudaStre
         constexpr int PACK = decltype(n)::value;
         const size_t packs = d.channels / PACK;
         const size_t fill = (kSms * 2048 + packs - 1) / packs, rows = d.sequences < fill ? d.sequences : fill;
-        const unsigned grid = static_cast<unsigned>((packs * rows + kFewThreads - 1) / kFewThreads);
+        const unsigned grid = static_cast<unsigned>((packs * rows + kSerialThreads - 1) / kSerialThreads);
         const unsigned a = static_cast<unsigned>(packs), b = static_cast<unsigned>(rows);
-        if constexpr (PACK % 4 == 0) {
-            if (quads) {
-                recurrence_few_steps<T, PACK, true><<<grid, kFewThreads, 0, st>>>(p, a, b);
-                return launched();
+        const auto launch = [&](auto wide, auto together) {
+            recurrence_serial<T, PACK, decltype(wide)::value, decltype(together)::value>
+                <<<grid, kSerialThreads, 0, st>>>(p, a, b);
+            return launched();
+        };
+        /* 500 x 16 x 1,023 bf16 33 us by fours, by twos 40; 1,024 x 128 x 1,024
+         * 233 and 268; one step 6.0 and 5.7; f32 500 x 100 x 1,024 147 and 131 */
+        const auto choose = [&](auto wide) {
+            if constexpr (PACK == 1 || sizeof(T) == 2) {
+                if (d.steps > (PACK == 1 ? 2 : kSteps)) return launch(wide, std::integral_constant<int, 4>{});
             }
+            return launch(wide, std::integral_constant<int, 2>{});
+        };
+        if constexpr (PACK % 4 == 0) {
+            if (quads) return choose(std::true_type{});
         }
-        recurrence_few_steps<T, PACK, false><<<grid, kFewThreads, 0, st>>>(p, a, b);
-        return launched();
+        return choose(std::false_type{});
     });
 }
 
@@ -1326,12 +1350,10 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
         return 0;
     cudaGetLastError(); /* report these launches only */
     ForwardArgs p{s, x, recurrence_gate, input_gate, decay, state_in, reset, lengths, h, state_out, checkpoints, 0, 0};
-    /* 16 steps of 4,096 x 512 bf16: 62 us, by spans 100; of 64 x 512 5.9 and 4.0 */
-    bool full;
-    const int few = few_steps_pack(p, size, &full);
-    if (s.steps <= (full ? kMostSteps : kFewSteps))
+    const int serial = serial_pack(p, size);
+    if (goes_serial(s, serial * size, s.sequences * s.channels / serial))
         return with_type(desc->type, [&](auto t) {
-            return launch_few_steps<decltype(t)>(p, few, static_cast<cudaStream_t>(stream));
+            return launch_serial<decltype(t)>(p, serial, static_cast<cudaStream_t>(stream));
         });
     const uintptr_t in = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(recurrence_gate) |
                          reinterpret_cast<uintptr_t>(input_gate);
