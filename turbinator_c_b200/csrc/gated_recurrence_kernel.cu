@@ -1257,8 +1257,7 @@ bool encode(CUtensorMap *map, int type, const void *tensor, const RecurrenceShap
                CUDA_SUCCESS;
 }
 /* Bulk copies from this many rounds of a unit on: encoding the maps takes the
- * host 1 to 2 us, which a call of one step of 64 x 512 channels (12 us of host
- * work) waits for; on the GPU short units gain nothing (256 x 64 x 1,024 bf16:
+ * host 1 to 2 us, which short calls wait for; on the GPU short units gain nothing (256 x 64 x 1,024 bf16:
  * 34 us with them and without, of few rounds). */
 constexpr unsigned kBulkRounds = 4;
 
