@@ -25,6 +25,11 @@ REF_ONBOARD_PATH = os.path.join(HERE, "_ref", "libtb_ref_onboard.so")
 REF_ONBOARD_CR_PATH = os.path.join(HERE, "_ref", "libtb_ref_onboard_cr.so")
 REF_ACTOR_INPUTS_PATH = os.path.join(HERE, "_ref", "libtb_ref_actor_inputs.so")
 
+
+class ReferenceMissing(RuntimeError):
+    """A call into the reference's own code where its build (oracle/_ref) is not there."""
+
+
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _oracle = None
@@ -67,7 +72,7 @@ def ref_training() -> ctypes.CDLL:
     global _ref_training
     if _ref_training is None:
         if not have_reference():
-            raise RuntimeError(f"{REF_TRAINING_PATH} missing (reference build not available)")
+            raise ReferenceMissing(f"{REF_TRAINING_PATH} missing (reference build not available)")
         l = ctypes.CDLL(REF_TRAINING_PATH)
         l.tb_train_extract_features_cpu.restype = None
         l.tb_train_extract_features_cpu.argtypes = [_vp, _vp, _vp, _vp]
@@ -79,7 +84,7 @@ def ref_onboard() -> ctypes.CDLL:
     global _ref_onboard
     if _ref_onboard is None:
         if not os.path.exists(REF_ONBOARD_PATH):
-            raise RuntimeError(f"{REF_ONBOARD_PATH} missing (reference build not available)")
+            raise ReferenceMissing(f"{REF_ONBOARD_PATH} missing (reference build not available)")
         l = ctypes.CDLL(REF_ONBOARD_PATH)
         l.tb_ref_onboard_batch.restype = None
         l.tb_ref_onboard_batch.argtypes = [_vp, _vp, _sz, _vp]
@@ -148,7 +153,7 @@ def ref_onboard_cr() -> ctypes.CDLL:
     global _ref_onboard_cr
     if _ref_onboard_cr is None:
         if not os.path.exists(REF_ONBOARD_CR_PATH):
-            raise RuntimeError(f"{REF_ONBOARD_CR_PATH} missing (reference build not available)")
+            raise ReferenceMissing(f"{REF_ONBOARD_CR_PATH} missing (reference build not available)")
         l = ctypes.CDLL(REF_ONBOARD_CR_PATH)
         l.tb_ref_onboard_cr_batch.restype = None
         l.tb_ref_onboard_cr_batch.argtypes = [_vp, _vp, _sz, _vp]
@@ -273,7 +278,7 @@ def ref_sensors() -> ctypes.CDLL:
     global _ref_sensors
     if _ref_sensors is None:
         if not have_reference_sensors():
-            raise RuntimeError(f"{REF_SENSORS_PATH} missing (reference build not available)")
+            raise ReferenceMissing(f"{REF_SENSORS_PATH} missing (reference build not available)")
         l = ctypes.CDLL(REF_SENSORS_PATH)
         l.ref_sensors_render.restype = ctypes.c_double
         l.ref_sensors_render.argtypes = [_vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp,
@@ -418,7 +423,7 @@ def ref_cuda_features() -> ctypes.CDLL:
     global _ref_cuda_features
     if _ref_cuda_features is None:
         if not have_reference_gpu_features():
-            raise RuntimeError(f"{REF_CUDA_FEATURES_PATH} missing (reference build not available)")
+            raise ReferenceMissing(f"{REF_CUDA_FEATURES_PATH} missing (reference build not available)")
         l = ctypes.CDLL(REF_CUDA_FEATURES_PATH, mode=ctypes.RTLD_LOCAL)
         l.tb_cuda_extract_features_device.restype = ctypes.c_int
         l.tb_cuda_extract_features_device.argtypes = [_vp, _vp, _vp, _vp, _sz, _vp]
