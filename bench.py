@@ -1264,7 +1264,10 @@ def run_ours(args, rank: int, world: int, local_rank: int):
                     "sample": f"first {k} aircraft: the reference simulator's renderers ({t_r:.2f} s) then "
                               f"tb_train_extract_features_cpu ({t_f:.2f} s), oracle/_ref, {threads} threads"}
         if onboard is not None:
-            onboard["cpu_baseline"] = time_onboard_reference_cpu(obs, mission, args.cpu_seconds / 2)
+            import oracle  # test infrastructure: the CPU baseline only
+
+            if os.path.exists(oracle.REF_ONBOARD_PATH):
+                onboard["cpu_baseline"] = time_onboard_reference_cpu(obs, mission, args.cpu_seconds / 2)
         if sensors is not None:
             import oracle  # test infrastructure: the CPU baseline only
 
