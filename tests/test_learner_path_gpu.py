@@ -158,3 +158,68 @@ def test_route_best_experts_next_to_each_other(kind, experts):
     torch.cuda.synchronize()
     distinct = torch.arange(t, device="cuda") % 5 != 0
     assert torch.equal(ids.long()[distinct], want[distinct])
+
+
+def _routed(kind, logits, bias, top_k, score, groups=1):
+    t, experts = logits.shape
+    desc = tb.ExpertRouteDesc(tokens=t, experts=experts, top_k=top_k, groups=groups, top_groups=1, group_best=1,
+                              type={torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[kind], score=score,
+                              renormalise=1, weight_scale=1.0)
+    whole = lambda *s: torch.full(s, -77, dtype=torch.int32, device="cuda")  # noqa: E731
+    ids, weights = whole(t, top_k), torch.full((t, top_k), float("nan"), device="cuda")
+    offsets, order, position = whole(experts + 1), whole(t * top_k), whole(t, top_k)
+    work = torch.empty(tb.tb_cuda_route_experts_workspace(desc), dtype=torch.uint8, device="cuda")
+    assert tb.tb_cuda_route_experts_device(desc, logits, bias, ids, weights, offsets, order, position, work) == 1
+    torch.cuda.synchronize()
+    return ids.long(), weights, offsets.long()
+
+
+@pytest.mark.parametrize("kind", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("experts", (256, 512, 1024))
+@pytest.mark.parametrize("top_k", (5, 6, 8, 17, 32))
+def test_route_takes_every_expert_that_is_there(kind, experts, top_k):
+    """A token with few available experts, all in one run of experts/32 of them, gets all that it has slots for."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(8)
+    run, t = experts // 32, 32 * (experts // 32)
+    token = torch.arange(t, device="cuda")
+    first, many = token % 32 * run, token // 32 + 1  # 1 .. run of them
+    place = torch.rand((t, run), generator=gen, device="cuda").argsort(1)
+    logits = torch.full((t, experts), float("-inf"), device="cuda")
+    values = place.float() * 0.25 - 3.0  # distinct in every type, and so are their sigmoids
+    chosen = torch.rand((t, run), generator=gen, device="cuda").argsort(1) < many[:, None]
+    logits.scatter_(1, first[:, None] + torch.arange(run, device="cuda"),
+                    torch.where(chosen, values, float("-inf")))
+    logits = logits.to(kind)
+    l64 = logits.double()
+    want = l64.sort(dim=1, descending=True, stable=True)[1][:, :top_k]
+    taken = torch.arange(top_k, device="cuda") < many.clamp(max=top_k)[:, None]
+    want = torch.where(taken, want, -1)
+    counts = torch.zeros(experts, dtype=torch.long, device="cuda").index_add_(0, want[taken], torch.ones_like(want[taken]))
+    for score, bias in ((tb.TB_SCORE_SOFTMAX, None), (tb.TB_SCORE_SIGMOID, None),
+                        (tb.TB_SCORE_SIGMOID, torch.zeros(experts, device="cuda"))):
+        ids, weights, offsets = _routed(kind, logits, bias, top_k, score)
+        assert torch.equal(ids, want)
+        assert torch.equal(offsets.diff(), counts)
+        picked = torch.where(taken, l64.gather(1, want.clamp(min=0)), float("-inf"))
+        s = picked.softmax(1) if score == tb.TB_SCORE_SOFTMAX else torch.sigmoid(picked)
+        # scores within 16 U, their sum of at most 32 terms within 48, one division
+        assert ((weights.double() - s / s.sum(1, keepdim=True)).abs() <= 96 * 2.0 ** -24 * s / s.sum(1, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("kind", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("experts", (256, 512, 1024))
+def test_route_takes_the_whole_of_a_group_in_one_run(kind, experts):
+    """Groups of experts/32: all slots come from the token's one group."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(9)
+    per, t = experts // 32, 96
+    logits = (torch.rand((t, experts), generator=gen, device="cuda").argsort(1).float() / experts * 4 - 2)
+    group = torch.arange(t, device="cuda") % 32
+    inside = torch.arange(experts, device="cuda")[None] // per == group[:, None]
+    logits = torch.where(inside, torch.rand((t, experts), generator=gen, device="cuda").argsort(1) * (1 / 128) + 3.0, logits)
+    logits = logits.to(kind)
+    want = logits.float().masked_fill(~inside, float("-inf")).sort(dim=1, descending=True, stable=True)[1][:, :min(per, 32)]
+    for top_k in {5, 8, min(per, 32)}:
+        ids, _, _ = _routed(kind, logits, None, top_k, tb.TB_SCORE_SOFTMAX, groups=32)
+        assert torch.equal(ids, want[:, :top_k])

@@ -287,6 +287,7 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
         int from = 0, given = 0, expert = -1;
         for (int j = 0; j < d.top_k; ++j) {
             const unsigned best = __reduce_max_sync(0xffffffffu, head[0]);
+            if (best == 0) break; /* no head is left: nothing is given */
             bool wins = head[0] == best;
             if constexpr (!TAGGED) { /* of equal ones the first lane */
                 const int winner = __ffs(__ballot_sync(0xffffffffu, wins)) - 1;
