@@ -2,6 +2,9 @@
 refuse before they touch a device."""
 from __future__ import annotations
 
+import os
+import subprocess
+
 import pytest
 
 import turbinator_c_b200 as tb
@@ -199,3 +202,14 @@ def test_combine_refuses_pointers():
 def test_descriptors_take_their_fields_only():
     with pytest.raises(TypeError):
         tb.GroupNormDesc(sample=3)
+
+
+def test_shared_memory_limits_only_grow(tmp_path):
+    """Of two threads that first ask for different sizes, the smaller one does not take away what the larger one has."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = str(tmp_path / "shared_limit")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-I",
+                    os.path.join(os.path.dirname(here), "turbinator_c_b200", "csrc"),
+                    os.path.join(here, "shared_limit.cpp"), "-o", exe], check=True, timeout=120)
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stdout

@@ -15,6 +15,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "tb_shared_limit.h"
 #include "turbinator/training/cuda_learner.h"
 
 namespace tb_learn {
@@ -312,15 +313,13 @@ inline int multiprocessors(int *device) {
 /* Lets a kernel have `shared` bytes of dynamic shared memory; set once per
  * kernel and device, and again only where more is asked for. */
 template <auto Kernel> bool allow_shared(size_t shared) {
-    static std::atomic<size_t> allowed[kMaxDevices];
+    static SharedLimit limits[kMaxDevices];
     if (shared <= 32 * 1024) return true; /* 48 KB are allowed anyway, static shared memory included */
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
-    if (shared <= allowed[dev].load(std::memory_order_relaxed)) return true;
-    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess)
-        return false;
-    allowed[dev].store(shared, std::memory_order_relaxed);
-    return true;
+    return limits[dev].raise(shared, [](size_t bytes) {
+        return cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
+    });
 }
 
 /* A pack is 16 bytes, 4 bytes or an element: the widest one that divides all of
