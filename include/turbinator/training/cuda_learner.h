@@ -105,8 +105,8 @@ size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_desc *desc);
 /* decay [channels] f32; reset [sequences, steps] bytes or NULL; lengths
  * [sequences] int32, taken into [0, steps], or NULL; state_in [sequences,
  * channels] f32 or NULL for zero; state_out likewise (the state after the last
- * step of each sequence) or NULL; it may be state_in, so that a program that
- * acts steps its states in place (steps = 1).  checkpoints [sequences,
+ * step of each sequence) or NULL; it may be state_in, however many the steps,
+ * so that a program steps its states in place.  checkpoints [sequences,
  * ceil(steps/16), channels] f32 receives the state before every 16th step for
  * the backward pass, or NULL. */
 int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *desc, const void *x,
@@ -117,7 +117,7 @@ int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *desc, const 
 
 /* Gradients of the same from dh and dstate_out (f32, or NULL for zero).
  * ddecay [channels] f32 (NULL: not written), dstate_in [sequences, channels]
- * f32 (NULL: not written). */
+ * f32 (NULL: not written); dstate_in may be dstate_out. */
 int tb_cuda_gated_recurrence_backward_device(const tb_gated_recurrence_desc *desc, const void *x,
                                              const void *recurrence_gate, const void *input_gate,
                                              const float *decay, const uint8_t *reset,

@@ -562,3 +562,42 @@ def test_calls_follow_their_stream():
         assert tb.tb_cuda_group_norm_device(desc, x, None, None, y, None, None, work, side) == 1
     side.synchronize()
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("shape,kind", [((3, 3001, 321), "f32"), ((2, 257, 64), "bf16"), ((8, 1000, 512), "bf16"),
+                                        ((1, 4099, 40), "f16"), ((5, 700, 96), "f32"), ((4, 5, 24), "f32")], ids=str)
+@pytest.mark.parametrize("busy", (False, True))
+def test_gated_recurrence_in_place_over_many_steps(shape, kind, busy):
+    """state_out on state_in, and dstate_in on dstate_out, give the bits of separate buffers, also where the steps are
+    cut into strips and other work holds up some of them."""
+    b, t, d = shape
+    s = _recurrence_case((b, t, d, 0, 0), kind, True, True, 13)
+    new = lambda *n, dtype=torch.float32: torch.full(n, NAN, dtype=dtype, device="cuda")  # noqa: E731
+    args = (s["desc"], s["x"], s["rec"], s["inp"], s["decay"], s["reset"], s["lengths"])
+    other, m = torch.cuda.Stream(), torch.ones((2048, 2048), device="cuda")
+
+    def run(in_place):
+        out, dout = new(b, d), new(b, d)
+        first, last = s["state"], s["dstate"]
+        if in_place:
+            first, last = out, dout = s["state"].clone(), s["dstate"].clone()
+        h, saved = new(b, t, d, dtype=s["dtype"]), new(b, -(-t // 16), d)
+        grads, ddecay = new(b, t, 3 * d, dtype=s["dtype"]), new(d)
+        torch.cuda.synchronize()
+        if busy:
+            with torch.cuda.stream(other):
+                for _ in range(4):
+                    m @ m
+        assert tb.tb_cuda_gated_recurrence_device(*args, first, h, out, saved, s["work"]) == 1
+        assert tb.tb_cuda_gated_recurrence_backward_device(*args, saved, s["dh"], last, grads, grads[..., d:],
+                                                           grads[..., 2 * d:], ddecay, dout, s["work"]) == 1
+        torch.cuda.synchronize()
+        return h, saved, grads, ddecay, out, dout
+
+    want = run(False)
+    for _ in range(4):
+        assert all(torch.equal(a, c) for a, c in zip(want, run(True)))
+    if not busy:
+        exact = _recurrence_reference(s, True)
+        for name, got in (("state", want[4]), ("dstate", want[5])):
+            ref.check(name, got, *exact[name])

@@ -83,6 +83,7 @@ struct Split {
     unsigned tiles, tiles_per_sequence, rounds, strips, strip_rounds;
     unsigned magic_tiles, magic_sequence; /* floor((2^32 - 1) / tiles), .. / tiles_per_sequence) */
     float *maps;                          /* [tiles, strips, 2, channels of a tile] where strips > 1 */
+    float *first;                         /* [sequences, channels]: the state before the scan, or NULL (keep_first) */
 };
 
 /* log(1 + e^l) = max(l, 0) + log(1 + e) with e = e^-|l|, log(1 + e) =
@@ -425,6 +426,21 @@ __device__ Lane<V> before_strip(const Split &s, unsigned unit, const Lane<V> &in
     return h;
 }
 
+/* Every strip starts from the state before the scan, and the last strip's CTA
+ * writes the state after it: nothing orders the two.  Where one buffer holds
+ * both, the CTA that finds the first strip's map leaves a copy that the strips
+ * start from. */
+template <int V>
+__device__ __forceinline__ void keep_first(const Split &s, const Place &at, const RecurrenceShape &d, const float *states,
+                                           int warp, int lane) {
+    if (!s.first || at.round != 0 || warp != 0) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const size_t c = at.c0 + lane * V + v;
+        if (c < d.channels) s.first[at.b * d.channels + c] = states[at.b * d.channels + c];
+    }
+}
+
 /* A strip's map from those of its warps' parts, in the order of the scan. */
 template <int CT, int V>
 __device__ __forceinline__ void leave_map(const Split &s, unsigned unit, const Lane<V> &a, const Lane<V> &b, float (*sa)[CT],
@@ -671,6 +687,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
     const unsigned units = s.tiles * (s.strips - 1);
     for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const Place at = place_of<CT>(unit, d, p.lengths, s);
+        keep_first<V>(s, at, d, p.state_in, warp, lane);
         const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
         const int first = static_cast<int>(at.round * warps + warp * s.strip_rounds);
         const int spans = of_span((at.live + kSteps - 1) / kSteps, first, static_cast<int>(s.strip_rounds)); /* that live */
@@ -1092,6 +1109,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
     const unsigned units = s.tiles * (s.strips - 1);
     for (unsigned unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const Place at = place_of<CT>(unit, d, p.lengths, s);
+        keep_first<2>(s, at, d, p.dstate_out, warp, lane);
         const int left = static_cast<int>(d.channels) - at.c0, columns = left < CT ? left : CT;
         /* the strip's spans from its last steps on; warp 0 takes the first ones of the scan */
         const int spans = static_cast<int>(s.strip_rounds);
@@ -1207,6 +1225,9 @@ Split split_of(const RecurrenceShape &d, const Pass &p, int *warps) {
 }
 size_t map_bytes(const Split &s, int tile) {
     return s.strips > 1 ? static_cast<size_t>(s.tiles) * s.strips * 2 * tile * sizeof(float) : 0;
+}
+size_t first_bytes(const RecurrenceShape &d, const Split &s) {
+    return s.strips > 1 ? d.sequences * d.channels * sizeof(float) : 0;
 }
 
 /* Rows of partial sums for ddecay, and behind them the parts that they are first summed into. */
@@ -1329,9 +1350,9 @@ extern "C" size_t tb_cuda_gated_recurrence_workspace(const tb_gated_recurrence_d
     if (!recurrence_shape(desc, &s)) return 0;
     int warps;
     const Pass forward = forward_pass(desc->type), backward = backward_pass(desc->type);
-    const size_t f = map_bytes(split_of(s, forward, &warps), forward.tile);
-    const Split b = split_of(s, backward, &warps);
-    const size_t back = map_bytes(b, backward.tile) + partial_bytes(s, b);
+    const Split a = split_of(s, forward, &warps), b = split_of(s, backward, &warps);
+    const size_t f = map_bytes(a, forward.tile) + first_bytes(s, a);
+    const size_t back = map_bytes(b, backward.tile) + partial_bytes(s, b) + first_bytes(s, b);
     return f > back ? f : back;
 }
 
@@ -1362,6 +1383,8 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     const Pass pass = forward_pass(desc->type);
     Split split = split_of(s, pass, &warps);
     split.maps = static_cast<float *>(workspace);
+    if (split.strips > 1 && state_in && state_in == state_out)
+        split.first = split.maps + map_bytes(split, pass.tile) / sizeof(float);
     const size_t shared = static_cast<size_t>(warps) * 2 * 3 * pass.span * pass.tile * size + kBoxAlign;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
@@ -1369,6 +1392,7 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
         if (split.strips > 1 && !launch_units<recurrence_forward_maps<T>>(split.tiles * (split.strips - 1), pass, warps,
                                                                           shared, st, p, split))
             return 0;
+        if (split.first) p.state_in = split.first;
         const unsigned units = split.tiles * split.strips;
         if (split.strip_rounds < kBulkRounds)
             return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
@@ -1413,6 +1437,8 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     Split split = split_of(s, pass, &warps);
     split.maps = static_cast<float *>(workspace);
     float *partial = split.maps + map_bytes(split, pass.tile) / sizeof(float);
+    if (split.strips > 1 && dstate_out && dstate_out == dstate_in)
+        split.first = partial + partial_bytes(s, split) / sizeof(float);
     BackwardArgs p{s, x, recurrence_gate, input_gate, dh, decay, checkpoints, dstate_out, reset, lengths, dx,
                    drecurrence_gate, dinput_gate, ddecay ? partial : nullptr, dstate_in, 0, 0, 0};
     p.in_piece = piece_of(reinterpret_cast<const void *>(ins), s.is, s.it, size, 4);
@@ -1425,6 +1451,7 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
         if (split.strips > 1 && !launch_units<recurrence_backward_maps<T>>(split.tiles * (split.strips - 1), pass, warps,
                                                                            shared, st, p, split))
             return 0;
+        if (split.first) p.dstate_out = split.first;
         const unsigned units = split.tiles * split.strips;
         Maps maps{};
         bool bulk = split.strip_rounds >= kBulkRounds && p.in_piece == 16 && p.dh_piece == 16 && p.out_piece == 16 &&
