@@ -87,7 +87,8 @@ int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc, const voi
  *   log a_t = -decay_scale softplus(l) sigmoid(r_t)
  *   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t
  * A step whose reset flag is set starts anew (a_t = 0: an episode's first
- * step).  Steps at and past a sequence's length change no state; their h and
+ * step), whatever the state before it, an infinite or NaN one too: where step
+ * 0 is one, state_in may be left unset.  Steps at and past a sequence's length change no state; their h and
  * their gradients are written as zero and their inputs (NaN included) are not
  * used. */
 typedef struct tb_gated_recurrence_desc {

@@ -601,3 +601,89 @@ def test_gated_recurrence_in_place_over_many_steps(shape, kind, busy):
         exact = _recurrence_reference(s, True)
         for name, got in (("state", want[4]), ("dstate", want[5])):
             ref.check(name, got, *exact[name])
+
+
+RESET_SHAPES = [(2, 15, 33), (3, 100, 48), (2, 257, 64), (1, 1000, 96), (5, 129, 321), (8, 1000, 128), (150, 260, 136),
+                (310, 300, 40), (64, 1, 512), (90, 8, 37), (600, 50, 136), (700, 1, 190)]
+
+
+def _recurrence_run(s, shape, state, dh, dstate):
+    """Every output of both directions, the backward pass from the forward pass's checkpoints."""
+    b, t, d = shape
+    new = lambda *n, dtype=torch.float32: torch.full(n, 7.0, dtype=dtype, device="cuda")  # noqa: E731
+    o = {"h": new(b, t, d, dtype=s["dtype"]), "state": new(b, d), "checkpoints": new(b, -(-t // 16), d),
+         "grads": new(b, t, 3 * d, dtype=s["dtype"]), "ddecay": new(d), "dstate": new(b, d)}
+    args = (s["desc"], s["x"], s["rec"], s["inp"], s["decay"], s["reset"], s["lengths"])
+    assert tb.tb_cuda_gated_recurrence_device(*args, state, o["h"], o["state"], o["checkpoints"], s["work"]) == 1
+    assert tb.tb_cuda_gated_recurrence_backward_device(
+        *args, o["checkpoints"], dh, dstate, o["grads"], o["grads"][..., d:], o["grads"][..., 2 * d:], o["ddecay"],
+        o["dstate"], s["work"]) == 1
+    torch.cuda.synchronize()
+    return o
+
+
+@pytest.mark.parametrize("shape", RESET_SHAPES, ids=str)
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_gated_recurrence_starts_anew_from_any_state(shape, kind):
+    """An episode's first step forgets a state that nobody set: with a reset at step 0, states of NaN and infinities
+    give the bits that zeros give, forward and backward."""
+    b, t, d = shape
+    s = _recurrence_case((b, t, d, 0, 0), kind, True, False, 51)
+    s["reset"][:, 0] = 1
+    want = _recurrence_run(s, shape, torch.zeros((b, d), device="cuda"), s["dh"], s["dstate"])
+    state = torch.full((b, d), NAN, device="cuda")
+    state[:, 1::3] = float("inf")
+    state[:, 2::3] = -float("inf")
+    got = _recurrence_run(s, shape, state, s["dh"], s["dstate"])
+    assert torch.equal(got["checkpoints"][:, 1:], want["checkpoints"][:, 1:])
+    for name in ("h", "state", "grads", "ddecay", "dstate"):
+        assert torch.equal(got[name], want[name]), name
+
+
+@pytest.mark.parametrize("shape", [n for n in RESET_SHAPES if n[1] > 8], ids=str)
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_gated_recurrence_keeps_episodes_apart(shape, kind):
+    """NaN inputs of an episode's last step reach its state and no later step, and a NaN gradient of the last state no
+    place past a sequence's length."""
+    b, t, d = shape
+    s = _recurrence_case((b, t, d, 0, 0), kind, True, False, 52)
+    turn = torch.randint(2, t, (b,), generator=_gen(53), device="cuda")  # an episode's first step
+    row = torch.arange(b, device="cuda")
+    s["reset"][row, turn], s["reset"][row, turn - 1] = 1, 0
+    want = _recurrence_run(s, shape, s["state"], s["dh"], s["dstate"])
+    step = torch.arange(t, device="cuda")[None]
+    later, last = step >= turn[:, None], step == turn[:, None] - 1
+    clean = [s[name].clone() for name in ("x", "rec", "inp")]
+    for i, name in enumerate(("x", "rec", "inp")):  # a third of the channels each
+        s[name][..., i::3] = torch.where(last[..., None], NAN, s[name][..., i::3])
+    got = _recurrence_run(s, shape, s["state"], s["dh"], s["dstate"])
+    assert torch.isnan(got["h"][last]).all()
+    assert torch.equal(got["h"][later], want["h"][later]) and torch.equal(got["state"], want["state"])
+    saved = torch.arange(0, t, 16, device="cuda")[None] > turn[:, None]  # the state before the step
+    assert torch.equal(got["checkpoints"][saved], want["checkpoints"][saved])
+    for v, name in zip(clean, ("x", "rec", "inp")):
+        s[name].copy_(v)
+    s["lengths"] = turn.to(torch.int32)
+    got = _recurrence_run(s, shape, s["state"], s["dh"], torch.full((b, d), NAN, device="cuda"))
+    assert float(got["grads"][later].abs().max()) == 0.0 and float(got["h"][later].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("shape", RESET_SHAPES, ids=str)
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_gated_recurrence_of_empty_sequences(shape, kind):
+    """Sequences of length 0 hand their state on, NaN too, and leave no trace in the gradients."""
+    b, t, d = shape
+    s = _recurrence_case((b + 1, t, d, 0, 0), kind, False, False, 54)
+    shape = (b + 1, t, d)
+    s["lengths"] = torch.full((b + 1,), t, dtype=torch.int32, device="cuda")
+    s["lengths"][b // 2] = 0
+    want = _recurrence_run(s, shape, s["state"], s["dh"], s["dstate"])
+    state = s["state"].clone()
+    state[b // 2] = NAN
+    for name in ("x", "rec", "inp"):
+        s[name][b // 2] = float("inf")
+    got = _recurrence_run(s, shape, state, s["dh"], s["dstate"])
+    assert torch.isnan(got["state"][b // 2]).all() and float(got["h"][b // 2].abs().max()) == 0.0
+    for name in ("grads", "ddecay", "dstate"):
+        assert torch.equal(got[name], want[name]), name
+    assert torch.equal(got["dstate"][b // 2], s["dstate"][b // 2])

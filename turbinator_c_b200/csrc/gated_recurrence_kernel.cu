@@ -319,18 +319,34 @@ template <int V> struct Lane {
     float v[V];
 };
 
+/* A reset starts anew whatever the state was, an infinite or NaN one too, of
+ * which 0 times it is not 0.  So a map of states over a reset has the
+ * coefficient -0, which says that it takes nothing from the state before (no
+ * other coefficient has this sign). */
+constexpr float kAnew = -0.0f;
+__device__ __forceinline__ bool starts_anew(float a) { return __float_as_int(a) < 0; }
+/* Through the map (a, b): a state; the coefficient of a map before it.  Maps of
+ * gradients (STATES false) have no such mark. */
+template <bool STATES = true> __device__ __forceinline__ float carried(float a, float state, float b) {
+    return STATES && starts_anew(a) ? b : fmaf(a, state, b);
+}
+template <bool STATES = true> __device__ __forceinline__ float carried(float a, float before) {
+    return STATES && starts_anew(a) ? kAnew : a * before;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+
 /* Joins the spans of a CTA's round: each warp brings its span's map of V
  * channels a lane (`order`: its place in the scan) and the state before the
  * round; it leaves with the state before its own span, *state with that after
  * the round.  Every warp folds all spans, so one barrier a round does, given
  * buffers sa, sh that alternate. */
-template <int CT, int V>
+template <bool STATES, int CT, int V>
 __device__ __forceinline__ Lane<V> join(const Lane<V> &map_a, const Lane<V> &map_h, Lane<V> *state, float (*sa)[CT],
                                         float (*sh)[CT], int order, int warps, int lane) {
     Lane<V> h = *state, mine = h;
     if (warps == 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) state->v[v] = fmaf(map_a.v[v], h.v[v], map_h.v[v]);
+        for (int v = 0; v < V; ++v) state->v[v] = carried<STATES>(map_a.v[v], h.v[v], map_h.v[v]);
         return mine;
     }
 #pragma unroll
@@ -345,7 +361,7 @@ __device__ __forceinline__ Lane<V> join(const Lane<V> &map_a, const Lane<V> &map
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if (w == order) mine.v[v] = h.v[v];
-            h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
+            h.v[v] = carried<STATES>(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
         }
     }
     *state = h;
@@ -394,7 +410,7 @@ __device__ __forceinline__ Place place_after(const Place &at, const RecurrenceSh
 /* The state before a strip from `initial`, that before the first one: through
  * the maps of the strips before it, four parts of them at a time, one for each
  * of the warps that there are. */
-template <int CT, int V>
+template <bool STATES, int CT, int V>
 __device__ Lane<V> before_strip(const Split &s, unsigned unit, const Lane<V> &initial, float (*sa)[CT], float (*sh)[CT],
                                 int warp, int warps, int lane) {
     Lane<V> h = initial;
@@ -409,8 +425,8 @@ __device__ Lane<V> before_strip(const Split &s, unsigned unit, const Lane<V> &in
     for (unsigned i = first; i < last; ++i, m += 2 * CT)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            b[v] = fmaf(m[v], b[v], m[CT + v]);
-            a[v] *= m[v];
+            b[v] = carried<STATES>(m[v], b[v], m[CT + v]);
+            a[v] = carried<STATES>(m[v], a[v]);
         }
     __syncthreads(); /* the round before has read sa, sh */
 #pragma unroll
@@ -421,7 +437,7 @@ __device__ Lane<V> before_strip(const Split &s, unsigned unit, const Lane<V> &in
     __syncthreads();
     for (int w = 0; w < warps; ++w)
 #pragma unroll
-        for (int v = 0; v < V; ++v) h.v[v] = fmaf(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
+        for (int v = 0; v < V; ++v) h.v[v] = carried<STATES>(sa[w][lane * V + v], h.v[v], sh[w][lane * V + v]);
     __syncthreads(); /* sa, sh are free again */
     return h;
 }
@@ -442,7 +458,7 @@ __device__ __forceinline__ void keep_first(const Split &s, const Place &at, cons
 }
 
 /* A strip's map from those of its warps' parts, in the order of the scan. */
-template <int CT, int V>
+template <bool STATES, int CT, int V>
 __device__ __forceinline__ void leave_map(const Split &s, unsigned unit, const Lane<V> &a, const Lane<V> &b, float (*sa)[CT],
                                           float (*sh)[CT], int order, int warps, int lane) {
     __syncthreads(); /* the unit before has read sa, sh */
@@ -459,8 +475,8 @@ __device__ __forceinline__ void leave_map(const Split &s, unsigned unit, const L
     for (int v = 0; v < V; ++v) {
         float all = 1.0f, h = 0.0f;
         for (int w = 0; w < warps; ++w) {
-            all *= sa[w][lane * V + v];
-            h = fmaf(sa[w][lane * V + v], h, sh[w][lane * V + v]);
+            all = carried<STATES>(sa[w][lane * V + v], all);
+            h = carried<STATES>(sa[w][lane * V + v], h, sh[w][lane * V + v]);
         }
         m[v] = all;
         m[CT + v] = h;
@@ -504,6 +520,7 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
             const int j1 = V == 2 ? j : j + 1;
             if (anew >> j & 1) a0 = 0.0f, b0 = u0;
             if (anew >> j1 & 1) a1 = 0.0f, b1 = u1;
+            if (V == 2 && (anew >> j & 1)) a_all = h = both(0.0f); /* nothing before it is carried on */
             if (j >= live) a0 = 1.0f, b0 = 0.0f;
             if (j1 >= live) a1 = 1.0f, b1 = 0.0f;
             a = pair(a0, a1);
@@ -518,8 +535,10 @@ __device__ __forceinline__ void forward_span(const T *xs, const T *rs, const T *
             float a0, a1, b0, b1;
             split(a, a0, a1);
             split(b, b0, b1);
+            if (!FAST && (anew >> j & 1)) a_one = h_one = 0.0f; /* nothing before it is carried on */
             prod[j][0] = a_one *= a0;
             local[j][0] = h_one = fmaf(a0, h_one, b0);
+            if (!FAST && (anew >> (j + 1) & 1)) a_one = h_one = 0.0f;
             prod[j + 1][0] = a_one *= a1;
             local[j + 1][0] = h_one = fmaf(a1, h_one, b1);
         }
@@ -600,7 +619,7 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
                 state.v[v] = p.state_in && in ? p.state_in[at.b * d.channels + c] : 0.0f;
             }
             near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
-            if (at.round > 0) state = before_strip<CT, V>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
+            if (at.round > 0) state = before_strip<true, CT, V>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
         if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
         else copies_wait<1>();
@@ -619,11 +638,11 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
                 forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                map_a.v[v] = prod[kSteps - 1][v];
+                map_a.v[v] = anew ? kAnew : prod[kSteps - 1][v];
                 map_h.v[v] = local[kSteps - 1][v];
             }
         }
-        const Lane<V> h0 = join<CT, V>(map_a, map_h, &state, sa[stage], sh[stage], warp, warps, lane);
+        const Lane<V> h0 = join<true, CT, V>(map_a, map_h, &state, sa[stage], sh[stage], warp, warps, lane);
         if (BULK && next.unit < units) start(next, stage ^ 1); /* half a round ahead: the other slot has been read */
         fresh = at.round == at.last;
         const bool ends = at.round + 1 == s.rounds && p.state_out && warp == 0;
@@ -634,12 +653,17 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             if (p.checkpoints && rows > 0) p.checkpoints[(at.b * saved + t / kSteps) * d.channels + c] = h0.v[v];
             if (ends) p.state_out[at.b * d.channels + c] = state.v[v];
         }
-        if (live > 0) {
+        const auto leave = [&](auto cut) {
+            Lane<V> from = h0;
 #pragma unroll
             for (int j = 0; j < kSteps; j += 3 - V) {
                 float o0, o1;
-                split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(h0.v[0], h0.v[V - 1]),
+                if (decltype(cut)::value && (anew >> j & 1)) from.v[0] = from.v[V - 1] = 0.0f;
+                float second = from.v[V - 1];
+                if (decltype(cut)::value && V == 1 && (anew >> (j + 1) & 1)) second = 0.0f;
+                split(fma2(pair(prod[j][0], prod[j + 2 - V][V - 1]), pair(from.v[0], second),
                            pair(local[j][0], local[j + 2 - V][V - 1])), o0, o1);
+                if (V == 1) from.v[0] = second;
                 if constexpr (V == 2) {
                     *reinterpret_cast<Pack<T, 2> *>(xs + j * CT + lane * 2) = {{from_float<T>(o0), from_float<T>(o1)}};
                 } else {
@@ -647,7 +671,9 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
                     xs[(j + 1) * CT + lane] = from_float<T>(o1);
                 }
             }
-        }
+        };
+        if (anew) leave(std::true_type{}); /* an infinite or NaN state ends at the first reset */
+        else if (live > 0) leave(std::false_type{});
         if (live < kSteps) { /* steps past the sequence's length */
 #pragma unroll
             for (int j = 0; j < kSteps; ++j)
@@ -725,12 +751,13 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
                 forward_span<T, V, false>(xs, xs + kSteps * CT, xs + 2 * kSteps * CT, rate, live, anew, prod, local, lane);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                b.v[v] = fmaf(prod[kSteps - 1][v], b.v[v], local[kSteps - 1][v]);
-                a.v[v] *= prod[kSteps - 1][v];
+                const float through = anew ? kAnew : prod[kSteps - 1][v];
+                b.v[v] = carried(through, b.v[v], local[kSteps - 1][v]);
+                a.v[v] = carried(through, a.v[v]);
             }
             __syncwarp();
         }
-        leave_map<CT, V>(s, unit, a, b, sa, sh, warp, warps, lane);
+        leave_map<true, CT, V>(s, unit, a, b, sa, sh, warp, warps, lane);
     }
 }
 
@@ -910,7 +937,7 @@ __device__ __forceinline__ void backward_span(const T *xs, const T *rs, const T 
         for (int j = 0; j < kHalf; ++j)
             if (still >> j & 1) g.near_q[j] = g.far_q[j] = both(0.0f);
     }
-    *map_a = prod;
+    *map_a = anew ? both(kAnew) : prod;
     *map_h = h;
 }
 
@@ -1021,7 +1048,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
             const F2 last = p.dstate_out ? two_floats(p.dstate_out + at.b * d.channels, c) : both(0.0f);
             split(last, state.v[0], state.v[1]);
             sum_all = both(0.0f);
-            if (at.round > 0) state = before_strip<CT, 2>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
+            if (at.round > 0) state = before_strip<false, CT, 2>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
         if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
         else copies_wait<1>();
@@ -1038,11 +1065,17 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
         split(grad, from_zero.v[0], from_zero.v[1]);
         if (warps > 1) split(map_h, forward_h[stage][warp][lane * 2], forward_h[stage][warp][lane * 2 + 1]);
         const int order = warps - 1 - warp;
-        const Lane<2> after = join<CT, 2>(all, from_zero, &state, sa[stage], sh[stage], order, warps, lane);
+        const Lane<2> after = join<false, CT, 2>(all, from_zero, &state, sa[stage], sh[stage], order, warps, lane);
         grad = pair(after.v[0], after.v[1]);
-        if (warp & 1)
-            h0 = fma2(pair(sa[stage][order + 1][lane * 2], sa[stage][order + 1][lane * 2 + 1]), h0,
-                      pair(forward_h[stage][warp - 1][lane * 2], forward_h[stage][warp - 1][lane * 2 + 1]));
+        if (warp & 1) {
+            float h_one[2];
+            split(h0, h_one[0], h_one[1]);
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+                h_one[v] = carried(sa[stage][order + 1][lane * 2 + v], h_one[v], forward_h[stage][warp - 1][lane * 2 + v]);
+            h0 = pair(h_one[0], h_one[1]);
+        }
+        if ((anew & 1) | (live == 0)) h0 = both(0.0f); /* no step of the span takes it, whatever it is */
         if (BULK && next.unit < units) start(next, stage ^ 1); /* half a round ahead: the other slot has been read */
         fresh = at.round == at.last;
         if (at.round + 1 == s.rounds && p.dstate_in && warp == 0)
@@ -1062,6 +1095,13 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
             leave(to + kSlot, mul2(mul2(dlog, rate), g.m[j]));
             leave(to + 2 * kSlot, mul2(gx, g.z[j]));
             sum_all = add2(sum_all, dlog);
+        }
+        if (live < kHalf) { /* steps past the sequence's length, whatever dstate_out is */
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j)
+                if (j >= live)
+                    for (int n = 0; n < 3; ++n)
+                        *reinterpret_cast<Pack<T, 2> *>(xs + n * kSlot + j * CT + lane * 2) = {{from_float<T>(0.0f), from_float<T>(0.0f)}};
         }
         if constexpr (BULK) {
             tb_pipe::fence_proxy_async_shared();
@@ -1153,7 +1193,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
         Lane<2> map_a, map_h;
         split(all, map_a.v[0], map_a.v[1]);
         split(grad, map_h.v[0], map_h.v[1]);
-        leave_map<CT, 2>(s, unit, map_a, map_h, sa, sh, warp, warps, lane);
+        leave_map<false, CT, 2>(s, unit, map_a, map_h, sa, sh, warp, warps, lane);
     }
 }
 
