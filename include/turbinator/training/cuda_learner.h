@@ -14,7 +14,8 @@
  * into a CUDA graph and return 1 if the launches succeeded, 0 on a rejected
  * argument (NULL where it is not allowed, a size of zero or beyond the stated
  * limits, a stride smaller than its row, a pointer not aligned to its
- * element, an output on an input where that is not stated) or a launch error.
+ * element, an output or a workspace at the address of an input or of another
+ * output where that is not stated) or a launch error.
  * A descriptor is read during the call only.  Strides are in elements, 0 means
  * dense.  Tensors of `type` may be f32, bf16 or f16; parameters, statistics,
  * states and weights are f32, all sums and states are held in f32, and each

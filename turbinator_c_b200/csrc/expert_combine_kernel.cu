@@ -196,9 +196,11 @@ extern "C" int tb_cuda_combine_experts_device(const tb_expert_combine_desc *desc
                                               const int32_t *position, const float *weights, void *out,
                                               void *stream) {
     CombineShape s;
-    if (!combine_shape(desc, &s) || !rows || !position || !out || rows == out) return 0;
+    if (!combine_shape(desc, &s) || !rows || !position || !out) return 0;
     const size_t size = type_size(desc->type);
-    if (!aligned(rows, size) || !aligned(out, size) || !aligned(position, 4) || !aligned(weights, 4)) return 0;
+    if (!aligned(rows, size) || !aligned(out, size) || !aligned(position, 4) || !aligned(weights, 4) ||
+        collide({out}, {rows, position, weights}))
+        return 0;
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
@@ -227,12 +229,11 @@ extern "C" int tb_cuda_combine_experts_backward_device(const tb_expert_combine_d
                                                        const void *dout, void *drows, float *dweights,
                                                        void *stream) {
     CombineShape s;
-    if (!combine_shape(desc, &s) || (!rows && dweights) || !position || !dout || !drows || drows == rows ||
-        drows == dout)
-        return 0;
+    if (!combine_shape(desc, &s) || (!rows && dweights) || !position || !dout || !drows) return 0;
     const size_t size = type_size(desc->type);
     if (!aligned(rows, size) || !aligned(dout, size) || !aligned(drows, size) || !aligned(position, 4) ||
-        !aligned(weights, 4) || !aligned(dweights, 4))
+        !aligned(weights, 4) || !aligned(dweights, 4) ||
+        collide({drows, dweights}, {rows, position, weights, dout}))
         return 0;
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {

@@ -668,7 +668,8 @@ extern "C" int tb_cuda_route_experts_device(const tb_expert_route_desc *desc, co
         !offsets != !position)
         return 0;
     if (!aligned(logits, type_size(desc->type)) || !aligned(bias, 4) || !aligned(ids, 4) || !aligned(weights, 4) ||
-        !aligned(offsets, 4) || !aligned(order, 4) || !aligned(position, 4) || !aligned(workspace, 16))
+        !aligned(offsets, 4) || !aligned(order, 4) || !aligned(position, 4) || !aligned(workspace, 16) ||
+        collide({ids, weights, offsets, order, position, workspace}, {logits, bias}))
         return 0;
     cudaGetLastError(); /* report these launches only */
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -702,9 +703,11 @@ extern "C" int tb_cuda_route_experts_backward_device(const tb_expert_route_desc 
                                                      const int32_t *ids, const float *dweights, void *dlogits,
                                                      void *stream) {
     RouteShape s;
-    if (!route_shape(desc, &s) || !logits || !ids || !dweights || !dlogits || logits == dlogits) return 0;
+    if (!route_shape(desc, &s) || !logits || !ids || !dweights || !dlogits) return 0;
     const size_t size = type_size(desc->type);
-    if (!aligned(logits, size) || !aligned(dlogits, size) || !aligned(ids, 4) || !aligned(dweights, 4)) return 0;
+    if (!aligned(logits, size) || !aligned(dlogits, size) || !aligned(ids, 4) || !aligned(dweights, 4) ||
+        collide({dlogits}, {logits, ids, dweights}))
+        return 0;
     cudaGetLastError(); /* report this launch only */
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);

@@ -1406,7 +1406,9 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
     const size_t size = type_size(desc->type);
     if (!aligned(x, size) || !aligned(recurrence_gate, size) || !aligned(input_gate, size) || !aligned(h, size) ||
         !aligned(decay, 4) || !aligned(lengths, 4) || !aligned(state_in, 4) || !aligned(state_out, 4) ||
-        !aligned(checkpoints, 4) || !aligned(workspace, 16) || h == x || h == recurrence_gate || h == input_gate)
+        !aligned(checkpoints, 4) || !aligned(workspace, 16) ||
+        collide({h, state_out, checkpoints, workspace}, {x, recurrence_gate, input_gate, decay, reset, lengths}) ||
+        collide({h, checkpoints, workspace}, {state_in}))
         return 0;
     cudaGetLastError(); /* report these launches only */
     ForwardArgs p{s, x, recurrence_gate, input_gate, decay, state_in, reset, lengths, h, state_out, checkpoints, 0, 0};
@@ -1460,14 +1462,14 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
     if (!aligned(x, size) || !aligned(recurrence_gate, size) || !aligned(input_gate, size) || !aligned(dh, size) ||
         !aligned(dx, size) || !aligned(drecurrence_gate, size) || !aligned(dinput_gate, size) ||
         !aligned(decay, 4) || !aligned(lengths, 4) || !aligned(checkpoints, 4) || !aligned(dstate_out, 4) ||
-        !aligned(ddecay, 4) || !aligned(dstate_in, 4) || !aligned(workspace, 16))
+        !aligned(ddecay, 4) || !aligned(dstate_in, 4) || !aligned(workspace, 16) ||
+        collide({dx, drecurrence_gate, dinput_gate, ddecay, dstate_in, workspace},
+                {x, recurrence_gate, input_gate, decay, reset, lengths, checkpoints, dh}) ||
+        collide({dx, drecurrence_gate, dinput_gate, ddecay, workspace}, {dstate_out}))
         return 0;
     const void *in[] = {x, recurrence_gate, input_gate, dh}, *out[] = {dx, drecurrence_gate, dinput_gate};
     uintptr_t ins = 0, outs = 0;
     for (int i = 0; i < 3; ++i) {
-        for (const void *p : in)
-            if (out[i] == p) return 0;
-        if (out[i] == out[(i + 1) % 3]) return 0;
         ins |= reinterpret_cast<uintptr_t>(in[i]);
         outs |= reinterpret_cast<uintptr_t>(out[i]);
     }

@@ -987,7 +987,8 @@ extern "C" int tb_cuda_group_norm_device(const tb_group_norm_desc *desc, const v
     if (!norm_shape(desc, &s) || !x || !y || !workspace || !mean != !rstd) return 0;
     const size_t size = type_size(desc->type);
     if (!aligned(x, size) || !aligned(y, size) || !aligned(gamma, 4) || !aligned(beta, 4) || !aligned(mean, 4) ||
-        !aligned(rstd, 4) || !aligned(workspace, 16) || (x == y && (s.xs != s.ys || s.xp != s.yp)))
+        !aligned(rstd, 4) || !aligned(workspace, 16) || (x == y && (s.xs != s.ys || s.xp != s.yp)) ||
+        collide({y, mean, rstd, workspace}, {gamma, beta}) || collide({mean, rstd, workspace}, {x}))
         return 0;
     cudaGetLastError(); /* report these launches only */
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1028,7 +1029,8 @@ extern "C" int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc
     if (!aligned(x, size) || !aligned(dy, size) || !aligned(dx, size) || !aligned(gamma, 4) || !aligned(beta, 4) ||
         !aligned(mean, 4) || !aligned(rstd, 4) || !aligned(dgamma, 4) || !aligned(dbeta, 4) ||
         !aligned(workspace, 16) || (dx == dy && (s.gs != s.ys || s.gp != s.yp)) ||
-        (dx == x && (s.gs != s.xs || s.gp != s.xp)))
+        (dx == x && (s.gs != s.xs || s.gp != s.xp)) ||
+        collide({dx, dgamma, dbeta, workspace}, {gamma, beta, mean, rstd}) || collide({dgamma, dbeta, workspace}, {x, dy}))
         return 0;
     cudaGetLastError(); /* report these launches only */
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

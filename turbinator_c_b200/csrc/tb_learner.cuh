@@ -283,6 +283,20 @@ inline bool type_known(int type) { return type == TB_TYPE_F32 || type == TB_TYPE
 inline bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline size_t align_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
+/* Whether an output lies at the address of an input or of another output (NULL
+ * lies nowhere). */
+template <size_t OUTS, size_t INS>
+inline bool collide(const void *const (&outs)[OUTS], const void *const (&ins)[INS]) {
+    for (size_t i = 0; i < OUTS; ++i) {
+        if (!outs[i]) continue;
+        for (const void *in : ins)
+            if (outs[i] == in) return true;
+        for (size_t j = 0; j < i; ++j)
+            if (outs[i] == outs[j]) return true;
+    }
+    return false;
+}
+
 /* a * b, or false where it passes `most`. */
 inline bool product(size_t a, size_t b, size_t most, size_t *out) {
     if (a != 0 && b > most / a) return false;
