@@ -47,7 +47,9 @@ extern "C" {
 #define TB_ACT_SILU 2
 #define TB_ACT_GELU 3 /* u/2 (1 + erf(u/sqrt 2)) */
 
-/* x [samples, positions, channels]; group i holds channels
+/* samples * groups < 2^31, channels < 2^31.
+ *
+ * x [samples, positions, channels]; group i holds channels
  * [i*channels/groups, (i+1)*channels/groups).  Per (sample, group), over its
  * positions*channels/groups values:
  *   mean = E x,  rstd = 1/sqrt(E (x-mean)^2 + epsilon)
@@ -83,7 +85,10 @@ int tb_cuda_group_norm_backward_device(const tb_group_norm_desc *desc, const voi
 /* Steps between two saved states (tb_cuda_gated_recurrence_device). */
 #define TB_RECURRENCE_CHECKPOINT 16
 
-/* x, recurrence gate r, input gate i [sequences, steps, channels], per channel
+/* steps <= 2^31 - 256, sequences * channels < 2^31, sequences *
+ * ceil(channels/32) * ceil(steps/8) < 2^31.
+ *
+ * x, recurrence gate r, input gate i [sequences, steps, channels], per channel
  * a learned decay l, all channels independent:
  *   log a_t = -decay_scale softplus(l) sigmoid(r_t)
  *   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t
@@ -183,7 +188,7 @@ int tb_cuda_route_experts_backward_device(const tb_expert_route_desc *desc, cons
  * With weights NULL every weight is 1: the gradient of the gather that handed
  * the tokens out. */
 typedef struct tb_expert_combine_desc {
-    size_t tokens, rows, width;
+    size_t tokens, rows, width;     /* tokens * top_k < 2^31, rows < 2^31 */
     size_t rows_stride, out_stride; /* of rows and drows; of out and dout */
     int top_k;                      /* <= TB_ROUTE_MAX_TOP_K */
     int type;

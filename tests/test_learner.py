@@ -213,3 +213,10 @@ def test_shared_memory_limits_only_grow(tmp_path):
                     os.path.join(here, "shared_limit.cpp"), "-o", exe], check=True, timeout=120)
     run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0, run.stdout
+
+
+@pytest.mark.parametrize("over", (0, 1))
+def test_recurrence_limit_of_steps(over):
+    """The kernels count steps in 31 bits, and the last round of warps goes up to 64 steps past the end."""
+    d = _rec(sequences=1, channels=1, steps=2 ** 31 - 256 + over)
+    assert (tb.tb_cuda_gated_recurrence_workspace(d) == 0) == bool(over)

@@ -48,6 +48,8 @@ namespace {
 constexpr int kSteps = TB_RECURRENCE_CHECKPOINT; /* steps of a warp's span, forward */
 constexpr int kHalf = kSteps / 2;                /* and backward */
 constexpr int kWarps = 4;                        /* warps of a CTA at most */
+constexpr size_t kMostSteps = 0x7fffff00;        /* so that the last round's steps, of which some lie past the end, are ints */
+static_assert(kMostSteps + 2 * kWarps * kSteps <= 0x7fffffff, "a round and the next one");
 
 struct RecurrenceShape {
     size_t sequences, steps, channels;
@@ -1208,7 +1210,7 @@ struct DecayGradient {
 
 bool recurrence_shape(const tb_gated_recurrence_desc *d, RecurrenceShape *s) {
     if (!d || !d->sequences || !d->steps || !d->channels || !type_known(d->type) || !(d->decay_scale >= 0.0f) ||
-        d->steps > 0x7fffffffu)
+        d->steps > kMostSteps)
         return false;
     size_t rows, all, items;
     if (!product(d->sequences, d->channels, 0x7fffffffu, &rows) || !product(rows, d->steps, SIZE_MAX / 64, &all) ||
