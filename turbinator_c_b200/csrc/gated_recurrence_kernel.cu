@@ -290,12 +290,15 @@ __device__ __forceinline__ void boxes_read() { asm volatile("cp.async.bulk.wait_
 __device__ __forceinline__ void boxes_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 /* A warp's wait for its boxes, bounded: after a first timeout the stream's
- * status word says so and the kernel goes to its end without waiting again. */
+ * status word says so and the kernel goes to its end without waiting again, nor
+ * does it ask for boxes: a barrier whose boxes are still under way takes no
+ * further arrival. */
 struct BoxWait {
     unsigned long long limit = kWaitNs;
-    __device__ __forceinline__ void operator()(uint32_t bar, unsigned parity, unsigned *status, int lane) {
+    __device__ __forceinline__ bool gave_up() const { return limit == 0; }
+    __device__ __forceinline__ void operator()(uint32_t bar, unsigned parity, unsigned *status) {
         if (tb_pipe::mbar_wait(bar, parity, limit)) return;
-        if (lane == 0) atomicOr(status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
+        atomicOr(status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
         limit = 0;
     }
     /* At the end: the lane's stores are done, and after a timeout boxes that are
@@ -562,11 +565,12 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
     const unsigned units = s.tiles * s.strips;
 
+    BoxWait wait;
     const auto step_of = [&](const Place &to) { return static_cast<int>(to.round * warps + warp) * kSteps; };
     const auto start = [&](const Place &to, int stage) {
         const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0;
         if constexpr (BULK) {
-            if (lane == 0) {
+            if (lane == 0 && !wait.gave_up()) {
                 boxes_read(); /* the slot's outputs of two rounds ago have left */
                 const uint32_t bar = shared_address(&bars[warp][stage]);
                 const bool any = t < to.live;
@@ -586,7 +590,6 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
         const int t = step_of(to);
         return reset_byte(p.reset, to.b * d.steps + t, of_span(to.live, t), lane);
     };
-    BoxWait wait;
     if (BULK && lane == 0) {
         for (int n = 0; n < 2; ++n) tb_pipe::mbar_init(shared_address(&bars[warp][n]), 1);
         tb_pipe::fence_mbar_init();
@@ -623,7 +626,7 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
             if (at.round > 0) state = before_strip<true, CT, V>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
+        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status);
         else copies_wait<1>();
         __syncwarp();
         float prod[kSteps][V], local[kSteps][V];
@@ -959,6 +962,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
     const size_t saved = (d.steps + kSteps - 1) / kSteps;
     const unsigned units = s.tiles * s.strips;
 
+    BoxWait wait;
     /* rounds in the order of the scan: the last steps first */
     const auto step_of = [&](const Place &to) {
         return static_cast<int>((s.rounds - 1 - to.round) * warps + warp) * kHalf;
@@ -967,7 +971,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
         const int t = step_of(to), left = static_cast<int>(d.channels) - to.c0, columns = left < CT ? left : CT;
         const int live = of_span<kHalf>(to.live, t);
         if constexpr (BULK) {
-            if (lane == 0) {
+            if (lane == 0 && !wait.gave_up()) {
                 boxes_read(); /* the slot's outputs of two rounds ago have left */
                 const uint32_t bar = shared_address(&bars[warp][stage]);
                 tb_pipe::mbar_arrive_expect_tx(bar, 4 * kSlot * sizeof(T));
@@ -989,7 +993,6 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
         const int t = step_of(to);
         return reset_byte(p.reset, to.b * d.steps + t, of_span<kHalf>(to.live, t), lane);
     };
-    BoxWait wait;
     if (BULK && lane == 0) {
         for (int n = 0; n < 2; ++n) tb_pipe::mbar_init(shared_address(&bars[warp][n]), 1);
         tb_pipe::fence_mbar_init();
@@ -1052,7 +1055,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
             sum_all = both(0.0f);
             if (at.round > 0) state = before_strip<false, CT, 2>(s, at.unit, state, sa[stage], sh[stage], warp, warps, lane);
         }
-        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status, lane);
+        if (BULK) wait(shared_address(&bars[warp][stage]), parity, maps.status);
         else copies_wait<1>();
         __syncwarp();
         BackwardSpan g;
