@@ -27,6 +27,12 @@ def _call(ok: int) -> None:
         raise RuntimeError("the learner call was refused")
 
 
+def _finish() -> None:
+    """Waits for the stream; an error if a kernel's wait for its own copies ran out since the last time."""
+    if tb.tb_cuda_synchronize(torch.cuda.current_stream()) != 1:
+        raise RuntimeError("a kernel gave up waiting: the results since the last check are not valid")
+
+
 def _scratch(need: int) -> torch.Tensor:
     return torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
 
@@ -231,6 +237,7 @@ def train(actor: Actor, aircraft=16, steps=33, updates=40, rate=2e-3, seed=0):
         loss.backward()
         optimiser.step()
         actor.balance += 0.001 * torch.sign(loads.float().mean() - loads)  # the busy experts' scores go down
+        _finish()
         losses.append(loss.item())
     return losses
 
@@ -243,6 +250,7 @@ def act(actor: Actor, proprio, luma, reset):
     for t in range(proprio.shape[1]):
         guess, state, _ = actor(proprio[:, t:t + 1], luma[:, t:t + 1], state, reset[:, t:t + 1].contiguous())
         out.append(guess)
+    _finish()
     return torch.cat(out, 1)
 
 

@@ -16,6 +16,9 @@
  * limits, a stride smaller than its row, a pointer not aligned to its
  * element, an output or a workspace at the address of an input or of another
  * output where that is not stated) or a launch error.
+ * The recurrence's kernels wait for copies of their own, for a second at most;
+ * where that runs out their results are wrong, and tb_cuda_synchronize(stream)
+ * (cuda_features.h) says so by returning 0.
  * A descriptor is read during the call only.  Strides are in elements, 0 means
  * dense.  Tensors of `type` may be f32, bf16 or f16; parameters, statistics,
  * states and weights are f32, all sums and states are held in f32, and each

@@ -223,3 +223,16 @@ def test_route_takes_the_whole_of_a_group_in_one_run(kind, experts):
     for top_k in {5, 8, min(per, 32)}:
         ids, _, _ = _routed(kind, logits, None, top_k, tb.TB_SCORE_SOFTMAX, groups=32)
         assert torch.equal(ids, want[:, :top_k])
+
+
+def test_example_reports_a_wait_that_ran_out(example, monkeypatch):
+    """Training and acting end with an error where the stream's status says that a kernel gave up waiting."""
+    actor = example.Actor(width=32, experts=4, stem=16, dtype=torch.float32)
+    proprio, luma, reset = example.trajectories(2, 3)
+    asked = []
+    monkeypatch.setattr(tb, "tb_cuda_synchronize", lambda stream=None: asked.append(stream) or 0)
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        example.act(actor, proprio, luma, reset)
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        example.train(actor, aircraft=2, steps=3, updates=1)
+    assert [s.cuda_stream for s in asked] == [torch.cuda.current_stream().cuda_stream] * 2
