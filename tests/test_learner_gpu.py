@@ -687,3 +687,39 @@ def test_gated_recurrence_of_empty_sequences(shape, kind):
     for name in ("grads", "ddecay", "dstate"):
         assert torch.equal(got[name], want[name]), name
     assert torch.equal(got["dstate"][b // 2], s["dstate"][b // 2])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("shape", [(1, 20000, 272, 1, 3), (2, 9000, 1300, 2, 1), (1, 700, 2304, 1, 0),
+                                   (5, 1, 2304, 1, 0), (6, 3, 1300, 2, 1), (2, 7, 4100, 4, 0), (2, 15, 5000, 2, 0)], ids=str)
+def test_group_norm_of_wide_groups_and_many_positions(shape, kind):
+    """Groups wider than a CTA's rows: hundreds of thousands of values a thread, of one sign and nearly one size, cost
+    no more digits than the bounds allow."""
+    n, p, c, g, pad = shape
+    dtype, code = TYPES[kind]
+    gen = _gen(61)
+    x, _ = _lay(_normal(gen, n, p, c) + 1003.0, dtype, pad)
+    y, ybuf = _lay(torch.full((n, p, c), NAN, device="cuda"), dtype, pad)
+    desc = tb.GroupNormDesc(samples=n, positions=p, channels=c, groups=g, type=code, activation=ACTS["none"],
+                            epsilon=1e-5, x_sample_stride=p * (c + pad), x_position_stride=c + pad,
+                            y_sample_stride=p * (c + pad), y_position_stride=c + pad)
+    mean, rstd = torch.full((2, n, g), NAN, device="cuda")
+    work = _scratch(tb.tb_cuda_group_norm_workspace(desc))
+    assert tb.tb_cuda_group_norm_device(desc, x, None, None, y, mean, rstd, work) == 1
+    torch.cuda.synchronize()
+    ga, be = _param64(None, None, c)
+    want = ref.group_norm(x.double(), ga, be, g, 1e-5, "none")
+    errs = ref.group_norm_errors(x.double(), ga, be, g, 1e-5, "none")
+    for name, got, w, e in zip(("y", "mean", "rstd"), (y, mean, rstd), want, errs):
+        ref.check(name, got, w, e)
+    assert _untouched(y, ybuf, 0)
+    mean, rstd = want[1].float(), want[2].float()
+    del want, errs, y, ybuf
+    dy, _ = _lay(_normal(gen, n, p, c) * 0.01 + 1.003, dtype, pad)
+    dx = torch.full((n, p, c), NAN, dtype=dtype, device="cuda")
+    dgamma, dbeta = torch.full((2, c), NAN, device="cuda")
+    assert tb.tb_cuda_group_norm_backward_device(desc, x, None, None, mean, rstd, dy, dx, dgamma, dbeta, work) == 1
+    torch.cuda.synchronize()
+    want, errs = ref.group_norm_backward(x.double(), ga, be, mean.double(), rstd.double(), dy.double(), g, "none")
+    for name, got, w, e in zip(("dx", "dgamma", "dbeta"), (dx, dgamma, dbeta), want, errs):
+        ref.check(name, got, w, e)
