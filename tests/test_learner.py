@@ -2,7 +2,9 @@
 refuse before they touch a device."""
 from __future__ import annotations
 
+import copy
 import os
+import pickle
 import subprocess
 
 import pytest
@@ -220,3 +222,17 @@ def test_recurrence_limit_of_steps(over):
     """The kernels count steps in 31 bits, and the last round of warps goes up to 64 steps past the end."""
     d = _rec(sequences=1, channels=1, steps=2 ** 31 - 256 + over)
     assert (tb.tb_cuda_gated_recurrence_workspace(d) == 0) == bool(over)
+
+
+def test_copied_descriptors_stand_for_themselves():
+    """A copy of a descriptor that is changed afterwards is what its calls read, and it outlives the original."""
+    first = _norm(samples=2, positions=4096)
+    need = tb.tb_cuda_group_norm_workspace(first)
+    fresh = _norm(samples=500, positions=4096)
+    for many in (copy.copy(first), copy.deepcopy(first), pickle.loads(pickle.dumps(first)),
+                 type(first).from_buffer_copy(bytes(first)), (type(first) * 2)(first, first)[1]):
+        many.samples = 500
+        assert tb.tb_cuda_group_norm_workspace(many) == tb.tb_cuda_group_norm_workspace(fresh) != need
+        many.samples = 0
+        assert tb.tb_cuda_group_norm_workspace(many) == 0
+    assert tb.tb_cuda_group_norm_workspace(first) == need

@@ -13,6 +13,8 @@ import ctypes as _c
 
 from . import _ptr, _stream_handle, load_library
 
+_address = _c.addressof
+
 TB_TYPE_F32, TB_TYPE_BF16, TB_TYPE_F16 = range(3)
 TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU, TB_ACT_GELU = range(4)
 TB_SCORE_SOFTMAX, TB_SCORE_SIGMOID = range(2)
@@ -29,7 +31,11 @@ class _Desc(_c.Structure):
         if unknown:
             raise TypeError(f"{type(self).__name__} has no field {sorted(unknown)}")
         super().__init__(**fields)
-        self.address = _c.addressof(self)
+
+    @property
+    def address(self) -> int:
+        """Where this descriptor lies: asked for at each call, since a copy lies elsewhere."""
+        return _address(self)
 
 
 class GroupNormDesc(_Desc):
@@ -66,30 +72,30 @@ class ExpertCombineDesc(_Desc):
 
 
 def tb_cuda_group_norm_workspace(desc: GroupNormDesc) -> int:
-    return load_library().tb_cuda_group_norm_workspace(desc.address)
+    return load_library().tb_cuda_group_norm_workspace(_address(desc))
 
 
 def tb_cuda_group_norm_device(desc: GroupNormDesc, x, gamma, beta, y, mean, rstd, workspace, stream=None) -> int:
     return load_library().tb_cuda_group_norm_device(
-        desc.address, _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(workspace),
+        _address(desc), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(workspace),
         _stream_handle(stream))
 
 
 def tb_cuda_group_norm_backward_device(desc: GroupNormDesc, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta,
                                        workspace, stream=None) -> int:
     return load_library().tb_cuda_group_norm_backward_device(
-        desc.address, _ptr(x), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dy), _ptr(dx), _ptr(dgamma),
+        _address(desc), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dy), _ptr(dx), _ptr(dgamma),
         _ptr(dbeta), _ptr(workspace), _stream_handle(stream))
 
 
 def tb_cuda_gated_recurrence_workspace(desc: GatedRecurrenceDesc) -> int:
-    return load_library().tb_cuda_gated_recurrence_workspace(desc.address)
+    return load_library().tb_cuda_gated_recurrence_workspace(_address(desc))
 
 
 def tb_cuda_gated_recurrence_device(desc: GatedRecurrenceDesc, x, recurrence_gate, input_gate, decay, reset, lengths,
                                     state_in, h, state_out, checkpoints, workspace, stream=None) -> int:
     return load_library().tb_cuda_gated_recurrence_device(
-        desc.address, _ptr(x), _ptr(recurrence_gate), _ptr(input_gate), _ptr(decay), _ptr(reset), _ptr(lengths),
+        _address(desc), _ptr(x), _ptr(recurrence_gate), _ptr(input_gate), _ptr(decay), _ptr(reset), _ptr(lengths),
         _ptr(state_in), _ptr(h), _ptr(state_out), _ptr(checkpoints), _ptr(workspace), _stream_handle(stream))
 
 
@@ -97,34 +103,34 @@ def tb_cuda_gated_recurrence_backward_device(desc: GatedRecurrenceDesc, x, recur
                                              lengths, checkpoints, dh, dstate_out, dx, drecurrence_gate,
                                              dinput_gate, ddecay, dstate_in, workspace, stream=None) -> int:
     return load_library().tb_cuda_gated_recurrence_backward_device(
-        desc.address, _ptr(x), _ptr(recurrence_gate), _ptr(input_gate), _ptr(decay), _ptr(reset), _ptr(lengths),
+        _address(desc), _ptr(x), _ptr(recurrence_gate), _ptr(input_gate), _ptr(decay), _ptr(reset), _ptr(lengths),
         _ptr(checkpoints), _ptr(dh), _ptr(dstate_out), _ptr(dx), _ptr(drecurrence_gate), _ptr(dinput_gate),
         _ptr(ddecay), _ptr(dstate_in), _ptr(workspace), _stream_handle(stream))
 
 
 def tb_cuda_route_experts_workspace(desc: ExpertRouteDesc) -> int:
-    return load_library().tb_cuda_route_experts_workspace(desc.address)
+    return load_library().tb_cuda_route_experts_workspace(_address(desc))
 
 
 def tb_cuda_route_experts_device(desc: ExpertRouteDesc, logits, bias, ids, weights, offsets, order, position,
                                  workspace, stream=None) -> int:
     return load_library().tb_cuda_route_experts_device(
-        desc.address, _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(offsets), _ptr(order), _ptr(position),
+        _address(desc), _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(offsets), _ptr(order), _ptr(position),
         _ptr(workspace), _stream_handle(stream))
 
 
 def tb_cuda_route_experts_backward_device(desc: ExpertRouteDesc, logits, ids, dweights, dlogits, stream=None) -> int:
     return load_library().tb_cuda_route_experts_backward_device(
-        desc.address, _ptr(logits), _ptr(ids), _ptr(dweights), _ptr(dlogits), _stream_handle(stream))
+        _address(desc), _ptr(logits), _ptr(ids), _ptr(dweights), _ptr(dlogits), _stream_handle(stream))
 
 
 def tb_cuda_combine_experts_device(desc: ExpertCombineDesc, rows, position, weights, out, stream=None) -> int:
     return load_library().tb_cuda_combine_experts_device(
-        desc.address, _ptr(rows), _ptr(position), _ptr(weights), _ptr(out), _stream_handle(stream))
+        _address(desc), _ptr(rows), _ptr(position), _ptr(weights), _ptr(out), _stream_handle(stream))
 
 
 def tb_cuda_combine_experts_backward_device(desc: ExpertCombineDesc, rows, position, weights, dout, drows, dweights,
                                             stream=None) -> int:
     return load_library().tb_cuda_combine_experts_backward_device(
-        desc.address, _ptr(rows), _ptr(position), _ptr(weights), _ptr(dout), _ptr(drows), _ptr(dweights),
+        _address(desc), _ptr(rows), _ptr(position), _ptr(weights), _ptr(dout), _ptr(drows), _ptr(dweights),
         _stream_handle(stream))
