@@ -723,3 +723,25 @@ def test_group_norm_of_wide_groups_and_many_positions(shape, kind):
     want, errs = ref.group_norm_backward(x.double(), ga, be, mean.double(), rstd.double(), dy.double(), g, "none")
     for name, got, w, e in zip(("dx", "dgamma", "dbeta"), (dx, dgamma, dbeta), want, errs):
         ref.check(name, got, w, e)
+
+
+@pytest.mark.parametrize("shape", [(2, 50, 40), (3, 1, 40), (2, 700, 40), (200, 40, 40)], ids=str)
+def test_gated_recurrence_of_infinite_decays(shape):
+    """A decay of +inf or near f32's highest forgets every state, one of -inf or near the lowest keeps it; NaN is
+    NaN, in its channel.  No gradient of the others is anything but finite."""
+    b, t, d = shape
+    s = _recurrence_case((b, t, d, 0, 0), "f32", True, False, 71)
+    ends = torch.tensor([float("inf"), 3.4e38, 1e33, -float("inf"), -3.4e38, -1e33], device="cuda")
+    s["decay"][:30] = ends.repeat(5)
+    s["decay"][39] = NAN
+    s["rec"].clamp_(min=-5.0)  # gates that are open at all
+    o = _recurrence_run(s, shape, s["state"], s["dh"], s["dstate"])
+    s["decay"][:30] = s["decay"][:30].clamp(-1e4, 1e4)  # as good as infinite: a is 0 or 1 in 64 bits too
+    want = _recurrence_reference(s, True)
+    keep = torch.arange(d, device="cuda") != 39
+    got = dict(o, dx=o["grads"][..., :d], drec=o["grads"][..., d:2 * d], dinp=o["grads"][..., 2 * d:])
+    for name in ("h", "state", "checkpoints", "dx", "drec", "dinp", "ddecay", "dstate"):
+        value, bound = want[name]
+        assert torch.isfinite(got[name][..., keep]).all(), name
+        ref.check(name, got[name][..., keep], value[..., keep], bound[..., keep] + 1e-30)
+    assert torch.isnan(o["ddecay"][39])

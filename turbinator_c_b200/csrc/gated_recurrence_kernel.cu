@@ -93,7 +93,7 @@ struct Split {
  * is below 2e-8 of it.  The exponent keeps the part that its product rounds
  * off, so that a far negative l has all its digits. */
 __device__ __forceinline__ float softplus(float l) {
-    const float n = -fabsf(l), t = n * kLog2e;
+    const float a = -fabsf(l), n = a < -126.0f ? -126.0f : a, t = n * kLog2e; /* e is 0 from there on */
     float e = fast_exp2(t);
     e = fmaf(e, fmaf(n, kLog2e, -t) * 0.69314718f, e);
     const float r = e * fast_rcp(2.0f + e), q = r * r;
@@ -104,6 +104,14 @@ __device__ __forceinline__ float softplus(float l) {
     f = fmaf(f, q, 1.0f / 3.0f);
     f = fmaf(f, q, 1.0f);
     return fmaxf(l, 0.0f) + 2.0f * r * f;
+}
+
+/* log a of a fully open gate.  An infinite decay is one of 1e30: a product with
+ * an infinite rate would be NaN where the other factor is 0. */
+__device__ __forceinline__ float rate_of(float scale, float decay) {
+    constexpr float most = 1e30f;
+    const float s = softplus(decay), r = -scale * (s > most ? most : s);
+    return r < -most ? -most : r;
 }
 
 /* Steps of sequence b that count. */
@@ -620,7 +628,7 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             for (int v = 0; v < V; ++v) {
                 const size_t c = at.c0 + lane * V + v;
                 const bool in = c < d.channels;
-                rate[v] = in ? -d.scale * softplus(p.decay[c]) : 0.0f;
+                rate[v] = in ? rate_of(d.scale, p.decay[c]) : 0.0f;
                 state.v[v] = p.state_in && in ? p.state_in[at.b * d.channels + c] : 0.0f;
             }
             near = __all_sync(0xffffffffu, fminf(rate[0], rate[V - 1]) >= -kNear);
@@ -736,7 +744,7 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_forward_m
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const size_t c = at.c0 + lane * V + v;
-            rate[v] = c < d.channels ? -d.scale * softplus(p.decay[c]) : 0.0f;
+            rate[v] = c < d.channels ? rate_of(d.scale, p.decay[c]) : 0.0f;
             a.v[v] = 1.0f;
             b.v[v] = 0.0f;
         }
@@ -812,7 +820,7 @@ recurrence_serial(const ForwardArgs p, unsigned packs, unsigned rows) {
         float l[PACK];
         load_floats<PACK, QUADS>(p.decay + c, l);
 #pragma unroll
-        for (int i = 0; i < PACK; ++i) l[i] = -d.scale * softplus(l[i]);
+        for (int i = 0; i < PACK; ++i) l[i] = rate_of(d.scale, l[i]);
 #pragma unroll
         for (int k = 0; k < N; ++k) rate[k] = pairs(l, k);
     }
@@ -1046,8 +1054,8 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
         if (fresh) {
             float l0, l1;
             split(two_floats(p.decay, c), l0, l1);
-            l0 = c < static_cast<int>(d.channels) ? -d.scale * softplus(l0) : 0.0f;
-            l1 = c + 1 < static_cast<int>(d.channels) ? -d.scale * softplus(l1) : 0.0f;
+            l0 = c < static_cast<int>(d.channels) ? rate_of(d.scale, l0) : 0.0f;
+            l1 = c + 1 < static_cast<int>(d.channels) ? rate_of(d.scale, l1) : 0.0f;
             rate = pair(l0, l1);
             near = __all_sync(0xffffffffu, fminf(l0, l1) >= -kNear);
             const F2 last = p.dstate_out ? two_floats(p.dstate_out + at.b * d.channels, c) : both(0.0f);
@@ -1173,8 +1181,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) recurrence_backward_
         unsigned flag = past < spans ? start(past, past & 1) : 0;
         copies_end();
         const int c = at.c0 + lane * 2;
-        const float l0 = left > lane * 2 ? -d.scale * softplus(p.decay[c]) : 0.0f;
-        const float l1 = left > lane * 2 + 1 ? -d.scale * softplus(p.decay[c + 1]) : 0.0f;
+        const float l0 = left > lane * 2 ? rate_of(d.scale, p.decay[c]) : 0.0f;
+        const float l1 = left > lane * 2 + 1 ? rate_of(d.scale, p.decay[c + 1]) : 0.0f;
         F2 all = both(1.0f), grad = both(0.0f);
         for (int i = past; i < spans; ++i) {
             const int live = of_span<kHalf>(at.live, (top - i) * kHalf);
