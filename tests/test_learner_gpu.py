@@ -745,3 +745,30 @@ def test_gated_recurrence_of_infinite_decays(shape):
         assert torch.isfinite(got[name][..., keep]).all(), name
         ref.check(name, got[name][..., keep], value[..., keep], bound[..., keep] + 1e-30)
     assert torch.isnan(o["ddecay"][39])
+
+
+@pytest.mark.parametrize("top_k", (1, 2, 5, 16))
+def test_route_renormalises_scores_near_the_smallest(top_k):
+    """Sigmoid scores down to f32's last powers of two, all of a token's alike far down: their weights are ratios of
+    order 1, and so are the gradients."""
+    t, e = 400, 24
+    gen = _gen(81)
+    logits = -88.6 + 1.5 * torch.rand((t, e), generator=gen, device="cuda")
+    logits[::3] += torch.rand((len(logits[::3]), 1), generator=gen, device="cuda") * 10
+    desc = _route_desc((t, e, top_k, 1, 1, 1, "sigmoid", False, True), 0, 0, 1.0)
+    ids, weights, *_ = _route(desc, logits, None, t, e, top_k)
+    l64 = logits.double().cpu().requires_grad_(True)
+    want, _, _ = ref.route(l64.detach(), None, "sigmoid", top_k, renormalise=True)
+    assert torch.equal(ids.cpu().long(), want)
+    w = ref.route_weights(l64, want, "sigmoid", True, 1.0)
+    # each score within 8 U, and as it may be below the normal numbers, 2^-150 of at least 2.9e-39: 4 U; then sums and a division
+    ref.check("weights", weights, w.detach().cuda(), 64 * ref.U * w.detach().cuda())
+    dw = _normal(gen, t, top_k)
+    dlogits = torch.full((t, e), NAN, device="cuda")
+    assert tb.tb_cuda_route_experts_backward_device(desc, logits, ids, dw, dlogits) == 1
+    torch.cuda.synchronize()
+    grad = torch.autograd.grad(w, l64, dw.double().cpu())[0].cuda()
+    size = torch.zeros((t, e), dtype=torch.float64, device="cuda")
+    w64, top = w.detach().cuda(), dw.double().abs()
+    size.scatter_add_(1, ids.long(), w64 * (top + (top * w64).sum(1, keepdim=True)))
+    ref.check("dlogits", dlogits, grad, 96 * ref.U * size)

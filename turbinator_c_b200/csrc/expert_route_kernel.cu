@@ -532,13 +532,15 @@ route_backward_selected(RouteShape d, int lanes, bool packs, const T *logits, co
         s = there ? s / total : 0.0f;
         gradient = s * (dw - sum_of(dw * s));
     } else {
-        const float s = there ? fast_sigmoid(l) : 0.0f, rest = there ? fast_sigmoid(-l) : 0.0f;
-        float ds = dw;
+        /* below -80 as the forward pass has it, where the fast one would soon be flushed to 0 */
+        float s = there ? l < -80.0f ? sigmoid(l) : fast_sigmoid(l) : 0.0f;
+        const float rest = there ? fast_sigmoid(-l) : 0.0f;
         if (d.renormalise) {
-            const float total = sum_of(s), inner = sum_of(dw * s);
-            ds = there && total > 0.0f ? (dw - inner / total) / total : 0.0f;
+            const float total = sum_of(s);
+            s = total > 0.0f ? s / total : 0.0f; /* the weight */
+            dw -= sum_of(dw * s);
         }
-        gradient = ds * s * rest;
+        gradient = dw * s * rest;
     }
     for (int i = 0; i < tokens && base + i < d.tokens; ++i) {
         const bool mine = there && lane / lanes == i;
