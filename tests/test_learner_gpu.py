@@ -772,3 +772,50 @@ def test_route_renormalises_scores_near_the_smallest(top_k):
     w64, top = w.detach().cuda(), dw.double().abs()
     size.scatter_add_(1, ids.long(), w64 * (top + (top * w64).sum(1, keepdim=True)))
     ref.check("dlogits", dlogits, grad, 96 * ref.U * size)
+
+
+@pytest.mark.parametrize("shape", [(6, 1, 72), (3, 100, 48), (5, 129, 321), (150, 100, 136), (310, 130, 40),
+                                   (600, 50, 136), (8, 700, 128)], ids=str)
+@pytest.mark.parametrize("order", ("steps first", "gaps", "steps first, rows apart"))
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_gated_recurrence_in_other_orders(shape, order, kind):
+    """Tensors with the steps outermost, sequences at a distance that is no whole number of steps, and steps outermost of
+    which each row is followed by a gap agree with the definition as dense ones do."""
+    b, t, d = shape
+    s = _recurrence_case((b, t, d, 0, 0), kind, True, True, 91)
+    dtype = s["dtype"]
+    wide = {"steps first": (d, b * d + 16), "gaps": (t * d + 24, d), "steps first, rows apart": (d + 8, b * (d + 8))}[order]
+    dense = tb.GatedRecurrenceDesc(sequences=b, steps=t, channels=d, type=TYPES[kind][1], decay_scale=8.0)
+    laid = tb.GatedRecurrenceDesc(
+        sequences=b, steps=t, channels=d, type=TYPES[kind][1], decay_scale=8.0, in_sequence_stride=wide[0],
+        in_step_stride=wide[1], out_sequence_stride=wide[0], out_step_stride=wide[1], grad_sequence_stride=wide[0],
+        grad_step_stride=wide[1])
+    size = (b - 1) * wide[0] + (t - 1) * wide[1] + d
+
+    def lay(v):
+        whole = torch.full((size + 8,), NAN, dtype=dtype, device="cuda")
+        view = whole.as_strided((b, t, d), (*wide, 1))
+        if v is not None:
+            view.copy_(v)
+        return view, whole
+
+    def run(desc, place):
+        x, rec, inp, dh = (place(s[n])[0] for n in ("x", "rec", "inp", "dh"))
+        (h, hw), *grads = (place(None) for _ in range(4))
+        out, dstate = torch.full((2, b, d), NAN, device="cuda")
+        saved, ddecay = torch.full((b, -(-t // 16), d), NAN, device="cuda"), torch.full((d,), NAN, device="cuda")
+        args = (desc, x, rec, inp, s["decay"], s["reset"], s["lengths"])
+        assert tb.tb_cuda_gated_recurrence_device(*args, s["state"], h, out, saved, s["work"]) == 1
+        assert tb.tb_cuda_gated_recurrence_backward_device(*args, saved, dh, s["dstate"], *(g for g, _ in grads), ddecay,
+                                                           dstate, s["work"]) == 1
+        torch.cuda.synchronize()
+        return [h, *(g for g, _ in grads), out, saved, ddecay, dstate], [hw, *(w for _, w in grads)]
+
+    want, _ = run(dense, lambda v: (v.contiguous() if v is not None else torch.empty((b, t, d), dtype=dtype, device="cuda"), None))
+    got, wholes = run(laid, lay)
+    exact = _recurrence_reference(s, True)
+    for name, g, w in zip(("h", "dx", "drec", "dinp", "state", "checkpoints", "ddecay", "dstate"), got, want):
+        ref.check(name, g, *exact[name])
+        ref.check(name, w, *exact[name])
+    for g, whole in zip(got, wholes):  # nothing between the rows is written
+        assert int(torch.isnan(whole).sum()) == whole.numel() - g.numel()

@@ -273,6 +273,7 @@ template <class T> __device__ __forceinline__ T *slots_of(unsigned char *dynamic
 struct alignas(64) Maps {
     CUtensorMap in[4], out[3]; /* x, rec, inp, dh; h or dx, drec, dinp */
     unsigned *status;
+    bool inner[3]; /* x, rec and inp; dh; the outputs: sequences lie within a step */
 };
 /* What a kernel without them takes in their place. */
 struct NoMaps {
@@ -281,15 +282,15 @@ struct NoMaps {
 template <bool BULK> using MapsOf = std::conditional_t<BULK, Maps, NoMaps>;
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
-__device__ __forceinline__ void load_box(void *to, const CUtensorMap *map, int c, int t, int b, uint32_t bar) {
+__device__ __forceinline__ void load_box(void *to, const CUtensorMap *map, int c, int t, int b, bool inner, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(shared_address(to)), "l"(map), "r"(c), "r"(t), "r"(b), "r"(bar)
+        ::"r"(shared_address(to)), "l"(map), "r"(c), "r"(inner ? b : t), "r"(inner ? t : b), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void store_box(const CUtensorMap *map, const void *from, int c, int t, int b) {
+__device__ __forceinline__ void store_box(const CUtensorMap *map, const void *from, int c, int t, int b, bool inner) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                 "r"(shared_address(from)), "r"(c), "r"(t), "r"(b)
+                 "r"(shared_address(from)), "r"(c), "r"(inner ? b : t), "r"(inner ? t : b)
                  : "memory");
 }
 __device__ __forceinline__ void boxes_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -584,7 +585,7 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
                 const bool any = t < to.live;
                 tb_pipe::mbar_arrive_expect_tx(bar, any ? 3 * kSteps * CT * sizeof(T) : 0);
                 for (int n = 0; n < 3 && any; ++n)
-                    load_box(slots + (stage * 3 + n) * kSteps * CT, &maps.in[n], to.c0, t, static_cast<int>(to.b), bar);
+                    load_box(slots + (stage * 3 + n) * kSteps * CT, &maps.in[n], to.c0, t, static_cast<int>(to.b), maps.inner[0], bar);
             }
             return;
         }
@@ -697,7 +698,7 @@ recurrence_forward(const ForwardArgs p, const Split s, const __grid_constant__ M
             tb_pipe::fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0 && rows > 0) {
-                store_box(&maps.out[0], xs, at.c0, t, static_cast<int>(at.b));
+                store_box(&maps.out[0], xs, at.c0, t, static_cast<int>(at.b), maps.inner[2]);
                 boxes_end();
             }
         } else {
@@ -984,7 +985,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
                 const uint32_t bar = shared_address(&bars[warp][stage]);
                 tb_pipe::mbar_arrive_expect_tx(bar, 4 * kSlot * sizeof(T));
                 for (int n = 0; n < 4; ++n)
-                    load_box(slots + (stage * 4 + n) * kSlot, &maps.in[n], to.c0, t, static_cast<int>(to.b), bar);
+                    load_box(slots + (stage * 4 + n) * kSlot, &maps.in[n], to.c0, t, static_cast<int>(to.b), maps.inner[n / 3], bar);
             }
             return;
         }
@@ -1120,7 +1121,7 @@ recurrence_backward(const BackwardArgs p, const Split s, const __grid_constant__
             tb_pipe::fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0 && rows > 0) {
-                for (int n = 0; n < 3; ++n) store_box(&maps.out[n], xs + n * kSlot, at.c0, t, static_cast<int>(at.b));
+                for (int n = 0; n < 3; ++n) store_box(&maps.out[n], xs + n * kSlot, at.c0, t, static_cast<int>(at.b), maps.inner[2]);
                 boxes_end();
             }
         } else {
@@ -1297,7 +1298,10 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
 }
 
 /* Tensor maps of [sequences, steps, channels] tensors in boxes of one warp's
- * span and tile.  False where the driver has no such copies or refuses them. */
+ * span and tile; of the two outer dimensions the one of smaller stride comes
+ * first (*inner: sequences do), since the driver's interface wants each stride
+ * to be a multiple of the one before.  False where the driver has no such copies
+ * or refuses them, or the larger stride is no such multiple. */
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1315,17 +1319,22 @@ EncodeTiled encoder() {
     }
     return f;
 }
-bool encode(CUtensorMap *map, int type, const void *tensor, const RecurrenceShape &d, size_t sequence_stride,
+bool encode(CUtensorMap *map, bool *inner, int type, const void *tensor, const RecurrenceShape &d, size_t sequence_stride,
             size_t step_stride, const Pass &pass) {
     const EncodeTiled f = encoder();
     const size_t size = type_size(type);
-    const cuuint64_t extent[3] = {d.channels, d.steps, d.sequences};
-    const cuuint64_t stride[2] = {step_stride * size, sequence_stride * size};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(pass.tile), static_cast<cuuint32_t>(pass.span), 1}, one[3] = {1, 1, 1};
+    const bool in = d.sequences > 1 && sequence_stride < step_stride; /* sequences lie within a step */
+    const size_t first = (in ? sequence_stride : step_stride) * size;
+    const size_t second = in ? step_stride * size : d.sequences > 1 ? sequence_stride * size : first;
+    *inner = in;
+    const cuuint64_t extent[3] = {d.channels, in ? d.sequences : d.steps, in ? d.steps : d.sequences};
+    const cuuint64_t stride[2] = {first, second};
+    const cuuint32_t span = static_cast<cuuint32_t>(pass.span);
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(pass.tile), in ? 1 : span, in ? span : 1}, one[3] = {1, 1, 1};
     const CUtensorMapDataType kind = type == TB_TYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : type == TB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return f && stride[0] < 1ull << 40 && stride[1] < 1ull << 40 &&
+    return f && second < 1ull << 40 && second % first == 0 &&
            f(map, kind, 3, const_cast<void *>(tensor), extent, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
                CUDA_SUCCESS;
@@ -1453,10 +1462,10 @@ extern "C" int tb_cuda_gated_recurrence_device(const tb_gated_recurrence_desc *d
             return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
         Maps maps{};
         if (p.in_piece == 16 && p.out_piece == 16 &&
-            (maps.status = tb_status_slot(stream)) && encode(&maps.in[0], desc->type, x, s, s.is, s.it, pass) &&
-            encode(&maps.in[1], desc->type, recurrence_gate, s, s.is, s.it, pass) &&
-            encode(&maps.in[2], desc->type, input_gate, s, s.is, s.it, pass) &&
-            encode(&maps.out[0], desc->type, h, s, s.os, s.ot, pass))
+            (maps.status = tb_status_slot(stream)) && encode(&maps.in[0], &maps.inner[0], desc->type, x, s, s.is, s.it, pass) &&
+            encode(&maps.in[1], &maps.inner[0], desc->type, recurrence_gate, s, s.is, s.it, pass) &&
+            encode(&maps.in[2], &maps.inner[0], desc->type, input_gate, s, s.is, s.it, pass) &&
+            encode(&maps.out[0], &maps.inner[2], desc->type, h, s, s.os, s.ot, pass))
             return launch_units<recurrence_forward<T, true>>(units, pass, warps, shared, st, p, split, maps);
         return launch_units<recurrence_forward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
     });
@@ -1512,8 +1521,8 @@ extern "C" int tb_cuda_gated_recurrence_backward_device(
         bool bulk = split.strip_rounds >= kBulkRounds && p.in_piece == 16 && p.dh_piece == 16 && p.out_piece == 16 &&
                     (maps.status = tb_status_slot(stream));
         for (int i = 0; i < 4 && bulk; ++i)
-            bulk = encode(&maps.in[i], desc->type, in[i], s, i < 3 ? s.is : s.os, i < 3 ? s.it : s.ot, pass);
-        for (int i = 0; i < 3 && bulk; ++i) bulk = encode(&maps.out[i], desc->type, out[i], s, s.gs, s.gt, pass);
+            bulk = encode(&maps.in[i], &maps.inner[i / 3], desc->type, in[i], s, i < 3 ? s.is : s.os, i < 3 ? s.it : s.ot, pass);
+        for (int i = 0; i < 3 && bulk; ++i) bulk = encode(&maps.out[i], &maps.inner[2], desc->type, out[i], s, s.gs, s.gt, pass);
         return bulk ? launch_units<recurrence_backward<T, true>>(units, pass, warps, shared, st, p, split, maps)
                     : launch_units<recurrence_backward<T, false>>(units, pass, warps, shared, st, p, split, NoMaps{});
     });
