@@ -1163,9 +1163,13 @@ def run_ours(args, rank: int, world: int, local_rank: int):
         checked, bad = sum_over_ranks([len(idx), e + l])
         parity["render_extract_checked"], parity["render_extract_mismatches"] = checked, bad
         parity["all_mismatches"] += bad
+        import oracle  # test infrastructure: the checker only
+
+        against = [f"the reference's {what} (oracle/_ref)" if there else f"the C restatement of its {what} (oracle/)"
+                   for what, there in (("renderers", oracle.have_reference_sensors()),
+                                       ("CPU features", oracle.have_reference()))]
         render_leg["parity"] = {"checked": checked, "mismatches": bad,
-                                "against": "the reference simulator's renderers then tb_train_extract_features_cpu "
-                                           "(oracle/_ref), every 97th aircraft"}
+                                "against": " then ".join(against) + ", every 97th aircraft"}
 
     clk = clocks.summary()
     clocks.close()
