@@ -146,8 +146,11 @@ int tb_cuda_gated_recurrence_backward_device(const tb_gated_recurrence_desc *des
 
 /* logits [tokens, experts].  An expert whose logit is -inf or NaN is not
  * available to that token.  score = softmax over the available experts, or
- * sigmoid.  Experts are ranked by score + bias (both rounded to f32; by the
- * logit itself where there is no bias), ties by the lower index.  With groups >
+ * sigmoid.  Experts are ranked by score + bias in f32 (by the logit itself where
+ * there is no bias), ties by the lower index: the score is the kernel's, a
+ * sigmoid within 2^-21 of itself, a softmax score within (4 + highest logit -
+ * logit) 2^-20 of itself, so that experts nearer to each other than that may
+ * change places.  A bias of -inf or NaN takes its expert out.  With groups >
  * 1, a token first keeps its top_groups groups of experts/groups consecutive
  * experts by the sum of each group's group_best (1 or 2) highest ranking
  * values, ties by the lower index (a group with one available expert counts

@@ -236,3 +236,50 @@ def test_example_reports_a_wait_that_ran_out(example, monkeypatch):
     with pytest.raises(RuntimeError, match="gave up waiting"):
         example.train(actor, aircraft=2, steps=3, updates=1)
     assert [s.cuda_stream for s in asked] == [torch.cuda.current_stream().cuda_stream] * 2
+
+
+@pytest.mark.parametrize("score", (tb.TB_SCORE_SOFTMAX, tb.TB_SCORE_SIGMOID))
+@pytest.mark.parametrize("experts,groups", ((40, 1), (64, 8), (300, 1)))
+def test_route_bias_takes_experts_out(score, experts, groups):
+    """No token gets an expert whose bias is -inf or NaN, and the others' lists are those of a call in which it is not
+    available."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(10)
+    t, k = 300, 4
+    logits = torch.randn((t, experts), generator=gen, device="cuda")
+    bias = torch.randint(-30, 31, (experts,), generator=gen, device="cuda") * 0.01
+    out = torch.randperm(experts, generator=gen, device="cuda")[:experts // 3]
+    gone = bias.clone()
+    gone[out[::2]], gone[out[1::2]] = -float("inf"), float("nan")
+    ids, weights, _ = _routed(torch.float32, logits, gone, k, score, groups)
+    taken = ids >= 0
+    assert not torch.isin(ids[taken], out).any()
+    if score == tb.TB_SCORE_SIGMOID:  # whose scores do not depend on the others
+        logits[:, out] = -float("inf")
+        ids2, weights2, _ = _routed(torch.float32, logits, bias, k, score, groups)
+        assert torch.equal(ids, ids2) and torch.equal(weights, weights2)
+    if groups == 1:
+        assert taken.all()
+
+
+def test_route_near_ties_of_softmax_scores_with_a_bias():
+    """Scores within a few roundings of each other, told apart by the bias alone or not at all: whichever comes first,
+    the ranking values fall by no more than the stated error of a score, and none is left out that is clearly above."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(11)
+    t, e, k = 500, 96, 7
+    logits = torch.randint(-8, 1, (t, e), generator=gen, device="cuda") * 0.5
+    logits += torch.randint(-3, 4, (t, e), generator=gen, device="cuda") * 2.0 ** -21
+    bias = torch.randint(-2, 3, (e,), generator=gen, device="cuda") * 2.0 ** -14
+    ids, _, _ = _routed(torch.float32, logits, bias, k, tb.TB_SCORE_SOFTMAX)
+    l64 = logits.double()
+    rank = l64.softmax(1) + bias.double()
+    spread = l64.amax(1, keepdim=True) - l64
+    # a score's stated error, and the rounding of its sum with the bias
+    error = (4 + spread) * 2.0 ** -20 * l64.softmax(1) + 2.0 ** -24 * rank.abs()
+    assert int(ids.min()) >= 0 and all(len(set(r)) == k for r in ids.tolist())
+    got, near = rank.gather(1, ids), error.gather(1, ids)
+    assert (got[:, 1:] - got[:, :-1] <= near[:, 1:] + near[:, :-1]).all()
+    rest = rank.scatter(1, ids, -float("inf"))
+    worst = (got - near)[:, -1:]
+    assert (rest - error.scatter(1, ids, 0.0) <= worst + 2 * near[:, -1:]).all()
