@@ -4,8 +4,10 @@
  *
  * Bound: the selection by issue (a few hundred instructions a token), the rest
  * by latency: the logits are read once, the outputs written once.  65,536
- * tokens, the best 8 of 256 experts, bf16: 51 us (selection 33, slot lists 13);
- * the gradient of their weights 16 us, 4.35 TB/s, most of it dlogits' zeros.
+ * tokens, the best 8 of 256 experts, bf16: 51 us (selection 33, slot lists 13).
+ * The gradient of their weights takes 16 us for 34 MB of dlogits, nearly all of
+ * them zeros, 4 MB of ids and weights, and the sectors of the selected logits, 17
+ * MB at most: 3.3 TB/s, the zeros' way through shared memory being the rest.
  *
  * Selection, one warp a token, its experts in registers (NV consecutive ones a
  * lane): each lane sorts out its four best keys, then top_k times the best of

@@ -13,10 +13,12 @@
  *
  * Bound: HBM with the gates' arithmetic close behind it (two sigmoids, a
  * softplus' share, an exponential and a square root a step and channel, on
- * packed pairs).  64 x 1,024 x 1,024 bf16, resets, states saved: forward 126 us
- * (4.4 TB/s), backward 256 us (3.7 TB/s).  Without bulk copies 135 and 277 us
- * (no resets: 120 and 243 with them); without the short series of decays that
- * stay near 1, 147 and 274 us.
+ * packed pairs).  64 x 1,024 x 1,024 bf16, resets, states saved: forward 128 us
+ * (4.3 TB/s), backward 258 us (3.7 TB/s), without resets 124 and 251.  Without
+ * bulk copies 145 and 295 us; without the short series of decays that stay near
+ * 1, 148 and 290 us.  What keeps both from their bounds is 18 % of the warps
+ * that an SM could hold: a span's products stay in registers, 127 or 128 a
+ * thread (backward some 150 bytes of them are spilled).
  *
  * Calls of few steps or of very many rows go step by step, a thread a pack of
  * channels (forward).

@@ -13,11 +13,13 @@
  *   - Larger maps take three: each tile's statistics, their merge, and the
  *     result from a second read, last tiles first, while they are in L2.
  *   - A group of more channels than a CTA has threads times its pack takes a
- *     CTA of its own and reads three times.
+ *     CTA of its own and reads three times, value by value: 1 x 20,000 x 272 bf16
+ *     on odd rows 6.6 ms, of which a split over the positions would leave little.
  *
  * 4,096 maps of 256 x 64 bf16, silu: forward 61 us (4.4 TB/s), backward 143 us
- * (2.8 TB/s: the activation's gradient, two sums a channel and du kept in f32 lie
- * between the reads and the writes); 8 maps of 65,536 x 128: 87 us.
+ * (2.8 TB/s: neither DRAM, at a third, nor issue, at half, is full; a tile's
+ * loads, sums and stores follow each other, and registers and shared memory
+ * leave two CTAs an SM); 8 maps of 65,536 x 128: 87 us.
  *
  * Statistics of tiles merge by counts, means and squares about the own mean, so
  * that a mean far from zero costs no digits.  Per-channel sums are the common
@@ -977,7 +979,8 @@ bool norm_shape(const tb_group_norm_desc *d, NormShape *s) {
 
 /* Bytes of a tile of x at most: six such CTAs (backward, with du: two of 16-bit
  * types, three of f32) share an SM.  64 channels of bf16, of 4,096 maps of 256
- * positions: 61 us forward, 138 backward; tiles of 16 KB 88 and 232.  1,024 maps
+ * positions (the same tensors over and over: with others from call to call
+ * the backward pass takes 143): 61 us forward, 138 backward; tiles of 16 KB 88 and 232.  1,024 maps
  * of 1,024 positions: 70 and 161 us; tiles of 56 KB 79 and 241; three kernels in
  * the place of clusters 82 and 208.  Where eight such tiles do not hold a map,
  * larger ones in a cluster lose against a second read of x: 512 maps of 4,096
