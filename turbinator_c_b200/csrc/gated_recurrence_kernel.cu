@@ -391,14 +391,6 @@ struct Place {
     int c0, live; /* first channel, steps of the sequence that count */
 };
 
-__device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
-    unsigned q = __umulhi(v, magic); /* at most 2 below */
-    unsigned r = v - q * by;
-    if (r >= by) ++q, r -= by;
-    if (r >= by) ++q;
-    return q;
-}
-
 /* The first round of a unit. */
 template <int CT>
 __device__ __forceinline__ Place place_of(unsigned unit, const RecurrenceShape &d, const int32_t *lengths, const Split &s) {

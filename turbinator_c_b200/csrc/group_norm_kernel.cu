@@ -61,15 +61,6 @@ struct Tiling {
     size_t tiles;            /* of all samples */
 };
 
-/* v / by for v < 2^31, from floor((2^32 - 1) / by). */
-__device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
-    unsigned q = __umulhi(v, magic); /* at most 2 below */
-    unsigned r = v - q * by;
-    if (r >= by) ++q, r -= by;
-    if (r >= by) ++q;
-    return q;
-}
-
 template <class V, int N> __device__ __forceinline__ void activate(V (&u)[N], int act) {
     if (act == TB_ACT_SILU) {
 #pragma unroll

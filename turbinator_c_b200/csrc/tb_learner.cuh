@@ -148,6 +148,15 @@ constexpr float kLog2e = 1.44269504f;
  * from the argument's product for |v| < 8, where it matters). */
 __device__ __forceinline__ float fast_sigmoid(float v) { return fast_rcp(1.0f + fast_exp2(-kLog2e * v)); }
 
+/* v / by for v < 2^31, from floor((2^32 - 1) / by). */
+__device__ __forceinline__ unsigned divided(unsigned v, unsigned by, unsigned magic) {
+    unsigned q = __umulhi(v, magic); /* at most 2 below */
+    unsigned r = v - q * by;
+    if (r >= by) ++q, r -= by;
+    if (r >= by) ++q;
+    return q;
+}
+
 /* ---- two f32 values in one register pair, each operation on both ---- */
 
 struct F2 {
