@@ -7,7 +7,9 @@ trajectory with resets at episode ends, and a trunk of routed experts predict th
     python examples/learner_step.py            # trains for some steps, then acts step by step from kept states
 
 The ``torch.autograd.Function`` wrappers below are all that a PyTorch program needs around the C entry points; matrix
-products and the convolution are PyTorch's."""
+products and the convolution are PyTorch's.  They make descriptors, workspaces and outputs anew in each call, which a
+program that counts microseconds, as one that acts does, makes once and keeps: a step of 64 aircraft is 2 us of the
+GPU's time and more than ten times that of the host's in this form."""
 from __future__ import annotations
 
 import os
