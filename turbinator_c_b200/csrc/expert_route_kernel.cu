@@ -534,13 +534,15 @@ route_backward_selected(RouteShape d, int lanes, bool packs, const T *logits, co
         s = there ? s / total : 0.0f;
         gradient = s * (dw - sum_of(dw * s));
     } else {
-        /* below -80 as the forward pass has it, where the fast one would soon be flushed to 0 */
-        float s = there ? l < -80.0f ? sigmoid(l) : fast_sigmoid(l) : 0.0f;
+        /* 2^24 of the score: not flushed where the forward pass's score is not */
+        float s = there ? fast_rcp((1.0f + fast_exp2(-kLog2e * l)) * 0x1p-24f) : 0.0f;
         const float rest = there ? fast_sigmoid(-l) : 0.0f;
         if (d.renormalise) {
-            const float total = sum_of(s);
-            s = total > 0.0f ? s / total : 0.0f; /* the weight */
-            dw -= sum_of(dw * s);
+            const float total = sum_of(s), inner = sum_of(dw * s), over = total > 0.0f ? fast_rcp(total) : 0.0f;
+            s *= over; /* the weight */
+            dw = fmaf(-inner, over, dw);
+        } else {
+            s *= 0x1p-24f;
         }
         gradient = dw * s * rest;
     }
