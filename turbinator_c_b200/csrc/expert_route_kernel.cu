@@ -289,7 +289,6 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
         int from = 0, given = 0, expert = -1;
         for (int j = 0; j < d.top_k; ++j) {
             const unsigned best = __reduce_max_sync(0xffffffffu, head[0]);
-            if (best == 0) break; /* no head is left: nothing is given */
             bool wins = head[0] == best;
             if constexpr (!TAGGED) { /* of equal ones the first lane */
                 const int winner = __ffs(__ballot_sync(0xffffffffu, wins)) - 1;
@@ -302,8 +301,9 @@ route_select(RouteShape d, int per_cta, bool packs, const T *logits, const float
             head[kHeads - 1] = wins ? 0u : head[kHeads - 1];
             given += wins;
         }
-        /* a lane that gave all its heads: its fifth may belong */
-        if (NV > kHeads && __any_sync(0xffffffffu, given == kHeads)) {
+        /* a lane that gave all its heads: its fifth may belong (rounds in which
+         * no head was left count too, and the search ends at once where nothing is) */
+        if (NV > kHeads && __any_sync(0xffffffffu, given >= kHeads)) {
             mine = 0;
             for (int j = 0; j < d.top_k; ++j) {
                 unsigned best = 0;
