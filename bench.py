@@ -1163,7 +1163,7 @@ def run_ours(args, rank: int, world: int, local_rank: int):
         checked, bad = sum_over_ranks([len(idx), e + l])
         parity["render_extract_checked"], parity["render_extract_mismatches"] = checked, bad
         parity["all_mismatches"] += bad
-        import oracle  # test infrastructure: the checker only
+        import oracle  # test infrastructure: the parity check only
 
         against = [f"the reference's {what} (oracle/_ref)" if there else f"the C restatement of its {what} (oracle/)"
                    for what, there in (("renderers", oracle.have_reference_sensors()),

@@ -22,7 +22,11 @@
  * A descriptor is read during the call only.  Strides are in elements, 0 means
  * dense.  Tensors of `type` may be f32, bf16 or f16; parameters, statistics,
  * states and weights are f32, all sums and states are held in f32, and each
- * result is rounded once.  Every result is the same bits on every run.
+ * result is rounded once.  Every result is the same bits on every run.  The
+ * exponentials, reciprocals and square roots in SiLU, in the recurrence's gates
+ * and in softmax scores are the special function unit's: within a few units in
+ * the last place of f32 (an exponential of -v within v/2 more), 0 below its
+ * normal numbers.
  * Workspaces are scratch: at least the stated bytes, 16-byte aligned, contents
  * irrelevant, not shared by calls that may overlap; NULL if 0 bytes are
  * needed.  Any alignment and stride is accepted; rows that start on 16-byte

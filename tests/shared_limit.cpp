@@ -12,7 +12,7 @@ int main() {
     tb_learn::SharedLimit limit;
     std::mutex m;
     std::condition_variable changed;
-    size_t attribute = 0; /* as the driver would hold it */
+    size_t attribute = 0; /* as the CUDA driver would hold it */
     bool large_set = false, small_done = false;
     const auto set = [&](size_t bytes) {
         std::unique_lock<std::mutex> hold(m);

@@ -819,3 +819,26 @@ def test_gated_recurrence_in_other_orders(shape, order, kind):
         ref.check(name, w, *exact[name])
     for g, whole in zip(got, wholes):  # nothing between the rows is written
         assert int(torch.isnan(whole).sum()) == whole.numel() - g.numel()
+
+
+@pytest.mark.parametrize("shape", [(3, 70, 1300, 1), (2, 5, 2304, 1), (1, 30000, 64, 8), (2, 3000, 64, 8), (40, 3, 12, 3)],
+                         ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+def test_group_norm_in_place_in_every_form(shape, kind):
+    """y over x, dx over dy and dx over x give the bits of buffers of their own, whichever kernels the shape takes."""
+    n, p, c, g = shape
+    gen, dtype, x, gamma, beta, desc = _norm_case((n, p, c, g, 0, 0), kind, "gelu", 95)
+    work = _scratch(tb.tb_cuda_group_norm_workspace(desc))
+    y, mean, rstd = torch.empty_like(x), *torch.empty((2, n, g), device="cuda")
+    assert tb.tb_cuda_group_norm_device(desc, x, gamma, beta, y, mean, rstd, work) == 1
+    dy = _normal(gen, n, p, c).to(dtype)
+    dx, dgamma, dbeta = torch.empty_like(x), *torch.empty((2, c), device="cuda")
+    assert tb.tb_cuda_group_norm_backward_device(desc, x, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta, work) == 1
+    over_x, over_dy, out = x.clone(), dy.clone(), x.clone()
+    sums = torch.empty((2, 2, c), device="cuda")
+    assert tb.tb_cuda_group_norm_backward_device(desc, over_x, gamma, beta, mean, rstd, dy, over_x, *sums[0], work) == 1
+    assert tb.tb_cuda_group_norm_backward_device(desc, x, gamma, beta, mean, rstd, over_dy, over_dy, *sums[1], work) == 1
+    assert tb.tb_cuda_group_norm_device(desc, out, gamma, beta, out, None, None, work) == 1
+    torch.cuda.synchronize()
+    assert torch.equal(over_x, dx) and torch.equal(over_dy, dx) and torch.equal(out, y)
+    assert all(torch.equal(s[0], dgamma) and torch.equal(s[1], dbeta) for s in sums)

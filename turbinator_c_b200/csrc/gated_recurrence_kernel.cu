@@ -1293,9 +1293,9 @@ int piece_of(const void *p, size_t sequence_stride, size_t step_stride, size_t s
 
 /* Tensor maps of [sequences, steps, channels] tensors in boxes of one warp's
  * span and tile; of the two outer dimensions the one of smaller stride comes
- * first (*inner: sequences do), since the driver's interface wants each stride
- * to be a multiple of the one before.  False where the driver has no such copies
- * or refuses them, or the larger stride is no such multiple. */
+ * first (*inner: sequences do), since CUDA's interface wants each stride to be
+ * a multiple of the one before.  False where CUDA has no such copies or refuses
+ * them, or the larger stride is no such multiple. */
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
