@@ -216,6 +216,128 @@ int tb_cuda_combine_experts_backward_device(const tb_expert_combine_desc *desc, 
                                             const int32_t *position, const float *weights,
                                             const void *dout, void *drows, float *dweights, void *stream);
 
+/* ---- Handing tokens out to the experts ---- */
+
+/* The way out that the combine is the way back of, with the same descriptor:
+ * rows_stride is that of rows and drows, out_stride that of x and dx.
+ *   rows[p] = weights[s] x[s / top_k],  s = order[p] (a slot of the lists above)
+ * for every p in [0, rows).  A row whose slot lies outside [0, tokens*top_k)
+ * (-1 past the lists' end) is left as it was.  With weights NULL every weight is
+ * 1. */
+int tb_cuda_hand_out_experts_device(const tb_expert_combine_desc *desc, const void *x, const int32_t *order,
+                                    const float *weights, void *rows, void *stream);
+
+/* dx[t] = sum_j weights[t,j] drows[position[t,j]], summed over j in order, and
+ * dweights[t,j] = <x[t], drows[position[t,j]]> (0 for a slot without a row);
+ * either may be NULL, and x too where dweights is.  A position outside [0, rows)
+ * adds nothing. */
+int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_desc *desc, const void *x,
+                                             const int32_t *position, const float *weights, const void *drows,
+                                             void *dx, float *dweights, void *stream);
+
+/* ---- The experts' products ---- */
+
+#define TB_WEIGHT_IN_OUT 0 /* weights [experts, in_width, out_width] */
+#define TB_WEIGHT_OUT_IN 1 /* weights [experts, out_width, in_width] */
+
+/* rows, widths < 2^31 - 256; experts <= TB_ROUTE_MAX_EXPERTS.
+ *
+ * Expert e's rows are offsets[e] .. offsets[e+1] of x [rows, in_width], as the
+ * routing lists them; offsets [experts+1] int32 on the device, never
+ * decreasing, are taken into [0, rows].  With one expert offsets may be NULL:
+ * all rows are its.
+ *   y[p] = x[p] W_e
+ * Rows of y and dx that are no expert's are left as they were, and what those of
+ * x and dy hold is not used.  Products are summed in f32 on the tensor cores;
+ * f32 tensors are multiplied as three bf16 parts each, which leaves out less
+ * than 2^-23 of the sum of the products' magnitudes, and an infinity in one
+ * gives NaN. */
+typedef struct tb_expert_product_desc {
+    size_t rows, experts, in_width, out_width;
+    size_t in_stride, din_stride; /* of the rows of x; of dx */
+    size_t out_stride;            /* of the rows of y and dy */
+    size_t weight_expert_stride, weight_row_stride; /* of the weights and their gradient */
+    int weight_order, type;
+} tb_expert_product_desc;
+
+/* Bytes of workspace that either direction needs (0 for a bad descriptor). */
+size_t tb_cuda_experts_product_workspace(const tb_expert_product_desc *desc);
+
+int tb_cuda_experts_product_device(const tb_expert_product_desc *desc, const void *x, const void *weight,
+                                   const int32_t *offsets, void *y, void *workspace, void *stream);
+
+/* dx[p] = dy[p] W_e^T and dweight_e = sum_p x[p]^T dy[p] over expert e's rows (in
+ * the weights' order; zero for an expert without rows).  Either may be NULL, and
+ * then weight or x too. */
+int tb_cuda_experts_product_backward_device(const tb_expert_product_desc *desc, const void *x, const void *weight,
+                                            const int32_t *offsets, const void *dy, void *dx, void *dweight,
+                                            void *workspace, void *stream);
+
+/* ---- The same in 8-bit integers, for acting ---- */
+
+/* rows < 2^31.  Each row of x [rows, width] in 8-bit integers with its scale:
+ *   m = max |x|,  q = x (127 / m) in f32, rounded to nearest even,  scale = m / 127
+ * A row whose 127 / m passes f32's range (m < 2^-121, or 0) has q = 0 and scale
+ * 0; one with an infinity or a NaN q = 0 and scale NaN, so that its products are
+ * NaN.  Weights [experts, out, in] are quantised by the same call, a row per
+ * output channel. */
+typedef struct tb_quantise_desc {
+    size_t rows, width;
+    size_t x_stride, q_stride;
+    int type; /* of x */
+} tb_quantise_desc;
+
+int tb_cuda_quantise_rows_device(const tb_quantise_desc *desc, const void *x, int8_t *q, float *scale, void *stream);
+
+#define TB_I8_MAX_WIDTH 131071 /* sums of products of two 8-bit integers stay in 32 bits */
+
+/* As tb_expert_product_desc, in_width <= TB_I8_MAX_WIDTH, weights [experts, out_width, in_width]:
+ *   y[p,c] = (sum_k q[p,k] weight_e[c,k]) (q_scale[p] weight_scale_e[c])
+ * The sum is exact; its conversion and the two products are f32. */
+typedef struct tb_expert_product_i8_desc {
+    size_t rows, experts, in_width, out_width;
+    size_t in_stride, out_stride; /* of the rows of q; of y */
+    size_t weight_expert_stride, weight_row_stride;
+    int type; /* of y */
+} tb_expert_product_i8_desc;
+
+size_t tb_cuda_experts_product_i8_workspace(const tb_expert_product_i8_desc *desc);
+
+/* q_scale [rows], weight_scale [experts, out_width]. */
+int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc *desc, const int8_t *q, const float *q_scale,
+                                      const int8_t *weight, const float *weight_scale, const int32_t *offsets, void *y,
+                                      void *workspace, void *stream);
+
+/* ---- Orthogonalised updates ---- */
+
+#define TB_ORTHOGONALISE_MAX_SIDE 65536
+
+/* matrices <= 65,535; rows, columns <= TB_ORTHOGONALISE_MAX_SIDE; 1 <= steps <= 64.
+ *
+ * Each matrix g [rows, columns] is divided by its Frobenius norm and its
+ * singular values are driven to where the odd polynomial keeps them:
+ *   x = g / (|g| + epsilon)
+ *   steps times: x = (a + b x x^T + c (x x^T)^2) x
+ *   out = scale x
+ * (3.4445, -4.7750, 2.0315 in five steps bring most singular values within 0.7
+ * to 1.2.)  The products are taken of pairs of f16 values on the tensor cores,
+ * 22 bits for values of an average element's size and up.  No element of x, x
+ * x^T or the polynomial may pass 15 in magnitude on the way: NaN otherwise.  A
+ * matrix of zeros gives zeros, one with an infinity or a NaN gives NaN. */
+typedef struct tb_orthogonalise_desc {
+    size_t matrices, rows, columns;
+    size_t in_matrix_stride, in_row_stride;   /* of g */
+    size_t out_matrix_stride, out_row_stride; /* of out */
+    int type, steps;
+    float a, b, c, epsilon, scale;
+} tb_orthogonalise_desc;
+
+size_t tb_cuda_orthogonalise_workspace(const tb_orthogonalise_desc *desc);
+
+/* out may be g (same strides). */
+int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, const void *g, void *out, void *workspace,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,16 @@ _LEARNER_ARGUMENTS = {
     "tb_cuda_route_experts_backward_device": [_vp] * 6,
     "tb_cuda_combine_experts_device": [_vp] * 6,
     "tb_cuda_combine_experts_backward_device": [_vp] * 8,
+    "tb_cuda_hand_out_experts_device": [_vp] * 6,
+    "tb_cuda_hand_out_experts_backward_device": [_vp] * 8,
+    "tb_cuda_experts_product_workspace": [_vp],
+    "tb_cuda_experts_product_device": [_vp] * 7,
+    "tb_cuda_experts_product_backward_device": [_vp] * 9,
+    "tb_cuda_quantise_rows_device": [_vp] * 5,
+    "tb_cuda_experts_product_i8_workspace": [_vp],
+    "tb_cuda_experts_product_i8_device": [_vp] * 9,
+    "tb_cuda_orthogonalise_workspace": [_vp],
+    "tb_cuda_orthogonalise_device": [_vp] * 5,
 }
 
 
@@ -429,9 +439,13 @@ def generate(seed: int, first: int, count: int, *, total: Optional[int] = None,
 # ---- learner layers (include/turbinator/training/cuda_learner.h) ----
 
 from .learner import (  # noqa: E402  (needs the helpers above)
-    ExpertCombineDesc, ExpertRouteDesc, GatedRecurrenceDesc, GroupNormDesc, RECURRENCE_CHECKPOINT, TB_ACT_GELU,
-    TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU, TB_SCORE_SIGMOID, TB_SCORE_SOFTMAX, TB_TYPE_BF16, TB_TYPE_F16, TB_TYPE_F32,
-    tb_cuda_combine_experts_backward_device, tb_cuda_combine_experts_device, tb_cuda_gated_recurrence_backward_device,
-    tb_cuda_gated_recurrence_device, tb_cuda_gated_recurrence_workspace, tb_cuda_group_norm_backward_device,
-    tb_cuda_group_norm_device, tb_cuda_group_norm_workspace, tb_cuda_route_experts_backward_device,
-    tb_cuda_route_experts_device, tb_cuda_route_experts_workspace)
+    ExpertCombineDesc, ExpertProductDesc, ExpertProductI8Desc, ExpertRouteDesc, GatedRecurrenceDesc, GroupNormDesc,
+    OrthogonaliseDesc, QuantiseDesc, RECURRENCE_CHECKPOINT, TB_ACT_GELU, TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU,
+    TB_SCORE_SIGMOID, TB_SCORE_SOFTMAX, TB_TYPE_BF16, TB_TYPE_F16, TB_TYPE_F32, TB_WEIGHT_IN_OUT, TB_WEIGHT_OUT_IN,
+    tb_cuda_combine_experts_backward_device, tb_cuda_combine_experts_device, tb_cuda_experts_product_backward_device,
+    tb_cuda_experts_product_device, tb_cuda_experts_product_i8_device, tb_cuda_experts_product_i8_workspace,
+    tb_cuda_experts_product_workspace, tb_cuda_gated_recurrence_backward_device, tb_cuda_gated_recurrence_device,
+    tb_cuda_gated_recurrence_workspace, tb_cuda_group_norm_backward_device, tb_cuda_group_norm_device,
+    tb_cuda_group_norm_workspace, tb_cuda_hand_out_experts_backward_device, tb_cuda_hand_out_experts_device,
+    tb_cuda_orthogonalise_device, tb_cuda_orthogonalise_workspace, tb_cuda_quantise_rows_device,
+    tb_cuda_route_experts_backward_device, tb_cuda_route_experts_device, tb_cuda_route_experts_workspace)

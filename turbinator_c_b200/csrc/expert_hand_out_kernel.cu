@@ -1,0 +1,201 @@
+/*
+ * Tokens handed out to their experts, weights applied on the way, and the
+ * gradient (include/turbinator/training/cuda_learner.h).
+ *
+ * Bound: HBM; a row of the output is written once, a token's row read from L2
+ * by all but the first of its slots.  The gradient reads every slot's row once.
+ */
+#include "tb_learner.cuh"
+
+using namespace tb_learn;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 4; /* rows of a token under way at once */
+
+struct HandShape {
+    size_t tokens, rows, width, rows_stride, token_stride;
+    int top_k;
+};
+
+/* lanes: of a team that takes a row's chunk of `lanes` packs; chunks: of a row. */
+template <class T, int PACK>
+__global__ void __launch_bounds__(kThreads)
+hand_out(HandShape d, int lanes, int chunks, const T *x, const int32_t *order, const float *weights, T *rows) {
+    const size_t team = (static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x) / lanes;
+    const int lane = threadIdx.x % lanes;
+    const size_t p = team / chunks, c = ((team - p * chunks) * lanes + lane) * PACK;
+    if (p >= d.rows || c >= d.width) return;
+    const int32_t slot = order[p];
+    if (slot < 0 || static_cast<size_t>(slot) >= d.tokens * d.top_k) return;
+    Held<T, PACK> v = *reinterpret_cast<const Held<T, PACK> *>(x + static_cast<size_t>(slot / d.top_k) * d.token_stride + c);
+    if (weights) {
+        const float w = weights[slot];
+        float e[PACK];
+        unpack(v, e);
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) e[i] *= w;
+        v = packed<T, PACK>(e);
+    }
+    store_once<T, PACK>(rows + p * d.rows_stride + c, v);
+}
+
+/* `warps` (1, 2, 4 or 8) take a token, every warps-th chunk of 32 packs each. */
+template <class T, int PACK>
+__global__ void __launch_bounds__(kThreads)
+hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, const float *weights, const T *drows, T *dx,
+                  float *dweights) {
+    __shared__ float dots[kWarps][TB_ROUTE_MAX_TOP_K];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % warps;
+    const size_t t = static_cast<size_t>(blockIdx.x) * (kWarps / warps) + warp / warps;
+    int32_t p = -1;
+    float w = 1.0f;
+    if (t < d.tokens && lane < d.top_k) {
+        p = position[t * d.top_k + lane];
+        if (p >= 0 && static_cast<size_t>(p) >= d.rows) p = -1;
+        if (weights) w = weights[t * d.top_k + lane];
+    }
+    dots[warp][lane] = 0.0f;
+    __syncwarp();
+    if (t < d.tokens)
+        for (size_t base = static_cast<size_t>(part) * 32 * PACK; base < d.width; base += static_cast<size_t>(warps) * 32 * PACK) {
+            const size_t c = base + lane * PACK;
+            const bool in = c < d.width;
+            float g[PACK], sum[PACK];
+#pragma unroll
+            for (int i = 0; i < PACK; ++i) g[i] = sum[i] = 0.0f;
+            if (dweights && in) unpack(*reinterpret_cast<const Held<T, PACK> *>(x + t * d.token_stride + c), g);
+            for (int j = 0; j < d.top_k; j += kAhead) {
+                Held<T, PACK> v[kAhead];
+                int32_t row[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    row[k] = __shfl_sync(0xffffffffu, p, min(j + k, d.top_k - 1));
+                    if (j + k >= d.top_k || !in) row[k] = -1;
+                    if (row[k] >= 0) v[k] = load_once<T, PACK>(drows + row[k] * d.rows_stride + c);
+                }
+                float dot[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const float s = __shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1));
+                    dot[k] = 0.0f;
+                    if (row[k] < 0) continue;
+                    float e[PACK];
+                    unpack(v[k], e);
+#pragma unroll
+                    for (int i = 0; i < PACK; ++i) {
+                        sum[i] = fmaf(s, e[i], sum[i]);
+                        dot[k] = fmaf(g[i], e[i], dot[k]);
+                    }
+                }
+                if (dweights) { /* each half of the warp sums half of the slots, and so on, down to eight lanes a slot */
+                    int spread = 16;
+#pragma unroll
+                    for (int n = kAhead / 2; n; n /= 2, spread /= 2) {
+                        const bool upper = lane & spread;
+#pragma unroll
+                        for (int k = 0; k < n; ++k) {
+                            const float mine = upper ? dot[k + n] : dot[k];
+                            dot[k] = mine + __shfl_xor_sync(0xffffffffu, upper ? dot[k] : dot[k + n], spread);
+                        }
+                    }
+                    for (; spread; spread /= 2) dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], spread);
+                    const int slot = j + lane / (32 / kAhead);
+                    if (lane % (32 / kAhead) == 0 && slot < d.top_k) dots[warp][slot] += dot[0];
+                }
+            }
+            if (dx && in) *reinterpret_cast<Held<T, PACK> *>(dx + t * d.token_stride + c) = packed<T, PACK>(sum);
+        }
+    if (!dweights) return;
+    __syncthreads();
+    if (t < d.tokens && part == 0 && lane < d.top_k) {
+        float sum = 0.0f;
+        for (int i = 0; i < warps; ++i) sum += dots[warp + i][lane];
+        dweights[t * d.top_k + lane] = sum;
+    }
+}
+
+bool hand_shape(const tb_expert_combine_desc *d, HandShape *s) {
+    if (!d || !d->tokens || !d->rows || !d->width || d->top_k < 1 || d->top_k > TB_ROUTE_MAX_TOP_K ||
+        !type_known(d->type) || d->rows > 0x7fffffffu)
+        return false;
+    size_t slots, all;
+    if (!product(d->tokens, d->top_k, 0x7fffffffu, &slots)) return false;
+    s->tokens = d->tokens;
+    s->rows = d->rows;
+    s->width = d->width;
+    s->rows_stride = d->rows_stride ? d->rows_stride : d->width;
+    s->token_stride = d->out_stride ? d->out_stride : d->width;
+    s->top_k = d->top_k;
+    return s->rows_stride >= d->width && s->token_stride >= d->width &&
+           product(d->rows, s->rows_stride, SIZE_MAX / 64, &all) && product(d->tokens, s->token_stride, SIZE_MAX / 64, &all);
+}
+
+/* Calls f with the widest pack that every row of the tensors allows, as a
+ * constant: 16, 8 or 4 bytes or an element. */
+template <class T, class F>
+int with_row_pack(const HandShape &s, const void *a, const void *b, const void *c, F &&f) {
+    const size_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
+                        (s.rows_stride | s.token_stride | s.width) * sizeof(T);
+    if (bits % 16 == 8) return f(std::integral_constant<int, 8 / static_cast<int>(sizeof(T))>{});
+    return with_pack<T>(pack_of(bits, sizeof(T)), f);
+}
+
+} /* namespace */
+
+extern "C" int tb_cuda_hand_out_experts_device(const tb_expert_combine_desc *desc, const void *x, const int32_t *order,
+                                               const float *weights, void *rows, void *stream) {
+    HandShape s;
+    if (!hand_shape(desc, &s) || !x || !order || !rows) return 0;
+    const size_t size = type_size(desc->type);
+    if (!aligned(x, size) || !aligned(rows, size) || !aligned(order, 4) || !aligned(weights, 4) ||
+        collide({rows}, {x, order, weights}))
+        return 0;
+    cudaGetLastError(); /* report this launch only */
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        return with_row_pack<T>(s, x, rows, nullptr, [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            const size_t packs = (s.width + P - 1) / P;
+            int lanes = 1;
+            while (lanes < 32 && static_cast<size_t>(lanes) < packs) lanes *= 2;
+            const auto places = [&](size_t n) { return (packs + n - 1) / n * n; };
+            while (lanes > 8 && places(lanes / 2) * 5 <= places(lanes) * 4) lanes /= 2;
+            const size_t chunks = (packs + lanes - 1) / lanes;
+            size_t teams;
+            if (!product(s.rows, chunks, 0x7fffffffull * (kThreads / lanes), &teams) || chunks > 0x7fffffffu) return 0;
+            hand_out<T, P><<<static_cast<unsigned>((teams * lanes + kThreads - 1) / kThreads), kThreads, 0,
+                             static_cast<cudaStream_t>(stream)>>>(s, lanes, static_cast<int>(chunks), static_cast<const T *>(x),
+                                                                  order, weights, static_cast<T *>(rows));
+            return launched();
+        });
+    });
+}
+
+extern "C" int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_desc *desc, const void *x,
+                                                        const int32_t *position, const float *weights, const void *drows,
+                                                        void *dx, float *dweights, void *stream) {
+    HandShape s;
+    if (!hand_shape(desc, &s) || (!x && dweights) || !position || !drows || (!dx && !dweights)) return 0;
+    const size_t size = type_size(desc->type);
+    if (!aligned(x, size) || !aligned(drows, size) || !aligned(dx, size) || !aligned(position, 4) || !aligned(weights, 4) ||
+        !aligned(dweights, 4) || collide({dx, dweights}, {x, position, weights, drows}))
+        return 0;
+    cudaGetLastError(); /* report this launch only */
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        return with_row_pack<T>(s, x, drows, dx, [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            int warps = 1;
+            while (warps < kWarps && static_cast<size_t>(warps) * 32 * P < s.width) warps *= 2;
+            const size_t per = kWarps / warps;
+            hand_out_backward<T, P><<<static_cast<unsigned>((s.tokens + per - 1) / per), kThreads, 0,
+                                      static_cast<cudaStream_t>(stream)>>>(
+                s, warps, static_cast<const T *>(x), position, weights, static_cast<const T *>(drows), static_cast<T *>(dx),
+                dweights);
+            return launched();
+        });
+    });
+}

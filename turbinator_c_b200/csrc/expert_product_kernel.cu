@@ -1,0 +1,520 @@
+/*
+ * The experts' products, forward and both gradients, and the same in 8-bit
+ * integers (include/turbinator/training/cuda_learner.h).
+ *
+ * y[p] = x[p] W_e and dx[p] = dy[p] W_e^T are one job: rows of one expert (up
+ * to 256, taken as they come: the tensor cores issue as many columns) against
+ * 128 of the output's channels; tiles of one set of rows follow each other, so
+ * the rows stay in L2 and so do the expert's weights.  Where an expert's rows
+ * start is read on the device.  dW_e = sum_p x[p]^T dy[p] sums over a run of
+ * rows that ends anywhere: what the last 16 of a run reads of the next
+ * expert's rows is cleared in shared memory.  The contiguous dimension of
+ * every output lies in the tensor core's rows (tb_tensor.cuh).
+ *
+ * f32 tensors are laid out as three bf16 planes that sum to them exactly (8
+ * bits each) and multiplied as six pairs, small ones first; what is left out
+ * is below 2^-24 of the factors.  Rows that do not start on 16 bytes are laid
+ * out anew too, in the workspace.
+ */
+#include "tb_tensor.cuh"
+
+using namespace tb_learn;
+using tb_tensor::Matrices;
+using tb_tensor::Operands;
+using tb_tensor::Tile;
+
+namespace {
+
+constexpr int kMaxExperts = TB_ROUTE_MAX_EXPERTS;
+
+struct Runs { /* of rows, one for each expert */
+    const int32_t *offsets; /* NULL: one expert, all rows */
+    int experts, rows;
+};
+/* Expert e's rows: offsets taken into [0, rows], a run that would end before its start is empty. */
+__device__ __forceinline__ int run_start(const Runs &r, int e) {
+    return r.offsets ? min(max(r.offsets[e], 0), r.rows) : 0;
+}
+__device__ __forceinline__ int run_end(const Runs &r, int e, int start) {
+    return r.offsets ? max(min(max(r.offsets[e + 1], 0), r.rows), start) : r.rows;
+}
+
+template <class T> __device__ __forceinline__ T stored(uint32_t r) { return from_float<T>(__uint_as_float(r)); }
+
+/* ---- O[p, m] = sum_k X[p, k] W_e[m, k] ---- */
+
+template <class T, int NT> struct RowJob {
+    static constexpr bool kRagged = false;
+    struct Shared {
+        int first[kMaxExperts + 1]; /* tile of rows that each expert's start with */
+        int start[kMaxExperts], end[kMaxExperts];
+    };
+    Runs runs;
+    int width, depth, tiles_m;
+    T *out;
+    size_t out_stride;
+
+    __device__ void setup(Shared &s) const {
+        for (int e = threadIdx.x; e < runs.experts; e += tb_tensor::kThreads) {
+            s.start[e] = run_start(runs, e);
+            s.end[e] = run_end(runs, e, s.start[e]);
+        }
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            int before = 0;
+            for (int base = 0; base < runs.experts; base += 32) {
+                const int e = base + threadIdx.x;
+                int n = e < runs.experts ? (s.end[e] - s.start[e] + NT - 1) / NT : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const int v = __shfl_up_sync(0xffffffffu, n, o);
+                    if (threadIdx.x >= o) n += v;
+                }
+                if (e < runs.experts) s.first[e + 1] = before + n;
+                before += __shfl_sync(0xffffffffu, n, 31);
+            }
+            if (threadIdx.x == 0) s.first[0] = 0;
+        }
+    }
+    __device__ int tiles(const Shared &s) const { return s.first[runs.experts] * tiles_m; }
+    __device__ Tile tile(const Shared &s, int t) const {
+        const int of = t / tiles_m;
+        int low = 0, high = runs.experts; /* first[low] <= of < first[high] */
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            if (s.first[mid] <= of) low = mid;
+            else high = mid;
+        }
+        Tile r;
+        r.m0 = (t - of * tiles_m) * tb_tensor::kTileM;
+        r.n0 = s.start[low] + (of - s.first[low]) * NT;
+        r.columns = min(NT, s.end[low] - r.n0);
+        r.k0 = 0;
+        r.depth = depth;
+        r.az = low;
+        r.bz = 0;
+        r.which = low;
+        return r;
+    }
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[32]) const {
+        if (m >= width) return;
+        T *o = out + (t.n0 + c) * out_stride + m;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (c + i < t.columns) o[i * out_stride] = stored<T>(r[i]);
+    }
+};
+
+/* The same of 8-bit integers, scaled by row and channel. */
+template <class T, int NT> struct IntegerJob : RowJob<T, NT> {
+    const float *row_scale, *channel_scale;
+    __device__ __forceinline__ void store(const typename RowJob<T, NT>::Shared &, const Tile &t, int m, int c,
+                                          const uint32_t (&r)[32]) const {
+        if (m >= this->width) return;
+        T *o = this->out + (t.n0 + c) * this->out_stride + m;
+        const float s = channel_scale[static_cast<size_t>(t.which) * this->width + m];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (c + i < t.columns)
+                o[i * this->out_stride] = from_float<T>(static_cast<float>(static_cast<int>(r[i])) * (row_scale[t.n0 + c + i] * s));
+    }
+};
+
+/* ---- O_e[n, m] = sum_p B[p, n] A[p, m] over expert e's rows ---- */
+
+template <class T, int NT> struct SumJob {
+    static constexpr bool kRagged = true;
+    struct Shared {};
+    Runs runs;
+    int width, height, tiles_m, tiles_n;
+    T *out;
+    size_t row_stride, matrix_stride;
+
+    __device__ void setup(Shared &) const {}
+    __device__ int tiles(const Shared &) const { return runs.experts * tiles_m * tiles_n; }
+    __device__ Tile tile(const Shared &, int t) const {
+        const int per = tiles_m * tiles_n, e = t / per, in = t - e * per, tn = in / tiles_m;
+        Tile r;
+        r.m0 = (in - tn * tiles_m) * tb_tensor::kTileM;
+        r.n0 = tn * NT;
+        r.columns = min(NT, height - r.n0);
+        r.k0 = run_start(runs, e);
+        r.depth = run_end(runs, e, r.k0) - r.k0;
+        r.az = r.bz = 0;
+        r.which = e;
+        return r;
+    }
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[32]) const {
+        if (m >= width) return;
+        T *o = out + t.which * matrix_stride + (t.n0 + c) * row_stride + m;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (c + i < t.columns) o[i * row_stride] = stored<T>(r[i]);
+    }
+};
+
+/* ---- laying operands out ---- */
+
+struct Layout {
+    size_t width, rows, count, row_stride, matrix_stride; /* of the source */
+    size_t line;                                          /* of the copy: a multiple of 16 bytes */
+};
+
+/* A value's planes: three bf16 that sum to it (the first alone where it is no
+ * finite number), or the value itself. */
+__device__ __forceinline__ void planes_of(float v, __nv_bfloat16 (&p)[3]) {
+    p[0] = __float2bfloat16_rn(v);
+    if (__hisinf(p[0]) && isfinite(v)) p[0] = __float2bfloat16_rz(v); /* rounded past the largest */
+    const float rest = isfinite(v) ? v - __bfloat162float(p[0]) : 0.0f;
+    p[1] = __float2bfloat16_rn(rest);
+    p[2] = __float2bfloat16_rn(rest - __bfloat162float(p[1]));
+}
+
+constexpr int kLayThreads = 256;
+template <class T>
+__global__ void __launch_bounds__(kLayThreads) lay_out(Layout d, const T *from, void *to) {
+    const size_t lines = d.rows * d.count, all = lines * d.line;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * kLayThreads + threadIdx.x; i < all;
+         i += static_cast<size_t>(gridDim.x) * kLayThreads) {
+        const size_t row = i / d.line, c = i - row * d.line, z = row / d.rows, r = row - z * d.rows;
+        const bool in = c < d.width;
+        const T *at = from + z * d.matrix_stride + r * d.row_stride + c;
+        if constexpr (sizeof(T) == 4) {
+            __nv_bfloat16 p[3];
+            planes_of(in ? to_float(*at) : 0.0f, p);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) static_cast<__nv_bfloat16 *>(to)[j * all + i] = p[j];
+        } else {
+            T v{};
+            if (in) v = *at;
+            static_cast<T *>(to)[i] = v;
+        }
+    }
+}
+
+/* A tensor of a call, and where it lies for the tensor cores. */
+struct Source {
+    const void *at;
+    size_t width, rows, count, row_stride, matrix_stride;
+};
+/* Elements of a laid-out line, and bytes of the whole. */
+size_t line_of(size_t width, size_t size) { return align_up(width, 16 / size); }
+size_t laid_bytes(size_t width, size_t rows, size_t count, bool wide, size_t size) {
+    return align_up(line_of(width, size) * rows * count * (wide ? 3 : 1) * size, 256);
+}
+
+template <class T> int lay(const Source &s, size_t size, unsigned char **scratch, Matrices *m, cudaStream_t st) {
+    const bool wide = sizeof(T) == 4;
+    *m = Matrices{s.at, s.width, s.rows, s.count, s.row_stride, s.matrix_stride, size};
+    if (!wide && m->straight()) return 1;
+    if (!*scratch) return 0;
+    const size_t line = line_of(s.width, size), all = line * s.rows * s.count;
+    const Layout d{s.width, s.rows, s.count, s.row_stride, s.matrix_stride, line};
+    const size_t blocks = (all + kLayThreads * 4 - 1) / (kLayThreads * 4);
+    lay_out<T><<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), kLayThreads, 0, st>>>(
+        d, static_cast<const T *>(s.at), *scratch);
+    if (!launched()) return 0;
+    *m = Matrices{*scratch, s.width, s.rows, s.count * (wide ? 3 : 1), line, line * s.rows, size};
+    *scratch += laid_bytes(s.width, s.rows, s.count, wide, size);
+    return 1;
+}
+
+/* The planes' pairs: all of the value, or six of three by three. */
+void pairs_of(Operands *ops, bool wide, size_t a_count, size_t b_count) {
+    static const int a[6] = {2, 0, 1, 1, 0, 0}, b[6] = {0, 2, 1, 0, 1, 0};
+    ops->pairs = wide ? 6 : 1;
+    for (int i = 0; i < ops->pairs; ++i) {
+        ops->a_plane[i] = wide ? a[i] * static_cast<int>(a_count) : 0;
+        ops->b_plane[i] = wide ? b[i] * static_cast<int>(b_count) : 0;
+    }
+}
+
+/* ---- shapes ---- */
+
+struct ProductShape {
+    size_t rows, experts, in, out, x_stride, dx_stride, y_stride, w_row, w_matrix;
+    bool turned; /* weights [out, in] */
+    size_t size;
+    bool wide;
+};
+
+bool product_shape(const tb_expert_product_desc *d, ProductShape *s) {
+    if (!d || !d->rows || !d->experts || !d->in_width || !d->out_width || !type_known(d->type) ||
+        d->experts > kMaxExperts || d->rows > 0x7fffff00u || d->in_width > 0x7fffff00u || d->out_width > 0x7fffff00u ||
+        (d->weight_order != TB_WEIGHT_IN_OUT && d->weight_order != TB_WEIGHT_OUT_IN))
+        return false;
+    s->rows = d->rows;
+    s->experts = d->experts;
+    s->in = d->in_width;
+    s->out = d->out_width;
+    s->turned = d->weight_order == TB_WEIGHT_OUT_IN;
+    s->x_stride = d->in_stride ? d->in_stride : s->in;
+    s->dx_stride = d->din_stride ? d->din_stride : s->in;
+    s->y_stride = d->out_stride ? d->out_stride : s->out;
+    const size_t w_width = s->turned ? s->in : s->out, w_rows = s->turned ? s->out : s->in;
+    s->w_row = d->weight_row_stride ? d->weight_row_stride : w_width;
+    size_t all;
+    if (s->w_row < w_width || !product(w_rows, s->w_row, SIZE_MAX / 64, &all)) return false;
+    s->w_matrix = d->weight_expert_stride ? d->weight_expert_stride : all;
+    s->wide = d->type == TB_TYPE_F32;
+    s->size = type_size(d->type);
+    return s->x_stride >= s->in && s->dx_stride >= s->in && s->y_stride >= s->out && s->w_matrix >= all &&
+           product(s->rows, s->x_stride, SIZE_MAX / 64, &all) && product(s->rows, s->dx_stride, SIZE_MAX / 64, &all) &&
+           product(s->rows, s->y_stride, SIZE_MAX / 64, &all) && product(s->experts, s->w_matrix, SIZE_MAX / 64, &all) &&
+           product(s->experts * ((s->in + 127) / 128), (s->out + 63) / 64, 0x7fffffffu, &all) &&
+           product((s->out + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all) &&
+           product((s->in + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all);
+}
+Source x_of(const ProductShape &s, const void *x) { return {x, s.in, s.rows, 1, s.x_stride, 0}; }
+Source y_of(const ProductShape &s, const void *y) { return {y, s.out, s.rows, 1, s.y_stride, 0}; }
+Source w_of(const ProductShape &s, const void *w) {
+    return {w, s.turned ? s.in : s.out, s.turned ? s.out : s.in, s.experts, s.w_row, s.w_matrix};
+}
+size_t laid_room(const Source &s, bool wide) { return laid_bytes(s.width, s.rows, s.count, wide, 2); }
+
+/* Columns of a tile of rows: twice the rows of an expert on average, so that
+ * most experts are one tile, but no more than 256. */
+template <class F> int with_columns(size_t rows, size_t experts, F &&f) {
+    const size_t average = rows / experts;
+    if (average <= 16) return f(std::integral_constant<int, 32>{});
+    if (average <= 32) return f(std::integral_constant<int, 64>{});
+    if (average <= 64) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+
+int kind_of(int type) { return type == TB_TYPE_F16 ? 0 : 1; }
+
+/* O [rows, width] of type T, from operands laid out. */
+template <class T>
+int rows_product(const Operands &base, const Matrices &w, bool w_outer, const Matrices &x, const Runs &runs, size_t width,
+                 size_t depth, void *out, size_t out_stride, int sms, cudaStream_t st) {
+    return with_columns(runs.rows, runs.experts, [&](auto n) {
+        constexpr int NT = decltype(n)::value;
+        Operands ops = base;
+        if (!encode(&ops, w, w_outer, x, false, NT)) return 0;
+        const int tiles_m = static_cast<int>((width + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
+        const RowJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(depth), tiles_m, static_cast<T *>(out), out_stride};
+        return tb_tensor::launch_products<RowJob<T, NT>, NT, false>(
+            ops, job, (static_cast<size_t>(runs.rows) / NT + runs.experts) * tiles_m, sms, st);
+    });
+}
+
+} /* namespace */
+
+extern "C" size_t tb_cuda_experts_product_workspace(const tb_expert_product_desc *desc) {
+    ProductShape s;
+    if (!product_shape(desc, &s)) return 0;
+    return laid_room(x_of(s, nullptr), s.wide) + laid_room(y_of(s, nullptr), s.wide) + laid_room(w_of(s, nullptr), s.wide);
+}
+
+extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc, const void *x, const void *weight,
+                                              const int32_t *offsets, void *y, void *workspace, void *stream) {
+    ProductShape s;
+    int device;
+    if (!product_shape(desc, &s) || !x || !weight || !y || !workspace || (!offsets && s.experts > 1)) return 0;
+    if (!aligned(x, s.size) || !aligned(weight, s.size) || !aligned(y, s.size) || !aligned(offsets, 4) ||
+        !aligned(workspace, 16) || collide({y, workspace}, {x, weight, offsets}))
+        return 0;
+    const int sms = multiprocessors(&device);
+    Operands ops{};
+    if (!sms || !(ops.status = tb_status_slot(stream))) return 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaGetLastError(); /* report these launches only */
+    ops.type = kind_of(desc->type);
+    pairs_of(&ops, s.wide, s.experts, 1);
+    const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        unsigned char *scratch = static_cast<unsigned char *>(workspace);
+        Matrices mw, mx;
+        return lay<T>(w_of(s, weight), 2, &scratch, &mw, st) && lay<T>(x_of(s, x), 2, &scratch, &mx, st) &&
+               rows_product<T>(ops, mw, !s.turned, mx, runs, s.out, s.in, y, s.y_stride, sms, st);
+    });
+}
+
+extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_desc *desc, const void *x,
+                                                       const void *weight, const int32_t *offsets, const void *dy,
+                                                       void *dx, void *dweight, void *workspace, void *stream) {
+    ProductShape s;
+    int device;
+    if (!product_shape(desc, &s) || (!x && dweight) || (!weight && dx) || !dy || (!dx && !dweight) || !workspace ||
+        (!offsets && s.experts > 1))
+        return 0;
+    if (!aligned(x, s.size) || !aligned(weight, s.size) || !aligned(dy, s.size) || !aligned(dx, s.size) ||
+        !aligned(dweight, s.size) || !aligned(offsets, 4) || !aligned(workspace, 16) ||
+        collide({dx, dweight, workspace}, {x, weight, offsets, dy}))
+        return 0;
+    const int sms = multiprocessors(&device);
+    Operands ops{};
+    if (!sms || !(ops.status = tb_status_slot(stream))) return 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaGetLastError(); /* report these launches only */
+    ops.type = kind_of(desc->type);
+    const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        unsigned char *scratch = static_cast<unsigned char *>(workspace);
+        Matrices mw, mx, my;
+        if (!lay<T>(y_of(s, dy), 2, &scratch, &my, st)) return 0;
+        if (dx) {
+            pairs_of(&ops, s.wide, s.experts, 1);
+            if (!lay<T>(w_of(s, weight), 2, &scratch, &mw, st) ||
+                !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, sms, st))
+                return 0;
+        }
+        if (!dweight) return 1;
+        if (!lay<T>(x_of(s, x), 2, &scratch, &mx, st)) return 0;
+        /* weights [in, out]: n counts in, m out; [out, in] the other way */
+        const size_t width = s.turned ? s.in : s.out, height = s.turned ? s.out : s.in;
+        pairs_of(&ops, s.wide, 1, 1);
+        constexpr int NT = 256;
+        if (!encode(&ops, s.turned ? mx : my, true, s.turned ? my : mx, true, NT)) return 0;
+        const int tiles_m = static_cast<int>((width + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
+        const int tiles_n = static_cast<int>((height + NT - 1) / NT);
+        const SumJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(height), tiles_m, tiles_n,
+                                static_cast<T *>(dweight), s.w_row, s.w_matrix};
+        return tb_tensor::launch_products<SumJob<T, NT>, NT, false>(ops, job, s.experts * tiles_m * tiles_n, sms, st);
+    });
+}
+
+/* ---- 8-bit integers ---- */
+
+namespace {
+
+constexpr int kQuantThreads = 256;
+
+/* A CTA a row: its largest magnitude, then its values.  A row whose largest
+ * magnitude has no finite reciprocal times 127 counts as zero; one with an
+ * infinity or a NaN gets the scale NaN. */
+template <class T, int PACK>
+__global__ void __launch_bounds__(kQuantThreads)
+quantise_rows(size_t width, size_t x_stride, size_t q_stride, const T *x, int8_t *q, float *scale) {
+    __shared__ float most[kQuantThreads / 32];
+    __shared__ int wrong[kQuantThreads / 32];
+    const size_t row = blockIdx.x;
+    const T *from = x + row * x_stride;
+    float m = 0.0f;
+    bool bad = false;
+    for (size_t c = threadIdx.x * PACK; c < width; c += kQuantThreads * PACK) {
+        float e[PACK];
+        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + c), e);
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) {
+            m = fmaxf(m, fabsf(e[i]));
+            bad |= !(fabsf(e[i]) <= 3.402823466e38f);
+        }
+    }
+    m = warp_max(m);
+    bad = __any_sync(0xffffffffu, bad);
+    if (threadIdx.x % 32 == 0) most[threadIdx.x / 32] = m, wrong[threadIdx.x / 32] = bad;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kQuantThreads / 32; ++i) m = fmaxf(m, most[i]), bad |= wrong[i] != 0;
+    float up = __fdiv_rn(127.0f, m);
+    const bool none = bad || !(up <= 3.402823466e38f);
+    if (none) up = 0.0f;
+    for (size_t c = threadIdx.x * PACK; c < width; c += kQuantThreads * PACK) {
+        float e[PACK];
+        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + c), e);
+        Pack<int8_t, PACK> out;
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) out.v[i] = none ? 0 : static_cast<int8_t>(__float2int_rn(e[i] * up));
+        *reinterpret_cast<Pack<int8_t, PACK> *>(q + row * q_stride + c) = out;
+    }
+    if (threadIdx.x == 0) scale[row] = bad ? __int_as_float(0x7fc00000) : none ? 0.0f : __fdiv_rn(m, 127.0f);
+}
+
+struct IntegerShape {
+    size_t rows, experts, in, out, x_stride, y_stride, w_row, w_matrix;
+};
+bool integer_shape(const tb_expert_product_i8_desc *d, IntegerShape *s) {
+    if (!d || !d->rows || !d->experts || !d->in_width || !d->out_width || !type_known(d->type) ||
+        d->experts > kMaxExperts || d->rows > 0x7fffff00u || d->in_width > TB_I8_MAX_WIDTH || d->out_width > 0x7fffff00u)
+        return false;
+    s->rows = d->rows;
+    s->experts = d->experts;
+    s->in = d->in_width;
+    s->out = d->out_width;
+    s->x_stride = d->in_stride ? d->in_stride : s->in;
+    s->y_stride = d->out_stride ? d->out_stride : s->out;
+    s->w_row = d->weight_row_stride ? d->weight_row_stride : s->in;
+    size_t all;
+    if (s->w_row < s->in || !product(s->out, s->w_row, SIZE_MAX / 64, &all)) return false;
+    s->w_matrix = d->weight_expert_stride ? d->weight_expert_stride : all;
+    return s->x_stride >= s->in && s->y_stride >= s->out && s->w_matrix >= all &&
+           product(s->rows, s->x_stride, SIZE_MAX / 64, &all) && product(s->rows, s->y_stride, SIZE_MAX / 64, &all) &&
+           product(s->experts, s->w_matrix, SIZE_MAX / 64, &all) &&
+           product((s->out + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all);
+}
+
+} /* namespace */
+
+extern "C" int tb_cuda_quantise_rows_device(const tb_quantise_desc *desc, const void *x, int8_t *q, float *scale,
+                                            void *stream) {
+    if (!desc || !desc->rows || !desc->width || !type_known(desc->type) || desc->rows > 0x7fffffffu || !x || !q || !scale)
+        return 0;
+    const size_t x_stride = desc->x_stride ? desc->x_stride : desc->width, q_stride = desc->q_stride ? desc->q_stride : desc->width;
+    const size_t size = type_size(desc->type);
+    size_t all;
+    if (x_stride < desc->width || q_stride < desc->width || !product(desc->rows, x_stride, SIZE_MAX / 64, &all) ||
+        !product(desc->rows, q_stride, SIZE_MAX / 64, &all) || !aligned(x, size) || !aligned(scale, 4) ||
+        collide({q, scale}, {x}))
+        return 0;
+    cudaGetLastError(); /* report this launch only */
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        /* a pack of x and the q that it becomes both start on their own size */
+        const size_t bits = reinterpret_cast<uintptr_t>(x) | (x_stride | desc->width) * size |
+                            (reinterpret_cast<uintptr_t>(q) | q_stride) * size;
+        return with_pack<T>(pack_of(bits, size), [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            quantise_rows<T, P><<<static_cast<unsigned>(desc->rows), kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                desc->width, x_stride, q_stride, static_cast<const T *>(x), q, scale);
+            return launched();
+        });
+    });
+}
+
+extern "C" size_t tb_cuda_experts_product_i8_workspace(const tb_expert_product_i8_desc *desc) {
+    IntegerShape s;
+    if (!integer_shape(desc, &s)) return 0;
+    return laid_bytes(s.in, s.rows, 1, false, 1) + laid_bytes(s.in, s.out, s.experts, false, 1);
+}
+
+extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc *desc, const int8_t *q,
+                                                 const float *q_scale, const int8_t *weight, const float *weight_scale,
+                                                 const int32_t *offsets, void *y, void *workspace, void *stream) {
+    IntegerShape s;
+    int device;
+    if (!integer_shape(desc, &s) || !q || !q_scale || !weight || !weight_scale || !y || !workspace || (!offsets && s.experts > 1))
+        return 0;
+    if (!aligned(q_scale, 4) || !aligned(weight_scale, 4) || !aligned(offsets, 4) || !aligned(y, type_size(desc->type)) ||
+        !aligned(workspace, 16) || collide({y, workspace}, {q, q_scale, weight, weight_scale, offsets}))
+        return 0;
+    const int sms = multiprocessors(&device);
+    Operands ops{};
+    if (!sms || !(ops.status = tb_status_slot(stream))) return 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaGetLastError(); /* report these launches only */
+    ops.type = 1;
+    pairs_of(&ops, false, s.experts, 1);
+    const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
+    unsigned char *scratch = static_cast<unsigned char *>(workspace);
+    Matrices mw, mx;
+    if (!lay<int8_t>({weight, s.in, s.out, s.experts, s.w_row, s.w_matrix}, 1, &scratch, &mw, st) ||
+        !lay<int8_t>({q, s.in, s.rows, 1, s.x_stride, 0}, 1, &scratch, &mx, st))
+        return 0;
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        return with_columns(s.rows, s.experts, [&](auto n) {
+            constexpr int NT = decltype(n)::value;
+            if (!encode(&ops, mw, false, mx, false, NT)) return 0;
+            const int tiles_m = static_cast<int>((s.out + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
+            IntegerJob<T, NT> job;
+            static_cast<RowJob<T, NT> &>(job) = RowJob<T, NT>{runs, static_cast<int>(s.out), static_cast<int>(s.in), tiles_m, static_cast<T *>(y), s.y_stride};
+            job.row_scale = q_scale;
+            job.channel_scale = weight_scale;
+            return tb_tensor::launch_products<IntegerJob<T, NT>, NT, true>(ops, job, (s.rows / NT + s.experts) * tiles_m, sms, st);
+        });
+    });
+}

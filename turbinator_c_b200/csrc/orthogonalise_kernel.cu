@@ -1,0 +1,329 @@
+/*
+ * Orthogonalising updates by Newton-Schulz products
+ * (include/turbinator/training/cuda_learner.h).
+ *
+ * x = g / (|g| + epsilon), then `steps` times S = b A + c A A with A = x x^T
+ * and x = a x + S x (for a matrix taller than wide A = x^T x and x = a x + x S:
+ * no transposes, the tensor cores take either order).  Three products a step,
+ * A and S symmetric, so that a little over half of their tiles are computed and
+ * the others mirrored.
+ *
+ * x, A and S are kept as pairs of f16 values, the second what the rounding of
+ * the first left, times 2^12: 22 bits for values about the size of a unit
+ * matrix's share and 2^-37 absolute below.  A product of pairs is three
+ * products of f16 (the fourth is below 2^-22); the polynomial multiplies an
+ * error in a direction of a small singular value by up to a^steps, 485 for five
+ * steps of the quintic, so that plain bf16 products leave errors of 2 to 3 % in
+ * the result and f16 ones 0.2 to 0.4 %, pairs 1e-6.
+ */
+#include "tb_tensor.cuh"
+
+using namespace tb_learn;
+using tb_tensor::Matrices;
+using tb_tensor::Operands;
+using tb_tensor::Tile;
+
+namespace {
+
+constexpr float kUp = 4096.0f; /* of every kept value */
+constexpr float kDown = 1.0f / 4096.0f;
+
+/* A stack of matrices as two planes: the second `plane` elements on. */
+struct Pair {
+    __half *at;
+    size_t line, matrix, plane;
+    __device__ __forceinline__ float get(size_t i) const { return __half2float(at[i]) + __half2float(at[plane + i]); }
+    __device__ __forceinline__ void put(size_t i, float v) const {
+        const __half high = __float2half_rn(v);
+        at[i] = high;
+        at[plane + i] = __float2half_rn(v - __half2float(high));
+    }
+};
+
+/* ---- x = g / (|g| + epsilon) ---- */
+
+constexpr int kNormThreads = 256;
+constexpr size_t kMostParts = 64;
+
+struct Given {
+    size_t rows, columns, matrix_stride, row_stride;
+};
+
+template <class T>
+__global__ void __launch_bounds__(kNormThreads) squares(Given d, size_t rows_a_part, const T *g, double *sums) {
+    __shared__ double parts[kNormThreads / 32];
+    const T *from = g + blockIdx.y * d.matrix_stride;
+    const size_t first = blockIdx.x * rows_a_part, last = min(first + rows_a_part, d.rows);
+    double s = 0.0;
+    for (size_t i = threadIdx.x; i < (last > first ? last - first : 0) * d.columns; i += kNormThreads) {
+        const size_t r = i / d.columns;
+        const double v = to_float(from[(first + r) * d.row_stride + i - r * d.columns]);
+        s += v * v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kNormThreads / 32; ++i) s += parts[i];
+        sums[blockIdx.y * gridDim.x + blockIdx.x] = s;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kNormThreads)
+normalise(Given d, size_t rows_a_part, const T *g, const double *sums, double epsilon, Pair x) {
+    __shared__ double scale;
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (unsigned i = 0; i < gridDim.x; ++i) s += sums[blockIdx.y * gridDim.x + i];
+        /* nothing stays nothing; a matrix with an infinity or a NaN becomes NaN */
+        scale = s == 0.0 ? 0.0 : isfinite(s) ? kUp / (sqrt(s) + epsilon) : s - s;
+    }
+    __syncthreads();
+    const double up = scale;
+    const T *from = g + blockIdx.y * d.matrix_stride;
+    const size_t first = blockIdx.x * rows_a_part, last = min(first + rows_a_part, d.rows);
+    for (size_t i = threadIdx.x; i < (last > first ? last - first : 0) * d.columns; i += kNormThreads) {
+        const size_t r = i / d.columns, c = i - r * d.columns;
+        x.put(blockIdx.y * x.matrix + (first + r) * x.line + c,
+              static_cast<float>(static_cast<double>(to_float(from[(first + r) * d.row_stride + c])) * up));
+    }
+}
+
+/* ---- the products ---- */
+
+/* Tiles of a matrix [height, width] of the output; symmetric: those that touch
+ * m >= n, each mirrored where the tile across the diagonal is not computed. */
+template <int NT> struct Plan {
+    int matrices, width, height, depth, tiles_m, tiles_n, per;
+    bool symmetric;
+    static constexpr int kWide = NT >= 128 ? NT / 128 : 1; /* tiles of m that one of n spans */
+
+    __host__ __device__ void count() {
+        tiles_m = (width + tb_tensor::kTileM - 1) / tb_tensor::kTileM;
+        tiles_n = (height + NT - 1) / NT;
+        per = 0;
+        for (int n = 0; n < tiles_n; ++n) per += symmetric ? tiles_m - n * kWide : tiles_m;
+    }
+    __device__ __forceinline__ Tile tile(int t) const {
+        const int z = t / per;
+        int in = t - z * per, n = 0, m;
+        if (symmetric) {
+            for (int row = tiles_m; in >= row; row -= kWide, ++n) in -= row;
+            m = n * kWide + in;
+        } else {
+            n = in / tiles_m;
+            m = in - n * tiles_m;
+        }
+        Tile r;
+        r.m0 = m * tb_tensor::kTileM;
+        r.n0 = n * NT;
+        r.columns = min(NT, height - r.n0);
+        r.k0 = 0;
+        r.depth = depth;
+        r.az = r.bz = r.which = z;
+        return r;
+    }
+    /* Whether the columns from c of a tile are to be mirrored. */
+    __device__ __forceinline__ bool mirrored(const Tile &t, int c) const {
+        return symmetric && (t.n0 + c) / tb_tensor::kTileM < t.m0 / NT * kWide;
+    }
+};
+
+struct Nothing {};
+
+/* A = x x^T, or S = b A + c A A. */
+template <int NT> struct SquareJob {
+    static constexpr bool kRagged = false;
+    using Shared = Nothing;
+    Plan<NT> plan;
+    Pair out, old; /* old.at NULL: A */
+    float b, c;
+    __device__ void setup(Shared &) const {}
+    __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
+    __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[32]) const {
+        if (m >= plan.width) return;
+        const size_t base = t.which * out.matrix;
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            v[i] = __uint_as_float(r[i]) * kDown;
+            if (c0 + i < t.columns) {
+                const size_t at = base + (t.n0 + c0 + i) * out.line + m;
+                if (old.at) v[i] = fmaf(c, v[i], b * old.get(at));
+                out.put(at, v[i]);
+            }
+        }
+        if (plan.mirrored(t, c0)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (c0 + i < t.columns) out.put(base + m * out.line + t.n0 + c0 + i, v[i]);
+        }
+    }
+};
+
+/* x = a x + S x; the last step's goes to the output. */
+template <class T, int NT> struct StepJob {
+    static constexpr bool kRagged = false;
+    using Shared = Nothing;
+    Plan<NT> plan;
+    Pair x, next;
+    T *last; /* or NULL */
+    size_t row_stride, matrix_stride;
+    float a, scale;
+    __device__ void setup(Shared &) const {}
+    __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
+    __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[32]) const {
+        if (m >= plan.width) return;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (c0 + i >= t.columns) continue;
+            const size_t n = t.n0 + c0 + i, at = t.which * x.matrix + n * x.line + m;
+            const float v = fmaf(a, x.get(at), __uint_as_float(r[i]) * kDown);
+            if (last) last[t.which * matrix_stride + n * row_stride + m] = from_float<T>(v * kDown * scale);
+            else next.put(at, v);
+        }
+    }
+};
+
+struct OrthogonalShape {
+    size_t matrices, rows, columns, small, in_matrix, in_row, out_matrix, out_row;
+    bool tall;
+};
+bool orthogonal_shape(const tb_orthogonalise_desc *d, OrthogonalShape *s) {
+    if (!d || !d->matrices || !d->rows || !d->columns || !type_known(d->type) || d->steps < 1 || d->steps > 64 ||
+        d->rows > TB_ORTHOGONALISE_MAX_SIDE || d->columns > TB_ORTHOGONALISE_MAX_SIDE || d->matrices > 65535 ||
+        !(d->epsilon >= 0.0f))
+        return false;
+    s->matrices = d->matrices;
+    s->rows = d->rows;
+    s->columns = d->columns;
+    s->tall = s->rows > s->columns;
+    s->small = s->tall ? s->columns : s->rows;
+    s->in_row = d->in_row_stride ? d->in_row_stride : s->columns;
+    s->out_row = d->out_row_stride ? d->out_row_stride : s->columns;
+    if (s->in_row < s->columns || s->out_row < s->columns) return false;
+    size_t in, out, all;
+    if (!product(s->rows, s->in_row, SIZE_MAX / 64, &in) || !product(s->rows, s->out_row, SIZE_MAX / 64, &out)) return false;
+    s->in_matrix = d->in_matrix_stride ? d->in_matrix_stride : in;
+    s->out_matrix = d->out_matrix_stride ? d->out_matrix_stride : out;
+    return s->in_matrix >= in && s->out_matrix >= out && product(s->matrices, s->in_matrix, SIZE_MAX / 64, &all) &&
+           product(s->matrices, s->out_matrix, SIZE_MAX / 64, &all) &&
+           product(s->matrices, ((s->rows + 31) / 32) * ((s->columns + 127) / 128), 0x7fffffffu, &all);
+}
+size_t line_of(size_t width) { return align_up(width, 8); }
+size_t pair_bytes(size_t matrices, size_t rows, size_t width) { return align_up(matrices * rows * line_of(width) * 4, 256); }
+size_t sums_bytes(size_t matrices) { return align_up(matrices * kMostParts * sizeof(double), 256); }
+
+Pair take_pair(unsigned char **scratch, size_t matrices, size_t rows, size_t width) {
+    const Pair p{reinterpret_cast<__half *>(*scratch), line_of(width), rows * line_of(width), matrices * rows * line_of(width)};
+    *scratch += pair_bytes(matrices, rows, width);
+    return p;
+}
+Matrices matrices_of(const Pair &p, size_t matrices, size_t rows, size_t width) {
+    return Matrices{p.at, width, rows, matrices * 2, p.line, p.matrix, 2};
+}
+
+/* Columns of a tile: 64 at least where the other operand's lie contiguous. */
+template <class F> int with_columns(size_t height, bool outer, F &&f) {
+    if (height <= 32 && !outer) return f(std::integral_constant<int, 32>{});
+    if (height <= 64) return f(std::integral_constant<int, 64>{});
+    if (height <= 128) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+
+} /* namespace */
+
+extern "C" size_t tb_cuda_orthogonalise_workspace(const tb_orthogonalise_desc *desc) {
+    OrthogonalShape s;
+    if (!orthogonal_shape(desc, &s)) return 0;
+    return sums_bytes(s.matrices) + 2 * pair_bytes(s.matrices, s.rows, s.columns) + 2 * pair_bytes(s.matrices, s.small, s.small);
+}
+
+extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, const void *g, void *out, void *workspace,
+                                            void *stream) {
+    OrthogonalShape s;
+    int device;
+    if (!orthogonal_shape(desc, &s) || !g || !out || !workspace) return 0;
+    const size_t size = type_size(desc->type);
+    if (!aligned(g, size) || !aligned(out, size) || !aligned(workspace, 16) || workspace == g || workspace == out ||
+        (g == out && (s.in_row != s.out_row || s.in_matrix != s.out_matrix)))
+        return 0;
+    const int sms = multiprocessors(&device);
+    Operands ops{};
+    if (!sms || !(ops.status = tb_status_slot(stream))) return 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaGetLastError(); /* report these launches only */
+    unsigned char *scratch = static_cast<unsigned char *>(workspace);
+    double *sums = reinterpret_cast<double *>(scratch);
+    scratch += sums_bytes(s.matrices);
+    Pair x = take_pair(&scratch, s.matrices, s.rows, s.columns), next = take_pair(&scratch, s.matrices, s.rows, s.columns);
+    const Pair square = take_pair(&scratch, s.matrices, s.small, s.small), poly = take_pair(&scratch, s.matrices, s.small, s.small);
+    ops.type = 0;
+    ops.pairs = 3; /* low and high, high and low, high and high */
+    ops.a_plane[0] = ops.b_plane[1] = static_cast<int>(s.matrices);
+    return with_type(desc->type, [&](auto t) {
+        using T = decltype(t);
+        const Given given{s.rows, s.columns, s.in_matrix, s.in_row};
+        size_t parts = (s.rows * s.columns + 16383) / 16384;
+        if (parts > kMostParts) parts = kMostParts;
+        const size_t rows_a_part = (s.rows + parts - 1) / parts;
+        const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(s.matrices));
+        squares<T><<<grid, kNormThreads, 0, st>>>(given, rows_a_part, static_cast<const T *>(g), sums);
+        if (!launched()) return 0;
+        normalise<T><<<grid, kNormThreads, 0, st>>>(given, rows_a_part, static_cast<const T *>(g), sums, desc->epsilon, x);
+        if (!launched()) return 0;
+        const int z = static_cast<int>(s.matrices), small = static_cast<int>(s.small);
+        const int wide = static_cast<int>(s.columns), high = static_cast<int>(s.rows);
+        for (int step = 0; step < desc->steps; ++step) {
+            const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns);
+            const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
+            const int squared = with_columns(s.small, s.tall, [&](auto n) {
+                constexpr int NT = decltype(n)::value;
+                SquareJob<NT> job{};
+                job.plan = Plan<NT>{z, small, small, s.tall ? high : wide, 0, 0, 0, small > tb_tensor::kTileM};
+                job.plan.count();
+                job.out = square;
+                const size_t tiles = static_cast<size_t>(z) * job.plan.per;
+                if (!encode(&ops, mx, s.tall, mx, s.tall, NT) ||
+                    !tb_tensor::launch_products<SquareJob<NT>, NT, false>(ops, job, tiles, sms, st))
+                    return 0;
+                job.plan.depth = small;
+                job.out = poly;
+                job.old = square;
+                job.b = desc->b;
+                job.c = desc->c;
+                return encode(&ops, ma, false, ma, false, NT) &&
+                               tb_tensor::launch_products<SquareJob<NT>, NT, false>(ops, job, tiles, sms, st)
+                           ? 1 : 0;
+            });
+            if (!squared) return 0;
+            const int stepped = with_columns(s.rows, false, [&](auto n) {
+                constexpr int NT = decltype(n)::value;
+                StepJob<T, NT> job{};
+                job.plan = Plan<NT>{z, wide, high, small, 0, 0, 0, false};
+                job.plan.count();
+                job.x = x;
+                job.next = next;
+                job.last = step + 1 == desc->steps ? static_cast<T *>(out) : nullptr;
+                job.row_stride = s.out_row;
+                job.matrix_stride = s.out_matrix;
+                job.a = desc->a;
+                job.scale = desc->scale;
+                const size_t tiles = static_cast<size_t>(z) * job.plan.per;
+                /* x S: A is S (its own transpose), B is x; S x: A is x with its columns as m, B is S */
+                return (s.tall ? encode(&ops, mp, false, mx, false, NT) : encode(&ops, mx, true, mp, false, NT)) &&
+                               tb_tensor::launch_products<StepJob<T, NT>, NT, false>(ops, job, tiles, sms, st)
+                           ? 1 : 0;
+            });
+            if (!stepped) return 0;
+            const Pair swap = x;
+            x = next;
+            next = swap;
+        }
+        return 1;
+    });
+}

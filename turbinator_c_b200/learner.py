@@ -1,8 +1,9 @@
 """Learner layers -- Python view of ``include/turbinator/training/cuda_learner.h``.
 
-Group norm with an activation, the gated linear recurrence, routing to experts
-and the experts' combine, each forward and backward, under the names of the C
-functions.  A descriptor is made once and kept; the calls take device tensors
+Group norm with an activation, the gated linear recurrence, routing to experts,
+handing tokens out to them, the experts' products and their combine, each
+forward and backward, the products in 8-bit integers and the orthogonalised
+update, under the names of the C functions.  A descriptor is made once and kept; the calls take device tensors
 (or pointers), run on ``stream`` and return 1, or 0 on a rejected argument or a
 launch error, like the other device entry points.  The caller owns outputs and
 workspaces; nothing is allocated here.
@@ -18,6 +19,7 @@ _address = _c.addressof
 TB_TYPE_F32, TB_TYPE_BF16, TB_TYPE_F16 = range(3)
 TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU, TB_ACT_GELU = range(4)
 TB_SCORE_SOFTMAX, TB_SCORE_SIGMOID = range(2)
+TB_WEIGHT_IN_OUT, TB_WEIGHT_OUT_IN = range(2)
 
 #: Steps between two saved states of the recurrence (TB_RECURRENCE_CHECKPOINT).
 RECURRENCE_CHECKPOINT = 16
@@ -69,6 +71,37 @@ class ExpertCombineDesc(_Desc):
 
     _fields_ = [(n, _c.c_size_t) for n in ("tokens", "rows", "width", "rows_stride", "out_stride")] + [
         ("top_k", _c.c_int), ("type", _c.c_int)]
+
+
+class ExpertProductDesc(_Desc):
+    """Mirror of ``tb_expert_product_desc``."""
+
+    _fields_ = [(n, _c.c_size_t) for n in
+                ("rows", "experts", "in_width", "out_width", "in_stride", "din_stride", "out_stride",
+                 "weight_expert_stride", "weight_row_stride")] + [("weight_order", _c.c_int), ("type", _c.c_int)]
+
+
+class QuantiseDesc(_Desc):
+    """Mirror of ``tb_quantise_desc``."""
+
+    _fields_ = [(n, _c.c_size_t) for n in ("rows", "width", "x_stride", "q_stride")] + [("type", _c.c_int)]
+
+
+class ExpertProductI8Desc(_Desc):
+    """Mirror of ``tb_expert_product_i8_desc``."""
+
+    _fields_ = [(n, _c.c_size_t) for n in
+                ("rows", "experts", "in_width", "out_width", "in_stride", "out_stride", "weight_expert_stride",
+                 "weight_row_stride")] + [("type", _c.c_int)]
+
+
+class OrthogonaliseDesc(_Desc):
+    """Mirror of ``tb_orthogonalise_desc``."""
+
+    _fields_ = [(n, _c.c_size_t) for n in
+                ("matrices", "rows", "columns", "in_matrix_stride", "in_row_stride", "out_matrix_stride",
+                 "out_row_stride")] + [("type", _c.c_int), ("steps", _c.c_int)] + [
+        (n, _c.c_float) for n in ("a", "b", "c", "epsilon", "scale")]
 
 
 def tb_cuda_group_norm_workspace(desc: GroupNormDesc) -> int:
@@ -134,3 +167,56 @@ def tb_cuda_combine_experts_backward_device(desc: ExpertCombineDesc, rows, posit
     return load_library().tb_cuda_combine_experts_backward_device(
         _address(desc), _ptr(rows), _ptr(position), _ptr(weights), _ptr(dout), _ptr(drows), _ptr(dweights),
         _stream_handle(stream))
+
+
+def tb_cuda_hand_out_experts_device(desc: ExpertCombineDesc, x, order, weights, rows, stream=None) -> int:
+    return load_library().tb_cuda_hand_out_experts_device(
+        _address(desc), _ptr(x), _ptr(order), _ptr(weights), _ptr(rows), _stream_handle(stream))
+
+
+def tb_cuda_hand_out_experts_backward_device(desc: ExpertCombineDesc, x, position, weights, drows, dx, dweights,
+                                             stream=None) -> int:
+    return load_library().tb_cuda_hand_out_experts_backward_device(
+        _address(desc), _ptr(x), _ptr(position), _ptr(weights), _ptr(drows), _ptr(dx), _ptr(dweights),
+        _stream_handle(stream))
+
+
+def tb_cuda_experts_product_workspace(desc: ExpertProductDesc) -> int:
+    return load_library().tb_cuda_experts_product_workspace(_address(desc))
+
+
+def tb_cuda_experts_product_device(desc: ExpertProductDesc, x, weight, offsets, y, workspace, stream=None) -> int:
+    return load_library().tb_cuda_experts_product_device(
+        _address(desc), _ptr(x), _ptr(weight), _ptr(offsets), _ptr(y), _ptr(workspace), _stream_handle(stream))
+
+
+def tb_cuda_experts_product_backward_device(desc: ExpertProductDesc, x, weight, offsets, dy, dx, dweight, workspace,
+                                            stream=None) -> int:
+    return load_library().tb_cuda_experts_product_backward_device(
+        _address(desc), _ptr(x), _ptr(weight), _ptr(offsets), _ptr(dy), _ptr(dx), _ptr(dweight), _ptr(workspace),
+        _stream_handle(stream))
+
+
+def tb_cuda_quantise_rows_device(desc: QuantiseDesc, x, q, scale, stream=None) -> int:
+    return load_library().tb_cuda_quantise_rows_device(
+        _address(desc), _ptr(x), _ptr(q), _ptr(scale), _stream_handle(stream))
+
+
+def tb_cuda_experts_product_i8_workspace(desc: ExpertProductI8Desc) -> int:
+    return load_library().tb_cuda_experts_product_i8_workspace(_address(desc))
+
+
+def tb_cuda_experts_product_i8_device(desc: ExpertProductI8Desc, q, q_scale, weight, weight_scale, offsets, y, workspace,
+                                      stream=None) -> int:
+    return load_library().tb_cuda_experts_product_i8_device(
+        _address(desc), _ptr(q), _ptr(q_scale), _ptr(weight), _ptr(weight_scale), _ptr(offsets), _ptr(y),
+        _ptr(workspace), _stream_handle(stream))
+
+
+def tb_cuda_orthogonalise_workspace(desc: OrthogonaliseDesc) -> int:
+    return load_library().tb_cuda_orthogonalise_workspace(_address(desc))
+
+
+def tb_cuda_orthogonalise_device(desc: OrthogonaliseDesc, g, out, workspace, stream=None) -> int:
+    return load_library().tb_cuda_orthogonalise_device(
+        _address(desc), _ptr(g), _ptr(out), _ptr(workspace), _stream_handle(stream))
