@@ -276,9 +276,9 @@ int tb_cuda_experts_product_backward_device(const tb_expert_product_desc *desc, 
 /* ---- The same in 8-bit integers, for acting ---- */
 
 /* rows < 2^31.  Each row of x [rows, width] in 8-bit integers with its scale:
- *   m = max |x|,  q = x (127 / m) in f32, rounded to nearest even,  scale = m / 127
- * A row whose 127 / m passes f32's range (m < 2^-121, or 0) has q = 0 and scale
- * 0; one with an infinity or a NaN q = 0 and scale NaN, so that its products are
+ *   m = max |x|,  q = x ((1/m) 127) rounded to nearest even,  scale = m / 127
+ * every operation rounded in f32.  A row whose (1/m) 127 passes f32's range (m <
+ * 2^-121, or 0) has q = 0 and scale 0; one with an infinity or a NaN q = 0 and scale NaN, so that its products are
  * NaN.  Weights [experts, out, in] are quantised by the same call, a row per
  * output channel. */
 typedef struct tb_quantise_desc {

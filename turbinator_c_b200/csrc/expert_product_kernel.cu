@@ -16,6 +16,8 @@
  * is below 2^-24 of the factors.  Rows that do not start on 16 bytes are laid
  * out anew too, in the workspace.
  */
+#include <algorithm>
+
 #include "tb_tensor.cuh"
 
 using namespace tb_learn;
@@ -50,7 +52,7 @@ template <class T, int NT> struct RowJob {
         int start[kMaxExperts], end[kMaxExperts];
     };
     Runs runs;
-    int width, depth, tiles_m;
+    int width, depth, tile_m, tiles_m;
     T *out;
     size_t out_stride;
 
@@ -86,7 +88,7 @@ template <class T, int NT> struct RowJob {
             else high = mid;
         }
         Tile r;
-        r.m0 = (t - of * tiles_m) * tb_tensor::kTileM;
+        r.m0 = (t - of * tiles_m) * tile_m;
         r.n0 = s.start[low] + (of - s.first[low]) * NT;
         r.columns = min(NT, s.end[low] - r.n0);
         r.k0 = 0;
@@ -126,7 +128,7 @@ template <class T, int NT> struct SumJob {
     static constexpr bool kRagged = true;
     struct Shared {};
     Runs runs;
-    int width, height, tiles_m, tiles_n;
+    int width, height, tile_m, tiles_m, tiles_n;
     T *out;
     size_t row_stride, matrix_stride;
 
@@ -135,7 +137,7 @@ template <class T, int NT> struct SumJob {
     __device__ Tile tile(const Shared &, int t) const {
         const int per = tiles_m * tiles_n, e = t / per, in = t - e * per, tn = in / tiles_m;
         Tile r;
-        r.m0 = (in - tn * tiles_m) * tb_tensor::kTileM;
+        r.m0 = (in - tn * tiles_m) * tile_m;
         r.n0 = tn * NT;
         r.columns = min(NT, height - r.n0);
         r.k0 = run_start(runs, e);
@@ -219,16 +221,6 @@ template <class T> int lay(const Source &s, size_t size, unsigned char **scratch
     return 1;
 }
 
-/* The planes' pairs: all of the value, or six of three by three. */
-void pairs_of(Operands *ops, bool wide, size_t a_count, size_t b_count) {
-    static const int a[6] = {2, 0, 1, 1, 0, 0}, b[6] = {0, 2, 1, 0, 1, 0};
-    ops->pairs = wide ? 6 : 1;
-    for (int i = 0; i < ops->pairs; ++i) {
-        ops->a_plane[i] = wide ? a[i] * static_cast<int>(a_count) : 0;
-        ops->b_plane[i] = wide ? b[i] * static_cast<int>(b_count) : 0;
-    }
-}
-
 /* ---- shapes ---- */
 
 struct ProductShape {
@@ -272,29 +264,36 @@ Source w_of(const ProductShape &s, const void *w) {
 }
 size_t laid_room(const Source &s, bool wide) { return laid_bytes(s.width, s.rows, s.count, wide, 2); }
 
-/* Columns of a tile of rows: twice the rows of an expert on average, so that
- * most experts are one tile, but no more than 256. */
-template <class F> int with_columns(size_t rows, size_t experts, F &&f) {
-    const size_t average = rows / experts;
-    if (average <= 16) return f(std::integral_constant<int, 32>{});
-    if (average <= 32) return f(std::integral_constant<int, 64>{});
-    if (average <= 64) return f(std::integral_constant<int, 128>{});
-    return f(std::integral_constant<int, 256>{});
+/* Calls f with a tile's columns and whether two CTAs share it: twice the rows
+ * of an expert on average, so that most experts are one tile, but no more than
+ * 256; pairs where a tile of 256 x 256 has most of its m and n; a lone CTA's
+ * three planes are too large for 256 columns. */
+template <int PLANES, class F> int with_tile(size_t width, size_t rows, F &&f) {
+    if (rows <= 16) return f(std::integral_constant<int, 32>{}, std::false_type{});
+    if (rows <= 32) return f(std::integral_constant<int, 64>{}, std::false_type{});
+    if (rows > 64 && width > tb_tensor::kRows) return f(std::integral_constant<int, 256>{}, std::true_type{});
+    if (rows <= 64 || PLANES == 3) return f(std::integral_constant<int, 128>{}, std::false_type{});
+    return f(std::integral_constant<int, PLANES == 3 ? 128 : 256>{}, std::false_type{});
 }
 
 int kind_of(int type) { return type == TB_TYPE_F16 ? 0 : 1; }
+int tiles_of(size_t width, int tile) { return static_cast<int>((width + tile - 1) / tile); }
 
 /* O [rows, width] of type T, from operands laid out. */
 template <class T>
-int rows_product(const Operands &base, const Matrices &w, bool w_outer, const Matrices &x, const Runs &runs, size_t width,
+int rows_product(Operands ops, const Matrices &w, bool w_outer, const Matrices &x, const Runs &runs, size_t width,
                  size_t depth, void *out, size_t out_stride, int sms, cudaStream_t st) {
-    return with_columns(runs.rows, runs.experts, [&](auto n) {
+    constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    return with_tile<PLANES>(width, runs.rows / runs.experts, [&](auto n, auto pair) {
         constexpr int NT = decltype(n)::value;
-        Operands ops = base;
-        if (!encode(&ops, w, w_outer, x, false, NT)) return 0;
-        const int tiles_m = static_cast<int>((width + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
-        const RowJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(depth), tiles_m, static_cast<T *>(out), out_stride};
-        return tb_tensor::launch_products<RowJob<T, NT>, NT, false>(
+        constexpr bool PAIR = decltype(pair)::value;
+        constexpr int TM = tb_tensor::Shape<NT, PLANES, PAIR>::kTileM;
+        if (!tb_tensor::encode<NT, PAIR>(&ops, w, w_outer, x, false)) return 0;
+        ops.a_plane = runs.experts;
+        ops.b_plane = 1;
+        const int tiles_m = tiles_of(width, TM);
+        const RowJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(depth), TM, tiles_m, static_cast<T *>(out), out_stride};
+        return tb_tensor::launch_products<NT, PLANES, false, PAIR>(
             ops, job, (static_cast<size_t>(runs.rows) / NT + runs.experts) * tiles_m, sms, st);
     });
 }
@@ -321,7 +320,6 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaGetLastError(); /* report these launches only */
     ops.type = kind_of(desc->type);
-    pairs_of(&ops, s.wide, s.experts, 1);
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
@@ -357,7 +355,6 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
         Matrices mw, mx, my;
         if (!lay<T>(y_of(s, dy), 2, &scratch, &my, st)) return 0;
         if (dx) {
-            pairs_of(&ops, s.wide, s.experts, 1);
             if (!lay<T>(w_of(s, weight), 2, &scratch, &mw, st) ||
                 !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, sms, st))
                 return 0;
@@ -366,14 +363,18 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
         if (!lay<T>(x_of(s, x), 2, &scratch, &mx, st)) return 0;
         /* weights [in, out]: n counts in, m out; [out, in] the other way */
         const size_t width = s.turned ? s.in : s.out, height = s.turned ? s.out : s.in;
-        pairs_of(&ops, s.wide, 1, 1);
-        constexpr int NT = 256;
-        if (!encode(&ops, s.turned ? mx : my, true, s.turned ? my : mx, true, NT)) return 0;
-        const int tiles_m = static_cast<int>((width + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
-        const int tiles_n = static_cast<int>((height + NT - 1) / NT);
-        const SumJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(height), tiles_m, tiles_n,
-                                static_cast<T *>(dweight), s.w_row, s.w_matrix};
-        return tb_tensor::launch_products<SumJob<T, NT>, NT, false>(ops, job, s.experts * tiles_m * tiles_n, sms, st);
+        constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+        return with_tile<PLANES>(width, std::max<size_t>(height, 33), [&](auto n, auto pair) { /* n contiguous: 64 columns at least */
+            constexpr int NT = decltype(n)::value;
+            constexpr bool PAIR = decltype(pair)::value;
+            constexpr int TM = tb_tensor::Shape<NT, PLANES, PAIR>::kTileM;
+            if (!tb_tensor::encode<NT, PAIR>(&ops, s.turned ? mx : my, true, s.turned ? my : mx, true)) return 0;
+            ops.a_plane = ops.b_plane = 1;
+            const int tiles_m = tiles_of(width, TM), tiles_n = tiles_of(height, NT);
+            const SumJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(height), TM, tiles_m, tiles_n,
+                                    static_cast<T *>(dweight), s.w_row, s.w_matrix};
+            return tb_tensor::launch_products<NT, PLANES, false, PAIR>(ops, job, s.experts * tiles_m * tiles_n, sms, st);
+        });
     });
 }
 
@@ -410,7 +411,7 @@ quantise_rows(size_t width, size_t x_stride, size_t q_stride, const T *x, int8_t
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kQuantThreads / 32; ++i) m = fmaxf(m, most[i]), bad |= wrong[i] != 0;
-    float up = __fdiv_rn(127.0f, m);
+    float up = __fmul_rn(__frcp_rn(m), 127.0f);
     const bool none = bad || !(up <= 3.402823466e38f);
     if (none) up = 0.0f;
     for (size_t c = threadIdx.x * PACK; c < width; c += kQuantThreads * PACK) {
@@ -497,7 +498,6 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaGetLastError(); /* report these launches only */
     ops.type = 1;
-    pairs_of(&ops, false, s.experts, 1);
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     unsigned char *scratch = static_cast<unsigned char *>(workspace);
     Matrices mw, mx;
@@ -506,15 +506,18 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
         return 0;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return with_columns(s.rows, s.experts, [&](auto n) {
+        return with_tile<1>(s.out, s.rows / s.experts, [&](auto n, auto pair) {
             constexpr int NT = decltype(n)::value;
-            if (!encode(&ops, mw, false, mx, false, NT)) return 0;
-            const int tiles_m = static_cast<int>((s.out + tb_tensor::kTileM - 1) / tb_tensor::kTileM);
+            constexpr bool PAIR = decltype(pair)::value;
+            constexpr int TM = tb_tensor::Shape<NT, 1, PAIR>::kTileM;
+            if (!tb_tensor::encode<NT, PAIR>(&ops, mw, false, mx, false)) return 0;
+            const int tiles_m = tiles_of(s.out, TM);
             IntegerJob<T, NT> job;
-            static_cast<RowJob<T, NT> &>(job) = RowJob<T, NT>{runs, static_cast<int>(s.out), static_cast<int>(s.in), tiles_m, static_cast<T *>(y), s.y_stride};
+            static_cast<RowJob<T, NT> &>(job) = RowJob<T, NT>{runs, static_cast<int>(s.out), static_cast<int>(s.in), TM,
+                                                              tiles_m, static_cast<T *>(y), s.y_stride};
             job.row_scale = q_scale;
             job.channel_scale = weight_scale;
-            return tb_tensor::launch_products<IntegerJob<T, NT>, NT, true>(ops, job, (s.rows / NT + s.experts) * tiles_m, sms, st);
+            return tb_tensor::launch_products<NT, 1, true, PAIR>(ops, job, (s.rows / NT + s.experts) * tiles_m, sms, st);
         });
     });
 }

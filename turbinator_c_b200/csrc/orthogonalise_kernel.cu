@@ -95,49 +95,49 @@ normalise(Given d, size_t rows_a_part, const T *g, const double *sums, double ep
 
 /* Tiles of a matrix [height, width] of the output; symmetric: those that touch
  * m >= n, each mirrored where the tile across the diagonal is not computed. */
-template <int NT> struct Plan {
-    int matrices, width, height, depth, tiles_m, tiles_n, per;
+struct Plan {
+    int matrices, width, height, depth, tile_m, tile_n; /* symmetric: tiles of 128 or 256 */
     bool symmetric;
-    static constexpr int kWide = NT >= 128 ? NT / 128 : 1; /* tiles of m that one of n spans */
+    int tiles_m, per;
 
-    __host__ __device__ void count() {
-        tiles_m = (width + tb_tensor::kTileM - 1) / tb_tensor::kTileM;
-        tiles_n = (height + NT - 1) / NT;
+    __host__ __device__ int first(int n) const { return symmetric ? n * tile_n / tile_m : 0; }
+    void count() {
+        tiles_m = (width + tile_m - 1) / tile_m;
         per = 0;
-        for (int n = 0; n < tiles_n; ++n) per += symmetric ? tiles_m - n * kWide : tiles_m;
+        for (int n = 0; n * tile_n < height; ++n) per += tiles_m - first(n);
     }
     __device__ __forceinline__ Tile tile(int t) const {
         const int z = t / per;
         int in = t - z * per, n = 0, m;
         if (symmetric) {
-            for (int row = tiles_m; in >= row; row -= kWide, ++n) in -= row;
-            m = n * kWide + in;
+            for (; in >= tiles_m - first(n); ++n) in -= tiles_m - first(n);
+            m = first(n) + in;
         } else {
             n = in / tiles_m;
             m = in - n * tiles_m;
         }
         Tile r;
-        r.m0 = m * tb_tensor::kTileM;
-        r.n0 = n * NT;
-        r.columns = min(NT, height - r.n0);
+        r.m0 = m * tile_m;
+        r.n0 = n * tile_n;
+        r.columns = min(tile_n, height - r.n0);
         r.k0 = 0;
         r.depth = depth;
         r.az = r.bz = r.which = z;
         return r;
     }
-    /* Whether the columns from c of a tile are to be mirrored. */
-    __device__ __forceinline__ bool mirrored(const Tile &t, int c) const {
-        return symmetric && (t.n0 + c) / tb_tensor::kTileM < t.m0 / NT * kWide;
+    /* Whether what lies across the diagonal from row m of the columns from c (32 of them) is in no tile. */
+    __device__ __forceinline__ bool mirrored(const Tile &t, int m, int c) const {
+        return symmetric && (t.n0 + c) / tile_m < first(m / tile_n);
     }
 };
 
 struct Nothing {};
 
 /* A = x x^T, or S = b A + c A A. */
-template <int NT> struct SquareJob {
+struct SquareJob {
     static constexpr bool kRagged = false;
     using Shared = Nothing;
-    Plan<NT> plan;
+    Plan plan;
     Pair out, old; /* old.at NULL: A */
     float b, c;
     __device__ void setup(Shared &) const {}
@@ -156,19 +156,29 @@ template <int NT> struct SquareJob {
                 out.put(at, v[i]);
             }
         }
-        if (plan.mirrored(t, c0)) {
+        if (plan.mirrored(t, m, c0)) { /* 16 bytes at a time; a line's end is a multiple of eight */
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (c0 + i < t.columns) out.put(base + m * out.line + t.n0 + c0 + i, v[i]);
+            for (int i = 0; i < 32; i += 8) {
+                if (c0 + i >= t.columns) break;
+                float high[8], low[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    high[j] = __half2float(__float2half_rn(v[i + j]));
+                    low[j] = v[i + j] - high[j];
+                }
+                const size_t at = base + m * out.line + t.n0 + c0 + i;
+                *reinterpret_cast<Held<__half, 8> *>(out.at + at) = packed<__half, 8>(high);
+                *reinterpret_cast<Held<__half, 8> *>(out.at + out.plane + at) = packed<__half, 8>(low);
+            }
         }
     }
 };
 
 /* x = a x + S x; the last step's goes to the output. */
-template <class T, int NT> struct StepJob {
+template <class T> struct StepJob {
     static constexpr bool kRagged = false;
     using Shared = Nothing;
-    Plan<NT> plan;
+    Plan plan;
     Pair x, next;
     T *last; /* or NULL */
     size_t row_stride, matrix_stride;
@@ -227,12 +237,13 @@ Matrices matrices_of(const Pair &p, size_t matrices, size_t rows, size_t width) 
     return Matrices{p.at, width, rows, matrices * 2, p.line, p.matrix, 2};
 }
 
-/* Columns of a tile: 64 at least where the other operand's lie contiguous. */
-template <class F> int with_columns(size_t height, bool outer, F &&f) {
-    if (height <= 32 && !outer) return f(std::integral_constant<int, 32>{});
-    if (height <= 64) return f(std::integral_constant<int, 64>{});
-    if (height <= 128) return f(std::integral_constant<int, 128>{});
-    return f(std::integral_constant<int, 256>{});
+/* Calls f with a tile's columns and whether two CTAs share it; 64 columns at
+ * least where the other operand's lie contiguous. */
+template <class F> int with_tile(size_t height, size_t width, bool outer, F &&f) {
+    if (height <= 32 && !outer) return f(std::integral_constant<int, 32>{}, std::false_type{});
+    if (height <= 64) return f(std::integral_constant<int, 64>{}, std::false_type{});
+    if (height <= 128 || width <= tb_tensor::kRows) return f(std::integral_constant<int, 128>{}, std::false_type{});
+    return f(std::integral_constant<int, 256>{}, std::true_type{});
 }
 
 } /* namespace */
@@ -263,8 +274,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
     Pair x = take_pair(&scratch, s.matrices, s.rows, s.columns), next = take_pair(&scratch, s.matrices, s.rows, s.columns);
     const Pair square = take_pair(&scratch, s.matrices, s.small, s.small), poly = take_pair(&scratch, s.matrices, s.small, s.small);
     ops.type = 0;
-    ops.pairs = 3; /* low and high, high and low, high and high */
-    ops.a_plane[0] = ops.b_plane[1] = static_cast<int>(s.matrices);
+    ops.a_plane = ops.b_plane = static_cast<int>(s.matrices);
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
         const Given given{s.rows, s.columns, s.in_matrix, s.in_row};
@@ -281,30 +291,32 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         for (int step = 0; step < desc->steps; ++step) {
             const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
-            const int squared = with_columns(s.small, s.tall, [&](auto n) {
+            const int squared = with_tile(s.small, s.small, s.tall, [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
-                SquareJob<NT> job{};
-                job.plan = Plan<NT>{z, small, small, s.tall ? high : wide, 0, 0, 0, small > tb_tensor::kTileM};
+                constexpr bool PAIR = decltype(pair)::value;
+                SquareJob job{};
+                job.plan = Plan{z, small, small, s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, small > tb_tensor::kRows};
                 job.plan.count();
                 job.out = square;
                 const size_t tiles = static_cast<size_t>(z) * job.plan.per;
-                if (!encode(&ops, mx, s.tall, mx, s.tall, NT) ||
-                    !tb_tensor::launch_products<SquareJob<NT>, NT, false>(ops, job, tiles, sms, st))
+                if (!tb_tensor::encode<NT, PAIR>(&ops, mx, s.tall, mx, s.tall) ||
+                    !tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st))
                     return 0;
                 job.plan.depth = small;
                 job.out = poly;
                 job.old = square;
                 job.b = desc->b;
                 job.c = desc->c;
-                return encode(&ops, ma, false, ma, false, NT) &&
-                               tb_tensor::launch_products<SquareJob<NT>, NT, false>(ops, job, tiles, sms, st)
+                return tb_tensor::encode<NT, PAIR>(&ops, ma, false, ma, false) &&
+                               tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
                            ? 1 : 0;
             });
             if (!squared) return 0;
-            const int stepped = with_columns(s.rows, false, [&](auto n) {
+            const int stepped = with_tile(s.rows, s.columns, false, [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
-                StepJob<T, NT> job{};
-                job.plan = Plan<NT>{z, wide, high, small, 0, 0, 0, false};
+                constexpr bool PAIR = decltype(pair)::value;
+                StepJob<T> job{};
+                job.plan = Plan{z, wide, high, small, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, false};
                 job.plan.count();
                 job.x = x;
                 job.next = next;
@@ -315,8 +327,9 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                 job.scale = desc->scale;
                 const size_t tiles = static_cast<size_t>(z) * job.plan.per;
                 /* x S: A is S (its own transpose), B is x; S x: A is x with its columns as m, B is S */
-                return (s.tall ? encode(&ops, mp, false, mx, false, NT) : encode(&ops, mx, true, mp, false, NT)) &&
-                               tb_tensor::launch_products<StepJob<T, NT>, NT, false>(ops, job, tiles, sms, st)
+                return (s.tall ? tb_tensor::encode<NT, PAIR>(&ops, mp, false, mx, false)
+                               : tb_tensor::encode<NT, PAIR>(&ops, mx, true, mp, false)) &&
+                               tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
                            ? 1 : 0;
             });
             if (!stepped) return 0;

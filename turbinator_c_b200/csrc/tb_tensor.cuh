@@ -10,15 +10,25 @@
  * columns, to the next 16, as it has.  Either operand may lie with k
  * contiguous or with m (n) contiguous; the tensor cores take both.
  *
- * A CTA of six warps: one asks for the copies, one issues the products, four
+ * A CTA of ten warps: one asks for the copies, one issues the products, eight
  * read the accumulators.  A ring of 128-byte-deep stages (64 values of 16 bits,
  * 128 of 8) feeds the products; two accumulators of 256 columns let the
- * storing of one tile run under the products of the next.  CTAs are persistent
- * and take every gridDim-th tile of a job.
+ * storing of one tile run under the products of the next.  Two CTAs on
+ * neighbouring SMs share a tile of 256 m where there are as many (PAIR): each
+ * brings its 128 rows of A and half of B's, so that a product's 128 x 256 x 64
+ * take 32 KB from L2 and not 48.  L2 gave a lone CTA some 46 bytes a cycle
+ * and SM, which held it at half of the tensor cores' rate.
+ * CTAs (pairs) are persistent and take every so-many-th tile of a job.
+ *
+ * Operands of more than 16 bits come as planes that sum to them; a stage holds
+ * all planes, and the pairs of planes whose product counts are multiplied one
+ * after the other, small ones first.  Their sums are taken out of the tensor
+ * cores every kSegment stages and go on in f32 registers: the tensor cores'
+ * own additions cut what does not fit, which over thousands of k left errors of
+ * 4e-6 to 2e-5 in results that f32 arithmetic has to 1e-6.
  *
  * A job says what its tiles are and stores them (struct Job: setup, tiles,
- * tile, store); operands of more than 16 bits come as planes that sum to them,
- * and a job lists the pairs of planes to multiply.
+ * tile, store).
  *
  * Waits are bounded by a second; one that runs out reports
  * TB_FEATURE_STATUS_WAIT_TIMEOUT through the stream's status word, after which
@@ -41,45 +51,66 @@ using tb_pipe::mbar_arrive_expect_tx;
 using tb_pipe::mbar_init;
 using tb_pipe::smem_addr;
 
-constexpr int kTileM = 128;
-constexpr int kBlockBytes = 128;             /* of k in a stage */
-constexpr int kChunk = 64;                   /* 16-bit values of m (n) in a swizzled row, where those are contiguous */
+constexpr int kRows = 128;                    /* of m in a CTA's part of a tile */
+constexpr int kBlockBytes = 128;              /* of k in a stage */
+constexpr int kChunk = 64;                    /* 16-bit values of m (n) in a swizzled row, where those are contiguous */
 constexpr int kChunkBytes = 64 * kBlockBytes; /* 64 such rows, one for each k of a stage */
-constexpr int kThreads = 192;
-constexpr int kStoreWarps = 4, kStoreThreads = 32 * kStoreWarps;
-constexpr int kMaxPairs = 6;
+constexpr int kStoreWarps = 8;
+constexpr int kThreads = 64 + 32 * kStoreWarps;
 constexpr int kColumns = 512; /* of TMEM: two accumulators of 256 */
+constexpr int kSegment = 2;   /* stages of operands in planes between two readings of the accumulator */
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
 /* ---- instructions ---- */
 
-__device__ __forceinline__ void tmem_alloc(uint32_t result, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(result), "r"(columns) : "memory");
+/* One lane of a whole warp, the same each time.  The compiler knows that it is
+ * one, and issues copies and products without a loop over lanes: with `lane ==
+ * 0` in its place four products took 394 cycles to issue. */
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
-__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t result, uint32_t columns) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(result), "r"(columns) : "memory");
+    else
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(result), "r"(columns) : "memory");
+}
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    } else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    }
 }
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-/* `bar` completes a phase when the products issued so far by this thread are done. */
-__device__ __forceinline__ void tensor_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-template <bool I8> __device__ __forceinline__ void tensor_product(uint32_t d, uint64_t a, uint64_t b, uint32_t how, bool add) {
-    if constexpr (I8)
+/* `bar` (of both CTAs of a pair) completes a phase when the products issued so far by this thread are done. */
+template <bool PAIR> __device__ __forceinline__ void tensor_commit(uint32_t bar) {
+    if constexpr (PAIR)
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(how),
-            "r"(static_cast<uint32_t>(add))
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"(static_cast<uint16_t>(3))
             : "memory");
     else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(how),
-            "r"(static_cast<uint32_t>(add))
-            : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+#define TB_TENSOR_PRODUCT(GROUP, KIND)                                                                          \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::" KIND \
+                 " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) \
+                 : "memory")
+template <bool I8, bool PAIR>
+__device__ __forceinline__ void tensor_product(uint32_t d, uint64_t a, uint64_t b, uint32_t how, bool add) {
+    if constexpr (I8 && PAIR) TB_TENSOR_PRODUCT("2", "i8");
+    else if constexpr (I8) TB_TENSOR_PRODUCT("1", "i8");
+    else if constexpr (PAIR) TB_TENSOR_PRODUCT("2", "f16");
+    else TB_TENSOR_PRODUCT("1", "f16");
+}
+#undef TB_TENSOR_PRODUCT
 /* 32 columns of this warp's 32 lanes; tensor_wait_load() before the values are used. */
 __device__ __forceinline__ void tensor_load(uint32_t tmem, uint32_t (&r)[32]) {
     asm volatile(
@@ -93,11 +124,44 @@ __device__ __forceinline__ void tensor_load(uint32_t tmem, uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tensor_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+/* `bar` lies in this CTA, or (PAIR) in either of the two. */
+template <bool PAIR>
 __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+            "[%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+            ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+}
+
+/* ---- the other CTA of a pair ---- */
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+/* Where the first CTA of the pair has what lies at `at` here. */
+__device__ __forceinline__ uint32_t in_first(uint32_t at) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(at));
+    return r;
+}
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+/* Relaxed: it publishes nothing, and a release waits for this thread's stores and copies, a microsecond a stage. */
+__device__ __forceinline__ void remote_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 /* An operand in shared memory, rows of 128 bytes in the 128-byte swizzle.
@@ -109,11 +173,11 @@ __device__ __forceinline__ uint64_t operand(uint32_t at, bool outer_contiguous) 
            (1ull << 46) | (2ull << 61);
 }
 /* How the products are taken: type of the operands (0 f16, 1 bf16; 1 signed 8
- * bits), their orders, columns; 128 rows, 32-bit accumulators. */
-__device__ __forceinline__ uint32_t product_form(bool i8, int type, bool a_outer, bool b_outer, int columns) {
+ * bits), their orders, rows and columns; 32-bit accumulators. */
+__device__ __forceinline__ uint32_t product_form(bool i8, int type, bool a_outer, bool b_outer, int rows, int columns) {
     return (i8 ? 2u : 1u) << 4 | static_cast<uint32_t>(type) << 7 | static_cast<uint32_t>(type) << 10 |
            static_cast<uint32_t>(a_outer) << 15 | static_cast<uint32_t>(b_outer) << 16 |
-           static_cast<uint32_t>(columns / 8) << 17 | static_cast<uint32_t>(kTileM / 16) << 24;
+           static_cast<uint32_t>(columns / 8) << 17 | static_cast<uint32_t>(rows / 16) << 24;
 }
 
 /* ---- jobs ---- */
@@ -123,10 +187,9 @@ __device__ __forceinline__ uint32_t product_form(bool i8, int type, bool a_outer
 struct Operands {
     CUtensorMap a, b;
     unsigned *status;
-    int a_outer, b_outer;   /* m (n) contiguous instead of k */
-    int type;               /* 0 f16, 1 bf16, 1 signed 8 bits */
-    int pairs;              /* of planes, in the order of their sum */
-    int a_plane[kMaxPairs], b_plane[kMaxPairs]; /* z of each pair's planes, to be added to a tile's */
+    int a_outer, b_outer; /* m (n) contiguous instead of k */
+    int type;             /* 0 f16, 1 bf16, 1 signed 8 bits */
+    int a_plane, b_plane; /* z of the second plane */
 };
 
 /* k in [k0, k0 + depth) of rows m0.. of A's matrix az and n0.. (columns of
@@ -138,23 +201,30 @@ struct Tile {
 
 /* ---- the kernel ---- */
 
-template <int NT> struct Shape {
-    static constexpr int kABytes = kTileM * kBlockBytes, kBBytes = NT * kBlockBytes, kStage = kABytes + kBBytes;
+template <int NT, int PLANES, bool PAIR> struct Shape {
+    static constexpr int kTileM = PAIR ? 2 * kRows : kRows;
+    static constexpr int kPart = PAIR ? NT / 2 : NT; /* rows of B that a CTA brings */
+    static constexpr int kABytes = kRows * kBlockBytes, kBBytes = kPart * kBlockBytes;
+    static constexpr int kStage = PLANES * (kABytes + kBBytes);
     static constexpr int kStages = 196608 / kStage > 12 ? 12 : 196608 / kStage;
     static constexpr int kShared = kStages * kStage + 1024; /* + alignment */
+    static constexpr int kHalf = NT >= 64 ? NT / 2 : 32;    /* columns that a storing warp reads */
+    static_assert(kStages >= 2, "a ring");
 };
 
 struct Waits {
     unsigned *status;
     volatile int *gave_up; /* in shared memory */
     __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) const {
-        if (tb_pipe::mbar_try_wait(bar, parity)) return true;
-        const unsigned long long t0 = tb_pipe::global_ns();
+        /* the clock is read late: reading it takes longer than most waits */
+        unsigned long long t0 = 0;
         for (;;) {
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 256; ++i)
                 if (tb_pipe::mbar_try_wait(bar, parity)) return true;
             if (*gave_up) return false;
-            if (tb_pipe::global_ns() - t0 > kWaitNs) break;
+            const unsigned long long now = tb_pipe::global_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > kWaitNs) break;
         }
         if (!*gave_up) atomicOr(status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
         *gave_up = 1;
@@ -162,141 +232,266 @@ struct Waits {
     }
 };
 
-/* Rows of k at and past `from` of a stage's operand of `chunks` chunks (m or n
- * contiguous) become zero, up to the next 16; by a warp. */
+/* Rows of k at and past `from` of a stage's chunks (m or n contiguous) become
+ * zero, up to the next 16; by a warp. */
 __device__ __forceinline__ void clear_past(unsigned char *at, int chunks, int from, int lane) {
     const int rows = (from + 15) / 16 * 16 - from, words = rows * 8; /* of 16 bytes */
     for (int c = 0; c < chunks; ++c)
         for (int i = lane; i < words; i += 32)
             *reinterpret_cast<uint4 *>(at + c * kChunkBytes + from * kBlockBytes + i * 16) = uint4{0, 0, 0, 0};
+    tb_pipe::fence_proxy_async_shared();
+    __syncwarp();
 }
 
-template <class Job, int NT, bool I8>
+template <class Job, int NT, int PLANES, bool I8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Job job) {
-    using S = Shape<NT>;
+    using S = Shape<NT, PLANES, PAIR>;
     constexpr int kDepth = I8 ? 128 : 64, kStep = I8 ? 32 : 16; /* of k: in a stage, in an instruction */
+    constexpr bool kSums = PLANES > 1;                          /* of segments, in registers */
+    constexpr int kCtas = PAIR ? 2 : 1;
+    constexpr int kBChunks = (S::kPart + kChunk - 1) / kChunk;
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages], done[2], freed[2];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], done[2], freed[2], tail[S::kStages];
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up;
     __shared__ typename Job::Shared shared;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const bool first = rank == 0; /* the CTA whose warp issues the products */
     unsigned char *stages = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) mbar_init(smem_addr(&full[i]), 1), mbar_init(smem_addr(&empty[i]), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&done[i]), 1), mbar_init(smem_addr(&freed[i]), kStoreWarps);
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(smem_addr(&full[i]), kCtas);
+            mbar_init(smem_addr(&empty[i]), 1);
+            mbar_init(smem_addr(&tail[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&done[i]), 1), mbar_init(smem_addr(&freed[i]), kCtas * kStoreWarps);
         gave_up = 0;
         tb_pipe::fence_mbar_init();
     }
-    if (warp == 1) tmem_alloc(smem_addr(&tmem_at), kColumns);
+    if (warp == 1) tmem_alloc<PAIR>(smem_addr(&tmem_at), kColumns);
     tensor_fence_before();
     job.setup(shared);
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     tensor_fence_after();
     const uint32_t tmem = tmem_at;
     const Waits w{ops.status, &gave_up};
-    const int tiles = job.tiles(shared);
+    const int tiles = job.tiles(shared), start = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
+    /* Whether a stage's last rows of k belong to another matrix. */
+    const auto ends_inside = [&](int left) { return Job::kRagged && left < kDepth && left % kStep != 0; };
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t n = 0; /* stages asked for */
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const Tile tile = job.tile(shared, t);
-                for (int p = 0; ok && p < ops.pairs; ++p) {
-                    const int az = tile.az + ops.a_plane[p], bz = tile.bz + ops.b_plane[p];
-                    for (int k = 0; k < tile.depth; k += kDepth, ++n) {
-                        const int s = n % S::kStages;
-                        if (n >= S::kStages && !(ok = w.wait(smem_addr(&empty[s]), (n / S::kStages - 1) & 1))) break;
-                        const uint32_t bar = smem_addr(&full[s]), at = smem_addr(stages + s * S::kStage);
-                        mbar_arrive_expect_tx(bar, S::kStage);
-                        if (ops.a_outer) {
-                            load_box(at, &ops.a, tile.m0, tile.k0 + k, az, bar);
-                            load_box(at + kChunkBytes, &ops.a, tile.m0 + kChunk, tile.k0 + k, az, bar);
+        uint32_t n = 0; /* stages asked for */
+        bool ok = true;
+        for (int t = start; ok && t < tiles; t += stride) {
+            const Tile tile = job.tile(shared, t);
+            const int m0 = tile.m0 + static_cast<int>(rank) * kRows;
+            const int n0 = tile.n0 + static_cast<int>(rank) * ((tile.columns + 15) / 16 * 8);
+            for (int k = 0; k < tile.depth; k += kDepth, ++n) {
+                const int s = n % S::kStages;
+                if (n >= S::kStages && !(ok = w.wait(smem_addr(&empty[s]), (n / S::kStages - 1) & 1))) break;
+                if (elected()) {
+                    uint32_t bar = smem_addr(&full[s]), at = smem_addr(stages + s * S::kStage);
+                    if (PAIR && !first) {
+                        if (ends_inside(tile.depth - k)) { /* this CTA clears its own rows, and then says so */
+                            bar = smem_addr(&tail[s]);
+                            mbar_arrive_expect_tx(bar, S::kStage);
                         } else {
-                            load_box(at, &ops.a, tile.k0 + k, tile.m0, az, bar);
+                            bar = in_first(bar);
+                            remote_arrive_expect_tx(bar, S::kStage);
                         }
+                    } else {
+                        mbar_arrive_expect_tx(bar, S::kStage);
+                    }
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p, at += S::kABytes) {
+                        const int z = tile.az + p * ops.a_plane;
+                        if (ops.a_outer) {
+                            load_box<PAIR>(at, &ops.a, m0, tile.k0 + k, z, bar);
+                            load_box<PAIR>(at + kChunkBytes, &ops.a, m0 + kChunk, tile.k0 + k, z, bar);
+                        } else {
+                            load_box<PAIR>(at, &ops.a, tile.k0 + k, m0, z, bar);
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p, at += S::kBBytes) {
+                        const int z = tile.bz + p * ops.b_plane;
                         if (ops.b_outer) {
 #pragma unroll
-                            for (int c = 0; c < (NT + kChunk - 1) / kChunk; ++c)
-                                load_box(at + S::kABytes + c * kChunkBytes, &ops.b, tile.n0 + c * kChunk, tile.k0 + k, bz, bar);
+                            for (int c = 0; c < kBChunks; ++c)
+                                load_box<PAIR>(at + c * kChunkBytes, &ops.b, n0 + c * kChunk, tile.k0 + k, z, bar);
                         } else {
-                            load_box(at + S::kABytes, &ops.b, tile.k0 + k, tile.n0, bz, bar);
+                            load_box<PAIR>(at, &ops.b, tile.k0 + k, n0, z, bar);
                         }
                     }
                 }
+                __syncwarp();
             }
-            /* copies land before the CTA leaves, also where the products gave up on them */
+        }
+        /* copies land before the CTA leaves, also where the products gave up on them (a pair's
+         * are all counted by its first CTA, and both leave together) */
+        if (first)
             for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
                 tb_pipe::mbar_wait(smem_addr(&full[i % S::kStages]), (i / S::kStages) & 1, kWaitNs);
-        }
-    } else if (warp == 1) {
-        uint32_t n = 0, number = 0; /* stages taken, tiles */
+    } else if (warp == 1 && first) {
+        uint32_t n = 0, number = 0; /* stages taken, accumulators begun */
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++number) {
+        for (int t = start; ok && t < tiles; t += stride) {
             const Tile tile = job.tile(shared, t);
-            const uint32_t buffer = number & 1, d = tmem + buffer * 256;
-            if (number >= 2 && !(ok = w.wait(smem_addr(&freed[buffer]), (number / 2 - 1) & 1))) break;
-            tensor_fence_after();
-            const uint32_t how = product_form(I8, ops.type, ops.a_outer, ops.b_outer, (tile.columns + 15) / 16 * 16);
-            for (int p = 0; ok && p < ops.pairs; ++p)
-                for (int k = 0; k < tile.depth; k += kDepth, ++n) {
-                    const int s = n % S::kStages, left = tile.depth - k;
+            const uint32_t how =
+                product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, (tile.columns + 15) / 16 * 16);
+            uint32_t d = 0;
+            for (int k = 0, in = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++in) {
+                if (k == 0 || (kSums && in == kSegment)) { /* the next accumulator */
+                    in = 0;
+                    const uint32_t buffer = number & 1;
+                    d = tmem + buffer * 256;
+                    if (number >= 2 && !(ok = w.wait(smem_addr(&freed[buffer]), (number / 2 - 1) & 1))) break;
+                    tensor_fence_after();
+                    ++number;
+                }
+                const int s = n % S::kStages, left = tile.depth - k;
+                if (left > 0) {
                     if (!(ok = w.wait(smem_addr(&full[s]), (n / S::kStages) & 1))) break;
                     unsigned char *at = stages + s * S::kStage;
-                    if (Job::kRagged && left < kDepth && left % kStep) { /* what follows belongs to another matrix */
-                        clear_past(at, kTileM / kChunk, left, lane);
-                        clear_past(at + S::kABytes, (NT + kChunk - 1) / kChunk, left, lane);
-                        tb_pipe::fence_proxy_async_shared();
-                        __syncwarp();
+                    if (ends_inside(left)) {
+                        clear_past(at, PLANES * (kRows / kChunk), left, lane);
+                        clear_past(at + PLANES * S::kABytes, PLANES * kBChunks, left, lane);
                     }
                     tensor_fence_after();
-                    if (lane == 0) {
-                        const uint64_t a = operand(smem_addr(at), ops.a_outer), b = operand(smem_addr(at + S::kABytes), ops.b_outer);
+                    if (elected()) {
                         const int steps = min(kDepth, left + kStep - 1) / kStep;
                         const uint32_t ia = (ops.a_outer ? kStep * kBlockBytes : 32) >> 4, ib = (ops.b_outer ? kStep * kBlockBytes : 32) >> 4;
+                        bool add = in > 0;
+                        /* planes i and j count while i + j < PLANES: the small products first */
 #pragma unroll
-                        for (int i = 0; i < kDepth / kStep; ++i)
-                            if (i < steps) tensor_product<I8>(d, a + i * ia, b + i * ib, how, p > 0 || k > 0 || i > 0);
-                        tensor_commit(smem_addr(&empty[s]));
+                        for (int small = PLANES - 1; small >= 0; --small)
+#pragma unroll
+                            for (int p = 0; p <= small; ++p) {
+                                uint64_t a = operand(smem_addr(at + p * S::kABytes), ops.a_outer);
+                                uint64_t b = operand(smem_addr(at + PLANES * S::kABytes + (small - p) * S::kBBytes), ops.b_outer);
+                                if (steps == kDepth / kStep) {
+#pragma unroll
+                                    for (int i = 0; i < kDepth / kStep; ++i) {
+                                        tensor_product<I8, PAIR>(d, a + i * ia, b + i * ib, how, add);
+                                        add = true;
+                                    }
+                                } else {
+                                    for (int i = 0; i < steps; ++i, a += ia, b += ib) {
+                                        tensor_product<I8, PAIR>(d, a, b, how, add);
+                                        add = true;
+                                    }
+                                }
+                            }
+                        tensor_commit<PAIR>(smem_addr(&empty[s]));
                     }
                     __syncwarp();
+                    ++n;
                 }
-            if (lane == 0) tensor_commit(smem_addr(&done[buffer]));
-            __syncwarp();
+                if (left <= kDepth || (kSums && in == kSegment - 1)) {
+                    if (elected()) tensor_commit<PAIR>(smem_addr(&done[(number - 1) & 1]));
+                    __syncwarp();
+                }
+            }
         }
         /* products end before the TMEM is freed, also where the storing warps gave up on them */
         if (n > 0) tb_pipe::mbar_wait(smem_addr(&empty[(n - 1) % S::kStages]), ((n - 1) / S::kStages) & 1, kWaitNs);
-    } else {
-        const int part = warp % 4; /* the lanes of TMEM that this warp may read */
-        uint32_t number = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++number) {
-            const Tile tile = job.tile(shared, t);
-            const uint32_t buffer = number & 1;
-            if (!w.wait(smem_addr(&done[buffer]), (number / 2) & 1)) break;
-            tensor_fence_after();
-            const int m = tile.m0 + part * 32 + lane;
-            for (int c = 0; c < tile.columns; c += 32) {
-                uint32_t r[32];
-                if (tile.depth > 0) {
-                    tensor_load(tmem + buffer * 256 + (static_cast<uint32_t>(part) << 21) + c, r);
-                    tensor_wait_load();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = 0;
+    } else if (warp == 1) {
+        if (Job::kRagged) { /* the second CTA's rows past a matrix's end, stage by stage as the first takes them */
+            uint32_t n = 0, phases = 0; /* a bit for each stage */
+            bool ok = true;
+            for (int t = start; ok && t < tiles; t += stride) {
+                const Tile tile = job.tile(shared, t);
+                for (int k = 0; k < tile.depth; k += kDepth, ++n) {
+                    if (!ends_inside(tile.depth - k)) continue;
+                    const int s = n % S::kStages;
+                    if (!(ok = w.wait(smem_addr(&tail[s]), phases >> s & 1))) { /* the copies land all the same */
+                        tb_pipe::mbar_wait(smem_addr(&tail[s]), phases >> s & 1, kWaitNs);
+                        break;
+                    }
+                    phases ^= 1u << s;
+                    unsigned char *at = stages + s * S::kStage;
+                    clear_past(at, PLANES * (kRows / kChunk), tile.depth - k, lane);
+                    clear_past(at + PLANES * S::kABytes, PLANES * kBChunks, tile.depth - k, lane);
+                    if (lane == 0) remote_arrive(in_first(smem_addr(&full[s])));
+                    __syncwarp();
                 }
-                job.store(shared, tile, m, c, r);
             }
+        }
+    } else {
+        const int part = warp % 4, half = (warp - 2) / 4; /* the lanes of TMEM that this warp may read; its columns */
+        const uint32_t lanes = static_cast<uint32_t>(part) << 21;
+        uint32_t number = 0;
+        bool ok = true;
+        const auto free = [&](uint32_t buffer) {
             tensor_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&freed[buffer]));
+            if (lane == 0) {
+                if constexpr (PAIR) remote_arrive(in_first(smem_addr(&freed[buffer])));
+                else mbar_arrive(smem_addr(&freed[buffer]));
+            }
+        };
+        for (int t = start; ok && t < tiles; t += stride) {
+            const Tile tile = job.tile(shared, t);
+            const int m = tile.m0 + static_cast<int>(rank) * kRows + part * 32 + lane;
+            const int c0 = half * S::kHalf, columns = NT >= 64 || half == 0 ? min(tile.columns - c0, S::kHalf) : 0;
+            if constexpr (kSums) {
+                float sum[S::kHalf];
+                for (int k = 0; ok && (k < tile.depth || k == 0); k += kSegment * kDepth, ++number) {
+                    const uint32_t buffer = number & 1;
+                    if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
+                    tensor_fence_after();
+#pragma unroll
+                    for (int c = 0; c < S::kHalf; c += 32) {
+                        if (c < columns && tile.depth > 0) {
+                            uint32_t r[32];
+                            tensor_load(tmem + buffer * 256 + lanes + c0 + c, r);
+                            tensor_wait_load();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[c + i] = k == 0 ? __uint_as_float(r[i]) : sum[c + i] + __uint_as_float(r[i]);
+                        } else if (k == 0) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[c + i] = 0.0f;
+                        }
+                    }
+                    free(buffer);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < S::kHalf; c += 32)
+                    if (c < columns) {
+                        uint32_t r[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[c + i]);
+                        job.store(shared, tile, m, c0 + c, r);
+                    }
+            } else {
+                const uint32_t buffer = number & 1;
+                if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
+                tensor_fence_after();
+                for (int c = 0; c < columns; c += 32) {
+                    uint32_t r[32];
+                    if (tile.depth > 0) {
+                        tensor_load(tmem + buffer * 256 + lanes + c0 + c, r);
+                        tensor_wait_load();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = 0;
+                    }
+                    job.store(shared, tile, m, c0 + c, r);
+                }
+                free(buffer);
+                ++number;
+            }
         }
     }
     __syncwarp();
     tensor_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     tensor_fence_after();
-    if (warp == 1) tmem_free(tmem, kColumns);
+    if (warp == 1) tmem_free<PAIR>(tmem, kColumns);
 }
 
 /* ---- host side ---- */
@@ -344,20 +539,33 @@ inline bool encode(CUtensorMap *map, const Matrices &m, int box_rows) {
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-/* Both operands' maps for tiles of `columns` of n (64 at least where n is contiguous in b). */
-inline bool encode(Operands *ops, const Matrices &a, bool a_outer, const Matrices &b, bool b_outer, int columns) {
+/* Both operands' maps for tiles of NT columns (64 at least a CTA where n is contiguous in b). */
+template <int NT, bool PAIR> bool encode(Operands *ops, const Matrices &a, bool a_outer, const Matrices &b, bool b_outer) {
+    constexpr int kPart = PAIR ? NT / 2 : NT;
     ops->a_outer = a_outer;
     ops->b_outer = b_outer;
-    if (b_outer && columns < kChunk) return false;
-    return encode(&ops->a, a, a_outer ? kChunk : kTileM) && encode(&ops->b, b, b_outer ? kChunk : columns);
+    return (!b_outer || kPart >= kChunk) && encode(&ops->a, a, a_outer ? kChunk : kRows) &&
+           encode(&ops->b, b, b_outer ? kChunk : kPart);
 }
 
-template <class Job, int NT, bool I8>
-int launch_products(const Operands &ops, const Job &job, size_t most_tiles, int sms, cudaStream_t st) {
-    if (!tb_learn::allow_shared<tensor_products<Job, NT, I8>>(Shape<NT>::kShared)) return 0;
-    const unsigned grid = static_cast<unsigned>(most_tiles < static_cast<size_t>(sms) ? most_tiles : sms);
-    tensor_products<Job, NT, I8><<<grid, kThreads, Shape<NT>::kShared, st>>>(ops, job);
-    return tb_learn::launched();
+/* tiles: at most. */
+template <int NT, int PLANES, bool I8, bool PAIR, class Job>
+int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, cudaStream_t st) {
+    constexpr auto kernel = tensor_products<Job, NT, PLANES, I8, PAIR>;
+    constexpr int kCtas = PAIR ? 2 : 1, kShared = Shape<NT, PLANES, PAIR>::kShared;
+    if (!tb_learn::allow_shared<tensor_products<Job, NT, PLANES, I8, PAIR>>(kShared)) return 0;
+    const size_t most = static_cast<size_t>(sms) / kCtas;
+    cudaLaunchConfig_t config{};
+    config.gridDim = static_cast<unsigned>(tiles < most ? tiles : most) * kCtas;
+    config.blockDim = kThreads;
+    config.dynamicSmemBytes = kShared;
+    config.stream = st;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim = {kCtas, 1, 1};
+    config.attrs = &attribute;
+    config.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, ops, job) == cudaSuccess && tb_learn::launched();
 }
 
 } /* namespace tb_tensor */
