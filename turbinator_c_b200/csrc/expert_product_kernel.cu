@@ -57,7 +57,7 @@ template <class T, int NT> struct RowJob {
     size_t out_stride;
 
     __device__ void setup(Shared &s) const {
-        for (int e = threadIdx.x; e < runs.experts; e += tb_tensor::kThreads) {
+        for (int e = threadIdx.x; e < runs.experts; e += blockDim.x) {
             s.start[e] = run_start(runs, e);
             s.end[e] = run_end(runs, e, s.start[e]);
         }
@@ -98,11 +98,11 @@ template <class T, int NT> struct RowJob {
         r.which = low;
         return r;
     }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[32]) const {
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[8]) const {
         if (m >= width) return;
         T *o = out + (t.n0 + c) * out_stride + m;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 8; ++i)
             if (c + i < t.columns) o[i * out_stride] = stored<T>(r[i]);
     }
 };
@@ -111,12 +111,12 @@ template <class T, int NT> struct RowJob {
 template <class T, int NT> struct IntegerJob : RowJob<T, NT> {
     const float *row_scale, *channel_scale;
     __device__ __forceinline__ void store(const typename RowJob<T, NT>::Shared &, const Tile &t, int m, int c,
-                                          const uint32_t (&r)[32]) const {
+                                          const uint32_t (&r)[8]) const {
         if (m >= this->width) return;
         T *o = this->out + (t.n0 + c) * this->out_stride + m;
         const float s = channel_scale[static_cast<size_t>(t.which) * this->width + m];
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 8; ++i)
             if (c + i < t.columns)
                 o[i * this->out_stride] = from_float<T>(static_cast<float>(static_cast<int>(r[i])) * (row_scale[t.n0 + c + i] * s));
     }
@@ -146,11 +146,11 @@ template <class T, int NT> struct SumJob {
         r.which = e;
         return r;
     }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[32]) const {
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c, const uint32_t (&r)[8]) const {
         if (m >= width) return;
         T *o = out + t.which * matrix_stride + (t.n0 + c) * row_stride + m;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < 8; ++i)
             if (c + i < t.columns) o[i * row_stride] = stored<T>(r[i]);
     }
 };

@@ -32,7 +32,20 @@ constexpr float kDown = 1.0f / 4096.0f;
 struct Pair {
     __half *at;
     size_t line, matrix, plane;
-    __device__ __forceinline__ float get(size_t i) const { return __half2float(at[i]) + __half2float(at[plane + i]); }
+    /* Eight values `line` apart, all under way before the first is used. */
+    __device__ __forceinline__ void get(size_t i, int count, float (&v)[8]) const {
+        __half high[8], low[8];
+        const __half *from = at + i;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, from += line)
+            if (j < count) {
+                high[j] = from[0];
+                low[j] = from[plane];
+            }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) v[j] = __half2float(high[j]) + __half2float(low[j]);
+    }
     __device__ __forceinline__ void put(size_t i, float v) const {
         const __half high = __float2half_rn(v);
         at[i] = high;
@@ -143,33 +156,36 @@ struct SquareJob {
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[32]) const {
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
         if (m >= plan.width) return;
-        const size_t base = t.which * out.matrix;
-        float v[32];
+        const size_t base = t.which * out.matrix, at = base + (t.n0 + c0) * out.line + m;
+        const int count = t.columns - c0;
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            v[i] = __uint_as_float(r[i]) * kDown;
-            if (c0 + i < t.columns) {
-                const size_t at = base + (t.n0 + c0 + i) * out.line + m;
-                if (old.at) v[i] = fmaf(c, v[i], b * old.get(at));
-                out.put(at, v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]) * kDown;
+        if (old.at) {
+            float was[8];
+            old.get(at, count, was);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(c, v[i], b * was[i]);
+        }
+        __half high[8], low[8], *to = out.at + at;
+#pragma unroll
+        for (int i = 0; i < 8; ++i, to += out.line) {
+            high[i] = __float2half_rn(v[i]);
+            low[i] = __float2half_rn(v[i] - __half2float(high[i]));
+            if (i < count) {
+                to[0] = high[i];
+                to[out.plane] = low[i];
             }
         }
         if (plan.mirrored(t, m, c0)) { /* 16 bytes at a time; a line's end is a multiple of eight */
+            __half *across = out.at + base + m * out.line + t.n0 + c0;
+            Pack<__half, 8> h, l;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-                if (c0 + i >= t.columns) break;
-                float high[8], low[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    high[j] = __half2float(__float2half_rn(v[i + j]));
-                    low[j] = v[i + j] - high[j];
-                }
-                const size_t at = base + m * out.line + t.n0 + c0 + i;
-                *reinterpret_cast<Held<__half, 8> *>(out.at + at) = packed<__half, 8>(high);
-                *reinterpret_cast<Held<__half, 8> *>(out.at + out.plane + at) = packed<__half, 8>(low);
-            }
+            for (int i = 0; i < 8; ++i) h.v[i] = high[i], l.v[i] = low[i];
+            *reinterpret_cast<Pack<__half, 8> *>(across) = h;
+            *reinterpret_cast<Pack<__half, 8> *>(across + out.plane) = l;
         }
     }
 };
@@ -186,15 +202,24 @@ template <class T> struct StepJob {
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[32]) const {
+    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
         if (m >= plan.width) return;
+        const int count = t.columns - c0;
+        const size_t n = t.n0 + c0, at = t.which * x.matrix + n * x.line + m;
+        float v[8];
+        x.get(at, count, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if (c0 + i >= t.columns) continue;
-            const size_t n = t.n0 + c0 + i, at = t.which * x.matrix + n * x.line + m;
-            const float v = fmaf(a, x.get(at), __uint_as_float(r[i]) * kDown);
-            if (last) last[t.which * matrix_stride + n * row_stride + m] = from_float<T>(v * kDown * scale);
-            else next.put(at, v);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(a, v[i], __uint_as_float(r[i]) * kDown);
+        if (last) {
+            T *o = last + t.which * matrix_stride + n * row_stride + m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i, o += row_stride)
+                if (i < count) *o = from_float<T>(v[i] * kDown * scale);
+        } else {
+            size_t to = at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i, to += x.line)
+                if (i < count) next.put(to, v[i]);
         }
     }
 };

@@ -10,14 +10,14 @@
  * columns, to the next 16, as it has.  Either operand may lie with k
  * contiguous or with m (n) contiguous; the tensor cores take both.
  *
- * A CTA of ten warps: one asks for the copies, one issues the products, eight
- * read the accumulators.  A ring of 128-byte-deep stages (64 values of 16 bits,
+ * One warp of a CTA asks for the copies, one issues the products, eight or
+ * sixteen read the accumulators.  A ring of 128-byte-deep stages (64 values of 16 bits,
  * 128 of 8) feeds the products; two accumulators of 256 columns let the
  * storing of one tile run under the products of the next.  Two CTAs on
  * neighbouring SMs share a tile of 256 m where there are as many (PAIR): each
  * brings its 128 rows of A and half of B's, so that a product's 128 x 256 x 64
  * take 32 KB from L2 and not 48.  L2 gave a lone CTA some 46 bytes a cycle
- * and SM, which held it at half of the tensor cores' rate.
+ * and SM at best.
  * CTAs (pairs) are persistent and take every so-many-th tile of a job.
  *
  * Operands of more than 16 bits come as planes that sum to them; a stage holds
@@ -28,7 +28,7 @@
  * 4e-6 to 2e-5 in results that f32 arithmetic has to 1e-6.
  *
  * A job says what its tiles are and stores them (struct Job: setup, tiles,
- * tile, store).
+ * tile, store: eight columns of a row of the tensor core's).
  *
  * Waits are bounded by a second; one that runs out reports
  * TB_FEATURE_STATUS_WAIT_TIMEOUT through the stream's status word, after which
@@ -55,8 +55,6 @@ constexpr int kRows = 128;                    /* of m in a CTA's part of a tile 
 constexpr int kBlockBytes = 128;              /* of k in a stage */
 constexpr int kChunk = 64;                    /* 16-bit values of m (n) in a swizzled row, where those are contiguous */
 constexpr int kChunkBytes = 64 * kBlockBytes; /* 64 such rows, one for each k of a stage */
-constexpr int kStoreWarps = 8;
-constexpr int kThreads = 64 + 32 * kStoreWarps;
 constexpr int kColumns = 512; /* of TMEM: two accumulators of 256 */
 constexpr int kSegment = 2;   /* stages of operands in planes between two readings of the accumulator */
 constexpr unsigned long long kWaitNs = 1000000000ull;
@@ -111,7 +109,7 @@ __device__ __forceinline__ void tensor_product(uint32_t d, uint64_t a, uint64_t 
     else TB_TENSOR_PRODUCT("1", "f16");
 }
 #undef TB_TENSOR_PRODUCT
-/* 32 columns of this warp's 32 lanes; tensor_wait_load() before the values are used. */
+/* 32 or 16 columns of this warp's 32 lanes; tensor_wait_load() before the values are used. */
 __device__ __forceinline__ void tensor_load(uint32_t tmem, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -120,6 +118,13 @@ __device__ __forceinline__ void tensor_load(uint32_t tmem, uint32_t (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(tmem));
+}
+__device__ __forceinline__ void tensor_load(uint32_t tmem, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(tmem));
 }
 __device__ __forceinline__ void tensor_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -152,10 +157,11 @@ __device__ __forceinline__ uint32_t in_first(uint32_t at) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(at));
     return r;
 }
+/* Relaxed: they publish nothing, and a release waits for this thread's stores
+ * and copies, a microsecond each. */
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-/* Relaxed: it publishes nothing, and a release waits for this thread's stores and copies, a microsecond a stage. */
 __device__ __forceinline__ void remote_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
@@ -204,11 +210,21 @@ struct Tile {
 template <int NT, int PLANES, bool PAIR> struct Shape {
     static constexpr int kTileM = PAIR ? 2 * kRows : kRows;
     static constexpr int kPart = PAIR ? NT / 2 : NT; /* rows of B that a CTA brings */
-    static constexpr int kABytes = kRows * kBlockBytes, kBBytes = kPart * kBlockBytes;
-    static constexpr int kStage = PLANES * (kABytes + kBBytes);
+    static constexpr int kABytes = kRows * kBlockBytes, kBBytes = kPart * kBlockBytes; /* of a block: 128 bytes of k */
+    /* Blocks of k in a stage: two of a single plane, so that a stage's waits and its commit, some 250 cycles to issue,
+     * come with eight products of 128 cycles and not four. */
+    static constexpr int kBlocks = PLANES == 1 ? 2 : 1;
+    static constexpr int kStage = kBlocks * PLANES * (kABytes + kBBytes);
     static constexpr int kStages = 196608 / kStage > 12 ? 12 : 196608 / kStage;
     static constexpr int kShared = kStages * kStage + 1024; /* + alignment */
-    static constexpr int kHalf = NT >= 64 ? NT / 2 : 32;    /* columns that a storing warp reads */
+    /* Sums of 256 columns in registers: 128 each of eight warps, which take the registers that the others leave (216 and
+     * 72 of 168 each); in sixteen warps of 96 registers the sums spilled and a tile's storing took four times as long. */
+    static constexpr bool kWide = PLANES > 1 && NT == 256;
+    static constexpr int kShare = kWide ? 128 : NT >= 128 ? 64 : 32; /* columns that a storing warp reads */
+    static constexpr int kFirstStore = kWide ? 4 : 2, kStoreWarps = 4 * (NT / kShare);
+    static constexpr int kThreads = 32 * (kFirstStore + kStoreWarps);
+    static constexpr int kLaunchRegisters = 168, kStoreRegisters = 216, kOtherRegisters = 72;
+    static_assert(!kWide || kThreads * kLaunchRegisters == 32 * (kStoreWarps * kStoreRegisters + 4 * kOtherRegisters), "a split");
     static_assert(kStages >= 2, "a ring");
 };
 
@@ -232,7 +248,7 @@ struct Waits {
     }
 };
 
-/* Rows of k at and past `from` of a stage's chunks (m or n contiguous) become
+/* Rows of k at and past `from` of a block's chunks (m or n contiguous) become
  * zero, up to the next 16; by a warp. */
 __device__ __forceinline__ void clear_past(unsigned char *at, int chunks, int from, int lane) {
     const int rows = (from + 15) / 16 * 16 - from, words = rows * 8; /* of 16 bytes */
@@ -244,10 +260,12 @@ __device__ __forceinline__ void clear_past(unsigned char *at, int chunks, int fr
 }
 
 template <class Job, int NT, int PLANES, bool I8, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<NT, PLANES, PAIR>::kThreads, 1)
 tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Job job) {
     using S = Shape<NT, PLANES, PAIR>;
-    constexpr int kDepth = I8 ? 128 : 64, kStep = I8 ? 32 : 16; /* of k: in a stage, in an instruction */
+    constexpr int kBlock = I8 ? 128 : 64, kStep = I8 ? 32 : 16; /* of k: in a block, in an instruction */
+    constexpr int kDepth = S::kBlocks * kBlock;                 /* in a stage */
+    constexpr int kParts = S::kBlocks * PLANES;
     constexpr bool kSums = PLANES > 1;                          /* of segments, in registers */
     constexpr int kCtas = PAIR ? 2 : 1;
     constexpr int kBChunks = (S::kPart + kChunk - 1) / kChunk;
@@ -266,7 +284,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             mbar_init(smem_addr(&empty[i]), 1);
             mbar_init(smem_addr(&tail[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&done[i]), 1), mbar_init(smem_addr(&freed[i]), kCtas * kStoreWarps);
+        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&done[i]), 1), mbar_init(smem_addr(&freed[i]), kCtas * S::kStoreWarps);
         gave_up = 0;
         tb_pipe::fence_mbar_init();
     }
@@ -281,99 +299,100 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     const int tiles = job.tiles(shared), start = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
     /* Whether a stage's last rows of k belong to another matrix. */
     const auto ends_inside = [&](int left) { return Job::kRagged && left < kDepth && left % kStep != 0; };
-    if (warp == 0) {
-        uint32_t n = 0; /* stages asked for */
-        bool ok = true;
-        for (int t = start; ok && t < tiles; t += stride) {
-            const Tile tile = job.tile(shared, t);
-            const int m0 = tile.m0 + static_cast<int>(rank) * kRows;
-            const int n0 = tile.n0 + static_cast<int>(rank) * ((tile.columns + 15) / 16 * 8);
-            for (int k = 0; k < tile.depth; k += kDepth, ++n) {
-                const int s = n % S::kStages;
-                if (n >= S::kStages && !(ok = w.wait(smem_addr(&empty[s]), (n / S::kStages - 1) & 1))) break;
-                if (elected()) {
-                    uint32_t bar = smem_addr(&full[s]), at = smem_addr(stages + s * S::kStage);
-                    if (PAIR && !first) {
-                        if (ends_inside(tile.depth - k)) { /* this CTA clears its own rows, and then says so */
-                            bar = smem_addr(&tail[s]);
-                            mbar_arrive_expect_tx(bar, S::kStage);
-                        } else {
-                            bar = in_first(bar);
-                            remote_arrive_expect_tx(bar, S::kStage);
-                        }
-                    } else {
-                        mbar_arrive_expect_tx(bar, S::kStage);
-                    }
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p, at += S::kABytes) {
-                        const int z = tile.az + p * ops.a_plane;
-                        if (ops.a_outer) {
-                            load_box<PAIR>(at, &ops.a, m0, tile.k0 + k, z, bar);
-                            load_box<PAIR>(at + kChunkBytes, &ops.a, m0 + kChunk, tile.k0 + k, z, bar);
-                        } else {
-                            load_box<PAIR>(at, &ops.a, tile.k0 + k, m0, z, bar);
-                        }
-                    }
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p, at += S::kBBytes) {
-                        const int z = tile.bz + p * ops.b_plane;
-                        if (ops.b_outer) {
-#pragma unroll
-                            for (int c = 0; c < kBChunks; ++c)
-                                load_box<PAIR>(at + c * kChunkBytes, &ops.b, n0 + c * kChunk, tile.k0 + k, z, bar);
-                        } else {
-                            load_box<PAIR>(at, &ops.b, tile.k0 + k, n0, z, bar);
-                        }
-                    }
-                }
-                __syncwarp();
-            }
-        }
-        /* copies land before the CTA leaves, also where the products gave up on them (a pair's
-         * are all counted by its first CTA, and both leave together) */
-        if (first)
-            for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
-                tb_pipe::mbar_wait(smem_addr(&full[i % S::kStages]), (i / S::kStages) & 1, kWaitNs);
-    } else if (warp == 1 && first) {
-        uint32_t n = 0, number = 0; /* stages taken, accumulators begun */
-        bool ok = true;
-        for (int t = start; ok && t < tiles; t += stride) {
-            const Tile tile = job.tile(shared, t);
-            const uint32_t how =
-                product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, (tile.columns + 15) / 16 * 16);
-            uint32_t d = 0;
-            for (int k = 0, in = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++in) {
-                if (k == 0 || (kSums && in == kSegment)) { /* the next accumulator */
-                    in = 0;
-                    const uint32_t buffer = number & 1;
-                    d = tmem + buffer * 256;
-                    if (number >= 2 && !(ok = w.wait(smem_addr(&freed[buffer]), (number / 2 - 1) & 1))) break;
-                    tensor_fence_after();
-                    ++number;
-                }
-                const int s = n % S::kStages, left = tile.depth - k;
-                if (left > 0) {
-                    if (!(ok = w.wait(smem_addr(&full[s]), (n / S::kStages) & 1))) break;
-                    unsigned char *at = stages + s * S::kStage;
-                    if (ends_inside(left)) {
-                        clear_past(at, PLANES * (kRows / kChunk), left, lane);
-                        clear_past(at + PLANES * S::kABytes, PLANES * kBChunks, left, lane);
-                    }
-                    tensor_fence_after();
+    /* Those rows, in the block that they lie in; by a warp. */
+    const auto clear_end = [&](unsigned char *at, int left) {
+        static_assert(S::kBlocks == 1 || PLANES == 1, "blocks of one plane, or planes of one block");
+        const int block = S::kBlocks > 1 ? left / kBlock : 0, from = left - block * kBlock, n = kParts / S::kBlocks;
+        clear_past(at + block * S::kABytes, n * (kRows / kChunk), from, lane);
+        clear_past(at + kParts * S::kABytes + block * S::kBBytes, n * kBChunks, from, lane);
+    };
+    if (warp < S::kFirstStore) {
+        if constexpr (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
+        if (warp == 0) {
+            uint32_t n = 0; /* stages asked for */
+            bool ok = true;
+            for (int t = start; ok && t < tiles; t += stride) {
+                const Tile tile = job.tile(shared, t);
+                const int m0 = tile.m0 + static_cast<int>(rank) * kRows;
+                const int n0 = tile.n0 + static_cast<int>(rank) * ((tile.columns + 15) / 16 * 8);
+                for (int k = 0; k < tile.depth; k += kDepth, ++n) {
+                    const int s = n % S::kStages;
+                    if (n >= S::kStages && !(ok = w.wait(smem_addr(&empty[s]), (n / S::kStages - 1) & 1))) break;
                     if (elected()) {
-                        const int steps = min(kDepth, left + kStep - 1) / kStep;
-                        const uint32_t ia = (ops.a_outer ? kStep * kBlockBytes : 32) >> 4, ib = (ops.b_outer ? kStep * kBlockBytes : 32) >> 4;
-                        bool add = in > 0;
-                        /* planes i and j count while i + j < PLANES: the small products first */
+                        uint32_t bar = smem_addr(&full[s]), at = smem_addr(stages + s * S::kStage);
+                        if (PAIR && !first) {
+                            if (ends_inside(tile.depth - k)) { /* this CTA clears its own rows, and then says so */
+                                bar = smem_addr(&tail[s]);
+                                mbar_arrive_expect_tx(bar, S::kStage);
+                            } else {
+                                bar = in_first(bar);
+                                remote_arrive_expect_tx(bar, S::kStage);
+                            }
+                        } else {
+                            mbar_arrive_expect_tx(bar, S::kStage);
+                        }
 #pragma unroll
-                        for (int small = PLANES - 1; small >= 0; --small)
+                        for (int p = 0; p < kParts; ++p, at += S::kABytes) {
+                            const int z = tile.az + (p % PLANES) * ops.a_plane, at_k = tile.k0 + k + p / PLANES * kBlock;
+                            if (ops.a_outer) {
+                                load_box<PAIR>(at, &ops.a, m0, at_k, z, bar);
+                                load_box<PAIR>(at + kChunkBytes, &ops.a, m0 + kChunk, at_k, z, bar);
+                            } else {
+                                load_box<PAIR>(at, &ops.a, at_k, m0, z, bar);
+                            }
+                        }
 #pragma unroll
-                            for (int p = 0; p <= small; ++p) {
-                                uint64_t a = operand(smem_addr(at + p * S::kABytes), ops.a_outer);
-                                uint64_t b = operand(smem_addr(at + PLANES * S::kABytes + (small - p) * S::kBBytes), ops.b_outer);
-                                if (steps == kDepth / kStep) {
+                        for (int p = 0; p < kParts; ++p, at += S::kBBytes) {
+                            const int z = tile.bz + (p % PLANES) * ops.b_plane, at_k = tile.k0 + k + p / PLANES * kBlock;
+                            if (ops.b_outer) {
 #pragma unroll
-                                    for (int i = 0; i < kDepth / kStep; ++i) {
+                                for (int c = 0; c < kBChunks; ++c)
+                                    load_box<PAIR>(at + c * kChunkBytes, &ops.b, n0 + c * kChunk, at_k, z, bar);
+                            } else {
+                                load_box<PAIR>(at, &ops.b, at_k, n0, z, bar);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            /* copies land before the CTA leaves, also where the products gave up on them (a pair's
+             * are all counted by its first CTA, and both leave together) */
+            if (first)
+                for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
+                    tb_pipe::mbar_wait(smem_addr(&full[i % S::kStages]), (i / S::kStages) & 1, kWaitNs);
+        } else if (warp == 1 && first) {
+            uint32_t n = 0, number = 0; /* stages taken, accumulators begun */
+            bool ok = true;
+            for (int t = start; ok && t < tiles; t += stride) {
+                const Tile tile = job.tile(shared, t);
+                const uint32_t how =
+                    product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, (tile.columns + 15) / 16 * 16);
+                uint32_t d = 0;
+                for (int k = 0, in = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++in) {
+                    if (k == 0 || (kSums && in == kSegment)) { /* the next accumulator */
+                        in = 0;
+                        const uint32_t buffer = number & 1;
+                        d = tmem + buffer * 256;
+                        if (number >= 2 && !(ok = w.wait(smem_addr(&freed[buffer]), (number / 2 - 1) & 1))) break;
+                        tensor_fence_after();
+                        ++number;
+                    }
+                    const int s = n % S::kStages, left = tile.depth - k;
+                    if (left > 0) {
+                        if (!(ok = w.wait(smem_addr(&full[s]), (n / S::kStages) & 1))) break;
+                        unsigned char *at = stages + s * S::kStage;
+                        if (ends_inside(left)) clear_end(at, left);
+                        tensor_fence_after();
+                        if (elected()) {
+                            const uint32_t ia = (ops.a_outer ? kStep * kBlockBytes : 32) >> 4, ib = (ops.b_outer ? kStep * kBlockBytes : 32) >> 4;
+                            bool add = in > 0;
+                            const auto multiply = [&](int pa, int pb, int steps) {
+                                uint64_t a = operand(smem_addr(at + pa * S::kABytes), ops.a_outer);
+                                uint64_t b = operand(smem_addr(at + kParts * S::kABytes + pb * S::kBBytes), ops.b_outer);
+                                if (steps >= kBlock / kStep) {
+#pragma unroll
+                                    for (int i = 0; i < kBlock / kStep; ++i) {
                                         tensor_product<I8, PAIR>(d, a + i * ia, b + i * ib, how, add);
                                         add = true;
                                     }
@@ -383,44 +402,55 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                                         add = true;
                                     }
                                 }
+                            };
+                            const int steps = (left + kStep - 1) / kStep;
+                            if constexpr (PLANES == 1) {
+#pragma unroll
+                                for (int j = 0; j < S::kBlocks; ++j) multiply(j, j, steps - j * (kBlock / kStep));
+                            } else { /* planes i and j count while i + j < PLANES: the small products first */
+#pragma unroll
+                                for (int small = PLANES - 1; small >= 0; --small)
+#pragma unroll
+                                    for (int p = 0; p <= small; ++p) multiply(p, small - p, steps);
                             }
-                        tensor_commit<PAIR>(smem_addr(&empty[s]));
+                            tensor_commit<PAIR>(smem_addr(&empty[s]));
+                        }
+                        __syncwarp();
+                        ++n;
                     }
-                    __syncwarp();
-                    ++n;
-                }
-                if (left <= kDepth || (kSums && in == kSegment - 1)) {
-                    if (elected()) tensor_commit<PAIR>(smem_addr(&done[(number - 1) & 1]));
-                    __syncwarp();
+                    if (left <= kDepth || (kSums && in == kSegment - 1)) {
+                        if (elected()) tensor_commit<PAIR>(smem_addr(&done[(number - 1) & 1]));
+                        __syncwarp();
+                    }
                 }
             }
-        }
-        /* products end before the TMEM is freed, also where the storing warps gave up on them */
-        if (n > 0) tb_pipe::mbar_wait(smem_addr(&empty[(n - 1) % S::kStages]), ((n - 1) / S::kStages) & 1, kWaitNs);
-    } else if (warp == 1) {
-        if (Job::kRagged) { /* the second CTA's rows past a matrix's end, stage by stage as the first takes them */
-            uint32_t n = 0, phases = 0; /* a bit for each stage */
-            bool ok = true;
-            for (int t = start; ok && t < tiles; t += stride) {
-                const Tile tile = job.tile(shared, t);
-                for (int k = 0; k < tile.depth; k += kDepth, ++n) {
-                    if (!ends_inside(tile.depth - k)) continue;
-                    const int s = n % S::kStages;
-                    if (!(ok = w.wait(smem_addr(&tail[s]), phases >> s & 1))) { /* the copies land all the same */
-                        tb_pipe::mbar_wait(smem_addr(&tail[s]), phases >> s & 1, kWaitNs);
-                        break;
+            /* products end before the TMEM is freed, also where the storing warps gave up on them */
+            if (n > 0) tb_pipe::mbar_wait(smem_addr(&empty[(n - 1) % S::kStages]), ((n - 1) / S::kStages) & 1, kWaitNs);
+        } else if (warp == 1) {
+            if (Job::kRagged) { /* the second CTA's rows past a matrix's end, stage by stage as the first takes them */
+                uint32_t n = 0, phases = 0; /* a bit for each stage */
+                bool ok = true;
+                for (int t = start; ok && t < tiles; t += stride) {
+                    const Tile tile = job.tile(shared, t);
+                    for (int k = 0; k < tile.depth; k += kDepth, ++n) {
+                        if (!ends_inside(tile.depth - k)) continue;
+                        const int s = n % S::kStages;
+                        if (!(ok = w.wait(smem_addr(&tail[s]), phases >> s & 1))) { /* the copies land all the same */
+                            tb_pipe::mbar_wait(smem_addr(&tail[s]), phases >> s & 1, kWaitNs);
+                            break;
+                        }
+                        phases ^= 1u << s;
+                        unsigned char *at = stages + s * S::kStage;
+                        clear_end(at, tile.depth - k);
+                        if (lane == 0) remote_arrive(in_first(smem_addr(&full[s])));
+                        __syncwarp();
                     }
-                    phases ^= 1u << s;
-                    unsigned char *at = stages + s * S::kStage;
-                    clear_past(at, PLANES * (kRows / kChunk), tile.depth - k, lane);
-                    clear_past(at + PLANES * S::kABytes, PLANES * kBChunks, tile.depth - k, lane);
-                    if (lane == 0) remote_arrive(in_first(smem_addr(&full[s])));
-                    __syncwarp();
                 }
             }
         }
     } else {
-        const int part = warp % 4, half = (warp - 2) / 4; /* the lanes of TMEM that this warp may read; its columns */
+        if constexpr (S::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kStoreRegisters));
+        const int part = warp % 4, share = (warp - S::kFirstStore) / 4; /* the lanes of TMEM that this warp may read; its columns */
         const uint32_t lanes = static_cast<uint32_t>(part) << 21;
         uint32_t number = 0;
         bool ok = true;
@@ -435,36 +465,36 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
         for (int t = start; ok && t < tiles; t += stride) {
             const Tile tile = job.tile(shared, t);
             const int m = tile.m0 + static_cast<int>(rank) * kRows + part * 32 + lane;
-            const int c0 = half * S::kHalf, columns = NT >= 64 || half == 0 ? min(tile.columns - c0, S::kHalf) : 0;
+            const int c0 = share * S::kShare, columns = min(tile.columns - c0, S::kShare);
             if constexpr (kSums) {
-                float sum[S::kHalf];
+                float sum[S::kShare];
+#pragma unroll
+                for (int i = 0; i < S::kShare; ++i) sum[i] = 0.0f;
                 for (int k = 0; ok && (k < tile.depth || k == 0); k += kSegment * kDepth, ++number) {
                     const uint32_t buffer = number & 1;
                     if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
                     tensor_fence_after();
+                    if (tile.depth > 0) {
 #pragma unroll
-                    for (int c = 0; c < S::kHalf; c += 32) {
-                        if (c < columns && tile.depth > 0) {
-                            uint32_t r[32];
+                        for (int c = 0; c < S::kShare; c += 16) { /* columns past the tile's are read too, and not stored */
+                            uint32_t r[16];
                             tensor_load(tmem + buffer * 256 + lanes + c0 + c, r);
                             tensor_wait_load();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[c + i] = k == 0 ? __uint_as_float(r[i]) : sum[c + i] + __uint_as_float(r[i]);
-                        } else if (k == 0) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[c + i] = 0.0f;
+                            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
                         }
                     }
                     free(buffer);
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < S::kHalf; c += 32)
+                for (int c = 0; c < S::kShare; c += 8)
                     if (c < columns) {
-                        uint32_t r[32];
+                        uint32_t r[8];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sum[c + i]);
+                        for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[c + i]);
                         job.store(shared, tile, m, c0 + c, r);
+                        asm volatile("" ::: "memory"); /* the next eight's loads stay behind: they would take registers that the sums need */
                     }
             } else {
                 const uint32_t buffer = number & 1;
@@ -479,7 +509,13 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
 #pragma unroll
                         for (int i = 0; i < 32; ++i) r[i] = 0;
                     }
-                    job.store(shared, tile, m, c0 + c, r);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t eight[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) eight[j] = r[i + j];
+                        if (c + i < columns) job.store(shared, tile, m, c0 + c + i, eight);
+                    }
                 }
                 free(buffer);
                 ++number;
@@ -554,10 +590,20 @@ int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, 
     constexpr auto kernel = tensor_products<Job, NT, PLANES, I8, PAIR>;
     constexpr int kCtas = PAIR ? 2 : 1, kShared = Shape<NT, PLANES, PAIR>::kShared;
     if (!tb_learn::allow_shared<tensor_products<Job, NT, PLANES, I8, PAIR>>(kShared)) return 0;
+    if constexpr (Shape<NT, PLANES, PAIR>::kWide) { /* warps that ask for more than the launch gave would wait forever */
+        static std::atomic<int> registers{0};
+        int n = registers.load(std::memory_order_relaxed);
+        if (n == 0) {
+            cudaFuncAttributes a;
+            if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) return 0;
+            registers.store(n = a.numRegs, std::memory_order_relaxed);
+        }
+        if (n < Shape<NT, PLANES, PAIR>::kLaunchRegisters) return 0;
+    }
     const size_t most = static_cast<size_t>(sms) / kCtas;
     cudaLaunchConfig_t config{};
     config.gridDim = static_cast<unsigned>(tiles < most ? tiles : most) * kCtas;
-    config.blockDim = kThreads;
+    config.blockDim = Shape<NT, PLANES, PAIR>::kThreads;
     config.dynamicSmemBytes = kShared;
     config.stream = st;
     cudaLaunchAttribute attribute;
