@@ -47,6 +47,7 @@ template <class T> __device__ __forceinline__ T stored(uint32_t r) { return from
 
 template <class T, int NT> struct RowJob {
     static constexpr bool kRagged = false;
+    static constexpr int kStaging = 0;
     struct Shared {
         int first[kMaxExperts + 1]; /* tile of rows that each expert's start with */
         int start[kMaxExperts], end[kMaxExperts];
@@ -126,6 +127,7 @@ template <class T, int NT> struct IntegerJob : RowJob<T, NT> {
 
 template <class T, int NT> struct SumJob {
     static constexpr bool kRagged = true;
+    static constexpr int kStaging = 0;
     struct Shared {};
     Runs runs;
     int width, height, tile_m, tiles_m, tiles_n;

@@ -32,20 +32,6 @@ constexpr float kDown = 1.0f / 4096.0f;
 struct Pair {
     __half *at;
     size_t line, matrix, plane;
-    /* Eight values `line` apart, all under way before the first is used. */
-    __device__ __forceinline__ void get(size_t i, int count, float (&v)[8]) const {
-        __half high[8], low[8];
-        const __half *from = at + i;
-#pragma unroll
-        for (int j = 0; j < 8; ++j, from += line)
-            if (j < count) {
-                high[j] = from[0];
-                low[j] = from[plane];
-            }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < count) v[j] = __half2float(high[j]) + __half2float(low[j]);
-    }
     __device__ __forceinline__ void put(size_t i, float v) const {
         const __half high = __float2half_rn(v);
         at[i] = high;
@@ -138,7 +124,7 @@ struct Plan {
         r.az = r.bz = r.which = z;
         return r;
     }
-    /* Whether what lies across the diagonal from row m of the columns from c (32 of them) is in no tile. */
+    /* Whether what lies across the diagonal from row m of the 32 columns from c is in no tile. */
     __device__ __forceinline__ bool mirrored(const Tile &t, int m, int c) const {
         return symmetric && (t.n0 + c) / tile_m < first(m / tile_n);
     }
@@ -146,81 +132,100 @@ struct Plan {
 
 struct Nothing {};
 
+constexpr int kBoxBytes = 32 * 32 * sizeof(__half);
+
+/* 32 columns of 32 rows of the tensor cores as pairs, [column][row] (or
+ * [row][column]) in a warp's staging, and from there in whole boxes: to global
+ * memory directly, 64 bytes at a time, a tile's storing took twice as long. */
+struct Boxes {
+    int lane;
+    __half *at;
+    __device__ __forceinline__ float get(int i) const {
+        return __half2float(at[i * 32 + lane]) + __half2float(at[1024 + i * 32 + lane]);
+    }
+    __device__ __forceinline__ void put(int i, float v, __half *high, __half *low) const {
+        at[i * 32 + lane] = *high = __float2half_rn(v);
+        at[1024 + i * 32 + lane] = *low = __float2half_rn(v - __half2float(*high));
+    }
+    __device__ __forceinline__ void across(const __half (&high)[32], const __half (&low)[32]) const {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            Pack<__half, 8> h, l;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h.v[j] = high[i + j], l.v[j] = low[i + j];
+            *reinterpret_cast<Pack<__half, 8> *>(at + lane * 32 + i) = h;
+            *reinterpret_cast<Pack<__half, 8> *>(at + 1024 + lane * 32 + i) = l;
+        }
+    }
+};
+
 /* A = x x^T, or S = b A + c A A. */
 struct SquareJob {
     static constexpr bool kRagged = false;
+    static constexpr int kStaging = 2 * kBoxBytes;
     using Shared = Nothing;
+    CUtensorMap out, old; /* boxes of 32 x 32 */
     Plan plan;
-    Pair out, old; /* old.at NULL: A */
+    bool second; /* S */
     float b, c;
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
-        if (m >= plan.width) return;
-        const size_t base = t.which * out.matrix, at = base + (t.n0 + c0) * out.line + m;
-        const int count = t.columns - c0;
-        float v[8];
+    __device__ __forceinline__ bool store(const Tile &t, int m, int c0, float (&v)[32], tb_tensor::Staging &s) const {
+        const int x = m - s.lane, y = t.n0 + c0;
+        if (x >= plan.width) return true;
+        const Boxes boxes{s.lane, reinterpret_cast<__half *>(s.at)};
+        __half high[32], low[32];
+        if (second) {
+            if (!s.load(&old, x, y, t.which, plan.matrices, kBoxBytes)) return false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]) * kDown;
-        if (old.at) {
-            float was[8];
-            old.get(at, count, was);
+            for (int i = 0; i < 32; ++i) boxes.put(i, fmaf(c, v[i] * kDown, b * boxes.get(i)), &high[i], &low[i]);
+        } else {
+            s.free();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fmaf(c, v[i], b * was[i]);
+            for (int i = 0; i < 32; ++i) boxes.put(i, v[i] * kDown, &high[i], &low[i]);
         }
-        __half high[8], low[8], *to = out.at + at;
-#pragma unroll
-        for (int i = 0; i < 8; ++i, to += out.line) {
-            high[i] = __float2half_rn(v[i]);
-            low[i] = __float2half_rn(v[i] - __half2float(high[i]));
-            if (i < count) {
-                to[0] = high[i];
-                to[out.plane] = low[i];
-            }
+        s.store(&out, x, y, t.which, plan.matrices, kBoxBytes);
+        if (plan.mirrored(t, x, c0)) {
+            s.free();
+            boxes.across(high, low);
+            s.store(&out, y, x, t.which, plan.matrices, kBoxBytes);
         }
-        if (plan.mirrored(t, m, c0)) { /* 16 bytes at a time; a line's end is a multiple of eight */
-            __half *across = out.at + base + m * out.line + t.n0 + c0;
-            Pack<__half, 8> h, l;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h.v[i] = high[i], l.v[i] = low[i];
-            *reinterpret_cast<Pack<__half, 8> *>(across) = h;
-            *reinterpret_cast<Pack<__half, 8> *>(across + out.plane) = l;
-        }
+        return true;
     }
 };
 
 /* x = a x + S x; the last step's goes to the output. */
 template <class T> struct StepJob {
     static constexpr bool kRagged = false;
+    static constexpr int kStaging = 2 * kBoxBytes;
     using Shared = Nothing;
+    CUtensorMap x, next; /* boxes of 32 x 32 */
     Plan plan;
-    Pair x, next;
     T *last; /* or NULL */
     size_t row_stride, matrix_stride;
     float a, scale;
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
-    __device__ __forceinline__ void store(const Shared &, const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
-        if (m >= plan.width) return;
-        const int count = t.columns - c0;
-        const size_t n = t.n0 + c0, at = t.which * x.matrix + n * x.line + m;
-        float v[8];
-        x.get(at, count, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(a, v[i], __uint_as_float(r[i]) * kDown);
+    __device__ __forceinline__ bool store(const Tile &t, int m, int c0, float (&v)[32], tb_tensor::Staging &s) const {
+        const int left = m - s.lane, y = t.n0 + c0;
+        if (left >= plan.width) return true;
+        const Boxes boxes{s.lane, reinterpret_cast<__half *>(s.at)};
+        if (!s.load(&x, left, y, t.which, plan.matrices, kBoxBytes)) return false;
         if (last) {
-            T *o = last + t.which * matrix_stride + n * row_stride + m;
+            T *o = last + t.which * matrix_stride + y * row_stride + m;
 #pragma unroll
-            for (int i = 0; i < 8; ++i, o += row_stride)
-                if (i < count) *o = from_float<T>(v[i] * kDown * scale);
+            for (int i = 0; i < 32; ++i, o += row_stride)
+                if (m < plan.width && c0 + i < t.columns) *o = from_float<T>(fmaf(a, boxes.get(i), v[i] * kDown) * kDown * scale);
+            __syncwarp(); /* the next boxes come where these were */
         } else {
-            size_t to = at;
+            __half high, low;
 #pragma unroll
-            for (int i = 0; i < 8; ++i, to += x.line)
-                if (i < count) next.put(to, v[i]);
+            for (int i = 0; i < 32; ++i) boxes.put(i, fmaf(a, boxes.get(i), v[i] * kDown), &high, &low);
+            s.store(&next, left, y, t.which, plan.matrices, kBoxBytes);
         }
+        return true;
     }
 };
 
@@ -314,7 +319,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         const int z = static_cast<int>(s.matrices), small = static_cast<int>(s.small);
         const int wide = static_cast<int>(s.columns), high = static_cast<int>(s.rows);
         for (int step = 0; step < desc->steps; ++step) {
-            const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns);
+            const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns), mn = matrices_of(next, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
             const int squared = with_tile(s.small, s.small, s.tall, [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
@@ -322,17 +327,16 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                 SquareJob job{};
                 job.plan = Plan{z, small, small, s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, small > tb_tensor::kRows};
                 job.plan.count();
-                job.out = square;
                 const size_t tiles = static_cast<size_t>(z) * job.plan.per;
-                if (!tb_tensor::encode<NT, PAIR>(&ops, mx, s.tall, mx, s.tall) ||
+                if (!tb_tensor::encode<NT, PAIR>(&ops, mx, s.tall, mx, s.tall) || !tb_tensor::encode(&job.out, ma, 32, 32) ||
                     !tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st))
                     return 0;
                 job.plan.depth = small;
-                job.out = poly;
-                job.old = square;
+                job.old = job.out;
+                job.second = true;
                 job.b = desc->b;
                 job.c = desc->c;
-                return tb_tensor::encode<NT, PAIR>(&ops, ma, false, ma, false) &&
+                return tb_tensor::encode<NT, PAIR>(&ops, ma, false, ma, false) && tb_tensor::encode(&job.out, mp, 32, 32) &&
                                tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
                            ? 1 : 0;
             });
@@ -343,8 +347,6 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                 StepJob<T> job{};
                 job.plan = Plan{z, wide, high, small, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, false};
                 job.plan.count();
-                job.x = x;
-                job.next = next;
                 job.last = step + 1 == desc->steps ? static_cast<T *>(out) : nullptr;
                 job.row_stride = s.out_row;
                 job.matrix_stride = s.out_matrix;
@@ -354,6 +356,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                 /* x S: A is S (its own transpose), B is x; S x: A is x with its columns as m, B is S */
                 return (s.tall ? tb_tensor::encode<NT, PAIR>(&ops, mp, false, mx, false)
                                : tb_tensor::encode<NT, PAIR>(&ops, mx, true, mp, false)) &&
+                               tb_tensor::encode(&job.x, mx, 32, 32) && tb_tensor::encode(&job.next, mn, 32, 32) &&
                                tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
                            ? 1 : 0;
             });

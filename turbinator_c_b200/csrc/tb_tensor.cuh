@@ -28,7 +28,8 @@
  * 4e-6 to 2e-5 in results that f32 arithmetic has to 1e-6.
  *
  * A job says what its tiles are and stores them (struct Job: setup, tiles,
- * tile, store: eight columns of a row of the tensor core's).
+ * tile, store: eight columns of a row of the tensor core's; or, where kStaging
+ * is not 0, 32 columns of 32 rows by a warp with so many bytes of its own).
  *
  * Waits are bounded by a second; one that runs out reports
  * TB_FEATURE_STATUS_WAIT_TIMEOUT through the stream's status word, after which
@@ -207,7 +208,7 @@ struct Tile {
 
 /* ---- the kernel ---- */
 
-template <int NT, int PLANES, bool PAIR> struct Shape {
+template <int NT, int PLANES, bool PAIR, int STAGING = 0> struct Shape {
     static constexpr int kTileM = PAIR ? 2 * kRows : kRows;
     static constexpr int kPart = PAIR ? NT / 2 : NT; /* rows of B that a CTA brings */
     static constexpr int kABytes = kRows * kBlockBytes, kBBytes = kPart * kBlockBytes; /* of a block: 128 bytes of k */
@@ -216,13 +217,13 @@ template <int NT, int PLANES, bool PAIR> struct Shape {
     static constexpr int kBlocks = PLANES == 1 ? 2 : 1;
     static constexpr int kStage = kBlocks * PLANES * (kABytes + kBBytes);
     static constexpr int kStages = 196608 / kStage > 12 ? 12 : 196608 / kStage;
-    static constexpr int kShared = kStages * kStage + 1024; /* + alignment */
     /* Sums of 256 columns in registers: 128 each of eight warps, which take the registers that the others leave (216 and
      * 72 of 168 each); in sixteen warps of 96 registers the sums spilled and a tile's storing took four times as long. */
     static constexpr bool kWide = PLANES > 1 && NT == 256;
     static constexpr int kShare = kWide ? 128 : NT >= 128 ? 64 : 32; /* columns that a storing warp reads */
     static constexpr int kFirstStore = kWide ? 4 : 2, kStoreWarps = 4 * (NT / kShare);
     static constexpr int kThreads = 32 * (kFirstStore + kStoreWarps);
+    static constexpr int kShared = kStages * kStage + kStoreWarps * STAGING + 1024; /* + alignment */
     static constexpr int kLaunchRegisters = 168, kStoreRegisters = 216, kOtherRegisters = 72;
     static_assert(!kWide || kThreads * kLaunchRegisters == 32 * (kStoreWarps * kStoreRegisters + 4 * kOtherRegisters), "a split");
     static_assert(kStages >= 2, "a ring");
@@ -248,6 +249,47 @@ struct Waits {
     }
 };
 
+/* A storing warp's own shared memory, which bulk tensor copies fill and empty. */
+struct Staging {
+    unsigned char *at;
+    uint32_t bar, phase;
+    int lane;
+    const Waits *w;
+    /* What was put in has been read. */
+    __device__ __forceinline__ void free() const {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+    }
+    __device__ __forceinline__ void stored() const {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    /* Boxes of `bytes` of planes z and z + next; false where the wait for them ran out. */
+    __device__ __forceinline__ bool load(const CUtensorMap *map, int x, int y, int z, int next, int bytes) {
+        free();
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bar, 2 * bytes);
+            load_box<false>(smem_addr(at), map, x, y, z, bar);
+            load_box<false>(smem_addr(at) + bytes, map, x, y, z + next, bar);
+        }
+        const bool ok = w->wait(bar, phase);
+        if (!ok) tb_pipe::mbar_wait(bar, phase, kWaitNs); /* they land all the same */
+        phase ^= 1;
+        return ok;
+    }
+    /* The same out of shared memory, as this warp has written it. */
+    __device__ __forceinline__ void store(const CUtensorMap *map, int x, int y, int z, int next, int bytes) const {
+        tb_pipe::fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            for (int p = 0; p < 2; ++p)
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map),
+                             "r"(x), "r"(y), "r"(z + p * next), "r"(smem_addr(at) + p * bytes)
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+};
+
 /* Rows of k at and past `from` of a block's chunks (m or n contiguous) become
  * zero, up to the next 16; by a warp. */
 __device__ __forceinline__ void clear_past(unsigned char *at, int chunks, int from, int lane) {
@@ -262,7 +304,7 @@ __device__ __forceinline__ void clear_past(unsigned char *at, int chunks, int fr
 template <class Job, int NT, int PLANES, bool I8, bool PAIR>
 __global__ void __launch_bounds__(Shape<NT, PLANES, PAIR>::kThreads, 1)
 tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Job job) {
-    using S = Shape<NT, PLANES, PAIR>;
+    using S = Shape<NT, PLANES, PAIR, Job::kStaging>;
     constexpr int kBlock = I8 ? 128 : 64, kStep = I8 ? 32 : 16; /* of k: in a block, in an instruction */
     constexpr int kDepth = S::kBlocks * kBlock;                 /* in a stage */
     constexpr int kParts = S::kBlocks * PLANES;
@@ -273,6 +315,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     __shared__ uint64_t full[S::kStages], empty[S::kStages], done[2], freed[2], tail[S::kStages];
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up;
+    __shared__ uint64_t staged[S::kStoreWarps];
     __shared__ typename Job::Shared shared;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
@@ -285,6 +328,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             mbar_init(smem_addr(&tail[i]), 1);
         }
         for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&done[i]), 1), mbar_init(smem_addr(&freed[i]), kCtas * S::kStoreWarps);
+        if (Job::kStaging)
+            for (int i = 0; i < S::kStoreWarps; ++i) mbar_init(smem_addr(&staged[i]), 1);
         gave_up = 0;
         tb_pipe::fence_mbar_init();
     }
@@ -454,6 +499,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
         const uint32_t lanes = static_cast<uint32_t>(part) << 21;
         uint32_t number = 0;
         bool ok = true;
+        Staging staging{stages + S::kStages * S::kStage + (warp - S::kFirstStore) * Job::kStaging,
+                        smem_addr(&staged[warp - S::kFirstStore]), 0, lane, &w};
         const auto free = [&](uint32_t buffer) {
             tensor_fence_before();
             __syncwarp();
@@ -476,26 +523,37 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                     tensor_fence_after();
                     if (tile.depth > 0) {
 #pragma unroll
-                        for (int c = 0; c < S::kShare; c += 16) { /* columns past the tile's are read too, and not stored */
-                            uint32_t r[16];
+                        for (int c = 0; c < S::kShare; c += 32) { /* columns past the tile's are read too, and not stored */
+                            uint32_t r[32];
                             tensor_load(tmem + buffer * 256 + lanes + c0 + c, r);
                             tensor_wait_load();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
+                            for (int i = 0; i < 32; ++i) sum[c + i] += __uint_as_float(r[i]);
                         }
                     }
                     free(buffer);
                 }
                 if (!ok) break;
+                if constexpr (Job::kStaging != 0) {
 #pragma unroll
-                for (int c = 0; c < S::kShare; c += 8)
-                    if (c < columns) {
-                        uint32_t r[8];
+                    for (int c = 0; c < S::kShare; c += 32)
+                        if (ok && c < columns) {
+                            float v[32];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[c + i]);
-                        job.store(shared, tile, m, c0 + c, r);
-                        asm volatile("" ::: "memory"); /* the next eight's loads stay behind: they would take registers that the sums need */
-                    }
+                            for (int i = 0; i < 32; ++i) v[i] = sum[c + i];
+                            ok = job.store(tile, m, c0 + c, v, staging);
+                        }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < S::kShare; c += 8)
+                        if (c < columns) {
+                            uint32_t r[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[c + i]);
+                            job.store(shared, tile, m, c0 + c, r);
+                            asm volatile("" ::: "memory"); /* the next eight's loads stay behind: they would take registers that the sums need */
+                        }
+                }
             } else {
                 const uint32_t buffer = number & 1;
                 if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
@@ -521,6 +579,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 ++number;
             }
         }
+        if constexpr (Job::kStaging != 0) staging.stored();
     }
     __syncwarp();
     tensor_fence_before();
@@ -563,16 +622,16 @@ struct Matrices {
     }
 };
 
-/* Boxes of 128 bytes by `box_rows`. */
-inline bool encode(CUtensorMap *map, const Matrices &m, int box_rows) {
+/* Boxes of 128 bytes by `box_rows`, swizzled; or plain ones of box_width elements. */
+inline bool encode(CUtensorMap *map, const Matrices &m, int box_rows, int box_width = 0) {
     const EncodeTiled f = encoder();
     const cuuint64_t extent[3] = {m.width, m.rows, m.count};
     const cuuint64_t stride[2] = {m.row_stride * m.size, (m.count > 1 ? m.matrix_stride : m.row_stride) * m.size};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(kBlockBytes / m.size), static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_width ? box_width : kBlockBytes / m.size), static_cast<cuuint32_t>(box_rows), 1};
     const cuuint32_t one[3] = {1, 1, 1};
     return f && f(map, m.size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
                   const_cast<void *>(m.at), extent, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  box_width ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 /* Both operands' maps for tiles of NT columns (64 at least a CTA where n is contiguous in b). */
@@ -588,7 +647,7 @@ template <int NT, bool PAIR> bool encode(Operands *ops, const Matrices &a, bool 
 template <int NT, int PLANES, bool I8, bool PAIR, class Job>
 int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, cudaStream_t st) {
     constexpr auto kernel = tensor_products<Job, NT, PLANES, I8, PAIR>;
-    constexpr int kCtas = PAIR ? 2 : 1, kShared = Shape<NT, PLANES, PAIR>::kShared;
+    constexpr int kCtas = PAIR ? 2 : 1, kShared = Shape<NT, PLANES, PAIR, Job::kStaging>::kShared;
     if (!tb_learn::allow_shared<tensor_products<Job, NT, PLANES, I8, PAIR>>(kShared)) return 0;
     if constexpr (Shape<NT, PLANES, PAIR>::kWide) { /* warps that ask for more than the launch gave would wait forever */
         static std::atomic<int> registers{0};
