@@ -162,6 +162,13 @@ template <class T, int NT> struct SumJob {
 struct Layout {
     size_t width, rows, count, row_stride, matrix_stride; /* of the source */
     size_t line;                                          /* of the copy: a multiple of 16 bytes */
+    const void *from;
+    void *to;
+};
+constexpr int kMostLayouts = 3;
+struct Layouts {
+    Layout of[kMostLayouts];
+    int count;
 };
 
 /* A value's planes: three bf16 that sum to it (the first alone where it is no
@@ -175,23 +182,31 @@ __device__ __forceinline__ void planes_of(float v, __nv_bfloat16 (&p)[3]) {
 }
 
 constexpr int kLayThreads = 256;
+/* A warp a line at a time, two neighbours a lane; blockIdx.y: of the tensors. */
 template <class T>
-__global__ void __launch_bounds__(kLayThreads) lay_out(Layout d, const T *from, void *to) {
-    const size_t lines = d.rows * d.count, all = lines * d.line;
-    for (size_t i = static_cast<size_t>(blockIdx.x) * kLayThreads + threadIdx.x; i < all;
-         i += static_cast<size_t>(gridDim.x) * kLayThreads) {
-        const size_t row = i / d.line, c = i - row * d.line, z = row / d.rows, r = row - z * d.rows;
-        const bool in = c < d.width;
-        const T *at = from + z * d.matrix_stride + r * d.row_stride + c;
-        if constexpr (sizeof(T) == 4) {
-            __nv_bfloat16 p[3];
-            planes_of(in ? to_float(*at) : 0.0f, p);
+__global__ void __launch_bounds__(kLayThreads) lay_out(const __grid_constant__ Layouts all) {
+    const Layout &d = all.of[blockIdx.y];
+    const size_t lines = d.rows * d.count, plane = lines * d.line;
+    const int lane = threadIdx.x % 32;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * (kLayThreads / 32) + threadIdx.x / 32; i < lines;
+         i += static_cast<size_t>(gridDim.x) * (kLayThreads / 32)) {
+        const size_t z = d.count > 1 ? i / d.rows : 0, r = i - z * d.rows;
+        const T *from = static_cast<const T *>(d.from) + z * d.matrix_stride + r * d.row_stride;
+        for (size_t c = lane * 2; c < d.line; c += 64) { /* a line's length is even */
+            T v[2] = {};
+            if (c < d.width) v[0] = from[c];
+            if (c + 1 < d.width) v[1] = from[c + 1];
+            if constexpr (sizeof(T) == 4) {
+                __nv_bfloat16 p[2][3];
+                planes_of(v[0], p[0]);
+                planes_of(v[1], p[1]);
+                __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(d.to) + i * d.line + c;
 #pragma unroll
-            for (int j = 0; j < 3; ++j) static_cast<__nv_bfloat16 *>(to)[j * all + i] = p[j];
-        } else {
-            T v{};
-            if (in) v = *at;
-            static_cast<T *>(to)[i] = v;
+                for (int j = 0; j < 3; ++j)
+                    *reinterpret_cast<Pack<__nv_bfloat16, 2> *>(to + j * plane) = Pack<__nv_bfloat16, 2>{{p[0][j], p[1][j]}};
+            } else {
+                *reinterpret_cast<Pack<T, 2> *>(static_cast<T *>(d.to) + i * d.line + c) = Pack<T, 2>{{v[0], v[1]}};
+            }
         }
     }
 }
@@ -207,20 +222,24 @@ size_t laid_bytes(size_t width, size_t rows, size_t count, bool wide, size_t siz
     return align_up(line_of(width, size) * rows * count * (wide ? 3 : 1) * size, 256);
 }
 
-template <class T> int lay(const Source &s, size_t size, unsigned char **scratch, Matrices *m, cudaStream_t st) {
+/* Notes a tensor to be laid out, if it has to be. */
+template <class T> void lay(const Source &s, size_t size, unsigned char **scratch, Layouts *all, Matrices *m) {
     const bool wide = sizeof(T) == 4;
     *m = Matrices{s.at, s.width, s.rows, s.count, s.row_stride, s.matrix_stride, size};
-    if (!wide && m->straight()) return 1;
-    if (!*scratch) return 0;
-    const size_t line = line_of(s.width, size), all = line * s.rows * s.count;
-    const Layout d{s.width, s.rows, s.count, s.row_stride, s.matrix_stride, line};
-    const size_t blocks = (all + kLayThreads * 4 - 1) / (kLayThreads * 4);
-    lay_out<T><<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), kLayThreads, 0, st>>>(
-        d, static_cast<const T *>(s.at), *scratch);
-    if (!launched()) return 0;
+    if (!wide && m->straight()) return;
+    const size_t line = line_of(s.width, size);
+    all->of[all->count++] = Layout{s.width, s.rows, s.count, s.row_stride, s.matrix_stride, line, s.at, *scratch};
     *m = Matrices{*scratch, s.width, s.rows, s.count * (wide ? 3 : 1), line, line * s.rows, size};
     *scratch += laid_bytes(s.width, s.rows, s.count, wide, size);
-    return 1;
+}
+/* Lays out what has been noted, in one launch. */
+template <class T> int laid(const Layouts &all, int sms, cudaStream_t st) {
+    size_t most = 0;
+    for (int i = 0; i < all.count; ++i) most = std::max(most, all.of[i].rows * all.of[i].count);
+    if (!most) return 1;
+    const size_t blocks = std::min((most + kLayThreads / 32 - 1) / (kLayThreads / 32), static_cast<size_t>(sms) * 8);
+    lay_out<T><<<dim3(static_cast<unsigned>(blocks), all.count), kLayThreads, 0, st>>>(all);
+    return launched();
 }
 
 /* ---- shapes ---- */
@@ -266,27 +285,26 @@ Source w_of(const ProductShape &s, const void *w) {
 }
 size_t laid_room(const Source &s, bool wide) { return laid_bytes(s.width, s.rows, s.count, wide, 2); }
 
-/* Calls f with a tile's columns and whether two CTAs share it: twice the rows
- * of an expert on average, so that most experts are one tile, but no more than
- * 256; pairs where a tile of 256 x 256 has most of its m and n; a lone CTA's
- * three planes are too large for 256 columns. */
-template <int PLANES, class F> int with_tile(size_t width, size_t rows, F &&f) {
-    if (rows <= 16) return f(std::integral_constant<int, 32>{}, std::false_type{});
-    if (rows <= 32) return f(std::integral_constant<int, 64>{}, std::false_type{});
-    if (rows > 64 && width > tb_tensor::kRows) return f(std::integral_constant<int, 256>{}, std::true_type{});
-    if (rows <= 64 || PLANES == 3) return f(std::integral_constant<int, 128>{}, std::false_type{});
-    return f(std::integral_constant<int, PLANES == 3 ? 128 : 256>{}, std::false_type{});
-}
-
 int kind_of(int type) { return type == TB_TYPE_F16 ? 0 : 1; }
 int tiles_of(size_t width, int tile) { return static_cast<int>((width + tile - 1) / tile); }
+
+/* Tiles of rows: an expert's last is half full on average. */
+tb_tensor::Fit rows_fit(int planes, const Runs &runs, size_t width, int sms) {
+    const size_t average = (static_cast<size_t>(runs.rows) + runs.experts - 1) / runs.experts;
+    return tb_tensor::best_fit(planes, 32, average, sms, [&](int columns, int m) {
+        const size_t of_rows = runs.experts > 1 && average > static_cast<size_t>(columns)
+                                   ? static_cast<size_t>(runs.rows) / columns + runs.experts / 2
+                                   : (average + columns - 1) / columns * runs.experts;
+        return of_rows * tiles_of(width, m);
+    });
+}
 
 /* O [rows, width] of type T, from operands laid out. */
 template <class T>
 int rows_product(Operands ops, const Matrices &w, bool w_outer, const Matrices &x, const Runs &runs, size_t width,
                  size_t depth, void *out, size_t out_stride, int sms, cudaStream_t st) {
     constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-    return with_tile<PLANES>(width, runs.rows / runs.experts, [&](auto n, auto pair) {
+    return tb_tensor::with_fit<PLANES>(rows_fit(PLANES, runs, width, sms), [&](auto n, auto pair) {
         constexpr int NT = decltype(n)::value;
         constexpr bool PAIR = decltype(pair)::value;
         constexpr int TM = tb_tensor::Shape<NT, PLANES, PAIR>::kTileM;
@@ -327,7 +345,10 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
         using T = decltype(t);
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx;
-        return lay<T>(w_of(s, weight), 2, &scratch, &mw, st) && lay<T>(x_of(s, x), 2, &scratch, &mx, st) &&
+        Layouts all{};
+        lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
+        lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
+        return laid<T>(all, sms, st) &&
                rows_product<T>(ops, mw, !s.turned, mx, runs, s.out, s.in, y, s.y_stride, sms, st);
     });
 }
@@ -355,21 +376,24 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
         using T = decltype(t);
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx, my;
-        if (!lay<T>(y_of(s, dy), 2, &scratch, &my, st)) return 0;
-        if (dx) {
-            if (!lay<T>(w_of(s, weight), 2, &scratch, &mw, st) ||
-                !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, sms, st))
-                return 0;
-        }
+        Layouts all{};
+        lay<T>(y_of(s, dy), 2, &scratch, &all, &my);
+        if (dx) lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
+        if (dweight) lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
+        if (!laid<T>(all, sms, st)) return 0;
+        if (dx && !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, sms, st)) return 0;
         if (!dweight) return 1;
-        if (!lay<T>(x_of(s, x), 2, &scratch, &mx, st)) return 0;
         /* weights [in, out]: n counts in, m out; [out, in] the other way */
         const size_t width = s.turned ? s.in : s.out, height = s.turned ? s.out : s.in;
         constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-        return with_tile<PLANES>(width, std::max<size_t>(height, 33), [&](auto n, auto pair) { /* n contiguous: 64 columns at least */
+        const tb_tensor::Fit fit = tb_tensor::best_fit(PLANES, 64, height, sms, [&](int columns, int m) {
+            return s.experts * tiles_of(width, m) * tiles_of(height, columns);
+        });
+        return tb_tensor::with_fit<PLANES>(fit, [&](auto n, auto pair) {
             constexpr int NT = decltype(n)::value;
             constexpr bool PAIR = decltype(pair)::value;
             constexpr int TM = tb_tensor::Shape<NT, PLANES, PAIR>::kTileM;
+            if constexpr (NT < tb_tensor::kChunk) return 0;
             if (!tb_tensor::encode<NT, PAIR>(&ops, s.turned ? mx : my, true, s.turned ? my : mx, true)) return 0;
             ops.a_plane = ops.b_plane = 1;
             const int tiles_m = tiles_of(width, TM), tiles_n = tiles_of(height, NT);
@@ -503,12 +527,13 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     unsigned char *scratch = static_cast<unsigned char *>(workspace);
     Matrices mw, mx;
-    if (!lay<int8_t>({weight, s.in, s.out, s.experts, s.w_row, s.w_matrix}, 1, &scratch, &mw, st) ||
-        !lay<int8_t>({q, s.in, s.rows, 1, s.x_stride, 0}, 1, &scratch, &mx, st))
-        return 0;
+    Layouts all{};
+    lay<int8_t>({weight, s.in, s.out, s.experts, s.w_row, s.w_matrix}, 1, &scratch, &all, &mw);
+    lay<int8_t>({q, s.in, s.rows, 1, s.x_stride, 0}, 1, &scratch, &all, &mx);
+    if (!laid<int8_t>(all, sms, st)) return 0;
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return with_tile<1>(s.out, s.rows / s.experts, [&](auto n, auto pair) {
+        return tb_tensor::with_fit<1>(rows_fit(1, runs, s.out, sms), [&](auto n, auto pair) {
             constexpr int NT = decltype(n)::value;
             constexpr bool PAIR = decltype(pair)::value;
             constexpr int TM = tb_tensor::Shape<NT, 1, PAIR>::kTileM;

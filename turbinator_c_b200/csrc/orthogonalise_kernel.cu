@@ -16,6 +16,8 @@
  * steps of the quintic, so that plain bf16 products leave errors of 2 to 3 % in
  * the result and f16 ones 0.2 to 0.4 %, pairs 1e-6.
  */
+#include <algorithm>
+
 #include "tb_tensor.cuh"
 
 using namespace tb_learn;
@@ -42,23 +44,34 @@ struct Pair {
 /* ---- x = g / (|g| + epsilon) ---- */
 
 constexpr int kNormThreads = 256;
-constexpr size_t kMostParts = 64;
+constexpr size_t kMostParts = 128; /* of a matrix */
+constexpr size_t kPartValues = 8192;
 
 struct Given {
-    size_t rows, columns, matrix_stride, row_stride;
+    size_t rows, columns, matrix_stride, row_stride, rows_a_part;
+    int lanes; /* that take a row together, a power of two */
 };
 
-template <class T>
-__global__ void __launch_bounds__(kNormThreads) squares(Given d, size_t rows_a_part, const T *g, double *sums) {
+/* Calls f(row, column) for this lane's packs of the part of the matrix that blockIdx.x takes. */
+template <int PACK, class F> __device__ __forceinline__ void each_pack(const Given &d, F &&f) {
+    const size_t first = blockIdx.x * d.rows_a_part, last = min(first + d.rows_a_part, d.rows);
+    const unsigned team = threadIdx.x / d.lanes, teams = kNormThreads / d.lanes;
+    for (size_t r = first + team; r < last; r += teams)
+        for (size_t c = (threadIdx.x - team * d.lanes) * PACK; c < d.columns; c += static_cast<size_t>(d.lanes) * PACK) f(r, c);
+}
+
+/* The squares are summed in 64 bits: those of f32 may pass f32's range either way. */
+template <class T, int PACK>
+__global__ void __launch_bounds__(kNormThreads) squares(Given d, const T *g, double *sums) {
     __shared__ double parts[kNormThreads / 32];
     const T *from = g + blockIdx.y * d.matrix_stride;
-    const size_t first = blockIdx.x * rows_a_part, last = min(first + rows_a_part, d.rows);
     double s = 0.0;
-    for (size_t i = threadIdx.x; i < (last > first ? last - first : 0) * d.columns; i += kNormThreads) {
-        const size_t r = i / d.columns;
-        const double v = to_float(from[(first + r) * d.row_stride + i - r * d.columns]);
-        s += v * v;
-    }
+    each_pack<PACK>(d, [&](size_t r, size_t c) {
+        float e[PACK];
+        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + r * d.row_stride + c), e);
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) s = fma(static_cast<double>(e[i]), static_cast<double>(e[i]), s);
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = s;
@@ -69,25 +82,36 @@ __global__ void __launch_bounds__(kNormThreads) squares(Given d, size_t rows_a_p
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kNormThreads)
-normalise(Given d, size_t rows_a_part, const T *g, const double *sums, double epsilon, Pair x) {
+template <class T, int PACK>
+__global__ void __launch_bounds__(kNormThreads) normalise(Given d, const T *g, const double *sums, double epsilon, Pair x) {
     __shared__ double scale;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 32) {
         double s = 0.0;
-        for (unsigned i = 0; i < gridDim.x; ++i) s += sums[blockIdx.y * gridDim.x + i];
+        for (unsigned i = threadIdx.x; i < gridDim.x; i += 32) s += sums[blockIdx.y * gridDim.x + i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         /* nothing stays nothing; a matrix with an infinity or a NaN becomes NaN */
-        scale = s == 0.0 ? 0.0 : isfinite(s) ? kUp / (sqrt(s) + epsilon) : s - s;
+        if (threadIdx.x == 0) scale = s == 0.0 ? 0.0 : isfinite(s) ? kUp / (sqrt(s) + epsilon) : s - s;
     }
     __syncthreads();
     const double up = scale;
+    const float near = static_cast<float>(up); /* where f32 holds it, the products do too */
+    const bool plain = fabsf(near) < 1e30f && (near > 1e-30f || up == 0.0);
     const T *from = g + blockIdx.y * d.matrix_stride;
-    const size_t first = blockIdx.x * rows_a_part, last = min(first + rows_a_part, d.rows);
-    for (size_t i = threadIdx.x; i < (last > first ? last - first : 0) * d.columns; i += kNormThreads) {
-        const size_t r = i / d.columns, c = i - r * d.columns;
-        x.put(blockIdx.y * x.matrix + (first + r) * x.line + c,
-              static_cast<float>(static_cast<double>(to_float(from[(first + r) * d.row_stride + c])) * up));
-    }
+    __half *to = x.at + blockIdx.y * x.matrix;
+    each_pack<PACK>(d, [&](size_t r, size_t c) {
+        float e[PACK];
+        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + r * d.row_stride + c), e);
+        Pack<__half, PACK> high, low;
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) {
+            const float v = plain ? e[i] * near : static_cast<float>(static_cast<double>(e[i]) * up);
+            high.v[i] = __float2half_rn(v);
+            low.v[i] = __float2half_rn(v - __half2float(high.v[i]));
+        }
+        *reinterpret_cast<Pack<__half, PACK> *>(to + r * x.line + c) = high;
+        *reinterpret_cast<Pack<__half, PACK> *>(to + x.plane + r * x.line + c) = low;
+    });
 }
 
 /* ---- the products ---- */
@@ -267,13 +291,15 @@ Matrices matrices_of(const Pair &p, size_t matrices, size_t rows, size_t width) 
     return Matrices{p.at, width, rows, matrices * 2, p.line, p.matrix, 2};
 }
 
-/* Calls f with a tile's columns and whether two CTAs share it; 64 columns at
- * least where the other operand's lie contiguous. */
-template <class F> int with_tile(size_t height, size_t width, bool outer, F &&f) {
-    if (height <= 32 && !outer) return f(std::integral_constant<int, 32>{}, std::false_type{});
-    if (height <= 64) return f(std::integral_constant<int, 64>{}, std::false_type{});
-    if (height <= 128 || width <= tb_tensor::kRows) return f(std::integral_constant<int, 128>{}, std::false_type{});
-    return f(std::integral_constant<int, 256>{}, std::true_type{});
+/* Tiles that know which of them a symmetric product needs have 128 or 256 columns. */
+bool half_needed(size_t small, int columns) { return small > static_cast<size_t>(tb_tensor::kRows) && columns >= tb_tensor::kRows; }
+
+tb_tensor::Fit plan_fit(int matrices, size_t height, size_t width, bool square, bool outer, int sms) {
+    return tb_tensor::best_fit(2, outer ? 64 : 32, height, sms, [&](int columns, int m) {
+        Plan plan{matrices, static_cast<int>(width), static_cast<int>(height), 0, m, columns, square && half_needed(height, columns)};
+        plan.count();
+        return static_cast<size_t>(matrices) * plan.per;
+    });
 }
 
 } /* namespace */
@@ -307,25 +333,30 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
     ops.a_plane = ops.b_plane = static_cast<int>(s.matrices);
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        const Given given{s.rows, s.columns, s.in_matrix, s.in_row};
-        size_t parts = (s.rows * s.columns + 16383) / 16384;
-        if (parts > kMostParts) parts = kMostParts;
-        const size_t rows_a_part = (s.rows + parts - 1) / parts;
+        const int pack = pack_of(reinterpret_cast<uintptr_t>(g) | (s.in_row | s.columns | (s.matrices > 1 ? s.in_matrix : 0)) * size, size);
+        size_t parts = (s.rows * s.columns + kPartValues - 1) / kPartValues;
+        parts = std::min(parts, std::min(kMostParts, s.rows));
+        Given given{s.rows, s.columns, s.in_matrix, s.in_row, (s.rows + parts - 1) / parts, 1};
+        while (given.lanes < kNormThreads && static_cast<size_t>(given.lanes) * pack < s.columns) given.lanes *= 2;
         const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(s.matrices));
-        squares<T><<<grid, kNormThreads, 0, st>>>(given, rows_a_part, static_cast<const T *>(g), sums);
-        if (!launched()) return 0;
-        normalise<T><<<grid, kNormThreads, 0, st>>>(given, rows_a_part, static_cast<const T *>(g), sums, desc->epsilon, x);
-        if (!launched()) return 0;
+        const int normalised = with_pack<T>(pack, [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            squares<T, P><<<grid, kNormThreads, 0, st>>>(given, static_cast<const T *>(g), sums);
+            if (!launched()) return 0;
+            normalise<T, P><<<grid, kNormThreads, 0, st>>>(given, static_cast<const T *>(g), sums, desc->epsilon, x);
+            return launched();
+        });
+        if (!normalised) return 0;
         const int z = static_cast<int>(s.matrices), small = static_cast<int>(s.small);
         const int wide = static_cast<int>(s.columns), high = static_cast<int>(s.rows);
         for (int step = 0; step < desc->steps; ++step) {
             const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns), mn = matrices_of(next, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
-            const int squared = with_tile(s.small, s.small, s.tall, [&](auto n, auto pair) {
+            const int squared = tb_tensor::with_fit<2>(plan_fit(z, s.small, s.small, true, s.tall, sms), [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
                 constexpr bool PAIR = decltype(pair)::value;
                 SquareJob job{};
-                job.plan = Plan{z, small, small, s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, small > tb_tensor::kRows};
+                job.plan = Plan{z, small, small, s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, half_needed(s.small, NT)};
                 job.plan.count();
                 const size_t tiles = static_cast<size_t>(z) * job.plan.per;
                 if (!tb_tensor::encode<NT, PAIR>(&ops, mx, s.tall, mx, s.tall) || !tb_tensor::encode(&job.out, ma, 32, 32) ||
@@ -341,7 +372,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                            ? 1 : 0;
             });
             if (!squared) return 0;
-            const int stepped = with_tile(s.rows, s.columns, false, [&](auto n, auto pair) {
+            const int stepped = tb_tensor::with_fit<2>(plan_fit(z, s.rows, s.columns, false, false, sms), [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
                 constexpr bool PAIR = decltype(pair)::value;
                 StepJob<T> job{};

@@ -643,6 +643,48 @@ template <int NT, bool PAIR> bool encode(Operands *ops, const Matrices &a, bool 
            encode(&ops->b, b, b_outer ? kChunk : kPart);
 }
 
+/* ---- which tiles ---- */
+
+struct Fit {
+    int columns;
+    bool pair;
+};
+/* The tiles that should be done first: as many as there are go round the SMs in
+ * so many turns, and a turn takes as long as its products (two cycles a column
+ * and block of k, times the pairs of planes) or its copies (some 46 bytes a
+ * cycle and SM) do.  count(columns, m) says how many tiles of so many columns by
+ * m there are, `average` how many columns one has of them; least: 64 where n is
+ * contiguous in b. */
+template <class Count> Fit best_fit(int planes, int least, size_t average, int sms, Count &&count) {
+    Fit best{0, false};
+    double lowest = 0.0;
+    const auto consider = [&](int columns, bool pair) {
+        const double units = pair ? sms / 2 : sms, tiles = static_cast<double>(count(columns, pair ? 2 * kRows : kRows));
+        const double turns = static_cast<double>(static_cast<size_t>((tiles + units - 1) / units));
+        const double taken = average < static_cast<size_t>(columns) ? static_cast<double>(average) : columns;
+        const double products = 2.0 * taken * (planes * (planes + 1) / 2);
+        const double copies = planes * kBlockBytes * (kRows + columns / (pair ? 2.0 : 1.0)) / 46.0;
+        const double cost = turns * ((products > copies ? products : copies) + 40.0);
+        if (best.columns == 0 || cost < lowest) {
+            lowest = cost;
+            best = Fit{columns, pair};
+        }
+    };
+    consider(256, true);
+    if (planes == 1) consider(256, false);
+    for (int columns = 128; columns >= least; columns /= 2) consider(columns, false);
+    return best;
+}
+/* Calls f with the fit's columns and whether two CTAs share a tile, as constants. */
+template <int PLANES, class F> int with_fit(Fit fit, F &&f) {
+    if (fit.pair) return f(std::integral_constant<int, 256>{}, std::true_type{});
+    if constexpr (PLANES == 1)
+        if (fit.columns == 256) return f(std::integral_constant<int, 256>{}, std::false_type{});
+    if (fit.columns == 128) return f(std::integral_constant<int, 128>{}, std::false_type{});
+    if (fit.columns == 64) return f(std::integral_constant<int, 64>{}, std::false_type{});
+    return f(std::integral_constant<int, 32>{}, std::false_type{});
+}
+
 /* tiles: at most. */
 template <int NT, int PLANES, bool I8, bool PAIR, class Job>
 int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, cudaStream_t st) {
