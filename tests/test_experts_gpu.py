@@ -209,7 +209,8 @@ def test_product_gradient_is_the_difference():
 # ---- 8-bit products ----
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
-@pytest.mark.parametrize("rows,width,pad", [(1, 1, 0), (3, 7, 0), (5, 4096, 0), (64, 129, 3), (200, 1000, 8), (2, 20000, 0)])
+@pytest.mark.parametrize("rows,width,pad", [(1, 1, 0), (3, 7, 0), (5, 4096, 0), (64, 129, 3), (200, 1000, 8), (2, 20000, 0),
+                                            (2051, 33, 0), (3001, 512, 8), (2100, 4100, 0)])
 def test_quantise_is_its_definition(kind, rows, width, pad):
     x = _inside((rows, width), kind, pad, pad % 2)
     x.copy_(_normal(_gen(rows), rows, width, scale=3.0) * torch.logspace(-3, 3, rows, device="cuda")[:, None])

@@ -157,6 +157,150 @@ template <class T, int NT> struct SumJob {
     }
 };
 
+/* ---- few rows ---- */
+
+/* Where the rows are few, as in acting, the weights are what is read, once, and
+ * a product is a warp's sum over a row of weights, against up to four rows. */
+constexpr int kFewThreads = 256, kFewRows = 4;
+
+/* The dot product of 16 bytes (or 4, or an element) of weights and a row. */
+template <class T, int PACK> struct FewPack {
+    using Sum = float;
+    Held<T, PACK> h;
+    __device__ __forceinline__ void load(const T *p) { h = *reinterpret_cast<const Held<T, PACK> *>(p); }
+    __device__ __forceinline__ void load_once(const T *p) { h = tb_learn::load_once<T, PACK>(p); }
+    __device__ __forceinline__ float dot(const FewPack &o, float sum) const {
+        float a[PACK], b[PACK];
+        unpack(h, a);
+        unpack(o.h, b);
+#pragma unroll
+        for (int i = 0; i < PACK; ++i) sum = fmaf(a[i], b[i], sum);
+        return sum;
+    }
+};
+template <int PACK> struct FewPack<int8_t, PACK> {
+    using Sum = int;
+    static constexpr int kWords = PACK >= 4 ? PACK / 4 : 1;
+    int w[kWords];
+    __device__ __forceinline__ void load(const int8_t *p) {
+        if constexpr (PACK == 16) {
+            const int4 v = *reinterpret_cast<const int4 *>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (PACK == 4) {
+            w[0] = *reinterpret_cast<const int *>(p);
+        } else {
+            w[0] = *p;
+        }
+    }
+    __device__ __forceinline__ void load_once(const int8_t *p) {
+        if constexpr (PACK == 16) {
+            const int4 v = __ldcs(reinterpret_cast<const int4 *>(p));
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+            load(p);
+        }
+    }
+    __device__ __forceinline__ int dot(const FewPack &o, int sum) const {
+        if constexpr (PACK == 1) return sum + w[0] * o.w[0];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) sum = __dp4a(w[i], o.w[i], sum);
+        return sum;
+    }
+};
+
+struct FewShape {
+    int width, depth; /* of the output, of the sums */
+    size_t x_stride, w_row, w_matrix, out_stride;
+};
+
+/* W: of rows and weights, f32, bf16, f16 or 8 bits; T: of the output. */
+template <class W, class T, int PACK>
+__global__ void __launch_bounds__(kFewThreads)
+few_rows(FewShape d, Runs runs, const W *x, const W *weight, T *out, const float *row_scale, const float *channel_scale) {
+    using Sum = typename FewPack<W, PACK>::Sum;
+    constexpr int kAhead = 8; /* packs of a row of weights under way at once */
+    const int lane = threadIdx.x % 32, m = blockIdx.x * (kFewThreads / 32) + threadIdx.x / 32;
+    const int last = min(static_cast<int>(blockIdx.y + 1) * kFewRows, runs.rows);
+    after_earlier();
+    if (m >= d.width) return;
+    for (int row = blockIdx.y * kFewRows, count; row < last; row += count) {
+        int e = 0, start = 0, end = last; /* the row's expert and its run */
+        if (runs.experts == 1) { /* not waited for before the weights */
+            start = run_start(runs, 0);
+            end = run_end(runs, 0, start);
+            count = last - row;
+        } else {
+            e = -1;
+            for (int base = 0; base < runs.experts && e < 0; base += 32) {
+                const int mine = base + lane, from = mine < runs.experts ? run_start(runs, mine) : runs.rows;
+                const int to = mine < runs.experts ? run_end(runs, mine, from) : from;
+                const unsigned has = __ballot_sync(0xffffffffu, from <= row && row < to);
+                if (has) {
+                    e = base + __ffs(has) - 1;
+                    end = __shfl_sync(0xffffffffu, to, __ffs(has) - 1);
+                }
+            }
+            count = e < 0 ? 1 : min(end, last) - row;
+            if (e < 0) continue; /* no expert's: left as it was */
+        }
+        const W *w = weight + e * d.w_matrix + m * d.w_row, *from = x + row * d.x_stride;
+        Sum sum[kFewRows] = {};
+        for (int k = lane * PACK; k < d.depth; k += 32 * PACK * kAhead) {
+            FewPack<W, PACK> a[kAhead], b;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (k + i * 32 * PACK < d.depth) a[i].load_once(w + k + i * 32 * PACK);
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r)
+                if (r < count) {
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i)
+                        if (k + i * 32 * PACK < d.depth) {
+                            b.load(from + r * d.x_stride + k + i * 32 * PACK);
+                            sum[r] = a[i].dot(b, sum[r]);
+                        }
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+            if (lane == r && r < count && row + r >= start && row + r < end) {
+                float v = static_cast<float>(sum[r]);
+                if constexpr (std::is_same<W, int8_t>::value)
+                    v *= row_scale[row + r] * channel_scale[static_cast<size_t>(e) * d.width + m];
+                out[(row + r) * d.out_stride + m] = from_float<T>(v);
+            }
+        }
+    }
+}
+
+/* Up to eight rows, and some 2^25 products of theirs: 1 x 4,096 x 4,096 of 8 bits
+ * 6.6 us against 9.0 by tiles, of bf16 7.2 against 10.0, 8 x 1,024 x 1,024 4.4
+ * against 5.5; 4 x 4,096 x 4,096 12 against 9.  f32 weights are laid out as
+ * planes for the tensor cores, 16 bytes moved for each of 4: rows up to a dozen
+ * an expert (8 x 4,096 x 4,096: 32 us against 72). */
+bool few(size_t rows, size_t experts, size_t in, size_t out, bool wide) {
+    if (wide) return rows <= 12 * experts;
+    return rows <= 8 && static_cast<double>(rows) * in * out <= 33554432.0;
+}
+
+template <class W, class T>
+int few_product(const FewShape &d, const Runs &runs, const W *x, const W *weight, T *out, const float *row_scale,
+                const float *channel_scale, cudaStream_t st) {
+    const size_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) |
+                        (d.x_stride | d.w_row | d.w_matrix | static_cast<size_t>(d.depth)) * sizeof(W);
+    const dim3 grid(static_cast<unsigned>((d.width + kFewThreads / 32 - 1) / (kFewThreads / 32)),
+                    static_cast<unsigned>((runs.rows + kFewRows - 1) / kFewRows));
+    const auto launch = [&](auto p) {
+        return launch_early(few_rows<W, T, decltype(p)::value>, grid, kFewThreads, 0, 1, st, d, runs, x, weight, out, row_scale, channel_scale);
+    };
+    if (bits % 16 == 0) return launch(std::integral_constant<int, 16 / static_cast<int>(sizeof(W))>{});
+    if constexpr (sizeof(W) < 4)
+        if (bits % 4 == 0) return launch(std::integral_constant<int, 4 / static_cast<int>(sizeof(W))>{});
+    return launch(std::integral_constant<int, 1>{});
+}
+
 /* ---- laying operands out ---- */
 
 struct Layout {
@@ -289,32 +433,39 @@ int kind_of(int type) { return type == TB_TYPE_F16 ? 0 : 1; }
 int tiles_of(size_t width, int tile) { return static_cast<int>((width + tile - 1) / tile); }
 
 /* Tiles of rows: an expert's last is half full on average. */
-tb_tensor::Fit rows_fit(int planes, const Runs &runs, size_t width, int sms) {
-    const size_t average = (static_cast<size_t>(runs.rows) + runs.experts - 1) / runs.experts;
-    return tb_tensor::best_fit(planes, 32, average, sms, [&](int columns, int m) {
-        const size_t of_rows = runs.experts > 1 && average > static_cast<size_t>(columns)
-                                   ? static_cast<size_t>(runs.rows) / columns + runs.experts / 2
-                                   : (average + columns - 1) / columns * runs.experts;
-        return of_rows * tiles_of(width, m);
-    });
+tb_tensor::Fit rows_fit(int planes, size_t rows, size_t experts, size_t width, size_t blocks) {
+    const size_t average = (rows + experts - 1) / experts;
+    return tb_tensor::best_fit(
+        planes, 32, average, blocks, true,
+        [&](int columns, int m) {
+            const size_t of_rows = experts > 1 && average > static_cast<size_t>(columns) ? rows / columns + experts / 2
+                                                                                         : (average + columns - 1) / columns * experts;
+            return of_rows * tiles_of(width, m);
+        },
+        [&](int columns, int m) { return (rows / columns + experts) * tiles_of(width, m); });
+}
+tb_tensor::Fit sums_fit(int planes, size_t rows, size_t experts, size_t width, size_t height) {
+    const auto tiles = [&](int columns, int m) { return experts * tiles_of(width, m) * tiles_of(height, columns); };
+    return tb_tensor::best_fit(planes, 64, height, ((rows + experts - 1) / experts + 63) / 64, true, tiles, tiles);
 }
 
 /* O [rows, width] of type T, from operands laid out. */
 template <class T>
 int rows_product(Operands ops, const Matrices &w, bool w_outer, const Matrices &x, const Runs &runs, size_t width,
-                 size_t depth, void *out, size_t out_stride, int sms, cudaStream_t st) {
+                 size_t depth, void *out, size_t out_stride, void *sums, int sms, cudaStream_t st) {
     constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-    return tb_tensor::with_fit<PLANES>(rows_fit(PLANES, runs, width, sms), [&](auto n, auto pair) {
+    const tb_tensor::Fit fit = rows_fit(PLANES, runs.rows, runs.experts, width, (depth + 63) / 64);
+    ops.parts = fit.parts;
+    ops.sums = static_cast<uint32_t *>(sums);
+    return tb_tensor::with_fit<PLANES>(fit, [&](auto n, auto pair) {
         constexpr int NT = decltype(n)::value;
         constexpr bool PAIR = decltype(pair)::value;
         constexpr int TM = tb_tensor::Shape<NT, PLANES, PAIR>::kTileM;
         if (!tb_tensor::encode<NT, PAIR>(&ops, w, w_outer, x, false)) return 0;
         ops.a_plane = runs.experts;
         ops.b_plane = 1;
-        const int tiles_m = tiles_of(width, TM);
-        const RowJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(depth), TM, tiles_m, static_cast<T *>(out), out_stride};
-        return tb_tensor::launch_products<NT, PLANES, false, PAIR>(
-            ops, job, (static_cast<size_t>(runs.rows) / NT + runs.experts) * tiles_m, sms, st);
+        const RowJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(depth), TM, tiles_of(width, TM), static_cast<T *>(out), out_stride};
+        return tb_tensor::launch_products<NT, PLANES, false, PAIR>(ops, job, fit.tiles, sms, st);
     });
 }
 
@@ -323,7 +474,11 @@ int rows_product(Operands ops, const Matrices &w, bool w_outer, const Matrices &
 extern "C" size_t tb_cuda_experts_product_workspace(const tb_expert_product_desc *desc) {
     ProductShape s;
     if (!product_shape(desc, &s)) return 0;
-    return laid_room(x_of(s, nullptr), s.wide) + laid_room(y_of(s, nullptr), s.wide) + laid_room(w_of(s, nullptr), s.wide);
+    const int planes = s.wide ? 3 : 1;
+    const size_t sums = std::max({rows_fit(planes, s.rows, s.experts, s.out, (s.in + 63) / 64).room(),
+                                  rows_fit(planes, s.rows, s.experts, s.in, (s.out + 63) / 64).room(),
+                                  sums_fit(planes, s.rows, s.experts, s.turned ? s.in : s.out, s.turned ? s.out : s.in).room()});
+    return laid_room(x_of(s, nullptr), s.wide) + laid_room(y_of(s, nullptr), s.wide) + laid_room(w_of(s, nullptr), s.wide) + sums;
 }
 
 extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc, const void *x, const void *weight,
@@ -341,15 +496,18 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
     cudaGetLastError(); /* report these launches only */
     ops.type = kind_of(desc->type);
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
-    return with_type(desc->type, [&](auto t) {
+    return with_type(desc->type, [&](auto t) -> int {
         using T = decltype(t);
+        if (s.turned && few(s.rows, s.experts, s.in, s.out, s.wide))
+            return few_product<T, T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
+                                     static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), nullptr, nullptr, st);
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx;
         Layouts all{};
         lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
         lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
         return laid<T>(all, sms, st) &&
-               rows_product<T>(ops, mw, !s.turned, mx, runs, s.out, s.in, y, s.y_stride, sms, st);
+               rows_product<T>(ops, mw, !s.turned, mx, runs, s.out, s.in, y, s.y_stride, scratch, sms, st);
     });
 }
 
@@ -374,6 +532,13 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
+        if (dx && !s.turned && few(s.rows, s.experts, s.in, s.out, s.wide)) { /* weights' rows lie along this sum */
+            if (!few_product<T, T>({static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.w_row, s.w_matrix, s.dx_stride}, runs,
+                                   static_cast<const T *>(dy), static_cast<const T *>(weight), static_cast<T *>(dx), nullptr, nullptr, st))
+                return 0;
+            dx = nullptr;
+            if (!dweight) return 1;
+        }
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx, my;
         Layouts all{};
@@ -381,14 +546,14 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
         if (dx) lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
         if (dweight) lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
         if (!laid<T>(all, sms, st)) return 0;
-        if (dx && !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, sms, st)) return 0;
+        if (dx && !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, scratch, sms, st)) return 0;
         if (!dweight) return 1;
         /* weights [in, out]: n counts in, m out; [out, in] the other way */
         const size_t width = s.turned ? s.in : s.out, height = s.turned ? s.out : s.in;
         constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-        const tb_tensor::Fit fit = tb_tensor::best_fit(PLANES, 64, height, sms, [&](int columns, int m) {
-            return s.experts * tiles_of(width, m) * tiles_of(height, columns);
-        });
+        const tb_tensor::Fit fit = sums_fit(PLANES, s.rows, s.experts, width, height);
+        ops.parts = fit.parts;
+        ops.sums = reinterpret_cast<uint32_t *>(scratch);
         return tb_tensor::with_fit<PLANES>(fit, [&](auto n, auto pair) {
             constexpr int NT = decltype(n)::value;
             constexpr bool PAIR = decltype(pair)::value;
@@ -399,7 +564,7 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
             const int tiles_m = tiles_of(width, TM), tiles_n = tiles_of(height, NT);
             const SumJob<T, NT> job{runs, static_cast<int>(width), static_cast<int>(height), TM, tiles_m, tiles_n,
                                     static_cast<T *>(dweight), s.w_row, s.w_matrix};
-            return tb_tensor::launch_products<NT, PLANES, false, PAIR>(ops, job, s.experts * tiles_m * tiles_n, sms, st);
+            return tb_tensor::launch_products<NT, PLANES, false, PAIR>(ops, job, fit.tiles, sms, st);
         });
     });
 }
@@ -410,46 +575,68 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
-/* A CTA a row: its largest magnitude, then its values.  A row whose largest
- * magnitude has no finite reciprocal times 127 counts as zero; one with an
- * infinity or a NaN gets the scale NaN. */
-template <class T, int PACK>
+/* A team of a warp or a CTA a row: its largest magnitude, then its values, up
+ * to HELD packs a thread of which stay in registers.  A row whose largest magnitude
+ * has no finite reciprocal times 127 counts as zero; one with an infinity or a
+ * NaN gets the scale NaN. */
+template <class T, int PACK, int TEAM, int HELD>
 __global__ void __launch_bounds__(kQuantThreads)
-quantise_rows(size_t width, size_t x_stride, size_t q_stride, const T *x, int8_t *q, float *scale) {
+quantise_rows(size_t rows, size_t width, size_t x_stride, size_t q_stride, const T *x, int8_t *q, float *scale) {
     __shared__ float most[kQuantThreads / 32];
     __shared__ int wrong[kQuantThreads / 32];
-    const size_t row = blockIdx.x;
+    const size_t row = static_cast<size_t>(blockIdx.x) * (kQuantThreads / TEAM) + threadIdx.x / TEAM;
+    const unsigned lane = threadIdx.x % TEAM;
+    later_may_start();
+    if (TEAM == 32 && row >= rows) return;
     const T *from = x + row * x_stride;
     float m = 0.0f;
     bool bad = false;
-    for (size_t c = threadIdx.x * PACK; c < width; c += kQuantThreads * PACK) {
+    const auto look = [&](const Held<T, PACK> &h) {
         float e[PACK];
-        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + c), e);
+        unpack(h, e);
 #pragma unroll
         for (int i = 0; i < PACK; ++i) {
             m = fmaxf(m, fabsf(e[i]));
             bad |= !(fabsf(e[i]) <= 3.402823466e38f);
         }
-    }
+    };
+    const size_t first = static_cast<size_t>(lane) * PACK, step = TEAM * PACK;
+    Held<T, PACK> held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (first + i * step < width) held[i] = load_once<T, PACK>(from + first + i * step);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (first + i * step < width) look(held[i]);
+    for (size_t c = first + HELD * step; c < width; c += step) look(*reinterpret_cast<const Held<T, PACK> *>(from + c));
     m = warp_max(m);
     bad = __any_sync(0xffffffffu, bad);
-    if (threadIdx.x % 32 == 0) most[threadIdx.x / 32] = m, wrong[threadIdx.x / 32] = bad;
-    __syncthreads();
+    if constexpr (TEAM > 32) {
+        if (threadIdx.x % 32 == 0) most[threadIdx.x / 32] = m, wrong[threadIdx.x / 32] = bad;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kQuantThreads / 32; ++i) m = fmaxf(m, most[i]), bad |= wrong[i] != 0;
+        for (int i = 0; i < kQuantThreads / 32; ++i) m = fmaxf(m, most[i]), bad |= wrong[i] != 0;
+    }
     float up = __fmul_rn(__frcp_rn(m), 127.0f);
     const bool none = bad || !(up <= 3.402823466e38f);
     if (none) up = 0.0f;
-    for (size_t c = threadIdx.x * PACK; c < width; c += kQuantThreads * PACK) {
+    const auto put = [&](size_t c, const Held<T, PACK> &h) {
         float e[PACK];
-        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + c), e);
+        unpack(h, e);
         Pack<int8_t, PACK> out;
 #pragma unroll
         for (int i = 0; i < PACK; ++i) out.v[i] = none ? 0 : static_cast<int8_t>(__float2int_rn(e[i] * up));
         *reinterpret_cast<Pack<int8_t, PACK> *>(q + row * q_stride + c) = out;
-    }
-    if (threadIdx.x == 0) scale[row] = bad ? __int_as_float(0x7fc00000) : none ? 0.0f : __fdiv_rn(m, 127.0f);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (first + i * step < width) put(first + i * step, held[i]);
+    for (size_t c = first + HELD * step; c < width; c += step) put(c, *reinterpret_cast<const Held<T, PACK> *>(from + c));
+    if (lane == 0) scale[row] = bad ? __int_as_float(0x7fc00000) : none ? 0.0f : __fdiv_rn(m, 127.0f);
 }
+/* Rows for all warps of the GPU, each held by its warp: 16,384 x 4,096 bf16
+ * WARPUS us, a CTA a row 50. */
+constexpr size_t kQuantManyRows = 2048;
 
 struct IntegerShape {
     size_t rows, experts, in, out, x_stride, y_stride, w_row, w_matrix;
@@ -495,8 +682,14 @@ extern "C" int tb_cuda_quantise_rows_device(const tb_quantise_desc *desc, const 
                             (reinterpret_cast<uintptr_t>(q) | q_stride) * size;
         return with_pack<T>(pack_of(bits, size), [&](auto p) {
             constexpr int P = decltype(p)::value;
-            quantise_rows<T, P><<<static_cast<unsigned>(desc->rows), kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-                desc->width, x_stride, q_stride, static_cast<const T *>(x), q, scale);
+            const cudaStream_t st = static_cast<cudaStream_t>(stream);
+            constexpr int kTeams = kQuantThreads / 32;
+            if (desc->rows >= kQuantManyRows && desc->width <= static_cast<size_t>(32) * P * 16)
+                quantise_rows<T, P, 32, 16><<<static_cast<unsigned>((desc->rows + kTeams - 1) / kTeams), kQuantThreads, 0, st>>>(
+                    desc->rows, desc->width, x_stride, q_stride, static_cast<const T *>(x), q, scale);
+            else
+                quantise_rows<T, P, kQuantThreads, 4><<<static_cast<unsigned>(desc->rows), kQuantThreads, 0, st>>>(
+                    desc->rows, desc->width, x_stride, q_stride, static_cast<const T *>(x), q, scale);
             return launched();
         });
     });
@@ -505,7 +698,8 @@ extern "C" int tb_cuda_quantise_rows_device(const tb_quantise_desc *desc, const 
 extern "C" size_t tb_cuda_experts_product_i8_workspace(const tb_expert_product_i8_desc *desc) {
     IntegerShape s;
     if (!integer_shape(desc, &s)) return 0;
-    return laid_bytes(s.in, s.rows, 1, false, 1) + laid_bytes(s.in, s.out, s.experts, false, 1);
+    return laid_bytes(s.in, s.rows, 1, false, 1) + laid_bytes(s.in, s.out, s.experts, false, 1) +
+           rows_fit(1, s.rows, s.experts, s.out, (s.in + 127) / 128).room();
 }
 
 extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc *desc, const int8_t *q,
@@ -525,15 +719,24 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
     cudaGetLastError(); /* report these launches only */
     ops.type = 1;
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
+    if (few(s.rows, s.experts, s.in, s.out, false))
+        return with_type(desc->type, [&](auto t) {
+            using T = decltype(t);
+            return few_product<int8_t, T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
+                                          q, weight, static_cast<T *>(y), q_scale, weight_scale, st);
+        });
     unsigned char *scratch = static_cast<unsigned char *>(workspace);
     Matrices mw, mx;
     Layouts all{};
     lay<int8_t>({weight, s.in, s.out, s.experts, s.w_row, s.w_matrix}, 1, &scratch, &all, &mw);
     lay<int8_t>({q, s.in, s.rows, 1, s.x_stride, 0}, 1, &scratch, &all, &mx);
     if (!laid<int8_t>(all, sms, st)) return 0;
+    const tb_tensor::Fit fit = rows_fit(1, s.rows, s.experts, s.out, (s.in + 127) / 128);
+    ops.parts = fit.parts;
+    ops.sums = reinterpret_cast<uint32_t *>(scratch);
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        return tb_tensor::with_fit<1>(rows_fit(1, runs, s.out, sms), [&](auto n, auto pair) {
+        return tb_tensor::with_fit<1>(fit, [&](auto n, auto pair) {
             constexpr int NT = decltype(n)::value;
             constexpr bool PAIR = decltype(pair)::value;
             constexpr int TM = tb_tensor::Shape<NT, 1, PAIR>::kTileM;
@@ -544,7 +747,7 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
                                                               tiles_m, static_cast<T *>(y), s.y_stride};
             job.row_scale = q_scale;
             job.channel_scale = weight_scale;
-            return tb_tensor::launch_products<NT, 1, true, PAIR>(ops, job, (s.rows / NT + s.experts) * tiles_m, sms, st);
+            return tb_tensor::launch_products<NT, 1, true, PAIR>(ops, job, fit.tiles, sms, st);
         });
     });
 }

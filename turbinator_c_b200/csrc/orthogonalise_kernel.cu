@@ -44,31 +44,44 @@ struct Pair {
 /* ---- x = g / (|g| + epsilon) ---- */
 
 constexpr int kNormThreads = 256;
-constexpr size_t kMostParts = 128; /* of a matrix */
-constexpr size_t kPartValues = 8192;
+constexpr size_t kMostParts = 512; /* of a matrix */
+constexpr size_t kPartValues = 4096;
 
 struct Given {
     size_t rows, columns, matrix_stride, row_stride, rows_a_part;
     int lanes; /* that take a row together, a power of two */
 };
 
-/* Calls f(row, column) for this lane's packs of the part of the matrix that blockIdx.x takes. */
-template <int PACK, class F> __device__ __forceinline__ void each_pack(const Given &d, F &&f) {
+/* Calls f(row, column, values) for this lane's packs of the part of the matrix
+ * that blockIdx.x takes, four under way at once. */
+template <int PACK, class T, class F> __device__ __forceinline__ void each_pack(const Given &d, const T *from, F &&f) {
     const size_t first = blockIdx.x * d.rows_a_part, last = min(first + d.rows_a_part, d.rows);
-    const unsigned team = threadIdx.x / d.lanes, teams = kNormThreads / d.lanes;
+    const unsigned team = threadIdx.x / d.lanes, teams = kNormThreads / d.lanes, lane = threadIdx.x - team * d.lanes;
     for (size_t r = first + team; r < last; r += teams)
-        for (size_t c = (threadIdx.x - team * d.lanes) * PACK; c < d.columns; c += static_cast<size_t>(d.lanes) * PACK) f(r, c);
+        for (size_t c = lane * PACK; c < d.columns; c += static_cast<size_t>(d.lanes) * PACK * 4) {
+            Held<T, PACK> h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t at = c + static_cast<size_t>(i) * d.lanes * PACK;
+                if (at < d.columns) h[i] = *reinterpret_cast<const Held<T, PACK> *>(from + r * d.row_stride + at);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t at = c + static_cast<size_t>(i) * d.lanes * PACK;
+                float e[PACK];
+                if (at < d.columns) unpack(h[i], e), f(r, at, e);
+            }
+        }
 }
 
 /* The squares are summed in 64 bits: those of f32 may pass f32's range either way. */
 template <class T, int PACK>
 __global__ void __launch_bounds__(kNormThreads) squares(Given d, const T *g, double *sums) {
     __shared__ double parts[kNormThreads / 32];
+    later_may_start();
     const T *from = g + blockIdx.y * d.matrix_stride;
     double s = 0.0;
-    each_pack<PACK>(d, [&](size_t r, size_t c) {
-        float e[PACK];
-        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + r * d.row_stride + c), e);
+    each_pack<PACK>(d, from, [&](size_t, size_t, const float (&e)[PACK]) {
 #pragma unroll
         for (int i = 0; i < PACK; ++i) s = fma(static_cast<double>(e[i]), static_cast<double>(e[i]), s);
     });
@@ -85,6 +98,8 @@ __global__ void __launch_bounds__(kNormThreads) squares(Given d, const T *g, dou
 template <class T, int PACK>
 __global__ void __launch_bounds__(kNormThreads) normalise(Given d, const T *g, const double *sums, double epsilon, Pair x) {
     __shared__ double scale;
+    later_may_start();
+    after_earlier();
     if (threadIdx.x < 32) {
         double s = 0.0;
         for (unsigned i = threadIdx.x; i < gridDim.x; i += 32) s += sums[blockIdx.y * gridDim.x + i];
@@ -99,9 +114,7 @@ __global__ void __launch_bounds__(kNormThreads) normalise(Given d, const T *g, c
     const bool plain = fabsf(near) < 1e30f && (near > 1e-30f || up == 0.0);
     const T *from = g + blockIdx.y * d.matrix_stride;
     __half *to = x.at + blockIdx.y * x.matrix;
-    each_pack<PACK>(d, [&](size_t r, size_t c) {
-        float e[PACK];
-        unpack(*reinterpret_cast<const Held<T, PACK> *>(from + r * d.row_stride + c), e);
+    each_pack<PACK>(d, from, [&](size_t r, size_t c, const float (&e)[PACK]) {
         Pack<__half, PACK> high, low;
 #pragma unroll
         for (int i = 0; i < PACK; ++i) {
@@ -294,12 +307,13 @@ Matrices matrices_of(const Pair &p, size_t matrices, size_t rows, size_t width) 
 /* Tiles that know which of them a symmetric product needs have 128 or 256 columns. */
 bool half_needed(size_t small, int columns) { return small > static_cast<size_t>(tb_tensor::kRows) && columns >= tb_tensor::kRows; }
 
-tb_tensor::Fit plan_fit(int matrices, size_t height, size_t width, bool square, bool outer, int sms) {
-    return tb_tensor::best_fit(2, outer ? 64 : 32, height, sms, [&](int columns, int m) {
+tb_tensor::Fit plan_fit(int matrices, size_t height, size_t width, size_t depth, bool square, bool outer) {
+    const auto tiles = [&](int columns, int m) {
         Plan plan{matrices, static_cast<int>(width), static_cast<int>(height), 0, m, columns, square && half_needed(height, columns)};
         plan.count();
         return static_cast<size_t>(matrices) * plan.per;
-    });
+    };
+    return tb_tensor::best_fit(2, outer ? 64 : 32, height, (depth + 63) / 64, false, tiles, tiles);
 }
 
 } /* namespace */
@@ -330,6 +344,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
     Pair x = take_pair(&scratch, s.matrices, s.rows, s.columns), next = take_pair(&scratch, s.matrices, s.rows, s.columns);
     const Pair square = take_pair(&scratch, s.matrices, s.small, s.small), poly = take_pair(&scratch, s.matrices, s.small, s.small);
     ops.type = 0;
+    ops.parts = 1;
     ops.a_plane = ops.b_plane = static_cast<int>(s.matrices);
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
@@ -343,8 +358,8 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
             constexpr int P = decltype(p)::value;
             squares<T, P><<<grid, kNormThreads, 0, st>>>(given, static_cast<const T *>(g), sums);
             if (!launched()) return 0;
-            normalise<T, P><<<grid, kNormThreads, 0, st>>>(given, static_cast<const T *>(g), sums, desc->epsilon, x);
-            return launched();
+            return launch_early(normalise<T, P>, grid, kNormThreads, 0, 1, st, given, static_cast<const T *>(g),
+                                static_cast<const double *>(sums), static_cast<double>(desc->epsilon), x);
         });
         if (!normalised) return 0;
         const int z = static_cast<int>(s.matrices), small = static_cast<int>(s.small);
@@ -352,7 +367,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         for (int step = 0; step < desc->steps; ++step) {
             const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns), mn = matrices_of(next, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
-            const int squared = tb_tensor::with_fit<2>(plan_fit(z, s.small, s.small, true, s.tall, sms), [&](auto n, auto pair) {
+            const int squared = tb_tensor::with_fit<2>(plan_fit(z, s.small, s.small, (s.tall ? s.rows : s.columns), true, s.tall), [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
                 constexpr bool PAIR = decltype(pair)::value;
                 SquareJob job{};
@@ -372,7 +387,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                            ? 1 : 0;
             });
             if (!squared) return 0;
-            const int stepped = tb_tensor::with_fit<2>(plan_fit(z, s.rows, s.columns, false, false, sms), [&](auto n, auto pair) {
+            const int stepped = tb_tensor::with_fit<2>(plan_fit(z, s.rows, s.columns, s.small, false, false), [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
                 constexpr bool PAIR = decltype(pair)::value;
                 StepJob<T> job{};

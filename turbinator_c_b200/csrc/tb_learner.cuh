@@ -285,6 +285,32 @@ int sum_columns(float *partial, size_t rows, size_t columns, Last last, cudaStre
     return launched();
 }
 
+/* ---- kernels that begin before the one in front of them ends ---- */
+
+/* Waits until the kernels in front are done and what they wrote is there; first
+ * of all where launch_early was used. */
+__device__ __forceinline__ void after_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+/* From here on the CTAs of a kernel behind this one that launch_early launched may come onto free SMs. */
+__device__ __forceinline__ void later_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+/* Launches a kernel that calls after_earlier() before it touches memory. */
+template <class Kernel, class... Args>
+int launch_early(Kernel kernel, dim3 grid, unsigned threads, size_t shared, unsigned cluster, cudaStream_t st, const Args &...args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = threads;
+    config.dynamicSmemBytes = shared;
+    config.stream = st;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {cluster, 1, 1};
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess && launched();
+}
+
 /* ---- host side ---- */
 
 inline size_t type_size(int type) { return type == TB_TYPE_F32 ? 4 : 2; }

@@ -27,6 +27,10 @@
  * own additions cut what does not fit, which over thousands of k left errors of
  * 4e-6 to 2e-5 in results that f32 arithmetic has to 1e-6.
  *
+ * Where tiles are few and k is long, a tile's k is cut into parts of whole
+ * stages: each writes its sums to a workspace, and a second kernel adds them in
+ * order.
+ *
  * A job says what its tiles are and stores them (struct Job: setup, tiles,
  * tile, store: eight columns of a row of the tensor core's; or, where kStaging
  * is not 0, 32 columns of 32 rows by a warp with so many bytes of its own).
@@ -197,6 +201,8 @@ struct Operands {
     int a_outer, b_outer; /* m (n) contiguous instead of k */
     int type;             /* 0 f16, 1 bf16, 1 signed 8 bits */
     int a_plane, b_plane; /* z of the second plane */
+    int parts;            /* of a tile's k */
+    uint32_t *sums;       /* of the parts, if there are several: [tile][part][column][m] */
 };
 
 /* k in [k0, k0 + depth) of rows m0.. of A's matrix az and n0.. (columns of
@@ -205,6 +211,14 @@ struct Tile {
     int m0, n0, columns, k0, depth, az, bz;
     int which; /* the job's own */
 };
+/* A part of a tile's k: whole stages but for the last. */
+__device__ __forceinline__ Tile part_of(Tile t, int part, int parts, int stage) {
+    const int per = ((t.depth + stage - 1) / stage + parts - 1) / parts * stage;
+    const int first = min(part * per, t.depth);
+    t.k0 += first;
+    t.depth = min(per, t.depth - first);
+    return t;
+}
 
 /* ---- the kernel ---- */
 
@@ -335,13 +349,19 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     }
     if (warp == 1) tmem_alloc<PAIR>(smem_addr(&tmem_at), kColumns);
     tensor_fence_before();
+    tb_learn::later_may_start();
+    tb_learn::after_earlier();
     job.setup(shared);
     if constexpr (PAIR) cluster_sync();
     else __syncthreads();
     tensor_fence_after();
     const uint32_t tmem = tmem_at;
     const Waits w{ops.status, &gave_up};
-    const int tiles = job.tiles(shared), start = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
+    const int tiles = job.tiles(shared) * ops.parts, start = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
+    const auto tile_at = [&](int t) {
+        if (ops.parts == 1) return job.tile(shared, t);
+        return part_of(job.tile(shared, t / ops.parts), t % ops.parts, ops.parts, kDepth);
+    };
     /* Whether a stage's last rows of k belong to another matrix. */
     const auto ends_inside = [&](int left) { return Job::kRagged && left < kDepth && left % kStep != 0; };
     /* Those rows, in the block that they lie in; by a warp. */
@@ -357,7 +377,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             uint32_t n = 0; /* stages asked for */
             bool ok = true;
             for (int t = start; ok && t < tiles; t += stride) {
-                const Tile tile = job.tile(shared, t);
+                const Tile tile = tile_at(t);
                 const int m0 = tile.m0 + static_cast<int>(rank) * kRows;
                 const int n0 = tile.n0 + static_cast<int>(rank) * ((tile.columns + 15) / 16 * 8);
                 for (int k = 0; k < tile.depth; k += kDepth, ++n) {
@@ -410,7 +430,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             uint32_t n = 0, number = 0; /* stages taken, accumulators begun */
             bool ok = true;
             for (int t = start; ok && t < tiles; t += stride) {
-                const Tile tile = job.tile(shared, t);
+                const Tile tile = tile_at(t);
                 const uint32_t how =
                     product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, (tile.columns + 15) / 16 * 16);
                 uint32_t d = 0;
@@ -476,7 +496,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 uint32_t n = 0, phases = 0; /* a bit for each stage */
                 bool ok = true;
                 for (int t = start; ok && t < tiles; t += stride) {
-                    const Tile tile = job.tile(shared, t);
+                    const Tile tile = tile_at(t);
                     for (int k = 0; k < tile.depth; k += kDepth, ++n) {
                         if (!ends_inside(tile.depth - k)) continue;
                         const int s = n % S::kStages;
@@ -510,8 +530,19 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             }
         };
         for (int t = start; ok && t < tiles; t += stride) {
-            const Tile tile = job.tile(shared, t);
+            const Tile tile = tile_at(t);
             const int m = tile.m0 + static_cast<int>(rank) * kRows + part * 32 + lane;
+            [[maybe_unused]] const auto store = [&](int c, const uint32_t (&r)[8]) {
+                if constexpr (Job::kStaging == 0) {
+                    if (ops.parts == 1) {
+                        job.store(shared, tile, m, c, r);
+                    } else {
+                        uint32_t *to = ops.sums + (static_cast<size_t>(t) * NT + c) * S::kTileM + (m - tile.m0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) to[i * S::kTileM] = r[i];
+                    }
+                }
+            };
             const int c0 = share * S::kShare, columns = min(tile.columns - c0, S::kShare);
             if constexpr (kSums) {
                 float sum[S::kShare];
@@ -550,7 +581,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                             uint32_t r[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[c + i]);
-                            job.store(shared, tile, m, c0 + c, r);
+                            store(c0 + c, r);
                             asm volatile("" ::: "memory"); /* the next eight's loads stay behind: they would take registers that the sums need */
                         }
                 }
@@ -572,7 +603,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                         uint32_t eight[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) eight[j] = r[i + j];
-                        if (c + i < columns) job.store(shared, tile, m, c0 + c + i, eight);
+                        if (c + i < columns) store(c0 + c + i, eight);
                     }
                 }
                 free(buffer);
@@ -587,6 +618,35 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     else __syncthreads();
     tensor_fence_after();
     if (warp == 1) tmem_free<PAIR>(tmem, kColumns);
+}
+
+/* The parts' sums, in order, and from there to where the job puts them: a CTA
+ * eight columns of a tile, a thread an m. */
+template <class Job, int NT, int TM, bool I8>
+__global__ void __launch_bounds__(TM) join_parts(const __grid_constant__ Job job, int parts, const uint32_t *sums) {
+    __shared__ typename Job::Shared shared;
+    tb_learn::after_earlier();
+    job.setup(shared);
+    __syncthreads();
+    const int t = blockIdx.x;
+    if (t >= job.tiles(shared)) return;
+    const Tile tile = job.tile(shared, t);
+    const int c = blockIdx.y * 8;
+    if (c >= tile.columns) return;
+    const uint32_t *from = sums + (static_cast<size_t>(t) * parts * NT + c) * TM + threadIdx.x;
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = from[i * TM];
+    for (int p = 1; p < parts; ++p) {
+        from += NT * TM;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t v = from[i * TM];
+            if constexpr (I8) r[i] += v;
+            else r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(v));
+        }
+    }
+    job.store(shared, tile, tile.m0 + threadIdx.x, c, r);
 }
 
 /* ---- host side ---- */
@@ -648,26 +708,45 @@ template <int NT, bool PAIR> bool encode(Operands *ops, const Matrices &a, bool 
 struct Fit {
     int columns;
     bool pair;
+    int parts;
+    size_t tiles; /* at most, for the room of the parts' sums */
+    size_t room() const { return parts > 1 ? tiles * parts * columns * (pair ? 2 * kRows : kRows) * sizeof(uint32_t) : 0; }
 };
-/* The tiles that should be done first: as many as there are go round the SMs in
- * so many turns, and a turn takes as long as its products (two cycles a column
- * and block of k, times the pairs of planes) or its copies (some 46 bytes a
- * cycle and SM) do.  count(columns, m) says how many tiles of so many columns by
- * m there are, `average` how many columns one has of them; least: 64 where n is
- * contiguous in b. */
-template <class Count> Fit best_fit(int planes, int least, size_t average, int sms, Count &&count) {
-    Fit best{0, false};
+constexpr int kSms = 148; /* the fit is a shape's, whatever the device: a workspace is asked for without one */
+constexpr size_t kMostRoom = 64u << 20;
+
+/* The tiles, and parts of their k, that should be done first, in cycles: as many
+ * as there are go round the SMs in so many turns; a block of k takes as long as
+ * its products (two cycles a column, times the pairs of planes) or its copies
+ * (some 46 bytes a cycle and SM); every turn some 2,000 for what is not hidden
+ * of its beginning and end, and parts a second kernel and their sums' way
+ * through L2.  count(columns, m) says how many tiles of so many columns by m
+ * there are likely to be, `average` how many columns one has of them, most(columns, m) how
+ * many there may be; least: 64 where n is contiguous in b.
+ * 1 x 4,096 x 4,096 of 8 bits: 14.5 us in one part, 11.0 in four (in a graph). */
+template <class Count, class Most>
+Fit best_fit(int planes, int least, size_t average, size_t blocks, bool may_part, Count &&count, Most &&most) {
+    Fit best{0, false, 1, 0};
     double lowest = 0.0;
     const auto consider = [&](int columns, bool pair) {
-        const double units = pair ? sms / 2 : sms, tiles = static_cast<double>(count(columns, pair ? 2 * kRows : kRows));
-        const double turns = static_cast<double>(static_cast<size_t>((tiles + units - 1) / units));
+        const int m = pair ? 2 * kRows : kRows;
+        const double units = pair ? kSms / 2 : kSms, tiles = static_cast<double>(count(columns, m));
         const double taken = average < static_cast<size_t>(columns) ? static_cast<double>(average) : columns;
         const double products = 2.0 * taken * (planes * (planes + 1) / 2);
         const double copies = planes * kBlockBytes * (kRows + columns / (pair ? 2.0 : 1.0)) / 46.0;
-        const double cost = turns * ((products > copies ? products : copies) + 40.0);
-        if (best.columns == 0 || cost < lowest) {
-            lowest = cost;
-            best = Fit{columns, pair};
+        const double block = products > copies ? products : copies;
+        for (int parts = 1; parts <= 64 && (parts == 1 || may_part); parts += parts < 4 ? 1 : parts / 2) {
+            const size_t per = (blocks + parts - 1) / parts;
+            if (parts > 1 && per < 4) break;
+            const double turns = static_cast<double>(static_cast<size_t>((tiles * parts + units - 1) / units));
+            double cost = turns * (per * block + 2000.0);
+            Fit fit{columns, pair, parts, most(columns, m)};
+            if (parts > 1) cost += 5000.0 + tiles * parts * taken * m * 8.0 / (kSms * 40.0);
+            if (fit.room() > kMostRoom) break;
+            if (best.columns == 0 || cost < lowest) {
+                lowest = cost;
+                best = fit;
+            }
         }
     };
     consider(256, true);
@@ -701,18 +780,17 @@ int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, 
         }
         if (n < Shape<NT, PLANES, PAIR>::kLaunchRegisters) return 0;
     }
-    const size_t most = static_cast<size_t>(sms) / kCtas;
-    cudaLaunchConfig_t config{};
-    config.gridDim = static_cast<unsigned>(tiles < most ? tiles : most) * kCtas;
-    config.blockDim = Shape<NT, PLANES, PAIR>::kThreads;
-    config.dynamicSmemBytes = kShared;
-    config.stream = st;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim = {kCtas, 1, 1};
-    config.attrs = &attribute;
-    config.numAttrs = PAIR ? 1 : 0;
-    return cudaLaunchKernelEx(&config, kernel, ops, job) == cudaSuccess && tb_learn::launched();
+    const size_t most = static_cast<size_t>(sms) / kCtas, all = tiles * ops.parts;
+    const unsigned grid = static_cast<unsigned>(all < most ? all : most) * kCtas;
+    if (!tb_learn::launch_early(kernel, grid, Shape<NT, PLANES, PAIR>::kThreads, kShared, kCtas, st, ops, job)) return 0;
+    if constexpr (Job::kStaging == 0) {
+        if (ops.parts > 1) {
+            constexpr int TM = Shape<NT, PLANES, PAIR>::kTileM;
+            return tb_learn::launch_early(join_parts<Job, NT, TM, I8>, dim3(static_cast<unsigned>(tiles), NT / 8), TM, 0, 1, st, job,
+                                          ops.parts, static_cast<const uint32_t *>(ops.sums));
+        }
+    }
+    return 1;
 }
 
 } /* namespace tb_tensor */
