@@ -161,7 +161,7 @@ template <class T, int NT> struct SumJob {
 
 /* Where the rows are few, as in acting, the weights are what is read, once, and
  * a product is a warp's sum over a row of weights, against up to four rows. */
-constexpr int kFewThreads = 256, kFewRows = 4;
+constexpr int kFewThreads = 256, kFewRows = 4, kFewWide = 148;
 
 /* The dot product of 16 bytes (or 4, or an element) of weights and a row. */
 template <class T, int PACK> struct FewPack {
@@ -213,6 +213,21 @@ struct FewShape {
     size_t x_stride, w_row, w_matrix, out_stride;
 };
 
+/* The expert whose run row is in and where that ends, -1 (and `last`) for none; by a warp. */
+__device__ __forceinline__ int expert_of(const Runs &runs, int row, int last, int lane, int *end) {
+    *end = last;
+    for (int base = 0; base < runs.experts; base += 32) {
+        const int mine = base + lane, from = mine < runs.experts ? run_start(runs, mine) : runs.rows;
+        const int to = mine < runs.experts ? run_end(runs, mine, from) : from;
+        const unsigned has = __ballot_sync(0xffffffffu, from <= row && row < to);
+        if (has) {
+            *end = __shfl_sync(0xffffffffu, to, __ffs(has) - 1);
+            return base + __ffs(has) - 1;
+        }
+    }
+    return -1;
+}
+
 /* W: of rows and weights, f32, bf16, f16 or 8 bits; T: of the output. */
 template <class W, class T, int PACK>
 __global__ void __launch_bounds__(kFewThreads)
@@ -230,16 +245,7 @@ few_rows(FewShape d, Runs runs, const W *x, const W *weight, T *out, const float
             end = run_end(runs, 0, start);
             count = last - row;
         } else {
-            e = -1;
-            for (int base = 0; base < runs.experts && e < 0; base += 32) {
-                const int mine = base + lane, from = mine < runs.experts ? run_start(runs, mine) : runs.rows;
-                const int to = mine < runs.experts ? run_end(runs, mine, from) : from;
-                const unsigned has = __ballot_sync(0xffffffffu, from <= row && row < to);
-                if (has) {
-                    e = base + __ffs(has) - 1;
-                    end = __shfl_sync(0xffffffffu, to, __ffs(has) - 1);
-                }
-            }
+            e = expert_of(runs, row, last, lane, &end);
             count = e < 0 ? 1 : min(end, last) - row;
             if (e < 0) continue; /* no expert's: left as it was */
         }
@@ -275,6 +281,91 @@ few_rows(FewShape d, Runs runs, const W *x, const W *weight, T *out, const float
     }
 }
 
+/* The same where the weights lie the other way, [sum][channel]: lanes take
+ * neighbouring channels, a CTA's warps every so-many-th k, and their sums meet
+ * in shared memory. */
+constexpr int kAcrossThreads = 256, kAcrossWarps = kAcrossThreads / 32;
+template <class T, int PACK>
+__global__ void __launch_bounds__(kAcrossThreads) few_rows_across(FewShape d, Runs runs, const T *x, const T *weight, T *out) {
+    __shared__ float parts[kAcrossWarps][kFewRows][32 * PACK + 1];
+    constexpr int kAhead = 4; /* rows of weights under way at once */
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, m = (blockIdx.x * 32 + lane) * PACK;
+    const int last = min(static_cast<int>(blockIdx.y + 1) * kFewRows, runs.rows);
+    after_earlier();
+    for (int row = blockIdx.y * kFewRows, count; row < last; row += count) {
+        int end;
+        const int e = expert_of(runs, row, last, lane, &end);
+        count = e < 0 ? 1 : min(end, last) - row;
+        if (e < 0) continue; /* no expert's: left as it was */
+        const T *w = weight + e * d.w_matrix + m, *from = x + row * d.x_stride;
+        float sum[kFewRows][PACK] = {};
+        if (m < d.width)
+            for (int k = warp; k < d.depth; k += kAcrossWarps * kAhead) {
+                Held<T, PACK> h[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (k + i * kAcrossWarps < d.depth) h[i] = load_once<T, PACK>(w + (k + i * kAcrossWarps) * d.w_row);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (k + i * kAcrossWarps >= d.depth) break;
+                    float a[PACK];
+                    unpack(h[i], a);
+#pragma unroll
+                    for (int r = 0; r < kFewRows; ++r)
+                        if (r < count) {
+                            const float b = to_float(from[r * d.x_stride + k + i * kAcrossWarps]);
+#pragma unroll
+                            for (int j = 0; j < PACK; ++j) sum[r][j] = fmaf(a[j], b, sum[r][j]);
+                        }
+                }
+            }
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) parts[warp][r][lane * PACK + j] = sum[r][j];
+        __syncthreads();
+        for (int i = threadIdx.x; i < count * 32 * PACK; i += kAcrossThreads) {
+            const int r = i / (32 * PACK), c = i % (32 * PACK);
+            float v = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kAcrossWarps; ++p) v += parts[p][r][c];
+            const int at = blockIdx.x * 32 * PACK + c;
+            if (at < d.width) out[(row + r) * d.out_stride + at] = from_float<T>(v);
+        }
+        __syncthreads();
+    }
+}
+
+/* dW where an expert has few rows: what is written is most of the work.  A warp
+ * takes four lines of an expert's gradient, [line][column], lanes along them. */
+constexpr int kFewLines = 4;
+template <class T, int PACK>
+__global__ void __launch_bounds__(kFewThreads)
+few_sums(int width, int height, size_t line_stride, size_t column_stride, size_t w_row, size_t w_matrix, Runs runs, const T *lines,
+         const T *columns, T *out) {
+    const int lane = threadIdx.x % 32, n0 = (blockIdx.x * (kFewThreads / 32) + threadIdx.x / 32) * kFewLines, e = blockIdx.y;
+    after_earlier();
+    if (n0 >= height) return;
+    const int start = run_start(runs, e), end = run_end(runs, e, start);
+    for (int m = lane * PACK; m < width; m += 32 * PACK) {
+        float sum[kFewLines][PACK] = {};
+        for (int p = start; p < end; ++p) {
+            float b[PACK];
+            unpack(*reinterpret_cast<const Held<T, PACK> *>(columns + p * column_stride + m), b);
+#pragma unroll
+            for (int i = 0; i < kFewLines; ++i)
+                if (n0 + i < height) {
+                    const float a = to_float(lines[p * line_stride + n0 + i]);
+#pragma unroll
+                    for (int j = 0; j < PACK; ++j) sum[i][j] = fmaf(a, b[j], sum[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < kFewLines; ++i)
+            if (n0 + i < height) store_once<T, PACK>(out + e * w_matrix + (n0 + i) * w_row + m, packed<T, PACK>(sum[i]));
+    }
+}
+
 /* Up to eight rows, and some 2^25 products of theirs: 1 x 4,096 x 4,096 of 8 bits
  * 6.6 us against 9.0 by tiles, of bf16 7.2 against 10.0, 8 x 1,024 x 1,024 4.4
  * against 5.5; 4 x 4,096 x 4,096 12 against 9.  f32 weights are laid out as
@@ -299,6 +390,33 @@ int few_product(const FewShape &d, const Runs &runs, const W *x, const W *weight
     if constexpr (sizeof(W) < 4)
         if (bits % 4 == 0) return launch(std::integral_constant<int, 4 / static_cast<int>(sizeof(W))>{});
     return launch(std::integral_constant<int, 1>{});
+}
+
+template <class T>
+int few_product_across(const FewShape &d, const Runs &runs, const T *x, const T *weight, T *out, cudaStream_t st) {
+    const size_t bits = reinterpret_cast<uintptr_t>(weight) | (d.w_row | d.w_matrix | static_cast<size_t>(d.width)) * sizeof(T);
+    int pack = pack_of(bits, sizeof(T));
+    /* narrower where that gives every SM a CTA */
+    if (pack > 1 && d.width < 32 * pack * kFewWide) pack = bits % 4 == 0 && pack > 4 / static_cast<int>(sizeof(T)) ? 4 / static_cast<int>(sizeof(T)) : pack;
+    return with_pack<T>(pack, [&](auto p) {
+        constexpr int P = decltype(p)::value;
+        const dim3 grid(static_cast<unsigned>((d.width + 32 * P - 1) / (32 * P)), static_cast<unsigned>((runs.rows + kFewRows - 1) / kFewRows));
+        return launch_early(few_rows_across<T, P>, grid, kAcrossThreads, 0, 1, st, d, runs, x, weight, out);
+    });
+}
+
+/* Rows of lines and columns; out [experts][height][width]. */
+template <class T>
+int few_gradient(int width, int height, size_t line_stride, size_t column_stride, size_t w_row, size_t w_matrix, const Runs &runs,
+                 const T *lines, const T *columns, T *out, cudaStream_t st) {
+    const size_t bits = reinterpret_cast<uintptr_t>(columns) | reinterpret_cast<uintptr_t>(out) |
+                        (column_stride | w_row | w_matrix | static_cast<size_t>(width)) * sizeof(T);
+    return with_pack<T>(pack_of(bits, sizeof(T)), [&](auto p) {
+        constexpr int P = decltype(p)::value, kLines = kFewThreads / 32 * kFewLines;
+        const dim3 grid(static_cast<unsigned>((height + kLines - 1) / kLines), static_cast<unsigned>(runs.experts));
+        return launch_early(few_sums<T, P>, grid, kFewThreads, 0, 1, st, width, height, line_stride, column_stride, w_row, w_matrix, runs, lines,
+                            columns, out);
+    });
 }
 
 /* ---- laying operands out ---- */
@@ -498,7 +616,10 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) -> int {
         using T = decltype(t);
-        if (s.turned && few(s.rows, s.experts, s.in, s.out, s.wide))
+        if (!s.turned && few(s.rows, s.experts, s.in, s.out, s.wide))
+            return few_product_across<T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
+                                         static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), st);
+        if (few(s.rows, s.experts, s.in, s.out, s.wide))
             return few_product<T, T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
                                      static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), nullptr, nullptr, st);
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
@@ -532,12 +653,16 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        if (dx && !s.turned && few(s.rows, s.experts, s.in, s.out, s.wide)) { /* weights' rows lie along this sum */
-            if (!few_product<T, T>({static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.w_row, s.w_matrix, s.dx_stride}, runs,
-                                   static_cast<const T *>(dy), static_cast<const T *>(weight), static_cast<T *>(dx), nullptr, nullptr, st))
+        if (few(s.rows, s.experts, s.in, s.out, s.wide)) {
+            const FewShape d{static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.w_row, s.w_matrix, s.dx_stride};
+            const T *g = static_cast<const T *>(dy), *w = static_cast<const T *>(weight), *in = static_cast<const T *>(x);
+            T *dw = static_cast<T *>(dweight);
+            if (dx && !(s.turned ? few_product_across<T>(d, runs, g, w, static_cast<T *>(dx), st)
+                                 : few_product<T, T>(d, runs, g, w, static_cast<T *>(dx), nullptr, nullptr, st)))
                 return 0;
-            dx = nullptr;
             if (!dweight) return 1;
+            return s.turned ? few_gradient<T>(static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.x_stride, s.w_row, s.w_matrix, runs, g, in, dw, st)
+                            : few_gradient<T>(static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.y_stride, s.w_row, s.w_matrix, runs, in, g, dw, st);
         }
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx, my;
