@@ -44,8 +44,9 @@ struct Pair {
 /* ---- x = g / (|g| + epsilon) ---- */
 
 constexpr int kNormThreads = 256;
-constexpr size_t kMostParts = 512; /* of a matrix */
-constexpr size_t kPartValues = 4096;
+constexpr size_t kMostParts = 512;  /* of a matrix */
+constexpr size_t kPartValues = 2048; /* of a part at least */
+constexpr size_t kManyParts = 8192;  /* of all matrices */
 
 struct Given {
     size_t rows, columns, matrix_stride, row_stride, rows_a_part;
@@ -208,13 +209,16 @@ struct SquareJob {
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
+    __device__ __forceinline__ void ask(const Tile &t, int m, int c0, tb_tensor::Staging &s) const {
+        if (second && m - s.lane < plan.width) s.load(&old, m - s.lane, t.n0 + c0, t.which, plan.matrices, kBoxBytes);
+    }
     __device__ __forceinline__ bool store(const Tile &t, int m, int c0, float (&v)[32], tb_tensor::Staging &s) const {
         const int x = m - s.lane, y = t.n0 + c0;
         if (x >= plan.width) return true;
         const Boxes boxes{s.lane, reinterpret_cast<__half *>(s.at)};
         __half high[32], low[32];
         if (second) {
-            if (!s.load(&old, x, y, t.which, plan.matrices, kBoxBytes)) return false;
+            if (!s.loaded()) return false;
 #pragma unroll
             for (int i = 0; i < 32; ++i) boxes.put(i, fmaf(c, v[i] * kDown, b * boxes.get(i)), &high[i], &low[i]);
         } else {
@@ -245,11 +249,14 @@ template <class T> struct StepJob {
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
     __device__ Tile tile(const Shared &, int t) const { return plan.tile(t); }
+    __device__ __forceinline__ void ask(const Tile &t, int m, int c0, tb_tensor::Staging &s) const {
+        if (m - s.lane < plan.width) s.load(&x, m - s.lane, t.n0 + c0, t.which, plan.matrices, kBoxBytes);
+    }
     __device__ __forceinline__ bool store(const Tile &t, int m, int c0, float (&v)[32], tb_tensor::Staging &s) const {
         const int left = m - s.lane, y = t.n0 + c0;
         if (left >= plan.width) return true;
         const Boxes boxes{s.lane, reinterpret_cast<__half *>(s.at)};
-        if (!s.load(&x, left, y, t.which, plan.matrices, kBoxBytes)) return false;
+        if (!s.loaded()) return false;
         if (last) {
             T *o = last + t.which * matrix_stride + y * row_stride + m;
 #pragma unroll
@@ -350,7 +357,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         using T = decltype(t);
         const int pack = pack_of(reinterpret_cast<uintptr_t>(g) | (s.in_row | s.columns | (s.matrices > 1 ? s.in_matrix : 0)) * size, size);
         size_t parts = (s.rows * s.columns + kPartValues - 1) / kPartValues;
-        parts = std::min(parts, std::min(kMostParts, s.rows));
+        parts = std::min({parts, kMostParts, s.rows, std::max<size_t>(16, kManyParts / s.matrices)});
         Given given{s.rows, s.columns, s.in_matrix, s.in_row, (s.rows + parts - 1) / parts, 1};
         while (given.lanes < kNormThreads && static_cast<size_t>(given.lanes) * pack < s.columns) given.lanes *= 2;
         const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(s.matrices));

@@ -33,7 +33,8 @@
  *
  * A job says what its tiles are and stores them (struct Job: setup, tiles,
  * tile, store: eight columns of a row of the tensor core's; or, where kStaging
- * is not 0, 32 columns of 32 rows by a warp with so many bytes of its own).
+ * is not 0, 32 columns of 32 rows by a warp with so many bytes of its own, into
+ * which ask has asked for what it reads for them).
  *
  * Waits are bounded by a second; one that runs out reports
  * TB_FEATURE_STATUS_WAIT_TIMEOUT through the stream's status word, after which
@@ -147,6 +148,10 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap *map, in
             "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
             ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 /* ---- the other CTA of a pair ---- */
@@ -269,6 +274,7 @@ struct Staging {
     uint32_t bar, phase;
     int lane;
     const Waits *w;
+    bool under_way;
     /* What was put in has been read. */
     __device__ __forceinline__ void free() const {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -277,17 +283,23 @@ struct Staging {
     __device__ __forceinline__ void stored() const {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-    /* Boxes of `bytes` of planes z and z + next; false where the wait for them ran out. */
-    __device__ __forceinline__ bool load(const CUtensorMap *map, int x, int y, int z, int next, int bytes) {
+    /* Asks for boxes of `bytes` of planes z and z + next. */
+    __device__ __forceinline__ void load(const CUtensorMap *map, int x, int y, int z, int next, int bytes) {
         free();
         if (lane == 0) {
             mbar_arrive_expect_tx(bar, 2 * bytes);
             load_box<false>(smem_addr(at), map, x, y, z, bar);
             load_box<false>(smem_addr(at) + bytes, map, x, y, z + next, bar);
         }
+        under_way = true;
+    }
+    /* They are there; false where the wait for them ran out. */
+    __device__ __forceinline__ bool loaded() {
+        if (!under_way) return true;
         const bool ok = w->wait(bar, phase);
         if (!ok) tb_pipe::mbar_wait(bar, phase, kWaitNs); /* they land all the same */
         phase ^= 1;
+        under_way = false;
         return ok;
     }
     /* The same out of shared memory, as this warp has written it. */
@@ -336,6 +348,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     const bool first = rank == 0; /* the CTA whose warp issues the products */
     unsigned char *stages = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     if (threadIdx.x == 0) {
+        prefetch_map(&ops.a);
+        prefetch_map(&ops.b);
         for (int i = 0; i < S::kStages; ++i) {
             mbar_init(smem_addr(&full[i]), kCtas);
             mbar_init(smem_addr(&empty[i]), 1);
@@ -520,7 +534,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
         uint32_t number = 0;
         bool ok = true;
         Staging staging{stages + S::kStages * S::kStage + (warp - S::kFirstStore) * Job::kStaging,
-                        smem_addr(&staged[warp - S::kFirstStore]), 0, lane, &w};
+                        smem_addr(&staged[warp - S::kFirstStore]), 0, lane, &w, false};
         const auto free = [&](uint32_t buffer) {
             tensor_fence_before();
             __syncwarp();
@@ -548,6 +562,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 float sum[S::kShare];
 #pragma unroll
                 for (int i = 0; i < S::kShare; ++i) sum[i] = 0.0f;
+                if constexpr (Job::kStaging != 0)
+                    if (columns > 0) job.ask(tile, m, c0, staging);
                 for (int k = 0; ok && (k < tile.depth || k == 0); k += kSegment * kDepth, ++number) {
                     const uint32_t buffer = number & 1;
                     if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
@@ -573,6 +589,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = sum[c + i];
                             ok = job.store(tile, m, c0 + c, v, staging);
+                            if (ok && c + 32 < columns) job.ask(tile, m, c0 + c + 32, staging);
                         }
                 } else {
 #pragma unroll
@@ -610,7 +627,10 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 ++number;
             }
         }
-        if constexpr (Job::kStaging != 0) staging.stored();
+        if constexpr (Job::kStaging != 0) {
+            staging.loaded();
+            staging.stored();
+        }
     }
     __syncwarp();
     tensor_fence_before();
