@@ -140,6 +140,14 @@ def test_product_sums_a_long_axis(kind):
     _check_product(_gen(2), 20011, [0, 20011], 64, 72, kind, False)
 
 
+@pytest.mark.parametrize("kind", (torch.bfloat16, torch.float16), ids=str)
+@pytest.mark.parametrize("turned", (False, True), ids=("in_out", "out_in"))
+def test_product_of_many_wide_tiles(kind, turned):
+    """Runs that end anywhere in a tile of 256 x 256, and widths past its edges."""
+    _check_product(_gen(3), 20003, [0, 9000, 9001, 19700], 200, 1100, kind, turned)
+    _check_product(_gen(4), 5000, [3, 2100, 2100, 4990], 1100, 1304, kind, turned)
+
+
 def test_product_offsets_out_of_range_are_taken_into_it():
     gen = _gen(8)
     desc, x, w, dy, _ = _product_case(gen, 60, [0, 20, 40, 60], 64, 64, torch.bfloat16, False)
@@ -267,6 +275,14 @@ def test_i8_product(shape, kind):
     q = torch.randint(-128, 128, (rows, n), generator=gen, device="cuda").to(torch.int8)
     w = torch.randint(-128, 128, (e, m, n), generator=gen, device="cuda").to(torch.int8)
     _check_i8(q, torch.rand(rows, generator=gen, device="cuda"), w, torch.rand((e, m), generator=gen, device="cuda"), offsets, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+def test_i8_product_of_many_wide_tiles(kind):
+    gen = _gen(21)
+    q = torch.randint(-128, 128, (20003, 300), generator=gen, device="cuda").to(torch.int8)
+    w = torch.randint(-128, 128, (3, 1100, 300), generator=gen, device="cuda").to(torch.int8)
+    _check_i8(q, torch.rand(20003, generator=gen, device="cuda"), w, torch.rand((3, 1100), generator=gen, device="cuda"), [0, 9000, 9001, 19700], kind)
 
 
 @pytest.mark.parametrize("pad,shift", [(16, 0), (5, 0), (0, 1), (3, 7)])
