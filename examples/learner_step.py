@@ -2,12 +2,13 @@
 
 A small actor over aircraft trajectories: ``tb_cuda_prepare_actor_inputs_device`` turns observations, missions and
 cameras into proprio and luma; a camera stem (convolution, group norm + SiLU), a gated recurrence over each aircraft's
-trajectory with resets at episode ends, and a trunk of routed experts predict the next step's proprio.
+trajectory with resets at episode ends, and a trunk of routed experts predict the next step's proprio.  The experts'
+matrices are updated by orthogonalised momentum, everything else by Adam; for acting they may be held in 8 bits.
 
     python examples/learner_step.py            # trains for some steps, then acts step by step from kept states
 
-The ``torch.autograd.Function`` wrappers below are all that a PyTorch program needs around the C entry points; matrix
-products and the convolution are PyTorch's.  They make descriptors, workspaces and outputs anew in each call, which a
+The ``torch.autograd.Function`` wrappers below are all that a PyTorch program needs around the C entry points; the
+convolution and the products of dense layers are PyTorch's.  They make descriptors, workspaces and outputs anew in each call, which a
 program that counts microseconds, as one that acts does, makes once and keeps: a step of 64 aircraft is 2 us of the
 GPU's time and more than ten times that of the host's in this form."""
 from __future__ import annotations
@@ -133,18 +134,68 @@ class HandOut(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, order, position):
+        desc = _combine_desc(*position.shape, order.shape[0], x.shape[1], x.dtype)
+        rows = torch.empty((order.shape[0], x.shape[1]), dtype=x.dtype, device="cuda")
+        _call(tb.tb_cuda_hand_out_experts_device(desc, x.contiguous(), order, None, rows, torch.cuda.current_stream()))
         ctx.save_for_backward(position)
-        return x[order.long() // position.shape[1]]
+        ctx.desc = desc
+        return rows
 
     @staticmethod
     def backward(ctx, drows):
         (position,) = ctx.saved_tensors
-        t, k = position.shape
         drows = drows.contiguous()
-        dx = torch.empty((t, drows.shape[1]), dtype=drows.dtype, device="cuda")
-        _call(tb.tb_cuda_combine_experts_device(_combine_desc(t, k, *drows.shape, drows.dtype), drows, position, None, dx,
-                                                torch.cuda.current_stream()))
+        dx = torch.empty((position.shape[0], drows.shape[1]), dtype=drows.dtype, device="cuda")
+        _call(tb.tb_cuda_hand_out_experts_backward_device(ctx.desc, None, position, None, drows, dx, None,
+                                                          torch.cuda.current_stream()))
         return dx, None, None
+
+
+class Product(torch.autograd.Function):
+    """rows [rows, in] of the experts' runs, weights [experts, in, out] -> [rows, out]; offsets stay on the GPU."""
+
+    @staticmethod
+    def forward(ctx, rows, weight, offsets):
+        rows = rows.contiguous()
+        e, n, m = weight.shape
+        desc = tb.ExpertProductDesc(rows=rows.shape[0], experts=e, in_width=n, out_width=m, type=TYPE[rows.dtype],
+                                    weight_order=tb.TB_WEIGHT_IN_OUT)
+        out = torch.empty((rows.shape[0], m), dtype=rows.dtype, device="cuda")
+        work = _scratch(tb.tb_cuda_experts_product_workspace(desc))
+        _call(tb.tb_cuda_experts_product_device(desc, rows, weight, offsets, out, work, torch.cuda.current_stream()))
+        ctx.save_for_backward(rows, weight, offsets)
+        ctx.desc = desc
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        rows, weight, offsets = ctx.saved_tensors
+        drows, dweight = torch.empty_like(rows), torch.empty_like(weight)
+        work = _scratch(tb.tb_cuda_experts_product_workspace(ctx.desc))
+        _call(tb.tb_cuda_experts_product_backward_device(ctx.desc, rows, weight, offsets, dout.contiguous(), drows, dweight, work,
+                                                         torch.cuda.current_stream()))
+        return drows, dweight, None
+
+
+def quantised(x):
+    """Rows of x [.., width] in 8 bits, and their scales."""
+    x = x.contiguous()
+    q, scale = torch.empty(x.shape, dtype=torch.int8, device="cuda"), torch.empty(x.shape[:-1], device="cuda")
+    desc = tb.QuantiseDesc(rows=scale.numel(), width=x.shape[-1], type=TYPE[x.dtype])
+    _call(tb.tb_cuda_quantise_rows_device(desc, x, q, scale, torch.cuda.current_stream()))
+    return q, scale
+
+
+def product_8_bit(rows, weight, weight_scale, offsets):
+    """rows [rows, in] of the experts' runs by weights [experts, out, in] of 8 bits."""
+    e, m, n = weight.shape
+    q, scale = quantised(rows)
+    desc = tb.ExpertProductI8Desc(rows=rows.shape[0], experts=e, in_width=n, out_width=m, type=TYPE[rows.dtype])
+    out = torch.empty((rows.shape[0], m), dtype=rows.dtype, device="cuda")
+    work = _scratch(tb.tb_cuda_experts_product_i8_workspace(desc))
+    _call(tb.tb_cuda_experts_product_i8_device(desc, q, scale, weight, weight_scale, offsets, out, work,
+                                               torch.cuda.current_stream()))
+    return out
 
 
 class Combine(torch.autograd.Function):
@@ -187,6 +238,7 @@ class Actor(torch.nn.Module):
         self.register_buffer("balance", torch.zeros(experts, device="cuda"))
         self.up, self.down = new(experts, width, 2 * width, scale=0.09), new(experts, 2 * width, width, scale=0.06)
         self.head = new(width, 91, scale=0.05)
+        self.held = None  # the experts in 8 bits, for acting
 
     def forward(self, proprio, luma, state, reset):
         """proprio [aircraft, steps, 91], luma [.., 4, 64, 64] -> prediction, last state, experts' loads."""
@@ -201,11 +253,39 @@ class Actor(torch.nn.Module):
         tokens = h.reshape(b * t, self.width)
         weights, _, offsets, order, position = RouteExperts.apply(tokens @ self.router, self.balance, self.top_k)
         rows = HandOut.apply(tokens, order, position)
-        ends = offsets.tolist()  # each expert's rows: a program on the hot path keeps them on the GPU
-        done = [torch.nn.functional.silu(rows[a:z] @ self.up[e]) @ self.down[e]
-                for e, (a, z) in enumerate(zip(ends, ends[1:]))]
-        out = tokens + Combine.apply(torch.cat(done), position, weights)
+        silu = torch.nn.functional.silu
+        if self.held:
+            done = product_8_bit(silu(product_8_bit(rows, *self.held[0], offsets)), *self.held[1], offsets)
+        else:
+            done = Product.apply(silu(Product.apply(rows, self.up, offsets)), self.down, offsets)
+        out = tokens + Combine.apply(done, position, weights)
         return (out @ self.head).reshape(b, t, 91), state, offsets.diff()
+
+
+    @torch.no_grad()
+    def hold_experts_in_8_bits(self):
+        """For acting: a scale for each output channel, whose weights become a row."""
+        self.held = [quantised(w.transpose(1, 2)) for w in (self.up, self.down)]
+
+
+class OrthogonalMomentum:
+    """Momentum of stacks of matrices, orthogonalised before it is applied: every direction moves alike."""
+
+    def __init__(self, parameters, rate=0.02, momentum=0.95):
+        self.parameters, self.rate, self.momentum = list(parameters), rate, momentum
+        self.kept = [torch.zeros_like(p) for p in self.parameters]
+
+    @torch.no_grad()
+    def step(self):
+        for p, kept in zip(self.parameters, self.kept):
+            kept.mul_(self.momentum).add_(p.grad)
+            b, m, n = p.shape
+            desc = tb.OrthogonaliseDesc(matrices=b, rows=m, columns=n, type=TYPE[p.dtype], steps=5, a=3.4445, b=-4.7750,
+                                        c=2.0315, epsilon=1e-7, scale=max(1.0, n / m) ** 0.5)
+            update, work = torch.empty_like(p), _scratch(tb.tb_cuda_orthogonalise_workspace(desc))
+            _call(tb.tb_cuda_orthogonalise_device(desc, p.grad.add(kept, alpha=self.momentum), update, work,
+                                                  torch.cuda.current_stream()))
+            p.add_(update, alpha=-self.rate)
 
 
 def trajectories(aircraft: int, steps: int, seed: int = 0):
@@ -226,18 +306,21 @@ def trajectories(aircraft: int, steps: int, seed: int = 0):
     return proprio, luma, reset
 
 
-def train(actor: Actor, aircraft=16, steps=33, updates=40, rate=2e-3, seed=0):
-    """Predicts each step's successor; returns the losses."""
+def train(actor: Actor, aircraft=16, steps=33, updates=40, rate=2e-3, seed=0, orthogonal=False):
+    """Predicts each step's successor; returns the losses.  orthogonal: the experts' matrices by orthogonalised momentum."""
     proprio, luma, reset = trajectories(aircraft, steps + 1, seed)
     first = torch.zeros((aircraft, actor.width), device="cuda")
-    optimiser = torch.optim.Adam(actor.parameters(), lr=rate)
+    experts = [actor.up, actor.down] if orthogonal else []
+    optimiser = torch.optim.Adam([p for p in actor.parameters() if not any(p is e for e in experts)], lr=rate)
+    of_experts = OrthogonalMomentum(experts, rate=5 * rate)
     losses = []
     for _ in range(updates):
         guess, _, loads = actor(proprio[:, :-1], luma[:, :-1], first, reset[:, :-1].contiguous())
         loss = (guess.float() - proprio[:, 1:]).square().mean()
-        optimiser.zero_grad()
+        actor.zero_grad()
         loss.backward()
         optimiser.step()
+        of_experts.step()
         actor.balance += 0.001 * torch.sign(loads.float().mean() - loads)  # the busy experts' scores go down
         _finish()
         losses.append(loss.item())
@@ -258,7 +341,7 @@ def act(actor: Actor, proprio, luma, reset):
 
 def main() -> None:
     actor = Actor()
-    losses = train(actor)
+    losses = train(actor, orthogonal=True)
     print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f} over {len(losses)} updates")
     proprio, luma, reset = trajectories(4, 20, seed=1)
     with torch.no_grad():
@@ -268,6 +351,9 @@ def main() -> None:
     print(f"acting step by step differs from the whole trajectory by {float(off.median()):.2g} (median of the steps; "
           f"{float(off.max()):.2g} at most, where bf16 rounding decides between two experts) "
           f"of {float(whole.float().square().mean().sqrt()):.2g}")
+    actor.hold_experts_in_8_bits()
+    off = (act(actor, proprio, luma, reset) - stepped).float().square().mean(2).sqrt()
+    print(f"with the experts in 8 bits by {float(off.median()):.2g} (median of the steps)")
 
 
 if __name__ == "__main__":
