@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 4; /* rows of a token under way at once */
+constexpr int kAhead = 4; /* rows of a token under way at once; eight: 137 us for 78 (registers) */
 
 struct HandShape {
     size_t tokens, rows, width, rows_stride, token_stride;
@@ -47,6 +47,8 @@ template <class T, int PACK>
 __global__ void __launch_bounds__(kThreads)
 hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, const float *weights, const T *drows, T *dx,
                   float *dweights) {
+    using V = typename Values<PACK>::V;
+    constexpr int N = Values<PACK>::kCount;
     __shared__ float dots[kWarps][TB_ROUTE_MAX_TOP_K];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % warps;
     const size_t t = static_cast<size_t>(blockIdx.x) * (kWarps / warps) + warp / warps;
@@ -63,10 +65,15 @@ hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, c
         for (size_t base = static_cast<size_t>(part) * 32 * PACK; base < d.width; base += static_cast<size_t>(warps) * 32 * PACK) {
             const size_t c = base + lane * PACK;
             const bool in = c < d.width;
-            float g[PACK], sum[PACK];
+            Array<PACK> g, sum;
+            {
+                float e[PACK];
+                Held<T, PACK> v{};
+                if (dweights && in) v = *reinterpret_cast<const Held<T, PACK> *>(x + t * d.token_stride + c);
+                unpack(v, e);
 #pragma unroll
-            for (int i = 0; i < PACK; ++i) g[i] = sum[i] = 0.0f;
-            if (dweights && in) unpack(*reinterpret_cast<const Held<T, PACK> *>(x + t * d.token_stride + c), g);
+                for (int i = 0; i < N; ++i) g[i] = vload<V>(e + 2 * i), sum[i] = vall<V>(0.0f);
+            }
             for (int j = 0; j < d.top_k; j += kAhead) {
                 Held<T, PACK> v[kAhead];
                 int32_t row[kAhead];
@@ -79,16 +86,21 @@ hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, c
                 float dot[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const float s = __shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1));
+                    const V s = vall<V>(__shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1)));
                     dot[k] = 0.0f;
                     if (row[k] < 0) continue;
                     float e[PACK];
                     unpack(v[k], e);
+                    V of = vall<V>(0.0f);
 #pragma unroll
-                    for (int i = 0; i < PACK; ++i) {
-                        sum[i] = fmaf(s, e[i], sum[i]);
-                        dot[k] = fmaf(g[i], e[i], dot[k]);
+                    for (int i = 0; i < N; ++i) {
+                        const V r = vload<V>(e + 2 * i);
+                        sum[i] = vfma(s, r, sum[i]);
+                        of = vfma(g[i], r, of);
                     }
+                    float both[2] = {0.0f, 0.0f};
+                    vstore(both, of);
+                    dot[k] = both[0] + both[1];
                 }
                 if (dweights) { /* each half of the warp sums half of the slots, and so on, down to eight lanes a slot */
                     int spread = 16;
@@ -106,7 +118,12 @@ hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, c
                     if (lane % (32 / kAhead) == 0 && slot < d.top_k) dots[warp][slot] += dot[0];
                 }
             }
-            if (dx && in) *reinterpret_cast<Held<T, PACK> *>(dx + t * d.token_stride + c) = packed<T, PACK>(sum);
+            if (dx && in) {
+                float e[PACK];
+#pragma unroll
+                for (int i = 0; i < N; ++i) vstore(e + 2 * i, sum[i]);
+                *reinterpret_cast<Held<T, PACK> *>(dx + t * d.token_stride + c) = packed<T, PACK>(e);
+            }
         }
     if (!dweights) return;
     __syncthreads();

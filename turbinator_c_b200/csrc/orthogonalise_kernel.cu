@@ -34,6 +34,7 @@ constexpr float kDown = 1.0f / 4096.0f;
 struct Pair {
     __half *at;
     size_t line, matrix, plane;
+    __device__ __forceinline__ float get(size_t i) const { return __half2float(at[i]) + __half2float(at[plane + i]); }
     __device__ __forceinline__ void put(size_t i, float v) const {
         const __half high = __float2half_rn(v);
         at[i] = high;
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kNormThreads) normalise(Given d, const T *g, c
 /* Tiles of a matrix [height, width] of the output; symmetric: those that touch
  * m >= n, each mirrored where the tile across the diagonal is not computed. */
 struct Plan {
-    int matrices, width, height, depth, tile_m, tile_n; /* symmetric: tiles of 128 or 256 */
+    int matrices, width, height, depth, tile_m, tile_n;
     bool symmetric;
     int tiles_m, per;
 
@@ -204,7 +205,8 @@ struct SquareJob {
     using Shared = Nothing;
     CUtensorMap out, old; /* boxes of 32 x 32 */
     Plan plan;
-    bool second; /* S */
+    Pair to, from; /* the same */
+    bool second;   /* S */
     float b, c;
     __device__ void setup(Shared &) const {}
     __device__ int tiles(const Shared &) const { return plan.matrices * plan.per; }
@@ -234,6 +236,31 @@ struct SquareJob {
         }
         return true;
     }
+    __device__ __forceinline__ void store_joined(const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
+        if (m >= plan.width) return;
+        const size_t base = t.which * to.matrix;
+        __half *down = to.at + base + (t.n0 + c0) * to.line + m;
+        const size_t was = base + (t.n0 + c0) * from.line + m;
+        Pack<__half, 8> high, low;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float e = __uint_as_float(r[i]) * kDown;
+            if (second && c0 + i < t.columns) e = fmaf(c, e, b * from.get(was + i * from.line));
+            high.v[i] = __float2half_rn(e);
+            low.v[i] = __float2half_rn(e - __half2float(high.v[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < t.columns) {
+                down[i * to.line] = high.v[i];
+                down[to.plane + i * to.line] = low.v[i];
+            }
+        if (plan.mirrored(t, m, c0)) { /* a line's end is a multiple of eight */
+            __half *across = to.at + base + m * to.line + t.n0 + c0;
+            *reinterpret_cast<Pack<__half, 8> *>(across) = high;
+            *reinterpret_cast<Pack<__half, 8> *>(across + to.plane) = low;
+        }
+    }
 };
 
 /* x = a x + S x; the last step's goes to the output. */
@@ -243,6 +270,7 @@ template <class T> struct StepJob {
     using Shared = Nothing;
     CUtensorMap x, next; /* boxes of 32 x 32 */
     Plan plan;
+    Pair to, from; /* the same */
     T *last; /* or NULL */
     size_t row_stride, matrix_stride;
     float a, scale;
@@ -270,6 +298,20 @@ template <class T> struct StepJob {
             s.store(&next, left, y, t.which, plan.matrices, kBoxBytes);
         }
         return true;
+    }
+    __device__ __forceinline__ void store_joined(const Tile &t, int m, int c0, const uint32_t (&r)[8]) const {
+        if (m >= plan.width) return;
+        const size_t n = t.n0 + c0, at = t.which * from.matrix + n * from.line + m;
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            e[i] = c0 + i < t.columns ? fmaf(a, from.get(at + i * from.line), __uint_as_float(r[i]) * kDown) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < t.columns) {
+                if (last) last[t.which * matrix_stride + (n + i) * row_stride + m] = from_float<T>(e[i] * kDown * scale);
+                else to.put(at + i * to.line, e[i]);
+            }
     }
 };
 
@@ -311,16 +353,23 @@ Matrices matrices_of(const Pair &p, size_t matrices, size_t rows, size_t width) 
     return Matrices{p.at, width, rows, matrices * 2, p.line, p.matrix, 2};
 }
 
-/* Tiles that know which of them a symmetric product needs have 128 or 256 columns. */
-bool half_needed(size_t small, int columns) { return small > static_cast<size_t>(tb_tensor::kRows) && columns >= tb_tensor::kRows; }
+/* A symmetric product of one tile of rows has nothing across its diagonal to leave out. */
+bool half_needed(size_t small) { return small > static_cast<size_t>(tb_tensor::kRows); }
 
 tb_tensor::Fit plan_fit(int matrices, size_t height, size_t width, size_t depth, bool square, bool outer) {
     const auto tiles = [&](int columns, int m) {
-        Plan plan{matrices, static_cast<int>(width), static_cast<int>(height), 0, m, columns, square && half_needed(height, columns)};
+        Plan plan{matrices, static_cast<int>(width), static_cast<int>(height), 0, m, columns, square && half_needed(height)};
         plan.count();
         return static_cast<size_t>(matrices) * plan.per;
     };
-    return tb_tensor::best_fit(2, outer ? 64 : 32, height, (depth + 63) / 64, false, tiles, tiles);
+    return tb_tensor::best_fit(2, outer ? 64 : 32, height, (depth + 63) / 64, true, tiles, tiles);
+}
+
+tb_tensor::Fit square_fit(const OrthogonalShape &s, bool first) {
+    return plan_fit(static_cast<int>(s.matrices), s.small, s.small, !first ? s.small : s.tall ? s.rows : s.columns, true, first && s.tall);
+}
+tb_tensor::Fit step_fit(const OrthogonalShape &s) {
+    return plan_fit(static_cast<int>(s.matrices), s.rows, s.columns, s.small, false, false);
 }
 
 } /* namespace */
@@ -328,7 +377,8 @@ tb_tensor::Fit plan_fit(int matrices, size_t height, size_t width, size_t depth,
 extern "C" size_t tb_cuda_orthogonalise_workspace(const tb_orthogonalise_desc *desc) {
     OrthogonalShape s;
     if (!orthogonal_shape(desc, &s)) return 0;
-    return sums_bytes(s.matrices) + 2 * pair_bytes(s.matrices, s.rows, s.columns) + 2 * pair_bytes(s.matrices, s.small, s.small);
+    return sums_bytes(s.matrices) + 2 * pair_bytes(s.matrices, s.rows, s.columns) + 2 * pair_bytes(s.matrices, s.small, s.small) +
+           std::max({square_fit(s, true).room(), square_fit(s, false).room(), step_fit(s).room()});
 }
 
 extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, const void *g, void *out, void *workspace,
@@ -351,7 +401,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
     Pair x = take_pair(&scratch, s.matrices, s.rows, s.columns), next = take_pair(&scratch, s.matrices, s.rows, s.columns);
     const Pair square = take_pair(&scratch, s.matrices, s.small, s.small), poly = take_pair(&scratch, s.matrices, s.small, s.small);
     ops.type = 0;
-    ops.parts = 1;
+    ops.sums = reinterpret_cast<uint32_t *>(scratch);
     ops.a_plane = ops.b_plane = static_cast<int>(s.matrices);
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
@@ -374,43 +424,48 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         for (int step = 0; step < desc->steps; ++step) {
             const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns), mn = matrices_of(next, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
-            const int squared = tb_tensor::with_fit<2>(plan_fit(z, s.small, s.small, (s.tall ? s.rows : s.columns), true, s.tall), [&](auto n, auto pair) {
-                constexpr int NT = decltype(n)::value;
-                constexpr bool PAIR = decltype(pair)::value;
-                SquareJob job{};
-                job.plan = Plan{z, small, small, s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, half_needed(s.small, NT)};
-                job.plan.count();
-                const size_t tiles = static_cast<size_t>(z) * job.plan.per;
-                if (!tb_tensor::encode<NT, PAIR>(&ops, mx, s.tall, mx, s.tall) || !tb_tensor::encode(&job.out, ma, 32, 32) ||
-                    !tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st))
-                    return 0;
-                job.plan.depth = small;
-                job.old = job.out;
-                job.second = true;
-                job.b = desc->b;
-                job.c = desc->c;
-                return tb_tensor::encode<NT, PAIR>(&ops, ma, false, ma, false) && tb_tensor::encode(&job.out, mp, 32, 32) &&
-                               tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
-                           ? 1 : 0;
-            });
-            if (!squared) return 0;
-            const int stepped = tb_tensor::with_fit<2>(plan_fit(z, s.rows, s.columns, s.small, false, false), [&](auto n, auto pair) {
+            for (const bool first : {true, false}) {
+                const tb_tensor::Fit fit = square_fit(s, first);
+                const int squared = tb_tensor::with_fit<2>(fit, [&](auto n, auto pair) {
+                    constexpr int NT = decltype(n)::value;
+                    constexpr bool PAIR = decltype(pair)::value;
+                    SquareJob job{};
+                    job.plan = Plan{z, small, small, !first ? small : s.tall ? high : wide, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, half_needed(s.small)};
+                    job.plan.count();
+                    job.to = first ? square : poly;
+                    job.from = square;
+                    job.second = !first;
+                    job.b = desc->b;
+                    job.c = desc->c;
+                    ops.parts = fit.parts;
+                    const Matrices &from = first ? mx : ma;
+                    return tb_tensor::encode<NT, PAIR>(&ops, from, first && s.tall, from, first && s.tall) &&
+                                   tb_tensor::encode(&job.out, first ? ma : mp, 32, 32) && tb_tensor::encode(&job.old, ma, 32, 32) &&
+                                   tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, fit.tiles, sms, st)
+                               ? 1 : 0;
+                });
+                if (!squared) return 0;
+            }
+            const tb_tensor::Fit fit = step_fit(s);
+            ops.parts = fit.parts;
+            const int stepped = tb_tensor::with_fit<2>(fit, [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;
                 constexpr bool PAIR = decltype(pair)::value;
                 StepJob<T> job{};
                 job.plan = Plan{z, wide, high, small, tb_tensor::Shape<NT, 2, PAIR>::kTileM, NT, false};
                 job.plan.count();
+                job.to = next;
+                job.from = x;
                 job.last = step + 1 == desc->steps ? static_cast<T *>(out) : nullptr;
                 job.row_stride = s.out_row;
                 job.matrix_stride = s.out_matrix;
                 job.a = desc->a;
                 job.scale = desc->scale;
-                const size_t tiles = static_cast<size_t>(z) * job.plan.per;
                 /* x S: A is S (its own transpose), B is x; S x: A is x with its columns as m, B is S */
                 return (s.tall ? tb_tensor::encode<NT, PAIR>(&ops, mp, false, mx, false)
                                : tb_tensor::encode<NT, PAIR>(&ops, mx, true, mp, false)) &&
                                tb_tensor::encode(&job.x, mx, 32, 32) && tb_tensor::encode(&job.next, mn, 32, 32) &&
-                               tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, tiles, sms, st)
+                               tb_tensor::launch_products<NT, 2, false, PAIR>(ops, job, fit.tiles, sms, st)
                            ? 1 : 0;
             });
             if (!stepped) return 0;

@@ -563,7 +563,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
 #pragma unroll
                 for (int i = 0; i < S::kShare; ++i) sum[i] = 0.0f;
                 if constexpr (Job::kStaging != 0)
-                    if (columns > 0) job.ask(tile, m, c0, staging);
+                    if (columns > 0 && ops.parts == 1) job.ask(tile, m, c0, staging);
                 for (int k = 0; ok && (k < tile.depth || k == 0); k += kSegment * kDepth, ++number) {
                     const uint32_t buffer = number & 1;
                     if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
@@ -588,8 +588,14 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                             float v[32];
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = sum[c + i];
-                            ok = job.store(tile, m, c0 + c, v, staging);
-                            if (ok && c + 32 < columns) job.ask(tile, m, c0 + c + 32, staging);
+                            if (ops.parts == 1) {
+                                ok = job.store(tile, m, c0 + c, v, staging);
+                                if (ok && c + 32 < columns) job.ask(tile, m, c0 + c + 32, staging);
+                            } else {
+                                uint32_t *to = ops.sums + (static_cast<size_t>(t) * NT + c0 + c) * S::kTileM + (m - tile.m0);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) to[i * S::kTileM] = __float_as_uint(v[i]);
+                            }
                         }
                 } else {
 #pragma unroll
@@ -666,7 +672,8 @@ __global__ void __launch_bounds__(TM) join_parts(const __grid_constant__ Job job
             else r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(v));
         }
     }
-    job.store(shared, tile, tile.m0 + threadIdx.x, c, r);
+    if constexpr (Job::kStaging == 0) job.store(shared, tile, tile.m0 + threadIdx.x, c, r);
+    else job.store_joined(tile, tile.m0 + threadIdx.x, c, r);
 }
 
 /* ---- host side ---- */
@@ -739,11 +746,13 @@ constexpr size_t kMostRoom = 64u << 20;
  * as there are go round the SMs in so many turns; a block of k takes as long as
  * its products (two cycles a column, times the pairs of planes) or its copies
  * (some 46 bytes a cycle and SM); every turn some 2,000 for what is not hidden
- * of its beginning and end, and parts a second kernel and their sums' way
+ * of its beginning and end, 90 more for each of a storing warp's columns where
+ * their sums leave no room for the next tile's, and parts a second kernel and their sums' way
  * through L2.  count(columns, m) says how many tiles of so many columns by m
  * there are likely to be, `average` how many columns one has of them, most(columns, m) how
  * many there may be; least: 64 where n is contiguous in b.
- * 1 x 4,096 x 4,096 of 8 bits: 14.5 us in one part, 11.0 in four (in a graph). */
+ * An update of 2 x 1,792 x 242 f32 takes 222 us in one part, 172 in several; one
+ * of 2,501 x 1,537 the same either way. */
 template <class Count, class Most>
 Fit best_fit(int planes, int least, size_t average, size_t blocks, bool may_part, Count &&count, Most &&most) {
     Fit best{0, false, 1, 0};
@@ -755,13 +764,14 @@ Fit best_fit(int planes, int least, size_t average, size_t blocks, bool may_part
         const double products = 2.0 * taken * (planes * (planes + 1) / 2);
         const double copies = planes * kBlockBytes * (kRows + columns / (pair ? 2.0 : 1.0)) / 46.0;
         const double block = products > copies ? products : copies;
+        const double ends = 2000.0 + (planes > 1 ? 90.0 * (columns == 256 ? 128 : columns == 128 ? 64 : 32) : 0.0);
         for (int parts = 1; parts <= 64 && (parts == 1 || may_part); parts += parts < 4 ? 1 : parts / 2) {
             const size_t per = (blocks + parts - 1) / parts;
             if (parts > 1 && per < 4) break;
             const double turns = static_cast<double>(static_cast<size_t>((tiles * parts + units - 1) / units));
-            double cost = turns * (per * block + 2000.0);
+            double cost = turns * (per * block + ends);
             Fit fit{columns, pair, parts, most(columns, m)};
-            if (parts > 1) cost += 5000.0 + tiles * parts * taken * m * 8.0 / (kSms * 40.0);
+            if (parts > 1) cost += (planes > 1 ? 12000.0 : 8000.0) + tiles * parts * taken * m * 8.0 / (kSms * 20.0);
             if (fit.room() > kMostRoom) break;
             if (best.columns == 0 || cost < lowest) {
                 lowest = cost;
@@ -803,12 +813,10 @@ int launch_products(const Operands &ops, const Job &job, size_t tiles, int sms, 
     const size_t most = static_cast<size_t>(sms) / kCtas, all = tiles * ops.parts;
     const unsigned grid = static_cast<unsigned>(all < most ? all : most) * kCtas;
     if (!tb_learn::launch_early(kernel, grid, Shape<NT, PLANES, PAIR>::kThreads, kShared, kCtas, st, ops, job)) return 0;
-    if constexpr (Job::kStaging == 0) {
-        if (ops.parts > 1) {
-            constexpr int TM = Shape<NT, PLANES, PAIR>::kTileM;
-            return tb_learn::launch_early(join_parts<Job, NT, TM, I8>, dim3(static_cast<unsigned>(tiles), NT / 8), TM, 0, 1, st, job,
-                                          ops.parts, static_cast<const uint32_t *>(ops.sums));
-        }
+    if (ops.parts > 1) {
+        constexpr int TM = Shape<NT, PLANES, PAIR>::kTileM;
+        return tb_learn::launch_early(join_parts<Job, NT, TM, I8>, dim3(static_cast<unsigned>(tiles), NT / 8), TM, 0, 1, st, job,
+                                      ops.parts, static_cast<const uint32_t *>(ops.sums));
     }
     return 1;
 }
