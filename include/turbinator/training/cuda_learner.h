@@ -7,6 +7,9 @@
  *   gated linear recurrence with resets              forward (one step included), backward
  *   routing to experts with slot lists               forward, backward
  *   combining the experts' rows into their tokens    forward, backward
+ *   handing tokens out to the experts                forward, backward
+ *   the experts' products                            forward, backward; in 8 bits for acting
+ *   orthogonalised updates of their matrices
  *
  * Conventions (those of cuda_features.h): device pointers, row-major, the
  * last dimension contiguous; `stream` is a cudaStream_t or NULL for the legacy
@@ -16,8 +19,8 @@
  * limits, a stride smaller than its row, a pointer not aligned to its
  * element, an output or a workspace at the address of an input or of another
  * output where that is not stated) or a launch error.
- * The recurrence's kernels wait for copies of their own, for a second at most;
- * where that runs out their results are wrong, and tb_cuda_synchronize(stream)
+ * The recurrence's and the products' kernels wait for copies of their own, for a
+ * second at most; where that runs out their results are wrong, and tb_cuda_synchronize(stream)
  * (cuda_features.h) says so by returning 0.
  * A descriptor is read during the call only.  Strides are in elements, 0 means
  * dense.  Tensors of `type` may be f32, bf16 or f16; parameters, statistics,
@@ -221,7 +224,7 @@ int tb_cuda_combine_experts_backward_device(const tb_expert_combine_desc *desc, 
 /* The way out that the combine is the way back of, with the same descriptor:
  * rows_stride is that of rows and drows, out_stride that of x and dx.
  *   rows[p] = weights[s] x[s / top_k],  s = order[p] (a slot of the lists above)
- * for every p in [0, rows).  A row whose slot lies outside [0, tokens*top_k)
+ * for every p in [0, rows): order has that many entries.  A row whose slot lies outside [0, tokens*top_k)
  * (-1 past the lists' end) is left as it was.  With weights NULL every weight is
  * 1. */
 int tb_cuda_hand_out_experts_device(const tb_expert_combine_desc *desc, const void *x, const int32_t *order,
@@ -248,10 +251,9 @@ int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_desc *desc,
  * all rows are its.
  *   y[p] = x[p] W_e
  * Rows of y and dx that are no expert's are left as they were, and what those of
- * x and dy hold is not used.  Products are summed in f32 on the tensor cores;
- * f32 tensors are multiplied as three bf16 parts each, which leaves out less
- * than 2^-23 of the sum of the products' magnitudes, and an infinity in one
- * gives NaN. */
+ * x and dy hold is not used.  All sums are f32.  On the tensor cores f32 tensors
+ * are multiplied as three bf16 parts each, which leaves out less than 2^-23 of
+ * the sum of the products' magnitudes; an infinity in one may give NaN there. */
 typedef struct tb_expert_product_desc {
     size_t rows, experts, in_width, out_width;
     size_t in_stride, din_stride; /* of the rows of x; of dx */

@@ -3,7 +3,10 @@
  * gradient (include/turbinator/training/cuda_learner.h).
  *
  * Bound: HBM; a row of the output is written once, a token's row read from L2
- * by all but the first of its slots.  The gradient reads every slot's row once.
+ * by all but the first of its slots.  The gradient reads every slot's row once: of
+ * 16,384 tokens x 8 slots x 1,024 bf16, a tenth without slots, in 78 us, 4.3 TB/s
+ * (eight rows ahead 137, in 64 registers for four CTAs an SM 86: the loads under
+ * way are what counts).
  */
 #include "tb_learner.cuh"
 
@@ -13,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 4; /* rows of a token under way at once; eight: 137 us for 78 (registers) */
+constexpr int kAhead = 4; /* rows of a token under way at once */
 
 struct HandShape {
     size_t tokens, rows, width, rows_stride, token_stride;

@@ -161,7 +161,7 @@ template <class T, int NT> struct SumJob {
 
 /* Where the rows are few, as in acting, the weights are what is read, once, and
  * a product is a warp's sum over a row of weights, against up to four rows. */
-constexpr int kFewThreads = 256, kFewRows = 4, kFewWide = 148;
+constexpr int kFewThreads = 256, kFewRows = 4;
 
 /* The dot product of 16 bytes (or 4, or an element) of weights and a row. */
 template <class T, int PACK> struct FewPack {
@@ -281,15 +281,17 @@ few_rows(FewShape d, Runs runs, const W *x, const W *weight, T *out, const float
     }
 }
 
-/* The same where the weights lie the other way, [sum][channel]: lanes take
- * neighbouring channels, a CTA's warps every so-many-th k, and their sums meet
- * in shared memory. */
-constexpr int kAcrossThreads = 256, kAcrossWarps = kAcrossThreads / 32;
-template <class T, int PACK>
-__global__ void __launch_bounds__(kAcrossThreads) few_rows_across(FewShape d, Runs runs, const T *x, const T *weight, T *out) {
-    __shared__ float parts[kAcrossWarps][kFewRows][32 * PACK + 1];
-    constexpr int kAhead = 4; /* rows of weights under way at once */
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, m = (blockIdx.x * 32 + lane) * PACK;
+/* The same where the weights lie the other way, [sum][channel]: a lane takes a
+ * channel, a CTA's 32 warps every 32nd k, and their sums meet in shared memory.
+ * For f32 alone (1 x 4,096 x 4,096: 27 us against 72 on the tensor cores; 16
+ * bytes a lane: 61): of 16 bits the tensor cores' parts of a sum are faster (bf16
+ * 9 us, this way 30). */
+constexpr int kAcrossThreads = 1024, kAcrossWarps = kAcrossThreads / 32;
+__global__ void __launch_bounds__(kAcrossThreads)
+few_rows_across(FewShape d, Runs runs, const float *x, const float *weight, float *out) {
+    __shared__ float parts[kAcrossWarps][kFewRows][32];
+    constexpr int kAhead = 8; /* rows of weights under way at once */
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, m = blockIdx.x * 32 + lane;
     const int last = min(static_cast<int>(blockIdx.y + 1) * kFewRows, runs.rows);
     after_earlier();
     for (int row = blockIdx.y * kFewRows, count; row < last; row += count) {
@@ -297,40 +299,30 @@ __global__ void __launch_bounds__(kAcrossThreads) few_rows_across(FewShape d, Ru
         const int e = expert_of(runs, row, last, lane, &end);
         count = e < 0 ? 1 : min(end, last) - row;
         if (e < 0) continue; /* no expert's: left as it was */
-        const T *w = weight + e * d.w_matrix + m, *from = x + row * d.x_stride;
-        float sum[kFewRows][PACK] = {};
+        const float *w = weight + e * d.w_matrix + m, *from = x + row * d.x_stride;
+        float sum[kFewRows] = {};
         if (m < d.width)
             for (int k = warp; k < d.depth; k += kAcrossWarps * kAhead) {
-                Held<T, PACK> h[kAhead];
+                float a[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
-                    if (k + i * kAcrossWarps < d.depth) h[i] = load_once<T, PACK>(w + (k + i * kAcrossWarps) * d.w_row);
+                    if (k + i * kAcrossWarps < d.depth) a[i] = __ldcs(w + (k + i * kAcrossWarps) * d.w_row);
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
                     if (k + i * kAcrossWarps >= d.depth) break;
-                    float a[PACK];
-                    unpack(h[i], a);
 #pragma unroll
                     for (int r = 0; r < kFewRows; ++r)
-                        if (r < count) {
-                            const float b = to_float(from[r * d.x_stride + k + i * kAcrossWarps]);
-#pragma unroll
-                            for (int j = 0; j < PACK; ++j) sum[r][j] = fmaf(a[j], b, sum[r][j]);
-                        }
+                        if (r < count) sum[r] = fmaf(a[i], from[r * d.x_stride + k + i * kAcrossWarps], sum[r]);
                 }
             }
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r)
-#pragma unroll
-            for (int j = 0; j < PACK; ++j) parts[warp][r][lane * PACK + j] = sum[r][j];
+        for (int r = 0; r < kFewRows; ++r) parts[warp][r][lane] = sum[r];
         __syncthreads();
-        for (int i = threadIdx.x; i < count * 32 * PACK; i += kAcrossThreads) {
-            const int r = i / (32 * PACK), c = i % (32 * PACK);
+        if (warp < count && m < d.width) {
             float v = 0.0f;
 #pragma unroll
-            for (int p = 0; p < kAcrossWarps; ++p) v += parts[p][r][c];
-            const int at = blockIdx.x * 32 * PACK + c;
-            if (at < d.width) out[(row + r) * d.out_stride + at] = from_float<T>(v);
+            for (int p = 0; p < kAcrossWarps; ++p) v += parts[p][warp][lane];
+            out[(row + warp) * d.out_stride + m] = v;
         }
         __syncthreads();
     }
@@ -367,13 +359,15 @@ few_sums(int width, int height, size_t line_stride, size_t column_stride, size_t
 }
 
 /* Up to eight rows, and some 2^25 products of theirs: 1 x 4,096 x 4,096 of 8 bits
- * 6.6 us against 9.0 by tiles, of bf16 7.2 against 10.0, 8 x 1,024 x 1,024 4.4
- * against 5.5; 4 x 4,096 x 4,096 12 against 9.  f32 weights are laid out as
- * planes for the tensor cores, 16 bytes moved for each of 4: rows up to a dozen
- * an expert (8 x 4,096 x 4,096: 32 us against 72). */
-bool few(size_t rows, size_t experts, size_t in, size_t out, bool wide) {
-    if (wide) return rows <= 12 * experts;
-    return rows <= 8 && static_cast<double>(rows) * in * out <= 33554432.0;
+ * 6.2 us against 7.7 by tiles, of bf16 6.7 against 9.1, 8 x 1,024 x 1,024 4.0
+ * against 4.8; 8 x 8,192 x 8,192 47 against 12.  f32 weights are laid out as planes
+ * for the tensor cores, 16 bytes moved for each of 4: rows up to a dozen an expert
+ * (8 x 4,096 x 4,096: 32 us against 72), up to four where the weights' rows lie
+ * across the sum (4 x 4,096 x 4,096: 30 against 72, 8: 57). */
+bool few(size_t rows, size_t experts, size_t in, size_t out, bool wide, bool across) {
+    if (in > 1u << 30 || out > 1u << 30) return false; /* 32-bit places, some packs ahead */
+    if (wide) return rows <= (across ? 4 : 12) * experts;
+    return !across && rows <= 8 && static_cast<double>(rows) * in * out <= 33554432.0;
 }
 
 template <class W, class T>
@@ -392,17 +386,9 @@ int few_product(const FewShape &d, const Runs &runs, const W *x, const W *weight
     return launch(std::integral_constant<int, 1>{});
 }
 
-template <class T>
-int few_product_across(const FewShape &d, const Runs &runs, const T *x, const T *weight, T *out, cudaStream_t st) {
-    const size_t bits = reinterpret_cast<uintptr_t>(weight) | (d.w_row | d.w_matrix | static_cast<size_t>(d.width)) * sizeof(T);
-    int pack = pack_of(bits, sizeof(T));
-    /* narrower where that gives every SM a CTA */
-    if (pack > 1 && d.width < 32 * pack * kFewWide) pack = bits % 4 == 0 && pack > 4 / static_cast<int>(sizeof(T)) ? 4 / static_cast<int>(sizeof(T)) : pack;
-    return with_pack<T>(pack, [&](auto p) {
-        constexpr int P = decltype(p)::value;
-        const dim3 grid(static_cast<unsigned>((d.width + 32 * P - 1) / (32 * P)), static_cast<unsigned>((runs.rows + kFewRows - 1) / kFewRows));
-        return launch_early(few_rows_across<T, P>, grid, kAcrossThreads, 0, 1, st, d, runs, x, weight, out);
-    });
+inline int few_product_across(const FewShape &d, const Runs &runs, const float *x, const float *weight, float *out, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>((d.width + 31) / 32), static_cast<unsigned>((runs.rows + kFewRows - 1) / kFewRows));
+    return launch_early(few_rows_across, grid, kAcrossThreads, 0, 1, st, d, runs, x, weight, out);
 }
 
 /* Rows of lines and columns; out [experts][height][width]. */
@@ -536,7 +522,7 @@ bool product_shape(const tb_expert_product_desc *d, ProductShape *s) {
     return s->x_stride >= s->in && s->dx_stride >= s->in && s->y_stride >= s->out && s->w_matrix >= all &&
            product(s->rows, s->x_stride, SIZE_MAX / 64, &all) && product(s->rows, s->dx_stride, SIZE_MAX / 64, &all) &&
            product(s->rows, s->y_stride, SIZE_MAX / 64, &all) && product(s->experts, s->w_matrix, SIZE_MAX / 64, &all) &&
-           product(s->experts * ((s->in + 127) / 128), (s->out + 63) / 64, 0x7fffffffu, &all) &&
+           product(s->experts * ((s->in + 63) / 64), (s->out + 63) / 64, 0x7fffffffu, &all) &&
            product((s->out + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all) &&
            product((s->in + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all);
 }
@@ -616,10 +602,12 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) -> int {
         using T = decltype(t);
-        if (!s.turned && few(s.rows, s.experts, s.in, s.out, s.wide))
-            return few_product_across<T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
-                                         static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), st);
-        if (few(s.rows, s.experts, s.in, s.out, s.wide))
+        const bool by_rows = few(s.rows, s.experts, s.in, s.out, s.wide, !s.turned);
+        if constexpr (sizeof(T) == 4)
+            if (!s.turned && by_rows)
+                return few_product_across({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
+                                             static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), st);
+        if (s.turned && by_rows)
             return few_product<T, T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,
                                      static_cast<const T *>(x), static_cast<const T *>(weight), static_cast<T *>(y), nullptr, nullptr, st);
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
@@ -653,17 +641,24 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
     return with_type(desc->type, [&](auto t) {
         using T = decltype(t);
-        if (few(s.rows, s.experts, s.in, s.out, s.wide)) {
+        const T *g = static_cast<const T *>(dy), *w = static_cast<const T *>(weight), *in = static_cast<const T *>(x);
+        if (dx && few(s.rows, s.experts, s.in, s.out, s.wide, s.turned)) {
             const FewShape d{static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.w_row, s.w_matrix, s.dx_stride};
-            const T *g = static_cast<const T *>(dy), *w = static_cast<const T *>(weight), *in = static_cast<const T *>(x);
-            T *dw = static_cast<T *>(dweight);
-            if (dx && !(s.turned ? few_product_across<T>(d, runs, g, w, static_cast<T *>(dx), st)
-                                 : few_product<T, T>(d, runs, g, w, static_cast<T *>(dx), nullptr, nullptr, st)))
-                return 0;
-            if (!dweight) return 1;
-            return s.turned ? few_gradient<T>(static_cast<int>(s.in), static_cast<int>(s.out), s.y_stride, s.x_stride, s.w_row, s.w_matrix, runs, g, in, dw, st)
-                            : few_gradient<T>(static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.y_stride, s.w_row, s.w_matrix, runs, in, g, dw, st);
+            int ok = 0;
+            if (!s.turned) ok = few_product<T, T>(d, runs, g, w, static_cast<T *>(dx), nullptr, nullptr, st);
+            if constexpr (sizeof(T) == 4)
+                if (s.turned) ok = few_product_across(d, runs, g, w, static_cast<T *>(dx), st);
+            if (!ok) return 0;
+            dx = nullptr;
         }
+        if (dweight && few(s.rows, s.experts, s.in, s.out, s.wide, false)) {
+            const int width = static_cast<int>(s.turned ? s.in : s.out), height = static_cast<int>(s.turned ? s.out : s.in);
+            if (!few_gradient<T>(width, height, s.turned ? s.y_stride : s.x_stride, s.turned ? s.x_stride : s.y_stride, s.w_row, s.w_matrix, runs,
+                                 s.turned ? g : in, s.turned ? in : g, static_cast<T *>(dweight), st))
+                return 0;
+            dweight = nullptr;
+        }
+        if (!dx && !dweight) return 1;
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx, my;
         Layouts all{};
@@ -759,8 +754,8 @@ quantise_rows(size_t rows, size_t width, size_t x_stride, size_t q_stride, const
     for (size_t c = first + HELD * step; c < width; c += step) put(c, *reinterpret_cast<const Held<T, PACK> *>(from + c));
     if (lane == 0) scale[row] = bad ? __int_as_float(0x7fc00000) : none ? 0.0f : __fdiv_rn(m, 127.0f);
 }
-/* Rows for all warps of the GPU, each held by its warp: 16,384 x 4,096 bf16
- * WARPUS us, a CTA a row 50. */
+/* Rows for all warps of the GPU, each held by its warp: 16,384 x 4,096 bf16 43 us, a
+ * CTA a row 50. */
 constexpr size_t kQuantManyRows = 2048;
 
 struct IntegerShape {
@@ -844,7 +839,7 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
     cudaGetLastError(); /* report these launches only */
     ops.type = 1;
     const Runs runs{offsets, static_cast<int>(s.experts), static_cast<int>(s.rows)};
-    if (few(s.rows, s.experts, s.in, s.out, false))
+    if (few(s.rows, s.experts, s.in, s.out, false, false))
         return with_type(desc->type, [&](auto t) {
             using T = decltype(t);
             return few_product<int8_t, T>({static_cast<int>(s.out), static_cast<int>(s.in), s.x_stride, s.w_row, s.w_matrix, s.y_stride}, runs,

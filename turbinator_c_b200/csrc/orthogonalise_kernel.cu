@@ -421,11 +421,12 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
         if (!normalised) return 0;
         const int z = static_cast<int>(s.matrices), small = static_cast<int>(s.small);
         const int wide = static_cast<int>(s.columns), high = static_cast<int>(s.rows);
+        const tb_tensor::Fit square_fits[2] = {square_fit(s, true), square_fit(s, false)}, whole_fit = step_fit(s);
         for (int step = 0; step < desc->steps; ++step) {
             const Matrices mx = matrices_of(x, s.matrices, s.rows, s.columns), mn = matrices_of(next, s.matrices, s.rows, s.columns);
             const Matrices ma = matrices_of(square, s.matrices, s.small, s.small), mp = matrices_of(poly, s.matrices, s.small, s.small);
             for (const bool first : {true, false}) {
-                const tb_tensor::Fit fit = square_fit(s, first);
+                const tb_tensor::Fit &fit = square_fits[first ? 0 : 1];
                 const int squared = tb_tensor::with_fit<2>(fit, [&](auto n, auto pair) {
                     constexpr int NT = decltype(n)::value;
                     constexpr bool PAIR = decltype(pair)::value;
@@ -446,7 +447,7 @@ extern "C" int tb_cuda_orthogonalise_device(const tb_orthogonalise_desc *desc, c
                 });
                 if (!squared) return 0;
             }
-            const tb_tensor::Fit fit = step_fit(s);
+            const tb_tensor::Fit &fit = whole_fit;
             ops.parts = fit.parts;
             const int stepped = tb_tensor::with_fit<2>(fit, [&](auto n, auto pair) {
                 constexpr int NT = decltype(n)::value;

@@ -16,8 +16,11 @@
  * storing of one tile run under the products of the next.  Two CTAs on
  * neighbouring SMs share a tile of 256 m where there are as many (PAIR): each
  * brings its 128 rows of A and half of B's, so that a product's 128 x 256 x 64
- * take 32 KB from L2 and not 48.  L2 gave a lone CTA some 46 bytes a cycle
- * and SM at best.
+ * take 32 KB from L2 and not 48 (L2 gives some 45 to 51 bytes a cycle and SM):
+ * 131,072 rows x 1,024 x 2,048 bf16 425 us, 519 without pairs, 581 in tiles of
+ * 128 x 128.  There the power cap is what bounds it, 1.3 PFLOP/s of the 1.39 that
+ * a library's product keeps up; tiles of 256 x 512, whose products run without
+ * a pause, took as long at a lower clock.
  * CTAs (pairs) are persistent and take every so-many-th tile of a job.
  *
  * Operands of more than 16 bits come as planes that sum to them; a stage holds
@@ -36,7 +39,7 @@
  * is not 0, 32 columns of 32 rows by a warp with so many bytes of its own, into
  * which ask has asked for what it reads for them).
  *
- * Waits are bounded by a second; one that runs out reports
+ * Waits are bounded by a second (a tile's sums by 10 us a stage more); one that runs out reports
  * TB_FEATURE_STATUS_WAIT_TIMEOUT through the stream's status word, after which
  * every warp goes to its end: no further copies or products are asked for,
  * those under way are waited for (again with a bound) and the TMEM is freed.
@@ -251,7 +254,8 @@ template <int NT, int PLANES, bool PAIR, int STAGING = 0> struct Shape {
 struct Waits {
     unsigned *status;
     volatile int *gave_up; /* in shared memory */
-    __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) const {
+    /* stages: of work in front of what is waited for, some microseconds each at most. */
+    __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int stages = 0) const {
         /* the clock is read late: reading it takes longer than most waits */
         unsigned long long t0 = 0;
         for (;;) {
@@ -260,7 +264,7 @@ struct Waits {
             if (*gave_up) return false;
             const unsigned long long now = tb_pipe::global_ns();
             if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitNs) break;
+            else if (now - t0 > kWaitNs + stages * 10000ull) break;
         }
         if (!*gave_up) atomicOr(status, TB_FEATURE_STATUS_WAIT_TIMEOUT);
         *gave_up = 1;
@@ -610,7 +614,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 }
             } else {
                 const uint32_t buffer = number & 1;
-                if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
+                if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1, tile.depth / kDepth))) break;
                 tensor_fence_after();
                 for (int c = 0; c < columns; c += 32) {
                     uint32_t r[32];
