@@ -82,10 +82,10 @@ def orthogonalise(g, steps, a, b, c, epsilon, scale, noise=None):
 
 def orthogonalise_error(g, steps, a, b, c, epsilon, scale):
     """Bound on each element.  Every kept value is rounded to 22 bits (2^-22 of itself, or 2^-37), every product leaves
-    out 2^-21 of its magnitudes and adds them in sums that are cut every 128 of k: 8 instructions of three products
-    each, 4 U of the magnitudes each, so 2^-22 (2 + 24) < 2^-17 of them at worst, 2^-18 of them in the mean.  The steps
-    carry these errors on linearly; the definition with errors of that size and random signs says how far, and 16 times
-    the root mean square of what it does in four runs covers every element."""
+    out 2^-21 of its magnitudes and adds them in sums of 64 of k: 4 instructions of three products each, 4 U of the
+    magnitudes each, so 2^-22 (2 + 12) < 2^-18 of them at worst.  The steps carry these errors on linearly; the
+    definition with errors of that size and random signs says how far, and 16 times the root mean square of what it
+    does in four runs covers every element."""
     gen = torch.Generator(device=g.device)
     gen.manual_seed(99)
 
