@@ -412,6 +412,7 @@ struct Layout {
     size_t line;                                          /* of the copy: a multiple of 16 bytes */
     const void *from;
     void *to;
+    const int32_t *first, *last; /* of the rows that are any expert's, or NULL: all */
 };
 constexpr int kMostLayouts = 3;
 struct Layouts {
@@ -430,30 +431,55 @@ __device__ __forceinline__ void planes_of(float v, __nv_bfloat16 (&p)[3]) {
 }
 
 constexpr int kLayThreads = 256;
-/* A warp a line at a time, two neighbours a lane; blockIdx.y: of the tensors. */
+/* N neighbours of a line. */
+template <class T, int N> __device__ __forceinline__ void lay_some(const Layout &d, const T (&v)[N], size_t at, size_t plane) {
+    if constexpr (sizeof(T) == 4) {
+        Pack<__nv_bfloat16, N> part[3];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __nv_bfloat16 p[3];
+            planes_of(v[i], p);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) part[j].v[i] = p[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<Pack<__nv_bfloat16, N> *>(static_cast<__nv_bfloat16 *>(d.to) + at + j * plane) = part[j];
+    } else {
+        Pack<T, N> part;
+#pragma unroll
+        for (int i = 0; i < N; ++i) part.v[i] = v[i];
+        *reinterpret_cast<Pack<T, N> *>(static_cast<T *>(d.to) + at) = part;
+    }
+}
+/* A warp a line at a time, two neighbours a lane, or four where an f32 line
+ * lies on 16 bytes; blockIdx.y: of the tensors. */
 template <class T>
 __global__ void __launch_bounds__(kLayThreads) lay_out(const __grid_constant__ Layouts all) {
     const Layout &d = all.of[blockIdx.y];
     const size_t lines = d.rows * d.count, plane = lines * d.line;
     const int lane = threadIdx.x % 32;
-    for (size_t i = static_cast<size_t>(blockIdx.x) * (kLayThreads / 32) + threadIdx.x / 32; i < lines;
+    const size_t begin = d.first ? static_cast<size_t>(max(*d.first, 0)) : 0;
+    const size_t end = d.last ? min(static_cast<size_t>(max(*d.last, 0)), lines) : lines;
+    for (size_t i = begin + static_cast<size_t>(blockIdx.x) * (kLayThreads / 32) + threadIdx.x / 32; i < end;
          i += static_cast<size_t>(gridDim.x) * (kLayThreads / 32)) {
         const size_t z = d.count > 1 ? i / d.rows : 0, r = i - z * d.rows;
         const T *from = static_cast<const T *>(d.from) + z * d.matrix_stride + r * d.row_stride;
-        for (size_t c = lane * 2; c < d.line; c += 64) { /* a line's length is even */
-            T v[2] = {};
-            if (c < d.width) v[0] = from[c];
-            if (c + 1 < d.width) v[1] = from[c + 1];
-            if constexpr (sizeof(T) == 4) {
-                __nv_bfloat16 p[2][3];
-                planes_of(v[0], p[0]);
-                planes_of(v[1], p[1]);
-                __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(d.to) + i * d.line + c;
+        if (sizeof(T) == 4 && d.width % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+            for (size_t c = lane * 4; c < d.line; c += 128) { /* a line's length is a multiple of eight */
+                T v[4] = {};
+                if (c < d.width) {
+                    const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4> *>(from + c);
 #pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    *reinterpret_cast<Pack<__nv_bfloat16, 2> *>(to + j * plane) = Pack<__nv_bfloat16, 2>{{p[0][j], p[1][j]}};
-            } else {
-                *reinterpret_cast<Pack<T, 2> *>(static_cast<T *>(d.to) + i * d.line + c) = Pack<T, 2>{{v[0], v[1]}};
+                    for (int j = 0; j < 4; ++j) v[j] = p.v[j];
+                }
+                lay_some(d, v, i * d.line + c, plane);
+            }
+        } else {
+            for (size_t c = lane * 2; c < d.line; c += 64) {
+                T v[2] = {};
+                if (c < d.width) v[0] = from[c];
+                if (c + 1 < d.width) v[1] = from[c + 1];
+                lay_some(d, v, i * d.line + c, plane);
             }
         }
     }
@@ -463,6 +489,7 @@ __global__ void __launch_bounds__(kLayThreads) lay_out(const __grid_constant__ L
 struct Source {
     const void *at;
     size_t width, rows, count, row_stride, matrix_stride;
+    const int32_t *first = nullptr, *last = nullptr; /* of its rows that are any expert's */
 };
 /* Elements of a laid-out line, and bytes of the whole. */
 size_t line_of(size_t width, size_t size) { return align_up(width, 16 / size); }
@@ -476,7 +503,7 @@ template <class T> void lay(const Source &s, size_t size, unsigned char **scratc
     *m = Matrices{s.at, s.width, s.rows, s.count, s.row_stride, s.matrix_stride, size};
     if (!wide && m->straight()) return;
     const size_t line = line_of(s.width, size);
-    all->of[all->count++] = Layout{s.width, s.rows, s.count, s.row_stride, s.matrix_stride, line, s.at, *scratch};
+    all->of[all->count++] = Layout{s.width, s.rows, s.count, s.row_stride, s.matrix_stride, line, s.at, *scratch, s.first, s.last};
     *m = Matrices{*scratch, s.width, s.rows, s.count * (wide ? 3 : 1), line, line * s.rows, size};
     *scratch += laid_bytes(s.width, s.rows, s.count, wide, size);
 }
@@ -526,8 +553,11 @@ bool product_shape(const tb_expert_product_desc *d, ProductShape *s) {
            product((s->out + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all) &&
            product((s->in + 127) / 128, s->rows / 32 + s->experts, 0x7fffffffu, &all);
 }
-Source x_of(const ProductShape &s, const void *x) { return {x, s.in, s.rows, 1, s.x_stride, 0}; }
-Source y_of(const ProductShape &s, const void *y) { return {y, s.out, s.rows, 1, s.y_stride, 0}; }
+Source rows_of(const void *at, size_t width, size_t rows, size_t stride, const int32_t *offsets, size_t experts) {
+    return {at, width, rows, 1, stride, 0, offsets, offsets ? offsets + experts : nullptr};
+}
+Source x_of(const ProductShape &s, const void *x, const int32_t *offsets) { return rows_of(x, s.in, s.rows, s.x_stride, offsets, s.experts); }
+Source y_of(const ProductShape &s, const void *y, const int32_t *offsets) { return rows_of(y, s.out, s.rows, s.y_stride, offsets, s.experts); }
 Source w_of(const ProductShape &s, const void *w) {
     return {w, s.turned ? s.in : s.out, s.turned ? s.out : s.in, s.experts, s.w_row, s.w_matrix};
 }
@@ -582,7 +612,7 @@ extern "C" size_t tb_cuda_experts_product_workspace(const tb_expert_product_desc
     const size_t sums = std::max({rows_fit(planes, s.rows, s.experts, s.out, (s.in + 63) / 64).room(),
                                   rows_fit(planes, s.rows, s.experts, s.in, (s.out + 63) / 64).room(),
                                   sums_fit(planes, s.rows, s.experts, s.turned ? s.in : s.out, s.turned ? s.out : s.in).room()});
-    return laid_room(x_of(s, nullptr), s.wide) + laid_room(y_of(s, nullptr), s.wide) + laid_room(w_of(s, nullptr), s.wide) + sums;
+    return laid_room(x_of(s, nullptr, nullptr), s.wide) + laid_room(y_of(s, nullptr, nullptr), s.wide) + laid_room(w_of(s, nullptr), s.wide) + sums;
 }
 
 extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc, const void *x, const void *weight,
@@ -614,7 +644,7 @@ extern "C" int tb_cuda_experts_product_device(const tb_expert_product_desc *desc
         Matrices mw, mx;
         Layouts all{};
         lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
-        lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
+        lay<T>(x_of(s, x, offsets), 2, &scratch, &all, &mx);
         return laid<T>(all, sms, st) &&
                rows_product<T>(ops, mw, !s.turned, mx, runs, s.out, s.in, y, s.y_stride, scratch, sms, st);
     });
@@ -662,9 +692,9 @@ extern "C" int tb_cuda_experts_product_backward_device(const tb_expert_product_d
         unsigned char *scratch = static_cast<unsigned char *>(workspace);
         Matrices mw, mx, my;
         Layouts all{};
-        lay<T>(y_of(s, dy), 2, &scratch, &all, &my);
+        lay<T>(y_of(s, dy, offsets), 2, &scratch, &all, &my);
         if (dx) lay<T>(w_of(s, weight), 2, &scratch, &all, &mw);
-        if (dweight) lay<T>(x_of(s, x), 2, &scratch, &all, &mx);
+        if (dweight) lay<T>(x_of(s, x, offsets), 2, &scratch, &all, &mx);
         if (!laid<T>(all, sms, st)) return 0;
         if (dx && !rows_product<T>(ops, mw, s.turned, my, runs, s.in, s.out, dx, s.dx_stride, scratch, sms, st)) return 0;
         if (!dweight) return 1;
@@ -849,7 +879,7 @@ extern "C" int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc
     Matrices mw, mx;
     Layouts all{};
     lay<int8_t>({weight, s.in, s.out, s.experts, s.w_row, s.w_matrix}, 1, &scratch, &all, &mw);
-    lay<int8_t>({q, s.in, s.rows, 1, s.x_stride, 0}, 1, &scratch, &all, &mx);
+    lay<int8_t>(rows_of(q, s.in, s.rows, s.x_stride, offsets, s.experts), 1, &scratch, &all, &mx);
     if (!laid<int8_t>(all, sms, st)) return 0;
     const tb_tensor::Fit fit = rows_fit(1, s.rows, s.experts, s.out, (s.in + 127) / 128);
     ops.parts = fit.parts;

@@ -664,17 +664,25 @@ __global__ void __launch_bounds__(TM) join_parts(const __grid_constant__ Job job
     const int c = blockIdx.y * 8;
     if (c >= tile.columns) return;
     const uint32_t *from = sums + (static_cast<size_t>(t) * parts * NT + c) * TM + threadIdx.x;
-    uint32_t r[8];
+    constexpr int kAhead = 4; /* parts under way at once */
+    uint32_t r[8] = {};
+    for (int p = 0; p < parts; p += kAhead) {
+        uint32_t v[kAhead][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = from[i * TM];
-    for (int p = 1; p < parts; ++p) {
-        from += NT * TM;
+        for (int a = 0; a < kAhead; ++a)
+            if (p + a < parts) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t v = from[i * TM];
-            if constexpr (I8) r[i] += v;
-            else r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(v));
-        }
+                for (int i = 0; i < 8; ++i) v[a][i] = from[(static_cast<size_t>(p + a) * NT + i) * TM];
+            }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (p + a < parts) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (I8) r[i] += v[a][i];
+                    else r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(v[a][i]));
+                }
+            }
     }
     if constexpr (Job::kStaging == 0) job.store(shared, tile, tile.m0 + threadIdx.x, c, r);
     else job.store_joined(tile, tile.m0 + threadIdx.x, c, r);
