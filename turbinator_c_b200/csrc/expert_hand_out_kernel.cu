@@ -3,10 +3,10 @@
  * gradient (include/turbinator/training/cuda_learner.h).
  *
  * Bound: HBM; a row of the output is written once, a token's row read from L2
- * by all but the first of its slots.  The gradient reads every slot's row once: of
- * 16,384 tokens x 8 slots x 1,024 bf16, a tenth without slots, in 78 us, 4.3 TB/s
- * (eight rows ahead 137, in 64 registers for four CTAs an SM 86: the loads under
- * way are what counts).
+ * by all but the first of its slots.  The gradient reads every slot's row once,
+ * as a whole, by the warp that holds its token: 16,384 tokens x 8 slots x 1,024
+ * bf16, a tenth without slots, in 80 us (a token's chunks spread over four warps,
+ * four rows ahead: 89).
  */
 #include "tb_learner.cuh"
 
@@ -16,7 +16,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 4; /* rows of a token under way at once */
+constexpr int kAhead = 2; /* rows of a token under way at once */
+constexpr int kHeld = 4;  /* chunks of a row, of 32 packs, under way at once */
 
 struct HandShape {
     size_t tokens, rows, width, rows_stride, token_stride;
@@ -45,96 +46,81 @@ hand_out(HandShape d, int lanes, int chunks, const T *x, const int32_t *order, c
     store_once<T, PACK>(rows + p * d.rows_stride + c, v);
 }
 
-/* `warps` (1, 2, 4 or 8) take a token, every warps-th chunk of 32 packs each. */
+/* A warp a token: kHeld chunks of 32 packs of its x and of the sums stay in
+ * registers while its slots' rows pass by, two at a time, each read as a whole. */
 template <class T, int PACK>
-__global__ void __launch_bounds__(kThreads)
-hand_out_backward(HandShape d, int warps, const T *x, const int32_t *position, const float *weights, const T *drows, T *dx,
-                  float *dweights) {
+__global__ void __launch_bounds__(kThreads, 2)
+hand_out_backward(HandShape d, const T *x, const int32_t *position, const float *weights, const T *drows, T *dx, float *dweights) {
     using V = typename Values<PACK>::V;
     constexpr int N = Values<PACK>::kCount;
-    __shared__ float dots[kWarps][TB_ROUTE_MAX_TOP_K];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % warps;
-    const size_t t = static_cast<size_t>(blockIdx.x) * (kWarps / warps) + warp / warps;
+    const int lane = threadIdx.x % 32;
+    const size_t t = static_cast<size_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
+    if (t >= d.tokens) return;
     int32_t p = -1;
-    float w = 1.0f;
-    if (t < d.tokens && lane < d.top_k) {
+    float w = 1.0f, dot = 0.0f; /* of slot `lane` */
+    if (lane < d.top_k) {
         p = position[t * d.top_k + lane];
         if (p >= 0 && static_cast<size_t>(p) >= d.rows) p = -1;
         if (weights) w = weights[t * d.top_k + lane];
     }
-    dots[warp][lane] = 0.0f;
-    __syncwarp();
-    if (t < d.tokens)
-        for (size_t base = static_cast<size_t>(part) * 32 * PACK; base < d.width; base += static_cast<size_t>(warps) * 32 * PACK) {
-            const size_t c = base + lane * PACK;
-            const bool in = c < d.width;
-            Array<PACK> g, sum;
-            {
-                float e[PACK];
-                Held<T, PACK> v{};
-                if (dweights && in) v = *reinterpret_cast<const Held<T, PACK> *>(x + t * d.token_stride + c);
-                unpack(v, e);
+    for (size_t base = lane * PACK; base - lane * PACK < d.width; base += kHeld * 32 * PACK) {
+        Array<PACK> g[kHeld], sum[kHeld];
 #pragma unroll
-                for (int i = 0; i < N; ++i) g[i] = vload<V>(e + 2 * i), sum[i] = vall<V>(0.0f);
+        for (int h = 0; h < kHeld; ++h) {
+            float e[PACK];
+            Held<T, PACK> v{};
+            if (dweights && base + h * 32 * PACK < d.width) v = load_once<T, PACK>(x + t * d.token_stride + base + h * 32 * PACK);
+            unpack(v, e);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[h][i] = vload<V>(e + 2 * i), sum[h][i] = vall<V>(0.0f);
+        }
+        for (int j = 0; j < d.top_k; j += kAhead) {
+            Held<T, PACK> v[kAhead][kHeld];
+            int32_t row[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                row[k] = __shfl_sync(0xffffffffu, p, min(j + k, d.top_k - 1));
+                if (j + k >= d.top_k) row[k] = -1;
+#pragma unroll
+                for (int h = 0; h < kHeld; ++h)
+                    if (row[k] >= 0 && base + h * 32 * PACK < d.width)
+                        v[k][h] = load_once<T, PACK>(drows + row[k] * d.rows_stride + base + h * 32 * PACK);
             }
-            for (int j = 0; j < d.top_k; j += kAhead) {
-                Held<T, PACK> v[kAhead];
-                int32_t row[kAhead];
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    row[k] = __shfl_sync(0xffffffffu, p, min(j + k, d.top_k - 1));
-                    if (j + k >= d.top_k || !in) row[k] = -1;
-                    if (row[k] >= 0) v[k] = load_once<T, PACK>(drows + row[k] * d.rows_stride + c);
-                }
-                float dot[kAhead];
+            for (int k = 0; k < kAhead; ++k) {
+                if (row[k] < 0) continue; /* the same for the whole warp */
+                const V s = vall<V>(__shfl_sync(0xffffffffu, w, j + k));
+                V of = vall<V>(0.0f);
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const V s = vall<V>(__shfl_sync(0xffffffffu, w, min(j + k, d.top_k - 1)));
-                    dot[k] = 0.0f;
-                    if (row[k] < 0) continue;
+                for (int h = 0; h < kHeld; ++h) {
+                    if (base + h * 32 * PACK >= d.width) continue;
                     float e[PACK];
-                    unpack(v[k], e);
-                    V of = vall<V>(0.0f);
+                    unpack(v[k][h], e);
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
                         const V r = vload<V>(e + 2 * i);
-                        sum[i] = vfma(s, r, sum[i]);
-                        of = vfma(g[i], r, of);
+                        sum[h][i] = vfma(s, r, sum[h][i]);
+                        of = vfma(g[h][i], r, of);
                     }
+                }
+                if (dweights) {
                     float both[2] = {0.0f, 0.0f};
                     vstore(both, of);
-                    dot[k] = both[0] + both[1];
+                    const float all = warp_sum(both[0] + both[1]);
+                    if (lane == j + k) dot += all;
                 }
-                if (dweights) { /* each half of the warp sums half of the slots, and so on, down to eight lanes a slot */
-                    int spread = 16;
-#pragma unroll
-                    for (int n = kAhead / 2; n; n /= 2, spread /= 2) {
-                        const bool upper = lane & spread;
-#pragma unroll
-                        for (int k = 0; k < n; ++k) {
-                            const float mine = upper ? dot[k + n] : dot[k];
-                            dot[k] = mine + __shfl_xor_sync(0xffffffffu, upper ? dot[k] : dot[k + n], spread);
-                        }
-                    }
-                    for (; spread; spread /= 2) dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], spread);
-                    const int slot = j + lane / (32 / kAhead);
-                    if (lane % (32 / kAhead) == 0 && slot < d.top_k) dots[warp][slot] += dot[0];
-                }
-            }
-            if (dx && in) {
-                float e[PACK];
-#pragma unroll
-                for (int i = 0; i < N; ++i) vstore(e + 2 * i, sum[i]);
-                *reinterpret_cast<Held<T, PACK> *>(dx + t * d.token_stride + c) = packed<T, PACK>(e);
             }
         }
-    if (!dweights) return;
-    __syncthreads();
-    if (t < d.tokens && part == 0 && lane < d.top_k) {
-        float sum = 0.0f;
-        for (int i = 0; i < warps; ++i) sum += dots[warp + i][lane];
-        dweights[t * d.top_k + lane] = sum;
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+            if (dx && base + h * 32 * PACK < d.width) {
+                float e[PACK];
+#pragma unroll
+                for (int i = 0; i < N; ++i) vstore(e + 2 * i, sum[h][i]);
+                *reinterpret_cast<Held<T, PACK> *>(dx + t * d.token_stride + base + h * 32 * PACK) = packed<T, PACK>(e);
+            }
     }
+    if (dweights && lane < d.top_k) dweights[t * d.top_k + lane] = dot;
 }
 
 bool hand_shape(const tb_expert_combine_desc *d, HandShape *s) {
@@ -208,13 +194,9 @@ extern "C" int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_
         using T = decltype(t);
         return with_row_pack<T>(s, x, drows, dx, [&](auto p) {
             constexpr int P = decltype(p)::value;
-            int warps = 1;
-            while (warps < kWarps && static_cast<size_t>(warps) * 32 * P < s.width) warps *= 2;
-            const size_t per = kWarps / warps;
-            hand_out_backward<T, P><<<static_cast<unsigned>((s.tokens + per - 1) / per), kThreads, 0,
+            hand_out_backward<T, P><<<static_cast<unsigned>((s.tokens + kWarps - 1) / kWarps), kThreads, 0,
                                       static_cast<cudaStream_t>(stream)>>>(
-                s, warps, static_cast<const T *>(x), position, weights, static_cast<const T *>(drows), static_cast<T *>(dx),
-                dweights);
+                s, static_cast<const T *>(x), position, weights, static_cast<const T *>(drows), static_cast<T *>(dx), dweights);
             return launched();
         });
     });
