@@ -7,7 +7,7 @@
  * lanes), up to 256 of n its columns, so that a warp that reads a column of
  * the accumulator holds 32 neighbours of one row of O and stores them without
  * a transpose.  n may be ragged: a tile issues its instructions for as many
- * columns, to the next 16, as it has.  Either operand may lie with k
+ * columns, to the next 16 (32), as it has (tb_product_columns.h).  Either operand may lie with k
  * contiguous or with m (n) contiguous; the tensor cores take both.
  *
  * One warp of a CTA asks for the copies, one issues the products, eight or
@@ -54,6 +54,7 @@
 #include "tb_features_internal.h"
 #include "tb_learner.cuh"
 #include "tb_pipeline.cuh"
+#include "tb_product_columns.h"
 
 namespace tb_tensor {
 
@@ -248,6 +249,7 @@ template <int NT, int PLANES, bool PAIR, int STAGING = 0> struct Shape {
     static constexpr int kLaunchRegisters = 168, kStoreRegisters = 216, kOtherRegisters = 72;
     static_assert(!kWide || kThreads * kLaunchRegisters == 32 * (kStoreWarps * kStoreRegisters + 4 * kOtherRegisters), "a split");
     static_assert(kStages >= 2, "a ring");
+    static_assert(NT % 32 == 0 && NT <= kMostColumns, "whole tiles are issued as they are");
 };
 
 struct Waits {
@@ -397,7 +399,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             for (int t = start; ok && t < tiles; t += stride) {
                 const Tile tile = tile_at(t);
                 const int m0 = tile.m0 + static_cast<int>(rank) * kRows;
-                const int n0 = tile.n0 + static_cast<int>(rank) * ((tile.columns + 15) / 16 * 8);
+                const int n0 = tile.n0 + static_cast<int>(rank) * second_half(I8, tile.columns);
                 for (int k = 0; k < tile.depth; k += kDepth, ++n) {
                     const int s = n % S::kStages;
                     if (n >= S::kStages && !(ok = w.wait(smem_addr(&empty[s]), (n / S::kStages - 1) & 1))) break;
@@ -449,8 +451,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
             bool ok = true;
             for (int t = start; ok && t < tiles; t += stride) {
                 const Tile tile = tile_at(t);
-                const uint32_t how =
-                    product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, (tile.columns + 15) / 16 * 16);
+                const uint32_t how = product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, issued_columns(I8, PAIR, tile.columns));
                 uint32_t d = 0;
                 for (int k = 0, in = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++in) {
                     if (k == 0 || (kSums && in == kSegment)) { /* the next accumulator */
