@@ -247,7 +247,8 @@ int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_desc *desc,
  *
  * Expert e's rows are offsets[e] .. offsets[e+1] of x [rows, in_width], as the
  * routing lists them; offsets [experts+1] int32 on the device, never
- * decreasing, are taken into [0, rows].  With one expert offsets may be NULL:
+ * decreasing, are taken into [0, rows] (those that fall give wrong results, and
+ * nothing outside the tensors is touched).  With one expert offsets may be NULL:
  * all rows are its.
  *   y[p] = x[p] W_e
  * Rows of y and dx that are no expert's are left as they were, and what those of

@@ -64,17 +64,22 @@ template <class T, int NT> struct RowJob {
         }
         __syncthreads();
         if (threadIdx.x < 32) {
-            int before = 0;
-            for (int base = 0; base < runs.experts; base += 32) {
+            int before = 0, past = 0; /* tiles and rows of the experts so far: a run begins behind all others, */
+            for (int base = 0; base < runs.experts; base += 32) { /* so that there are no more tiles than room for their sums */
                 const int e = base + threadIdx.x;
-                int n = e < runs.experts ? (s.end[e] - s.start[e] + NT - 1) / NT : 0;
+                int start = max(e < runs.experts ? s.start[e] : 0, past);
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) start = max(start, __shfl_up_sync(0xffffffffu, start, o));
+                const int end = max(e < runs.experts ? s.end[e] : 0, start);
+                int n = (end - start + NT - 1) / NT;
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) {
                     const int v = __shfl_up_sync(0xffffffffu, n, o);
                     if (threadIdx.x >= o) n += v;
                 }
-                if (e < runs.experts) s.first[e + 1] = before + n;
+                if (e < runs.experts) s.start[e] = start, s.end[e] = end, s.first[e + 1] = before + n;
                 before += __shfl_sync(0xffffffffu, n, 31);
+                past = __shfl_sync(0xffffffffu, end, 31);
             }
             if (threadIdx.x == 0) s.first[0] = 0;
         }
