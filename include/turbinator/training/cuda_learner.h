@@ -323,8 +323,9 @@ int tb_cuda_experts_product_i8_device(const tb_expert_product_i8_desc *desc, con
  *   steps times: x = (a + b x x^T + c (x x^T)^2) x
  *   out = scale x
  * (3.4445, -4.7750, 2.0315 in five steps bring most singular values within 0.7
- * to 1.2.)  The products are taken of pairs of f16 values on the tensor cores,
- * 22 bits for values of an average element's size and up.  No element of x, x
+ * to 1.2.)  The products are taken of pairs of f16 values on the tensor cores:
+ * 22 bits of x, x x^T and the polynomial down to 2^-26, 2^-48 absolute below, so
+ * that rows a millionth of others' size keep their digits.  No element of x, x
  * x^T or the polynomial may pass 15 in magnitude on the way: NaN otherwise.  A
  * matrix of zeros gives zeros, one with an infinity or a NaN gives NaN. */
 typedef struct tb_orthogonalise_desc {

@@ -8,9 +8,10 @@
  * A and S symmetric, so that a little over half of their tiles are computed and
  * the others mirrored.
  *
- * x, A and S are kept as pairs of f16 values, the second what the rounding of
- * the first left, times 2^12: 22 bits for values about the size of a unit
- * matrix's share and 2^-37 absolute below.  A product of pairs is three
+ * x, A and S are kept times 2^12 as pairs of f16 values, the second what the
+ * rounding of the first left, 2^11 higher: 22 bits for values down to 2^-26 (a
+ * unit matrix's share is some 2^-5 to 2^-12) and 2^-48 absolute below, so that rows
+ * far smaller than others keep their digits.  A product of pairs is three
  * products of f16 (the fourth is below 2^-22); the polynomial multiplies an
  * error in a direction of a small singular value by up to a^steps, 485 for five
  * steps of the quintic, so that plain bf16 products leave errors of 2 to 3 % in
@@ -29,17 +30,20 @@ namespace {
 
 constexpr float kUp = 4096.0f; /* of every kept value */
 constexpr float kDown = 1.0f / 4096.0f;
+constexpr float kLowUp = 1 << tb_tensor::kPlaneRise<2>; /* of the second plane beyond that */
+constexpr float kLowDown = 1.0f / kLowUp;
+__device__ __forceinline__ float joined(__half high, __half low) { return fmaf(__half2float(low), kLowDown, __half2float(high)); }
+__device__ __forceinline__ void part(float v, __half *high, __half *low) {
+    *high = __float2half_rn(v);
+    *low = __float2half_rn((v - __half2float(*high)) * kLowUp);
+}
 
 /* A stack of matrices as two planes: the second `plane` elements on. */
 struct Pair {
     __half *at;
     size_t line, matrix, plane;
-    __device__ __forceinline__ float get(size_t i) const { return __half2float(at[i]) + __half2float(at[plane + i]); }
-    __device__ __forceinline__ void put(size_t i, float v) const {
-        const __half high = __float2half_rn(v);
-        at[i] = high;
-        at[plane + i] = __float2half_rn(v - __half2float(high));
-    }
+    __device__ __forceinline__ float get(size_t i) const { return joined(at[i], at[plane + i]); }
+    __device__ __forceinline__ void put(size_t i, float v) const { part(v, &at[i], &at[plane + i]); }
 };
 
 /* ---- x = g / (|g| + epsilon) ---- */
@@ -121,8 +125,7 @@ __global__ void __launch_bounds__(kNormThreads) normalise(Given d, const T *g, c
 #pragma unroll
         for (int i = 0; i < PACK; ++i) {
             const float v = plain ? e[i] * near : static_cast<float>(static_cast<double>(e[i]) * up);
-            high.v[i] = __float2half_rn(v);
-            low.v[i] = __float2half_rn(v - __half2float(high.v[i]));
+            part(v, &high.v[i], &low.v[i]);
         }
         *reinterpret_cast<Pack<__half, PACK> *>(to + r * x.line + c) = high;
         *reinterpret_cast<Pack<__half, PACK> *>(to + x.plane + r * x.line + c) = low;
@@ -179,12 +182,11 @@ constexpr int kBoxBytes = 32 * 32 * sizeof(__half);
 struct Boxes {
     int lane;
     __half *at;
-    __device__ __forceinline__ float get(int i) const {
-        return __half2float(at[i * 32 + lane]) + __half2float(at[1024 + i * 32 + lane]);
-    }
+    __device__ __forceinline__ float get(int i) const { return joined(at[i * 32 + lane], at[1024 + i * 32 + lane]); }
     __device__ __forceinline__ void put(int i, float v, __half *high, __half *low) const {
-        at[i * 32 + lane] = *high = __float2half_rn(v);
-        at[1024 + i * 32 + lane] = *low = __float2half_rn(v - __half2float(*high));
+        part(v, high, low);
+        at[i * 32 + lane] = *high;
+        at[1024 + i * 32 + lane] = *low;
     }
     __device__ __forceinline__ void across(const __half (&high)[32], const __half (&low)[32]) const {
 #pragma unroll
@@ -246,8 +248,7 @@ struct SquareJob {
         for (int i = 0; i < 8; ++i) {
             float e = __uint_as_float(r[i]) * kDown;
             if (second && c0 + i < t.columns) e = fmaf(c, e, b * from.get(was + i * from.line));
-            high.v[i] = __float2half_rn(e);
-            low.v[i] = __float2half_rn(e - __half2float(high.v[i]));
+            part(e, &high.v[i], &low.v[i]);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)

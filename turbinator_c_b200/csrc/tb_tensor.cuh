@@ -23,9 +23,12 @@
  * a pause, took as long at a lower clock.
  * CTAs (pairs) are persistent and take every so-many-th tile of a job.
  *
- * Operands of more than 16 bits come as planes that sum to them; a stage holds
- * all planes, and the pairs of planes whose product counts are multiplied one
- * after the other, small ones first.  Their sums are taken out of the tensor
+ * Operands of more than 16 bits come as planes that sum to them, each held
+ * 2^kPlaneRise higher than the one in front of it, so that its values are as far
+ * from the type's least ones; a stage holds all planes, and the pairs of planes
+ * whose product counts are multiplied one after the other, small ones first.  The
+ * instruction with which a larger kind of pair begins takes what the smaller ones
+ * left 2^kPlaneRise lower.  Their sums are taken out of the tensor
  * cores after every stage and go on in f32 registers: the tensor cores' own
  * additions cut what does not fit, which over thousands of k left errors of 4e-6
  * to 2e-5 in results that f32 arithmetic has to 1e-6.  Every second stage would
@@ -68,7 +71,9 @@ constexpr int kBlockBytes = 128;              /* of k in a stage */
 constexpr int kChunk = 64;                    /* 16-bit values of m (n) in a swizzled row, where those are contiguous */
 constexpr int kChunkBytes = 64 * kBlockBytes; /* 64 such rows, one for each k of a stage */
 constexpr int kColumns = 512; /* of TMEM: two accumulators of 256 */
-constexpr int kSegment = 1;   /* stages of operands in planes between two readings of the accumulator */
+/* How many powers of two a plane is held higher than the one in front of it: two f16, what the rounding of one leaves is
+ * 2^-11 of it at most. */
+template <int PLANES> constexpr int kPlaneRise = PLANES == 2 ? 11 : 0;
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
 /* ---- instructions ---- */
@@ -109,16 +114,20 @@ template <bool PAIR> __device__ __forceinline__ void tensor_commit(uint32_t bar)
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-#define TB_TENSOR_PRODUCT(GROUP, KIND)                                                                          \
+#define TB_TENSOR_PRODUCT(GROUP, KIND, LOWER, ...)                                                              \
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::" KIND \
-                 " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)) \
+                 " [%0], %1, %2, %3, p" LOWER ";\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(how), "r"(static_cast<uint32_t>(add)), ##__VA_ARGS__ \
                  : "memory")
-template <bool I8, bool PAIR>
+/* LOWER: what is in d already counts 2^-LOWER of itself. */
+template <bool I8, bool PAIR, int LOWER = 0>
 __device__ __forceinline__ void tensor_product(uint32_t d, uint64_t a, uint64_t b, uint32_t how, bool add) {
-    if constexpr (I8 && PAIR) TB_TENSOR_PRODUCT("2", "i8");
-    else if constexpr (I8) TB_TENSOR_PRODUCT("1", "i8");
-    else if constexpr (PAIR) TB_TENSOR_PRODUCT("2", "f16");
-    else TB_TENSOR_PRODUCT("1", "f16");
+    static_assert(LOWER >= 0 && LOWER <= 15 && (!I8 || LOWER == 0), "what the instruction takes");
+    if constexpr (I8 && PAIR) TB_TENSOR_PRODUCT("2", "i8", "");
+    else if constexpr (I8) TB_TENSOR_PRODUCT("1", "i8", "");
+    else if constexpr (PAIR && LOWER != 0) TB_TENSOR_PRODUCT("2", "f16", ", %5", "n"(LOWER));
+    else if constexpr (PAIR) TB_TENSOR_PRODUCT("2", "f16", "");
+    else if constexpr (LOWER != 0) TB_TENSOR_PRODUCT("1", "f16", ", %5", "n"(LOWER));
+    else TB_TENSOR_PRODUCT("1", "f16", "");
 }
 #undef TB_TENSOR_PRODUCT
 /* 32 columns of this warp's 32 lanes; tensor_wait_load() before the values are used. */
@@ -339,7 +348,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
     constexpr int kBlock = I8 ? 128 : 64, kStep = I8 ? 32 : 16; /* of k: in a block, in an instruction */
     constexpr int kDepth = S::kBlocks * kBlock;                 /* in a stage */
     constexpr int kParts = S::kBlocks * PLANES;
-    constexpr bool kSums = PLANES > 1;                          /* of segments, in registers */
+    constexpr bool kSums = PLANES > 1;                          /* of stages, in registers */
+    constexpr int kRise = kPlaneRise<PLANES>;
     constexpr int kCtas = PAIR ? 2 : 1;
     constexpr int kBChunks = (S::kPart + kChunk - 1) / kChunk;
     extern __shared__ unsigned char raw[];
@@ -453,9 +463,8 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 const Tile tile = tile_at(t);
                 const uint32_t how = product_form(I8, ops.type, ops.a_outer, ops.b_outer, S::kTileM, issued_columns(I8, PAIR, tile.columns));
                 uint32_t d = 0;
-                for (int k = 0, in = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++in) {
-                    if (k == 0 || (kSums && in == kSegment)) { /* the next accumulator */
-                        in = 0;
+                for (int k = 0; ok && (k < tile.depth || k == 0); k += kDepth) {
+                    if (k == 0 || kSums) { /* the next accumulator */
                         const uint32_t buffer = number & 1;
                         d = tmem + buffer * 256;
                         if (number >= 2 && !(ok = w.wait(smem_addr(&freed[buffer]), (number / 2 - 1) & 1))) break;
@@ -470,39 +479,41 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                         tensor_fence_after();
                         if (elected()) {
                             const uint32_t ia = (ops.a_outer ? kStep * kBlockBytes : 32) >> 4, ib = (ops.b_outer ? kStep * kBlockBytes : 32) >> 4;
-                            bool add = in > 0;
-                            const auto multiply = [&](int pa, int pb, int steps) {
+                            bool add = !kSums && k > 0;
+                            const auto multiply = [&](int pa, int pb, int steps, auto lower) {
                                 uint64_t a = operand(smem_addr(at + pa * S::kABytes), ops.a_outer);
                                 uint64_t b = operand(smem_addr(at + kParts * S::kABytes + pb * S::kBBytes), ops.b_outer);
+                                if (steps <= 0) return;
+                                tensor_product<I8, PAIR, decltype(lower)::value>(d, a, b, how, add);
+                                add = true;
                                 if (steps >= kBlock / kStep) {
 #pragma unroll
-                                    for (int i = 0; i < kBlock / kStep; ++i) {
-                                        tensor_product<I8, PAIR>(d, a + i * ia, b + i * ib, how, add);
-                                        add = true;
-                                    }
+                                    for (int i = 1; i < kBlock / kStep; ++i) tensor_product<I8, PAIR>(d, a + i * ia, b + i * ib, how, true);
                                 } else {
-                                    for (int i = 0; i < steps; ++i, a += ia, b += ib) {
-                                        tensor_product<I8, PAIR>(d, a, b, how, add);
-                                        add = true;
-                                    }
+                                    for (int i = 1; i < steps; ++i) tensor_product<I8, PAIR>(d, a + i * ia, b + i * ib, how, true);
                                 }
                             };
+                            constexpr std::integral_constant<int, 0> kAsItIs{};
+                            constexpr std::integral_constant<int, kRise> kLower{};
                             const int steps = (left + kStep - 1) / kStep;
                             if constexpr (PLANES == 1) {
 #pragma unroll
-                                for (int j = 0; j < S::kBlocks; ++j) multiply(j, j, steps - j * (kBlock / kStep));
+                                for (int j = 0; j < S::kBlocks; ++j) multiply(j, j, steps - j * (kBlock / kStep), kAsItIs);
                             } else { /* planes i and j count while i + j < PLANES: the small products first */
 #pragma unroll
-                                for (int small = PLANES - 1; small >= 0; --small)
+                                for (int small = PLANES - 1; small >= 0; --small) {
+                                    if (small == PLANES - 1) multiply(0, small, steps, kAsItIs);
+                                    else multiply(0, small, steps, kLower);
 #pragma unroll
-                                    for (int p = 0; p <= small; ++p) multiply(p, small - p, steps);
+                                    for (int p = 1; p <= small; ++p) multiply(p, small - p, steps, kAsItIs);
+                                }
                             }
                             tensor_commit<PAIR>(smem_addr(&empty[s]));
                         }
                         __syncwarp();
                         ++n;
                     }
-                    if (left <= kDepth || (kSums && in == kSegment - 1)) {
+                    if (left <= kDepth || kSums) {
                         if (elected()) tensor_commit<PAIR>(smem_addr(&done[(number - 1) & 1]));
                         __syncwarp();
                     }
@@ -569,7 +580,7 @@ tensor_products(const __grid_constant__ Operands ops, const __grid_constant__ Jo
                 for (int i = 0; i < S::kShare; ++i) sum[i] = 0.0f;
                 if constexpr (Job::kStaging != 0)
                     if (columns > 0 && ops.parts == 1) job.ask(tile, m, c0, staging);
-                for (int k = 0; ok && (k < tile.depth || k == 0); k += kSegment * kDepth, ++number) {
+                for (int k = 0; ok && (k < tile.depth || k == 0); k += kDepth, ++number) {
                     const uint32_t buffer = number & 1;
                     if (!(ok = w.wait(smem_addr(&done[buffer]), (number / 2) & 1))) break;
                     tensor_fence_after();
