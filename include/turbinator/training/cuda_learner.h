@@ -254,7 +254,8 @@ int tb_cuda_hand_out_experts_backward_device(const tb_expert_combine_desc *desc,
  * Rows of y and dx that are no expert's are left as they were, and what those of
  * x and dy hold is not used.  All sums are f32.  On the tensor cores f32 tensors
  * are multiplied as three bf16 parts each, which leaves out less than 2^-23 of
- * the sum of the products' magnitudes; an infinity in one may give NaN there. */
+ * the sum of the products' magnitudes (and 2^-148 of a factor: no more than that
+ * down to 2^-125); an infinity in one may give NaN there. */
 typedef struct tb_expert_product_desc {
     size_t rows, experts, in_width, out_width;
     size_t in_stride, din_stride; /* of the rows of x; of dx */

@@ -71,9 +71,10 @@ constexpr int kBlockBytes = 128;              /* of k in a stage */
 constexpr int kChunk = 64;                    /* 16-bit values of m (n) in a swizzled row, where those are contiguous */
 constexpr int kChunkBytes = 64 * kBlockBytes; /* 64 such rows, one for each k of a stage */
 constexpr int kColumns = 512; /* of TMEM: two accumulators of 256 */
-/* How many powers of two a plane is held higher than the one in front of it: two f16, what the rounding of one leaves is
- * 2^-11 of it at most. */
-template <int PLANES> constexpr int kPlaneRise = PLANES == 2 ? 11 : 0;
+/* How many powers of two a plane is held higher than the one in front of it.  Two f16: what the rounding of one leaves is
+ * 2^-11 of it at most.  Three bf16: 2^-9 of it, or 2^-8 where the largest values are cut; seven, so that nothing passes
+ * f32's range that did not before. */
+template <int PLANES> constexpr int kPlaneRise = PLANES == 3 ? 7 : PLANES == 2 ? 11 : 0;
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
 /* ---- instructions ---- */
