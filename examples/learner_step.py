@@ -151,15 +151,31 @@ class HandOut(torch.autograd.Function):
         return dx, None, None
 
 
+def _fit_together(rows, weight, offsets, n):
+    """The C entry points see addresses only: what a tensor says of itself is checked here."""
+    if rows.ndim != 2 or weight.ndim != 3 or rows.shape[1] != n:
+        raise ValueError(f"rows {tuple(rows.shape)} and weights {tuple(weight.shape)} do not go together")
+    if offsets.dtype != torch.int32 or offsets.shape != (weight.shape[0] + 1,) or not offsets.is_contiguous():
+        raise ValueError("offsets are one more 32-bit whole number than there are experts")
+    if not rows.device == weight.device == offsets.device:
+        raise ValueError("rows, weights and offsets lie on different devices")
+
+
 class Product(torch.autograd.Function):
-    """rows [rows, in] of the experts' runs, weights [experts, in, out] -> [rows, out]; offsets stay on the GPU."""
+    """rows [rows, in] of the experts' runs, weights [experts, in, out] of the same type -> [rows, out]; offsets stay on
+    the GPU.  Weights that lie [experts, out, in] (a transposed view) are multiplied as they lie, others copied."""
 
     @staticmethod
     def forward(ctx, rows, weight, offsets):
-        rows = rows.contiguous()
         e, n, m = weight.shape
+        _fit_together(rows, weight, offsets, n)
+        if rows.dtype != weight.dtype:
+            raise TypeError(f"rows of {rows.dtype} and weights of {weight.dtype}")
+        rows = rows.contiguous()
+        turned = not weight.is_contiguous() and weight.transpose(1, 2).is_contiguous()
+        weight = weight if turned else weight.contiguous()
         desc = tb.ExpertProductDesc(rows=rows.shape[0], experts=e, in_width=n, out_width=m, type=TYPE[rows.dtype],
-                                    weight_order=tb.TB_WEIGHT_IN_OUT)
+                                    weight_order=tb.TB_WEIGHT_OUT_IN if turned else tb.TB_WEIGHT_IN_OUT)
         out = torch.empty((rows.shape[0], m), dtype=rows.dtype, device="cuda")
         work = _scratch(tb.tb_cuda_experts_product_workspace(desc))
         _call(tb.tb_cuda_experts_product_device(desc, rows, weight, offsets, out, work, torch.cuda.current_stream()))
@@ -170,7 +186,7 @@ class Product(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         rows, weight, offsets = ctx.saved_tensors
-        drows, dweight = torch.empty_like(rows), torch.empty_like(weight)
+        drows, dweight = torch.empty_like(rows), torch.empty_like(weight)  # which keeps the weights' order
         work = _scratch(tb.tb_cuda_experts_product_workspace(ctx.desc))
         _call(tb.tb_cuda_experts_product_backward_device(ctx.desc, rows, weight, offsets, dout.contiguous(), drows, dweight, work,
                                                          torch.cuda.current_stream()))
@@ -189,6 +205,10 @@ def quantised(x):
 def product_8_bit(rows, weight, weight_scale, offsets):
     """rows [rows, in] of the experts' runs by weights [experts, out, in] of 8 bits."""
     e, m, n = weight.shape
+    _fit_together(rows, weight, offsets, n)
+    if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32 or weight_scale.shape != (e, m):
+        raise TypeError("weights of 8 bits with an f32 scale for each output channel")
+    weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
     q, scale = quantised(rows)
     desc = tb.ExpertProductI8Desc(rows=rows.shape[0], experts=e, in_width=n, out_width=m, type=TYPE[rows.dtype])
     out = torch.empty((rows.shape[0], m), dtype=rows.dtype, device="cuda")
