@@ -302,9 +302,9 @@ class OrthogonalMomentum:
             b, m, n = p.shape
             desc = tb.OrthogonaliseDesc(matrices=b, rows=m, columns=n, type=TYPE[p.dtype], steps=5, a=3.4445, b=-4.7750,
                                         c=2.0315, epsilon=1e-7, scale=max(1.0, n / m) ** 0.5)
-            update, work = torch.empty_like(p), _scratch(tb.tb_cuda_orthogonalise_workspace(desc))
-            _call(tb.tb_cuda_orthogonalise_device(desc, p.grad.add(kept, alpha=self.momentum), update, work,
-                                                  torch.cuda.current_stream()))
+            g = p.grad.add(kept, alpha=self.momentum).contiguous()  # however the parameter lies
+            update, work = torch.empty_like(g), _scratch(tb.tb_cuda_orthogonalise_workspace(desc))
+            _call(tb.tb_cuda_orthogonalise_device(desc, g, update, work, torch.cuda.current_stream()))
             p.add_(update, alpha=-self.rate)
 
 

@@ -70,3 +70,18 @@ def test_8_bit_products_of_weights_that_lie_otherwise(example):  # noqa: F811
     assert torch.equal(example.product_8_bit(rows, *turned, off)[:57], want)
     wide = torch.cat([held, held], 2)[..., :24], torch.stack([scale, scale], 2)[..., 0]
     assert torch.equal(example.product_8_bit(rows, *wide, off)[:57], want)
+
+
+@pytest.mark.parametrize("way", ("transposed", "slices", "experts inside"))
+def test_momentum_of_parameters_that_lie_otherwise(example, way):  # noqa: F811
+    """Two steps move the values as they move those of a dense parameter."""
+    gen = _gen(44)
+    values = _normal(gen, 2, 40, 60)
+    plain, lying = torch.nn.Parameter(values.clone()), torch.nn.Parameter(_lying(values.clone(), way))
+    moments = [example.OrthogonalMomentum([p], rate=0.5) for p in (plain, lying)]
+    for _ in range(2):
+        grad = _normal(gen, 2, 40, 60)
+        plain.grad, lying.grad = grad.clone(), _lying(grad.clone(), way)
+        for m in moments:
+            m.step()
+    assert torch.equal(plain.detach(), lying.detach()) and not torch.equal(plain.detach(), values)
