@@ -7,16 +7,17 @@ matrices are updated by orthogonalised momentum, everything else by Adam; for ac
 
     python examples/learner_step.py            # trains for some steps, then acts step by step from kept states
 
-The ``torch.autograd.Function`` wrappers below are all that a PyTorch program needs around the C entry points; the
-convolution and the products of dense layers are PyTorch's.  They make descriptors, workspaces and outputs anew in each call, which a
-program that counts microseconds, as one that acts does, makes once and keeps: a step of 64 aircraft is 2 us of the
-GPU's time and more than ten times that of the host's in this form."""
+The ``torch.autograd.Function`` wrappers below, each differentiable once, are all that a PyTorch program needs around
+the C entry points; the convolution and the products of dense layers are PyTorch's.  They make descriptors, workspaces
+and outputs anew in each call, which a program that counts microseconds, as one that acts does, makes once and keeps: a
+step of 64 aircraft is 2 us of the GPU's time and more than ten times that of the host's in this form."""
 from __future__ import annotations
 
 import os
 import sys
 
 import torch
+from torch.autograd.function import once_differentiable
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
@@ -56,6 +57,7 @@ class GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, gamma, beta, mean, rstd = ctx.saved_tensors
         dy, dx = dy.contiguous(), torch.empty_like(x)
@@ -85,6 +87,7 @@ class GatedRecurrence(torch.autograd.Function):
         return h, last
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh, dlast):
         xgg, decay, reset, saved = ctx.saved_tensors
         d = xgg.shape[2] // 3
@@ -117,6 +120,7 @@ class RouteExperts(torch.autograd.Function):
         return weights, ids, offsets, order, position
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dweights, *_):
         logits, ids = ctx.saved_tensors
         dlogits = torch.empty_like(logits)
@@ -142,6 +146,7 @@ class HandOut(torch.autograd.Function):
         return rows
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, drows):
         (position,) = ctx.saved_tensors
         drows = drows.contiguous()
@@ -184,6 +189,7 @@ class Product(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         rows, weight, offsets = ctx.saved_tensors
         drows, dweight = torch.empty_like(rows), torch.empty_like(weight)  # which keeps the weights' order
@@ -233,6 +239,7 @@ class Combine(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         rows, position, weights = ctx.saved_tensors
         drows, dweights = torch.empty_like(rows), torch.empty_like(weights)

@@ -85,3 +85,25 @@ def test_momentum_of_parameters_that_lie_otherwise(example, way):  # noqa: F811
         for m in moments:
             m.step()
     assert torch.equal(plain.detach(), lying.detach()) and not torch.equal(plain.detach(), values)
+
+
+def test_second_derivatives_are_refused(example):  # noqa: F811
+    """The backward passes are kernels too, which autograd does not see into: an error, not a derivative without them."""
+    gen = _gen(45)
+    order = torch.randperm(60, generator=gen, device="cuda").int()
+    position = torch.empty(60, dtype=torch.int32, device="cuda")
+    position[order.long()] = torch.arange(60, dtype=torch.int32, device="cuda")
+    position, off = position.reshape(30, 2), _whole([0, 25, 25, 60])
+    x, w, logits, share = _normal(gen, 30, 24), _normal(gen, 3, 24, 40), _normal(gen, 30, 3), torch.rand((30, 2), generator=gen, device="cuda")
+    gates, decay = _normal(gen, 2, 5, 72), _normal(gen, 24)
+    reset, state = torch.zeros((2, 5), dtype=torch.uint8, device="cuda"), torch.zeros((2, 24), device="cuda")
+    calls = [lambda v: example.HandOut.apply(v, order, position), lambda v: example.Product.apply(v.repeat(2, 1), w, off),
+             lambda v: example.Combine.apply(v.repeat(2, 1), position, share),
+             lambda v: example.RouteExperts.apply(logits + v[:, :3], torch.zeros(3, device="cuda"), 2)[0],
+             lambda v: example.GatedRecurrence.apply(gates + v[:2, None, :1], decay, state, reset)[0],
+             lambda v: example.GroupNormAct.apply(v.reshape(3, 10, 24), torch.ones(24, device="cuda"), torch.zeros(24, device="cuda"), 4)]
+    for call in calls:
+        v = x.clone().requires_grad_()
+        (grad,) = torch.autograd.grad(call(v).square().sum(), v, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice"):
+            grad.square().sum().backward()
