@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 
 from tests import experts_reference as ref  # noqa: E402
 from tests.learner_reference import check  # noqa: E402
-from tests.test_experts_gpu import KINDS, _check_i8, _gen, _product_case, _synchronised, _whole  # noqa: E402
+from tests.test_experts_gpu import KINDS, _check_i8, _check_product, _gen, _normal, _product_case, _synchronised, _whole, _work  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,57 @@ def test_offsets_that_fall_stay_inside_the_tensors(kind, turned):
         if offsets[1] == offsets[-1] == rows:  # a run begins where all in front of it end: the first has all rows
             want, size = ref.product(x.double(), w.double(), [0] + [rows] * 8, turned)
             check("y", y[:-4096].reshape(rows, m), want, ref.sum_error(n, size, kind == torch.float32))
+
+
+FEW = [  # rows, offsets, in, out: runs that begin and end inside four rows, rows of no expert among them
+    (11, [1, 2, 4, 4, 9, 10], 70, 130),
+    (7, [0, 1, 3, 6], 64, 96),
+    (8, [2, 2, 3, 7, 7, 7], 33, 40),
+    (16, [0, 0, 5, 6, 16], 520, 520),
+]
+
+
+@pytest.mark.parametrize("turned", (False, True), ids=("in_out", "out_in"))
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("shape", FEW, ids=str)
+def test_few_rows_of_several_experts(shape, kind, turned):
+    rows, offsets, n, m = shape
+    _check_product(_gen(rows + n), rows, offsets, n, m, kind, turned)
+
+
+@pytest.mark.parametrize("shape", FEW, ids=str)
+def test_few_8_bit_rows_of_several_experts(shape):
+    rows, offsets, n, m = shape
+    gen, e = _gen(rows), len(offsets) - 1
+    q = torch.randint(-128, 128, (rows, n), generator=gen, device="cuda").to(torch.int8)
+    w = torch.randint(-128, 128, (e, m, n), generator=gen, device="cuda").to(torch.int8)
+    _check_i8(q, torch.rand(rows, generator=gen, device="cuda"), w, torch.rand((e, m), generator=gen, device="cuda"), offsets, KINDS[rows % 3])
+
+
+def test_products_over_2_31_elements_with_the_room_they_ask_for():
+    """Each call has the workspace that its own query names; the last expert's rows lie far behind 2^31 elements."""
+    rows, n, m, tail = 4_300_000, 512, 520, 700
+    gen = _gen(16)
+    x, dy = (torch.empty((rows, width), dtype=torch.bfloat16, device="cuda") for width in (n, m))
+    for v in (x, dy):
+        for part in v.split(1 << 19):
+            part.copy_(torch.randn(part.shape, generator=gen, device="cuda"))
+    w = _normal(gen, 2, m, n, kind=torch.bfloat16, scale=0.05)
+    got = []
+    for xs, dys, offsets in [(x, dy, [0, rows - tail, rows]), (x[-tail:].clone(), dy[-tail:].clone(), [0, 0, tail])]:
+        count = xs.shape[0]
+        desc = tb.ExpertProductDesc(rows=count, experts=2, in_width=n, out_width=m, weight_order=tb.TB_WEIGHT_OUT_IN, type=tb.TB_TYPE_BF16)
+        work, off = torch.empty(tb.tb_cuda_experts_product_workspace(desc), dtype=torch.uint8, device="cuda"), _whole(offsets)
+        y, dx, dw = torch.empty_like(dys), torch.empty_like(xs), torch.empty_like(w)
+        assert tb.tb_cuda_experts_product_device(desc, xs, w, off, y, work, torch.cuda.current_stream()) == 1
+        assert tb.tb_cuda_experts_product_backward_device(desc, xs, w, off, dys, dx, dw, work, torch.cuda.current_stream()) == 1
+        _synchronised()
+        got.append((y[-tail:].clone(), dx[-tail:].clone(), dw[1]))
+        del work, y, dx
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    right, left = x[-tail:].double(), dy[-tail:].double().T
+    want, size = left @ right, left.abs() @ right.abs()
+    for _, _, dw in got:  # the sums' parts go by the average run, so that the bits may differ
+        check("dw", dw, want, ref.sum_error(tail, size))
+    del x, dy
+    torch.cuda.empty_cache()
