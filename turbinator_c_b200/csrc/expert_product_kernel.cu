@@ -288,8 +288,8 @@ few_rows(FewShape d, Runs runs, const W *x, const W *weight, T *out, const float
 
 /* The same where the weights lie the other way, [sum][channel]: a lane takes a
  * channel, a CTA's 32 warps every 32nd k, and their sums meet in shared memory.
- * For f32 alone (1 x 4,096 x 4,096: 27 us against 72 on the tensor cores; 16
- * bytes a lane: 61): of 16 bits the tensor cores' parts of a sum are faster (bf16
+ * For f32 alone (1 x 4,096 x 4,096: 27 us against 72 on the tensor cores where the
+ * weights lie in L2, 45 where they do not; 16 bytes a lane: 61): of 16 bits the tensor cores' parts of a sum are faster (bf16
  * 9 us, this way 30). */
 constexpr int kAcrossThreads = 1024, kAcrossWarps = kAcrossThreads / 32;
 __global__ void __launch_bounds__(kAcrossThreads)
